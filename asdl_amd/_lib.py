@@ -16,6 +16,7 @@ _lib = None
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_f32 = ctypes.c_float
+c_f64 = ctypes.c_double
 c_ptr = ctypes.c_void_p
 c_size = ctypes.c_size_t
 
@@ -64,6 +65,15 @@ _SIGNATURES = {
     'ak_event_destroy': (c_int, [c_ptr]),
     'ak_event_record': (c_int, [c_ptr, c_ptr]),
     'ak_sample_categorical': (c_int, [c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
+    'ak_sample_filtered': (c_int, [c_ptr, c_int, c_i64, c_i64, c_i64, c_ptr, c_int, c_f64, c_ptr, c_i64, c_ptr, c_f64, c_ptr, c_f64,
+                                   c_ptr, c_ptr, c_ptr, c_ptr]),
+    'ak_layer_norm': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_ptr, c_int, c_i64, c_i64, c_f32, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr]),
+    'ak_layer_norm_backward_ws_bytes': (c_size, [c_i64, c_i64, c_int]),
+    'ak_layer_norm_backward': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_i64, c_i64, c_ptr,
+                                       c_i64, c_ptr, c_ptr, c_ptr, c_f32, c_f32, c_ptr, c_size, c_ptr]),
+    'ak_grad_norm_ws_bytes': (c_size, [c_int]),
+    'ak_grad_norm': (c_int, [c_ptr, c_int, c_int, c_ptr, c_ptr, c_size, c_ptr]),
+    'ak_clip_grad_norm': (c_int, [c_ptr, c_int, c_int, c_f64, c_ptr, c_ptr, c_size, c_ptr]),
     'ak_event_synchronize': (c_int, [c_ptr]),
     'ak_kron_finish': (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_int, c_ptr, c_ptr]),
     'ak_kron_precond_deep_ws_bytes': (c_size, [c_ptr, c_int]),

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 
-AK_F32, AK_BF16, AK_F32_AS_BF16, AK_F32_IN_ORDER = 0, 1, 2, 3
+AK_F32, AK_BF16, AK_F32_AS_BF16, AK_F32_IN_ORDER, AK_F16 = 0, 1, 2, 3, 4
 
 _ws_lock = threading.Lock()
 _workspaces = {}
@@ -153,6 +153,41 @@ def _dtype_code(t):
     if t.dtype == torch.bfloat16:
         return AK_BF16
     raise TypeError(f'unsupported dtype {t.dtype}: the kernels take float32 or bfloat16 inputs')
+
+
+_ELEMENT_TYPES = {torch.float32: AK_F32, torch.bfloat16: AK_BF16, torch.float16: AK_F16}
+
+
+def _element_type(t, what):
+    """The code of a tensor that may be float32, bfloat16 or float16 (layer norm, gradient norms, filtered draws)."""
+    code = _ELEMENT_TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f'{what} has to be float32, bfloat16 or float16. Got {t.dtype}.')
+    return code
+
+
+def _require_one_gpu(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f'{name} is on {t.device}, the first operand on {device}.')
+
+
+def _device_of(t):
+    """Context in which launches for ``t`` run on its device, current or not."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _scratch(nbytes, device):
+    """Scratch memory of one call, from torch's allocator and not from workspace(): under a stream capture it belongs to that graph, so
+    that graphs which are replayed side by side share none."""
+    with _on_launch_stream():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _pointer(t):
+    return t.data_ptr() if t is not None else None
 
 
 def workspace(nbytes, device):
@@ -1186,6 +1221,318 @@ def sample_categorical(logits, late=False):
     if valid is not None:
         valid.check()
     return targets
+
+
+def _filter_argument(value, name, rows, device, dtype, off):
+    """(number, tensor or None) of a filter that is one number for all rows, one per row, or None."""
+    if value is None:
+        return off, None
+    if not isinstance(value, torch.Tensor):
+        return value, None
+    if value.dtype != dtype or value.numel() != rows:
+        raise ValueError(f'{name} has to be a number or a {dtype} tensor with one element per row ({rows}). Got {value.dtype}, '
+                         f'{tuple(value.shape)}.')
+    _require_gpu(value)
+    _require_one_gpu(device, **{name: value})
+    return off, _contiguous(value.detach())
+
+
+def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min_p=None, late=False, check=True):
+    """One class per row of ``logits`` [..., classes] (float32, bfloat16, float16; any row stride) from softmax(logits / temperature)
+    restricted to
+      top_k  the k most probable classes (the lowest index first among equal ones; None or <= 0: all),
+      top_p  of those the most probable ones whose probability reaches top_p: a class is kept while the probability in front of it is
+             below top_p (None or >= 1: all),
+      min_p  classes of at least min_p times the largest probability (None or <= 0: all).
+    The most probable class is always kept; temperature 0 takes it.  The class is the first, by index, at which the probability of the
+    kept classes up to it exceeds ``u`` (float32 or float64, one number in [0, 1) per row; None: drawn here).  Each of the four may be a
+    tensor with one element per row instead (float32; top_k int64).  Logits of -inf are never drawn.
+    A row that holds NaN or +inf or nothing but -inf, or whose parameters or number are NaN, has no distribution: its class is -1 and,
+    as sample_categorical() does, the call raises torch.multinomial's RuntimeError, which waits for the draw; ``late``: returns (classes,
+    SampledLogits) instead, whose check() raises it; ``check=False``: the -1 is all.  (A stream capture has no check.)"""
+    _require_gpu(logits, u)
+    code = _element_type(logits, 'logits')
+    if logits.ndim == 0 or logits.shape[-1] == 0:
+        raise ValueError(f'logits have to have classes in their last dimension. Got the shape {tuple(logits.shape)}.')
+    classes = logits.shape[-1]
+    shape = logits.shape[:-1]
+    rows = logits.numel() // classes
+    device = logits.device
+    with _device_of(logits):
+        t, ts = _filter_argument(temperature, 'temperature', rows, device, torch.float32, 1.0)
+        k, ks = _filter_argument(top_k, 'top_k', rows, device, torch.int64, 0)
+        k = max(0, min(int(k), classes))
+        p, ps = _filter_argument(top_p, 'top_p', rows, device, torch.float32, 1.0)
+        m, ms = _filter_argument(min_p, 'min_p', rows, device, torch.float32, 0.0)
+        if not t >= 0:
+            raise ValueError(f'temperature has to be at least 0. Got {t}.')
+        if p != p or m != m:
+            raise ValueError(f'top_p and min_p have to be numbers. Got {p} and {m}.')
+        with _on_launch_stream():
+            if u is None:
+                u = torch.rand(shape, dtype=torch.float64, device=device)
+            targets = torch.empty(shape, dtype=torch.int64, device=device)
+        if u.dtype not in (torch.float32, torch.float64) or u.numel() != rows:
+            raise ValueError(f'u has to be a float32 or float64 tensor with one element per row ({rows}). Got {u.dtype}, {tuple(u.shape)}.')
+        _require_one_gpu(device, u=u)
+        u = _contiguous(u.detach())
+        x, ld = _rows_of(logits.detach(), classes, 'logits')
+        valid = SampledLogits(device) if (late or check) and rows and not torch.cuda.is_current_stream_capturing() else None
+        rc = _lib.load().ak_sample_filtered(x.data_ptr(), code, rows, classes, ld, u.data_ptr(), u.dtype == torch.float64, t, _pointer(ts),
+                                            k, _pointer(ks), p, _pointer(ps), m, _pointer(ms), targets.data_ptr(),
+                                            valid.address if valid is not None else None, _stream(device))
+        _lib.check(rc, 'ak_sample_filtered')
+        if valid is not None:
+            valid.record()
+    if late:
+        return targets, valid
+    if valid is not None:
+        valid.check()
+    return targets
+
+
+# ------------------------------------------------------------------------------ layer norm
+def _rows_of(t, F, what):
+    """``t`` as rows of F contiguous elements: (tensor that holds them, row stride).  Copied where one stride cannot reach the rows."""
+    if t.ndim == 0 or t.shape[-1] != F:
+        raise ValueError(f'{what} has to have {F} elements in its last dimension. Got the shape {tuple(t.shape)}.')
+    if t.is_contiguous():
+        return t, F
+    if t.stride(-1) == 1 or F == 1:
+        expect = None
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if expect is None:
+                first, expect = stride, stride * size
+            elif stride == expect:
+                expect *= size
+            else:
+                first = None
+                break
+        else:
+            if expect is None:
+                return t, F
+        if first is not None and first >= F:
+            return t, first
+    return _contiguous(t), F
+
+
+def _norm_vector(v, F, device, what):
+    """A weight or bias as F contiguous elements."""
+    if v is None:
+        return None
+    if v.numel() != F:
+        raise ValueError(f'{what} has to have {F} elements. Got {v.numel()}.')
+    _require_one_gpu(device, **{what: v})
+    return _contiguous(v.detach().reshape(-1))
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
+    """(y, mean, rstd) of layer norm over the last dimension of ``x``: y = (x - mean) * rstd * weight + bias,
+    rstd = (variance + eps)^(-1/2).  x: float32, bfloat16 or float16, any leading dimensions and row stride; weight and bias (each may
+    be None): one type of the three.  y has the type of x, or float32 with ``out_dtype=torch.float32``; mean and rstd (float32, one per
+    row) are what layer_norm_backward() needs."""
+    _require_gpu(x, weight, bias)
+    x_code = _element_type(x, 'x')
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError(f'x has to have elements in its last dimension. Got the shape {tuple(x.shape)}.')
+    if not eps >= 0:
+        raise ValueError(f'eps has to be at least 0. Got {eps}.')
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f'the result is {x.dtype} or float32. Got {out_dtype}.')
+    F = x.shape[-1]
+    rows = x.numel() // F
+    with _device_of(x):
+        x2, ldx = _rows_of(x.detach(), F, 'x')
+        weight, bias = _norm_vector(weight, F, x.device, 'weight'), _norm_vector(bias, F, x.device, 'bias')
+        given = weight if weight is not None else bias
+        w_code = _element_type(given, 'weight' if given is weight else 'bias') if given is not None else AK_F32
+        if weight is not None and bias is not None and weight.dtype != bias.dtype:
+            raise TypeError(f'weight and bias have to be of one type. Got {weight.dtype} and {bias.dtype}.')
+        with _on_launch_stream():
+            y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+            mean, rstd = torch.empty(2, *x.shape[:-1], dtype=torch.float32, device=x.device)
+        rc = _lib.load().ak_layer_norm(x2.data_ptr(), x_code, ldx, _pointer(weight), _pointer(bias), w_code, rows, F, eps, y.data_ptr(),
+                                       _ELEMENT_TYPES[out_dtype], F, mean.data_ptr(), rstd.data_ptr(), _stream(x.device))
+    _lib.check(rc, 'ak_layer_norm')
+    return y, mean, rstd
+
+
+def layer_norm_backward(g, x, mean, rstd, weight=None, blocks=None, alpha=1.0, beta=0.0, need_x=True, need_weight=True, need_bias=True,
+                        weight_dtype=None):
+    """(dx, dw, db) of layer_norm() for the gradient ``g`` of its result; None for what is not needed.  dx has the type of x, dw and db
+    that of the weight (without a weight: ``weight_dtype``, float32).  ``blocks`` (contiguous float32 [F, 2, 2]) receives the unit-wise
+    Fisher blocks in the same pass, blocks <- beta*blocks + alpha * sum over rows of [[gw^2, gw*gb], [gw*gb, gb^2]] with gw = g h,
+    gb = g: unit_wise_stats() of y and g, without its division by the weight."""
+    _require_gpu(g, x, mean, rstd, weight, blocks)
+    x_code, g_code = _element_type(x, 'x'), _element_type(g, 'g')
+    if g.shape != x.shape:
+        raise ValueError(f'shapes differ: {tuple(g.shape)} vs {tuple(x.shape)}')
+    if g.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f'g has to be {x.dtype} or float32. Got {g.dtype}.')
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError(f'x has to have elements in its last dimension. Got the shape {tuple(x.shape)}.')
+    F = x.shape[-1]
+    rows = x.numel() // F
+    for name, t in (('mean', mean), ('rstd', rstd)):
+        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
+            raise ValueError(f'{name} has to be the contiguous float32 tensor of layer_norm(), one element per row.')
+    if blocks is not None and (blocks.dtype != torch.float32 or blocks.shape != (F, 2, 2) or not blocks.is_contiguous()):
+        raise ValueError('blocks has to be a contiguous float32 [f, 2, 2] tensor')
+    _require_one_gpu(x.device, g=g, mean=mean, rstd=rstd, blocks=blocks)
+    with _device_of(x):
+        x2, ldx = _rows_of(x.detach(), F, 'x')
+        g2, ldg = _rows_of(g.detach(), F, 'g')
+        weight = _norm_vector(weight, F, x.device, 'weight')
+        if weight is not None:
+            weight_dtype = weight.dtype
+        weight_dtype = torch.float32 if weight_dtype is None else weight_dtype
+        if weight_dtype not in _ELEMENT_TYPES:
+            raise TypeError(f'weight has to be float32, bfloat16 or float16. Got {weight_dtype}.')
+        lib = _lib.load()
+        dx = dw = db = ws = None
+        with _on_launch_stream():
+            if need_x:
+                dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            if need_weight:
+                dw = torch.empty(F, dtype=weight_dtype, device=x.device)
+            if need_bias:
+                db = torch.empty(F, dtype=weight_dtype, device=x.device)
+        need = 0
+        if need_weight or need_bias or blocks is not None:
+            need = _ws_need('ak_layer_norm_backward_ws_bytes', rows, F, blocks is not None)
+            ws = _scratch(need, x.device)
+        rc = lib.ak_layer_norm_backward(g2.data_ptr(), g_code, ldg, x2.data_ptr(), x_code, ldx, mean.data_ptr(), rstd.data_ptr(),
+                                        _pointer(weight), _ELEMENT_TYPES[weight_dtype], rows, F, _pointer(dx), F, _pointer(dw),
+                                        _pointer(db), _pointer(blocks), alpha, beta, _pointer(ws), need, _stream(x.device))
+    _lib.check(rc, 'ak_layer_norm_backward')
+    return dx, dw, db
+
+
+# ------------------------------------------------------------------------------ norm of all gradients
+_NORM_KINDS = {2.0: 0, 1.0: 1, float('inf'): 2}
+
+
+def _dense(t):
+    """Whether the elements of ``t`` fill one run of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, si) for si, st in zip(t.shape, t.stride()) if si != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _norm_items(grads, outs):
+    """(device, rows of ak_clip_grad_norm, [(tensor, dense one whose values it takes after the launch)]) of gradients and where their
+    scaled values go; outs None: only the norm is asked for."""
+    rows, late, device, seen = [], [], None, {}
+    for i, grad in enumerate(grads):
+        code = _ELEMENT_TYPES.get(grad.dtype)
+        if code is None or grad.device != device:
+            _require_gpu(grad)
+            _element_type(grad, 'a gradient')
+            if device is None:
+                device = grad.device
+            _require_one_gpu(device, gradient=grad)
+        out = None if outs is None else outs[i]
+        if out is not None and out is not grad:
+            _require_gpu(out)
+            _require_one_gpu(device, result=out)
+            if out.shape != grad.shape or out.dtype not in (grad.dtype, torch.float32):
+                raise ValueError(f'the result of a gradient has its shape and its type or float32. Got {tuple(out.shape)}, {out.dtype} for '
+                                 f'{tuple(grad.shape)}, {grad.dtype}.')
+        n = grad.numel()
+        if n == 0:
+            continue
+        if out is not None and any(st == 0 and size > 1 for st, size in zip(out.stride(), out.shape)):
+            raise ValueError('a tensor whose elements share memory (an expanded one) cannot take scaled values.')
+        dense = _dense(grad)
+        key = (grad.data_ptr(), n) if dense else (grad.data_ptr(), grad.shape, grad.stride())
+        if key in seen:                       # a gradient that two parameters share counts once
+            first, first_out = seen[key]
+            if out is not None and out.data_ptr() != first_out.data_ptr():
+                if first.stride() != grad.stride() and not (first.is_contiguous() and grad.is_contiguous()):
+                    raise ValueError('a gradient that is listed twice, in two orders of its elements, has no two results.')
+                late.append((out, first_out))
+            continue
+        seen[key] = grad, out
+        src, dst = grad, out
+        if out is None:
+            src = grad if dense else _contiguous(grad)
+        elif not (grad.stride() == out.stride() and dense) and not (grad.is_contiguous() and out.is_contiguous()):
+            src = _contiguous(grad)
+            if out is grad:
+                dst = src
+            elif not out.is_contiguous():
+                with _on_launch_stream():
+                    dst = torch.empty(out.shape, dtype=out.dtype, device=device)
+            if dst is not out:
+                late.append((out, dst))
+        rows.append((src, dst, n, code))
+    return device, rows, late
+
+
+def _launch_norm(rows, device, norm_type, max_norm):
+    lib = _lib.load()
+    table = []
+    for src, dst, n, code in rows:
+        table += (src.data_ptr(), 0 if dst is None else dst.data_ptr(), n, code, code if dst is None else _ELEMENT_TYPES[dst.dtype])
+    table = (ctypes.c_int64 * len(table))(*table)
+    need = lib.ak_grad_norm_ws_bytes(len(rows))
+    with _on_launch_stream():
+        norm = torch.empty((), dtype=torch.float32, device=device)
+    ws = _scratch(need, device)
+    kind = _NORM_KINDS[norm_type]
+    if max_norm is None:
+        _lib.check(lib.ak_grad_norm(table, len(rows), kind, norm.data_ptr(), ws.data_ptr(), need, _stream(device)), 'ak_grad_norm')
+    else:
+        rc = lib.ak_clip_grad_norm(table, len(rows), kind, max_norm, norm.data_ptr(), ws.data_ptr(), need, _stream(device))
+        _lib.check(rc, 'ak_clip_grad_norm')
+    return norm
+
+
+def _norm_arguments(grads, norm_type):
+    grads = [g.detach() for g in grads]
+    if not grads:
+        raise ValueError('there is no gradient to take a norm of.')
+    if float(norm_type) not in _NORM_KINDS:
+        raise ValueError(f'norm_type has to be 2, 1 or inf. Got {norm_type}.')
+    _require_gpu(grads[0])
+    return grads
+
+
+def grad_norm(grads, norm_type=2.0):
+    """The norm of all elements of ``grads`` (tensors of float32, bfloat16 or float16 on one device) as one vector, a 0-d float32 tensor:
+    norm_type 2, 1 or inf.  Sums are double, in a fixed order.  A gradient that is listed twice counts once."""
+    grads = _norm_arguments(grads, norm_type)
+    with _device_of(grads[0]):
+        device, rows, _ = _norm_items(grads, None)
+        return _launch_norm(rows, device, float(norm_type), None)
+
+
+def clip_grad_norm(grads, max_norm, norm_type=2.0, outs=None):
+    """Scales ``grads`` in place by min(1, max_norm / (norm + 1e-6)) and returns their norm before, as grad_norm() gives it; with ``outs``
+    the gradients stay and the scaled values go to these tensors (of the same shapes; of the gradient's type or float32).  A norm that is
+    infinite gives the factor 0, one that is NaN the factor NaN, as torch.nn.utils.clip_grad_norm_ does.  Gradients (results) of
+    different entries may not overlap, except that one listed twice is scaled once.  Nothing is read by the host."""
+    grads = _norm_arguments(grads, norm_type)
+    if not max_norm >= 0:
+        raise ValueError(f'max_norm has to be at least 0. Got {max_norm}.')
+    outs = grads if outs is None else [o.detach() for o in outs]
+    if len(outs) != len(grads):
+        raise ValueError(f'{len(grads)} gradients and {len(outs)} results.')
+    with _device_of(grads[0]):
+        device, rows, late = _norm_items(grads, outs)
+        norm = _launch_norm(rows, device, float(norm_type), max_norm)
+        with _on_launch_stream():
+            for out, dense in late:
+                out.copy_(dense.reshape(out.shape))
+    return norm
 
 
 # ------------------------------------------------------------------------------ low-rank (swift) factors

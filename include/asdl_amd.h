@@ -43,6 +43,8 @@ extern "C" {
                               * for statistics whose inverse roots are taken with a ridge of 1e-6 of the largest eigenvalue,
                               * where another order moves the root of a rank-deficient statistic by 0.5-1 % */
 
+#define AK_F16 4             /* IEEE half: ak_layer_norm*, ak_grad_norm, ak_clip_grad_norm, ak_sample_filtered */
+
 #define AK_OK 0
 #define AK_ERR_ARG -1        /* null pointer, negative size, unknown dtype */
 #define AK_ERR_WORKSPACE -2  /* workspace missing or too small */
@@ -195,6 +197,19 @@ int ak_kron_precond_deep(const int64_t* items, int count, const int64_t* units, 
 int ak_sample_categorical(const float* logits, const float* q, int64_t rows, int64_t classes, int64_t* targets,
                           int* invalid, ak_stream_t stream);
 
+/* targets[r] = a draw of softmax(logits[r] / T) restricted by top-k, top-p and min-p, from the uniform number u[r] in [0, 1).
+ * Classes in the order of their logits, equal ones by index; weights exp((logit - max) / T).  top-k (<= 0: off) keeps the first k;
+ * top-p (>= 1: off; <= 0: the first class) keeps a class while the weight in front of it is below top_p times the weight that top-k
+ * left; min-p (<= 0: off) keeps weights of at least min_p.  The most probable class is always kept.  The draw is the lowest index at
+ * which the kept weight up to it exceeds u times all of it.  T = 0 takes the first class.  Sums are integers: the draw depends on no
+ * order of sums.  logits: `dtype` AK_F32 / AK_BF16 / AK_F16, row stride ld >= classes, classes contiguous, any alignment; logits of
+ * -inf are never drawn.  u: float or double (u_is_double) [rows].  temperatures, top_ks, top_ps, min_ps [rows] (device, each may be
+ * null) replace the four numbers.  A row with a NaN or +inf, with nothing but -inf, with a NaN parameter, a NaN u or a negative T has
+ * target -1 and sets *invalid (may be null; device or pinned host word, cleared by the caller) to 1. */
+int ak_sample_filtered(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t ld, const void* u, int u_is_double,
+                       double temperature, const float* temperatures, int64_t top_k, const int64_t* top_ks, double top_p,
+                       const float* top_ps, double min_p, const float* min_ps, int64_t* targets, int* invalid, ak_stream_t stream);
+
 /* ak_kron_damping for pairs whose factors may be n x d row matrices: dims = device int64 [batch,4]
  * (rows_A, d_A, rows_B, d_B; rows = 0: square d x d factor, eigenvalue mean trace/d; rows > 0: sum(x^2)/d),
  * eig_scale = device float [batch,2] multiplied into the eigenvalue means (may be null).
@@ -297,6 +312,34 @@ int ak_unit_wise_mvp(const float* mat, int64_t F, float* vec_weight, float* vec_
  * vec_weight, vec_bias (addresses), F, first_block (running sum of ceil(F/256)); total_blocks that sum over all
  * rows.  The unit-wise modules of the loop at asdl/precondition/natural_gradient.py:481-486. */
 int ak_unit_wise_mvp_grouped(const int64_t* table, int count, int64_t total_blocks, float scale, ak_stream_t stream);
+
+/* ---- layer norm --------------------------------------------------------------------- */
+
+/* y[r] = (x[r] - mean[r]) rstd[r] weight + bias over rows of F elements (strides ldx, ldy; elements contiguous, any alignment), with
+ * rstd = (variance + eps)^(-1/2); mean and rstd [rows] are for the backward pass.  x: AK_F32 / AK_BF16 / AK_F16, y: the type of x or
+ * AK_F32; weight, bias (each may be null): w_dtype. */
+int ak_layer_norm(const void* x, int x_dtype, int64_t ldx, const void* weight, const void* bias, int w_dtype, int64_t rows, int64_t F,
+                  float eps, void* y, int y_dtype, int64_t ldy, float* mean, float* rstd, ak_stream_t stream);
+
+/* dx (type of x), dw = sum_rows g h, db = sum_rows g (w_dtype) for h = (x - mean) rstd and the gradient g of y (type of x or AK_F32);
+ * each may be null.  blocks (may be null; fp32 [F, 2, 2]) <- beta blocks + alpha sum_rows [[(g h)^2, g^2 h], [g^2 h, g^2]]: what
+ * ak_unit_wise_stats gives from y and g, without dividing by the weight.  g may be null when rows is 0. */
+size_t ak_layer_norm_backward_ws_bytes(int64_t rows, int64_t F, int with_blocks);
+int ak_layer_norm_backward(const void* g, int g_dtype, int64_t ldg, const void* x, int x_dtype, int64_t ldx, const float* mean,
+                           const float* rstd, const void* weight, int w_dtype, int64_t rows, int64_t F, void* dx, int64_t lddx,
+                           void* dw, void* db, float* blocks, float alpha, float beta, void* ws, size_t ws_bytes, ak_stream_t stream);
+
+/* ---- norm of all gradients ------------------------------------------------------------ */
+
+/* norm <- (sum x^2)^(1/2) (kind 0), sum |x| (1) or max |x| (2) over the elements of all tensors; ak_clip_grad_norm also writes
+ * min(1, max_norm / (norm + 1e-6)) x of every tensor to its result.  Sums are double, in a fixed order; a NaN or an infinity shows in
+ * the norm, and the factor is then NaN or 0.  items (HOST memory): rows of 5 int64: x, result (may be x; ak_grad_norm ignores it),
+ * elements (dense, aligned to the element), type of x (AK_F32 / AK_BF16 / AK_F16), type of the result (that of x or AK_F32).  Results
+ * do not overlap each other or another tensor. */
+size_t ak_grad_norm_ws_bytes(int count);
+int ak_grad_norm(const int64_t* items, int count, int kind, float* norm, void* ws, size_t ws_bytes, ak_stream_t stream);
+int ak_clip_grad_norm(const int64_t* items, int count, int kind, double max_norm, float* norm, void* ws, size_t ws_bytes,
+                      ak_stream_t stream);
 
 /* ---- saved factors ----------------------------------------------------------------- */
 
