@@ -23,17 +23,39 @@ inline int with_type(int dtype, Fn&& fn) {
 
 inline bool is_element_type(int dtype) { return dtype == AK_F32 || dtype == AK_BF16 || dtype == AK_F16; }
 
-// One element of a type known at run time (weights, biases: a few per lane).
-__device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t i) {
-  if (dtype == AK_F32) return static_cast<const float*>(p)[i];
-  if (dtype == AK_BF16) return static_cast<float>(static_cast<const __bf16*>(p)[i]);
-  return static_cast<float>(static_cast<const _Float16*>(p)[i]);
+// N neighbouring elements on their way, at any alignment (unaligned 16-byte loads and stores are one instruction).
+template <typename T, int N>
+struct Some {
+  typedef T vec __attribute__((ext_vector_type(N)));
+  vec v;
+  __device__ __forceinline__ void load(const T* __restrict__ p) { __builtin_memcpy(&v, p, sizeof(T) * N); }
+  __device__ __forceinline__ void clear() { v = vec{}; }
+  __device__ __forceinline__ float get(int e) const { return static_cast<float>(v[e]); }
+  __device__ __forceinline__ void set(int e, float x) { v[e] = static_cast<T>(x); }
+  __device__ __forceinline__ void store(T* __restrict__ p) const { __builtin_memcpy(p, &v, sizeof(T) * N); }
+};
+
+// v + v of the lane that a data-parallel-primitive control selects.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 
-__device__ __forceinline__ void store_from_float(void* p, int dtype, int64_t i, float v) {
-  if (dtype == AK_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == AK_BF16) static_cast<__bf16*>(p)[i] = static_cast<__bf16>(v);
-  else static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
+// The sum over L = 16 or 64 neighbouring lanes, in each of them: swaps of neighbours, of pairs, mirrored halves and rows of 16 (moves
+// between lanes as operands of the addition, where __shfl_xor goes through the LDS six times), then the four rows of a wave.
+template <int L = 64>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = add_dpp<0xB1>(v);          // quad_perm 1 0 3 2
+  v = add_dpp<0x4E>(v);          // quad_perm 2 3 0 1
+  v = add_dpp<0x141>(v);         // row_half_mirror
+  v = add_dpp<0x140>(v);         // row_mirror
+  if constexpr (L == 64) {
+    const int b = __builtin_bit_cast(int, v);
+    const float r0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0)), r1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16));
+    const float r2 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 32)), r3 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48));
+    v = (r0 + r1) + (r2 + r3);
+  }
+  return v;
 }
 
 template <typename V>
@@ -41,6 +63,10 @@ __device__ __forceinline__ V wave_sum(V v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
+}
+template <>
+__device__ __forceinline__ float wave_sum<float>(float v) {
+  return lanes_sum<64>(v);
 }
 
 // The sum over a work group of WAVES waves, in every thread; `red` has WAVES words.  The barrier in front keeps the words of the

@@ -40,9 +40,12 @@ __device__ __forceinline__ int gn_find(const Table& t, int chunk) {
   return lo;
 }
 
-// Types in the tables: 0 fp32, 1 bf16, 2 fp16.
-__device__ __forceinline__ float gn_load(const void* p, int type, int64_t i) {
-  return load_as_float(p, type == 0 ? AK_F32 : type == 1 ? AK_BF16 : AK_F16, i);
+// Types in the tables: 0 fp32, 1 bf16, 2 fp16.  fn(Type<T>{}), the same for all lanes.
+template <typename Fn>
+__device__ __forceinline__ void gn_with_type(int type, Fn&& fn) {
+  if (type == 0) fn(Type<float>{});
+  else if (type == 1) fn(Type<__bf16>{});
+  else fn(Type<_Float16>{});
 }
 
 // KIND 0: sum x^2, 1: sum |x|, 2: max |x| (as the bits of a float's magnitude: NaN is above all numbers)
@@ -80,7 +83,11 @@ static __global__ __launch_bounds__(kGnThreads) void gn_partial_kernel(GnNormTab
     const int i = gn_find(t, chunk);
     const int64_t n = t.size[i] >> 2, from = (chunk - t.first[i]) * kGnChunk, to = from + kGnChunk < n ? from + kGnChunk : n;
     const int type = static_cast<int>(t.size[i] & 3);
-    for (int64_t e = from + threadIdx.x; e < to; e += kGnThreads) acc = gn_take<KIND>(acc, gn_load(t.src[i], type, e));
+    gn_with_type(type, [&](auto xt) {
+      using X = typename decltype(xt)::type;
+      const X* __restrict__ x = static_cast<const X*>(t.src[i]);
+      for (int64_t e = from + threadIdx.x; e < to; e += kGnThreads) acc = gn_take<KIND>(acc, static_cast<float>(x[e]));
+    });
   }
   acc = gn_group<KIND>(acc, red);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
@@ -114,8 +121,17 @@ static __global__ __launch_bounds__(kGnThreads) void gn_clip_kernel(GnClipTable 
     if (c == 1.f && t.src[i] == t.dst[i]) continue;
     const int64_t n_el = t.size[i] >> 4, from = (chunk - t.first[i]) * kGnChunk, to = from + kGnChunk < n_el ? from + kGnChunk : n_el;
     const int type = static_cast<int>(t.size[i] & 3), to_type = static_cast<int>(t.size[i] >> 2 & 3);
-    for (int64_t e = from + threadIdx.x; e < to; e += kGnThreads)
-      store_from_float(t.dst[i], to_type == 0 ? AK_F32 : to_type == 1 ? AK_BF16 : AK_F16, e, c * gn_load(t.src[i], type, e));
+    gn_with_type(type, [&](auto xt) {
+      using X = typename decltype(xt)::type;
+      auto scale = [&](auto yt) {
+        using Y = typename decltype(yt)::type;
+        const X* x = static_cast<const X*>(t.src[i]);
+        Y* y = static_cast<Y*>(t.dst[i]);
+        for (int64_t e = from + threadIdx.x; e < to; e += kGnThreads) y[e] = static_cast<Y>(c * static_cast<float>(x[e]));
+      };
+      if (to_type == type) scale(Type<X>{});
+      else scale(Type<float>{});
+    });
   }
 }
 

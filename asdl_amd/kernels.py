@@ -1331,7 +1331,7 @@ def _norm_vector(v, F, device, what):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     """(y, mean, rstd) of layer norm over the last dimension of ``x``: y = (x - mean) * rstd * weight + bias,
     rstd = (variance + eps)^(-1/2).  x: float32, bfloat16 or float16, any leading dimensions and row stride; weight and bias (each may
-    be None): one type of the three.  y has the type of x, or float32 with ``out_dtype=torch.float32``; mean and rstd (float32, one per
+    be None): of the type of x or float32, both of one.  y has the type of x, or float32 with ``out_dtype=torch.float32``; mean and rstd (float32, one per
     row) are what layer_norm_backward() needs."""
     _require_gpu(x, weight, bias)
     x_code = _element_type(x, 'x')
@@ -1351,6 +1351,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
         w_code = _element_type(given, 'weight' if given is weight else 'bias') if given is not None else AK_F32
         if weight is not None and bias is not None and weight.dtype != bias.dtype:
             raise TypeError(f'weight and bias have to be of one type. Got {weight.dtype} and {bias.dtype}.')
+        if w_code not in (x_code, AK_F32):
+            raise TypeError(f'weight and bias have to be {x.dtype} or float32. Got {given.dtype}.')
         with _on_launch_stream():
             y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
             mean, rstd = torch.empty(2, *x.shape[:-1], dtype=torch.float32, device=x.device)
@@ -1389,8 +1391,8 @@ def layer_norm_backward(g, x, mean, rstd, weight=None, blocks=None, alpha=1.0, b
         if weight is not None:
             weight_dtype = weight.dtype
         weight_dtype = torch.float32 if weight_dtype is None else weight_dtype
-        if weight_dtype not in _ELEMENT_TYPES:
-            raise TypeError(f'weight has to be float32, bfloat16 or float16. Got {weight_dtype}.')
+        if weight_dtype not in (x.dtype, torch.float32):
+            raise TypeError(f'the weight has to be {x.dtype} or float32. Got {weight_dtype}.')
         lib = _lib.load()
         dx = dw = db = ws = None
         with _on_launch_stream():

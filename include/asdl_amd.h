@@ -317,7 +317,7 @@ int ak_unit_wise_mvp_grouped(const int64_t* table, int count, int64_t total_bloc
 
 /* y[r] = (x[r] - mean[r]) rstd[r] weight + bias over rows of F elements (strides ldx, ldy; elements contiguous, any alignment), with
  * rstd = (variance + eps)^(-1/2); mean and rstd [rows] are for the backward pass.  x: AK_F32 / AK_BF16 / AK_F16, y: the type of x or
- * AK_F32; weight, bias (each may be null): w_dtype. */
+ * AK_F32; weight, bias (each may be null): w_dtype, the type of x or AK_F32. */
 int ak_layer_norm(const void* x, int x_dtype, int64_t ldx, const void* weight, const void* bias, int w_dtype, int64_t rows, int64_t F,
                   float eps, void* y, int y_dtype, int64_t ldy, float* mean, float* rstd, ak_stream_t stream);
 

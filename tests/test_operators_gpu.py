@@ -209,7 +209,7 @@ def test_layer_norm_refuses(K):
     x, w = rand(4, 64, seed=1), rand(64, seed=2)
     _, mean, rstd = K.layer_norm(x)
     for call, kind in [(lambda: K.layer_norm(x.double()), TypeError), (lambda: K.layer_norm(x, w[:63]), ValueError),
-                       (lambda: K.layer_norm(x, w, w.bfloat16()), TypeError), (lambda: K.layer_norm(x, eps=-1e-5), ValueError),
+                       (lambda: K.layer_norm(x, w, w.bfloat16()), TypeError), (lambda: K.layer_norm(x, w.bfloat16()), TypeError), (lambda: K.layer_norm(x, eps=-1e-5), ValueError),
                        (lambda: K.layer_norm(x, eps=float('nan')), ValueError), (lambda: K.layer_norm(x, out_dtype=F16), TypeError),
                        (lambda: K.layer_norm(x.bfloat16(), out_dtype=F16), TypeError), (lambda: K.layer_norm(x[:, :0]), ValueError),
                        (lambda: K.layer_norm(x[0, 0]), ValueError), (lambda: K.layer_norm(x, w.cpu()), RuntimeError),
