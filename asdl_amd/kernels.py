@@ -172,11 +172,12 @@ def _require_one_gpu(device, **tensors):
             raise ValueError(f'{name} is on {t.device}, the first operand on {device}.')
 
 
-def _device_of(t):
-    """Context in which launches for ``t`` run on its device, current or not."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+_here = contextlib.nullcontext()
+
+
+def _device_of(device):
+    """Context in which launches for a tensor run on its device, current or not."""
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _scratch(nbytes, device):
@@ -346,7 +347,7 @@ def _on_launch_stream():
     """Context for the few framework ops (copies to a contiguous layout, casts) that feed a kernel: they have to run
     on the stream the kernel is launched on."""
     st = getattr(_override, 'stream', None)
-    return torch.cuda.stream(st) if st is not None else contextlib.nullcontext()
+    return torch.cuda.stream(st) if st is not None else _here
 
 
 def _contiguous(x):
@@ -1232,9 +1233,10 @@ def _filter_argument(value, name, rows, device, dtype, off):
     if value.dtype != dtype or value.numel() != rows:
         raise ValueError(f'{name} has to be a number or a {dtype} tensor with one element per row ({rows}). Got {value.dtype}, '
                          f'{tuple(value.shape)}.')
-    _require_gpu(value)
-    _require_one_gpu(device, **{name: value})
-    return off, _contiguous(value.detach())
+    if value.device != device:
+        _require_gpu(value)
+        _require_one_gpu(device, **{name: value})
+    return off, _contiguous(value)
 
 
 def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min_p=None, late=False, check=True):
@@ -1250,15 +1252,17 @@ def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min
     A row that holds NaN or +inf or nothing but -inf, or whose parameters or number are NaN, has no distribution: its class is -1 and,
     as sample_categorical() does, the call raises torch.multinomial's RuntimeError, which waits for the draw; ``late``: returns (classes,
     SampledLogits) instead, whose check() raises it; ``check=False``: the -1 is all.  (A stream capture has no check.)"""
-    _require_gpu(logits, u)
-    code = _element_type(logits, 'logits')
+    code = _ELEMENT_TYPES.get(logits.dtype)
+    if code is None or not logits.is_cuda:
+        _require_gpu(logits)
+        _element_type(logits, 'logits')
     if logits.ndim == 0 or logits.shape[-1] == 0:
         raise ValueError(f'logits have to have classes in their last dimension. Got the shape {tuple(logits.shape)}.')
     classes = logits.shape[-1]
     shape = logits.shape[:-1]
     rows = logits.numel() // classes
     device = logits.device
-    with _device_of(logits):
+    with _device_of(device):
         t, ts = _filter_argument(temperature, 'temperature', rows, device, torch.float32, 1.0)
         k, ks = _filter_argument(top_k, 'top_k', rows, device, torch.int64, 0)
         k = max(0, min(int(k), classes))
@@ -1274,13 +1278,15 @@ def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min
             targets = torch.empty(shape, dtype=torch.int64, device=device)
         if u.dtype not in (torch.float32, torch.float64) or u.numel() != rows:
             raise ValueError(f'u has to be a float32 or float64 tensor with one element per row ({rows}). Got {u.dtype}, {tuple(u.shape)}.')
-        _require_one_gpu(device, u=u)
-        u = _contiguous(u.detach())
-        x, ld = _rows_of(logits.detach(), classes, 'logits')
+        if u.device != device:
+            _require_gpu(u)
+            _require_one_gpu(device, u=u)
+        u = _contiguous(u)
+        x, ld = _rows_of(logits, classes)
         valid = SampledLogits(device) if (late or check) and rows and not torch.cuda.is_current_stream_capturing() else None
         rc = _lib.load().ak_sample_filtered(x.data_ptr(), code, rows, classes, ld, u.data_ptr(), u.dtype == torch.float64, t, _pointer(ts),
                                             k, _pointer(ks), p, _pointer(ps), m, _pointer(ms), targets.data_ptr(),
-                                            valid.address if valid is not None else None, _stream(device))
+                                            valid.address if valid is not None else None, _stream_handle(device))
         _lib.check(rc, 'ak_sample_filtered')
         if valid is not None:
             valid.record()
@@ -1292,10 +1298,8 @@ def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min
 
 
 # ------------------------------------------------------------------------------ layer norm
-def _rows_of(t, F, what):
+def _rows_of(t, F):
     """``t`` as rows of F contiguous elements: (tensor that holds them, row stride).  Copied where one stride cannot reach the rows."""
-    if t.ndim == 0 or t.shape[-1] != F:
-        raise ValueError(f'{what} has to have {F} elements in its last dimension. Got the shape {tuple(t.shape)}.')
     if t.is_contiguous():
         return t, F
     if t.stride(-1) == 1 or F == 1:
@@ -1315,49 +1319,62 @@ def _rows_of(t, F, what):
                 return t, F
         if first is not None and first >= F:
             return t, first
-    return _contiguous(t), F
+    return _contiguous(t.detach()), F
 
 
-def _norm_vector(v, F, device, what):
-    """A weight or bias as F contiguous elements."""
-    if v is None:
-        return None
+def _norm_vector(v, F, x, what):
+    """A weight or bias of a layer norm as F contiguous elements of the type of ``x`` or float32."""
     if v.numel() != F:
         raise ValueError(f'{what} has to have {F} elements. Got {v.numel()}.')
-    _require_one_gpu(device, **{what: v})
-    return _contiguous(v.detach().reshape(-1))
+    if v.dtype != torch.float32 and v.dtype != x.dtype:
+        raise TypeError(f'{what} has to be {x.dtype} or float32. Got {v.dtype}.')
+    if v.device != x.device:
+        _require_gpu(v)
+        _require_one_gpu(x.device, **{what: v})
+    return v if v.is_contiguous() else _contiguous(v.detach().reshape(-1))
+
+
+def _norm_rows(x):
+    """(type code, features, rows) of a tensor whose last dimension is normalised."""
+    code = _ELEMENT_TYPES.get(x.dtype)
+    if code is None or not x.is_cuda:
+        _require_gpu(x)
+        _element_type(x, 'x')
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError(f'x has to have elements in its last dimension. Got the shape {tuple(x.shape)}.')
+    F = x.shape[-1]
+    return code, F, x.numel() // F
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     """(y, mean, rstd) of layer norm over the last dimension of ``x``: y = (x - mean) * rstd * weight + bias,
     rstd = (variance + eps)^(-1/2).  x: float32, bfloat16 or float16, any leading dimensions and row stride; weight and bias (each may
-    be None): of the type of x or float32, both of one.  y has the type of x, or float32 with ``out_dtype=torch.float32``; mean and rstd (float32, one per
-    row) are what layer_norm_backward() needs."""
-    _require_gpu(x, weight, bias)
-    x_code = _element_type(x, 'x')
-    if x.ndim == 0 or x.shape[-1] == 0:
-        raise ValueError(f'x has to have elements in its last dimension. Got the shape {tuple(x.shape)}.')
+    be None): of the type of x or float32, both of one.  y has the type of x, or float32 with ``out_dtype=torch.float32``; mean and rstd
+    (float32, one per row) are what layer_norm_backward() needs."""
+    x_code, F, rows = _norm_rows(x)
     if not eps >= 0:
         raise ValueError(f'eps has to be at least 0. Got {eps}.')
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in (x.dtype, torch.float32):
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype != x.dtype and out_dtype != torch.float32:
         raise TypeError(f'the result is {x.dtype} or float32. Got {out_dtype}.')
-    F = x.shape[-1]
-    rows = x.numel() // F
-    with _device_of(x):
-        x2, ldx = _rows_of(x.detach(), F, 'x')
-        weight, bias = _norm_vector(weight, F, x.device, 'weight'), _norm_vector(bias, F, x.device, 'bias')
-        given = weight if weight is not None else bias
-        w_code = _element_type(given, 'weight' if given is weight else 'bias') if given is not None else AK_F32
-        if weight is not None and bias is not None and weight.dtype != bias.dtype:
-            raise TypeError(f'weight and bias have to be of one type. Got {weight.dtype} and {bias.dtype}.')
-        if w_code not in (x_code, AK_F32):
-            raise TypeError(f'weight and bias have to be {x.dtype} or float32. Got {given.dtype}.')
+    device = x.device
+    with _device_of(device):
+        x, ldx = _rows_of(x, F)
+        w_dtype = torch.float32
+        if bias is not None:
+            bias = _norm_vector(bias, F, x, 'bias')
+            w_dtype = bias.dtype
+        if weight is not None:
+            weight = _norm_vector(weight, F, x, 'weight')
+            if bias is not None and weight.dtype != w_dtype:
+                raise TypeError(f'weight and bias have to be of one type. Got {weight.dtype} and {w_dtype}.')
+            w_dtype = weight.dtype
         with _on_launch_stream():
-            y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-            mean, rstd = torch.empty(2, *x.shape[:-1], dtype=torch.float32, device=x.device)
-        rc = _lib.load().ak_layer_norm(x2.data_ptr(), x_code, ldx, _pointer(weight), _pointer(bias), w_code, rows, F, eps, y.data_ptr(),
-                                       _ELEMENT_TYPES[out_dtype], F, mean.data_ptr(), rstd.data_ptr(), _stream(x.device))
+            y = torch.empty(x.shape, dtype=out_dtype, device=device)
+            mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=device)
+        rc = _lib.load().ak_layer_norm(x.data_ptr(), x_code, ldx, _pointer(weight), _pointer(bias), _ELEMENT_TYPES[w_dtype], rows, F, eps,
+                                       y.data_ptr(), _ELEMENT_TYPES[out_dtype], F, mean.data_ptr(), rstd.data_ptr(), _stream_handle(device))
     _lib.check(rc, 'ak_layer_norm')
     return y, mean, rstd
 
@@ -1368,47 +1385,47 @@ def layer_norm_backward(g, x, mean, rstd, weight=None, blocks=None, alpha=1.0, b
     that of the weight (without a weight: ``weight_dtype``, float32).  ``blocks`` (contiguous float32 [F, 2, 2]) receives the unit-wise
     Fisher blocks in the same pass, blocks <- beta*blocks + alpha * sum over rows of [[gw^2, gw*gb], [gw*gb, gb^2]] with gw = g h,
     gb = g: unit_wise_stats() of y and g, without its division by the weight."""
-    _require_gpu(g, x, mean, rstd, weight, blocks)
-    x_code, g_code = _element_type(x, 'x'), _element_type(g, 'g')
+    x_code, F, rows = _norm_rows(x)
+    g_code = _ELEMENT_TYPES.get(g.dtype)
     if g.shape != x.shape:
         raise ValueError(f'shapes differ: {tuple(g.shape)} vs {tuple(x.shape)}')
-    if g.dtype not in (x.dtype, torch.float32):
+    if g_code != x_code and g_code != AK_F32:
         raise TypeError(f'g has to be {x.dtype} or float32. Got {g.dtype}.')
-    if x.ndim == 0 or x.shape[-1] == 0:
-        raise ValueError(f'x has to have elements in its last dimension. Got the shape {tuple(x.shape)}.')
-    F = x.shape[-1]
-    rows = x.numel() // F
     for name, t in (('mean', mean), ('rstd', rstd)):
         if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
             raise ValueError(f'{name} has to be the contiguous float32 tensor of layer_norm(), one element per row.')
     if blocks is not None and (blocks.dtype != torch.float32 or blocks.shape != (F, 2, 2) or not blocks.is_contiguous()):
         raise ValueError('blocks has to be a contiguous float32 [f, 2, 2] tensor')
-    _require_one_gpu(x.device, g=g, mean=mean, rstd=rstd, blocks=blocks)
-    with _device_of(x):
-        x2, ldx = _rows_of(x.detach(), F, 'x')
-        g2, ldg = _rows_of(g.detach(), F, 'g')
-        weight = _norm_vector(weight, F, x.device, 'weight')
+    device = x.device
+    if g.device != device or mean.device != device or rstd.device != device or (blocks is not None and blocks.device != device):
+        _require_gpu(g, mean, rstd, blocks)
+        _require_one_gpu(device, g=g, mean=mean, rstd=rstd, blocks=blocks)
+    with _device_of(device):
+        x, ldx = _rows_of(x, F)
+        g, ldg = _rows_of(g, F)
         if weight is not None:
+            weight = _norm_vector(weight, F, x, 'weight')
             weight_dtype = weight.dtype
-        weight_dtype = torch.float32 if weight_dtype is None else weight_dtype
-        if weight_dtype not in (x.dtype, torch.float32):
+        elif weight_dtype is None:
+            weight_dtype = torch.float32
+        elif weight_dtype != x.dtype and weight_dtype != torch.float32:
             raise TypeError(f'the weight has to be {x.dtype} or float32. Got {weight_dtype}.')
         lib = _lib.load()
         dx = dw = db = ws = None
+        need = 0
         with _on_launch_stream():
             if need_x:
-                dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                dx = torch.empty(x.shape, dtype=x.dtype, device=device)
             if need_weight:
-                dw = torch.empty(F, dtype=weight_dtype, device=x.device)
+                dw = torch.empty(F, dtype=weight_dtype, device=device)
             if need_bias:
-                db = torch.empty(F, dtype=weight_dtype, device=x.device)
-        need = 0
-        if need_weight or need_bias or blocks is not None:
-            need = _ws_need('ak_layer_norm_backward_ws_bytes', rows, F, blocks is not None)
-            ws = _scratch(need, x.device)
-        rc = lib.ak_layer_norm_backward(g2.data_ptr(), g_code, ldg, x2.data_ptr(), x_code, ldx, mean.data_ptr(), rstd.data_ptr(),
+                db = torch.empty(F, dtype=weight_dtype, device=device)
+            if need_weight or need_bias or blocks is not None:
+                need = _ws_need('ak_layer_norm_backward_ws_bytes', rows, F, blocks is not None)
+                ws = torch.empty(need, dtype=torch.uint8, device=device)
+        rc = lib.ak_layer_norm_backward(g.data_ptr(), g_code, ldg, x.data_ptr(), x_code, ldx, mean.data_ptr(), rstd.data_ptr(),
                                         _pointer(weight), _ELEMENT_TYPES[weight_dtype], rows, F, _pointer(dx), F, _pointer(dw),
-                                        _pointer(db), _pointer(blocks), alpha, beta, _pointer(ws), need, _stream(x.device))
+                                        _pointer(db), _pointer(blocks), alpha, beta, _pointer(ws), need, _stream_handle(device))
     _lib.check(rc, 'ak_layer_norm_backward')
     return dx, dw, db
 
@@ -1491,9 +1508,9 @@ def _launch_norm(rows, device, norm_type, max_norm):
     ws = _scratch(need, device)
     kind = _NORM_KINDS[norm_type]
     if max_norm is None:
-        _lib.check(lib.ak_grad_norm(table, len(rows), kind, norm.data_ptr(), ws.data_ptr(), need, _stream(device)), 'ak_grad_norm')
+        _lib.check(lib.ak_grad_norm(table, len(rows), kind, norm.data_ptr(), ws.data_ptr(), need, _stream_handle(device)), 'ak_grad_norm')
     else:
-        rc = lib.ak_clip_grad_norm(table, len(rows), kind, max_norm, norm.data_ptr(), ws.data_ptr(), need, _stream(device))
+        rc = lib.ak_clip_grad_norm(table, len(rows), kind, max_norm, norm.data_ptr(), ws.data_ptr(), need, _stream_handle(device))
         _lib.check(rc, 'ak_clip_grad_norm')
     return norm
 
@@ -1512,7 +1529,7 @@ def grad_norm(grads, norm_type=2.0):
     """The norm of all elements of ``grads`` (tensors of float32, bfloat16 or float16 on one device) as one vector, a 0-d float32 tensor:
     norm_type 2, 1 or inf.  Sums are double, in a fixed order.  A gradient that is listed twice counts once."""
     grads = _norm_arguments(grads, norm_type)
-    with _device_of(grads[0]):
+    with _device_of(grads[0].device):
         device, rows, _ = _norm_items(grads, None)
         return _launch_norm(rows, device, float(norm_type), None)
 
@@ -1528,7 +1545,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, outs=None):
     outs = grads if outs is None else [o.detach() for o in outs]
     if len(outs) != len(grads):
         raise ValueError(f'{len(grads)} gradients and {len(outs)} results.')
-    with _device_of(grads[0]):
+    with _device_of(grads[0].device):
         device, rows, late = _norm_items(grads, outs)
         norm = _launch_norm(rows, device, float(norm_type), max_norm)
         with _on_launch_stream():
