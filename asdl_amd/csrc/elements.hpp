@@ -58,6 +58,20 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+typedef unsigned long long u64;
+
+template <int CTRL>
+__device__ __forceinline__ u64 add_dpp(u64 v) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, 0xf, 0xf, true));
+  return v + (static_cast<u64>(hi) << 32 | lo);
+}
+
+__device__ __forceinline__ u64 read_lane(u64 v, int lane) {
+  return static_cast<u64>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+
 template <typename V>
 __device__ __forceinline__ V wave_sum(V v) {
 #pragma unroll
@@ -67,6 +81,14 @@ __device__ __forceinline__ V wave_sum(V v) {
 template <>
 __device__ __forceinline__ float wave_sum<float>(float v) {
   return lanes_sum<64>(v);
+}
+template <>
+__device__ __forceinline__ u64 wave_sum<u64>(u64 v) {
+  v = add_dpp<0xB1>(v);
+  v = add_dpp<0x4E>(v);
+  v = add_dpp<0x141>(v);
+  v = add_dpp<0x140>(v);
+  return (read_lane(v, 0) + read_lane(v, 16)) + (read_lane(v, 32) + read_lane(v, 48));
 }
 
 // The sum over a work group of WAVES waves, in every thread; `red` has WAVES words.  The barrier in front keeps the words of the

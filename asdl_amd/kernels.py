@@ -1245,7 +1245,7 @@ def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min
       top_k  the k most probable classes (the lowest index first among equal ones; None or <= 0: all),
       top_p  of those the most probable ones whose probability reaches top_p: a class is kept while the probability in front of it is
              below top_p (None or >= 1: all),
-      min_p  classes of at least min_p times the largest probability (None or <= 0: all).
+      min_p  classes of at least min_p times the largest probability (None or <= 0: all; above 1: as 1).
     The most probable class is always kept; temperature 0 takes it.  The class is the first, by index, at which the probability of the
     kept classes up to it exceeds ``u`` (float32 or float64, one number in [0, 1) per row; None: drawn here).  Each of the four may be a
     tensor with one element per row instead (float32; top_k int64).  Logits of -inf are never drawn.

@@ -200,7 +200,8 @@ int ak_sample_categorical(const float* logits, const float* q, int64_t rows, int
 /* targets[r] = a draw of softmax(logits[r] / T) restricted by top-k, top-p and min-p, from the uniform number u[r] in [0, 1).
  * Classes in the order of their logits, equal ones by index; weights exp((logit - max) / T).  top-k (<= 0: off) keeps the first k;
  * top-p (>= 1: off; <= 0: the first class) keeps a class while the weight in front of it is below top_p times the weight that top-k
- * left; min-p (<= 0: off) keeps weights of at least min_p.  The most probable class is always kept.  The draw is the lowest index at
+ * left; min-p (<= 0: off) keeps weights of at
+ * least min(min_p, 1).  The most probable class is always kept.  The draw is the lowest index at
  * which the kept weight up to it exceeds u times all of it.  T = 0 takes the first class.  Sums are integers: the draw depends on no
  * order of sums.  logits: `dtype` AK_F32 / AK_BF16 / AK_F16, row stride ld >= classes, classes contiguous, any alignment; logits of
  * -inf are never drawn.  u: float or double (u_is_double) [rows].  temperatures, top_ks, top_ps, min_ps [rows] (device, each may be

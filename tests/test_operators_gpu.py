@@ -250,8 +250,7 @@ def draw64(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
         if ps[r] < 1:
             before = np.concatenate([[0], np.cumsum(w)[:-1]])
             keep = before < ps[r] * w.sum()
-        if ms[r] > 0:
-            keep &= w >= ms[r]
+        keep &= w >= min(ms[r], 1)
         keep[0] = True
         at = order[keep]
         by_index = np.argsort(at)
