@@ -64,37 +64,6 @@ struct SfWeight {
   __device__ __forceinline__ u64 operator()(float x) const { return whole(scaled(x)); }
 };
 
-struct SfShared {
-  u64 mass[256];
-  uint32_t count[256];
-  u64 red[16];
-  int red_int[16];
-  u64 above;
-  uint32_t digit;
-  int found;
-};
-
-// The first bin from the top at which the sum of `v` reaches `target`; one wave, lane l has bins 255 - 4 l ... 252 - 4 l.
-__device__ __forceinline__ void sf_crossing(const u64* v, u64 target, uint32_t& digit, u64& above) {
-  const int lane = threadIdx.x & 63;
-  u64 own[4], sum = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sum += own[e] = v[255 - 4 * lane - e];
-  u64 upto = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 before = __shfl_up(upto, o);
-    if (lane >= o) upto += before;
-  }
-  u64 at = upto - sum;
-  if (at < target && upto >= target) {
-    int e = 0;
-    while (at + own[e] < target) at += own[e++];
-    digit = 255 - 4 * lane - e;
-    above = at;
-  }
-}
-
 // What a row is drawn with.
 struct SfFilter {
   double t, p, m, u;
@@ -126,147 +95,6 @@ __device__ __forceinline__ u64 sf_border(double p, u64 all) {
   return target < all ? target : all;
 }
 
-__device__ __forceinline__ void sf_no_distribution(const SfParams& p, int64_t row) {
-  p.targets[row] = -1;
-  if (p.invalid != nullptr) *p.invalid = 1;
-}
-
-// A row of any length and any distribution that is not greedy, read from memory in every step.  The key at which a sum of counts or
-// weights from the top reaches a number is found digit by digit, 8 bits of it a step, from histograms.
-template <typename T, int NT>
-__device__ __forceinline__ void sf_general(const SfParams& p, int64_t row, const SfFilter& filter, float top, SfShared& sh) {
-  constexpr int WAVES = NT / 64;
-  u64* bins = sh.mass;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.classes;
-  const T* __restrict__ x = static_cast<const T*>(p.logits) + row * p.ld;
-  const int64_t k = filter.k;
-  const double top_p = filter.p;
-  const SfWeight weight{static_cast<double>(top), filter.exponent(), static_cast<double>(1ull << p.shift), p.shift};
-  uint32_t key = 0;           // classes above it are kept, and the first `ties` equal to it
-  uint32_t ties = 0xffffffffu, equal = 0;
-  // The digits of the key at which the count (by weight: the weight) from the top reaches `target`; `floor_key`, `floor_ties`:
-  // classes below are out, and of those equal so many are in.
-  auto select = [&](bool by_weight, u64 target, uint32_t floor_key, uint32_t floor_ties, uint32_t& out_key, u64& above_all, uint32_t& out_equal) {
-    uint32_t prefix = 0;
-    u64 above = 0;
-    for (int at = 24; at >= 0; at -= 8) {
-      for (int b = tid; b < 256; b += NT) {
-        bins[b] = 0;
-        sh.count[b] = 0;
-      }
-      __syncthreads();
-      for (int c = tid; c < n; c += NT) {
-        const float v = static_cast<float>(x[c]);
-        const uint32_t kk = sf_key(v);
-        if (at < 24 && (kk >> (at + 8)) != prefix) continue;
-        if (kk < floor_key || (kk == floor_key && floor_ties != 0xffffffffu)) continue;
-        atomicAdd(&sh.count[kk >> at & 255], 1u);
-        if (by_weight) atomicAdd(&bins[kk >> at & 255], weight(v));
-      }
-      __syncthreads();
-      if (tid == 0 && floor_ties != 0xffffffffu && (at == 24 || (floor_key >> (at + 8)) == prefix)) {
-        sh.count[floor_key >> at & 255] += floor_ties;
-        bins[floor_key >> at & 255] += floor_ties * weight(sf_value(floor_key));
-      }
-      __syncthreads();
-      if (!by_weight) {
-        for (int b = tid; b < 256; b += NT) bins[b] = sh.count[b];
-        __syncthreads();
-      }
-      if (wave == 0) sf_crossing(bins, target - above, sh.digit, sh.above);
-      __syncthreads();
-      above += sh.above;
-      prefix = prefix << 8 | sh.digit;
-      out_equal = sh.count[sh.digit];
-      __syncthreads();
-    }
-    out_key = prefix;
-    above_all = above;
-  };
-
-  if (k > 0 && k < n) {
-    u64 above;
-    select(false, static_cast<u64>(k), 0, 0xffffffffu, key, above, equal);
-    ties = static_cast<uint32_t>(static_cast<u64>(k) - above);
-    if (ties >= equal) ties = 0xffffffffu;
-  }
-  auto in_k = [&](uint32_t kk) { return kk > key || (kk == key && ties == 0xffffffffu); };
-  if (top_p < 1.) {
-    u64 all = 0;
-    for (int c = tid; c < n; c += NT) {
-      const float v = static_cast<float>(x[c]);
-      if (in_k(sf_key(v))) all += weight(v);
-    }
-    all = group_sum<WAVES>(all, sh.red);
-    if (ties != 0xffffffffu) all += ties * weight(sf_value(key));
-    const u64 target = sf_border(top_p, all);
-    uint32_t key2;
-    u64 above;
-    select(true, target, key, ties, key2, above, equal);
-    const u64 w = weight(sf_value(key2));
-    const u64 need = w == 0 ? equal : (target - above + w - 1) / w;
-    key = key2;
-    ties = need >= equal ? (ties != 0xffffffffu && equal == ties ? ties : 0xffffffffu) : static_cast<uint32_t>(need);
-  }
-
-  // the index behind which classes equal to the key are out
-  int last_tie = 0x7fffffff;
-  if (ties != 0xffffffffu) {
-    uint32_t before = 0;
-    for (int c0 = 0; c0 < n; c0 += NT) {
-      const int c = c0 + tid;
-      const bool is = c < n && sf_key(static_cast<float>(x[c])) == key;
-      const u64 mask = __ballot(is);
-      if (lane == 0) sh.red_int[wave] = __popcll(mask);
-      __syncthreads();
-      uint32_t rank = before + __popcll(mask & ((1ull << lane) - 1)), sum = 0;
-      for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) rank += sh.red_int[w];
-        sum += sh.red_int[w];
-      }
-      if (is && rank == ties - 1) sh.found = c;
-      before += sum;
-      __syncthreads();
-      if (before >= ties) break;
-    }
-    last_tie = sh.found;
-  }
-  auto kept = [&](int c) -> u64 {
-    const float v = static_cast<float>(x[c]);
-    const uint32_t kk = sf_key(v);
-    if (kk < key || (kk == key && c > last_tie)) return 0;
-    const double w = weight.scaled(v);
-    return w < filter.least(weight.scale) ? 0 : SfWeight::whole(w);
-  };
-  u64 all = 0;
-  for (int c = tid; c < n; c += NT) all += kept(c);
-  all = group_sum<WAVES>(all, sh.red);
-  const u64 target = sf_target(filter.u, all);
-  u64 before = 0;
-  for (int c0 = 0; c0 < n; c0 += NT) {
-    const int c = c0 + tid;
-    const u64 w = c < n ? kept(c) : 0;
-    u64 upto = w;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const u64 lower = __shfl_up(upto, o);
-      if (lane >= o) upto += lower;
-    }
-    __syncthreads();
-    if (lane == 63) sh.red[wave] = upto;
-    __syncthreads();
-    u64 sum = 0;
-    for (int v = 0; v < WAVES; ++v) {
-      if (v < wave) upto += sh.red[v];
-      sum += sh.red[v];
-    }
-    upto += before;
-    if (upto > target && upto - w <= target) p.targets[row] = c;
-    before += sum;
-    if (before > target) return;
-  }
-}
-
 // The largest and smallest over a work group.
 struct SfRange {
   float top, low, least;      // largest; smallest finite one; smallest of the lanes' largest ones
@@ -292,13 +120,13 @@ __device__ __forceinline__ SfRange sf_range(SfRange r, SfRange* red) {
 }
 
 // Sums of the threads before and of all threads.
-template <int WAVES>
-__device__ __forceinline__ void sf_scan(u64 own, u64* red, u64& before, u64& total) {
+template <int WAVES, typename A>
+__device__ __forceinline__ void sf_scan(A own, A* red, A& before, A& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 upto = own;
+  A upto = own;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const u64 lower = __shfl_up(upto, o);
+    const A lower = __shfl_up(upto, o);
     if (lane >= o) upto += lower;
   }
   __syncthreads();
@@ -313,67 +141,95 @@ __device__ __forceinline__ void sf_scan(u64 own, u64* red, u64& before, u64& tot
   }
 }
 
-constexpr int kSfBins = 2048, kSfCandidates = 1024, kSfMostSteps = 64;
+constexpr int kSfBins = 2048, kSfListed = 2048, kSfSteps = 64, kSfAhead = 4;
 
 template <int CELLS>
-struct SfRowShared {
+struct SfShared {
   u64 bins[kSfBins];
-  u64 weight[kSfCandidates];
-  uint32_t key[kSfCandidates];
-  int index[kSfCandidates];
+  u64 order[kSfListed];                 // listed classes: key, 2^32 - 1 - index; the later class has the smaller number
   u64 cells[CELLS];
   u64 red[16];
+  double red_double[16];
   SfRange range[16];
   u64 above;
-  int where, candidates, found_index;
-  uint32_t found_key;
+  int where, listed, found;
+  uint32_t found_key, lowest, highest;
+  int found_index;
 };
 
-// A row in vectors of E elements, step after step NT of them: class (step NT + thread) E + e; the last n % E classes are a step of
-// their own, one for each of the first threads.  Held in registers, or read in every pass.
-template <typename T, int NT, int V, bool HELD>
+__device__ __forceinline__ u64 sf_order(uint32_t key, int c) { return static_cast<u64>(key) << 32 | (0xffffffffu - static_cast<uint32_t>(c)); }
+__device__ __forceinline__ uint32_t sf_order_key(u64 o) { return static_cast<uint32_t>(o >> 32); }
+__device__ __forceinline__ int sf_order_class(u64 o) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(o)); }
+
+// The first `count` numbers in falling order: a bitonic network over the power of two above (numbers of 0 are added).
+template <int NT>
+__device__ __forceinline__ void sf_sort(u64* order, int count) {
+  const int tid = threadIdx.x;
+  int n = 2;
+  while (n < count) n *= 2;
+  __syncthreads();
+  for (int i = count + tid; i < n; i += NT) order[i] = 0;
+  __syncthreads();
+  for (int size = 2; size <= n; size *= 2)
+    for (int gap = size / 2; gap > 0; gap /= 2) {
+      for (int t = tid; t < n / 2; t += NT) {
+        const int i = 2 * t - (t & (gap - 1));
+        const u64 a = order[i], b = order[i + gap];
+        if ((a < b) == ((i & size) == 0)) {
+          order[i] = b;
+          order[i + gap] = a;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+// A row in vectors of E elements, step after step NT runs of U of them: run (step NT + thread) is one thread's; the last n % E classes
+// are a step of their own, one for each of the first threads.  U is 1 up to kSfSteps steps.  Every pass reads the row again, from the
+// caches but for the first one; kSfAhead steps are on their way.
+template <typename T, int NT>
 struct SfRow {
   static constexpr int E = 16 / sizeof(T);
   const T* __restrict__ x;
-  int whole, rest, steps;
-  Some<T, E> held[HELD ? V : 1];
-  T last;
-  __device__ __forceinline__ SfRow(const T* __restrict__ x_, int n) : x(x_), whole(n / E * E), rest(n % E), steps(HELD ? V : (n / E + NT - 1) / NT) {
-    if constexpr (HELD) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        held[v].clear();
-        if ((v * NT + static_cast<int>(threadIdx.x)) * E < whole) held[v].load(x + (v * NT + threadIdx.x) * E);
-      }
-    }
-    last = static_cast<T>(0.f);
-    if (static_cast<int>(threadIdx.x) < rest) last = x[whole + threadIdx.x];
+  int whole, rest, run, steps;         // run: U E classes
+  __device__ __forceinline__ SfRow(const T* __restrict__ x_, int n) : x(x_), whole(n / E * E), rest(n % E) {
+    const int vectors = n / E, most = NT * kSfSteps;
+    run = vectors > most ? (vectors + most - 1) / most * E : E;
+    const int64_t all = static_cast<int64_t>(NT) * run;
+    steps = static_cast<int>((whole + all - 1) / all);
   }
-  // fn(value, class) for the classes of this thread, done(step) behind every step
+  // fn(value, class) for the classes of this thread, done(step) behind every step, for all threads at once
   template <typename Fn, typename Done>
   __device__ __forceinline__ void each(Fn&& fn, Done&& done) const {
-    if constexpr (HELD) {
+    const int tid = static_cast<int>(threadIdx.x);
+    if (run == E) {
+      Some<T, E> ahead[kSfAhead];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int at = (v * NT + static_cast<int>(threadIdx.x)) * E;
-        if (at < whole)
+      for (int i = 0; i < kSfAhead; ++i) {
+        ahead[i].clear();
+        if ((i * NT + tid) * E < whole) ahead[i].load(x + (i * NT + tid) * E);
+      }
+      for (int v = 0; v < steps; v += kSfAhead) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) fn(held[v].get(e), at + e);
-        done(v);
+        for (int i = 0; i < kSfAhead; ++i) {
+          const int at = ((v + i) * NT + tid) * E, later = at + kSfAhead * NT * E;
+          const Some<T, E> some = ahead[i];
+          if (later < whole) ahead[i].load(x + later);
+          if (at < whole)
+#pragma unroll
+            for (int e = 0; e < E; ++e) fn(some.get(e), at + e);
+          if (v + i < steps) done(v + i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     } else {
       for (int v = 0; v < steps; ++v) {
-        const int at = (v * NT + static_cast<int>(threadIdx.x)) * E;
-        if (at < whole) {
-          Some<T, E> some;
-          some.load(x + at);
-#pragma unroll
-          for (int e = 0; e < E; ++e) fn(some.get(e), at + e);
-        }
+        const int64_t first = (static_cast<int64_t>(v) * NT + tid) * run;
+        for (int64_t at = first; at < first + run && at < whole; ++at) fn(static_cast<float>(x[at]), static_cast<int>(at));
         done(v);
       }
     }
-    if (static_cast<int>(threadIdx.x) < rest) fn(static_cast<float>(last), whole + static_cast<int>(threadIdx.x));
+    if (tid < rest) fn(static_cast<float>(x[whole + tid]), whole + tid);
     done(steps);
   }
   template <typename Fn>
@@ -381,19 +237,26 @@ struct SfRow {
     each(fn, [](int) {});
   }
   // the cell (step and wave) of a class
-  __device__ __forceinline__ int cell(int c) const { return c < whole ? c / (NT * E) * (NT / 64) + c % (NT * E) / (64 * E) : steps * (NT / 64); }
+  __device__ __forceinline__ int cell(int c) const { return c < whole ? c / run / 64 : steps * (NT / 64); }
+  // fn(value, class) for the classes of lane `lane` of a cell: wave `wave` of step `step`
+  template <typename Fn>
+  __device__ __forceinline__ void each_of_cell(int step, int wave, int lane, Fn&& fn) const {
+    const bool of_rest = step == steps;
+    const int64_t begin = of_rest ? whole + lane : (static_cast<int64_t>(step) * NT + wave * 64 + lane) * run;
+    const int64_t end = of_rest ? begin + (lane < rest ? 1 : 0) : begin + run < whole ? begin + run : whole;
+    for (int64_t c = begin; c < end; ++c) fn(static_cast<float>(x[c]), static_cast<int>(c));
+  }
 };
 
-// One work group per row, in three or four passes over it: the range; with top-k the counts of 2048 bins between its ends, which say in
-// what bin the border lies; with top-p the weights of such bins; the kept weight of every cell (a step of a wave).  The classes of a
-// border's bin are listed and ranked by counting; more than kSfCandidates of them go to sf_general.
-template <typename T, int NT, int V, bool HELD>
+// One work group per row, in a few passes over it: the range; with top-k the counts of 2048 bins between its ends, which say in what bin
+// the border lies; with top-p the weights of such bins.  Where the classes up to the border's bin are at most kSfListed, they are listed
+// in the LDS and ranked there by counting, and the draw is among them.  Otherwise the border is narrowed to a key and an index, and one
+// more pass sums the kept weight of every cell (a step of a wave).
+template <typename T, int NT>
 static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
-  constexpr int WAVES = NT / 64, CELLS = ((HELD ? V : kSfMostSteps) + 1) * WAVES;
-  using Row = SfRow<T, NT, V, HELD>;
-  constexpr int E = Row::E;
-  __shared__ SfRowShared<CELLS> sh;
-  __shared__ SfShared general;
+  constexpr int WAVES = NT / 64, CELLS = (kSfSteps + 1) * WAVES;
+  using Row = SfRow<T, NT>;
+  __shared__ SfShared<CELLS> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.classes;
   const int64_t row_index = blockIdx.x;
   const Row row(static_cast<const T*>(p.logits) + row_index * p.ld, n);
@@ -411,7 +274,10 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   range = sf_range<WAVES>(range, sh.range);
   const float top = range.top;
   if (bad != 0 || top == -INFINITY) {
-    if (tid == 0) sf_no_distribution(p, row_index);
+    if (tid == 0) {
+      p.targets[row_index] = -1;
+      if (p.invalid != nullptr) *p.invalid = 1;
+    }
     return;
   }
   if (filter.greedy()) {
@@ -425,10 +291,13 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     return;
   }
 
+  const SfWeight weight{static_cast<double>(top), filter.exponent(), static_cast<double>(1ull << p.shift), p.shift};
+  const double least = filter.least(weight.scale);
+  auto drawn = [&](double w) -> u64 { return w < least ? 0 : SfWeight::whole(w); };
   uint32_t key = 0;                  // kept: above the key, and equal to it up to the index
   int last = 0x7fffffff;
-  float scale = 0.f;
   auto kept = [&](uint32_t kk, int c) { return kk > key || (kk == key && c <= last); };
+  float scale = 0.f;
   auto bin_of = [&](float v) {       // the same or a later bin for a smaller logit
     const float b = (top - v) * scale;
     return b < static_cast<float>(kSfBins - 1) ? static_cast<int>(b) : kSfBins - 1;
@@ -438,34 +307,209 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     scale = top > low && s < INFINITY ? s : 0.f;
   };
   auto clear_bins = [&] {
+    __syncthreads();
     for (int b = tid; b < kSfBins; b += NT) sh.bins[b] = 0;
-    if (tid == 0) sh.candidates = 0;
     __syncthreads();
   };
-  // The first bin at which the sum reaches `target` (made from the sum of all bins); false if it does not.
-  auto cross = [&](auto value, auto make_target, u64& target) {
+  // The first bin at which the sum reaches `target` (made from the sum of all): its number and the sum in front of it in `sh`.
+  // False if none does.
+  auto cross = [&](auto&& make_target, u64& target) {
     constexpr int PER = kSfBins / NT;
+    __syncthreads();
     u64 own = 0, before, total;
 #pragma unroll
-    for (int b = 0; b < PER; ++b) own += value(tid * PER + b);
+    for (int b = 0; b < PER; ++b) own += sh.bins[tid * PER + b];
     sf_scan<WAVES>(own, sh.red, before, total);
     target = make_target(total);
     if (before < target && before + own >= target) {
       int b = tid * PER;
-      for (u64 v = value(b); before + v < target; v = value(++b)) before += v;
+      for (; before + sh.bins[b] < target; ++b) before += sh.bins[b];
       sh.where = b;
       sh.above = before;
     }
     __syncthreads();
     return total >= target;
   };
-  auto list = [&](uint32_t kk, int c, u64 w) {
-    const int i = atomicAdd(&sh.candidates, 1);
-    if (i < kSfCandidates) {
-      sh.key[i] = kk;
-      sh.index[i] = c;
-      sh.weight[i] = w;
+  bool full = false;                 // the list, as far as this wave knows
+  auto clear_list = [&] {
+    __syncthreads();
+    full = false;
+    if (tid == 0) {
+      sh.listed = 0;
+      sh.lowest = 0xffffffffu;
+      sh.highest = 0;
     }
+    __syncthreads();
+  };
+  // Lists the class of every lane that wants it; one addition to the counter a wave, and none once the list is full.
+  auto list = [&](bool want, uint32_t kk, int c) {
+    const u64 mask = __ballot(want && !full);
+    if (mask == 0) return;
+    int base = 0;
+    const int leader = __ffsll(mask) - 1;
+    if (lane == leader) base = atomicAdd(&sh.listed, __popcll(mask));
+    base = __builtin_amdgcn_readlane(base, leader);
+    full = base + __popcll(mask) > kSfListed;
+    if (want && !full) sh.order[base + __popcll(mask & ((1ull << lane) - 1))] = sf_order(kk, c);
+  };
+  // Of the listed classes in order, fn(class of the list, its weight as worth(logit), the weight in front of it).
+  constexpr int PER = kSfListed / NT;
+  auto each_listed = [&](int count, auto&& worth, auto&& fn) {
+    u64 w[PER], own = 0, before, total;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int j = tid * PER + q;
+      w[q] = j < count ? worth(j, sh.order[j]) : 0;
+      own += w[q];
+    }
+    sf_scan<WAVES>(own, sh.red, before, total);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int j = tid * PER + q;
+      if (j < count) fn(j, sh.order[j], w[q], before, total);
+      before += w[q];
+    }
+  };
+  // The class of index order at which the sums of the cells exceed `target`: its cell in sh.where, the sum in front in sh.above.
+  auto cell_of = [&](auto&& make_target, u64& target) {
+    __syncthreads();
+    const int cells = (row.steps + 1) * WAVES, per = (cells + NT - 1) / NT;
+    u64 own = 0, before, all;
+    for (int i = 0; i < per; ++i)
+      if (tid * per + i < cells) own += sh.cells[tid * per + i];
+    sf_scan<WAVES>(own, sh.red, before, all);
+    target = make_target(all);
+    if (before <= target && before + own > target) {
+      int i = tid * per;
+      for (; before + sh.cells[i] <= target; ++i) before += sh.cells[i];
+      sh.where = i;
+      sh.above = before;
+    }
+    __syncthreads();
+  };
+  // In that cell (by one wave): found(class) for the class at which `value`s exceed the target.
+  auto class_of = [&](u64 target, auto&& value, auto&& found) {
+    if (wave != 0) return;
+    const int step = sh.where / WAVES, of_wave = sh.where % WAVES;
+    u64 mine = 0;
+    row.each_of_cell(step, of_wave, lane, [&](float v, int c) { mine += value(v, c); });
+    u64 upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const u64 lower = __shfl_up(upto, o);
+      if (lane >= o) upto += lower;
+    }
+    u64 from = sh.above + upto - mine;
+    if (from <= target && from + mine > target)
+      row.each_of_cell(step, of_wave, lane, [&](float v, int c) {
+        const u64 w = value(v, c);
+        if (from <= target && from + w > target) found(c);
+        from += w;
+      });
+  };
+  u64 sum = 0;
+  auto to_cell = [&](int step) {
+    const u64 s = wave_sum(sum);
+    if (lane == 0) sh.cells[step * WAVES + wave] = s;
+    sum = 0;
+  };
+  // The border in bin sh.where, `target` counts (weights) from the top, as a key and an index: of the classes in(v, key, class) in
+  // this bin.  Where they are too many for the list, bins of equal parts of their keys take the place of the bin, until it is few
+  // enough classes or one key, whose classes are counted by index.
+  auto narrow = [&](u64 target, auto&& in, auto&& worth) {
+    const int border = sh.where;
+    u64 above = sh.above;
+    uint32_t low = 0, high = 0xffffffffu;
+    for (;;) {
+      uint32_t least_key = 0xffffffffu, most_key = 0;
+      clear_list();
+      row.each([&](float v, int c) {
+        const uint32_t kk = sf_key(v);
+        const bool want = kk >= low && kk <= high && bin_of(v) == border && in(v, kk, c);
+        list(want, kk, c);
+        least_key = want && kk < least_key ? kk : least_key;
+        most_key = want && kk > most_key ? kk : most_key;
+      });
+      if (most_key >= least_key) {
+        atomicMin(&sh.lowest, least_key);
+        atomicMax(&sh.highest, most_key);
+      }
+      __syncthreads();
+      const int count = sh.listed;
+      low = sh.lowest;
+      high = sh.highest;
+      if (count <= kSfListed) {
+        sf_sort<NT>(sh.order, count);
+        each_listed(count, [&](int, u64 o) { return worth(sf_value(sf_order_key(o))); }, [&](int, u64 o, u64 w, u64 before, u64) {
+          if (above + before < target && above + before + w >= target) {
+            sh.found_key = sf_order_key(o);
+            sh.found_index = sf_order_class(o);
+          }
+        });
+        break;
+      }
+      if (low == high) {
+        const u64 w = worth(sf_value(low)), nth = (target - above + w - 1) / w - 1;
+        auto equal = [&](float v, int c) -> u64 {
+          const uint32_t kk = sf_key(v);
+          return kk == low && in(v, kk, c) ? 1 : 0;
+        };
+        row.each([&](float v, int c) { sum += equal(v, c); }, to_cell);
+        u64 unused;
+        cell_of([&](u64) { return nth; }, unused);
+        class_of(nth, equal, [&](int c) {
+          sh.found_key = low;
+          sh.found_index = c;
+        });
+        break;
+      }
+      const int bits = 32 - __clz(high - low), shift = bits > 11 ? bits - 11 : 0;
+      clear_bins();
+      row.each([&](float v, int c) {
+        const uint32_t kk = sf_key(v);
+        if (kk < low || kk > high || !in(v, kk, c) || bin_of(v) != border) return;
+        const u64 w = worth(v);
+        if (w != 0) atomicAdd(sh.bins + ((high - kk) >> shift), w);
+      });
+      u64 rest;
+      cross([&](u64) { return target - above; }, rest);
+      above += sh.above;
+      high -= static_cast<uint32_t>(sh.where) << shift;
+      const uint32_t span = (1u << shift) - 1;
+      low = high - low > span ? high - span : low;
+    }
+    __syncthreads();
+    key = sh.found_key;
+    last = sh.found_index;
+  };
+  // The draw among the listed classes, of which the first k are kept, and of them those with less than `border` (made from the weight
+  // of them all) in front.  They are put in order, and those that are kept in the order of their indices.
+  auto draw_listed = [&](int k, auto&& make_border) {
+    __syncthreads();
+    const int count = sh.listed < k ? sh.listed : k;
+    sf_sort<NT>(sh.order, sh.listed);
+    u64 keep[PER];
+#pragma unroll
+    for (int q = 0; q < PER; ++q) keep[q] = 0;
+    each_listed(count, [&](int, u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](int j, u64 o, u64, u64 before, u64 total) {
+      keep[j % PER] = before < make_border(total) ? o << 32 | o >> 32 : 0;
+    });
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < PER; ++q)
+      if (tid * PER + q < count) sh.order[tid * PER + q] = keep[q];
+    sf_sort<NT>(sh.order, count);
+    each_listed(count, [&](int, u64 o) { return o == 0 ? 0 : drawn(weight.scaled(sf_value(static_cast<uint32_t>(o)))); }, [&](int, u64 o, u64 w, u64 before, u64 all) {
+      const u64 target = sf_target(filter.u, all);
+      if (before <= target && before + w > target) p.targets[row_index] = sf_order_class(o >> 32);
+    });
+  };
+
+  auto value = [&](float v, int c) -> u64 { return kept(sf_key(v), c) ? drawn(weight.scaled(v)) : 0; };
+  auto draw_cells = [&] {
+    u64 target;
+    cell_of([&](u64 all) { return sf_target(filter.u, all); }, target);
+    class_of(target, value, [&](int c) { p.targets[row_index] = c; });
   };
 
   if (filter.k > 0 && filter.k < n) {
@@ -473,50 +517,88 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     const float low = filter.k <= NT && range.least > -INFINITY ? range.least : range.low;
     set_scale(low);
     clear_bins();
-    uint32_t* counts = reinterpret_cast<uint32_t*>(sh.bins);
     row.each([&](float v, int) {
-      if (v >= low) atomicAdd(counts + bin_of(v), 1u);
+      if (v >= low) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(v)), 1u);
+    });
+    u64 target;
+    if (cross([&](u64) { return static_cast<u64>(filter.k); }, target)) {
+      const int border = sh.where;
+      if (sh.above + sh.bins[border] <= kSfListed) {
+        clear_list();
+        row.each([&](float v, int c) { list(v >= low && bin_of(v) <= border, sf_key(v), c); });
+        return draw_listed(static_cast<int>(filter.k), [&](u64 all) { return filter.p < 1. ? sf_border(filter.p, all) : ~0ull; });
+      }
+      narrow(target, [&](float v, uint32_t, int) { return v >= low; }, [](float) -> u64 { return 1; });
+    }
+  }
+  if (filter.p < 1.) {
+    // Where the border will be, from counts: of a bin's classes, all weights are taken for that of its middle.  (Weights of classes
+    // further down than 37 T round to 0.)
+    set_scale(fmaxf(range.low, static_cast<float>(static_cast<double>(top) - 37. * filter.t)));
+    clear_bins();
+    row.each([&](float v, int c) {
+      if (kept(sf_key(v), c)) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(v)), 1u);
     });
     __syncthreads();
-    u64 target;
-    if (cross([&](int b) { return static_cast<u64>(counts[b]); }, [&](u64) { return static_cast<u64>(filter.k); }, target)) {
-      const int border = sh.where;
-      row.each([&](float v, int c) {
-        if (v >= low && bin_of(v) == border) list(sf_key(v), c, 0);
+    {
+      constexpr int PER_BINS = kSfBins / NT;
+      const float width = scale > 0.f ? 1.f / scale : 0.f;
+      const float fall = static_cast<float>(-weight.c * static_cast<double>(width));        // log2 of a bin's weight over the one before
+      double own[PER_BINS], sum_of = 0., before, total;
+#pragma unroll
+      for (int q = 0; q < PER_BINS; ++q)
+        sum_of += own[q] = static_cast<double>(sh.bins[tid * PER_BINS + q]) * static_cast<double>(exp2f((static_cast<float>(tid * PER_BINS + q) + 0.5f) * fall));
+      sf_scan<WAVES>(sum_of, sh.red_double, before, total);
+      if (tid == 0) sh.where = kSfBins - 2;
+      __syncthreads();
+      const double border = filter.p * total;
+#pragma unroll
+      for (int q = 0; q < PER_BINS; ++q) {
+        if (before <= border && before + own[q] > border) sh.where = tid * PER_BINS + q;
+        before += own[q];
+      }
+      clear_list();
+    }
+    // One pass with exact weights: all of them; of the bins in front of the border's and its neighbours', by cells; these bins' classes.
+    const int middle = sh.where, from_bin = middle > 0 ? middle - 1 : 0, to_bin = middle + 1;
+    u64 own = 0, own_above = 0;
+    row.each(
+        [&](float v, int c) {
+          const uint32_t kk = sf_key(v);
+          const bool in = kept(kk, c);
+          const int b = bin_of(v);
+          const double w = weight.scaled(v);
+          const u64 whole = SfWeight::whole(w);
+          own += in ? whole : 0;
+          own_above += in && b < from_bin ? whole : 0;
+          sum += in && b < from_bin && w >= least ? whole : 0;
+          list(in && b >= from_bin && b <= to_bin, kk, c);
+        },
+        to_cell);
+    const u64 all = group_sum<WAVES>(own, sh.red), above = group_sum<WAVES>(own_above, sh.red), target = sf_border(filter.p, all);
+    const int count = sh.listed;
+    if (tid == 0) sh.found = 0;
+    if (count <= kSfListed) {
+      sf_sort<NT>(sh.order, count);
+      each_listed(count, [&](int, u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](int, u64 o, u64 w, u64 before, u64) {
+        if (above + before >= target) return;
+        const int c = sf_order_class(o);
+        const u64 d = drawn(weight.scaled(sf_value(sf_order_key(o))));
+        if (d != 0) atomicAdd(sh.cells + row.cell(c), d);
+        if (above + before + w >= target) {
+          sh.found_key = sf_order_key(o);
+          sh.found_index = c;
+          sh.found = 1;
+        }
       });
       __syncthreads();
-      const int count = sh.candidates;
-      if (count > kSfCandidates) return sf_general<T, NT>(p, row_index, filter, top, general);
-      const int nth = static_cast<int>(target - sh.above) - 1;
-      for (int j = tid; j < count; j += NT) {
-        const uint32_t kk = sh.key[j];
-        const int c = sh.index[j];
-        int rank = 0;
-        for (int i = 0; i < count; ++i) rank += sh.key[i] > kk || (sh.key[i] == kk && sh.index[i] < c) ? 1 : 0;
-        if (rank == nth) {
-          sh.found_key = kk;
-          sh.found_index = c;
-        }
+      if (sh.found) {
+        key = sh.found_key;
+        last = sh.found_index;
+        return draw_cells();
       }
-      __syncthreads();
-      key = sh.found_key;
-      last = sh.found_index;
     }
-    __syncthreads();
-  }
-
-  const SfWeight weight{static_cast<double>(top), filter.exponent(), static_cast<double>(1ull << p.shift), p.shift};
-  const double least = filter.least(weight.scale);
-  auto drawn = [&](double w) -> u64 { return w < least ? 0 : SfWeight::whole(w); };
-  u64 sum = 0;
-  auto to_cell = [&](int step) {
-    const u64 s = wave_sum(sum);
-    if (lane == 0) sh.cells[step * WAVES + wave] = s;
-    sum = 0;
-  };
-  if (filter.p < 1.) {
-    // (weights of classes further down than 37 T round to 0)
-    set_scale(fmaxf(range.low, static_cast<float>(static_cast<double>(top) - 37. * filter.t)));
+    // The counts were misleading, or the classes there too many: the weights of bins, and the border's bin in parts.
     clear_bins();
     row.each([&](float v, int c) {
       if (kept(sf_key(v), c)) {
@@ -524,131 +606,20 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
         if (w != 0) atomicAdd(sh.bins + bin_of(v), w);
       }
     });
-    __syncthreads();
-    u64 target;
-    cross([&](int b) { return sh.bins[b]; }, [&](u64 total) { return sf_border(filter.p, total); }, target);
-    const int border = sh.where;
-    const u64 above = sh.above;
-    row.each(
-        [&](float v, int c) {
-          const int b = bin_of(v);
-          if (b > border || !kept(sf_key(v), c)) return;
-          const double w = weight.scaled(v);
-          if (b < border) sum += drawn(w);
-          else if (const u64 whole = SfWeight::whole(w); whole != 0) list(sf_key(v), c, whole);
-        },
-        to_cell);
-    __syncthreads();
-    const int count = sh.candidates;
-    if (count > kSfCandidates) return sf_general<T, NT>(p, row_index, filter, top, general);
-    for (int j = tid; j < count; j += NT) {
-      const uint32_t kk = sh.key[j];
-      const int c = sh.index[j];
-      u64 before = above;
-      for (int i = 0; i < count; ++i)
-        if (sh.key[i] > kk || (sh.key[i] == kk && sh.index[i] < c)) before += sh.weight[i];
-      if (before < target && before + sh.weight[j] >= target) {
-        sh.found_key = kk;
-        sh.found_index = c;
-      }
-    }
-    __syncthreads();
-    key = sh.found_key;
-    last = sh.found_index;
-    for (int j = tid; j < count; j += NT)
-      if (kept(sh.key[j], sh.index[j])) {
-        const u64 w = drawn(weight.scaled(sf_value(sh.key[j])));
-        if (w != 0) atomicAdd(sh.cells + row.cell(sh.index[j]), w);
-      }
-  } else {
-    row.each([&](float v, int c) { if (kept(sf_key(v), c)) sum += drawn(weight.scaled(v)); }, to_cell);
+    u64 same;
+    cross([&](u64) { return target; }, same);
+    narrow(target, [&](float, uint32_t kk, int c) { return kept(kk, c); }, weight);
   }
-  __syncthreads();
-
-  // the cell in which the draw lies, then the class
-  const int cells = (row.steps + 1) * WAVES, per = (cells + NT - 1) / NT;
-  u64 own = 0, before, all;
-  for (int i = 0; i < per; ++i)
-    if (tid * per + i < cells) own += sh.cells[tid * per + i];
-  sf_scan<WAVES>(own, sh.red, before, all);
-  const u64 target = sf_target(filter.u, all);
-  if (before <= target && before + own > target) {
-    int i = tid * per;
-    for (; before + sh.cells[i] <= target; ++i) before += sh.cells[i];
-    sh.where = i;
-    sh.above = before;
-  }
-  __syncthreads();
-  if (wave != 0) return;
-  const int step = sh.where / WAVES, of_wave = sh.where % WAVES;
-  const int at = step < row.steps ? (step * NT + of_wave * 64 + lane) * E : row.whole + lane;
-  const int count = step < row.steps ? (at < row.whole ? E : 0) : lane < row.rest ? 1 : 0;
-  u64 w[E], mine = 0;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    w[e] = 0;
-    if (e < count) {
-      const float v = static_cast<float>(row.x[at + e]);
-      if (kept(sf_key(v), at + e)) w[e] = drawn(weight.scaled(v));
-    }
-    mine += w[e];
-  }
-  u64 upto = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 lower = __shfl_up(upto, o);
-    if (lane >= o) upto += lower;
-  }
-  u64 from = sh.above + upto - mine;
-  if (from <= target && from + mine > target) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (from <= target && from + w[e] > target) p.targets[row_index] = at + e;
-      from += w[e];
-    }
-  }
-}
-
-// Rows beyond the steps of the kernel above.
-template <typename T>
-static __global__ __launch_bounds__(1024) void sf_long_kernel(SfParams p) {
-  __shared__ SfShared sh;
-  __shared__ SfRange red[16];
-  __shared__ int first;
-  const int64_t row = blockIdx.x;
-  const T* __restrict__ x = static_cast<const T*>(p.logits) + row * p.ld;
-  const SfFilter filter(p, row);
-  SfRange range{-INFINITY, 0.f, 0.f};
-  int bad = filter.good() ? 0 : 1;
-  for (int c = threadIdx.x; c < p.classes; c += 1024) {
-    const float v = static_cast<float>(x[c]);
-    bad |= v < INFINITY ? 0 : 1;
-    range.top = fmaxf(range.top, v);
-  }
-  if (threadIdx.x == 0) first = 0x7fffffff;
-  bad = __syncthreads_or(bad);
-  range = sf_range<16>(range, red);
-  if (bad != 0 || range.top == -INFINITY) {
-    if (threadIdx.x == 0) sf_no_distribution(p, row);
-    return;
-  }
-  if (!filter.greedy()) return sf_general<T, 1024>(p, row, filter, range.top, sh);
-  for (int c = threadIdx.x; c < p.classes; c += 1024)
-    if (static_cast<float>(x[c]) == range.top) {
-      atomicMin(&first, c);
-      break;
-    }
-  __syncthreads();
-  if (threadIdx.x == 0) p.targets[row] = first;
+  row.each([&](float v, int c) { sum += value(v, c); }, to_cell);
+  draw_cells();
 }
 
 template <typename T>
 static void sf_launch(const SfParams& p, int64_t rows, hipStream_t s) {
-  constexpr int E = 16 / sizeof(T);
   const dim3 grid(static_cast<unsigned>(rows));
-  if (p.classes <= 2048) hipLaunchKernelGGL((sf_row_kernel<T, 256, 1, false>), grid, dim3(256), 0, s, p);
-  else if (p.classes / E <= kSfMostSteps * 1024) hipLaunchKernelGGL((sf_row_kernel<T, 1024, 1, false>), grid, dim3(1024), 0, s, p);
-  else hipLaunchKernelGGL(sf_long_kernel<T>, grid, dim3(1024), 0, s, p);
+  if (p.classes <= 2048) hipLaunchKernelGGL((sf_row_kernel<T, 256>), grid, dim3(256), 0, s, p);
+  else if (rows > 256) hipLaunchKernelGGL((sf_row_kernel<T, 512>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((sf_row_kernel<T, 1024>), grid, dim3(1024), 0, s, p);
 }
 
 }  // namespace ak
