@@ -41,10 +41,7 @@ struct SfWeight {
   double top, c, scale;
   int shift;
   __device__ __forceinline__ double scaled(float x) const {
-    double y = (static_cast<double>(x) - top) * c;
-    y = fmax(y, -2000.);
-    if (x == -INFINITY) y = -2000.;                      // (also where c is 0)
-    const double whole = rint(y), f = y - whole;
+    const double y = fmax((static_cast<double>(x) - top) * c, -2000.), whole = rint(y), f = y - whole;      // (-inf and its NaN: 0)
     double q = 7.070977866508138e-09;
     q = fma(q, f, 1.0205905413765595e-07);
     q = fma(q, f, 1.3215451633221434e-06);
@@ -57,9 +54,9 @@ struct SfWeight {
     q = fma(q, f, 0.6931471805599462);
     return ldexp(fma(q, f, 1.), static_cast<int>(whole) + shift);
   }
-  // rounded to an integer by the addition of 2^52 (scaled() is at most that)
+  // rounded to an integer by the addition of 2^52: the fraction's bits (scaled() is at most 2^51)
   static __device__ __forceinline__ u64 whole(double scaled) {
-    return __builtin_bit_cast(u64, scaled + 4503599627370496.) - 0x4330000000000000ull;
+    return __builtin_bit_cast(u64, scaled + 4503599627370496.) & 0x000fffffffffffffull;
   }
   __device__ __forceinline__ u64 operator()(float x) const { return whole(scaled(x)); }
 };
@@ -198,7 +195,7 @@ struct SfRow {
     const int64_t all = static_cast<int64_t>(NT) * run;
     steps = static_cast<int>((whole + all - 1) / all);
   }
-  // fn(value, class) for the classes of this thread, done(step) behind every step, for all threads at once
+  // fn(values, first class) for neighbouring classes of this thread (E of them, or one), done(step) behind every step, for all threads
   template <typename Fn, typename Done>
   __device__ __forceinline__ void each(Fn&& fn, Done&& done) const {
     const int tid = static_cast<int>(threadIdx.x);
@@ -213,11 +210,11 @@ struct SfRow {
 #pragma unroll
         for (int i = 0; i < kSfAhead; ++i) {
           const int at = ((v + i) * NT + tid) * E, later = at + kSfAhead * NT * E;
-          const Some<T, E> some = ahead[i];
-          if (later < whole) ahead[i].load(x + later);
-          if (at < whole)
+          float value[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) fn(some.get(e), at + e);
+          for (int e = 0; e < E; ++e) value[e] = ahead[i].get(e);
+          if (later < whole) ahead[i].load(x + later);
+          if (at < whole) fn(value, at);
           if (v + i < steps) done(v + i);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -225,11 +222,17 @@ struct SfRow {
     } else {
       for (int v = 0; v < steps; ++v) {
         const int64_t first = (static_cast<int64_t>(v) * NT + tid) * run;
-        for (int64_t at = first; at < first + run && at < whole; ++at) fn(static_cast<float>(x[at]), static_cast<int>(at));
+        for (int64_t at = first; at < first + run && at < whole; ++at) {
+          const float value[1] = {static_cast<float>(x[at])};
+          fn(value, static_cast<int>(at));
+        }
         done(v);
       }
     }
-    if (tid < rest) fn(static_cast<float>(x[whole + tid]), whole + tid);
+    if (tid < rest) {
+      const float value[1] = {static_cast<float>(x[whole + tid])};
+      fn(value, whole + tid);
+    }
     done(steps);
   }
   template <typename Fn>
@@ -263,17 +266,20 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   const SfFilter filter(p, row_index);
 
   SfRange range{-INFINITY, INFINITY, 0.f};
-  int bad = filter.good() ? 0 : 1;
-  row.each([&](float v, int) {
-    bad |= v < INFINITY ? 0 : 1;
-    range.top = fmaxf(range.top, v);
-    range.low = fminf(range.low, v > -INFINITY ? v : INFINITY);
+  bool bad = !filter.good();
+  row.each([&](const auto& v, int) {
+#pragma unroll
+    for (const float x : v) {
+      bad = bad || !(x < INFINITY);
+      range.top = fmaxf(range.top, x);
+      range.low = fminf(range.low, x);
+    }
   });
   range.least = range.top;
-  bad = __syncthreads_or(bad);
+  bad = __syncthreads_or(bad) != 0;
   range = sf_range<WAVES>(range, sh.range);
   const float top = range.top;
-  if (bad != 0 || top == -INFINITY) {
+  if (bad || top == -INFINITY) {
     if (tid == 0) {
       p.targets[row_index] = -1;
       if (p.invalid != nullptr) *p.invalid = 1;
@@ -282,7 +288,13 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   }
   if (filter.greedy()) {
     int best = 0x7fffffff;
-    row.each([&](float v, int c) { best = v == top && c < best ? c : best; });
+    row.each([&](const auto& v, int at) {
+      int c = at;
+      for (const float x : v) {
+        best = x == top && c < best ? c : best;
+        ++c;
+      }
+    });
     if (tid == 0) sh.where = 0x7fffffff;
     __syncthreads();
     if (best != 0x7fffffff) atomicMin(&sh.where, best);
@@ -294,14 +306,12 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   const SfWeight weight{static_cast<double>(top), filter.exponent(), static_cast<double>(1ull << p.shift), p.shift};
   const double least = filter.least(weight.scale);
   auto drawn = [&](double w) -> u64 { return w < least ? 0 : SfWeight::whole(w); };
-  uint32_t key = 0;                  // kept: above the key, and equal to it up to the index
-  int last = 0x7fffffff;
-  auto kept = [&](uint32_t kk, int c) { return kk > key || (kk == key && c <= last); };
+  float border_value = -INFINITY;    // kept: above the value, and equal to it up to the index
+  int border_index = -1;
+  auto kept = [&](float v, int c) { return v > border_value || (v == border_value && c <= border_index); };
   float scale = 0.f;
-  auto bin_of = [&](float v) {       // the same or a later bin for a smaller logit
-    const float b = (top - v) * scale;
-    return b < static_cast<float>(kSfBins - 1) ? static_cast<int>(b) : kSfBins - 1;
-  };
+  auto place_of = [&](float v) { return (top - v) * scale; };       // 0 and up, does not fall for a smaller logit
+  auto bin_of = [&](float v) { return static_cast<int>(__builtin_amdgcn_fmed3f(place_of(v), 0.f, static_cast<float>(kSfBins - 1))); };
   auto set_scale = [&](float low) {
     const float s = static_cast<float>(kSfBins - 1) / (top - low);
     scale = top > low && s < INFINITY ? s : 0.f;
@@ -342,7 +352,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     __syncthreads();
   };
   // Lists the class of every lane that wants it; one addition to the counter a wave, and none once the list is full.
-  auto list = [&](bool want, uint32_t kk, int c) {
+  auto list = [&](bool want, float v, int c) {
     const u64 mask = __ballot(want && !full);
     if (mask == 0) return;
     int base = 0;
@@ -350,7 +360,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     if (lane == leader) base = atomicAdd(&sh.listed, __popcll(mask));
     base = __builtin_amdgcn_readlane(base, leader);
     full = base + __popcll(mask) > kSfListed;
-    if (want && !full) sh.order[base + __popcll(mask & ((1ull << lane) - 1))] = sf_order(kk, c);
+    if (want && !full) sh.order[base + __popcll(mask & ((1ull << lane) - 1))] = sf_order(sf_key(v), c);
   };
   // Of the listed classes in order, fn(class of the list, its weight as worth(logit), the weight in front of it).
   constexpr int PER = kSfListed / NT;
@@ -413,22 +423,26 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     if (lane == 0) sh.cells[step * WAVES + wave] = s;
     sum = 0;
   };
-  // The border in bin sh.where, `target` counts (weights) from the top, as a key and an index: of the classes in(v, key, class) in
+  // The border in bin sh.where, `target` counts (weights) from the top, as a value and an index: of the classes in(value, class) in
   // this bin.  Where they are too many for the list, bins of equal parts of their keys take the place of the bin, until it is few
   // enough classes or one key, whose classes are counted by index.
   auto narrow = [&](u64 target, auto&& in, auto&& worth) {
-    const int border = sh.where;
+    const int bin = sh.where;
     u64 above = sh.above;
     uint32_t low = 0, high = 0xffffffffu;
     for (;;) {
       uint32_t least_key = 0xffffffffu, most_key = 0;
       clear_list();
-      row.each([&](float v, int c) {
-        const uint32_t kk = sf_key(v);
-        const bool want = kk >= low && kk <= high && bin_of(v) == border && in(v, kk, c);
-        list(want, kk, c);
-        least_key = want && kk < least_key ? kk : least_key;
-        most_key = want && kk > most_key ? kk : most_key;
+      row.each([&](const auto& v, int at) {
+        int c = at;
+        for (const float x : v) {
+          const uint32_t kk = sf_key(x);
+          const bool want = kk >= low && kk <= high && bin_of(x) == bin && in(x, c);
+          list(want, x, c);
+          least_key = want && kk < least_key ? kk : least_key;
+          most_key = want && kk > most_key ? kk : most_key;
+          ++c;
+        }
       });
       if (most_key >= least_key) {
         atomicMin(&sh.lowest, least_key);
@@ -450,11 +464,11 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
       }
       if (low == high) {
         const u64 w = worth(sf_value(low)), nth = (target - above + w - 1) / w - 1;
-        auto equal = [&](float v, int c) -> u64 {
-          const uint32_t kk = sf_key(v);
-          return kk == low && in(v, kk, c) ? 1 : 0;
-        };
-        row.each([&](float v, int c) { sum += equal(v, c); }, to_cell);
+        auto equal = [&](float v, int c) -> u64 { return sf_key(v) == low && in(v, c) ? 1 : 0; };
+        row.each([&](const auto& v, int at) {
+          int c = at;
+          for (const float x : v) sum += equal(x, c++);
+        }, to_cell);
         u64 unused;
         cell_of([&](u64) { return nth; }, unused);
         class_of(nth, equal, [&](int c) {
@@ -465,22 +479,27 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
       }
       const int bits = 32 - __clz(high - low), shift = bits > 11 ? bits - 11 : 0;
       clear_bins();
-      row.each([&](float v, int c) {
-        const uint32_t kk = sf_key(v);
-        if (kk < low || kk > high || !in(v, kk, c) || bin_of(v) != border) return;
-        const u64 w = worth(v);
-        if (w != 0) atomicAdd(sh.bins + ((high - kk) >> shift), w);
+      row.each([&](const auto& v, int at) {
+        int c = at;
+        for (const float x : v) {
+          const uint32_t kk = sf_key(x);
+          if (kk >= low && kk <= high && bin_of(x) == bin && in(x, c)) {
+            const u64 w = worth(x);
+            if (w != 0) atomicAdd(sh.bins + ((high - kk) >> shift), w);
+          }
+          ++c;
+        }
       });
-      u64 rest;
-      cross([&](u64) { return target - above; }, rest);
+      u64 left;
+      cross([&](u64) { return target - above; }, left);
       above += sh.above;
       high -= static_cast<uint32_t>(sh.where) << shift;
       const uint32_t span = (1u << shift) - 1;
       low = high - low > span ? high - span : low;
     }
     __syncthreads();
-    key = sh.found_key;
-    last = sh.found_index;
+    border_value = sf_value(sh.found_key);
+    border_index = sh.found_index;
   };
   // The draw among the listed classes, of which the first k are kept, and of them those with less than `border` (made from the weight
   // of them all) in front.  They are put in order, and those that are kept in the order of their indices.
@@ -505,7 +524,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     });
   };
 
-  auto value = [&](float v, int c) -> u64 { return kept(sf_key(v), c) ? drawn(weight.scaled(v)) : 0; };
+  auto value = [&](float v, int c) -> u64 { return kept(v, c) ? drawn(weight.scaled(v)) : 0; };
   auto draw_cells = [&] {
     u64 target;
     cell_of([&](u64 all) { return sf_target(filter.u, all); }, target);
@@ -514,36 +533,45 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
 
   if (filter.k > 0 && filter.k < n) {
     // of as many classes as there are threads, the largest of each thread's, none is below the least of them
-    const float low = filter.k <= NT && range.least > -INFINITY ? range.least : range.low;
+    const float low = filter.k <= NT ? range.least : range.low;
     set_scale(low);
     clear_bins();
-    row.each([&](float v, int) {
-      if (v >= low) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(v)), 1u);
+    row.each([&](const auto& v, int) {
+      for (const float x : v)
+        if (x >= low) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(x)), 1u);
     });
     u64 target;
-    if (cross([&](u64) { return static_cast<u64>(filter.k); }, target)) {
-      const int border = sh.where;
-      if (sh.above + sh.bins[border] <= kSfListed) {
-        clear_list();
-        row.each([&](float v, int c) { list(v >= low && bin_of(v) <= border, sf_key(v), c); });
-        return draw_listed(static_cast<int>(filter.k), [&](u64 all) { return filter.p < 1. ? sf_border(filter.p, all) : ~0ull; });
-      }
-      narrow(target, [&](float v, uint32_t, int) { return v >= low; }, [](float) -> u64 { return 1; });
+    cross([&](u64) { return static_cast<u64>(filter.k); }, target);
+    const int bin = sh.where;
+    if (sh.above + sh.bins[bin] <= kSfListed) {
+      clear_list();
+      row.each([&](const auto& v, int at) {
+        int c = at;
+        for (const float x : v) {
+          list(x >= low && bin_of(x) <= bin, x, c);
+          ++c;
+        }
+      });
+      return draw_listed(static_cast<int>(filter.k), [&](u64 all) { return filter.p < 1. ? sf_border(filter.p, all) : ~0ull; });
     }
+    narrow(target, [&](float v, int) { return v >= low; }, [](float) -> u64 { return 1; });
   }
   if (filter.p < 1.) {
     // Where the border will be, from counts: of a bin's classes, all weights are taken for that of its middle.  (Weights of classes
     // further down than 37 T round to 0.)
     set_scale(fmaxf(range.low, static_cast<float>(static_cast<double>(top) - 37. * filter.t)));
     clear_bins();
-    row.each([&](float v, int c) {
-      if (kept(sf_key(v), c)) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(v)), 1u);
+    row.each([&](const auto& v, int at) {
+      int c = at;
+      for (const float x : v) {
+        if (kept(x, c)) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(x)), 1u);
+        ++c;
+      }
     });
     __syncthreads();
     {
       constexpr int PER_BINS = kSfBins / NT;
-      const float width = scale > 0.f ? 1.f / scale : 0.f;
-      const float fall = static_cast<float>(-weight.c * static_cast<double>(width));        // log2 of a bin's weight over the one before
+      const float fall = scale > 0.f ? static_cast<float>(-weight.c / static_cast<double>(scale)) : 0.f;     // log2 of a bin's weight over the one before
       double own[PER_BINS], sum_of = 0., before, total;
 #pragma unroll
       for (int q = 0; q < PER_BINS; ++q)
@@ -559,58 +587,82 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
       }
       clear_list();
     }
-    // One pass with exact weights: all of them; of the bins in front of the border's and its neighbours', by cells; these bins' classes.
-    const int middle = sh.where, from_bin = middle > 0 ? middle - 1 : 0, to_bin = middle + 1;
-    u64 own = 0, own_above = 0;
+    // One pass with exact weights: of the bins in front of the border's and its neighbours', by cells; of all others; the classes of
+    // these bins.
+    const int middle = sh.where;
+    const float from_place = middle > 0 ? static_cast<float>(middle - 1) : -INFINITY, to_place = middle + 2 < kSfBins ? static_cast<float>(middle + 2) : INFINITY;
+    u64 own_behind = 0, own_above = 0;
     row.each(
-        [&](float v, int c) {
-          const uint32_t kk = sf_key(v);
-          const bool in = kept(kk, c);
-          const int b = bin_of(v);
-          const double w = weight.scaled(v);
-          const u64 whole = SfWeight::whole(w);
-          own += in ? whole : 0;
-          own_above += in && b < from_bin ? whole : 0;
-          sum += in && b < from_bin && w >= least ? whole : 0;
-          list(in && b >= from_bin && b <= to_bin, kk, c);
+        [&](const auto& v, int at) {
+          uint32_t wanted = 0, bit = 1;
+          int c = at;
+          for (const float x : v) {
+            const bool in = kept(x, c);
+            const float place = place_of(x);
+            const u64 w = weight(x);
+            const bool front = in && place < from_place;
+            sum += front ? w : 0;
+            own_behind += in && !front ? w : 0;
+            wanted |= in && !front && !(place >= to_place) ? bit : 0;
+            bit *= 2;
+            ++c;
+          }
+          if (__ballot(wanted != 0) != 0) {
+            c = at;
+            for (const float x : v) {
+              list((wanted & 1) != 0, x, c);
+              wanted >>= 1;
+              ++c;
+            }
+          }
         },
-        to_cell);
-    const u64 all = group_sum<WAVES>(own, sh.red), above = group_sum<WAVES>(own_above, sh.red), target = sf_border(filter.p, all);
+        [&](int step) {
+          own_above += sum;
+          to_cell(step);
+        });
+    const u64 above = group_sum<WAVES>(own_above, sh.red), all = above + group_sum<WAVES>(own_behind, sh.red), target = sf_border(filter.p, all);
     const int count = sh.listed;
     if (tid == 0) sh.found = 0;
-    if (count <= kSfListed) {
+    if (count <= kSfListed && above < target) {
       sf_sort<NT>(sh.order, count);
       each_listed(count, [&](int, u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](int, u64 o, u64 w, u64 before, u64) {
         if (above + before >= target) return;
         const int c = sf_order_class(o);
-        const u64 d = drawn(weight.scaled(sf_value(sf_order_key(o))));
-        if (d != 0) atomicAdd(sh.cells + row.cell(c), d);
+        if (w != 0) atomicAdd(sh.cells + row.cell(c), w);
         if (above + before + w >= target) {
           sh.found_key = sf_order_key(o);
           sh.found_index = c;
           sh.found = 1;
         }
       });
-      __syncthreads();
-      if (sh.found) {
-        key = sh.found_key;
-        last = sh.found_index;
-        return draw_cells();
-      }
     }
-    // The counts were misleading, or the classes there too many: the weights of bins, and the border's bin in parts.
-    clear_bins();
-    row.each([&](float v, int c) {
-      if (kept(sf_key(v), c)) {
-        const u64 w = weight(v);
-        if (w != 0) atomicAdd(sh.bins + bin_of(v), w);
-      }
-    });
-    u64 same;
-    cross([&](u64) { return target; }, same);
-    narrow(target, [&](float, uint32_t kk, int c) { return kept(kk, c); }, weight);
+    __syncthreads();
+    if (sh.found) {
+      border_value = sf_value(sh.found_key);
+      border_index = sh.found_index;
+      if (weight.scaled(border_value) >= least) return draw_cells();       // (else the cells hold what min-p leaves out)
+    } else {
+      // The counts were misleading, or the classes there too many: the weights of bins, and the border's bin in parts.
+      clear_bins();
+      row.each([&](const auto& v, int at) {
+        int c = at;
+        for (const float x : v) {
+          if (kept(x, c)) {
+            const u64 w = weight(x);
+            if (w != 0) atomicAdd(sh.bins + bin_of(x), w);
+          }
+          ++c;
+        }
+      });
+      u64 same;
+      cross([&](u64) { return target; }, same);
+      narrow(target, kept, weight);
+    }
   }
-  row.each([&](float v, int c) { sum += value(v, c); }, to_cell);
+  row.each([&](const auto& v, int at) {
+    int c = at;
+    for (const float x : v) sum += value(x, c++);
+  }, to_cell);
   draw_cells();
 }
 
@@ -635,7 +687,7 @@ extern "C" int ak_sample_filtered(const void* logits, int dtype, int64_t rows, i
   if (classes > (1 << 30) || rows > 0x7fffffff) return AK_ERR_TOO_LARGE;
   int bits = 0;
   while ((1ll << bits) < classes) ++bits;
-  const int shift = 62 - bits < 52 ? 62 - bits : 52;
+  const int shift = 62 - bits < 51 ? 62 - bits : 51;
   const SfParams p{logits, u, temperatures, top_ks, top_ps, min_ps, targets, invalid, ld, temperature, top_p, min_p, top_k,
                    static_cast<int>(classes), u_is_double, shift};
   hipStream_t s = static_cast<hipStream_t>(stream);
