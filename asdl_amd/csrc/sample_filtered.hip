@@ -35,6 +35,14 @@ __device__ __forceinline__ float sf_value(uint32_t key) {
   return __builtin_bit_cast(float, key ^ ((key >> 31) != 0 ? 0x80000000u : 0xffffffffu));
 }
 
+// a b + c with c in scalar registers.  (The compiler takes the form that overwrites c, and copies it to vector registers every time: a
+// third of the instructions of a weight.)
+__device__ __forceinline__ double sf_fma(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+}
+
 // w = exp((x - top) / T) = 2^y in units of 2^-shift: y = (x - top) (log2 e / T) is split into the nearest integer and a rest in
 // [-1/2, 1/2], whose power is 1 + f q(f), q interpolated at the ten Chebyshev points (off by at most 6e-16; exactly 1 at f = 0).
 struct SfWeight {
@@ -42,16 +50,15 @@ struct SfWeight {
   int shift;
   __device__ __forceinline__ double scaled(float x) const {
     const double y = fmax((static_cast<double>(x) - top) * c, -2000.), whole = rint(y), f = y - whole;      // (-inf and its NaN: 0)
-    double q = 7.070977866508138e-09;
-    q = fma(q, f, 1.0205905413765595e-07);
-    q = fma(q, f, 1.3215451633221434e-06);
-    q = fma(q, f, 1.5252672924850737e-05);
-    q = fma(q, f, 0.00015403530424776529);
-    q = fma(q, f, 0.0013333558200794592);
-    q = fma(q, f, 0.009618129107618665);
-    q = fma(q, f, 0.05550410866465167);
-    q = fma(q, f, 0.24022650695910075);
-    q = fma(q, f, 0.6931471805599462);
+    double q = sf_fma(7.070977866508138e-09, f, 1.0205905413765595e-07);
+    q = sf_fma(q, f, 1.3215451633221434e-06);
+    q = sf_fma(q, f, 1.5252672924850737e-05);
+    q = sf_fma(q, f, 0.00015403530424776529);
+    q = sf_fma(q, f, 0.0013333558200794592);
+    q = sf_fma(q, f, 0.009618129107618665);
+    q = sf_fma(q, f, 0.05550410866465167);
+    q = sf_fma(q, f, 0.24022650695910075);
+    q = sf_fma(q, f, 0.6931471805599462);
     return ldexp(fma(q, f, 1.), static_cast<int>(whole) + shift);
   }
   // rounded to an integer by the addition of 2^52: the fraction's bits (scaled() is at most 2^51)
@@ -308,7 +315,8 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   auto drawn = [&](double w) -> u64 { return w < least ? 0 : SfWeight::whole(w); };
   float border_value = -INFINITY;    // kept: above the value, and equal to it up to the index
   int border_index = -1;
-  auto kept = [&](float v, int c) { return v > border_value || (v == border_value && c <= border_index); };
+  // (bit by bit: no branches)
+  auto kept = [&](float v, int c) -> bool { return (v > border_value) | ((v == border_value) & (c <= border_index)); };
   float scale = 0.f;
   auto place_of = [&](float v) { return (top - v) * scale; };       // 0 and up, does not fall for a smaller logit
   auto bin_of = [&](float v) { return static_cast<int>(__builtin_amdgcn_fmed3f(place_of(v), 0.f, static_cast<float>(kSfBins - 1))); };
@@ -600,10 +608,10 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
             const bool in = kept(x, c);
             const float place = place_of(x);
             const u64 w = weight(x);
-            const bool front = in && place < from_place;
+            const bool front = in & (place < from_place);
             sum += front ? w : 0;
-            own_behind += in && !front ? w : 0;
-            wanted |= in && !front && !(place >= to_place) ? bit : 0;
+            own_behind += in & !front ? w : 0;
+            wanted |= in & !front & !(place >= to_place) ? bit : 0;
             bit *= 2;
             ++c;
           }
