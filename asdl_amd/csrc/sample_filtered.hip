@@ -24,6 +24,7 @@ struct SfParams {
   double temperature, top_p, min_p;
   int64_t top_k;
   int classes, u_double, shift;
+  uint32_t unit;          // so large that one for every class fits 32 bits
 };
 
 __device__ __forceinline__ uint32_t sf_key(float x) {
@@ -160,7 +161,7 @@ struct SfShared {
   double red_double[16];
   SfRange range[16];
   u64 above;
-  int where, listed, found;
+  int where, until, listed, found;
   uint32_t found_key, lowest, highest;
   int found_index;
 };
@@ -263,7 +264,7 @@ struct SfRow {
 };
 
 // One work group per row, in a few passes over it: the range; with top-k the counts of 2048 bins between its ends, which say in what bin
-// the border lies; with top-p the weights of such bins.  Where the classes up to the border's bin are at most kSfListed, they are listed
+// the border lies; with top-p the fp32 weights of such bins.  Where the classes up to the border's bin are at most kSfListed, they are listed
 // in the LDS and ranked there by counting, and the draw is among them.  Otherwise the border is narrowed to a key and an index, and one
 // more pass sums the kept weight of every cell (a step of a wave).
 template <typename T, int NT>
@@ -335,17 +336,17 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   };
   // The first bin at which the sum reaches `target` (made from the sum of all): its number and the sum in front of it in `sh`.
   // False if none does.
-  auto cross = [&](auto&& make_target, u64& target) {
+  auto cross = [&](const auto* bins, auto&& make_target, u64& target) {
     constexpr int PER = kSfBins / NT;
     __syncthreads();
     u64 own = 0, before, total;
 #pragma unroll
-    for (int b = 0; b < PER; ++b) own += sh.bins[tid * PER + b];
+    for (int b = 0; b < PER; ++b) own += bins[tid * PER + b];
     sf_scan<WAVES>(own, sh.red, before, total);
     target = make_target(total);
     if (before < target && before + own >= target) {
       int b = tid * PER;
-      for (; before + sh.bins[b] < target; ++b) before += sh.bins[b];
+      for (; before + bins[b] < target; ++b) before += bins[b];
       sh.where = b;
       sh.above = before;
     }
@@ -503,7 +504,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
         }
       });
       u64 left;
-      cross([&](u64) { return target - above; }, left);
+      cross(sh.bins, [&](u64) { return target - above; }, left);
       above += sh.above;
       high -= static_cast<uint32_t>(sh.where) << shift;
       const uint32_t span = (1u << shift) - 1;
@@ -548,14 +549,15 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     const float low = filter.k <= NT ? range.least : range.low;
     set_scale(low);
     clear_bins();
+    uint32_t* counts = reinterpret_cast<uint32_t*>(sh.bins);
     row.each([&](const auto& v, int) {
       for (const float x : v)
-        if (x >= low) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(x)), 1u);
+        if (x >= low) atomicAdd(counts + bin_of(x), 1u);
     });
     u64 target;
-    cross([&](u64) { return static_cast<u64>(filter.k); }, target);
+    cross(counts, [&](u64) { return static_cast<u64>(filter.k); }, target);
     const int bin = sh.where;
-    if (sh.above + sh.bins[bin] <= kSfListed) {
+    if (sh.above + counts[bin] <= kSfListed) {
       clear_list();
       row.each([&](const auto& v, int at) {
         int c = at;
@@ -569,40 +571,46 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     narrow(target, [&](float v, int) { return v >= low; }, [](float) -> u64 { return 1; });
   }
   if (filter.p < 1.) {
-    // Where the border will be, from counts: of a bin's classes, all weights are taken for that of its middle.  (Weights of classes
-    // further down than 37 T round to 0.)
+    // Where the border will be, from 32-bit sums: a bin's weights fall from 1 to 2^-drop of that at its upper end, taken as a straight
+    // line (off by 4e-5 at most).  Additions of fp32 numbers in the LDS take three times as long as all the rest of the pass.
+    // (Weights of classes further down than 37 T round to 0.)
     set_scale(fmaxf(range.low, static_cast<float>(static_cast<double>(top) - 37. * filter.t)));
     clear_bins();
+    uint32_t* sums = reinterpret_cast<uint32_t*>(sh.bins);
+    const float drop = scale > 0.f ? static_cast<float>(weight.c / static_cast<double>(scale)) : 0.f;
+    const float unit = static_cast<float>(p.unit), slope = unit * (exp2f(-drop) - 1.f);
     row.each([&](const auto& v, int at) {
       int c = at;
       for (const float x : v) {
-        if (kept(x, c)) atomicAdd(reinterpret_cast<uint32_t*>(sh.bins + bin_of(x)), 1u);
+        if (kept(x, c)) atomicAdd(sums + bin_of(x), static_cast<uint32_t>(__builtin_fmaf(__builtin_amdgcn_fractf(place_of(x)), slope, unit)));
         ++c;
       }
     });
     __syncthreads();
     {
       constexpr int PER_BINS = kSfBins / NT;
-      const float fall = scale > 0.f ? static_cast<float>(-weight.c / static_cast<double>(scale)) : 0.f;     // log2 of a bin's weight over the one before
       double own[PER_BINS], sum_of = 0., before, total;
 #pragma unroll
       for (int q = 0; q < PER_BINS; ++q)
-        sum_of += own[q] = static_cast<double>(sh.bins[tid * PER_BINS + q]) * static_cast<double>(exp2f((static_cast<float>(tid * PER_BINS + q) + 0.5f) * fall));
+        sum_of += own[q] = static_cast<double>(sums[tid * PER_BINS + q]) * static_cast<double>(exp2f(-drop * static_cast<float>(tid * PER_BINS + q)));
       sf_scan<WAVES>(sum_of, sh.red_double, before, total);
-      if (tid == 0) sh.where = kSfBins - 2;
+      if (tid == 0) sh.where = sh.until = kSfBins - 1;
       __syncthreads();
-      const double border = filter.p * total;
+      const double border = filter.p * total, margin = 1e-4 * total;
 #pragma unroll
       for (int q = 0; q < PER_BINS; ++q) {
-        if (before <= border && before + own[q] > border) sh.where = tid * PER_BINS + q;
+        if (before <= border && before + own[q] > border) {
+          const int bin = tid * PER_BINS + q;
+          sh.where = border - before < margin && bin > 0 ? bin - 1 : bin;
+          sh.until = before + own[q] - border < margin && bin < kSfBins - 1 ? bin + 1 : bin;
+        }
         before += own[q];
       }
       clear_list();
     }
-    // One pass with exact weights: of the bins in front of the border's and its neighbours', by cells; of all others; the classes of
-    // these bins.
-    const int middle = sh.where;
-    const float from_place = middle > 0 ? static_cast<float>(middle - 1) : -INFINITY, to_place = middle + 2 < kSfBins ? static_cast<float>(middle + 2) : INFINITY;
+    // One pass with exact weights: of the bins in front of the border's (and of a neighbour, where the border is near its edge), by
+    // cells; of all others; the classes of these bins.
+    const float from_place = sh.where > 0 ? static_cast<float>(sh.where) : -INFINITY, to_place = sh.until < kSfBins - 1 ? static_cast<float>(sh.until + 1) : INFINITY;
     u64 own_behind = 0, own_above = 0;
     row.each(
         [&](const auto& v, int at) {
@@ -654,7 +662,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
       border_index = sh.found_index;
       if (weight.scaled(border_value) >= least) return draw_cells();       // (else the cells hold what min-p leaves out)
     } else {
-      // The counts were misleading, or the classes there too many: the weights of bins, and the border's bin in parts.
+      // The border was not there, or the classes too many: the weights of bins, and the border's bin in parts.
       clear_bins();
       row.each([&](const auto& v, int at) {
         int c = at;
@@ -667,7 +675,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
         }
       });
       u64 same;
-      cross([&](u64) { return target; }, same);
+      cross(sh.bins, [&](u64) { return target; }, same);
       narrow(target, kept, weight);
     }
   }
@@ -701,7 +709,7 @@ extern "C" int ak_sample_filtered(const void* logits, int dtype, int64_t rows, i
   while ((1ll << bits) < classes) ++bits;
   const int shift = 62 - bits < 51 ? 62 - bits : 51;
   const SfParams p{logits, u, temperatures, top_ks, top_ps, min_ps, targets, invalid, ld, temperature, top_p, min_p, top_k,
-                   static_cast<int>(classes), u_is_double, shift};
+                   static_cast<int>(classes), u_is_double, shift, (1u << (bits < 32 ? 31 - bits : 0))};
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto type) {
     sf_launch<typename decltype(type)::type>(p, rows, s);
