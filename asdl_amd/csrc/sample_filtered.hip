@@ -7,6 +7,7 @@
 // the point for 50257 classes), and integers add exactly.  w itself is computed in double.
 // The kept classes are those above a key (the logit's bits in an order that integers keep) and, of those equal to it, the ones up to an
 // index.
+#include <type_traits>
 #include "elements.hpp"
 
 namespace ak {
@@ -579,13 +580,19 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     uint32_t* sums = reinterpret_cast<uint32_t*>(sh.bins);
     const float drop = scale > 0.f ? static_cast<float>(weight.c / static_cast<double>(scale)) : 0.f;
     const float unit = static_cast<float>(p.unit), slope = unit * (exp2f(-drop) - 1.f);
-    row.each([&](const auto& v, int at) {
-      int c = at;
-      for (const float x : v) {
-        if (kept(x, c)) atomicAdd(sums + bin_of(x), static_cast<uint32_t>(__builtin_fmaf(__builtin_amdgcn_fractf(place_of(x)), slope, unit)));
-        ++c;
-      }
-    });
+    auto add_sums = [&](auto all) {        // all: every class is kept (of -inf, in the last bin, nothing is taken)
+      row.each([&](const auto& v, int at) {
+        int c = at;
+        for (const float x : v) {
+          const uint32_t w = static_cast<uint32_t>(__builtin_fmaf(__builtin_amdgcn_fractf(place_of(x)), slope, unit));
+          if (decltype(all)::value ? x > -INFINITY : kept(x, c)) atomicAdd(sums + bin_of(x), w);
+          ++c;
+        }
+      });
+    };
+    const bool unrestricted = border_index < 0;
+    if (unrestricted) add_sums(std::true_type{});
+    else add_sums(std::false_type{});
     __syncthreads();
     {
       constexpr int PER_BINS = kSfBins / NT;
@@ -611,36 +618,35 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     // One pass with exact weights: of the bins in front of the border's (and of a neighbour, where the border is near its edge), by
     // cells; of all others; the classes of these bins.
     const float from_place = sh.where > 0 ? static_cast<float>(sh.where) : -INFINITY, to_place = sh.until < kSfBins - 1 ? static_cast<float>(sh.until + 1) : INFINITY;
-    u64 own_behind = 0, own_above = 0;
-    row.each(
-        [&](const auto& v, int at) {
-          uint32_t wanted = 0, bit = 1;
-          int c = at;
-          for (const float x : v) {
-            const bool in = kept(x, c);
-            const float place = place_of(x);
-            const u64 w = weight(x);
-            const bool front = in & (place < from_place);
-            sum += front ? w : 0;
-            own_behind += in & !front ? w : 0;
-            wanted |= in & !front & !(place >= to_place) ? bit : 0;
-            bit *= 2;
-            ++c;
-          }
-          if (__ballot(wanted != 0) != 0) {
-            c = at;
-            for (const float x : v) {
-              list((wanted & 1) != 0, x, c);
-              wanted >>= 1;
-              ++c;
+    u64 own_all = 0, own_above = 0;
+    auto add_weights = [&](auto every) {
+      row.each(
+          [&](const auto& v, int at) {
+            constexpr int N = sizeof(v) / sizeof(float);
+            bool want[N], any = false;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float place = place_of(v[e]);
+              const bool in = decltype(every)::value ? true : kept(v[e], at + e);
+              const u64 w = in ? weight(v[e]) : 0;
+              const bool front = place < from_place;
+              sum += front ? w : 0;
+              own_all += w;
+              want[e] = in & !front & (place < to_place);
+              any |= want[e];
             }
-          }
-        },
-        [&](int step) {
-          own_above += sum;
-          to_cell(step);
-        });
-    const u64 above = group_sum<WAVES>(own_above, sh.red), all = above + group_sum<WAVES>(own_behind, sh.red), target = sf_border(filter.p, all);
+            if (__ballot(any) != 0)
+#pragma unroll
+              for (int e = 0; e < N; ++e) list(want[e], v[e], at + e);
+          },
+          [&](int step) {
+            own_above += sum;
+            to_cell(step);
+          });
+    };
+    if (unrestricted) add_weights(std::true_type{});
+    else add_weights(std::false_type{});
+    const u64 above = group_sum<WAVES>(own_above, sh.red), all = group_sum<WAVES>(own_all, sh.red), target = sf_border(filter.p, all);
     const int count = sh.listed;
     if (tid == 0) sh.found = 0;
     if (count <= kSfListed && above < target) {
