@@ -10,6 +10,7 @@ namespace ak {
 constexpr int kGnThreads = 256;
 constexpr int kGnBlocks = 1024;            // work groups of all norm launches of a call: so many partial sums
 constexpr int64_t kGnChunk = 16384;        // elements
+constexpr int kGnAhead = 4;                // 16-byte loads a thread has on their way
 constexpr int kGnNormTensors = 180, kGnClipTensors = 130;      // whose tables fit 4 KB of kernel arguments
 
 struct GnNormTable {
@@ -85,8 +86,21 @@ static __global__ __launch_bounds__(kGnThreads) void gn_partial_kernel(GnNormTab
     const int type = static_cast<int>(t.size[i] & 3);
     gn_with_type(type, [&](auto xt) {
       using X = typename decltype(xt)::type;
-      const X* __restrict__ x = static_cast<const X*>(t.src[i]);
-      for (int64_t e = from + threadIdx.x; e < to; e += kGnThreads) acc = gn_take<KIND>(acc, static_cast<float>(x[e]));
+      constexpr int E = 16 / sizeof(X), STEP = kGnThreads * E;
+      const X* __restrict__ x = static_cast<const X*>(t.src[i]) + from;
+      const int count = static_cast<int>(to - from), mine = static_cast<int>(threadIdx.x) * E;
+      int at = mine;
+      for (; at + (kGnAhead - 1) * STEP + E <= count; at += kGnAhead * STEP) {
+        Some<X, E> some[kGnAhead];
+#pragma unroll
+        for (int a = 0; a < kGnAhead; ++a) some[a].load(x + at + a * STEP);
+#pragma unroll
+        for (int a = 0; a < kGnAhead; ++a)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc = gn_take<KIND>(acc, some[a].get(e));
+      }
+      for (; at < count; at += STEP)
+        for (int e = at; e < at + E && e < count; ++e) acc = gn_take<KIND>(acc, static_cast<float>(x[e]));
     });
   }
   acc = gn_group<KIND>(acc, red);
@@ -116,7 +130,8 @@ static __global__ __launch_bounds__(kGnThreads) void gn_clip_kernel(GnClipTable 
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
   const double most = max_norm / (n + 1e-6);
   const float c = static_cast<float>(most > 1. ? 1. : most);           // (NaN stays)
-  for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+  // (from the end, which the pass before has read last)
+  for (int chunk = t.chunks - 1 - static_cast<int>(blockIdx.x); chunk >= 0; chunk -= gridDim.x) {
     const int i = gn_find(t, chunk);
     if (c == 1.f && t.src[i] == t.dst[i]) continue;
     const int64_t n_el = t.size[i] >> 4, from = (chunk - t.first[i]) * kGnChunk, to = from + kGnChunk < n_el ? from + kGnChunk : n_el;
@@ -125,9 +140,25 @@ static __global__ __launch_bounds__(kGnThreads) void gn_clip_kernel(GnClipTable 
       using X = typename decltype(xt)::type;
       auto scale = [&](auto yt) {
         using Y = typename decltype(yt)::type;
-        const X* x = static_cast<const X*>(t.src[i]);
-        Y* y = static_cast<Y*>(t.dst[i]);
-        for (int64_t e = from + threadIdx.x; e < to; e += kGnThreads) y[e] = static_cast<Y>(c * static_cast<float>(x[e]));
+        constexpr int E = 16 / sizeof(X), STEP = kGnThreads * E;
+        const X* x = static_cast<const X*>(t.src[i]) + from;         // (may be y)
+        Y* y = static_cast<Y*>(t.dst[i]) + from;
+        const int count = static_cast<int>(to - from);
+        int at = static_cast<int>(threadIdx.x) * E;
+        for (; at + (kGnAhead - 1) * STEP + E <= count; at += kGnAhead * STEP) {
+          Some<X, E> some[kGnAhead];
+#pragma unroll
+          for (int a = 0; a < kGnAhead; ++a) some[a].load(x + at + a * STEP);
+#pragma unroll
+          for (int a = 0; a < kGnAhead; ++a) {
+            Some<Y, E> out;
+#pragma unroll
+            for (int e = 0; e < E; ++e) out.set(e, c * some[a].get(e));
+            out.store(y + at + a * STEP);
+          }
+        }
+        for (; at < count; at += STEP)
+          for (int e = at; e < at + E && e < count; ++e) y[e] = static_cast<Y>(c * static_cast<float>(x[e]));
       };
       if (to_type == type) scale(Type<X>{});
       else scale(Type<float>{});

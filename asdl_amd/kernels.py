@@ -4,6 +4,7 @@ Every function takes tensors that live on a ROCm device, passes raw device point
 calling thread's current HIP stream to libasdl_amd.so, and returns without synchronising.
 There is no CPU path: a CPU tensor raises.
 """
+import array
 import contextlib
 import ctypes
 import struct
@@ -178,13 +179,6 @@ _here = contextlib.nullcontext()
 def _device_of(device):
     """Context in which launches for a tensor run on its device, current or not."""
     return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _scratch(nbytes, device):
-    """Scratch memory of one call, from torch's allocator and not from workspace(): under a stream capture it belongs to that graph, so
-    that graphs which are replayed side by side share none."""
-    with _on_launch_stream():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _pointer(t):
@@ -1446,45 +1440,65 @@ def _dense(t):
     return True
 
 
-def _norm_items(grads, outs):
-    """(device, rows of ak_clip_grad_norm, [(tensor, dense one whose values it takes after the launch)]) of gradients and where their
-    scaled values go; outs None: only the norm is asked for."""
-    rows, late, device, seen = [], [], None, {}
+def _norm_rows_of(grads, outs):
+    """(columns of the table of ak_clip_grad_norm, [(tensor, dense one whose values it takes after the launch)], what lives until then)
+    of gradients and where their scaled values go (None: only the norm is asked for).  A model has hundreds of them: what holds for
+    all is looked at in one sweep each."""
+    device = grads[0].device
+    index = grads[0].get_device()
+    types = [_ELEMENT_TYPES.get(g.dtype) for g in grads]
+    if None in types or any(g.get_device() != index for g in grads):
+        for g in grads:
+            _require_gpu(g)
+            _element_type(g, 'a gradient')
+            _require_one_gpu(device, gradient=g)
+    sizes = [g.numel() for g in grads]
+    sources = [g.data_ptr() for g in grads]
+    odd = {i for i, g in enumerate(grads) if not g.is_contiguous()}
+    results, result_types = sources, types
+    if outs is not None and outs is not grads:
+        result_types = [_ELEMENT_TYPES.get(o.dtype) for o in outs]
+        for i, (o, n, a, b) in enumerate(zip(outs, sizes, types, result_types)):
+            if o.get_device() != index or o.numel() != n or (a != b and b != AK_F32):
+                _require_gpu(o)
+                _require_one_gpu(device, result=o)
+                raise ValueError(f'the result of a gradient has its number of elements and its type or float32. Got {tuple(o.shape)}, '
+                                 f'{o.dtype} for {tuple(grads[i].shape)}, {grads[i].dtype}.')
+            if not o.is_contiguous():
+                odd.add(i)
+        results = [o.data_ptr() for o in outs]
+    late, keep = [], []
+    if not odd and 0 not in sources and len(set(sources)) == len(sources):
+        return sources, results, sizes, types, result_types, late, keep
+    # some without elements, in another order of elements, listed twice
+    sources, results = list(sources), list(results)
+    seen = {}
     for i, grad in enumerate(grads):
-        code = _ELEMENT_TYPES.get(grad.dtype)
-        if code is None or grad.device != device:
-            _require_gpu(grad)
-            _element_type(grad, 'a gradient')
-            if device is None:
-                device = grad.device
-            _require_one_gpu(device, gradient=grad)
-        out = None if outs is None else outs[i]
-        if out is not None and out is not grad:
-            _require_gpu(out)
-            _require_one_gpu(device, result=out)
-            if out.shape != grad.shape or out.dtype not in (grad.dtype, torch.float32):
-                raise ValueError(f'the result of a gradient has its shape and its type or float32. Got {tuple(out.shape)}, {out.dtype} for '
-                                 f'{tuple(grad.shape)}, {grad.dtype}.')
-        n = grad.numel()
-        if n == 0:
+        if sizes[i] == 0:
             continue
+        out = None if outs is None else outs[i]
         if out is not None and any(st == 0 and size > 1 for st, size in zip(out.stride(), out.shape)):
             raise ValueError('a tensor whose elements share memory (an expanded one) cannot take scaled values.')
-        dense = _dense(grad)
-        key = (grad.data_ptr(), n) if dense else (grad.data_ptr(), grad.shape, grad.stride())
+        dense = i not in odd or _dense(grad)
+        key = (sources[i], sizes[i]) if dense else (sources[i], grad.shape, grad.stride())
         if key in seen:                       # a gradient that two parameters share counts once
             first, first_out = seen[key]
             if out is not None and out.data_ptr() != first_out.data_ptr():
                 if first.stride() != grad.stride() and not (first.is_contiguous() and grad.is_contiguous()):
                     raise ValueError('a gradient that is listed twice, in two orders of its elements, has no two results.')
                 late.append((out, first_out))
+            sizes[i] = 0
             continue
         seen[key] = grad, out
-        src, dst = grad, out
-        if out is None:
-            src = grad if dense else _contiguous(grad)
-        elif not (grad.stride() == out.stride() and dense) and not (grad.is_contiguous() and out.is_contiguous()):
-            src = _contiguous(grad)
+        if i not in odd or (dense and (out is None or (grad.shape == out.shape and grad.stride() == out.stride()))):
+            continue
+        if out is not None and out.shape != grad.shape:
+            raise ValueError(f'the result of a gradient that is not contiguous has its shape. Got {tuple(out.shape)} for {tuple(grad.shape)}.')
+        src = grad if grad.is_contiguous() else _contiguous(grad.detach())
+        keep.append(src)
+        sources[i] = src.data_ptr()
+        if out is not None:
+            dst = out
             if out is grad:
                 dst = src
             elif not out.is_contiguous():
@@ -1492,66 +1506,66 @@ def _norm_items(grads, outs):
                     dst = torch.empty(out.shape, dtype=out.dtype, device=device)
             if dst is not out:
                 late.append((out, dst))
-        rows.append((src, dst, n, code))
-    return device, rows, late
+            results[i] = dst.data_ptr()
+    return sources, results, sizes, types, result_types, late, keep
 
 
-def _launch_norm(rows, device, norm_type, max_norm):
+def _launch_norm(grads, outs, norm_type, max_norm):
     lib = _lib.load()
-    table = []
-    for src, dst, n, code in rows:
-        table += (src.data_ptr(), 0 if dst is None else dst.data_ptr(), n, code, code if dst is None else _ELEMENT_TYPES[dst.dtype])
-    table = (ctypes.c_int64 * len(table))(*table)
-    need = lib.ak_grad_norm_ws_bytes(len(rows))
+    count, device = len(grads), grads[0].device
+    sources, results, sizes, types, result_types, late, keep = _norm_rows_of(grads, outs)
+    table = array.array('q', [0]) * (5 * count)
+    for column, values in enumerate((sources, results, sizes, types, result_types)):
+        table[column::5] = array.array('q', values)
+    need = lib.ak_grad_norm_ws_bytes(count)
     with _on_launch_stream():
         norm = torch.empty((), dtype=torch.float32, device=device)
-    ws = _scratch(need, device)
-    kind = _NORM_KINDS[norm_type]
-    if max_norm is None:
-        _lib.check(lib.ak_grad_norm(table, len(rows), kind, norm.data_ptr(), ws.data_ptr(), need, _stream_handle(device)), 'ak_grad_norm')
-    else:
-        rc = lib.ak_clip_grad_norm(table, len(rows), kind, max_norm, norm.data_ptr(), ws.data_ptr(), need, _stream_handle(device))
-        _lib.check(rc, 'ak_clip_grad_norm')
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+    address = table.buffer_info()[0]
+    if outs is None:
+        _lib.check(lib.ak_grad_norm(address, count, _NORM_KINDS[norm_type], norm.data_ptr(), ws.data_ptr(), need, _stream_handle(device)),
+                   'ak_grad_norm')
+        return norm
+    rc = lib.ak_clip_grad_norm(address, count, _NORM_KINDS[norm_type], max_norm, norm.data_ptr(), ws.data_ptr(), need, _stream_handle(device))
+    _lib.check(rc, 'ak_clip_grad_norm')
+    if late:
+        with torch.no_grad(), _on_launch_stream():
+            for out, dense in late:
+                out.copy_(dense.reshape(out.shape))
     return norm
 
 
 def _norm_arguments(grads, norm_type):
-    grads = [g.detach() for g in grads]
+    grads = list(grads)
     if not grads:
         raise ValueError('there is no gradient to take a norm of.')
     if float(norm_type) not in _NORM_KINDS:
         raise ValueError(f'norm_type has to be 2, 1 or inf. Got {norm_type}.')
     _require_gpu(grads[0])
-    return grads
+    return grads, float(norm_type)
 
 
 def grad_norm(grads, norm_type=2.0):
     """The norm of all elements of ``grads`` (tensors of float32, bfloat16 or float16 on one device) as one vector, a 0-d float32 tensor:
     norm_type 2, 1 or inf.  Sums are double, in a fixed order.  A gradient that is listed twice counts once."""
-    grads = _norm_arguments(grads, norm_type)
+    grads, norm_type = _norm_arguments(grads, norm_type)
     with _device_of(grads[0].device):
-        device, rows, _ = _norm_items(grads, None)
-        return _launch_norm(rows, device, float(norm_type), None)
+        return _launch_norm(grads, None, norm_type, None)
 
 
 def clip_grad_norm(grads, max_norm, norm_type=2.0, outs=None):
     """Scales ``grads`` in place by min(1, max_norm / (norm + 1e-6)) and returns their norm before, as grad_norm() gives it; with ``outs``
-    the gradients stay and the scaled values go to these tensors (of the same shapes; of the gradient's type or float32).  A norm that is
-    infinite gives the factor 0, one that is NaN the factor NaN, as torch.nn.utils.clip_grad_norm_ does.  Gradients (results) of
-    different entries may not overlap, except that one listed twice is scaled once.  Nothing is read by the host."""
-    grads = _norm_arguments(grads, norm_type)
+    the gradients stay and the scaled values go to these tensors (of as many elements in the same order, and of the gradient's type or
+    float32).  A norm that is infinite gives the factor 0, one that is NaN the factor NaN, as torch.nn.utils.clip_grad_norm_ does.
+    Gradients (results) of different entries may not overlap, except that one listed twice is scaled once.  Nothing is read by the host."""
+    grads, norm_type = _norm_arguments(grads, norm_type)
     if not max_norm >= 0:
         raise ValueError(f'max_norm has to be at least 0. Got {max_norm}.')
-    outs = grads if outs is None else [o.detach() for o in outs]
+    outs = grads if outs is None else list(outs)
     if len(outs) != len(grads):
         raise ValueError(f'{len(grads)} gradients and {len(outs)} results.')
     with _device_of(grads[0].device):
-        device, rows, late = _norm_items(grads, outs)
-        norm = _launch_norm(rows, device, float(norm_type), max_norm)
-        with _on_launch_stream():
-            for out, dense in late:
-                out.copy_(dense.reshape(out.shape))
-    return norm
+        return _launch_norm(grads, outs, norm_type, max_norm)
 
 
 # ------------------------------------------------------------------------------ low-rank (swift) factors
