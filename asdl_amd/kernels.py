@@ -176,6 +176,16 @@ def _require_one_gpu(device, **tensors):
 _here = contextlib.nullcontext()
 
 
+def _empty_on_launch_stream(*args, **kwargs):
+    with _on_launch_stream():
+        return torch.empty(*args, **kwargs)
+
+
+def _allocator():
+    """torch.empty, on the stream that this thread's launches go to."""
+    return torch.empty if getattr(_override, 'stream', None) is None else _empty_on_launch_stream
+
+
 def _device_of(device):
     """Context in which launches for a tensor run on its device, current or not."""
     return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
@@ -1353,22 +1363,24 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     elif out_dtype != x.dtype and out_dtype != torch.float32:
         raise TypeError(f'the result is {x.dtype} or float32. Got {out_dtype}.')
     device = x.device
-    with _device_of(device):
-        x, ldx = _rows_of(x, F)
-        w_dtype = torch.float32
-        if bias is not None:
-            bias = _norm_vector(bias, F, x, 'bias')
-            w_dtype = bias.dtype
-        if weight is not None:
-            weight = _norm_vector(weight, F, x, 'weight')
-            if bias is not None and weight.dtype != w_dtype:
-                raise TypeError(f'weight and bias have to be of one type. Got {weight.dtype} and {w_dtype}.')
-            w_dtype = weight.dtype
-        with _on_launch_stream():
-            y = torch.empty(x.shape, dtype=out_dtype, device=device)
-            mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=device)
-        rc = _lib.load().ak_layer_norm(x.data_ptr(), x_code, ldx, _pointer(weight), _pointer(bias), _ELEMENT_TYPES[w_dtype], rows, F, eps,
-                                       y.data_ptr(), _ELEMENT_TYPES[out_dtype], F, mean.data_ptr(), rstd.data_ptr(), _stream_handle(device))
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return layer_norm(x, weight, bias, eps, out_dtype)
+    empty = _allocator()
+    x, ldx = _rows_of(x, F)
+    w_dtype = torch.float32
+    if bias is not None:
+        bias = _norm_vector(bias, F, x, 'bias')
+        w_dtype = bias.dtype
+    if weight is not None:
+        weight = _norm_vector(weight, F, x, 'weight')
+        if bias is not None and weight.dtype != w_dtype:
+            raise TypeError(f'weight and bias have to be of one type. Got {weight.dtype} and {w_dtype}.')
+        w_dtype = weight.dtype
+    y = empty(x.shape, dtype=out_dtype, device=device)
+    mean, rstd = empty((2, *x.shape[:-1]), dtype=torch.float32, device=device).unbind()
+    rc = _lib.load().ak_layer_norm(x.data_ptr(), x_code, ldx, _pointer(weight), _pointer(bias), _ELEMENT_TYPES[w_dtype], rows, F, eps,
+                                   y.data_ptr(), _ELEMENT_TYPES[out_dtype], F, mean.data_ptr(), rstd.data_ptr(), _stream_handle(device))
     _lib.check(rc, 'ak_layer_norm')
     return y, mean, rstd
 
@@ -1394,32 +1406,34 @@ def layer_norm_backward(g, x, mean, rstd, weight=None, blocks=None, alpha=1.0, b
     if g.device != device or mean.device != device or rstd.device != device or (blocks is not None and blocks.device != device):
         _require_gpu(g, mean, rstd, blocks)
         _require_one_gpu(device, g=g, mean=mean, rstd=rstd, blocks=blocks)
-    with _device_of(device):
-        x, ldx = _rows_of(x, F)
-        g, ldg = _rows_of(g, F)
-        if weight is not None:
-            weight = _norm_vector(weight, F, x, 'weight')
-            weight_dtype = weight.dtype
-        elif weight_dtype is None:
-            weight_dtype = torch.float32
-        elif weight_dtype != x.dtype and weight_dtype != torch.float32:
-            raise TypeError(f'the weight has to be {x.dtype} or float32. Got {weight_dtype}.')
-        lib = _lib.load()
-        dx = dw = db = ws = None
-        need = 0
-        with _on_launch_stream():
-            if need_x:
-                dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-            if need_weight:
-                dw = torch.empty(F, dtype=weight_dtype, device=device)
-            if need_bias:
-                db = torch.empty(F, dtype=weight_dtype, device=device)
-            if need_weight or need_bias or blocks is not None:
-                need = _ws_need('ak_layer_norm_backward_ws_bytes', rows, F, blocks is not None)
-                ws = torch.empty(need, dtype=torch.uint8, device=device)
-        rc = lib.ak_layer_norm_backward(g.data_ptr(), g_code, ldg, x.data_ptr(), x_code, ldx, mean.data_ptr(), rstd.data_ptr(),
-                                        _pointer(weight), _ELEMENT_TYPES[weight_dtype], rows, F, _pointer(dx), F, _pointer(dw),
-                                        _pointer(db), _pointer(blocks), alpha, beta, _pointer(ws), need, _stream_handle(device))
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return layer_norm_backward(g, x, mean, rstd, weight, blocks, alpha, beta, need_x, need_weight, need_bias, weight_dtype)
+    x, ldx = _rows_of(x, F)
+    g, ldg = _rows_of(g, F)
+    if weight is not None:
+        weight = _norm_vector(weight, F, x, 'weight')
+        weight_dtype = weight.dtype
+    elif weight_dtype is None:
+        weight_dtype = torch.float32
+    elif weight_dtype != x.dtype and weight_dtype != torch.float32:
+        raise TypeError(f'the weight has to be {x.dtype} or float32. Got {weight_dtype}.')
+    empty = _allocator()
+    dx = dw = db = ws = None
+    need = 0
+    if need_x:
+        dx = empty(x.shape, dtype=x.dtype, device=device)
+    if need_weight:
+        dw = empty(F, dtype=weight_dtype, device=device)
+    if need_bias:
+        db = empty(F, dtype=weight_dtype, device=device)
+    if need_weight or need_bias or blocks is not None:
+        # not workspace(): under a stream capture this belongs to that graph, so that graphs replayed side by side share none
+        need = _ws_need('ak_layer_norm_backward_ws_bytes', rows, F, blocks is not None)
+        ws = empty(need, dtype=torch.uint8, device=device)
+    rc = _lib.load().ak_layer_norm_backward(g.data_ptr(), g_code, ldg, x.data_ptr(), x_code, ldx, mean.data_ptr(), rstd.data_ptr(),
+                                            _pointer(weight), _ELEMENT_TYPES[weight_dtype], rows, F, _pointer(dx), F, _pointer(dw),
+                                            _pointer(db), _pointer(blocks), alpha, beta, _pointer(ws), need, _stream_handle(device))
     _lib.check(rc, 'ak_layer_norm_backward')
     return dx, dw, db
 
@@ -1430,7 +1444,7 @@ _NORM_KINDS = {2.0: 0, 1.0: 1, float('inf'): 2}
 
 def _dense(t):
     """Whether the elements of ``t`` fill one run of memory, in whatever order."""
-    if t.is_contiguous():
+    if t.is_contiguous() or (t.ndim == 4 and t.is_contiguous(memory_format=torch.channels_last)):
         return True
     expect = 1
     for stride, size in sorted((st, si) for si, st in zip(t.shape, t.stride()) if si != 1):
@@ -1468,18 +1482,21 @@ def _norm_rows_of(grads, outs):
                 odd.add(i)
         results = [o.data_ptr() for o in outs]
     late, keep = [], []
-    if not odd and 0 not in sources and len(set(sources)) == len(sources):
+    plain = 0 not in sources and len(set(sources)) == len(sources)
+    if plain and not odd:
         return sources, results, sizes, types, result_types, late, keep
     # some without elements, in another order of elements, listed twice
     sources, results = list(sources), list(results)
     seen = {}
-    for i, grad in enumerate(grads):
+    for i in sorted(odd) if plain else range(len(grads)):
+        grad = grads[i]
         if sizes[i] == 0:
             continue
         out = None if outs is None else outs[i]
-        if out is not None and any(st == 0 and size > 1 for st, size in zip(out.stride(), out.shape)):
-            raise ValueError('a tensor whose elements share memory (an expanded one) cannot take scaled values.')
         dense = i not in odd or _dense(grad)
+        same = out is grad or out is None or (grad.shape == out.shape and grad.stride() == out.stride())
+        if not (dense and same) and out is not None and any(st == 0 and size > 1 for st, size in zip(out.stride(), out.shape)):
+            raise ValueError('a tensor whose elements share memory (an expanded one) cannot take scaled values.')
         key = (sources[i], sizes[i]) if dense else (sources[i], grad.shape, grad.stride())
         if key in seen:                       # a gradient that two parameters share counts once
             first, first_out = seen[key]
@@ -1490,7 +1507,7 @@ def _norm_rows_of(grads, outs):
             sizes[i] = 0
             continue
         seen[key] = grad, out
-        if i not in odd or (dense and (out is None or (grad.shape == out.shape and grad.stride() == out.stride()))):
+        if i not in odd or (dense and same):
             continue
         if out is not None and out.shape != grad.shape:
             raise ValueError(f'the result of a gradient that is not contiguous has its shape. Got {tuple(out.shape)} for {tuple(grad.shape)}.')
