@@ -16,4 +16,6 @@ from .prec_grad_maker import (PreconditionedGradientMaker, PreconditioningConfig
                               INTERVAL_CONSTANT, INTERVAL_STEP, INTERVAL_LINEAR, INTERVAL_TYPES)
 from .natural_gradient import NaturalGradientMaker, KfacGradientMaker
 from .shampoo import ShampooGradientMaker, Preconditioner, BlockPartitioner, compute_power
+from .layers import layer_norm, FusedLayerNorm, fuse_layer_norms
+from .clipping import clip_grad_norm_
 from . import kernels

@@ -8,6 +8,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.graph import GradientEdge
 
+from .layers import FusedLayerNorm
 from .matrices import *
 from .operations import *
 from .operations import FWD_OPS, BWD_OPS, BWD_OPS_WITH_INPUTS
@@ -109,11 +110,16 @@ def extend(model, *op_names, ignore_modules=None, map_rule=None, vectors=None, s
                 y = out_data.detach() if _needs_out else None
                 run_hook(lambda: _op.forward_post_process(x, y), x)
                 if _has_bwd and out_data.requires_grad:
+                    node = out_data.grad_fn if hasattr(_op, 'backward_of') and hasattr(out_data.grad_fn, 'takes_blocks_request') else None
+
                     def grad_hook(grad, _m=_module):
                         if not cxt.is_operation_registered(_m):
                             return None          # context already closed
                         g = grad.detach()
-                        run_hook(lambda: _op.backward_pre_process(g, None), g, backward=True)
+                        if node is not None:
+                            _op.backward_of(node, g)        # (launches nothing: the backward pass does that)
+                        else:
+                            run_hook(lambda: _op.backward_pre_process(g, None), g, backward=True)
                         return None
                     handles.append(out_data.register_hook(grad_hook))
                     # the graph edge the hook sits on: a backward pass restricted to these edges still fires
@@ -213,6 +219,8 @@ def module_wise_assignments(model, *assign_rules, ignore_modules=None, map_rule=
             values = specified[next(key for key in name_rules if key in name)]
         elif module.__class__ in specified:
             values = specified[module.__class__]
+        elif isinstance(module, FusedLayerNorm) and nn.LayerNorm in specified:      # it stands in for one
+            values = specified[nn.LayerNorm]
         else:
             if len(common) == 0:
                 continue

@@ -66,6 +66,16 @@ class FisherConfig:
     all_reduce: bool = False
     is_master: bool = True
     ignore_index: int = -1
+    # what the sampled Fisher draws its targets from: the model's predictive distribution at this temperature, restricted to its
+    # likely classes (kernels.sample_filtered); the defaults are the distribution itself
+    mc_temperature: float = 1.
+    mc_top_k: int = None
+    mc_top_p: float = None
+    mc_min_p: float = None
+
+    @property
+    def mc_filtered(self):
+        return self.mc_temperature != 1. or self.mc_top_k is not None or self.mc_top_p is not None or self.mc_min_p is not None
 
 
 class FisherMaker(GradientMaker):
@@ -349,13 +359,23 @@ class FisherMCCrossEntropy(FisherMaker):
         n_mc_samples = self.config.n_mc_samples
         log_probs = F.log_softmax(logits, dim=-1)
         dist = None
-        if self._sampling_replaced or not kernels.sampleable(logits):
+        filtered = self.config.mc_filtered and not self._sampling_replaced
+        if not filtered and (self._sampling_replaced or not kernels.sampleable(logits)):
             # validate_args=False: the check of the simplex constraint would synchronise the host with the forward
             # pass; the draw itself (normalisation + multinomial) is unchanged
             dist = torch.distributions.Categorical(F.softmax(logits, dim=-1), validate_args=False)
         for i in range(n_mc_samples):
             with torch.no_grad():
-                if dist is None:
+                if filtered:
+                    config = self.config
+                    filters = dict(temperature=config.mc_temperature, top_k=config.mc_top_k, top_p=config.mc_top_p, min_p=config.mc_min_p)
+                    if i == 0:
+                        targets, drawn = kernels.sample_filtered(logits, late=True, **filters)
+                        if drawn is not None:
+                            self._sampled.append(drawn)
+                    else:
+                        targets = kernels.sample_filtered(logits, check=False, **filters)
+                elif dist is None:
                     targets, drawn = kernels.sample_categorical(logits, late=True)
                     if i == 0 and drawn is not None:       # (the same logits every time)
                         self._sampled.append(drawn)
@@ -429,6 +449,8 @@ def get_fisher_maker(model: nn.Module, config: FisherConfig):
     loss_type = config.loss_type
     if fisher_type not in _supported_types:
         raise ValueError(f'Invalid fisher_type: {fisher_type}. {_supported_types} are supported.')
+    if config.mc_filtered and (fisher_type != FISHER_MC or loss_type != LOSS_CROSS_ENTROPY):
+        raise ValueError(f'mc_temperature, mc_top_k, mc_top_p and mc_min_p are for {FISHER_MC} with {LOSS_CROSS_ENTROPY}.')
     if fisher_type == FISHER_EMP:
         return FisherEmp(model, config)
     if loss_type not in [LOSS_CROSS_ENTROPY, LOSS_MSE]:

@@ -1,0 +1,99 @@
+"""Layer norm on the kernels of csrc/layer_norm.hip as a function and as a module that stands in for torch.nn.LayerNorm.
+
+Under the hooks of a gradient maker such a module has its unit-wise Fisher blocks computed by its own backward pass, from the values
+that pass reads anyway, where torch.nn.LayerNorm has its output and output gradient read once more
+(asdl/operations/layernorm.py:69-78)."""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import kernels
+
+__all__ = ['layer_norm', 'FusedLayerNorm', 'fuse_layer_norms']
+
+
+class BlocksRequest:
+    """Fisher blocks that a hook wants of a backward pass that is about to run: blocks <- beta*blocks + alpha * sums for the output
+    gradient ``g``.  Served once, by the backward pass or, where that does not run or sees another gradient, by settle()."""
+
+    def __init__(self, node, g, blocks, alpha, beta):
+        self.x, _, self.mean, self.rstd = node.saved_tensors
+        self.g, self.version = g, g._version
+        self.blocks, self.alpha, self.beta = blocks, alpha, beta
+        self.open = True
+
+    def fits(self, g):
+        return g.data_ptr() == self.g.data_ptr() and g.numel() == self.g.numel() and g.is_contiguous() and self.g.is_contiguous() and \
+            self.g._version == self.version
+
+    def settle(self):
+        if self.open:
+            self.open = False
+            kernels.layer_norm_backward(self.g.reshape(self.x.shape), self.x, self.mean, self.rstd, blocks=self.blocks, alpha=self.alpha, beta=self.beta,
+                                        need_x=False, need_weight=False, need_bias=False)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, out_dtype):
+        y, mean, rstd = kernels.layer_norm(x, weight, bias, eps, out_dtype)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.has_bias = bias is not None
+        ctx.weight_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else None
+        ctx.takes_blocks_request = True
+        ctx.request = None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, mean, rstd = ctx.saved_tensors
+        request, ctx.request = ctx.request, None
+        blocks, alpha, beta = None, 1.0, 0.0
+        if request is not None and request.open:
+            if request.fits(g):
+                request.open = False
+                blocks, alpha, beta = request.blocks, request.alpha, request.beta
+            else:
+                request.settle()
+        need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
+        dx, dw, db = kernels.layer_norm_backward(g, x, mean, rstd, weight, blocks, alpha, beta, need_x, need_weight, need_bias,
+                                                 weight_dtype=ctx.weight_dtype)
+        return dx, dw, db, None, None
+
+
+def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
+    """torch.nn.functional.layer_norm for tensors on a ROCm device (float32, bfloat16 or float16; weight and bias of the type of x or
+    float32), differentiable once.  Under autocast the result is float32, as there, and x is read as it is."""
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    if not shape or tuple(x.shape[-len(shape):]) != shape:
+        raise ValueError(f'x has to end in the dimensions {shape}. Got the shape {tuple(x.shape)}.')
+    for name, v in (('weight', weight), ('bias', bias)):
+        if v is not None and tuple(v.shape) != shape:
+            raise ValueError(f'{name} has to have the shape {shape}. Got {tuple(v.shape)}.')
+    autocast = torch.is_autocast_enabled()
+    out_dtype = torch.float32 if autocast else x.dtype
+    if autocast:
+        weight = weight.float() if weight is not None and weight.dtype != x.dtype else weight
+        bias = bias.float() if bias is not None and (bias.dtype != x.dtype or (weight is not None and weight.dtype != x.dtype)) else bias
+        weight = weight.float() if weight is not None and bias is not None and weight.dtype != bias.dtype else weight
+    if len(shape) == 1:
+        return _LayerNorm.apply(x, weight, bias, eps, out_dtype)
+    flat = x.flatten(-len(shape))
+    return _LayerNorm.apply(flat, None if weight is None else weight.flatten(), None if bias is None else bias.flatten(), eps, out_dtype).view(x.shape)
+
+
+class FusedLayerNorm(nn.LayerNorm):
+    """torch.nn.LayerNorm (the same arguments, parameters and state dict) on layer_norm() above."""
+
+    def forward(self, input):
+        return layer_norm(input, self.normalized_shape, self.weight, self.bias, self.eps)
+
+
+def fuse_layer_norms(model: nn.Module) -> int:
+    """Makes every torch.nn.LayerNorm of ``model`` (not subclasses of it) a FusedLayerNorm, in place: parameters, hooks and names stay.
+    Returns how many there were."""
+    found = [m for m in model.modules() if type(m) is nn.LayerNorm]
+    for m in found:
+        m.__class__ = FusedLayerNorm
+    return len(found)

@@ -76,7 +76,8 @@ class NaturalGradientMaker(PreconditionedGradientMaker):
 
     def __init__(self, model, config: PreconditioningConfig, fisher_type: str = FISHER_MC,
                  fisher_shape: Union[str, List[Any]] = SHAPE_KRON, loss_type: str = LOSS_CROSS_ENTROPY,
-                 scale: float = 1, grad_scale: float = 1, n_mc_samples: int = 1, var: float = 1., seed: int = None):
+                 scale: float = 1, grad_scale: float = 1, n_mc_samples: int = 1, var: float = 1., seed: int = None,
+                 mc_temperature: float = 1., mc_top_k: int = None, mc_top_p: float = None, mc_min_p: float = None):
         from torch.nn.parallel import DistributedDataParallel as DDP
         if isinstance(model, DDP):
             raise TypeError(f'{DDP} is not supported.')
@@ -116,7 +117,7 @@ class NaturalGradientMaker(PreconditionedGradientMaker):
 
         fisher_config = FisherConfig(fisher_type=fisher_type, fisher_shapes=fisher_shape, loss_type=loss_type,
                                      n_mc_samples=n_mc_samples, ignore_modules=config.ignore_modules, var=var,
-                                     seed=seed)
+                                     seed=seed, mc_temperature=mc_temperature, mc_top_k=mc_top_k, mc_top_p=mc_top_p, mc_min_p=mc_min_p)
         self.fisher_maker = get_fisher_maker(model, fisher_config)
         self.fisher_type = fisher_type
         self.fisher_shape = fisher_shape
@@ -584,12 +585,15 @@ class KfacGradientMaker(NaturalGradientMaker):
 
     BatchNorm1d/2d and LayerNorm modules get the unit-wise shape, as in the reference; ``swift=True`` keeps the
     factors of layers that see fewer samples than they have columns as row matrices (SKFAC).  Embedding modules
-    have no kernels in this build (exclude them through ``config.ignore_modules``)."""
+    have no kernels in this build (exclude them through ``config.ignore_modules``).  ``mc_temperature``, ``mc_top_k``, ``mc_top_p``,
+    ``mc_min_p``: FISHER_MC draws its targets from the predictive distribution so restricted (kernels.sample_filtered)."""
 
     def __init__(self, model, config: PreconditioningConfig, fisher_type: str = FISHER_MC,
                  loss_type: str = LOSS_CROSS_ENTROPY, scale: float = 1, grad_scale: float = 1, n_mc_samples: int = 1,
-                 var: float = 1., seed: int = None, swift=False):
+                 var: float = 1., seed: int = None, swift=False, mc_temperature: float = 1., mc_top_k: int = None, mc_top_p: float = None,
+                 mc_min_p: float = None):
         fisher_shape = [SHAPE_SWIFT_KRON if swift else SHAPE_KRON, (nn.BatchNorm1d, SHAPE_UNIT_WISE), (nn.BatchNorm2d, SHAPE_UNIT_WISE),
                         (nn.LayerNorm, SHAPE_UNIT_WISE)]
         super().__init__(model, config, fisher_type=fisher_type, fisher_shape=fisher_shape, loss_type=loss_type,
-                         scale=scale, grad_scale=grad_scale, n_mc_samples=n_mc_samples, var=var, seed=seed)
+                         scale=scale, grad_scale=grad_scale, n_mc_samples=n_mc_samples, var=var, seed=seed,
+                         mc_temperature=mc_temperature, mc_top_k=mc_top_k, mc_top_p=mc_top_p, mc_min_p=mc_min_p)

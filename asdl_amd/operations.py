@@ -20,6 +20,7 @@ import torch.nn as nn
 
 from . import kernels
 from . import profiling as _profiling
+from .layers import BlocksRequest
 from .profiling import nvtx_range
 from .symmatrix import Kron, LateUnitFlags, SymMatrix, UnitWise, batched_update_inv
 from .utils import UnfoldedInput, im2col_2d, original_requires_grad
@@ -438,6 +439,9 @@ class _NormOperation(Operation):
         """[samples, features, *positions] view of an output / output-gradient tensor."""
         return tensor
 
+    def _statistics(self, y, g, weight, bias, out, alpha, beta):
+        return kernels.unit_wise_stats(y, g, weight, bias, out=out, alpha=alpha, beta=beta)
+
     def backward_pre_process(self, out_grads, vector=None):
         with nvtx_range('cov_unit_wise'):
             self._backward_pre_process(out_grads, vector)
@@ -460,10 +464,10 @@ class _NormOperation(Operation):
             store = self._op_results.setdefault(OP_COV_UNIT_WISE, {})
             existing = store.get('data')
             if existing is None:
-                store['data'] = kernels.unit_wise_stats(y, g, weight, bias, alpha=self._cov_scale)
+                store['data'] = self._statistics(y, g, weight, bias, None, self._cov_scale, 0.0)
             else:
                 beta = self._first_beta.pop('data', 1.0)
-                kernels.unit_wise_stats(y, g, weight, bias, out=existing, alpha=self._cov_scale, beta=beta)
+                self._statistics(y, g, weight, bias, existing, self._cov_scale, beta)
         else:
             first = '_unit_tmp' not in self._op_results
             cache = getattr(module, _FACTOR_CACHE_ATTR, None)
@@ -474,7 +478,7 @@ class _NormOperation(Operation):
             if buf is None or buf.shape[0] != weight.numel() or buf.device != weight.device:
                 buf = torch.empty(weight.numel(), 2, 2, dtype=torch.float32, device=weight.device)
                 cache['unit'] = buf
-            kernels.unit_wise_stats(y, g, weight, bias, out=buf, alpha=self._cov_scale, beta=0.0 if first else 1.0)
+            self._statistics(y, g, weight, bias, buf, self._cov_scale, 0.0 if first else 1.0)
             self._op_results['_unit_tmp'] = buf
             self._n_backward += 1
             if self._context is not None:
@@ -494,12 +498,34 @@ class BatchNorm(_NormOperation):
 
 class LayerNorm(_NormOperation):
     """[n, *, normalized_shape]: every leading index is a sample, the normalized shape is flattened to the
-    features (asdl/operations/layernorm.py:20-42)."""
+    features (asdl/operations/layernorm.py:20-42).  A FusedLayerNorm's blocks come from its own backward pass, of several calls each
+    from its own input (in the reference the last call's output stands for all)."""
+    _node = None            # the autograd node whose output gradient the hook has, where it takes a BlocksRequest
 
     @staticmethod
     def as_samples(module, tensor):
         f = module.weight.numel()
         return tensor.reshape(-1, f)
+
+    def backward_of(self, node, out_grads):
+        """backward_pre_process() for the call of the module that ``node`` stands for."""
+        self._node = node
+        try:
+            self.backward_pre_process(out_grads, None)
+        finally:
+            self._node = None
+
+    def _statistics(self, y, g, weight, bias, out, alpha, beta):
+        node = self._node
+        if node is None or self._context is None:
+            return super()._statistics(y, g, weight, bias, out, alpha, beta)
+        self._context.settle_blocks(out)          # (an earlier call's that nothing has served yet comes first)
+        if out is None:
+            out = torch.empty(weight.numel(), 2, 2, dtype=torch.float32, device=g.device)
+            beta = 0.0
+        node.request = BlocksRequest(node, g, out, alpha, beta)
+        self._context.open_blocks.append(node.request)
+        return out
 
 
 EAGER_COST_FRACTION = 0.6
@@ -610,6 +636,7 @@ class OperationContext:
         self._unit_flags_deferred = False
         self.factor_stream = None
         self.grad_edges = []       # autograd edges of the hooked module outputs of the latest forward pass
+        self.open_blocks = []      # BlocksRequests that backward passes may still serve
         self._eager_total = 0.0
         self._eager_done = False
         self._inverse_cost = 0.0
@@ -635,6 +662,16 @@ class OperationContext:
         self._pending_inverse = []
         self._inverse_chunks = []
         self._pending_unit = []
+        for request in self.open_blocks:
+            request.open = False
+        self.open_blocks = []
+
+    def settle_blocks(self, of=None):
+        """Has the Fisher blocks that no backward pass has computed computed now (``of``: those of this tensor only)."""
+        for request in self.open_blocks:
+            if of is None or request.blocks is of:
+                request.settle()
+        self.open_blocks = [r for r in self.open_blocks if r.open]
 
     def call_operations_in_forward(self, module, in_data, out_data):
         self.get_operation(module).forward_post_process(in_data, out_data)
@@ -643,6 +680,7 @@ class OperationContext:
         self.get_operation(module).backward_pre_process(out_grads, None)
 
     def get_result(self, module, *keys, pop=False, default=None):
+        self.settle_blocks()
         try:
             return self.get_operation(module).get_result(*keys, pop=pop, default=default)
         except KeyError:
@@ -666,6 +704,7 @@ class OperationContext:
         """Orders the current stream after the statistics kernels that ran on the factor stream."""
         if self.factor_stream is not None:
             self.factor_stream.join()
+        self.settle_blocks()
 
     # ---- deferred, batched inverses
     def set_eager_inverse(self, total_cost):
@@ -706,6 +745,7 @@ class OperationContext:
     def _invert_units(self):
         """Damped inverses of the queued unit-wise blocks (one grouped launch); their singularity flags are read
         together in check_unit_flags()."""
+        self.settle_blocks()
         ops = self._pending_unit
         self._pending_unit = []
         todo = []
@@ -888,5 +928,6 @@ class OperationContext:
             operation._first_beta['data'] = first_beta
 
     def finish_registered(self):
+        self.settle_blocks()
         for operation in self._operations.values():
             operation.finish_registered()

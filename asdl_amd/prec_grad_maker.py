@@ -7,6 +7,7 @@ from typing import Any, List
 
 import torch.nn as nn
 
+from .clipping import clip_grad_norm_
 from .grad_maker import GradientMaker
 from .profiling import nvtx_range, phase_mark
 
@@ -28,7 +29,9 @@ class PreconditioningConfig:
 
     ``ema_decay`` is the weight of the NEW statistic:
     ``curv_ema = curv_ema * (1 - ema_decay) + curv_new * ema_decay``; -1 disables the moving average.
-    ``ignore_modules``: modules, module classes or (parts of) module names to leave alone."""
+    ``ignore_modules``: modules, module classes or (parts of) module names to leave alone.
+    ``max_grad_norm``: the gradients of all parameters, as they are when the step ends, are scaled down to this 2-norm as one vector
+    (None: not); the norm before is the maker's ``grad_norm``."""
     num_total_steps: int = None
     preconditioner_upd_interval: int = _default_interval
     preconditioner_warmup_steps: int = 0
@@ -44,6 +47,7 @@ class PreconditioningConfig:
     damping: float = 1.e-7
     ema_decay: float = _invalid_value
     ignore_modules: List[Any] = None
+    max_grad_norm: float = None
 
 
 class _Cadence:
@@ -78,6 +82,7 @@ class PreconditionedGradientMaker(GradientMaker):
         self.config = config
         self._preconditioner_cadence, self._curvature_cadence = self._cadences(config)
         self.state = dict(step=0)
+        self.grad_norm = None
         kept = {}
         for name, module in model.named_modules():
             if self._is_supported(name, module):
@@ -181,7 +186,8 @@ class PreconditionedGradientMaker(GradientMaker):
                   ('bwd', self.backward, lambda: run_passes),
                   ('upd_curv', self.update_curvature, lambda: self.do_update_curvature(step)),
                   ('upd_inv', self.update_preconditioner, lambda: self.do_update_preconditioner(step)),
-                  ('precond', self.precondition, lambda: True))
+                  ('precond', self.precondition, lambda: True),
+                  ('clip', self.clip_gradients, lambda: self.config.max_grad_norm is not None))
         for name, stage, wanted in stages:
             if wanted():
                 with nvtx_range(name):
@@ -203,6 +209,10 @@ class PreconditionedGradientMaker(GradientMaker):
 
     def precondition(self):
         raise NotImplementedError
+
+    def clip_gradients(self):
+        """Scales all gradients of the model down to config.max_grad_norm; their norm before is kept, on the device."""
+        self.grad_norm = clip_grad_norm_(self.model.parameters(), self.config.max_grad_norm)
 
     def _teardown(self):
         pass

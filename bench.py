@@ -72,6 +72,8 @@ def parse():
     ap.add_argument('--no-secondary', action='store_true',
                     help='default workload only: skip the second measurement with the other setting of --inverse-flags '
                          'and the brief runs of the linear4096, resnet18_cifar and shampoo_gpt2 workloads (the `secondary` object)')
+    ap.add_argument('--fused-layer-norm', action='store_true',
+                    help='shampoo_gpt2: the layer norms of the model on this framework\'s kernels (asdl_amd.fuse_layer_norms)')
     ap.add_argument('--no-inverse-roofline', action='store_true',
                     help='skip the stand-alone timing of the damped inverses (the `roofline_inverse` object)')
     ap.add_argument('--factor-launches', choices=['default', 'single', 'grouped'], default='default',
@@ -587,6 +589,9 @@ def main_shampoo(args, dev, steps=None, warmup=None, emit=True):
     from asdl_amd import PreconditioningConfig, ShampooGradientMaker
     torch.backends.cudnn.benchmark = False
     model = bench_models.gpt2_small().to(dev)       # token embedding and output head frozen (50257-wide)
+    if getattr(args, 'fused_layer_norm', False):
+        import asdl_amd
+        asdl_amd.fuse_layer_norms(model)
     bs = 8
     x = torch.randint(0, 50257, (bs, 1024)).to(dev)
     t = torch.randint(0, 50257, (bs * 1024,)).to(dev)

@@ -1,0 +1,273 @@
+"""Layer norm, filtered draws and gradient norms without a GPU: what is refused, and the host logic around the kernels with the
+kernels replaced by their definitions."""
+import copy
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+import asdl_amd
+from asdl_amd import (FISHER_EMP, FISHER_EXACT, FISHER_MC, FisherConfig, FusedLayerNorm, KfacGradientMaker, LOSS_CROSS_ENTROPY, LOSS_MSE,
+                      PreconditioningConfig, SHAPE_KRON, ShampooGradientMaker, get_fisher_maker, kernels)
+from tests import cpu_backend
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.randn(4, 8), torch.ones(8)
+    for call in (lambda: kernels.layer_norm(x, w), lambda: kernels.layer_norm_backward(x, x, w, w), lambda: kernels.sample_filtered(x, torch.rand(4)),
+                 lambda: kernels.grad_norm([x]), lambda: kernels.clip_grad_norm([x], 1.0), lambda: FusedLayerNorm(8)(x)):
+        with pytest.raises(RuntimeError, match='ROCm device'):
+            call()
+    with pytest.raises(ValueError):
+        kernels.grad_norm([])
+
+
+def test_entry_points_refuse_bad_arguments():
+    """Before anything is launched: return codes of the C interface."""
+    from asdl_amd import _lib
+    lib = _lib.load()
+    a = 4096                                   # stands for an address; nothing reads it
+    f32, bf16, f16, bad = 0, 1, 4, 7
+
+    def norm(x=a, xt=f32, ldx=64, wt=f32, rows=4, F=64, eps=1e-5, y=a, yt=f32, ldy=64, mean=a, rstd=a):
+        return lib.ak_layer_norm(x, xt, ldx, a, a, wt, rows, F, eps, y, yt, ldy, mean, rstd, None)
+    assert norm(rows=0) == 0
+    for kw in (dict(x=None), dict(y=None), dict(mean=None), dict(rstd=None), dict(xt=bad), dict(yt=bad), dict(wt=bad), dict(xt=bf16, yt=f16, wt=f32),
+               dict(xt=bf16, yt=bf16, wt=f16), dict(rows=-1), dict(F=0), dict(ldx=63), dict(ldy=63), dict(eps=-1.0), dict(eps=math.nan)):
+        assert norm(**kw) == -1, kw
+    assert norm(rows=1 << 31) == -3 and norm(F=(1 << 30) + 1, ldx=1 << 31, ldy=1 << 31) == -3
+
+    def back(g=a, gt=f32, ldg=64, x=a, xt=f32, ldx=64, wt=f32, rows=4, F=64, dx=a, lddx=64, dw=a, db=a, blocks=None, ws=a, need=1 << 40):
+        return lib.ak_layer_norm_backward(g, gt, ldg, x, xt, ldx, a, a, a, wt, rows, F, dx, lddx, dw, db, blocks, 1.0, 0.0, ws, need, None)
+    for kw in (dict(g=None), dict(x=None), dict(gt=bad), dict(gt=bf16), dict(xt=bad), dict(wt=bf16), dict(rows=-1), dict(F=0), dict(ldg=1), dict(lddx=1)):
+        assert back(**kw) == -1, kw
+    assert back(ws=None) == -2 and back(need=8) == -2 and back(blocks=a, need=lib.ak_layer_norm_backward_ws_bytes(4, 64, 0)) == -2
+    assert back(dx=None, dw=None, db=None, ws=None) == 0          # nothing is asked for
+    assert lib.ak_layer_norm_backward_ws_bytes(0, 64, 1) == 0 and lib.ak_layer_norm_backward_ws_bytes(4, 64, 1) > lib.ak_layer_norm_backward_ws_bytes(4, 64, 0) > 0
+
+    def draw(logits=a, dtype=f32, rows=4, classes=10, ld=10, u=a, t=1.0, ts=None, targets=a):
+        return lib.ak_sample_filtered(logits, dtype, rows, classes, ld, u, 0, t, ts, 0, None, 1.0, None, 0.0, None, targets, None, None)
+    assert draw(rows=0) == 0
+    for kw in (dict(logits=None), dict(dtype=bad), dict(rows=-1), dict(classes=0), dict(ld=9), dict(u=None), dict(t=-1.0), dict(t=math.nan), dict(targets=None)):
+        assert draw(**kw) == -1, kw
+    assert draw(rows=1 << 31) == -5 and draw(classes=(1 << 30) + 1, ld=1 << 31) == -5
+
+    def clip(rows, kind=0, most=1.0, norm=a, ws=a, need=1 << 20):
+        table = (ctypes.c_int64 * len(rows))(*rows)
+        return lib.ak_clip_grad_norm(table, len(rows) // 5, kind, most, norm, ws, need, None)
+    good = [a, a, 10, f32, f32]
+    for rows, kw in ((good, dict(kind=3)), (good, dict(kind=-1)), (good, dict(most=-1.0)), (good, dict(most=math.nan)), (good, dict(norm=None)),
+                     ([0, a, 10, f32, f32], {}), ([a, 0, 10, f32, f32], {}), ([a, a, -1, f32, f32], {}), ([a, a, 10, bad, bad], {}),
+                     ([a, a, 10, f32, bf16], {}), ([a, a, 10, bf16, f16], {})):
+        assert clip(rows, **kw) == -1, (rows, kw)
+    assert clip(good, ws=None) == -2 and clip(good, need=64) == -2 and clip([a, a, 1 << 46, f32, f32]) == -5
+    assert lib.ak_grad_norm_ws_bytes(1000) > lib.ak_grad_norm_ws_bytes(0) > 0 and lib.ak_grad_norm_ws_bytes(-1) == 0
+
+
+@pytest.mark.parametrize('filters', [dict(mc_temperature=0.5), dict(mc_top_k=3), dict(mc_top_p=0.9), dict(mc_min_p=0.1)])
+def test_filters_are_for_the_sampled_fisher_of_a_cross_entropy(filters):
+    model = nn.Sequential(nn.Linear(3, 4))
+    for fisher_type, loss in ((FISHER_EMP, LOSS_CROSS_ENTROPY), (FISHER_EXACT, LOSS_CROSS_ENTROPY), (FISHER_MC, LOSS_MSE)):
+        with pytest.raises(ValueError, match='mc_temperature'):
+            get_fisher_maker(model, FisherConfig(fisher_type, [SHAPE_KRON], loss_type=loss, **filters))
+    get_fisher_maker(model, FisherConfig(FISHER_MC, [SHAPE_KRON], loss_type=LOSS_CROSS_ENTROPY, **filters))
+    maker = KfacGradientMaker(model, PreconditioningConfig(data_size=2), **filters)
+    assert all(getattr(maker.fisher_maker.config, k) == v for k, v in filters.items())
+    assert not FisherConfig(FISHER_MC, [SHAPE_KRON]).mc_filtered
+
+
+def test_layer_norm_checks_its_shapes():
+    x = torch.randn(2, 3, 4)
+    for args in ((5,), ((2, 3),), ((),)):
+        with pytest.raises(ValueError, match='has to end'):
+            asdl_amd.layer_norm(x, *args)
+    with pytest.raises(ValueError, match='weight has to have the shape'):
+        asdl_amd.layer_norm(x, 4, torch.ones(3))
+    with pytest.raises(ValueError, match='bias has to have the shape'):
+        asdl_amd.layer_norm(x, (3, 4), torch.ones(3, 4), torch.ones(12))
+
+
+def test_fuse_layer_norms_keeps_parameters_and_subclasses():
+    class Mine(nn.LayerNorm):
+        pass
+    model = nn.Sequential(nn.LayerNorm(4), nn.Linear(4, 4), nn.Sequential(nn.LayerNorm(4, elementwise_affine=False)), Mine(4), FusedLayerNorm(4))
+    state = {k: v.clone() for k, v in model.state_dict().items()}
+    params = [id(p) for p in model.parameters()]
+    assert asdl_amd.fuse_layer_norms(model) == 2 and asdl_amd.fuse_layer_norms(model) == 0
+    assert [type(m) for m in (model[0], model[2][0], model[3])] == [FusedLayerNorm, FusedLayerNorm, Mine]
+    assert params == [id(p) for p in model.parameters()] and all(torch.equal(state[k], v) for k, v in model.state_dict().items())
+
+
+# ------------------------------------------------------------------------------------------------ hooks, with stand-ins for the kernels
+def _layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
+    m = x.mean(-1, keepdim=True)
+    r = ((x - m).square().mean(-1, keepdim=True) + eps).rsqrt()
+    h = (x - m) * r
+    y = h if weight is None else h * weight
+    return (y if bias is None else y + bias), m.squeeze(-1), r.squeeze(-1)
+
+
+class _Backward:
+    """layer_norm_backward() by its formula; counts who asks for what."""
+
+    def __init__(self):
+        self.fused = self.alone = 0
+
+    def __call__(self, g, x, mean, rstd, weight=None, blocks=None, alpha=1.0, beta=0.0, need_x=True, need_weight=True, need_bias=True, weight_dtype=None):
+        h = (x - mean.unsqueeze(-1)) * rstd.unsqueeze(-1)
+        gw = g if weight is None else g * weight
+        dx = rstd.unsqueeze(-1) * (gw - gw.mean(-1, keepdim=True) - h * (gw * h).mean(-1, keepdim=True))
+        g2, h2 = g.reshape(-1, g.shape[-1]), h.reshape(-1, h.shape[-1])
+        if blocks is not None:
+            self.fused, self.alone = self.fused + bool(need_x), self.alone + (not need_x)
+            a, b = g2 * h2, g2
+            new = torch.stack([(a * a).sum(0), (a * b).sum(0), (a * b).sum(0), (b * b).sum(0)], -1).view(-1, 2, 2)
+            blocks.copy_(alpha * new if beta == 0 else beta * blocks + alpha * new)
+        return dx if need_x else None, (g2 * h2).sum(0) if need_weight else None, g2.sum(0) if need_bias else None
+
+
+class _Net(nn.Module):
+    """Layer norms in front (its input needs no gradient), in the middle, and over two dimensions."""
+
+    def __init__(self):
+        super().__init__()
+        self.first, self.a, self.middle = nn.LayerNorm(6), nn.Linear(6, 6), nn.LayerNorm(6)
+        self.square, self.b = nn.LayerNorm((2, 3)), nn.Linear(6, 4)
+
+    def forward(self, x):
+        x = self.middle(self.a(self.first(x)).tanh())
+        return self.b(self.square(x.view(-1, 2, 3)).flatten(1))
+
+
+@pytest.mark.parametrize('ema', [-1, 0.3])
+@pytest.mark.parametrize('fisher_type', [FISHER_EMP, FISHER_MC, FISHER_EXACT])
+def test_blocks_of_fused_layer_norms_are_those_of_plain_ones(fisher_type, ema, monkeypatch):
+    cpu_backend.install(monkeypatch)
+    backward = _Backward()
+    monkeypatch.setattr(kernels, 'layer_norm', _layer_norm)
+    monkeypatch.setattr(kernels, 'layer_norm_backward', backward)
+    torch.manual_seed(1)
+    plain = _Net()
+    for m in plain.modules():
+        if isinstance(m, nn.LayerNorm):
+            nn.init.normal_(m.weight, 1.0, 0.1)
+            nn.init.normal_(m.bias, 0.0, 0.1)
+    fused = copy.deepcopy(plain)
+    assert asdl_amd.fuse_layer_norms(fused) == 3
+    x, t = torch.randn(5, 6), torch.randint(4, (5,))
+    makers = []
+    for model in (plain, fused):
+        maker = KfacGradientMaker(model, PreconditioningConfig(data_size=5, damping=1e-2, ema_decay=ema), fisher_type=fisher_type, seed=3)
+        for _ in range(3):
+            model.zero_grad()
+            maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), t)
+            maker.forward_and_backward()
+        makers.append(maker)
+    # float32 blocks of up to 50 with a damping of 1e-2: their inverses, and what is multiplied by them, magnify the 2^-24 of some ten
+    # roundings by up to 5000
+    def off(a, b):
+        return float((a - b).norm() / b.norm())
+    for (name, p), q in zip(plain.named_parameters(), fused.parameters()):
+        assert off(q.grad, p.grad) < 5000 * 10 * 2.0 ** -24, name
+    for m, n in zip(plain.modules(), fused.modules()):
+        if isinstance(m, nn.LayerNorm):
+            a, b = m.fisher.unit, n.fisher.unit
+            assert off(b.inv, a.inv) < 5000 * 10 * 2.0 ** -24
+            assert (a.data is None) == (b.data is None) and (a.data is None or off(b.data, a.data) < 64 * 2.0 ** -24)
+    # the first layer's backward pass does not run where only the edges to the hooked outputs are differentiated
+    assert backward.fused > 0 and (fisher_type == FISHER_EMP or backward.alone > 0)
+
+
+def test_a_layer_norm_called_twice_adds_the_blocks_of_both_calls(monkeypatch):
+    """Each from its own input.  (Of torch.nn.LayerNorm, as in the reference, the output of the last call stands for all.)"""
+    cpu_backend.install(monkeypatch)
+    monkeypatch.setattr(kernels, 'layer_norm', _layer_norm)
+    monkeypatch.setattr(kernels, 'layer_norm_backward', _Backward())
+    from asdl_amd import OP_COV_UNIT_WISE, OP_COV_UNIT_WISE_INV, extend
+    ln = FusedLayerNorm(4)
+    x = torch.randn(7, 4, requires_grad=True)
+    want = 0
+    y1 = ln(x)
+    y2 = ln(y1.sin())
+    y1.retain_grad()
+    y2.retain_grad()
+    (y2 ** 3).sum().backward()
+    for inp, g in ((x, y1.grad), (y1.sin(), y2.grad)):
+        h = _layer_norm(inp.detach())[0]
+        a, b = g * h, g
+        want = want + torch.stack([(a * a).sum(0), (a * b).sum(0), (a * b).sum(0), (b * b).sum(0)], -1).view(-1, 2, 2)
+    for op, key in ((OP_COV_UNIT_WISE, 'data'), (OP_COV_UNIT_WISE_INV, 'inv')):
+        with extend(ln, op) as cxt:
+            cxt.set_damping(1.0)
+            (ln(ln(x).sin()) ** 3).sum().backward()
+            cxt.flush_inverses()
+            got = cxt.get_result(ln, OP_COV_UNIT_WISE, key)
+        expect = want if key == 'data' else torch.inverse(want + torch.eye(2))
+        assert torch.allclose(got, expect, rtol=1e-3, atol=1e-5), key
+
+
+def test_a_gradient_that_another_hook_replaces_does_not_reach_the_blocks(monkeypatch):
+    cpu_backend.install(monkeypatch)
+    backward = _Backward()
+    monkeypatch.setattr(kernels, 'layer_norm', _layer_norm)
+    monkeypatch.setattr(kernels, 'layer_norm_backward', backward)
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    ln = FusedLayerNorm(4)
+    pre = nn.Linear(4, 4)
+    x = torch.randn(7, 4)
+    with extend(ln, OP_COV_UNIT_WISE) as cxt:
+        y = ln(pre(x))
+        y.register_hook(lambda g: 2 * g)
+        (y ** 2).sum().backward()
+        got = cxt.get_result(ln, OP_COV_UNIT_WISE, 'data')
+    assert backward.alone == 1 and backward.fused == 0
+    h, g = _layer_norm(pre(x).detach())[0], 2 * y.detach()
+    assert torch.allclose(got[:, 1, 1], (g * g).sum(0)) and torch.allclose(got[:, 0, 0], (g * h * g * h).sum(0), rtol=1e-4)
+
+
+@pytest.mark.parametrize('maker_class', [KfacGradientMaker, ShampooGradientMaker])
+def test_makers_clip_what_the_step_leaves(maker_class, monkeypatch):
+    calls = []
+
+    def clip(grads, max_norm, norm_type=2.0, outs=None):
+        calls.append((len(grads), max_norm, norm_type))
+        norm = torch.stack([g.norm() for g in grads]).norm()
+        for g in grads:
+            g.mul_(min(1.0, max_norm / (float(norm) + 1e-6)))
+        return norm
+    cpu_backend.install(monkeypatch)
+    monkeypatch.setattr(kernels, 'clip_grad_norm', clip)
+    if maker_class is ShampooGradientMaker:
+        pytest.importorskip('torch')
+        monkeypatch.setattr(ShampooGradientMaker, '__init__', lambda self, model, config: asdl_amd.PreconditionedGradientMaker.__init__(self, model, config))
+        for stage in ('update_curvature', 'update_preconditioner', 'precondition'):
+            monkeypatch.setattr(ShampooGradientMaker, stage, lambda self: None)
+    torch.manual_seed(0)
+    model = nn.Sequential(nn.Linear(5, 6), nn.Tanh(), nn.Linear(6, 4))
+    x, t = torch.randn(8, 5), torch.randint(4, (8,))
+    got = {}
+    for most in (None, 1e-3, 1e6):
+        kwargs = dict(fisher_type=FISHER_EMP) if maker_class is KfacGradientMaker else {}
+        maker = maker_class(model, PreconditioningConfig(data_size=8, damping=1e-2, max_grad_norm=most), **kwargs)
+        model.zero_grad()
+        maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), t)
+        maker.forward_and_backward()
+        got[most] = [p.grad.clone() for p in model.parameters()]
+        assert (maker.grad_norm is None) == (most is None)
+    norm = float(torch.stack([g.norm() for g in got[None]]).norm())
+    assert calls == [(4, 1e-3, 2.0), (4, 1e6, 2.0)] and norm > 1e-3
+    for a, b, c in zip(got[None], got[1e-3], got[1e6]):
+        assert torch.equal(a, c) and torch.allclose(b, a * (1e-3 / norm), rtol=1e-4)
+
+
+def test_clip_grad_norm_of_parameters_without_gradients():
+    p = nn.Parameter(torch.ones(3))
+    assert float(asdl_amd.clip_grad_norm_([p], 1.0)) == 0 and float(asdl_amd.clip_grad_norm_(p, 1.0)) == 0
+    p.grad = torch.ones(3)
+    with pytest.raises(ValueError, match='max_norm'):
+        asdl_amd.clip_grad_norm_([p], -1.0)
+    with pytest.raises(RuntimeError, match='ROCm device'):
+        asdl_amd.clip_grad_norm_([p], 1.0)

@@ -1,0 +1,282 @@
+"""The operators as a training step uses them, together: layer norm under autograd and autocast, Fisher blocks from its backward pass,
+targets drawn from a filtered distribution, and the gradients that the step leaves scaled to a largest norm."""
+import copy
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+import asdl_amd
+from asdl_amd import (FISHER_EMP, FISHER_MC, FusedLayerNorm, KfacGradientMaker, PreconditioningConfig, ShampooGradientMaker, kernels)
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def off(got, want):
+    want = want.double()
+    return float((got.detach().double() - want).norm() / want.norm().clamp_min(1e-300))
+
+
+def rand(*shape, seed, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, device='cuda', generator=torch.Generator('cuda').manual_seed(seed)) * scale).to(dtype)
+
+
+@pytest.mark.parametrize('shape,normalized', [((40, 96), (96,)), ((3, 7, 130), (130,)), ((5, 4, 6, 8), (6, 8)), ((2, 3, 1021), 1021)])
+@pytest.mark.parametrize('affine', ['both', 'weight', 'none'])
+def test_gradients_of_layer_norm(shape, normalized, affine):
+    """Against the gradients of the definition in 64 bits, and its differences along one direction: (f(x + h v) - f(x - h v)) / 2h in
+    64 bits is off by h^2 f''' / 6 + 2^-53 f / h, below 1e-8 of the derivative at h = 1e-4 with values of about 1."""
+    size = (normalized,) if isinstance(normalized, int) else normalized
+    x = rand(*shape, seed=1).requires_grad_()
+    w = (1 + rand(*size, seed=2, scale=0.2)).requires_grad_() if affine != 'none' else None
+    b = rand(*size, seed=3).requires_grad_() if affine == 'both' else None
+    g = rand(*shape, seed=4)
+    given = [t for t in (x, w, b) if t is not None]
+    y = asdl_amd.layer_norm(x, normalized, w, b)
+    got = torch.autograd.grad(y, given, g)
+    doubles = [t.detach().double().requires_grad_() for t in given]
+
+    def f(*args):
+        args = list(args)
+        return F.layer_norm(args[0], size, args[1] if w is not None else None, args[2] if b is not None else None)
+    want = torch.autograd.grad(f(*doubles), doubles, g.double())
+    assert off(y, f(*doubles).detach()) < 64 * U
+    for a, c in zip(got, want):
+        assert a.shape == c.shape and off(a, c) < 128 * U       # (sums over up to 40 rows of mixed sign: some three times their size)
+    for i in range(len(doubles)):
+        v = rand(*doubles[i].shape, seed=5).double()
+        ends = [(f(*[d + s * 1e-4 * v if j == i else d for j, d in enumerate(doubles)]).detach() * g.double()).sum() for s in (1, -1)]
+        slope = float((ends[0] - ends[1]) / 2e-4)
+        size_of = float(got[i].double().norm() * v.norm())
+        assert abs(float((got[i].double() * v).sum()) - slope) < (128 * U + 1e-6) * size_of
+
+
+@pytest.mark.parametrize('wt', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('xt', [torch.float32, torch.bfloat16])
+def test_layer_norm_under_autocast(xt, wt):
+    x, w, b = rand(30, 256, seed=1, dtype=xt), (1 + rand(256, seed=2, scale=0.1)).to(wt), rand(256, seed=3).to(wt)
+    x.requires_grad_()
+    w.requires_grad_()
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        y, plain = asdl_amd.layer_norm(x, 256, w, b), F.layer_norm(x, (256,), w, b)
+    assert y.dtype == plain.dtype == torch.float32
+    assert off(y, F.layer_norm(x.detach().double(), (256,), w.detach().double(), b.double())) < 64 * U
+    dx, dw = torch.autograd.grad(y.square().sum(), (x, w))
+    assert dx.dtype == xt and dw.dtype == wt
+    if xt == wt or wt == torch.float32:
+        assert asdl_amd.layer_norm(x, 256, w, b).dtype == xt
+    else:
+        with pytest.raises(TypeError):
+            asdl_amd.layer_norm(x, 256, w, b)
+
+
+def test_layer_norm_is_differentiable_once_and_only_where_asked():
+    x, w = rand(6, 32, seed=1).requires_grad_(), rand(32, seed=2)
+    y = asdl_amd.layer_norm(x, 32, w)
+    (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        dx.sum().backward()
+    with torch.no_grad():
+        assert not asdl_amd.layer_norm(x, 32, w).requires_grad
+    assert torch.equal(asdl_amd.layer_norm(x.detach(), 32, w), y.detach())
+
+
+class Decoder(nn.Module):
+    def __init__(self, d=64, heads=4, layers=2, vocab=211, context=32):
+        super().__init__()
+        self.wte, self.heads = nn.Embedding(vocab, d), heads
+        self.layers = nn.ModuleList()
+        for _ in range(layers):
+            self.layers.append(nn.ModuleList([nn.LayerNorm(d), nn.Linear(d, 3 * d), nn.Linear(d, d), nn.LayerNorm(d), nn.Linear(d, 4 * d), nn.Linear(4 * d, d)]))
+        self.ln, self.head = nn.LayerNorm(d), nn.Linear(d, vocab, bias=False)
+        self.wte.weight.requires_grad_(False)
+
+    def forward(self, idx):
+        x = self.wte(idx)
+        for ln1, qkv, proj, ln2, up, down in self.layers:
+            b, t, d = x.shape
+            q, k, v = (z.view(b, t, self.heads, -1).transpose(1, 2) for z in qkv(ln1(x)).split(d, 2))
+            x = x + proj(F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2).reshape(b, t, d))
+            x = x + down(F.gelu(up(ln2(x))))
+        return self.head(self.ln(x)).flatten(0, 1)
+
+
+def decoders():
+    torch.manual_seed(1)
+    plain = Decoder().cuda()
+    for m in plain.modules():
+        if isinstance(m, nn.LayerNorm):
+            nn.init.normal_(m.weight, 1.0, 0.2)
+            nn.init.normal_(m.bias, 0.0, 0.2)
+    fused = copy.deepcopy(plain)
+    assert asdl_amd.fuse_layer_norms(fused) == 5
+    return plain, fused
+
+
+@pytest.mark.parametrize('ema', [-1, 0.5])
+@pytest.mark.parametrize('fisher_type', [FISHER_EMP, FISHER_MC])
+def test_kfac_step_of_a_decoder_with_the_operators(fisher_type, ema):
+    """Two steps of the same decoder: with torch's layer norm, and with the operators (targets of the sampled Fisher at temperature 0,
+    which is the largest logit on either side; clipping by torch there).  float32 curvature with a damping of 1e-2 magnifies the
+    2^-24 of sums over 200 rows in another order by its condition of up to 1e4: 1e4 * 2^-24 * some 10 = 6e-3; 1e-2 is allowed."""
+    plain, fused = decoders()
+    gen = torch.Generator('cuda').manual_seed(2)
+    idx, t = torch.randint(0, 211, (8, 25), device='cuda', generator=gen), torch.randint(0, 211, (200,), device='cuda', generator=gen)
+    most = 0.25
+
+    def maker_of(model, **more):
+        config = PreconditioningConfig(data_size=200, damping=1e-2, ema_decay=ema, ignore_modules=[nn.Embedding, model.head], **more)
+        return KfacGradientMaker(model, config, fisher_type=fisher_type, mc_temperature=0.0 if fisher_type == FISHER_MC else 1.0)
+    norms = []
+    for model, more in ((plain, {}), (fused, dict(max_grad_norm=most))):
+        maker = maker_of(model, **more)
+        for _ in range(2):
+            model.zero_grad()
+            maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, idx), t)
+            maker.forward_and_backward()
+            if not more:
+                norm = torch.nn.utils.clip_grad_norm_(model.parameters(), most)
+        norms.append(float(maker.grad_norm if more else norm))
+    assert norms[0] > most and abs(norms[1] / norms[0] - 1) < 1e-2
+    for (name, p), q in zip(plain.named_parameters(), fused.parameters()):
+        if p.grad is not None:
+            assert off(q.grad, p.grad) < 1e-2, name
+    got = math.sqrt(sum(float(p.grad.double().square().sum()) for p in fused.parameters() if p.grad is not None))
+    assert abs(got - most) < 1e-5 * most
+    for m, n in zip(plain.modules(), fused.modules()):
+        if isinstance(m, nn.LayerNorm):
+            assert type(n) is FusedLayerNorm and off(n.fisher.unit.inv, m.fisher.unit.inv) < 1e-2
+
+
+def test_blocks_come_from_the_backward_pass(monkeypatch):
+    """Every layer norm's blocks but the first one's, whose backward pass is not part of the sampled pass, are by-products."""
+    _, fused = decoders()
+    calls = []
+    plain = kernels.layer_norm_backward
+
+    def counted(g, x, *args, **kwargs):
+        blocks = kwargs.get('blocks', args[3] if len(args) > 3 else None)
+        need_weight = kwargs.get('need_weight', args[7] if len(args) > 7 else True)
+        calls.append((blocks is not None, bool(need_weight)))
+        return plain(g, x, *args, **kwargs)
+    monkeypatch.setattr(kernels, 'layer_norm_backward', counted)
+    monkeypatch.setattr(kernels, 'unit_wise_stats', None)          # (nothing calls it)
+    idx = torch.randint(0, 211, (4, 20), device='cuda')
+    t = torch.randint(0, 211, (80,), device='cuda')
+    for fisher_type, first_alone in ((FISHER_MC, 1), (FISHER_EMP, 0)):
+        calls.clear()
+        maker = KfacGradientMaker(fused, PreconditioningConfig(data_size=80, damping=1e-2, ignore_modules=[nn.Embedding, fused.head]), fisher_type=fisher_type)
+        fused.zero_grad()
+        maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(fused, idx), t)
+        maker.forward_and_backward()
+        assert sum(b and w for b, w in calls) == 5 - first_alone and sum(b and not w for b, w in calls) == first_alone, calls
+
+
+@pytest.mark.parametrize('filters', [dict(mc_top_k=1), dict(mc_top_k=5), dict(mc_top_p=0.3, mc_temperature=0.7), dict(mc_min_p=0.9)])
+@pytest.mark.parametrize('samples', [1, 3])
+def test_sampled_fisher_draws_from_the_filtered_distribution(filters, samples, monkeypatch):
+    torch.manual_seed(0)
+    model = nn.Sequential(nn.Linear(20, 30), nn.Tanh(), nn.Linear(30, 12)).cuda()
+    x, t = rand(64, 20, seed=1), torch.zeros(64, dtype=torch.long, device='cuda')
+    drawn = []
+    plain = kernels.sample_filtered
+
+    def kept(logits, *args, **kwargs):
+        out = plain(logits, *args, **kwargs)
+        drawn.append((logits.detach().clone(), out[0] if isinstance(out, tuple) else out))
+        return out
+    monkeypatch.setattr(kernels, 'sample_filtered', kept)
+    maker = KfacGradientMaker(model, PreconditioningConfig(data_size=64, damping=1e-2), fisher_type=FISHER_MC, n_mc_samples=samples, seed=5, **filters)
+    maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), t)
+    maker.forward_and_backward()
+    assert len(drawn) == samples and all(p.grad is not None for p in model.parameters())
+    for logits, classes in drawn:
+        probs = torch.softmax(logits.double() / filters.get('mc_temperature', 1.0), -1)
+        order = torch.argsort(probs, dim=-1, descending=True, stable=True)
+        rank = torch.argsort(order, dim=-1).gather(1, classes[:, None]).squeeze(1)
+        if 'mc_top_k' in filters:
+            assert int(rank.max()) < filters['mc_top_k']
+        if 'mc_top_p' in filters:
+            before = probs.gather(1, order).cumsum(1).gather(1, (rank[:, None] - 1).clamp(min=0)).squeeze(1)
+            assert bool(((before < filters['mc_top_p']) | (rank == 0)).all())
+        if 'mc_min_p' in filters:
+            assert bool((probs.gather(1, classes[:, None]).squeeze(1) >= 0.9 * probs.amax(1) * (1 - 1e-6)).all())
+
+
+def test_sampled_fisher_refuses_logits_without_a_distribution():
+    model = nn.Sequential(nn.Linear(4, 6)).cuda()
+    x = rand(8, 4, seed=1)
+    x[3] = float('nan')
+    maker = KfacGradientMaker(model, PreconditioningConfig(data_size=8, damping=1e-2), fisher_type=FISHER_MC, mc_top_p=0.9)
+    maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), torch.zeros(8, dtype=torch.long, device='cuda'))
+    with pytest.raises(RuntimeError, match='probability tensor'):
+        maker.forward_and_backward()
+
+
+def test_shampoo_step_with_clipped_gradients():
+    torch.manual_seed(0)
+    model = nn.Sequential(nn.Linear(30, 40), FusedLayerNorm(40), nn.Linear(40, 10)).cuda()
+    x, t = rand(50, 30, seed=1), torch.randint(0, 10, (50,), device='cuda')
+    maker = ShampooGradientMaker(model, PreconditioningConfig(damping=1e-6, max_grad_norm=0.5))
+    maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), t)
+    maker.forward_and_backward()
+    got = math.sqrt(sum(float(p.grad.double().square().sum()) for p in model.parameters()))
+    before = float(maker.grad_norm)
+    assert abs(got - min(before, 0.5)) < 1e-5 * got
+
+
+@pytest.mark.parametrize('norm_type', [2.0, 1.0, math.inf])
+def test_clip_grad_norm_does_what_torch_does(norm_type):
+    """(torch adds float32 squares: a relative error of some sqrt(numel / blocks) roundings; 1e-5 is allowed.)"""
+    for dtype in (torch.float32, torch.bfloat16):
+        params = [nn.Parameter(rand(*s, seed=i, dtype=dtype)) for i, s in enumerate([(300, 40), (40,), (64, 3, 7, 7), (), (1000,)])]
+        params.append(nn.Parameter(torch.zeros(3, device='cuda')))          # has no gradient
+        for p, s in zip(params, range(5)):
+            p.grad = rand(*p.shape, seed=10 + s, dtype=dtype)
+        theirs = [nn.Parameter(p.detach().clone()) for p in params]
+        for a, b in zip(theirs, params):
+            a.grad = None if b.grad is None else b.grad.clone()
+        for most in (0.5, 1e9):
+            a = asdl_amd.clip_grad_norm_(params, most, norm_type)
+            b = torch.nn.utils.clip_grad_norm_(theirs, most, norm_type)
+            tol = 1e-5 if dtype == torch.float32 else 1e-2
+            assert abs(float(a) - float(b)) < tol * float(b)
+            for p, q in zip(params, theirs):
+                assert (p.grad is None) == (q.grad is None) and (p.grad is None or off(p.grad, q.grad) < tol)
+    params[1].grad[7] = float('inf')
+    before = [None if p.grad is None else p.grad.clone() for p in params]
+    with pytest.raises(RuntimeError, match='non-finite'):
+        asdl_amd.clip_grad_norm_(params, 1.0, norm_type, error_if_nonfinite=True)
+    assert all(p.grad is None or torch.equal(p.grad, g) for p, g in zip(params, before))
+    assert float(asdl_amd.clip_grad_norm_(params, math.inf, norm_type)) == math.inf and torch.equal(params[0].grad, before[0])
+
+
+def test_a_captured_forward_and_backward_pass():
+    """Captured on inputs that are no leaves of an eager graph; replayed several times with new values, against the eager pass."""
+    w, b = 1 + rand(96, seed=1, scale=0.2), rand(96, seed=2)
+    x, g = rand(500, 96, seed=3), rand(500, 96, seed=4)
+
+    def passes(x, w, b):
+        x, w, b = (t.detach().requires_grad_() for t in (x, w, b))
+        y = asdl_amd.layer_norm(x, 96, w, b)
+        return [y.detach(), *torch.autograd.grad(y, (x, w, b), g)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes(x, w, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = passes(x, w, b)
+    for turn in range(4):
+        x.mul_(1.5).add_(0.1)
+        g.mul_(0.5)
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, e) for o, e in zip(outs, passes(x, w, b))), turn
