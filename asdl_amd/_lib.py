@@ -142,6 +142,29 @@ def load():
     return lib
 
 
+HOST_PATH = os.path.join(_HERE, 'lib', 'asdl_amd_host_calls.so')
+_host = None
+
+
+def load_host():
+    """The module of csrc/host_calls.cpp, bound to the library (once)."""
+    global _host
+    if _host is not None:
+        return _host
+    lib = load()
+    if not os.path.exists(HOST_PATH):
+        raise RuntimeError(f'{HOST_PATH} is missing: build it with `python -m asdl_amd.build`.')
+    import importlib.util
+    spec = importlib.util.spec_from_file_location('asdl_amd_host_calls', HOST_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                  for name in ('ak_layer_norm', 'ak_layer_norm_backward', 'ak_layer_norm_backward_ws_bytes', 'ak_sample_filtered', 'ak_grad_norm',
+                               'ak_clip_grad_norm', 'ak_grad_norm_ws_bytes')))
+    _host = module
+    return module
+
+
 class KernelError(RuntimeError):
     pass
 

@@ -1,4 +1,4 @@
-"""Builds libasdl_amd.so (every HIP source under csrc/) for gfx950 with hipcc, in-tree."""
+"""Builds libasdl_amd.so (every HIP source under csrc/) for gfx950 with hipcc, and the module of host_calls.cpp with g++, in-tree."""
 import glob
 import os
 import subprocess
@@ -8,6 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB_DIR = os.path.join(HERE, 'lib')
 LIB_PATH = os.path.join(LIB_DIR, 'libasdl_amd.so')
+HOST_PATH = os.path.join(LIB_DIR, 'asdl_amd_host_calls.so')
 
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc',
@@ -21,13 +22,26 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, '*.hip')))
 
 
+def host_command():
+    import sysconfig
+    import torch
+    where = os.path.dirname(torch.__file__)
+    return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden',
+            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{where}/include', f'-I{where}/include/torch/csrc/api/include',
+            f'-I{sysconfig.get_paths()["include"]}', os.path.join(CSRC, 'host_calls.cpp'), '-o', HOST_PATH, f'-L{where}/lib', '-ltorch_python',
+            '-ltorch_cpu', '-ltorch', '-lc10']
+
+
 def build(verbose=True, jobs=8):
     """AK_TUNING_HOOKS=1 in the environment adds the ak_debug_set_* / ak_debug_force_* setters (tuning runs only)."""
     flags = FLAGS + (['-DAK_TUNING_HOOKS'] if os.environ.get('AK_TUNING_HOOKS') == '1' else [])
     os.makedirs(LIB_DIR, exist_ok=True)
     obj_dir = os.path.join(LIB_DIR, 'obj')
     os.makedirs(obj_dir, exist_ok=True)
-    procs = []
+    command = host_command()
+    if verbose:
+        print(' '.join(command), flush=True)
+    procs = [(command[-7], subprocess.Popen(command, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))]
     objs = []
     for src in sources():
         obj = os.path.join(obj_dir, os.path.basename(src)[:-4] + '.o')

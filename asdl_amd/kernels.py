@@ -1256,6 +1256,11 @@ def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min
     A row that holds NaN or +inf or nothing but -inf, or whose parameters or number are NaN, has no distribution: its class is -1 and,
     as sample_categorical() does, the call raises torch.multinomial's RuntimeError, which waits for the draw; ``late``: returns (classes,
     SampledLogits) instead, whose check() raises it; ``check=False``: the -1 is all.  (A stream capture has no check.)"""
+    host = None if check or late or u is None else _usual(logits)
+    if host is not None:
+        done = host.sample_filtered(logits, u, temperature, top_k, top_p, min_p, _raw_stream(logits.get_device()))
+        if done is not None:
+            return done if type(done) is not int else _lib.check(done, 'ak_sample_filtered')
     code = _ELEMENT_TYPES.get(logits.dtype)
     if code is None or not logits.is_cuda:
         _require_gpu(logits)
@@ -1326,6 +1331,17 @@ def _rows_of(t, F):
     return _contiguous(t.detach()), F
 
 
+_device_index = getattr(torch._C, '_cuda_getDevice', None)
+
+
+def _usual(t):
+    """The module that does the usual calls for tensors like ``t`` in one step, or None: ``t`` is on another device than the current
+    one or on none, or this thread's launches go to another stream than the current one."""
+    if not t.is_cuda or _raw_stream is None or t.get_device() != _device_index() or getattr(_override, 'handle', None) is not None:
+        return None
+    return _lib.load_host()
+
+
 def _norm_vector(v, F, x, what):
     """A weight or bias of a layer norm as F contiguous elements of the type of ``x`` or float32."""
     if v.numel() != F:
@@ -1355,6 +1371,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     rstd = (variance + eps)^(-1/2).  x: float32, bfloat16 or float16, any leading dimensions and row stride; weight and bias (each may
     be None): of the type of x or float32, both of one.  y has the type of x, or float32 with ``out_dtype=torch.float32``; mean and rstd
     (float32, one per row) are what layer_norm_backward() needs."""
+    host = _usual(x)
+    if host is not None and (out_dtype is None or out_dtype == torch.float32 or out_dtype == x.dtype):
+        done = host.layer_norm(x, weight, bias, float(eps), out_dtype == torch.float32, _raw_stream(x.get_device()))
+        if done is not None:
+            return done if type(done) is tuple else _lib.check(done, 'ak_layer_norm')
     x_code, F, rows = _norm_rows(x)
     if not eps >= 0:
         raise ValueError(f'eps has to be at least 0. Got {eps}.')
@@ -1391,6 +1412,12 @@ def layer_norm_backward(g, x, mean, rstd, weight=None, blocks=None, alpha=1.0, b
     that of the weight (without a weight: ``weight_dtype``, float32).  ``blocks`` (contiguous float32 [F, 2, 2]) receives the unit-wise
     Fisher blocks in the same pass, blocks <- beta*blocks + alpha * sum over rows of [[gw^2, gw*gb], [gw*gb, gb^2]] with gw = g h,
     gb = g: unit_wise_stats() of y and g, without its division by the weight."""
+    host = _usual(x)
+    if host is not None and (weight is not None or weight_dtype is None):
+        done = host.layer_norm_backward(g, x, mean, rstd, weight, blocks, float(alpha), float(beta),
+                                        (1 if need_x else 0) | (2 if need_weight else 0) | (4 if need_bias else 0), _raw_stream(x.get_device()))
+        if done is not None:
+            return done if type(done) is tuple else _lib.check(done, 'ak_layer_norm_backward')
     x_code, F, rows = _norm_rows(x)
     g_code = _ELEMENT_TYPES.get(g.dtype)
     if g.shape != x.shape:
@@ -1528,6 +1555,11 @@ def _norm_rows_of(grads, outs):
 
 
 def _launch_norm(grads, outs, norm_type, max_norm):
+    host = _usual(grads[0])
+    if host is not None:
+        norm = host.gradient_norm(grads, outs, _NORM_KINDS[norm_type], 0.0 if max_norm is None else float(max_norm), _raw_stream(grads[0].get_device()))
+        if norm is not None:
+            return norm if type(norm) is not int else _lib.check(norm, 'ak_grad_norm')
     lib = _lib.load()
     count, device = len(grads), grads[0].device
     sources, results, sizes, types, result_types, late, keep = _norm_rows_of(grads, outs)

@@ -271,3 +271,19 @@ def test_clip_grad_norm_of_parameters_without_gradients():
         asdl_amd.clip_grad_norm_([p], -1.0)
     with pytest.raises(RuntimeError, match='ROCm device'):
         asdl_amd.clip_grad_norm_([p], 1.0)
+
+
+def test_calls_in_one_step_leave_the_unusual_to_the_others():
+    """The module of host_calls.cpp says None to what it does not take, whatever it is."""
+    from asdl_amd import _lib
+    host = _lib.load_host()
+    x, w = torch.randn(4, 8), torch.ones(8)
+    assert host.layer_norm(x, w, None, 1e-5, False, 0) is None and host.layer_norm('x', w, None, 1e-5, False, 0) is None and host.layer_norm() is None
+    assert host.layer_norm_backward(x, x, w, w, None, None, 1.0, 0.0, 7, 0) is None and host.layer_norm_backward(1, 2) is None
+    assert host.sample_filtered(x, torch.rand(4), 1.0, None, None, None, 0) is None and host.sample_filtered(x, None, 1.0, None, None, None, 0) is None
+    assert host.gradient_norm([x], None, 0, 0.0, 0) is None and host.gradient_norm([], None, 0, 0.0, 0) is None and host.gradient_norm((x,), None, 0, 0.0, 0) is None
+    with pytest.raises(TypeError):
+        host.bind(1)
+    with pytest.raises(ValueError):
+        host.bind(0, 0, 0, 0, 0, 0, 0)
+    assert _lib.load_host() is host
