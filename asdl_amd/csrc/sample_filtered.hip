@@ -21,7 +21,7 @@ struct SfParams {
   const float* min_ps;
   int64_t* targets;
   int* invalid;
-  int64_t ld;
+  int64_t ld, first_row;
   double temperature, top_p, min_p;
   int64_t top_k;
   int classes, u_double, shift;
@@ -107,7 +107,7 @@ __device__ __forceinline__ u64 sf_border(double p, u64 all) {
 
 // The largest and smallest over a work group.
 struct SfRange {
-  float top, low, least;      // largest; smallest finite one; smallest of the lanes' largest ones
+  float top, low, least;      // largest; smallest; smallest of the threads' largest ones
 };
 template <int WAVES>
 __device__ __forceinline__ SfRange sf_range(SfRange r, SfRange* red) {
@@ -151,7 +151,7 @@ __device__ __forceinline__ void sf_scan(A own, A* red, A& before, A& total) {
   }
 }
 
-constexpr int kSfBins = 2048, kSfListed = 2048, kSfSteps = 64, kSfAhead = 4;
+constexpr int kSfBins = 2048, kSfListed = 2048, kSfSteps = 128;
 
 template <int CELLS>
 struct SfShared {
@@ -162,9 +162,10 @@ struct SfShared {
   double red_double[16];
   SfRange range[16];
   u64 above;
-  int where, until, listed, found;
+  int where, until, listed, gathered, found;
   uint32_t found_key, lowest, highest;
   int found_index;
+  u64 found_order;
 };
 
 __device__ __forceinline__ u64 sf_order(uint32_t key, int c) { return static_cast<u64>(key) << 32 | (0xffffffffu - static_cast<uint32_t>(c)); }
@@ -194,9 +195,9 @@ __device__ __forceinline__ void sf_sort(u64* order, int count) {
     }
 }
 
-// A row in vectors of E elements, step after step NT runs of U of them: run (step NT + thread) is one thread's; the last n % E classes
-// are a step of their own, one for each of the first threads.  U is 1 up to kSfSteps steps.  Every pass reads the row again, from the
-// caches but for the first one; kSfAhead steps are on their way.
+// A row in vectors of E elements, step after step 64 U neighbouring ones a wave; the last n % E classes are a step of their own, one for
+// each of the first threads.  U is 1 up to kSfSteps steps.  Every pass reads the row again, from the caches but for the first one;
+// the next step is on its way (with four on their way a draw of 8 rows takes 10% longer, one of 4096 as long).
 template <typename T, int NT>
 struct SfRow {
   static constexpr int E = 16 / sizeof(T);
@@ -213,30 +214,30 @@ struct SfRow {
   __device__ __forceinline__ void each(Fn&& fn, Done&& done) const {
     const int tid = static_cast<int>(threadIdx.x);
     if (run == E) {
-      Some<T, E> ahead[kSfAhead];
+      Some<T, E> next;
+      next.clear();
+      if (tid * E < whole) next.load(x + tid * E);
+      for (int v = 0; v < steps; ++v) {
+        const int at = (v * NT + tid) * E, later = at + NT * E;
+        float value[E];
 #pragma unroll
-      for (int i = 0; i < kSfAhead; ++i) {
-        ahead[i].clear();
-        if ((i * NT + tid) * E < whole) ahead[i].load(x + (i * NT + tid) * E);
-      }
-      for (int v = 0; v < steps; v += kSfAhead) {
-#pragma unroll
-        for (int i = 0; i < kSfAhead; ++i) {
-          const int at = ((v + i) * NT + tid) * E, later = at + kSfAhead * NT * E;
-          float value[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) value[e] = ahead[i].get(e);
-          if (later < whole) ahead[i].load(x + later);
-          if (at < whole) fn(value, at);
-          if (v + i < steps) done(v + i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int e = 0; e < E; ++e) value[e] = next.get(e);
+        if (later < whole) next.load(x + later);
+        if (at < whole) fn(value, at);
+        done(v);
       }
     } else {
+      const int64_t wave_first = (tid & ~63) * static_cast<int64_t>(run) + (tid & 63) * E;
       for (int v = 0; v < steps; ++v) {
-        const int64_t first = (static_cast<int64_t>(v) * NT + tid) * run;
-        for (int64_t at = first; at < first + run && at < whole; ++at) {
-          const float value[1] = {static_cast<float>(x[at])};
+        const int64_t first = v * static_cast<int64_t>(NT) * run + wave_first;
+        for (int j = 0; j < run / E; ++j) {
+          const int64_t at = first + j * 64 * E;
+          if (at >= whole) break;
+          Some<T, E> some;
+          some.load(x + at);
+          float value[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) value[e] = some.get(e);
           fn(value, static_cast<int>(at));
         }
         done(v);
@@ -274,7 +275,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   using Row = SfRow<T, NT>;
   __shared__ SfShared<CELLS> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.classes;
-  const int64_t row_index = blockIdx.x;
+  const int64_t row_index = p.first_row + blockIdx.x;
   const Row row(static_cast<const T*>(p.logits) + row_index * p.ld, n);
   const SfFilter filter(p, row_index);
 
@@ -323,6 +324,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   int border_index = -1;
   // (bit by bit: no branches)
   auto kept = [&](float v, int c) -> bool { return (v > border_value) | ((v == border_value) & (c <= border_index)); };
+  const float lightest = static_cast<float>(static_cast<double>(top) - 37. * filter.t);      // weights of classes below round to 0
   float scale = 0.f;
   auto place_of = [&](float v) { return (top - v) * scale; };       // 0 and up, does not fall for a smaller logit
   auto bin_of = [&](float v) { return static_cast<int>(__builtin_amdgcn_fmed3f(place_of(v), 0.f, static_cast<float>(kSfBins - 1))); };
@@ -376,21 +378,21 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     full = base + __popcll(mask) > kSfListed;
     if (want && !full) sh.order[base + __popcll(mask & ((1ull << lane) - 1))] = sf_order(sf_key(v), c);
   };
-  // Of the listed classes in order, fn(class of the list, its weight as worth(logit), the weight in front of it).
+  // Of `count` numbers, fn(number, its weight as worth(number), the weight in front of it).
   constexpr int PER = kSfListed / NT;
-  auto each_listed = [&](int count, auto&& worth, auto&& fn) {
+  auto each_of = [&](const u64* numbers, int count, auto&& worth, auto&& fn) {
     u64 w[PER], own = 0, before, total;
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
       const int j = tid * PER + q;
-      w[q] = j < count ? worth(j, sh.order[j]) : 0;
+      w[q] = j < count ? worth(numbers[j]) : 0;
       own += w[q];
     }
     sf_scan<WAVES>(own, sh.red, before, total);
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
       const int j = tid * PER + q;
-      if (j < count) fn(j, sh.order[j], w[q], before, total);
+      if (j < count) fn(numbers[j], w[q], before);
       before += w[q];
     }
   };
@@ -468,7 +470,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
       high = sh.highest;
       if (count <= kSfListed) {
         sf_sort<NT>(sh.order, count);
-        each_listed(count, [&](int, u64 o) { return worth(sf_value(sf_order_key(o))); }, [&](int, u64 o, u64 w, u64 before, u64) {
+        each_of(sh.order, count, [&](u64 o) { return worth(sf_value(sf_order_key(o))); }, [&](u64 o, u64 w, u64 before) {
           if (above + before < target && above + before + w >= target) {
             sh.found_key = sf_order_key(o);
             sh.found_index = sf_order_class(o);
@@ -515,26 +517,73 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     border_value = sf_value(sh.found_key);
     border_index = sh.found_index;
   };
-  // The draw among the listed classes, of which the first k are kept, and of them those with less than `border` (made from the weight
-  // of them all) in front.  They are put in order, and those that are kept in the order of their indices.
-  auto draw_listed = [&](int k, auto&& make_border) {
+  // The draw among the listed classes: of those in bin `bin` the first `need` are kept, and all in front of this bin.  Each of the
+  // three borders (top-k's, top-p's, the drawn class) is first a bin, of logits or of indices, and only its few classes are put in order.
+  auto draw_listed = [&](int bin, int need) {
     __syncthreads();
-    const int count = sh.listed < k ? sh.listed : k;
-    sf_sort<NT>(sh.order, sh.listed);
-    u64 keep[PER];
+    const int count = sh.listed;
+    u64 own[PER];                                   // 0: none, or not kept
 #pragma unroll
-    for (int q = 0; q < PER; ++q) keep[q] = 0;
-    each_listed(count, [&](int, u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](int j, u64 o, u64, u64 before, u64 total) {
-      keep[j % PER] = before < make_border(total) ? o << 32 | o >> 32 : 0;
-    });
-    __syncthreads();
+    for (int q = 0; q < PER; ++q) own[q] = q * NT + tid < count ? sh.order[q * NT + tid] : 0;
+    auto logit = [](u64 o) { return sf_value(sf_order_key(o)); };
+    // those wanted, as numbers in falling order in place of the bins
+    auto gather = [&](auto&& want, auto&& number) {
+      __syncthreads();
+      if (tid == 0) sh.gathered = 0;
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const bool in = own[q] != 0 && want(own[q]);
+        const u64 mask = __ballot(in);
+        if (mask == 0) continue;
+        int base = 0;
+        const int leader = __ffsll(mask) - 1;
+        if (lane == leader) base = atomicAdd(&sh.gathered, __popcll(mask));
+        base = __builtin_amdgcn_readlane(base, leader);
+        if (in) sh.bins[base + __popcll(mask & ((1ull << lane) - 1))] = number(own[q]);
+      }
+      __syncthreads();
+      const int found = sh.gathered;
+      sf_sort<NT>(sh.bins, found);
+      return found;
+    };
+    auto same = [](u64 o) { return o; };
+    auto keep_from = [&](u64 border) {
+#pragma unroll
+      for (int q = 0; q < PER; ++q) own[q] = own[q] >= border ? own[q] : 0;
+    };
+    gather([&](u64 o) { return bin_of(logit(o)) == bin; }, same);
+    keep_from(sh.bins[need - 1]);
+    if (filter.p < 1.) {
+      clear_bins();
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+        if (own[q] != 0) atomicAdd(sh.bins + bin_of(logit(own[q])), weight(logit(own[q])));
+      u64 target;
+      cross(sh.bins, [&](u64 all) { return sf_border(filter.p, all); }, target);
+      const int p_bin = sh.where;
+      const u64 above = sh.above;
+      const int found = gather([&](u64 o) { return bin_of(logit(o)) == p_bin; }, same);
+      each_of(sh.bins, found, [&](u64 o) { return weight(logit(o)); }, [&](u64 o, u64 w, u64 before) {
+        if (above + before < target && above + before + w >= target) sh.found_order = o;
+      });
+      __syncthreads();
+      keep_from(sh.found_order);
+    }
+    clear_bins();
+    const int bits = 32 - __clz(n - 1), part = bits > 11 ? bits - 11 : 0;
+    auto worth = [&](u64 o) { return drawn(weight.scaled(logit(o))); };
 #pragma unroll
     for (int q = 0; q < PER; ++q)
-      if (tid * PER + q < count) sh.order[tid * PER + q] = keep[q];
-    sf_sort<NT>(sh.order, count);
-    each_listed(count, [&](int, u64 o) { return o == 0 ? 0 : drawn(weight.scaled(sf_value(static_cast<uint32_t>(o)))); }, [&](int, u64 o, u64 w, u64 before, u64 all) {
-      const u64 target = sf_target(filter.u, all);
-      if (before <= target && before + w > target) p.targets[row_index] = sf_order_class(o >> 32);
+      if (own[q] != 0) atomicAdd(sh.bins + (sf_order_class(own[q]) >> part), worth(own[q]));
+    u64 target;                                     // (the sum exceeds one number: reaches the next)
+    cross(sh.bins, [&](u64 all) { return sf_target(filter.u, all) + 1; }, target);
+    const int drawn_part = sh.where;
+    const u64 above = sh.above;
+    auto turned = [](u64 o) { return o << 32 | o >> 32; };      // the index in front, the lowest first
+    const int found = gather([&](u64 o) { return sf_order_class(o) >> part == drawn_part; }, turned);
+    each_of(sh.bins, found, [&](u64 o) { return worth(turned(o)); }, [&](u64 o, u64 w, u64 before) {
+      if (above + before < target && above + before + w >= target) p.targets[row_index] = sf_order_class(turned(o));
     });
   };
 
@@ -546,8 +595,9 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   };
 
   if (filter.k > 0 && filter.k < n) {
-    // of as many classes as there are threads, the largest of each thread's, none is below the least of them
-    const float low = filter.k <= NT ? range.least : range.low;
+    // Of as many classes as there are threads, the largest of each thread's, none is below the least of them.  A class further down
+    // than 37 T has no weight, kept or not: masks of -inf or of the type's lowest value do not take the bins away from the others.
+    const float low = fmaxf(filter.k <= NT ? range.least : range.low, lightest);
     set_scale(low);
     clear_bins();
     uint32_t* counts = reinterpret_cast<uint32_t*>(sh.bins);
@@ -556,26 +606,26 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
         if (x >= low) atomicAdd(counts + bin_of(x), 1u);
     });
     u64 target;
-    cross(counts, [&](u64) { return static_cast<u64>(filter.k); }, target);
-    const int bin = sh.where;
-    if (sh.above + counts[bin] <= kSfListed) {
-      clear_list();
-      row.each([&](const auto& v, int at) {
-        int c = at;
-        for (const float x : v) {
-          list(x >= low && bin_of(x) <= bin, x, c);
-          ++c;
-        }
-      });
-      return draw_listed(static_cast<int>(filter.k), [&](u64 all) { return filter.p < 1. ? sf_border(filter.p, all) : ~0ull; });
+    if (cross(counts, [&](u64) { return static_cast<u64>(filter.k); }, target)) {        // (else all that have weight are kept)
+      const int bin = sh.where;
+      if (sh.above + counts[bin] <= kSfListed) {
+        clear_list();
+        row.each([&](const auto& v, int at) {
+          int c = at;
+          for (const float x : v) {
+            list(x >= low && bin_of(x) <= bin, x, c);
+            ++c;
+          }
+        });
+        return draw_listed(bin, static_cast<int>(target - sh.above));
+      }
+      narrow(target, [&](float v, int) { return v >= low; }, [](float) -> u64 { return 1; });
     }
-    narrow(target, [&](float v, int) { return v >= low; }, [](float) -> u64 { return 1; });
   }
   if (filter.p < 1.) {
     // Where the border will be, from 32-bit sums: a bin's weights fall from 1 to 2^-drop of that at its upper end, taken as a straight
     // line (off by 4e-5 at most).  Additions of fp32 numbers in the LDS take three times as long as all the rest of the pass.
-    // (Weights of classes further down than 37 T round to 0.)
-    set_scale(fmaxf(range.low, static_cast<float>(static_cast<double>(top) - 37. * filter.t)));
+    set_scale(fmaxf(range.low, lightest));
     clear_bins();
     uint32_t* sums = reinterpret_cast<uint32_t*>(sh.bins);
     const float drop = scale > 0.f ? static_cast<float>(weight.c / static_cast<double>(scale)) : 0.f;
@@ -651,7 +701,7 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     if (tid == 0) sh.found = 0;
     if (count <= kSfListed && above < target) {
       sf_sort<NT>(sh.order, count);
-      each_listed(count, [&](int, u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](int, u64 o, u64 w, u64 before, u64) {
+      each_of(sh.order, count, [&](u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](u64 o, u64 w, u64 before) {
         if (above + before >= target) return;
         const int c = sf_order_class(o);
         if (w != 0) atomicAdd(sh.cells + row.cell(c), w);
@@ -692,12 +742,20 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   draw_cells();
 }
 
+// Rows that fill the card take small groups, several on a CU, the others large ones; few classes do not fill those.
 template <typename T>
-static void sf_launch(const SfParams& p, int64_t rows, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(rows));
-  if (p.classes <= 2048) hipLaunchKernelGGL((sf_row_kernel<T, 256>), grid, dim3(256), 0, s, p);
-  else if (rows > 256) hipLaunchKernelGGL((sf_row_kernel<T, 512>), grid, dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((sf_row_kernel<T, 1024>), grid, dim3(1024), 0, s, p);
+static int sf_launch(SfParams p, int64_t rows, hipStream_t s) {
+  constexpr int64_t kMost = 1 << 22;                   // rows of a launch: the threads of one are counted in 32 bits
+  for (p.first_row = 0; p.first_row < rows; p.first_row += kMost) {
+    const dim3 grid(static_cast<unsigned>(rows - p.first_row < kMost ? rows - p.first_row : kMost));
+    const bool few = rows <= 256 || p.classes >= 512 * kSfSteps * SfRow<T, 512>::E;
+    if (p.classes <= (few ? 2048 : 8192)) hipLaunchKernelGGL((sf_row_kernel<T, 256>), grid, dim3(256), 0, s, p);
+    else if (!few || p.classes <= 8192) hipLaunchKernelGGL((sf_row_kernel<T, 512>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((sf_row_kernel<T, 1024>), grid, dim3(1024), 0, s, p);
+    const int rc = check_launch();
+    if (rc != AK_OK) return rc;
+  }
+  return AK_OK;
 }
 
 }  // namespace ak
@@ -710,15 +768,14 @@ extern "C" int ak_sample_filtered(const void* logits, int dtype, int64_t rows, i
   if (temperatures == nullptr && !(temperature >= 0.)) return AK_ERR_ARG;
   if (rows == 0) return AK_OK;
   if (logits == nullptr || u == nullptr || targets == nullptr) return AK_ERR_ARG;
-  if (classes > (1 << 30) || rows > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  if (classes > (1 << 30)) return AK_ERR_TOO_LARGE;
   int bits = 0;
   while ((1ll << bits) < classes) ++bits;
   const int shift = 62 - bits < 51 ? 62 - bits : 51;
-  const SfParams p{logits, u, temperatures, top_ks, top_ps, min_ps, targets, invalid, ld, temperature, top_p, min_p, top_k,
+  const SfParams p{logits, u, temperatures, top_ks, top_ps, min_ps, targets, invalid, ld, 0, temperature, top_p, min_p, top_k,
                    static_cast<int>(classes), u_is_double, shift, (1u << (bits < 32 ? 31 - bits : 0))};
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto type) {
-    sf_launch<typename decltype(type)::type>(p, rows, s);
-    return check_launch();
+    return sf_launch<typename decltype(type)::type>(p, rows, s);
   });
 }

@@ -591,3 +591,164 @@ def test_two_captured_graphs_replayed_side_by_side(K):
         for _, run, _, outs, _ in made:
             got = [o.clone() for o in outs]
             assert all(torch.equal(a, b) for a, b in zip(got, run())), turn
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('rows,n', [(300, 2500), (257, 9001)])
+def test_filtered_draws_of_many_rows(K, dtype, rows, n):
+    print(f'sample_filtered {rows}x{n} {dtype}', flush=True)
+    logits = rand(rows, n, seed=n, dtype=dtype, scale=2.5)
+    for i, filters in enumerate(FILTERS):
+        u = torch.rand(rows, device='cuda', dtype=torch.float64, generator=torch.Generator('cuda').manual_seed(i))
+        assert torch.equal(K.sample_filtered(logits, u, **filters).cpu(), draw64(logits, u, **filters)), filters
+
+
+@pytest.mark.parametrize('dtype,rows,n', [(F32, 2, 600001), (BF16, 1, 1100003), (F16, 2, 300007), (F32, 261, 140002)])
+def test_filtered_draws_of_long_rows(K, dtype, rows, n):
+    print(f'sample_filtered {rows}x{n} {dtype}', flush=True)
+    logits = rand(rows, n, seed=n, dtype=dtype, scale=2.5)
+    looked_at = slice(None, None, 52)
+    for i, filters in enumerate([dict(), dict(top_k=40), dict(top_k=30000, top_p=0.9), dict(top_p=0.7), dict(top_p=0.9999), dict(min_p=0.01), dict(temperature=0.0)]):
+        u = torch.rand(rows, device='cuda', dtype=torch.float64, generator=torch.Generator('cuda').manual_seed(i))
+        assert torch.equal(K.sample_filtered(logits, u, **filters)[looked_at].cpu(), draw64(logits[looked_at], u[looked_at], **filters)), filters
+
+
+@pytest.mark.parametrize('n', [5000, 60000])
+def test_filtered_draws_of_few_levels_and_of_clusters(K, n):
+    """Borders among thousands of equal classes, and among thousands whose logits differ in their last bits only."""
+    gen = torch.Generator('cuda').manual_seed(n)
+    rows = 6
+    levels = torch.randint(0, 4, (rows, n), device='cuda', generator=gen).float() * -0.75
+    levels[:, 17] = 0.5
+    cluster = -20 + torch.randn(rows, n, device='cuda', generator=gen) * 1e-4
+    cluster[:, n // 2] = 0
+    narrow = -20 + torch.randn(rows, n, device='cuda', generator=gen) * 1e-5
+    narrow[:, ::1000] -= 0.005
+    narrow[:, 3] = 0
+    u = torch.rand(rows, device='cuda', dtype=torch.float64, generator=gen)
+    for name, logits, t in (('levels', levels, 1.0), ('levels', levels.to(BF16), 0.9), ('cluster', cluster, 5.0), ('narrow', narrow, 4.0)):
+        for filters in (dict(top_p=0.3), dict(top_p=0.9), dict(top_p=0.9999), dict(top_k=2100), dict(top_k=n - 1), dict(top_k=3000, top_p=0.5),
+                        dict(top_k=n - n // 3, top_p=0.95), dict(top_p=0.8, min_p=0.2), dict(top_k=4000, top_p=0.97, min_p=0.01)):
+            got = K.sample_filtered(logits, u, temperature=t, **filters)
+            assert torch.equal(got.cpu(), draw64(logits, u, temperature=t, **filters)), (name, logits.dtype, filters)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('masked', ['infinite', 'lowest', 'large'])
+def test_filtered_draws_of_masked_rows(K, dtype, masked):
+    """Most classes masked, by -inf, the type's lowest value or -1e4: fewer classes than top_k are left in some rows."""
+    rows, n = 8, 20011
+    gen = torch.Generator('cuda').manual_seed(3)
+    logits = rand(rows, n, seed=1, dtype=dtype, scale=2.0)
+    left = torch.tensor([0.5, 0.1, 0.01, 0.001, 0.0005, 0.9, 0.0, 0.05], device='cuda').unsqueeze(1)
+    mask = torch.rand(rows, n, device='cuda', generator=gen) >= left
+    mask[:, 777] = False
+    logits[mask] = dict(infinite=-float('inf'), lowest=torch.finfo(dtype).min, large=-1e4)[masked]
+    u = torch.rand(rows, device='cuda', dtype=torch.float64, generator=gen)
+    for filters in (dict(top_k=4), dict(top_k=40), dict(top_k=1500), dict(top_k=5000), dict(top_k=40, top_p=0.9), dict(top_k=9000, top_p=0.99),
+                    dict(top_p=0.9), dict(top_k=30, min_p=0.1), dict(top_k=60, temperature=3.0), dict(top_k=60, temperature=1e-3)):
+        got = K.sample_filtered(logits, u, **filters)
+        assert torch.equal(got.cpu(), draw64(logits, u, **filters)), filters
+        assert int(got[6]) == 777
+
+
+def test_filtered_draws_of_infinite_temperature(K):
+    """All classes that are not masked are equally likely."""
+    logits, inf = rand(5, 4001, seed=1), float('inf')
+    logits[:, ::2] = -inf
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.9999], device='cuda', dtype=torch.float64)
+    want = [1, 1001, 2001, 3001, 3999]
+    assert K.sample_filtered(logits, u, temperature=inf).tolist() == want
+    assert K.sample_filtered(logits, u, temperature=inf, top_k=3999).tolist() == want
+    got = K.sample_filtered(logits, u, temperature=inf, top_k=4)
+    by_index = logits.topk(4).indices.sort(-1).values
+    assert got.tolist() == [int(by_index[i, min(3, int(4 * float(u[i])))]) for i in range(5)]
+
+
+def test_more_rows_than_a_launch_takes(K):
+    rows = (1 << 22) + 77
+    logits, u = rand(rows, 3, seed=1), torch.rand(rows, device='cuda', dtype=torch.float64, generator=torch.Generator('cuda').manual_seed(1))
+    w = (logits.double() - logits.double().amax(-1, keepdim=True)).exp()
+    want = (w.cumsum(-1)[:, :2] <= (u * w.sum(-1)).unsqueeze(-1)).sum(-1)
+    assert torch.equal(K.sample_filtered(logits, u), want)
+
+
+def test_draws_beyond_32_bits(K):
+    base = rand(8, 50257, seed=1, dtype=BF16, scale=2.0)
+    logits = base.repeat(5400, 1)
+    assert logits.numel() > 1 << 31
+    u = torch.rand(logits.shape[0], device='cuda', dtype=torch.float64, generator=torch.Generator('cuda').manual_seed(2))
+    for filters in (dict(), dict(top_k=50, top_p=0.9)):
+        got = K.sample_filtered(logits, u, **filters)
+        assert torch.equal(got[-24:].cpu(), draw64(logits[-24:], u[-24:], **filters))
+        assert torch.equal(got[-2400:], K.sample_filtered(base.repeat(300, 1), u[-2400:], **filters))
+    rows = torch.zeros(0, device='cuda', dtype=F16).new_empty((1 << 31) + 5000).as_strided((3, 5000), (1 << 30, 1))
+    rows.copy_(rand(3, 5000, seed=3, dtype=F16))
+    assert torch.equal(K.sample_filtered(rows, u[:3], top_p=0.7).cpu(), draw64(rows, u[:3], top_p=0.7))
+
+
+def test_layer_norm_beyond_32_bits(K):
+    """One block of rows again and again: each row's result is the block's, and sums over rows are its sums times the repetitions, up to
+    chains of at most rows / 512 + 512 additions, each off by u of the magnitudes' sum at most."""
+    F, block, times = 768, 4000, 700
+    x0, g0, w = rand(block, F, seed=1, dtype=BF16), rand(block, F, seed=2, dtype=BF16), rand(F, seed=3)
+    x, g = x0.repeat(times, 1), g0.repeat(times, 1)
+    assert x.numel() > 1 << 31
+    y, mean, rstd = K.layer_norm(x, w, None, 1e-5)
+    y0, mean0, rstd0 = K.layer_norm(x0, w, None, 1e-5)
+    assert torch.equal(y[-block:], y0) and torch.equal(y[:block], y0) and torch.equal(mean[-block:], mean0) and torch.equal(rstd[-block:], rstd0)
+    dx, dw, db = K.layer_norm_backward(g, x, mean, rstd, w)
+    dx0 = K.layer_norm_backward(g0, x0, mean0, rstd0, w)[0]
+    assert torch.equal(dx[-block:], dx0) and torch.equal(dx[block:2 * block], dx0)
+    h = (x0.double() - mean0.double().unsqueeze(-1)) * rstd0.double().unsqueeze(-1)
+    bound = (block * times / 512 + 512 + 64) * U
+    for got, terms in ((dw, g0.double() * h), (db, g0.double())):
+        assert bool(((got.double() - times * terms.sum(0)).abs() <= bound * times * terms.abs().sum(0)).all())
+
+
+def test_norms_beyond_32_bits(K):
+    n = (1 << 31) + 4099
+    big = torch.full((n,), 0.5, device='cuda', dtype=BF16)
+    small = torch.full((n % 1000, 3), 0.5, device='cuda')
+    total = 0.5 * math.sqrt(n + small.numel())
+    norm = K.clip_grad_norm([small, big], total / 4)
+    assert abs(float(norm) - total) <= 4 * U * total
+    want = 0.5 * (total / 4) / (float(norm) + 1e-6)
+    assert bool((big[-5000:] == torch.tensor(want, device='cuda').to(BF16)).all()) and bool((big[:5000] == big[-1]).all())
+    assert bool(((small.double() - want).abs() <= 4 * U * want).all())
+
+
+def test_two_threads_at_once(K):
+    """Two threads with a stream each call the operators at the same time: every call's result is that of the call alone."""
+    import threading
+
+    def inputs(seed):
+        return (rand(200, 768, seed=seed), rand(768, seed=seed + 1), rand(64, 5000, seed=seed + 2),
+                torch.rand(64, device='cuda', generator=torch.Generator('cuda').manual_seed(seed)), gradients([(300, 70), (4099,)] * 8, seed))
+
+    def run(x, w, logits, u, grads):
+        y, mean, rstd = K.layer_norm(x, w)
+        outs = [torch.empty_like(t) for t in grads]
+        return [y, *K.layer_norm_backward(y, x, mean, rstd, w), K.sample_filtered(logits, u, top_k=50), K.sample_filtered(logits, u, top_p=0.9, check=False),
+                K.clip_grad_norm(grads, 0.1, outs=outs), *outs]
+    made = [inputs(seed) for seed in (1, 50)]
+    want = [run(*m) for m in made]
+    torch.cuda.synchronize()
+    wrong, errors = [], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for turn in range(100):
+                    got = run(*made[i])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        wrong.append((i, turn))
+        except Exception as e:
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and not wrong
