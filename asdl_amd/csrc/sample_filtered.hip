@@ -25,7 +25,7 @@ struct SfParams {
   double temperature, top_p, min_p;
   int64_t top_k;
   int classes, u_double, shift;
-  uint32_t unit;          // so large that one for every class fits 32 bits
+  float unit;             // a weight of 1 in sums of 32 bits over all classes; at most 2^22, so that its whole part stays in a float
 };
 
 __device__ __forceinline__ uint32_t sf_key(float x) {
@@ -200,7 +200,7 @@ __device__ __forceinline__ void sf_sort(u64* order, int count) {
 // the next step is on its way (with four on their way a draw of 8 rows takes 10% longer, one of 4096 as long).
 template <typename T, int NT>
 struct SfRow {
-  static constexpr int E = 16 / sizeof(T);
+  static constexpr int E = 16 / sizeof(T), AHEAD = sizeof(T) == 4 ? 2 : 1;
   const T* __restrict__ x;
   int whole, rest, run, steps;         // run: U E classes
   __device__ __forceinline__ SfRow(const T* __restrict__ x_, int n) : x(x_), whole(n / E * E), rest(n % E) {
@@ -214,17 +214,24 @@ struct SfRow {
   __device__ __forceinline__ void each(Fn&& fn, Done&& done) const {
     const int tid = static_cast<int>(threadIdx.x);
     if (run == E) {
-      Some<T, E> next;
-      next.clear();
-      if (tid * E < whole) next.load(x + tid * E);
-      for (int v = 0; v < steps; ++v) {
-        const int at = (v * NT + tid) * E, later = at + NT * E;
-        float value[E];
+      Some<T, E> ahead[AHEAD];
 #pragma unroll
-        for (int e = 0; e < E; ++e) value[e] = next.get(e);
-        if (later < whole) next.load(x + later);
-        if (at < whole) fn(value, at);
-        done(v);
+      for (int i = 0; i < AHEAD; ++i) {
+        ahead[i].clear();
+        if ((i * NT + tid) * E < whole) ahead[i].load(x + (i * NT + tid) * E);
+      }
+      for (int v = 0; v < steps; v += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const int at = ((v + i) * NT + tid) * E, later = at + AHEAD * NT * E;
+          float value[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) value[e] = ahead[i].get(e);
+          if (later < whole) ahead[i].load(x + later);
+          if (at < whole) fn(value, at);
+          if (v + i < steps) done(v + i);
+          if constexpr (AHEAD > 1) __builtin_amdgcn_sched_barrier(0);
+        }
       }
     } else {
       const int64_t wave_first = (tid & ~63) * static_cast<int64_t>(run) + (tid & 63) * E;
@@ -270,7 +277,7 @@ struct SfRow {
 // in the LDS and ranked there by counting, and the draw is among them.  Otherwise the border is narrowed to a key and an index, and one
 // more pass sums the kept weight of every cell (a step of a wave).
 template <typename T, int NT>
-static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
+static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
   constexpr int WAVES = NT / 64, CELLS = (kSfSteps + 1) * WAVES;
   using Row = SfRow<T, NT>;
   __shared__ SfShared<CELLS> sh;
@@ -279,16 +286,52 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   const Row row(static_cast<const T*>(p.logits) + row_index * p.ld, n);
   const SfFilter filter(p, row_index);
 
+  // Bins of logits: number round(x a) - round(top a), a < 0, that is 0 for the largest and more for smaller ones.
+  float a = 0.f, base = 0.f;
+  auto bin_at = [&](float v) { return rintf(v * a) - base; };
+  auto bin_of = [&](float v) { return static_cast<int>(__builtin_amdgcn_fmed3f(bin_at(v), 0.f, static_cast<float>(kSfBins - 1))); };
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(sh.bins);
+  auto clear_bins = [&] {
+    __syncthreads();
+    for (int b = tid; b < kSfBins; b += NT) sh.bins[b] = 0;
+    __syncthreads();
+  };
+
+  // The range; for top-k in the same pass, before the top is known, the counts of bins that are T / 32 wide (or 1 / 64), whose numbers are
+  // taken modulo 2048.  They serve if the row's finite logits span no more than these 64 T.  (4096 rows of 50257 classes, top-k 40: 279 us
+  // for 356 with a pass of their own; for top-p, whose sums are dearer and whose bins hold more classes to put in order, nothing is won.)
+  const bool by_k = filter.k > 0 && filter.k < n;
+  bool early = by_k && filter.good() && !filter.greedy();
+  if (early) {
+    a = static_cast<float>(-32. / (filter.t < 0.5 ? 0.5 : filter.t));
+    early = a < -1e-30f;
+  }
   SfRange range{-INFINITY, INFINITY, 0.f};
   bool bad = !filter.good();
-  row.each([&](const auto& v, int) {
+  if (early) {
+    clear_bins();
+    row.each([&](const auto& v, int) {
 #pragma unroll
-    for (const float x : v) {
-      bad = bad || !(x < INFINITY);
-      range.top = fmaxf(range.top, x);
-      range.low = fminf(range.low, x);
-    }
-  });
+      for (const float x : v) {
+        bad = bad || !(x < INFINITY);
+        range.top = fmaxf(range.top, x);
+        if (x > -INFINITY) {
+          range.low = fminf(range.low, x);
+          // (the sum with 1.5 2^23 holds the integer in its low bits)
+          atomicAdd(counts + (__builtin_bit_cast(uint32_t, rintf(x * a) + 12582912.f) & (kSfBins - 1)), 1u);
+        }
+      }
+    });
+  } else {
+    row.each([&](const auto& v, int) {
+#pragma unroll
+      for (const float x : v) {
+        bad = bad || !(x < INFINITY);
+        range.top = fmaxf(range.top, x);
+        range.low = fminf(range.low, x);
+      }
+    });
+  }
   range.least = range.top;
   bad = __syncthreads_or(bad) != 0;
   range = sf_range<WAVES>(range, sh.range);
@@ -325,17 +368,17 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   // (bit by bit: no branches)
   auto kept = [&](float v, int c) -> bool { return (v > border_value) | ((v == border_value) & (c <= border_index)); };
   const float lightest = static_cast<float>(static_cast<double>(top) - 37. * filter.t);      // weights of classes below round to 0
-  float scale = 0.f;
-  auto place_of = [&](float v) { return (top - v) * scale; };       // 0 and up, does not fall for a smaller logit
-  auto bin_of = [&](float v) { return static_cast<int>(__builtin_amdgcn_fmed3f(place_of(v), 0.f, static_cast<float>(kSfBins - 1))); };
-  auto set_scale = [&](float low) {
-    const float s = static_cast<float>(kSfBins - 1) / (top - low);
-    scale = top > low && s < INFINITY ? s : 0.f;
-  };
-  auto clear_bins = [&] {
-    __syncthreads();
-    for (int b = tid; b < kSfBins; b += NT) sh.bins[b] = 0;
-    __syncthreads();
+  int start = 0;                     // the place of bin 0
+  if (early) {
+    early = fabsf(top * a) < 4e6f && fabsf(range.low * a) < 4e6f && rintf(range.low * a) - rintf(top * a) < static_cast<float>(kSfBins);
+    base = rintf(top * a);
+    start = static_cast<int>(early ? base : 0.f) & (kSfBins - 1);
+  }
+  auto set_bins = [&](float low) {
+    const float s = static_cast<float>(kSfBins - 2) / (top - low);
+    a = top > low && s < INFINITY ? -s : 0.f;
+    base = rintf(top * a);
+    start = 0;
   };
   // The first bin at which the sum reaches `target` (made from the sum of all): its number and the sum in front of it in `sh`.
   // False if none does.
@@ -344,12 +387,12 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     __syncthreads();
     u64 own = 0, before, total;
 #pragma unroll
-    for (int b = 0; b < PER; ++b) own += bins[tid * PER + b];
+    for (int b = 0; b < PER; ++b) own += bins[(start + tid * PER + b) & (kSfBins - 1)];
     sf_scan<WAVES>(own, sh.red, before, total);
     target = make_target(total);
     if (before < target && before + own >= target) {
       int b = tid * PER;
-      for (; before + bins[b] < target; ++b) before += bins[b];
+      for (; before + bins[(start + b) & (kSfBins - 1)] < target; ++b) before += bins[(start + b) & (kSfBins - 1)];
       sh.where = b;
       sh.above = before;
     }
@@ -367,16 +410,27 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     }
     __syncthreads();
   };
-  // Lists the class of every lane that wants it; one addition to the counter a wave, and none once the list is full.
-  auto list = [&](bool want, float v, int c) {
-    const u64 mask = __ballot(want && !full);
-    if (mask == 0) return;
+  // Lists the wanted of neighbouring classes; one addition to the counter a wave, and none once the list is full.
+  auto list = [&](const auto& want, const auto& v, int at) {
+    constexpr int N = sizeof(v) / sizeof(float);
+    u64 mask[N];
+    int count = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      mask[e] = __ballot(want[e] && !full);
+      count += __popcll(mask[e]);
+    }
+    if (count == 0) return;
     int base = 0;
-    const int leader = __ffsll(mask) - 1;
-    if (lane == leader) base = atomicAdd(&sh.listed, __popcll(mask));
-    base = __builtin_amdgcn_readlane(base, leader);
-    full = base + __popcll(mask) > kSfListed;
-    if (want && !full) sh.order[base + __popcll(mask & ((1ull << lane) - 1))] = sf_order(sf_key(v), c);
+    if (lane == __ffsll(__ballot(true)) - 1) base = atomicAdd(&sh.listed, count);
+    base = __builtin_amdgcn_readfirstlane(base);
+    full = base + count > kSfListed;
+    if (full) return;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (want[e]) sh.order[base + __popcll(mask[e] & ((1ull << lane) - 1))] = sf_order(sf_key(v[e]), at + e);
+      base += __popcll(mask[e]);
+    }
   };
   // Of `count` numbers, fn(number, its weight as worth(number), the weight in front of it).
   constexpr int PER = kSfListed / NT;
@@ -450,15 +504,16 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
       uint32_t least_key = 0xffffffffu, most_key = 0;
       clear_list();
       row.each([&](const auto& v, int at) {
-        int c = at;
-        for (const float x : v) {
-          const uint32_t kk = sf_key(x);
-          const bool want = kk >= low && kk <= high && bin_of(x) == bin && in(x, c);
-          list(want, x, c);
-          least_key = want && kk < least_key ? kk : least_key;
-          most_key = want && kk > most_key ? kk : most_key;
-          ++c;
+        constexpr int N = sizeof(v) / sizeof(float);
+        bool want[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const uint32_t kk = sf_key(v[e]);
+          want[e] = kk >= low && kk <= high && bin_of(v[e]) == bin && in(v[e], at + e);
+          least_key = want[e] && kk < least_key ? kk : least_key;
+          most_key = want[e] && kk > most_key ? kk : most_key;
         }
+        list(want, v, at);
       });
       if (most_key >= least_key) {
         atomicMin(&sh.lowest, least_key);
@@ -517,11 +572,51 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     border_value = sf_value(sh.found_key);
     border_index = sh.found_index;
   };
+  // The draw among up to 64 listed classes by one wave, one class a lane: lanes change places, by counting how many are in front of each,
+  // to the order of the filters and then to that of the indices.
+  auto draw_of_wave = [&](int count) {
+    auto moved = [&](u64 v, int to) {
+      const uint32_t low = __builtin_amdgcn_ds_permute(to * 4, static_cast<int>(v)), high = __builtin_amdgcn_ds_permute(to * 4, static_cast<int>(v >> 32));
+      return static_cast<u64>(high) << 32 | low;
+    };
+    auto of_lane = [](u64 v, int j) {
+      const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(v), j), high = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), j);
+      return static_cast<u64>(high) << 32 | low;
+    };
+    auto upto = [&](u64 w) {
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const u64 lower = __shfl_up(w, o);
+        if (lane >= o) w += lower;
+      }
+      return w;
+    };
+    const u64 listed = lane < count ? sh.order[lane] : 0;
+    int rank = lane < count ? 0 : lane;
+    for (int j = 0; j < count; ++j) rank += (of_lane(listed, j) > listed) & (lane < count) ? 1 : 0;
+    const u64 o = moved(listed, rank);
+    const double w = weight.scaled(sf_value(sf_order_key(o)));
+    bool keep = (lane < filter.k) & (lane < count);
+    if (filter.p < 1.) {
+      const u64 own = keep ? SfWeight::whole(w) : 0, sum = upto(own), border = sf_border(filter.p, of_lane(sum, 63));
+      keep = keep & (sum - own < border);
+    }
+    const int c = lane < count ? sf_order_class(o) : 0x40000000 + lane;
+    rank = 0;
+    for (int j = 0; j < 64; ++j) rank += __builtin_amdgcn_readlane(c, j) < c ? 1 : 0;
+    const u64 own = moved(keep ? drawn(w) : 0, rank), sum = upto(own), target = sf_target(filter.u, of_lane(sum, 63));
+    const int by_index = __builtin_amdgcn_ds_permute(rank * 4, c);
+    if (sum - own <= target && sum > target) p.targets[row_index] = by_index;
+  };
   // The draw among the listed classes: of those in bin `bin` the first `need` are kept, and all in front of this bin.  Each of the
   // three borders (top-k's, top-p's, the drawn class) is first a bin, of logits or of indices, and only its few classes are put in order.
   auto draw_listed = [&](int bin, int need) {
     __syncthreads();
     const int count = sh.listed;
+    if (count <= 64) {
+      if (wave == 0) draw_of_wave(count);
+      return;
+    }
     u64 own[PER];                                   // 0: none, or not kept
 #pragma unroll
     for (int q = 0; q < PER; ++q) own[q] = q * NT + tid < count ? sh.order[q * NT + tid] : 0;
@@ -594,48 +689,60 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     class_of(target, value, [&](int c) { p.targets[row_index] = c; });
   };
 
-  if (filter.k > 0 && filter.k < n) {
-    // Of as many classes as there are threads, the largest of each thread's, none is below the least of them.  A class further down
-    // than 37 T has no weight, kept or not: masks of -inf or of the type's lowest value do not take the bins away from the others.
-    const float low = fmaxf(filter.k <= NT ? range.least : range.low, lightest);
-    set_scale(low);
-    clear_bins();
-    uint32_t* counts = reinterpret_cast<uint32_t*>(sh.bins);
-    row.each([&](const auto& v, int) {
-      for (const float x : v)
-        if (x >= low) atomicAdd(counts + bin_of(x), 1u);
-    });
-    u64 target;
-    if (cross(counts, [&](u64) { return static_cast<u64>(filter.k); }, target)) {        // (else all that have weight are kept)
+  if (by_k) {
+    float low = range.low;
+    for (bool counted = early;; counted = false) {
+      if (!counted) {
+        // Of as many classes as there are threads, the largest of each thread's, none is below the least of them.  A class further down
+        // than 37 T has no weight, kept or not: masks of -inf or of the type's lowest value do not take the bins away from the others.
+        low = fmaxf(filter.k <= NT ? range.least : range.low, lightest);
+        set_bins(low);
+        clear_bins();
+        row.each([&](const auto& v, int) {
+          for (const float x : v)
+            if (x >= low) atomicAdd(counts + bin_of(x), 1u);
+        });
+      }
+      u64 target;
+      if (!cross(counts, [&](u64) { return static_cast<u64>(filter.k); }, target)) break;        // all that have weight are kept
       const int bin = sh.where;
-      if (sh.above + counts[bin] <= kSfListed) {
+      const u64 above = sh.above;
+      if (above + counts[(start + bin) & (kSfBins - 1)] <= kSfListed) {
+        start = 0;
         clear_list();
         row.each([&](const auto& v, int at) {
-          int c = at;
-          for (const float x : v) {
-            list(x >= low && bin_of(x) <= bin, x, c);
-            ++c;
-          }
+          constexpr int N = sizeof(v) / sizeof(float);
+          bool want[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) want[e] = v[e] >= low && bin_of(v[e]) <= bin;
+          list(want, v, at);
         });
-        return draw_listed(bin, static_cast<int>(target - sh.above));
+        return draw_listed(bin, static_cast<int>(target - above));
       }
+      if (counted) continue;
       narrow(target, [&](float v, int) { return v >= low; }, [](float) -> u64 { return 1; });
+      break;
     }
   }
   if (filter.p < 1.) {
-    // Where the border will be, from 32-bit sums: a bin's weights fall from 1 to 2^-drop of that at its upper end, taken as a straight
-    // line (off by 4e-5 at most).  Additions of fp32 numbers in the LDS take three times as long as all the rest of the pass.
-    set_scale(fmaxf(range.low, lightest));
+    // Where the border will be, from 32-bit sums: a weight in its bin, of unit 1 in the middle, is taken as a straight line over the bin
+    // (a chord of 2^-drop, off by 4e-5 at most).  (Additions of fp32 numbers in the LDS take three times as long as all the rest of the
+    // pass.)
+    set_bins(fmaxf(range.low, lightest));
     clear_bins();
-    uint32_t* sums = reinterpret_cast<uint32_t*>(sh.bins);
-    const float drop = scale > 0.f ? static_cast<float>(weight.c / static_cast<double>(scale)) : 0.f;
-    const float unit = static_cast<float>(p.unit), slope = unit * (exp2f(-drop) - 1.f);
+    uint32_t* const sums = counts;
+    const float drop = a < 0.f ? static_cast<float>(filter.exponent() / -static_cast<double>(a)) : 0.f;
+    const float up = exp2f(0.5f * drop), down = exp2f(-0.5f * drop);
+    const float middle = 0.5f * (up + down) * p.unit + 8388608.f, slope = (down - up) * p.unit;      // (2^23: as above)
+    auto share = [&](float v) {
+      const float u = v * a;
+      return __builtin_bit_cast(uint32_t, __builtin_fmaf(u - rintf(u), slope, middle)) - 0x4b000000u;
+    };
     auto add_sums = [&](auto all) {        // all: every class is kept (of -inf, in the last bin, nothing is taken)
       row.each([&](const auto& v, int at) {
         int c = at;
         for (const float x : v) {
-          const uint32_t w = static_cast<uint32_t>(__builtin_fmaf(__builtin_amdgcn_fractf(place_of(x)), slope, unit));
-          if (decltype(all)::value ? x > -INFINITY : kept(x, c)) atomicAdd(sums + bin_of(x), w);
+          if (decltype(all)::value ? x > -INFINITY : kept(x, c)) atomicAdd(sums + bin_of(x), share(x));
           ++c;
         }
       });
@@ -667,27 +774,24 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
     }
     // One pass with exact weights: of the bins in front of the border's (and of a neighbour, where the border is near its edge), by
     // cells; of all others; the classes of these bins.
-    const float from_place = sh.where > 0 ? static_cast<float>(sh.where) : -INFINITY, to_place = sh.until < kSfBins - 1 ? static_cast<float>(sh.until + 1) : INFINITY;
+    const float from_bin = sh.where > 0 ? static_cast<float>(sh.where) : -INFINITY, to_bin = sh.until < kSfBins - 1 ? static_cast<float>(sh.until) : INFINITY;
     u64 own_all = 0, own_above = 0;
     auto add_weights = [&](auto every) {
       row.each(
           [&](const auto& v, int at) {
             constexpr int N = sizeof(v) / sizeof(float);
-            bool want[N], any = false;
+            bool want[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-              const float place = place_of(v[e]);
+              const float bin = bin_at(v[e]);
               const bool in = decltype(every)::value ? true : kept(v[e], at + e);
               const u64 w = in ? weight(v[e]) : 0;
-              const bool front = place < from_place;
+              const bool front = bin < from_bin;
               sum += front ? w : 0;
               own_all += w;
-              want[e] = in & !front & (place < to_place);
-              any |= want[e];
+              want[e] = in & !front & (bin <= to_bin);
             }
-            if (__ballot(any) != 0)
-#pragma unroll
-              for (int e = 0; e < N; ++e) list(want[e], v[e], at + e);
+            list(want, v, at);
           },
           [&](int step) {
             own_above += sum;
@@ -742,15 +846,20 @@ static __global__ __launch_bounds__(NT) void sf_row_kernel(SfParams p) {
   draw_cells();
 }
 
-// Rows that fill the card take small groups, several on a CU, the others large ones; few classes do not fill those.
+// A group's threads: few where the rows are many, since the waves of small groups, four groups on a CU, wait for each other less
+// (4096 rows of 50257 bfloat16 classes, top-k 40: 190 us with 256 threads, 225 with 512), many where they do not fill the card (256 such
+// rows: 45, 33 and 33 us with 256, 512 and 1024; top-p 0.9 of 128 fp32 rows: 69, 49 and 46), not many for few classes (256 rows of 5000: 18
+// us with 512 and 20 with 1024; of 1000: 18.7 with 256 and 19.7 with 1024), and enough for kSfSteps steps (512 rows of 250000: 265 us in
+// steps, 754 in longer runs).
 template <typename T>
 static int sf_launch(SfParams p, int64_t rows, hipStream_t s) {
+  int threads = p.classes <= 2048 || rows >= 1024 ? 256 : p.classes <= 8192 || rows > 256 ? 512 : 1024;
+  while (threads < 1024 && p.classes >= threads * kSfSteps * SfRow<T, 512>::E) threads *= 2;
   constexpr int64_t kMost = 1 << 22;                   // rows of a launch: the threads of one are counted in 32 bits
   for (p.first_row = 0; p.first_row < rows; p.first_row += kMost) {
     const dim3 grid(static_cast<unsigned>(rows - p.first_row < kMost ? rows - p.first_row : kMost));
-    const bool few = rows <= 256 || p.classes >= 512 * kSfSteps * SfRow<T, 512>::E;
-    if (p.classes <= (few ? 2048 : 8192)) hipLaunchKernelGGL((sf_row_kernel<T, 256>), grid, dim3(256), 0, s, p);
-    else if (!few || p.classes <= 8192) hipLaunchKernelGGL((sf_row_kernel<T, 512>), grid, dim3(512), 0, s, p);
+    if (threads == 256) hipLaunchKernelGGL((sf_row_kernel<T, 256>), grid, dim3(256), 0, s, p);
+    else if (threads == 512) hipLaunchKernelGGL((sf_row_kernel<T, 512>), grid, dim3(512), 0, s, p);
     else hipLaunchKernelGGL((sf_row_kernel<T, 1024>), grid, dim3(1024), 0, s, p);
     const int rc = check_launch();
     if (rc != AK_OK) return rc;
@@ -773,7 +882,7 @@ extern "C" int ak_sample_filtered(const void* logits, int dtype, int64_t rows, i
   while ((1ll << bits) < classes) ++bits;
   const int shift = 62 - bits < 51 ? 62 - bits : 51;
   const SfParams p{logits, u, temperatures, top_ks, top_ps, min_ps, targets, invalid, ld, 0, temperature, top_p, min_p, top_k,
-                   static_cast<int>(classes), u_is_double, shift, (1u << (bits < 32 ? 31 - bits : 0))};
+                   static_cast<int>(classes), u_is_double, shift, static_cast<float>(1u << (bits > 9 ? 31 - bits : 22))};
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto type) {
     return sf_launch<typename decltype(type)::type>(p, rows, s);
