@@ -3,10 +3,16 @@
 // Sums are double: no square of an fp32 value overflows or vanishes there, and 2^53 of them lose nothing that a float holds.  Every
 // launch has its tensors' addresses in the kernel arguments: nothing is uploaded, so a captured graph needs no memory of the host.
 // Partial sums are added in a fixed order by every work group that needs the norm; no atomics.
+// Bound by the memory: the norm reads all elements once, clipping reads them again and writes them.  1.26 GB of fp32 gradients: 209 us the
+// norm (6.0 TB/s, part of it from the 256 MB cache), 690 us with clipped copies (5.5 TB/s for two reads and a write: the second read is not
+// to be had for less where the gradients do not fit the cache); 105 MB: 21 and 52 us; a few small tensors: 9 us, two launches.
 #include "elements.hpp"
 
 namespace ak {
 
+// Measured for 1.26 GB / 105 MB / 2.7 MB, norm and clipped copies: 209, 690 / 20.8, 52.5 / 9.3, 9.4 us.  One load ahead: 221, 706 / 23.5, 54.8 /
+// 10.7, 12.9; eight: 206, 695 / 21.6, 52.4 / 11.4, 11.2.  Chunks of 4096: 211, 688 / 21.8, 53.2 / 10.5, 12.4; of 65536: 209, 700 / 20.9, 50.9 /
+// 10.2, 14.5.  2048 work groups: 213, 694 / 23.1, 53.0 / 10.3, 11.1.
 constexpr int kGnThreads = 256;
 constexpr int kGnBlocks = 1024;            // work groups of all norm launches of a call: so many partial sums
 constexpr int64_t kGnChunk = 16384;        // elements
@@ -130,7 +136,7 @@ static __global__ __launch_bounds__(kGnThreads) void gn_clip_kernel(GnClipTable 
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
   const double most = max_norm / (n + 1e-6);
   const float c = static_cast<float>(most > 1. ? 1. : most);           // (NaN stays)
-  // (from the end, which the pass before has read last)
+  // (from the end, which the pass before has read last and the caches may hold: 690 us for 696 from the start)
   for (int chunk = t.chunks - 1 - static_cast<int>(blockIdx.x); chunk >= 0; chunk -= gridDim.x) {
     const int i = gn_find(t, chunk);
     if (c == 1.f && t.src[i] == t.dst[i]) continue;

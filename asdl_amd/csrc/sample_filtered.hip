@@ -151,6 +151,7 @@ __device__ __forceinline__ void sf_scan(A own, A* red, A& before, A& total) {
   }
 }
 
+// (up to kSfSteps steps of a group a wave's loads are one after the other; sums are kept for every step of every wave)
 constexpr int kSfBins = 2048, kSfListed = 2048, kSfSteps = 128;
 
 template <int CELLS>
@@ -197,7 +198,8 @@ __device__ __forceinline__ void sf_sort(u64* order, int count) {
 
 // A row in vectors of E elements, step after step 64 U neighbouring ones a wave; the last n % E classes are a step of their own, one for
 // each of the first threads.  U is 1 up to kSfSteps steps.  Every pass reads the row again, from the caches but for the first one;
-// the next step is on its way (with four on their way a draw of 8 rows takes 10% longer, one of 4096 as long).
+// the next step is on its way, of fp32 the next two.  (With four of bfloat16 a draw of 8 rows takes 10% longer and one of 4096 as long; fp32,
+// 4096 rows, top-p 0.9: 488 us with one, 458 with two, 451 with four, which cost 256 rows 55 us for 53.)
 template <typename T, int NT>
 struct SfRow {
   static constexpr int E = 16 / sizeof(T), AHEAD = sizeof(T) == 4 ? 2 : 1;
@@ -272,10 +274,16 @@ struct SfRow {
   }
 };
 
-// One work group per row, in a few passes over it: the range; with top-k the counts of 2048 bins between its ends, which say in what bin
-// the border lies; with top-p the fp32 weights of such bins.  Where the classes up to the border's bin are at most kSfListed, they are listed
-// in the LDS and ranked there by counting, and the draw is among them.  Otherwise the border is narrowed to a key and an index, and one
-// more pass sums the kept weight of every cell (a step of a wave).
+// One work group per row, in passes over it: the range, with top-k along with the counts of 2048 bins of logits, which say in what bin the
+// border lies.  Where the classes up to this bin are at most kSfListed, the next pass lists them in the LDS, and the draw is among them.
+// With top-p alone a pass adds the classes' weights to bins, about, and says where the border will be, and one with exact weights sums
+// those in front of it by cells (a step of a wave), lists those about it and finds it among them; the draw is in the cell at which the
+// sums pass the number.  Without either that pass sums all.  Where a list does not hold the classes of a border's bin (thousands of equal
+// or nearly equal ones), the border is narrowed by bins of their keys to a class.
+// What bounds it: 4096 rows of 50257 fp32 classes (823 MB; 161 us to read them once at the rate of a large copy) take 245 us with T = 0 and
+// 281 with top-k 40 (two reads, 5.9 TB/s), 354 without filters and 461 with top-p 0.9, of which 80% are vector instructions, 66 a class, most
+// of them for the exact weights.  8 rows take 10 us with T = 0, 22 with top-k 40 and 42 with top-p 0.9: one CU a row and the barriers
+// between the passes.
 template <typename T, int NT>
 static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
   constexpr int WAVES = NT / 64, CELLS = (kSfSteps + 1) * WAVES;
@@ -877,7 +885,7 @@ extern "C" int ak_sample_filtered(const void* logits, int dtype, int64_t rows, i
   if (temperatures == nullptr && !(temperature >= 0.)) return AK_ERR_ARG;
   if (rows == 0) return AK_OK;
   if (logits == nullptr || u == nullptr || targets == nullptr) return AK_ERR_ARG;
-  if (classes > (1 << 30)) return AK_ERR_TOO_LARGE;
+  if (classes > (1 << 30) || rows > 0x7fffffff) return AK_ERR_TOO_LARGE;
   int bits = 0;
   while ((1ll << bits) < classes) ++bits;
   const int shift = 62 - bits < 51 ? 62 - bits : 51;
