@@ -379,13 +379,12 @@ template <int I>
 struct LnInt {
   static constexpr int value = I;
 };
-template <typename Fn>
-static bool ln_layout(int64_t F, bool forward, Fn&& fn) {
+template <bool FORWARD, typename Fn>
+static bool ln_layout(int64_t F, Fn&& fn) {
   if (F <= 128) fn(LnInt<16>{}, LnInt<8>{});
   else if (F <= 512) fn(LnInt<64>{}, LnInt<8>{});
   else if (F <= 1024) fn(LnInt<64>{}, LnInt<16>{});
-  else if (F <= 2048 && forward) fn(LnInt<64>{}, LnInt<32>{});
-  else if (F <= 2048) fn(LnInt<256>{}, LnInt<8>{});
+  else if (F <= 2048) fn(LnInt<(FORWARD ? 64 : 256)>{}, LnInt<(FORWARD ? 32 : 8)>{});
   else if (F <= 4096) fn(LnInt<256>{}, LnInt<16>{});
   else if (F <= 8192) fn(LnInt<512>{}, LnInt<16>{});
   else return false;
@@ -402,7 +401,7 @@ constexpr int kLnMostChunks = 512;
 // the five sums of the blocks (with 512: 34.9 us both ways at 8192 x 768, with 256 30.3).
 static int64_t ln_backward_blocks(int64_t rows, int64_t F, bool blocks) {
   int groups = 0;
-  if (!ln_layout(F, false, [&](auto lanes, auto) { groups = 512 / decltype(lanes)::value; })) {
+  if (!ln_layout<false>(F, [&](auto lanes, auto) { groups = 512 / decltype(lanes)::value; })) {
     const int64_t per = (rows + kLnMostChunks - 1) / kLnMostChunks;          // chunks of 16 rows at least
     return (rows + (per < 16 ? 16 : per) - 1) / (per < 16 ? 16 : per);
   }
@@ -428,7 +427,7 @@ extern "C" int ak_layer_norm(const void* x, int x_dtype, int64_t ldx, const void
     auto launch = [&](auto yt, auto wt) {
       using Y = typename decltype(yt)::type;
       using W = typename decltype(wt)::type;
-      const bool held = ln_layout(F, true, [&](auto lanes, auto elements) {
+      const bool held = ln_layout<true>(F, [&](auto lanes, auto elements) {
         constexpr int L = decltype(lanes)::value, V = decltype(elements)::value * static_cast<int>(sizeof(X)) / 16;
         constexpr int threads = L > 256 ? L : 256;
         const int64_t need = (rows + threads / L - 1) / (threads / L);
@@ -473,7 +472,7 @@ extern "C" int ak_layer_norm_backward(const void* g, int g_dtype, int64_t ldg, c
         using G = typename decltype(gt)::type;
         using W = typename decltype(wt)::type;
         const dim3 grid(static_cast<unsigned>(chunks));
-        const bool held = ln_layout(F, false, [&](auto lanes, auto elements) {
+        const bool held = ln_layout<false>(F, [&](auto lanes, auto elements) {
           constexpr int L = decltype(lanes)::value, V = decltype(elements)::value * static_cast<int>(sizeof(X)) / 16;
           if (sums == 5) hipLaunchKernelGGL((ln_backward_fused_kernel<X, G, W, L, V, 512, 5>), grid, dim3(512), 0, s, p);
           else if (sums == 2) hipLaunchKernelGGL((ln_backward_fused_kernel<X, G, W, L, V, 512, 2>), grid, dim3(512), 0, s, p);

@@ -144,7 +144,7 @@ __device__ __forceinline__ void sf_scan(A own, A* red, A& before, A& total) {
   __syncthreads();
   before = upto - own;
   total = 0;
-#pragma unroll
+#pragma unroll 4              // (all 16 at once take registers that the passes need)
   for (int w = 0; w < WAVES; ++w) {
     if (w < wave) before += red[w];
     total += red[w];
@@ -440,22 +440,19 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
       base += __popcll(mask[e]);
     }
   };
-  // Of `count` numbers, fn(number, its weight as worth(number), the weight in front of it).
-  constexpr int PER = kSfListed / NT;
+  // Of `count` numbers, fn(number, its weight as worth(number), the weight in front of it).  (Weights are made twice: kept they take
+  // registers that the passes need.)
   auto each_of = [&](const u64* numbers, int count, auto&& worth, auto&& fn) {
-    u64 w[PER], own = 0, before, total;
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int j = tid * PER + q;
-      w[q] = j < count ? worth(numbers[j]) : 0;
-      own += w[q];
-    }
+    const int per = (count + NT - 1) / NT, from = tid * per, to = from + per < count ? from + per : count;
+    u64 own = 0, before, total;
+#pragma unroll 1
+    for (int j = from; j < to; ++j) own += worth(numbers[j]);
     sf_scan<WAVES>(own, sh.red, before, total);
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int j = tid * PER + q;
-      if (j < count) fn(numbers[j], w[q], before);
-      before += w[q];
+#pragma unroll 1
+    for (int j = from; j < to; ++j) {
+      const u64 w = worth(numbers[j]);
+      fn(numbers[j], w, before);
+      before += w;
     }
   };
   // The class of index order at which the sums of the cells exceed `target`: its cell in sh.where, the sum in front in sh.above.
@@ -625,25 +622,29 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
       if (wave == 0) draw_of_wave(count);
       return;
     }
-    u64 own[PER];                                   // 0: none, or not kept
-#pragma unroll
-    for (int q = 0; q < PER; ++q) own[q] = q * NT + tid < count ? sh.order[q * NT + tid] : 0;
+    const int rounds = (count + NT - 1) / NT;
+    uint32_t own = 0;                               // bit by bit: a class of this thread is kept
+    for (int q = 0; q < rounds; ++q) own |= q * NT + tid < count ? 1u << q : 0;
+    auto each_own = [&](auto&& fn) {
+      for (int q = 0; q < rounds; ++q)
+        if ((own >> q & 1) != 0) fn(q, sh.order[q * NT + tid]);
+    };
     auto logit = [](u64 o) { return sf_value(sf_order_key(o)); };
     // those wanted, as numbers in falling order in place of the bins
     auto gather = [&](auto&& want, auto&& number) {
       __syncthreads();
       if (tid == 0) sh.gathered = 0;
       __syncthreads();
-#pragma unroll
-      for (int q = 0; q < PER; ++q) {
-        const bool in = own[q] != 0 && want(own[q]);
+      for (int q = 0; q < rounds; ++q) {
+        const u64 o = sh.order[q * NT + tid];
+        const bool in = (own >> q & 1) != 0 && want(o);
         const u64 mask = __ballot(in);
         if (mask == 0) continue;
         int base = 0;
         const int leader = __ffsll(mask) - 1;
         if (lane == leader) base = atomicAdd(&sh.gathered, __popcll(mask));
         base = __builtin_amdgcn_readlane(base, leader);
-        if (in) sh.bins[base + __popcll(mask & ((1ull << lane) - 1))] = number(own[q]);
+        if (in) sh.bins[base + __popcll(mask & ((1ull << lane) - 1))] = number(o);
       }
       __syncthreads();
       const int found = sh.gathered;
@@ -652,16 +653,13 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
     };
     auto same = [](u64 o) { return o; };
     auto keep_from = [&](u64 border) {
-#pragma unroll
-      for (int q = 0; q < PER; ++q) own[q] = own[q] >= border ? own[q] : 0;
+      each_own([&](int q, u64 o) { own &= o >= border ? ~0u : ~(1u << q); });
     };
     gather([&](u64 o) { return bin_of(logit(o)) == bin; }, same);
     keep_from(sh.bins[need - 1]);
     if (filter.p < 1.) {
       clear_bins();
-#pragma unroll
-      for (int q = 0; q < PER; ++q)
-        if (own[q] != 0) atomicAdd(sh.bins + bin_of(logit(own[q])), weight(logit(own[q])));
+      each_own([&](int, u64 o) { atomicAdd(sh.bins + bin_of(logit(o)), weight(logit(o))); });
       u64 target;
       cross(sh.bins, [&](u64 all) { return sf_border(filter.p, all); }, target);
       const int p_bin = sh.where;
@@ -676,9 +674,7 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
     clear_bins();
     const int bits = 32 - __clz(n - 1), part = bits > 11 ? bits - 11 : 0;
     auto worth = [&](u64 o) { return drawn(weight.scaled(logit(o))); };
-#pragma unroll
-    for (int q = 0; q < PER; ++q)
-      if (own[q] != 0) atomicAdd(sh.bins + (sf_order_class(own[q]) >> part), worth(own[q]));
+    each_own([&](int, u64 o) { atomicAdd(sh.bins + (sf_order_class(o) >> part), worth(o)); });
     u64 target;                                     // (the sum exceeds one number: reaches the next)
     cross(sh.bins, [&](u64 all) { return sf_target(filter.u, all) + 1; }, target);
     const int drawn_part = sh.where;
