@@ -752,3 +752,19 @@ def test_two_threads_at_once(K):
     for t in threads:
         t.join()
     assert not errors and not wrong
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('n', [900, 30011])
+def test_filtered_draws_where_min_p_and_top_p_are_close(K, dtype, n):
+    """min-p from far below top-p's border to far above it, the share of its classes on both sides of top_p."""
+    rows = 12
+    logits = rand(rows, n, seed=n, dtype=dtype, scale=2.0)
+    u = torch.rand(rows, device='cuda', dtype=torch.float64, generator=torch.Generator('cuda').manual_seed(7))
+    w = torch.softmax(logits.double(), -1)
+    for min_p in (0.002, 0.05, 0.3, 1.0):
+        share = float((w * (w >= min_p * w.amax(-1, keepdim=True))).sum(-1).mean())
+        for top_p in (share - 0.05, share - 1e-3, share, share + 5e-4, share + 2e-3, share + 0.05):
+            filters = dict(top_p=min(max(top_p, 1e-3), 0.9999), min_p=min_p)
+            for t in (1.0, 0.3):
+                assert torch.equal(K.sample_filtered(logits, u, temperature=t, **filters).cpu(), draw64(logits, u, temperature=t, **filters)), (filters, t)
