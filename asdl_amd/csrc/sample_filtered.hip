@@ -280,8 +280,8 @@ struct SfRow {
 // those in front of it by cells (a step of a wave), lists those about it and finds it among them; the draw is in the cell at which the
 // sums pass the number.  Without either that pass sums all.  Where a list does not hold the classes of a border's bin (thousands of equal
 // or nearly equal ones), the border is narrowed by bins of their keys to a class.
-// What bounds it: 4096 rows of 50257 fp32 classes (823 MB; 161 us to read them once at the rate of a large copy) take 245 us with T = 0 and
-// 281 with top-k 40 (two reads, 5.9 TB/s), 354 without filters and 461 with top-p 0.9, of which 80% are vector instructions, 66 a class, most
+// What bounds it: 4096 rows of 50257 fp32 classes (823 MB; 161 us to read them once at the rate of a large copy) take 242 us with T = 0 and
+// 260 with top-k 40 (two reads, 6.3 TB/s), 362 without filters and 460 with top-p 0.9, of which 80% are vector instructions, 66 a class, most
 // of them for the exact weights.  8 rows take 10 us with T = 0, 22 with top-k 40 and 42 with top-p 0.9: one CU a row and the barriers
 // between the passes.
 template <typename T, int NT>
