@@ -324,7 +324,8 @@ int ak_layer_norm(const void* x, int x_dtype, int64_t ldx, const void* weight, c
 
 /* dx (type of x), dw = sum_rows g h, db = sum_rows g (w_dtype) for h = (x - mean) rstd and the gradient g of y (type of x or AK_F32);
  * each may be null.  blocks (may be null; fp32 [F, 2, 2]) <- beta blocks + alpha sum_rows [[(g h)^2, g^2 h], [g^2 h, g^2]]: what
- * ak_unit_wise_stats gives from y and g, without dividing by the weight.  g may be null when rows is 0. */
+ * ak_unit_wise_stats gives from y and g, without dividing by the weight.  g may be null when rows is 0.  Sums over rows are for up to
+ * 2^24 features (AK_ERR_UNSUPPORTED beyond). */
 size_t ak_layer_norm_backward_ws_bytes(int64_t rows, int64_t F, int with_blocks);
 int ak_layer_norm_backward(const void* g, int g_dtype, int64_t ldg, const void* x, int x_dtype, int64_t ldx, const float* mean,
                            const float* rstd, const void* weight, int w_dtype, int64_t rows, int64_t F, void* dx, int64_t lddx,

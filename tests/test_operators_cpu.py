@@ -287,3 +287,10 @@ def test_calls_in_one_step_leave_the_unusual_to_the_others():
     with pytest.raises(ValueError):
         host.bind(0, 0, 0, 0, 0, 0, 0)
     assert _lib.load_host() is host
+
+
+def test_sums_over_rows_refuse_more_features_than_a_launch_has_threads_for():
+    from asdl_amd import _lib
+    lib, a, F = _lib.load(), 4096, (1 << 24) + 1
+    for dw, blocks in ((a, None), (None, a)):
+        assert lib.ak_layer_norm_backward(a, 0, F, a, 0, F, a, a, a, 0, 4, F, a, F, dw, None, blocks, 1.0, 0.0, a, 1 << 40, None) == -3
