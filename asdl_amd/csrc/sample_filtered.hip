@@ -762,8 +762,9 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
       for (int q = 0; q < PER_BINS; ++q)
         sum_of += own[q] = static_cast<double>(sums[tid * PER_BINS + q]) * static_cast<double>(exp2f(-drop * static_cast<float>(tid * PER_BINS + q)));
       sf_scan<WAVES>(sum_of, sh.red_double, before, total);
-      // Where min-p keeps less than top-p would whatever the sums are off by (1e-4 at most), it alone decides, and its classes are summed
-      // below (256 requests with filters of their own: 56 us for 69).
+      // Where min-p seems to keep less than top-p would, its classes are summed at once (256 requests with filters of their own: 56 us for
+      // 69).  These sums are estimates, whose error grows with |logit| / T (the product with a is rounded) and with the number of classes
+      // (unit); 1e-3 is a margin that usually does.  What they say is proved below, as the border's bins are.
       const int least_bin = filter.m > 0. ? bin_of(top + static_cast<float>(filter.t) * __log2f(static_cast<float>(filter.m)) * 0.693147f) + 1 : kSfBins;
       if (tid == 0) {
         sh.where = sh.until = kSfBins - 1;
@@ -783,74 +784,92 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
       }
       clear_list();
     }
-    const bool least_decides = sh.found != 0;
-    if (!least_decides) {
-      // One pass with exact weights: of the bins in front of the border's (and of a neighbour, where the border is near its edge), by
-      // cells; of all others; the classes of these bins.
-      const float from_bin = sh.where > 0 ? static_cast<float>(sh.where) : -INFINITY, to_bin = sh.until < kSfBins - 1 ? static_cast<float>(sh.until) : INFINITY;
-      u64 own_all = 0, own_above = 0;
-      auto add_weights = [&](auto every) {
-        row.each(
-            [&](const auto& v, int at) {
-              constexpr int N = sizeof(v) / sizeof(float);
-              bool want[N];
-#pragma unroll
-              for (int e = 0; e < N; ++e) {
-                const float bin = bin_at(v[e]);
-                const bool in = decltype(every)::value ? true : kept(v[e], at + e);
-                const u64 w = in ? weight(v[e]) : 0;
-                const bool front = bin < from_bin;
-                sum += front ? w : 0;
-                own_all += w;
-                want[e] = in & !front & (bin <= to_bin);
-              }
-              list(want, v, at);
-            },
-            [&](int step) {
-              own_above += sum;
-              to_cell(step);
-            });
-      };
-      if (unrestricted) add_weights(std::true_type{});
-      else add_weights(std::false_type{});
-      const u64 above = group_sum<WAVES>(own_above, sh.red), all = group_sum<WAVES>(own_all, sh.red), target = sf_border(filter.p, all);
-      const int count = sh.listed;
-      if (tid == 0) sh.found = 0;
-      if (count <= kSfListed && above < target) {
-        sf_sort<NT>(sh.order, count);
-        each_of(sh.order, count, [&](u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](u64 o, u64 w, u64 before) {
-          if (above + before >= target) return;
-          const int c = sf_order_class(o);
-          if (w != 0) atomicAdd(sh.cells + row.cell(c), w);
-          if (above + before + w >= target) {
-            sh.found_key = sf_order_key(o);
-            sh.found_index = c;
-            sh.found = 1;
-          }
-        });
-      }
-      __syncthreads();
-      if (sh.found) {
-        border_value = sf_value(sh.found_key);
-        border_index = sh.found_index;
-        if (weight.scaled(border_value) >= least) return draw_cells();       // (else the cells hold what min-p leaves out)
-      } else {
-        // The border was not there, or the classes too many: the weights of bins, and the border's bin in parts.
-        clear_bins();
-        row.each([&](const auto& v, int at) {
-          int c = at;
-          for (const float x : v) {
-            if (kept(x, c)) {
-              const u64 w = weight(x);
-              if (w != 0) atomicAdd(sh.bins + bin_of(x), w);
+    if (sh.found != 0) {
+      // Exact sums of what min-p keeps, by cells, and of all.  Where the one is at most top-p's border, so is the weight in front of each of
+      // its classes: top-p keeps them all, and the draw is among them.
+      u64 own_kept = 0, own_all = 0;
+      row.each(
+          [&](const auto& v, int at) {
+            int c = at;
+            for (const float x : v) {
+              const double w = weight.scaled(x);
+              const u64 whole = kept(x, c++) ? SfWeight::whole(w) : 0;
+              own_all += whole;
+              sum += w < least ? 0 : whole;
             }
-            ++c;
+          },
+          [&](int step) {
+            own_kept += sum;
+            to_cell(step);
+          });
+      const u64 by_least = group_sum<WAVES>(own_kept, sh.red), all = group_sum<WAVES>(own_all, sh.red);
+      if (by_least <= sf_border(filter.p, all)) return draw_cells();
+    }
+    // One pass with exact weights: of the bins in front of the border's (and of a neighbour, where the border is near its edge), by
+    // cells; of all others; the classes of these bins.
+    const float from_bin = sh.where > 0 ? static_cast<float>(sh.where) : -INFINITY, to_bin = sh.until < kSfBins - 1 ? static_cast<float>(sh.until) : INFINITY;
+    u64 own_all = 0, own_above = 0;
+    auto add_weights = [&](auto every) {
+      row.each(
+          [&](const auto& v, int at) {
+            constexpr int N = sizeof(v) / sizeof(float);
+            bool want[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float bin = bin_at(v[e]);
+              const bool in = decltype(every)::value ? true : kept(v[e], at + e);
+              const u64 w = in ? weight(v[e]) : 0;
+              const bool front = bin < from_bin;
+              sum += front ? w : 0;
+              own_all += w;
+              want[e] = in & !front & (bin <= to_bin);
+            }
+            list(want, v, at);
+          },
+          [&](int step) {
+            own_above += sum;
+            to_cell(step);
+          });
+    };
+    if (unrestricted) add_weights(std::true_type{});
+    else add_weights(std::false_type{});
+    const u64 above = group_sum<WAVES>(own_above, sh.red), all = group_sum<WAVES>(own_all, sh.red), target = sf_border(filter.p, all);
+    const int count = sh.listed;
+    if (tid == 0) sh.found = 0;
+    if (count <= kSfListed && above < target) {
+      sf_sort<NT>(sh.order, count);
+      each_of(sh.order, count, [&](u64 o) { return weight(sf_value(sf_order_key(o))); }, [&](u64 o, u64 w, u64 before) {
+        if (above + before >= target) return;
+        const int c = sf_order_class(o);
+        if (w != 0) atomicAdd(sh.cells + row.cell(c), w);
+        if (above + before + w >= target) {
+          sh.found_key = sf_order_key(o);
+          sh.found_index = c;
+          sh.found = 1;
+        }
+      });
+    }
+    __syncthreads();
+    if (sh.found) {
+      border_value = sf_value(sh.found_key);
+      border_index = sh.found_index;
+      if (weight.scaled(border_value) >= least) return draw_cells();       // (else the cells hold what min-p leaves out)
+    } else {
+      // The border was not there, or the classes too many: the weights of bins, and the border's bin in parts.
+      clear_bins();
+      row.each([&](const auto& v, int at) {
+        int c = at;
+        for (const float x : v) {
+          if (kept(x, c)) {
+            const u64 w = weight(x);
+            if (w != 0) atomicAdd(sh.bins + bin_of(x), w);
           }
-        });
-        u64 same;
-        cross(sh.bins, [&](u64) { return target; }, same);
-        narrow(target, kept, weight);
-      }
+          ++c;
+        }
+      });
+      u64 same;
+      cross(sh.bins, [&](u64) { return target; }, same);
+      narrow(target, kept, weight);
     }
   }
   row.each([&](const auto& v, int at) {

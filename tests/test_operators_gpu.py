@@ -768,3 +768,57 @@ def test_filtered_draws_where_min_p_and_top_p_are_close(K, dtype, n):
             filters = dict(top_p=min(max(top_p, 1e-3), 0.9999), min_p=min_p)
             for t in (1.0, 0.3):
                 assert torch.equal(K.sample_filtered(logits, u, temperature=t, **filters).cpu(), draw64(logits, u, temperature=t, **filters)), (filters, t)
+
+
+def levels(rows_of, u):
+    """Logits of rows given as [(value, how often), ...], each row in an order of its own, and one number per row."""
+    n = sum(count for _, count in rows_of[0])
+    gen = torch.Generator().manual_seed(n)
+    rows = [torch.cat([torch.full((count,), value, dtype=torch.float64) for value, count in row])[torch.randperm(n, generator=gen)] for row in rows_of]
+    return torch.stack(rows).float().cuda(), torch.tensor(u, device='cuda', dtype=torch.float64).expand(len(rows)).contiguous()
+
+
+@pytest.mark.parametrize('row,t,p,m', [
+    ([(100000.0, 1), (99999.9921875, 145), (99999.9765625, 254)], 0.01, 0.7244, 0.277),
+    ([(1e6, 1), (999994.75, 3666), (999993.9375, 363)], 1.0, 0.95941, 0.0035),
+    ([(300.0, 1), (299.99475, 3666), (299.99395, 363)], 0.001, 0.9594, 0.0035),
+    ([(2000.0, 1), (1999.947, 3666), (1999.939, 363)], 0.01, 0.9594, 0.0035)])
+def test_filtered_draws_of_few_levels_far_from_zero(K, row, t, p, m):
+    """min-p keeps a little more than top-p would: top-p has to cut.  float32 has some steps only between these logits."""
+    for u in (0.0, 0.5, 0.99, 0.999, 0.9999, 0.99999, 1 - 2.0 ** -53):
+        logits, numbers = levels([row] * 8, u)
+        for top_p in (p, p - 1e-4, p + 1e-4, p + 2e-3):
+            filters = dict(temperature=t, top_p=top_p, min_p=m)
+            assert torch.equal(K.sample_filtered(logits, numbers, **filters).cpu(), draw64(logits, numbers, **filters)), (u, top_p)
+            each = dict(temperature=torch.full((8,), t, device='cuda'), top_p=torch.full((8,), top_p, device='cuda'), min_p=torch.full((8,), m, device='cuda'))
+            assert torch.equal(K.sample_filtered(logits, numbers, **each).cpu(), draw64(logits, numbers, **each)), (u, top_p)
+
+
+@pytest.mark.parametrize('n', [400, 3000, 30000])
+@pytest.mark.parametrize('offset', [-1e4, 1e4, 1e5, 1e6])
+def test_filtered_draws_with_an_offset_large_against_the_temperature(K, offset, n):
+    """Two levels below the largest logit, min-p between them, top_p on both sides of what min-p keeps; and spread logits."""
+    gen = torch.Generator().manual_seed(n)
+    rows = 8
+    for t in (0.01, 0.1, 1.0):
+        for _ in range(6):
+            r = torch.rand(3, generator=gen, dtype=torch.float64).tolist()
+            first = 1 + int((n - 2) * (0.1 + 0.8 * r[0]))
+            high = torch.tensor(offset, dtype=torch.float64)
+            step = float(torch.finfo(F32).eps) * abs(offset)           # one to two steps of float32
+            a, b = (float((high - max(t * d, least * step)).float()) for d, least in ((0.5 + 4 * r[1], 1), (5.0 + 3 * r[2], 3)))
+            wa, wb = (math.exp((x - offset) / t) for x in (a, b))
+            if wb < 1e-30 or wa / wb < 1.01:
+                continue
+            kept = 1 + first * wa
+            share, m = kept / (kept + (n - 1 - first) * wb), math.sqrt(wa * wb)
+            logits, u = levels([[(offset, 1), (a, first), (b, n - 1 - first)]] * rows, 0.0)
+            u = torch.linspace(0, 1, rows, device='cuda', dtype=torch.float64) * (1 - 1e-9)
+            for d in (-0.02, -2e-3, -1.1e-3, -5e-4, 5e-4, 1.1e-3, 2e-3):
+                if 0 < share + d < 1:
+                    filters = dict(temperature=t, top_p=share + d, min_p=m)
+                    assert torch.equal(K.sample_filtered(logits, u, **filters).cpu(), draw64(logits, u, **filters)), (t, first, a, b, d)
+        logits = rand(rows, n, seed=n, scale=2 * t, shift=offset)
+        for filters in (dict(top_p=0.6, min_p=0.05), dict(top_p=0.9, min_p=0.2), dict(top_k=n // 3, top_p=0.8, min_p=0.01), dict(top_p=0.3)):
+            got = K.sample_filtered(logits, u, temperature=t, **filters)
+            assert torch.equal(got.cpu(), draw64(logits, u, temperature=t, **filters)), (t, filters)
