@@ -739,8 +739,8 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
     const float up = exp2f(0.5f * drop), down = exp2f(-0.5f * drop);
     const float middle = 0.5f * (up + down) * p.unit + 8388608.f, slope = (down - up) * p.unit;      // (2^23: as above)
     auto share = [&](float v) {
-      const float u = v * a;
-      return __builtin_bit_cast(uint32_t, __builtin_fmaf(u - rintf(u), slope, middle)) - 0x4b000000u;
+      const float place = __builtin_fmaf(v, a, -rintf(v * a));       // (one rounding: v * a may be large)
+      return __builtin_bit_cast(uint32_t, __builtin_fmaf(place, slope, middle)) - 0x4b000000u;
     };
     auto add_sums = [&](auto all) {        // all: every class is kept (of -inf, in the last bin, nothing is taken)
       row.each([&](const auto& v, int at) {
