@@ -6,7 +6,7 @@ from contextlib import contextmanager, nullcontext
 
 import torch
 import torch.nn as nn
-from torch.autograd.graph import GradientEdge
+from torch.autograd.graph import get_gradient_edge
 
 from .layers import FusedLayerNorm
 from .matrices import *
@@ -123,8 +123,9 @@ def extend(model, *op_names, ignore_modules=None, map_rule=None, vectors=None, s
                         return None
                     handles.append(out_data.register_hook(grad_hook))
                     # the graph edge the hook sits on: a backward pass restricted to these edges still fires
-                    # every hook, without the weight-gradient kernels of the layers
-                    cxt.grad_edges.append(GradientEdge(out_data.grad_fn, out_data.output_nr))
+                    # every hook, without the weight-gradient kernels of the layers (an edge from a custom function's
+                    # output has to hold its node, which an output that the model drops does not)
+                    cxt.grad_edges.append(get_gradient_edge(out_data))
             handles.append(module.register_forward_hook(forward_hook))
         handles.append(model.register_forward_pre_hook(lambda *_: cxt.grad_edges.clear()))
         if not cxt.is_operation_registered(model):

@@ -294,3 +294,37 @@ def test_sums_over_rows_refuse_more_features_than_a_launch_has_threads_for():
     lib, a, F = _lib.load(), 4096, (1 << 24) + 1
     for dw, blocks in ((a, None), (None, a)):
         assert lib.ak_layer_norm_backward(a, 0, F, a, 0, F, a, a, a, 0, 4, F, a, F, dw, None, blocks, 1.0, 0.0, a, 1 << 40, None) == -3
+
+
+class _Dropped(nn.Module):
+    """A layer norm whose result nothing uses."""
+
+    def __init__(self):
+        super().__init__()
+        self.a, self.ln, self.b = nn.Linear(6, 6), nn.LayerNorm(6), nn.Linear(6, 4)
+
+    def forward(self, x):
+        x = self.a(x)
+        self.ln(x)
+        return self.b(x.tanh())
+
+
+@pytest.mark.parametrize('fisher_type', [FISHER_EMP, FISHER_MC, FISHER_EXACT])
+def test_a_fused_layer_norm_whose_result_is_dropped(fisher_type, monkeypatch):
+    """The pass differentiates with respect to its output, too, which is gone: no blocks, and the factors of the others."""
+    cpu_backend.install(monkeypatch)
+    monkeypatch.setattr(kernels, 'layer_norm', _layer_norm)
+    monkeypatch.setattr(kernels, 'layer_norm_backward', _Backward())
+    torch.manual_seed(1)
+    plain = _Dropped()
+    fused = copy.deepcopy(plain)
+    assert asdl_amd.fuse_layer_norms(fused) == 1
+    x, t = torch.randn(5, 6), torch.randint(4, (5,))
+    for model in (plain, fused):
+        shapes = [(nn.Linear, SHAPE_KRON), (nn.LayerNorm, asdl_amd.SHAPE_UNIT_WISE)]
+        maker = get_fisher_maker(model, FisherConfig(fisher_type, shapes, loss_type=LOSS_CROSS_ENTROPY, data_size=5, seed=1))
+        maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), t)
+        maker.forward_and_backward()
+    assert getattr(plain.ln, 'fisher', None) is None and getattr(fused.ln, 'fisher', None) is None
+    for m, n in ((plain.a, fused.a), (plain.b, fused.b)):
+        assert torch.equal(m.fisher.kron.A, n.fisher.kron.A) and torch.equal(m.fisher.kron.B, n.fisher.kron.B)
