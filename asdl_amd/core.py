@@ -106,6 +106,8 @@ def extend(model, *op_names, ignore_modules=None, map_rule=None, vectors=None, s
             needs_out = OP_SAVE_OUTPUTS in names or any(n in BWD_OPS_WITH_INPUTS for n in names)
 
             def forward_hook(_module, in_data, out_data, _has_bwd=has_bwd, _needs_out=needs_out, _op=op):
+                if cxt.settling:
+                    return               # (a checkpoint runs the forward pass again: its hooks have had their turn)
                 x = in_data[0].detach()
                 y = out_data.detach() if _needs_out else None
                 run_hook(lambda: _op.forward_post_process(x, y), x)

@@ -14,11 +14,13 @@ __all__ = ['layer_norm', 'FusedLayerNorm', 'fuse_layer_norms']
 
 class BlocksRequest:
     """Fisher blocks that a hook wants of a backward pass that is about to run: blocks <- beta*blocks + alpha * sums for the output
-    gradient ``g``.  Served once, by the backward pass or, where that does not run or sees another gradient, by settle()."""
+    gradient ``g``.  Served once, by the backward pass or, where that does not run or sees another gradient, by settle().
+
+    The saved tensors are unpacked by whoever serves, not for the request: torch.utils.checkpoint, which runs the forward pass again for
+    them, lets a pass unpack them once."""
 
     def __init__(self, node, g, blocks, alpha, beta):
-        self.x, _, self.mean, self.rstd = node.saved_tensors
-        self.g, self.version = g, g._version
+        self.node, self.g, self.version = node, g, g._version
         self.blocks, self.alpha, self.beta = blocks, alpha, beta
         self.open = True
 
@@ -26,11 +28,20 @@ class BlocksRequest:
         return g.data_ptr() == self.g.data_ptr() and g.numel() == self.g.numel() and g.is_contiguous() and self.g.is_contiguous() and \
             self.g._version == self.version
 
-    def settle(self):
+    def close(self):
+        """Holds nothing from here on."""
+        self.open = False
+        if self.node is not None and self.node.request is self:
+            self.node.request = None
+        self.node = self.g = self.blocks = None
+
+    def settle(self, saved=None):
+        """``saved``: the node's saved tensors, where the caller has them."""
         if self.open:
-            self.open = False
-            kernels.layer_norm_backward(self.g.reshape(self.x.shape), self.x, self.mean, self.rstd, blocks=self.blocks, alpha=self.alpha, beta=self.beta,
+            x, _, mean, rstd = self.node.saved_tensors if saved is None else saved
+            kernels.layer_norm_backward(self.g.reshape(x.shape), x, mean, rstd, blocks=self.blocks, alpha=self.alpha, beta=self.beta,
                                         need_x=False, need_weight=False, need_bias=False)
+            self.close()
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -47,15 +58,15 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, weight, mean, rstd = ctx.saved_tensors
-        request, ctx.request = ctx.request, None
-        blocks, alpha, beta = None, 1.0, 0.0
+        saved = ctx.saved_tensors
+        x, weight, mean, rstd = saved
+        request, blocks, alpha, beta = ctx.request, None, 1.0, 0.0
         if request is not None and request.open:
             if request.fits(g):
-                request.open = False
                 blocks, alpha, beta = request.blocks, request.alpha, request.beta
+                request.close()
             else:
-                request.settle()
+                request.settle(saved)
         need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
         dx, dw, db = kernels.layer_norm_backward(g, x, mean, rstd, weight, blocks, alpha, beta, need_x, need_weight, need_bias,
                                                  weight_dtype=ctx.weight_dtype)

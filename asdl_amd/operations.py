@@ -525,6 +525,8 @@ class LayerNorm(_NormOperation):
             beta = 0.0
         node.request = BlocksRequest(node, g, out, alpha, beta)
         self._context.open_blocks.append(node.request)
+        # (at the end of this pass, while its graph and what it saved are as they were)
+        torch.autograd.Variable._execution_engine.queue_callback(self._context.settle_blocks)
         return out
 
 
@@ -637,6 +639,7 @@ class OperationContext:
         self.factor_stream = None
         self.grad_edges = []       # autograd edges of the hooked module outputs of the latest forward pass
         self.open_blocks = []      # BlocksRequests that backward passes may still serve
+        self.settling = False      # whether these are being served
         self._eager_total = 0.0
         self._eager_done = False
         self._inverse_cost = 0.0
@@ -663,14 +666,21 @@ class OperationContext:
         self._inverse_chunks = []
         self._pending_unit = []
         for request in self.open_blocks:
-            request.open = False
+            request.close()
         self.open_blocks = []
 
     def settle_blocks(self, of=None):
-        """Has the Fisher blocks that no backward pass has computed computed now (``of``: those of this tensor only)."""
-        for request in self.open_blocks:
-            if of is None or request.blocks is of:
-                request.settle()
+        """Has the Fisher blocks that no backward pass has computed computed now (``of``: those of this tensor only).  Every pass ends
+        with it."""
+        if self.settling or not self.open_blocks:
+            return
+        self.settling = True
+        try:
+            for request in self.open_blocks:
+                if of is None or request.blocks is of:
+                    request.settle()
+        finally:
+            self.settling = False
         self.open_blocks = [r for r in self.open_blocks if r.open]
 
     def call_operations_in_forward(self, module, in_data, out_data):

@@ -328,3 +328,131 @@ def test_a_fused_layer_norm_whose_result_is_dropped(fisher_type, monkeypatch):
     assert getattr(plain.ln, 'fisher', None) is None and getattr(fused.ln, 'fisher', None) is None
     for m, n in ((plain.a, fused.a), (plain.b, fused.b)):
         assert torch.equal(m.fisher.kron.A, n.fisher.kron.A) and torch.equal(m.fisher.kron.B, n.fisher.kron.B)
+
+
+# ------------------------------------------------------------------------------------------------ blocks and what else users do with a pass
+class _Block(nn.Module):
+    def __init__(self, d=6, layer_norm_first=False):
+        super().__init__()
+        self.a, self.ln, self.b = nn.Linear(d, d), nn.LayerNorm(d), nn.Linear(d, d)
+        self.layer_norm_first = layer_norm_first
+
+    def forward(self, x):
+        return self.b((self.a(self.ln(x)) if self.layer_norm_first else self.ln(self.a(x))).tanh())
+
+
+class _Checkpointed(nn.Module):
+    def __init__(self, checkpointed, layer_norm_first):
+        super().__init__()
+        self.blocks = nn.ModuleList([_Block(layer_norm_first=layer_norm_first and i == 0) for i in range(2)])
+        self.head = nn.Linear(6, 4)
+        self.checkpointed = checkpointed
+
+    def forward(self, x):
+        from torch.utils.checkpoint import checkpoint
+        for block in self.blocks:
+            x = checkpoint(block, x, use_reentrant=False) if self.checkpointed else block(x)
+        return self.head(x)
+
+
+def _stand_ins(monkeypatch):
+    cpu_backend.install(monkeypatch)
+    backward = _Backward()
+    monkeypatch.setattr(kernels, 'layer_norm', _layer_norm)
+    monkeypatch.setattr(kernels, 'layer_norm_backward', backward)
+    return backward
+
+
+@pytest.mark.parametrize('layer_norm_first', [False, True])
+def test_blocks_under_checkpointing_are_those_without(layer_norm_first, monkeypatch):
+    """Saved tensors are unpacked once a pass, as torch.utils.checkpoint asks for."""
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    _stand_ins(monkeypatch)
+    torch.manual_seed(1)
+    plain = _Checkpointed(False, layer_norm_first)
+    x, t = torch.randn(5, 6), torch.randint(4, (5,))
+    got = []
+    for checkpointed in (False, True):
+        model = copy.deepcopy(plain)
+        model.checkpointed = checkpointed
+        assert asdl_amd.fuse_layer_norms(model) == 2
+        with extend(model, (nn.LayerNorm, OP_COV_UNIT_WISE)) as cxt:
+            F.cross_entropy(model(x), t, reduction='sum').backward()
+            got.append([cxt.get_result(b.ln, OP_COV_UNIT_WISE, 'data').clone() for b in model.blocks] + [p.grad for p in model.parameters() if p.grad is not None])
+    assert len(got[0]) == len(got[1]) > 2 and all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize('layer_norm_first', [False, True])
+@pytest.mark.parametrize('config', [dict(ema_decay=0.3), dict(ignore_modules=[nn.Linear])])
+@pytest.mark.parametrize('fisher_type,samples', [(FISHER_EMP, 1), (FISHER_MC, 1), (FISHER_MC, 2), (FISHER_EXACT, 1)])
+def test_a_checkpointed_step_with_fused_layer_norms_is_the_plain_one(fisher_type, samples, config, layer_norm_first, monkeypatch):
+    """The same factors and gradients as with torch.nn.LayerNorm, whatever the checkpoint runs again for the blocks.  float32 and a damping
+    of 1e-2, as above."""
+    _stand_ins(monkeypatch)
+    torch.manual_seed(2)
+    plain = _Checkpointed(True, layer_norm_first)
+    fused = copy.deepcopy(plain)
+    assert asdl_amd.fuse_layer_norms(fused) == 2
+    x, t = torch.randn(5, 6), torch.randint(4, (5,))
+    for model in (plain, fused):
+        maker = KfacGradientMaker(model, PreconditioningConfig(data_size=5, damping=1e-2, **config), fisher_type=fisher_type, n_mc_samples=samples, seed=3)
+        for _ in range(2):
+            model.zero_grad()
+            maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), t)
+            maker.forward_and_backward()
+
+    def off(a, b):
+        return float((a - b).norm() / b.norm())
+    for (name, p), q in zip(plain.named_parameters(), fused.named_parameters()):
+        assert (p.grad is None) == (q[1].grad is None) and (p.grad is None or off(q[1].grad, p.grad) < 5000 * 10 * 2.0 ** -24), name
+    held = 0
+    for m, n in zip(plain.modules(), fused.modules()):
+        if hasattr(m, 'fisher'):
+            a, b = (m.fisher.unit, n.fisher.unit) if isinstance(m, nn.LayerNorm) else (m.fisher.kron, n.fisher.kron)
+            for key in ('data', 'A', 'B'):
+                if isinstance(getattr(a, key, None), torch.Tensor):
+                    held += 1
+                    assert off(getattr(b, key), getattr(a, key)) < 64 * 2.0 ** -24, (m, key)
+            for key in ('inv', 'A_inv', 'B_inv'):
+                if getattr(a, key, None) is not None:
+                    held += 1
+                    assert off(getattr(b, key), getattr(a, key)) < 5000 * 10 * 2.0 ** -24, (m, key)
+    assert held >= 2
+
+
+def test_blocks_outlive_the_graph_of_a_pass_that_left_the_layer_norm_out(monkeypatch):
+    """A pass as far as the layer norm's output only: its blocks are computed when they are asked for, whatever is left of the graph."""
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    backward = _stand_ins(monkeypatch)
+    torch.manual_seed(3)
+    ln, x = FusedLayerNorm(6), torch.randn(5, 6)
+    with extend(ln, OP_COV_UNIT_WISE) as cxt:
+        y = ln(x)
+        loss = (y ** 3).sum()
+        (g,) = torch.autograd.grad(loss, y)
+        g, h = g.clone(), _layer_norm(x)[0]
+        del y, loss
+        got = cxt.get_result(ln, OP_COV_UNIT_WISE, 'data')
+    assert backward.alone == 1 and torch.allclose(got[:, 1, 1], (g * g).sum(0)) and torch.allclose(got[:, 0, 0], (g * h * g * h).sum(0))
+
+
+def test_blocks_of_two_passes_that_left_the_layer_norm_out(monkeypatch):
+    """Each pass ends with its blocks: a later forward pass, and new values in what the first one saved, do not reach them."""
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    backward = _stand_ins(monkeypatch)
+    torch.manual_seed(3)
+    ln, x = FusedLayerNorm(6), torch.randn(5, 6)
+    want = 0
+    with extend(ln, OP_COV_UNIT_WISE) as cxt:
+        for turn in range(2):
+            y = ln(x)
+            (g,) = torch.autograd.grad((y ** 3).sum(), y)
+            h = _layer_norm(x)[0]
+            want = want + torch.stack([(g * h * g * h).sum(0), (g * g).sum(0)])
+            del y
+            g.mul_(100)
+            x.normal_()
+            with torch.no_grad():
+                ln.weight.mul_(1.5)
+        got = cxt.get_result(ln, OP_COV_UNIT_WISE, 'data')
+    assert backward.alone == 2 and torch.allclose(got[:, 0, 0], want[0]) and torch.allclose(got[:, 1, 1], want[1])

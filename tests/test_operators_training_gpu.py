@@ -280,3 +280,41 @@ def test_a_captured_forward_and_backward_pass():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, e) for o, e in zip(outs, passes(x, w, b))), turn
+
+
+@pytest.mark.parametrize('fisher_type', [FISHER_EMP, FISHER_MC])
+def test_blocks_of_a_checkpointed_decoder(fisher_type):
+    """Blocks of every layer norm with the layers run again for the backward pass, and without: the same kernels on the same values."""
+    from torch.utils.checkpoint import checkpoint
+
+    class Layer(nn.Module):
+        def __init__(self, d=64):
+            super().__init__()
+            self.ln1, self.up, self.ln2, self.down = nn.LayerNorm(d), nn.Linear(d, 2 * d), nn.LayerNorm(2 * d), nn.Linear(2 * d, d)
+
+        def forward(self, x):
+            return x + self.down(self.ln2(F.gelu(self.up(self.ln1(x)))))
+
+    class Layers(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.layers, self.head, self.checkpointed = nn.ModuleList([Layer() for _ in range(3)]), nn.Linear(64, 11), False
+
+        def forward(self, x):
+            for layer in self.layers:
+                x = checkpoint(layer, x, use_reentrant=False) if self.checkpointed else layer(x)
+            return self.head(x)
+    torch.manual_seed(4)
+    model = Layers().cuda()
+    assert asdl_amd.fuse_layer_norms(model) == 6
+    x, t = rand(200, 64, seed=1), torch.randint(0, 11, (200,), device='cuda')
+    got = []
+    for model.checkpointed in (False, True):
+        model.zero_grad()
+        maker = KfacGradientMaker(model, PreconditioningConfig(data_size=200, damping=1e-2, ema_decay=0.5, ignore_modules=[nn.Linear]), fisher_type=fisher_type, seed=1)
+        maker.setup_loss_call(F.cross_entropy, maker.setup_model_call(model, x), t)
+        maker.forward_and_backward()
+        got.append([m.fisher.unit.data.clone() for m in model.modules() if isinstance(m, FusedLayerNorm)] + [p.grad.clone() for p in model.parameters()])
+        for m in model.modules():
+            m.__dict__.pop('fisher', None)
+    assert len(got[0]) == 6 + 26 and all(torch.equal(a, b) for a, b in zip(*got))
