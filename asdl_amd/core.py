@@ -112,18 +112,20 @@ def extend(model, *op_names, ignore_modules=None, map_rule=None, vectors=None, s
                 y = out_data.detach() if _needs_out else None
                 run_hook(lambda: _op.forward_post_process(x, y), x)
                 if _has_bwd and out_data.requires_grad:
-                    node = out_data.grad_fn if hasattr(_op, 'backward_of') and hasattr(out_data.grad_fn, 'takes_blocks_request') else None
+                    node = out_data.grad_fn if hasattr(_op, 'backward_of') and hasattr(out_data.grad_fn, 'blocks_requests') else None
 
                     def grad_hook(grad, _m=_module):
                         if not cxt.is_operation_registered(_m):
                             return None          # context already closed
                         g = grad.detach()
-                        if node is not None:
-                            _op.backward_of(node, g)        # (launches nothing: the backward pass does that)
+                        if node is not None:                # (launches nothing: the backward pass does that)
+                            _op.backward_of(node, g, keep=next(reversed(hooks), None) != handle.id)
                         else:
                             run_hook(lambda: _op.backward_pre_process(g, None), g, backward=True)
                         return None
-                    handles.append(out_data.register_hook(grad_hook))
+                    handle = out_data.register_hook(grad_hook)
+                    hooks = out_data._backward_hooks if node is not None else None        # in the order in which they run
+                    handles.append(handle)
                     # the graph edge the hook sits on: a backward pass restricted to these edges still fires
                     # every hook, without the weight-gradient kernels of the layers (an edge from a custom function's
                     # output has to hold its node, which an output that the model drops does not)

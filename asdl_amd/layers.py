@@ -17,12 +17,14 @@ class BlocksRequest:
     gradient ``g``.  Served once, by the backward pass or, where that does not run or sees another gradient, by settle().
 
     The saved tensors are unpacked by whoever serves, not for the request: torch.utils.checkpoint, which runs the forward pass again for
-    them, lets a pass unpack them once."""
+    them, lets a pass unpack them once.  ``keep``: other hooks follow, which may write to the gradient; the request has a copy then."""
 
-    def __init__(self, node, g, blocks, alpha, beta):
+    def __init__(self, node, g, blocks, alpha, beta, keep=False):
         self.node, self.g, self.version = node, g, g._version
+        self.kept = g.clone() if keep else None
         self.blocks, self.alpha, self.beta = blocks, alpha, beta
         self.open = True
+        node.blocks_requests.append(self)
 
     def fits(self, g):
         return g.data_ptr() == self.g.data_ptr() and g.numel() == self.g.numel() and g.is_contiguous() and self.g.is_contiguous() and \
@@ -31,15 +33,20 @@ class BlocksRequest:
     def close(self):
         """Holds nothing from here on."""
         self.open = False
-        if self.node is not None and self.node.request is self:
-            self.node.request = None
-        self.node = self.g = self.blocks = None
+        if self.node is not None:
+            self.node.blocks_requests.remove(self)
+        self.node = self.g = self.kept = self.blocks = None
 
     def settle(self, saved=None):
         """``saved``: the node's saved tensors, where the caller has them."""
         if self.open:
+            g = self.g if self.kept is None else self.kept
+            if self.kept is None and g._version != self.version:
+                self.close()
+                raise RuntimeError('The gradient of a layer norm\'s result was changed in place, behind the hooks on this result, before its Fisher '
+                                   'blocks were computed. Return a new gradient instead.')
             x, _, mean, rstd = self.node.saved_tensors if saved is None else saved
-            kernels.layer_norm_backward(self.g.reshape(x.shape), x, mean, rstd, blocks=self.blocks, alpha=self.alpha, beta=self.beta,
+            kernels.layer_norm_backward(g.reshape(x.shape), x, mean, rstd, blocks=self.blocks, alpha=self.alpha, beta=self.beta,
                                         need_x=False, need_weight=False, need_bias=False)
             self.close()
 
@@ -51,8 +58,7 @@ class _LayerNorm(torch.autograd.Function):
         ctx.save_for_backward(x, weight, mean, rstd)
         ctx.has_bias = bias is not None
         ctx.weight_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else None
-        ctx.takes_blocks_request = True
-        ctx.request = None
+        ctx.blocks_requests = []
         return y
 
     @staticmethod
@@ -60,9 +66,9 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, g):
         saved = ctx.saved_tensors
         x, weight, mean, rstd = saved
-        request, blocks, alpha, beta = ctx.request, None, 1.0, 0.0
-        if request is not None and request.open:
-            if request.fits(g):
+        blocks, alpha, beta = None, 1.0, 0.0
+        for request in list(ctx.blocks_requests):         # (one for each set of hooks on the module)
+            if blocks is None and request.fits(g):
                 blocks, alpha, beta = request.blocks, request.alpha, request.beta
                 request.close()
             else:

@@ -507,9 +507,9 @@ class LayerNorm(_NormOperation):
         f = module.weight.numel()
         return tensor.reshape(-1, f)
 
-    def backward_of(self, node, out_grads):
-        """backward_pre_process() for the call of the module that ``node`` stands for."""
-        self._node = node
+    def backward_of(self, node, out_grads, keep):
+        """backward_pre_process() for the call of the module that ``node`` stands for.  ``keep``: see BlocksRequest."""
+        self._node, self._keep = node, keep
         try:
             self.backward_pre_process(out_grads, None)
         finally:
@@ -523,8 +523,7 @@ class LayerNorm(_NormOperation):
         if out is None:
             out = torch.empty(weight.numel(), 2, 2, dtype=torch.float32, device=g.device)
             beta = 0.0
-        node.request = BlocksRequest(node, g, out, alpha, beta)
-        self._context.open_blocks.append(node.request)
+        self._context.open_blocks.append(BlocksRequest(node, g, out, alpha, beta, self._keep))
         # (at the end of this pass, while its graph and what it saved are as they were)
         torch.autograd.Variable._execution_engine.queue_callback(self._context.settle_blocks)
         return out

@@ -456,3 +456,66 @@ def test_blocks_of_two_passes_that_left_the_layer_norm_out(monkeypatch):
                 ln.weight.mul_(1.5)
         got = cxt.get_result(ln, OP_COV_UNIT_WISE, 'data')
     assert backward.alone == 2 and torch.allclose(got[:, 0, 0], want[0]) and torch.allclose(got[:, 1, 1], want[1])
+
+
+@pytest.mark.parametrize('where', ['tensor', 'two calls', 'checkpoint', 'full'])
+def test_a_gradient_that_another_hook_scales_in_place_does_not_reach_the_blocks(where, monkeypatch):
+    """The blocks are those of the gradient that the framework's hook sees, as with torch.nn.LayerNorm."""
+    from torch.utils.checkpoint import checkpoint
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    _stand_ins(monkeypatch)
+    torch.manual_seed(4)
+    pre = nn.Linear(6, 6)
+    x, got, grads = torch.randn(5, 6), [], []
+
+    def scale(g):
+        g.mul_(10)
+
+    def scale_of_module(module, grads, out_grads):
+        out_grads[0].mul_(10)
+    for ln in (nn.LayerNorm(6), FusedLayerNorm(6)):
+        pre.zero_grad()
+        with extend(ln, OP_COV_UNIT_WISE) as cxt:
+            if where == 'full':
+                ln.register_full_backward_hook(scale_of_module)
+            y = checkpoint(lambda z: ln(pre(z)), x, use_reentrant=False) if where == 'checkpoint' else ln(pre(x))
+            if where != 'full':
+                y.register_hook(scale)
+            if where == 'two calls':
+                y.register_hook(lambda g: g * 2)
+            (y ** 3).sum().backward()          # (of y ** 2 the sum is a constant, and the gradients in front all rounding)
+            got.append(cxt.get_result(ln, OP_COV_UNIT_WISE, 'data').clone())
+            grads.append(pre.weight.grad.clone())
+    assert torch.allclose(got[0], got[1], rtol=1e-4, atol=1e-5) and torch.allclose(grads[0], grads[1], rtol=1e-4, atol=1e-5)
+
+
+def test_a_gradient_that_changes_behind_all_hooks_is_refused(monkeypatch):
+    """A hook on the autograd node itself runs behind those on the tensor, unseen: what it writes to the gradient is noticed."""
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    _stand_ins(monkeypatch)
+    ln, pre, x = FusedLayerNorm(6), nn.Linear(6, 6), torch.randn(5, 6)
+    with pytest.raises(RuntimeError, match='in place'):
+        with extend(ln, OP_COV_UNIT_WISE):
+            y = ln(pre(x))
+
+            def scale(grads):
+                grads[0].mul_(10)
+            y.grad_fn.register_prehook(scale)
+            (y ** 2).sum().backward()
+
+
+@pytest.mark.parametrize('limited', [False, True])
+def test_two_sets_of_hooks_on_one_layer_norm_have_their_blocks_each(limited, monkeypatch):
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    backward = _stand_ins(monkeypatch)
+    torch.manual_seed(5)
+    ln, x = FusedLayerNorm(6), torch.randn(5, 6)
+    with extend(ln, OP_COV_UNIT_WISE) as first, extend(ln, OP_COV_UNIT_WISE) as second:
+        second.set_cov_scale(0.5)
+        y = ln(x)
+        loss = (y ** 3).sum()
+        torch.autograd.grad(loss, y) if limited else loss.backward()
+        got = [cxt.get_result(ln, OP_COV_UNIT_WISE, 'data').clone() for cxt in (first, second)]
+    h, g = _layer_norm(x)[0], 3 * y.detach() ** 2
+    assert torch.allclose(got[0][:, 1, 1], (g * g).sum(0)) and torch.allclose(got[0][:, 0, 0], (g * h * g * h).sum(0)) and torch.allclose(got[1], 0.5 * got[0])
+    assert backward.alone == 2          # (the input needs no gradient)

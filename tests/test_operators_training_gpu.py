@@ -318,3 +318,19 @@ def test_blocks_of_a_checkpointed_decoder(fisher_type):
         for m in model.modules():
             m.__dict__.pop('fisher', None)
     assert len(got[0]) == 6 + 26 and all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_a_hook_that_scales_the_gradient_in_place_does_not_reach_the_blocks():
+    from asdl_amd import OP_COV_UNIT_WISE, extend
+    torch.manual_seed(6)
+    pre, x, got = nn.Linear(96, 96).cuda(), rand(300, 96, seed=1), []
+    for scaled in (False, True):
+        ln = FusedLayerNorm(96).cuda()
+        with extend(ln, OP_COV_UNIT_WISE) as cxt:
+            y = ln(pre(x))
+            if scaled:
+                y.register_hook(lambda g: g.mul_(10))
+            (y ** 3).sum().backward()
+            got.append((cxt.get_result(ln, OP_COV_UNIT_WISE, 'data').clone(), ln.weight.grad))
+    # the blocks of a pass of their own and of the fused one: the same kernel, sums in the same order
+    assert torch.equal(got[0][0], got[1][0]) and off(got[1][1], 10 * got[0][1]) < 64 * U
