@@ -354,12 +354,18 @@ class FisherMCCrossEntropy(FisherMaker):
     def do_local_accumulate(self) -> bool:
         return self.config.n_mc_samples > 1
 
+    def forward_and_backward(self, *args, **kwargs):
+        if self.config.mc_filtered and self._sampling_replaced:
+            raise ValueError('mc_temperature, mc_top_k, mc_top_p and mc_min_p are for the targets that are drawn here. sample_targets() has been '
+                             'replaced.')
+        return super().forward_and_backward(*args, **kwargs)
+
     def _fisher_loop(self, closure):
         logits = self._logits
         n_mc_samples = self.config.n_mc_samples
         log_probs = F.log_softmax(logits, dim=-1)
         dist = None
-        filtered = self.config.mc_filtered and not self._sampling_replaced
+        filtered = self.config.mc_filtered
         if not filtered and (self._sampling_replaced or not kernels.sampleable(logits)):
             # validate_args=False: the check of the simplex constraint would synchronise the host with the forward
             # pass; the draw itself (normalisation + multinomial) is unchanged
@@ -393,7 +399,7 @@ class FisherMCCrossEntropy(FisherMaker):
         return 'sample_targets' in self.__dict__ or type(self).sample_targets is not FisherMCCrossEntropy.sample_targets
 
     def sample_targets(self, dist, i):
-        """One draw of the model's predictive distribution; override to replay fixed targets.  (Without an override,
+        """One draw of the model's predictive distribution; override to replay fixed targets (not with the mc_* filters).  (Without an override,
         float32 logits on the GPU are sampled by one kernel from the same random numbers, kernels.sample_categorical.)"""
         return dist.sample()
 

@@ -519,3 +519,30 @@ def test_two_sets_of_hooks_on_one_layer_norm_have_their_blocks_each(limited, mon
     h, g = _layer_norm(x)[0], 3 * y.detach() ** 2
     assert torch.allclose(got[0][:, 1, 1], (g * g).sum(0)) and torch.allclose(got[0][:, 0, 0], (g * h * g * h).sum(0)) and torch.allclose(got[1], 0.5 * got[0])
     assert backward.alone == 2          # (the input needs no gradient)
+
+
+@pytest.mark.parametrize('how', ['attribute', 'subclass'])
+@pytest.mark.parametrize('filters', [dict(mc_temperature=0.5), dict(mc_top_k=3), dict(mc_top_p=0.9), dict(mc_min_p=0.1)])
+def test_filters_with_replaced_targets_are_refused(filters, how, monkeypatch):
+    """sample_targets() gets the whole distribution: filters would be dropped.  Before the forward pass, so that no factor has changed."""
+    from asdl_amd import fisher
+    cpu_backend.install(monkeypatch)
+    model = nn.Sequential(nn.Linear(3, 4))
+    x, ran = torch.randn(2, 3), []
+    model.register_forward_pre_hook(lambda *_: ran.append(1))
+
+    class Mine(fisher.FisherMCCrossEntropy):
+        def sample_targets(self, dist, i):
+            return torch.zeros(2, dtype=torch.long)
+    for more in (filters, {}):
+        config = FisherConfig(FISHER_MC, [SHAPE_KRON], loss_type=LOSS_CROSS_ENTROPY, data_size=2, **more)
+        maker = Mine(model, config) if how == 'subclass' else get_fisher_maker(model, config)
+        if how == 'attribute':
+            maker.sample_targets = lambda dist, i: torch.zeros(2, dtype=torch.long)
+        maker.setup_model_call(model, x)
+        if more:
+            with pytest.raises(ValueError, match='sample_targets'):
+                maker.forward_and_backward()
+            assert not ran
+        else:
+            maker.forward_and_backward()
