@@ -264,6 +264,10 @@ PyObject* gradient_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
               : entries.grad_norm(table.data(), static_cast<int>(n), static_cast<int>(kind), norm.data_ptr<float>(), ws.data_ptr(), bytes, stream);
   }
   if (rc != AK_OK) return PyLong_FromLong(rc);
+  for (Py_ssize_t i = 0; clip && i < n; ++i) {
+    const at::Tensor& changed = THPVariable_Unpack(PyList_GET_ITEM(args[1], i));
+    if (!changed.is_inference()) changed.unsafeGetTensorImpl()->bump_version();       // (autograd notices what it keeps)
+  }
   return wrapped(norm);
   END_HANDLE_TH_ERRORS
 }

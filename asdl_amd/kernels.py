@@ -1581,6 +1581,7 @@ def _launch_norm(grads, outs, norm_type, max_norm):
         with torch.no_grad(), _on_launch_stream():
             for out, dense in late:
                 out.copy_(dense.reshape(out.shape))
+    torch.autograd.graph.increment_version([o for o in outs if not o.is_inference()])
     return norm
 
 

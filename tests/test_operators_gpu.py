@@ -822,3 +822,33 @@ def test_filtered_draws_with_an_offset_large_against_the_temperature(K, offset, 
         for filters in (dict(top_p=0.6, min_p=0.05), dict(top_p=0.9, min_p=0.2), dict(top_k=n // 3, top_p=0.8, min_p=0.01), dict(top_p=0.3)):
             got = K.sample_filtered(logits, u, temperature=t, **filters)
             assert torch.equal(got.cpu(), draw64(logits, u, temperature=t, **filters)), (t, filters)
+
+
+@pytest.mark.parametrize('results', ['in place', 'copies'])
+@pytest.mark.parametrize('usual', [True, False])
+def test_clipped_tensors_are_marked_as_changed(K, usual, results):
+    """As every operation in place does, for autograd to notice; the norm alone changes nothing.  ``usual``: the call in one step."""
+    grads = gradients([(30, 40), (7,), (64, 3, 5, 5)], 1)
+    if not usual:
+        grads.append(rand(20, 30, seed=2)[:, ::2])
+    outs = None if results == 'in place' else [torch.empty_like(g) for g in grads]
+    changed = grads if outs is None else outs
+    before = [t._version for t in changed]
+    K.grad_norm(grads)
+    assert [t._version for t in changed] == before
+    K.clip_grad_norm(grads, 0.5, outs=outs)
+    assert all(t._version > v for t, v in zip(changed, before))
+    if outs is not None:
+        assert all(g._version == 0 for g in grads)
+    # a graph that keeps one of them
+    x = torch.ones_like(changed[0]).requires_grad_()
+    loss = (x * changed[0]).sum()
+    K.clip_grad_norm(grads, 0.25, outs=outs)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    with torch.inference_mode():
+        made = gradients([(30, 40), (7,), (64, 3, 5, 5)], 3)
+        want = K.clip_grad_norm(made, 0.5)
+    assert abs(norm_of(made, 2) - 0.5) < 1e-5 and float(want) > 0.5
+    K.clip_grad_norm(made, 0.25)                   # (such tensors keep no count)
+    assert abs(norm_of(made, 2) - 0.25) < 1e-5
