@@ -852,3 +852,30 @@ def test_clipped_tensors_are_marked_as_changed(K, usual, results):
     assert abs(norm_of(made, 2) - 0.5) < 1e-5 and float(want) > 0.5
     K.clip_grad_norm(made, 0.25)                   # (such tensors keep no count)
     assert abs(norm_of(made, 2) - 0.25) < 1e-5
+
+
+@pytest.mark.parametrize('rows,F', [(1, 16), (257, 100), (300, 768), (19, 2050), (6, 8191), (3, 16400)])
+@pytest.mark.parametrize('xt', [F32, BF16, F16])
+def test_symmetric_fisher_blocks_stay_symmetric(K, rows, F, xt):
+    """To the bit: both cross terms are one sum.  Block by block against the definition: each term is an fp32 sum in chains of at most 256
+    products, joined by at most 64 more, each addition off by u of the sum of magnitudes; h is off by 64 u of what it is a difference of
+    (twice in its square) and the products' own roundings stay below another 64 u."""
+    x, g, w = rand(rows, F, seed=1, dtype=xt, scale=2.0, shift=0.5), rand(rows, F, seed=2, dtype=xt), rand(F, seed=3)
+    _, mean, rstd = K.layer_norm(x, w)
+    h = norm64(x, w, None, 1e-5)[3]
+    g64 = g.double()
+    size = h.abs() + 1 + x.double().abs() * rstd.double().unsqueeze(-1)
+    terms = torch.stack([(g64 * h).square().sum(0), (g64 * g64 * h).sum(0), (g64 * g64).sum(0)], -1)
+    sizes = torch.stack([(g64 * size).square().sum(0), (g64 * g64 * size).sum(0), (g64 * g64).sum(0)], -1)
+    blocks = rand(F, 2, 2, seed=5)
+    blocks[:, 1, 0] = blocks[:, 0, 1]
+    first = blocks.clone()
+    for beta in (0.5, 0.0):
+        before = first.double() if beta else torch.zeros_like(first, dtype=torch.float64)
+        blocks.copy_(first)
+        K.layer_norm_backward(g, x, mean, rstd, w, blocks=blocks, alpha=0.25, beta=beta)
+        assert torch.equal(blocks[:, 0, 1], blocks[:, 1, 0])
+        for at, q in (((0, 0), 0), ((0, 1), 1), ((1, 1), 2)):
+            old = before[:, at[0], at[1]]
+            want, most = beta * old + 0.25 * terms[:, q], beta * old.abs() + 0.25 * sizes[:, q]
+            assert bool(((blocks[:, at[0], at[1]].double() - want).abs() <= (min(rows, 256) + 3 * 64 + 64) * U * most).all()), (beta, at)
