@@ -5,7 +5,6 @@ that pass reads anyway, where torch.nn.LayerNorm has its output and output gradi
 (asdl/operations/layernorm.py:69-78)."""
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -62,9 +61,14 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        saved = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            x, weight, _, _ = saved = ctx.saved_tensors
+            return _Once.apply(ctx, saved, g, x, weight) + (None, None)
+        return _LayerNorm.gradients(ctx, ctx.saved_tensors, g) + (None, None)
+
+    @staticmethod
+    def gradients(ctx, saved, g):
         x, weight, mean, rstd = saved
         blocks, alpha, beta = None, 1.0, 0.0
         for request in list(ctx.blocks_requests):         # (one for each set of hooks on the module)
@@ -74,9 +78,21 @@ class _LayerNorm(torch.autograd.Function):
             else:
                 request.settle(saved)
         need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
-        dx, dw, db = kernels.layer_norm_backward(g, x, mean, rstd, weight, blocks, alpha, beta, need_x, need_weight, need_bias,
-                                                 weight_dtype=ctx.weight_dtype)
-        return dx, dw, db, None, None
+        return kernels.layer_norm_backward(g, x, mean, rstd, weight, blocks, alpha, beta, need_x, need_weight, need_bias,
+                                           weight_dtype=ctx.weight_dtype)
+
+
+class _Once(torch.autograd.Function):
+    """The gradients of _LayerNorm in a graph of their own, which has no way back.  (torch's once_differentiable() ends the graph at the
+    gradients: a second derivative with respect to x is None or 0 then, where the pass does not come across the end.)"""
+
+    @staticmethod
+    def forward(ctx, node, saved, g, x, weight):
+        return _LayerNorm.gradients(node, saved, g)
+
+    @staticmethod
+    def backward(ctx, *gradients):
+        raise RuntimeError('layer_norm() is differentiable once (once_differentiable): it has no second derivative.')
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):

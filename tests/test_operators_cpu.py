@@ -546,3 +546,27 @@ def test_filters_with_replaced_targets_are_refused(filters, how, monkeypatch):
             assert not ran
         else:
             maker.forward_and_backward()
+
+
+@pytest.mark.parametrize('loss', ['cubes', 'linear'])
+def test_a_second_derivative_of_layer_norm_raises(loss, monkeypatch):
+    """However it is asked for: a graph that ends at the gradient would give zeros."""
+    _stand_ins(monkeypatch)
+    torch.manual_seed(6)
+    ln, x, c = FusedLayerNorm(6), torch.randn(5, 6), torch.randn(5, 6)
+
+    def f(x):
+        return (ln(x) ** 3).sum() if loss == 'cubes' else (ln(x) * c).sum()
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        torch.autograd.functional.hessian(f, x)
+    x.requires_grad_()
+    for ask in (lambda dx: torch.autograd.grad(dx.square().sum(), x, allow_unused=True), lambda dx: dx.square().sum().backward(),
+                lambda dx: torch.autograd.grad(dx.square().sum(), ln.weight, allow_unused=True)):
+        (dx,) = torch.autograd.grad(f(x), x, create_graph=True)
+        with pytest.raises(RuntimeError, match='differentiable once'):
+            ask(dx)
+    (dx, db) = torch.autograd.grad(f(x), (x, ln.bias), create_graph=True)
+    (want,) = torch.autograd.grad(f(x), x)
+    assert torch.equal(dx.detach(), want) and db.shape == (6,)
+    plain = nn.LayerNorm(6)
+    assert torch.allclose(want, torch.autograd.grad((plain(x) ** 3).sum() if loss == 'cubes' else (plain(x) * c).sum(), x)[0], rtol=1e-4, atol=1e-5)
