@@ -6,7 +6,8 @@
 // h = 0 whatever their size), and the variance is the mean of centred squares, no difference of large sums.  Everything is fp32,
 // rounded when it is stored.
 // Each way reads its operands once and writes its result once.  8192 rows of 768 fp32 features with Fisher blocks: 10.9 us forward
-// (50 MB, 4.6 TB/s), 16.3 us backward (75 MB, 4.6 TB/s) and 3.9 us for the sums of the partial rows; 16384 rows of 4096 bfloat16 ones: 130 us
+// (50 MB, 4.6 TB/s), 16.3 us backward (75 MB, 4.6 TB/s) and 3.9 us for the sums of the partial rows, bfloat16 ones with half the bytes 8.4 us
+// forward and 15.7 us for both launches backward (14.7 without the blocks), which is not the memory's time; 16384 rows of 4096 bfloat16 ones: 130 us
 // both ways (671 MB, 5.2 TB/s, the rate of a large copy).  A few rows cost the launch, 5 to 6 us a call.
 #include "elements.hpp"
 
@@ -74,6 +75,8 @@ struct LnSlice {
   }
 };
 
+// The type of the weights is a template parameter, not a branch on a code: such a branch inside the per-lane conditions of load() left the
+// register pair of the lane's column offset undefined on one of its ways, and the addresses made from it faulted.
 template <typename W, int V, typename Layout>
 __device__ __forceinline__ void ln_vector(const Layout& at, const void* p, float none, float (&out)[Layout::N]) {
   if (p == nullptr) {
@@ -254,7 +257,8 @@ static __global__ __launch_bounds__(THREADS) void ln_backward_fused_kernel(LnBac
   }
 }
 
-// Rows of more than 8192 features: one work group per row, which is read four times, from the caches but for the first.
+// Rows of more than 8192 features: one work group per row, which is read four times, from the caches but for the first, an element a
+// load.  4096 rows of 16384 bfloat16 features: 214 us forward, 246 us backward (1.3 and 1.6 TB/s); 2048 of fp32 ones: 119 and 172 us.
 template <typename X, typename Y, typename W>
 static __global__ __launch_bounds__(256) void ln_forward_kernel(LnForward p) {
   __shared__ float red[4];

@@ -278,11 +278,12 @@ struct SfRow {
 // border lies.  Where the classes up to this bin are at most kSfListed, the next pass lists them in the LDS, and the draw is among them.
 // With top-p alone a pass adds the classes' weights to bins, about, and says where the border will be, and one with exact weights sums
 // those in front of it by cells (a step of a wave), lists those about it and finds it among them; the draw is in the cell at which the
-// sums pass the number.  Without either that pass sums all.  Where a list does not hold the classes of a border's bin (thousands of equal
+// sums pass the number.  Where min-p seems to decide before top-p does, a pass sums what it keeps and all, exactly; if these sums say so,
+// the draw is among those, else top-p's pass follows.  Without top-k and top-p one pass sums all.  Where a list does not hold the classes of a border's bin (thousands of equal
 // or nearly equal ones), the border is narrowed by bins of their keys to a class.
-// What bounds it: 4096 rows of 50257 fp32 classes (823 MB; 161 us to read them once at the rate of a large copy) take 242 us with T = 0 and
-// 260 with top-k 40 (two reads, 6.3 TB/s), 362 without filters and 460 with top-p 0.9, of which 80% are vector instructions, 66 a class, most
-// of them for the exact weights.  8 rows take 10 us with T = 0, 22 with top-k 40 and 42 with top-p 0.9: one CU a row and the barriers
+// What bounds it: 4096 rows of 50257 fp32 classes (823 MB; 161 us to read them once at the rate of a large copy; normal logits of deviation
+// 2) take 241 us with T = 0 and 258 with top-k 40 (two reads, 6.4 TB/s), 326 without filters, 322 with min-p 0.05, 426 with top-p 0.9 and
+// min-p 0.05, and 450 with top-p 0.9, of which 80% are vector instructions, 66 a class, most of them for the exact weights.  8 rows take 10 us with T = 0, 22 with top-k 40 and 42 with top-p 0.9: one CU a row and the barriers
 // between the passes.
 template <typename T, int NT>
 static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
@@ -762,7 +763,7 @@ static __global__ __launch_bounds__(NT, 4) void sf_row_kernel(SfParams p) {
       for (int q = 0; q < PER_BINS; ++q)
         sum_of += own[q] = static_cast<double>(sums[tid * PER_BINS + q]) * static_cast<double>(exp2f(-drop * static_cast<float>(tid * PER_BINS + q)));
       sf_scan<WAVES>(sum_of, sh.red_double, before, total);
-      // Where min-p seems to keep less than top-p would, its classes are summed at once (256 requests with filters of their own: 56 us for
+      // Where min-p seems to keep less than top-p would, its classes are summed at once (256 requests with filters of their own: 55 us for
       // 69).  These sums are estimates, whose error grows with |logit| / T (the product with a is rounded) and with the number of classes
       // (unit); 1e-3 is a margin that usually does.  What they say is proved below, as the border's bins are.
       const int least_bin = filter.m > 0. ? bin_of(top + static_cast<float>(filter.t) * __log2f(static_cast<float>(filter.m)) * 0.693147f) + 1 : kSfBins;

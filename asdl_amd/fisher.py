@@ -67,7 +67,8 @@ class FisherConfig:
     is_master: bool = True
     ignore_index: int = -1
     # what the sampled Fisher draws its targets from: the model's predictive distribution at this temperature, restricted to its
-    # likely classes (kernels.sample_filtered); the defaults are the distribution itself
+    # likely classes (kernels.sample_filtered); the defaults are the distribution itself.  With a filter the matrix is the second moment
+    # of the gradients for targets so drawn, and no longer an estimate of the model's Fisher matrix.  Not with sample_targets() overridden
     mc_temperature: float = 1.
     mc_top_k: int = None
     mc_top_p: float = None

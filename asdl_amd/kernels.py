@@ -1607,7 +1607,8 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, outs=None):
     """Scales ``grads`` in place by min(1, max_norm / (norm + 1e-6)) and returns their norm before, as grad_norm() gives it; with ``outs``
     the gradients stay and the scaled values go to these tensors (of as many elements in the same order, and of the gradient's type or
     float32).  A norm that is infinite gives the factor 0, one that is NaN the factor NaN, as torch.nn.utils.clip_grad_norm_ does.
-    Gradients (results) of different entries may not overlap, except that one listed twice is scaled once.  Nothing is read by the host."""
+    Gradients (results) of different entries may not overlap, except that one listed twice is scaled once.  Nothing is read by the host.
+    What is written counts as changed in place for autograd."""
     grads, norm_type = _norm_arguments(grads, norm_type)
     if not max_norm >= 0:
         raise ValueError(f'max_norm has to be at least 0. Got {max_norm}.')

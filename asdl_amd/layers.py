@@ -97,7 +97,8 @@ class _Once(torch.autograd.Function):
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     """torch.nn.functional.layer_norm for tensors on a ROCm device (float32, bfloat16 or float16; weight and bias of the type of x or
-    float32), differentiable once.  Under autocast the result is float32, as there, and x is read as it is."""
+    float32), differentiable once: a second derivative raises.  Under autocast the result is float32, as there, and x is read as it is.
+    Not taken, where torch's takes them: tensors on the CPU, float64, forward mode, and torch.func (grad, vmap and their kin); each raises."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     if not shape or tuple(x.shape[-len(shape):]) != shape:
         raise ValueError(f'x has to end in the dimensions {shape}. Got the shape {tuple(x.shape)}.')
@@ -117,7 +118,7 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
 
 
 class FusedLayerNorm(nn.LayerNorm):
-    """torch.nn.LayerNorm (the same arguments, parameters and state dict) on layer_norm() above."""
+    """torch.nn.LayerNorm (the same arguments, parameters and state dict) on layer_norm() above, which says what it does not take."""
 
     def forward(self, input):
         return layer_norm(input, self.normalized_shape, self.weight, self.bias, self.eps)
@@ -125,7 +126,7 @@ class FusedLayerNorm(nn.LayerNorm):
 
 def fuse_layer_norms(model: nn.Module) -> int:
     """Makes every torch.nn.LayerNorm of ``model`` (not subclasses of it) a FusedLayerNorm, in place: parameters, hooks and names stay.
-    Returns how many there were."""
+    Returns how many there were.  The model then runs on a ROCm device only, in float32, bfloat16 or float16 (see layer_norm())."""
     found = [m for m in model.modules() if type(m) is nn.LayerNorm]
     for m in found:
         m.__class__ = FusedLayerNorm

@@ -586,7 +586,8 @@ class KfacGradientMaker(NaturalGradientMaker):
     BatchNorm1d/2d and LayerNorm modules get the unit-wise shape, as in the reference; ``swift=True`` keeps the
     factors of layers that see fewer samples than they have columns as row matrices (SKFAC).  Embedding modules
     have no kernels in this build (exclude them through ``config.ignore_modules``).  ``mc_temperature``, ``mc_top_k``, ``mc_top_p``,
-    ``mc_min_p``: FISHER_MC draws its targets from the predictive distribution so restricted (kernels.sample_filtered)."""
+    ``mc_min_p``: FISHER_MC draws its targets from the predictive distribution so restricted (kernels.sample_filtered); the curvature is
+    then that of these targets, not an estimate of the model's Fisher matrix."""
 
     def __init__(self, model, config: PreconditioningConfig, fisher_type: str = FISHER_MC,
                  loss_type: str = LOSS_CROSS_ENTROPY, scale: float = 1, grad_scale: float = 1, n_mc_samples: int = 1,
