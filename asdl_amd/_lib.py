@@ -74,6 +74,19 @@ _SIGNATURES = {
     'ak_grad_norm_ws_bytes': (c_size, [c_int]),
     'ak_grad_norm': (c_int, [c_ptr, c_int, c_int, c_ptr, c_ptr, c_size, c_ptr]),
     'ak_clip_grad_norm': (c_int, [c_ptr, c_int, c_int, c_f64, c_ptr, c_ptr, c_size, c_ptr]),
+    'ak_linear_cross_entropy_ws_bytes': (c_size, [c_int, c_i64, c_i64, c_i64, c_int]),
+    'ak_linear_cross_entropy': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_i64, c_ptr, c_int, c_ptr, c_i64, c_i64, c_i64, c_i64, c_int, c_ptr,
+                                        c_ptr, c_ptr, c_size, c_ptr]),
+    'ak_linear_cross_entropy_backward': (c_int, [c_ptr, c_ptr, c_int, c_i64, c_ptr, c_i64, c_ptr, c_int, c_ptr, c_ptr, c_i64, c_i64, c_i64,
+                                                 c_i64, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
+    'ak_embedding': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_int, c_i64, c_i64, c_i64, c_f32, c_ptr, c_int, c_ptr]),
+    'ak_embedding_backward_ws_bytes': (c_size, [c_i64, c_i64, c_i64]),
+    'ak_embedding_backward': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_int, c_i64, c_i64, c_i64, c_f32, c_i64, c_f32, c_ptr, c_int, c_i64,
+                                      c_ptr, c_size, c_ptr]),
+    'ak_quantize_8bit': (c_int, [c_ptr, c_int, c_i64, c_i64, c_i64, c_int, c_ptr, c_ptr, c_ptr, c_ptr]),
+    'ak_dequantize_8bit': (c_int, [c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr, c_i64, c_ptr, c_int, c_ptr]),
+    'ak_weight_grad_8bit_ws_bytes': (c_size, [c_int, c_i64, c_i64, c_i64]),
+    'ak_weight_grad_8bit': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_int, c_ptr, c_size, c_ptr]),
     'ak_event_synchronize': (c_int, [c_ptr]),
     'ak_kron_finish': (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_int, c_ptr, c_ptr]),
     'ak_kron_precond_deep_ws_bytes': (c_size, [c_ptr, c_int]),

@@ -1,0 +1,421 @@
+// Rows of a table by token, times a factor, and the gradient of the table:
+//   y_n = c E[t(n)],   dE[v] = beta dE[v] + c * (sum of g_n over n with t(n) = v, in ascending order of n)
+// The gradient goes by tokens in sorted order, so that every row of it is written once and no addition depends on the order in which work
+// groups run (atomics on the 3 KB rows of a frequent token would also wait for each other: a twentieth of a text is its commonest token).
+//   sort:   a work group per range of rows; it reads all tokens, counts those in front of its range and those of each row, and puts the
+//           positions of its own in order (a stable counting sort without a word between work groups)
+//   sums:   a wave per chunk of sorted positions and 1 KB of columns; runs of equal tokens inside a chunk are written, parts of runs that
+//           cross its ends go to the workspace; other waves write the rows that no token names
+//   joins:  the parts of a run, in order
+// Bound by the memory: the gradients are read once, the table's gradient is written once.
+#include <algorithm>
+#include "elements.hpp"
+
+namespace ak {
+
+constexpr int kEmbBins = 512, kEmbWaves = 16;        // rows of a range at most, waves of a sorting work group
+
+template <typename I>
+struct Tokens {
+  const I* p;
+  int64_t count;
+  int rows;
+  int64_t padding;         // a token that takes no gradient; -1: none
+  __device__ __forceinline__ int64_t at(int64_t n) const { return static_cast<int64_t>(p[n]); }
+  // (positions behind the last, tokens that name no row and the padding: -1)
+  __device__ __forceinline__ int named(int64_t n) const {
+    if (n >= count) return -1;
+    const int64_t t = at(n);
+    return t >= 0 && t < rows && t != padding ? static_cast<int>(t) : -1;
+  }
+};
+
+// L lanes copy a row, V elements (16 bytes) at a time.
+template <typename T, typename O, typename I, int L>
+static __global__ __launch_bounds__(256) void emb_rows_kernel(Tokens<I> t, const T* __restrict__ table, int64_t ld, int D, float scale, O* __restrict__ out) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+  if (n >= t.count) return;
+  const int64_t token = t.at(n);
+  O* __restrict__ to = out + n * D;
+  if (token < 0 || token >= t.rows) {
+    for (int c = threadIdx.x % L; c < D; c += L) to[c] = static_cast<O>(NAN);
+    return;
+  }
+  const T* __restrict__ from = table + token * ld;
+  const int whole = D / V * V;
+#pragma unroll 4
+  for (int c = (threadIdx.x % L) * V; c < whole; c += L * V) {
+    Some<T, V> v;
+    Some<O, V> o;
+    v.load(from + c);
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.set(e, v.get(e) * scale);
+    o.store(to + c);
+  }
+  const int c = whole + threadIdx.x % L;
+  if (c < D && threadIdx.x % L < V) to[c] = static_cast<O>(static_cast<float>(from[c]) * scale);
+}
+
+// starts[v]: first sorted position of row v's tokens; order, sorted: position in the text and token of each.  Work group b: rows
+// b * bins .. of the table.  Every wave goes through a part of the text of its own, twice.
+template <typename I>
+static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(Tokens<I> t, int bins, int* __restrict__ starts, int* __restrict__ order,
+                                                                         int* __restrict__ sorted) {
+  __shared__ int count[kEmbWaves][kEmbBins];
+  __shared__ int sums[kEmbWaves], below_of[kEmbWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int v0 = blockIdx.x * bins, v1 = min(v0 + bins, t.rows);
+  for (int i = threadIdx.x; i < kEmbWaves * kEmbBins; i += 64 * kEmbWaves) (&count[0][0])[i] = 0;
+  __syncthreads();
+  const int64_t part = (t.count + 64 * kEmbWaves - 1) / (64 * kEmbWaves) * 64, n0 = wave * part, n1 = n0 + part < t.count ? n0 + part : t.count;
+  int below = 0;
+  constexpr int U = 8;
+  for (int64_t n = n0; n < n1; n += 64 * U) {
+    int v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = n + 64 * u < n1 ? t.named(n + 64 * u + lane) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      below += v[u] >= 0 && v[u] < v0 ? 1 : 0;
+      if (v[u] >= v0 && v[u] < v1) atomicAdd(&count[wave][v[u] - v0], 1);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o);
+  if (lane == 0) below_of[wave] = below;
+  __syncthreads();
+  // thread i < kEmbBins: row v0 + i; positions of the waves' tokens of that row from the exclusive sums over rows and waves
+  int mine = 0;
+  if (threadIdx.x < kEmbBins) {
+#pragma unroll
+    for (int w = 0; w < kEmbWaves; ++w) mine += count[w][threadIdx.x];
+  }
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  int at = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kEmbWaves; ++w) {
+    at += below_of[w];
+    if (w < wave) at += sums[w];
+  }
+  if (threadIdx.x < kEmbBins) {
+    const int v = v0 + threadIdx.x;
+    if (v < v1) {
+      starts[v] = at;
+      if (v == t.rows - 1) starts[t.rows] = at + mine;
+    }
+#pragma unroll
+    for (int w = 0; w < kEmbWaves; ++w) {
+      const int c = count[w][threadIdx.x];
+      count[w][threadIdx.x] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  volatile int* next = count[wave];
+  for (int64_t n = n0; n < n1; n += 64 * U) {
+    int v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = n + 64 * u < n1 ? t.named(n + 64 * u + lane) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = v[u] >= v0 && v[u] < v1;
+      u64 left = __ballot(in);
+      while (left != 0) {                      // the tokens among these 64 one by one, all of a kind at once
+        const int first = __builtin_ctzll(left);
+        const int token = __builtin_amdgcn_readlane(v[u], first);
+        const u64 same = __ballot(in && v[u] == token);
+        const int base = next[token - v0];
+        if (in && v[u] == token) {
+          const int to = base + __popcll(same & ((1ull << lane) - 1));
+          order[to] = static_cast<int>(n + 64 * u + lane);
+          sorted[to] = token;
+        }
+        next[token - v0] = base + __popcll(same);      // (every lane the same)
+        left &= ~same;
+      }
+    }
+  }
+}
+
+struct EmbSums {
+  const int *starts, *order, *sorted;
+  const void* g;
+  void* out;
+  float *lead, *trail;     // [chunks][ldp] parts of runs that began in front of a chunk; that begin in it and go on behind it
+  int64_t ldg, ldo, ldp;
+  int rows, D, chunk, chunks, slabs, row_groups;
+  float scale, beta;
+};
+
+// out <- beta*out + scale*sum, one lane's E columns from c on
+template <typename O, int E>
+__device__ __forceinline__ void emb_write(const EmbSums& p, int row, int c, const float (&sum)[E]) {
+  O* __restrict__ to = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.ldo + c;
+  if (c + E <= p.D) {
+    Some<O, E> o;
+    if (p.beta != 0.f) {
+      o.load(to);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.set(e, p.beta * o.get(e) + p.scale * sum[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.set(e, p.scale * sum[e]);
+    }
+    o.store(to);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (c + e < p.D) to[e] = static_cast<O>(p.beta != 0.f ? p.beta * static_cast<float>(to[e]) + p.scale * sum[e] : p.scale * sum[e]);
+  }
+}
+
+template <typename G, typename O>
+static __global__ __launch_bounds__(256) void emb_sums_kernel(EmbSums p) {
+  constexpr int E = 16 / sizeof(G), U = 8;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t units = static_cast<int64_t>(p.chunks) * p.slabs;
+  if (unit >= units) {
+    // 64 rows: those without a token
+    const int64_t v0 = (unit - units) * 64;
+    if (v0 >= p.rows) return;
+    const int64_t v = v0 + lane;
+    u64 none = __ballot(v < p.rows && p.starts[v < p.rows ? v : 0] == p.starts[v < p.rows ? v + 1 : 0]);
+    if (p.beta == 1.f) return;
+    const float zero[E] = {};
+    while (none != 0) {
+      const int row = static_cast<int>(v0) + __builtin_ctzll(none);
+      for (int c = lane * E; c < p.D; c += 64 * E) emb_write<O, E>(p, row, c, zero);
+      none &= none - 1;
+    }
+    return;
+  }
+  const int chunk = static_cast<int>(unit / p.slabs), slab = static_cast<int>(unit - static_cast<int64_t>(chunk) * p.slabs);
+  const int total = p.starts[p.rows];
+  const int p0 = chunk * p.chunk, p1 = min(p0 + p.chunk, total);
+  if (p0 >= p1) return;
+  const int c = slab * 64 * E + lane * E;
+  const bool has = c < p.D, full = c + E <= p.D;
+  const int my_row = p0 + lane < p1 ? p.order[p0 + lane] : 0;
+  const int my_token = p0 + lane < p1 ? p.sorted[p0 + lane] : -1;
+  const int before = p0 > 0 ? p.sorted[p0 - 1] : -1, behind = p1 < total ? p.sorted[p1] : -1;
+  float sum[E] = {};
+  auto flush = [&](int token, bool first, bool last) {
+    if (!has) return;
+    const bool from = first && token == before, on = last && token == behind;
+    if (!from && !on) {
+      emb_write<O, E>(p, token, c, sum);
+      return;
+    }
+    float* __restrict__ to = (from ? p.lead : p.trail) + chunk * p.ldp + c;       // (ldp holds whole vectors)
+#pragma unroll
+    for (int e = 0; e < E; ++e) to[e] = sum[e];
+  };
+  int token = __builtin_amdgcn_readlane(my_token, 0);
+  bool first = true;
+  for (int i = 0; i < p1 - p0; i += U) {
+    Some<G, E> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].clear();
+      if (i + u < p1 - p0) {
+        const G* __restrict__ from = static_cast<const G*>(p.g) + static_cast<int64_t>(__builtin_amdgcn_readlane(my_row, i + u)) * p.ldg + c;
+        if (full) {
+          v[u].load(from);
+        } else if (has) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (c + e < p.D) v[u].v[e] = from[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= p1 - p0) continue;
+      const int next = __builtin_amdgcn_readlane(my_token, i + u);
+      if (next != token) {
+        flush(token, first, false);
+        first = false;
+        token = next;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] += v[u].get(e);
+    }
+  }
+  flush(token, first, true);
+}
+
+// The run that begins in a chunk and ends in a later one; four waves take a part of the chunks each, 256 columns a work group.
+template <typename O>
+static __global__ __launch_bounds__(256) void emb_joins_kernel(EmbSums p) {
+  __shared__ floatx4 joined[4][64];
+  const int chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int total = p.starts[p.rows], p0 = chunk * p.chunk, p1 = p0 + p.chunk;
+  if (p1 >= total) return;
+  const int token = p.sorted[p1 - 1];
+  const int s0 = p.starts[token], s1 = p.starts[token + 1];
+  if (s0 < p0 || s1 <= p1) return;             // begins in front of this chunk, ends with it
+  const int last = (s1 - 1) / p.chunk, parts = last - chunk + 1, per = (parts + 3) / 4;
+  const int c = blockIdx.y * 256 + 4 * lane;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (c < p.D) {
+    const int k1 = min((wave + 1) * per, parts);
+#pragma unroll 8
+    for (int k = wave * per; k < k1; ++k)
+      sum += *reinterpret_cast<const floatx4*>((k == 0 ? p.trail : p.lead) + static_cast<int64_t>(chunk + k) * p.ldp + c);
+  }
+  joined[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || c >= p.D) return;
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ((joined[0][lane][e] + joined[1][lane][e]) + joined[2][lane][e]) + joined[3][lane][e];
+  emb_write<O, 4>(p, token, c, v);
+}
+
+// Sorted positions of a chunk: enough chunks for 32 waves a CU, few enough for little to be joined.
+inline int emb_chunk(int64_t tokens, int64_t D, int elements) {
+  const int64_t slabs = (D + 64 * elements - 1) / (64 * elements), want = tokens * slabs / 8192;
+  return want <= 8 ? 8 : want <= 16 ? 16 : want <= 32 ? 32 : 64;
+}
+
+template <typename F>
+inline int with_tokens(int type, F&& f) {
+  switch (type) {
+    case AK_I64: return f(Type<int64_t>{});
+    case AK_I32: return f(Type<int32_t>{});
+    default: return AK_ERR_ARG;
+  }
+}
+
+struct EmbSpace {
+  int *starts, *order, *sorted;
+  float *lead, *trail;
+  int chunk, chunks;
+  int64_t ldp;
+  size_t bytes;
+};
+
+inline EmbSpace emb_space(int64_t tokens, int64_t rows, int64_t D, int elements, void* ws) {
+  unsigned char* base = static_cast<unsigned char*>(ws);
+  size_t used = 0;
+  auto take = [&](int64_t words) {
+    void* at = base != nullptr ? base + used : nullptr;
+    used += static_cast<size_t>((words * 4 + 255) / 256 * 256);
+    return at;
+  };
+  EmbSpace s;
+  s.chunk = emb_chunk(tokens, D, elements);
+  s.chunks = static_cast<int>((tokens + s.chunk - 1) / s.chunk);
+  s.ldp = (D + 7) / 8 * 8;
+  s.starts = static_cast<int*>(take(rows + 1));
+  s.order = static_cast<int*>(take(tokens));
+  s.sorted = static_cast<int*>(take(tokens));
+  s.lead = static_cast<float*>(take(s.chunks * s.ldp));
+  s.trail = static_cast<float*>(take(s.chunks * s.ldp));
+  s.bytes = used;
+  return s;
+}
+
+inline int emb_check(int token_type, int64_t tokens, int64_t rows, int64_t D, int64_t ld) {
+  if ((token_type != AK_I64 && token_type != AK_I32) || tokens < 0 || rows < 0 || D <= 0 || ld < D) return AK_ERR_ARG;
+  if (tokens > (1ll << 30) || rows > (1ll << 30) || D > (1ll << 24)) return AK_ERR_TOO_LARGE;
+  return AK_OK;
+}
+
+}  // namespace ak
+
+extern "C" int ak_embedding(const void* tokens, int token_type, int64_t count, const void* table, int dtype, int64_t ld, int64_t rows, int64_t width,
+                            float scale, void* out, int out_dtype, ak_stream_t stream) {
+  using namespace ak;
+  const int rc = emb_check(token_type, count, rows, width, ld);
+  if (rc != AK_OK) return rc;
+  if (!is_element_type(dtype) || (out_dtype != dtype && out_dtype != AK_F32)) return AK_ERR_ARG;
+  if (count == 0) return AK_OK;
+  if (tokens == nullptr || out == nullptr || (table == nullptr && rows > 0)) return AK_ERR_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return with_type(dtype, [&](auto t) {
+    using T = typename decltype(t)::type;
+    auto go = [&](auto o) {
+      using O = typename decltype(o)::type;
+      return with_tokens(token_type, [&](auto i) {
+        using I = typename decltype(i)::type;
+        const Tokens<I> tk{static_cast<const I*>(tokens), count, static_cast<int>(rows), -1};
+        auto launch = [&](auto lanes) {
+          constexpr int L = decltype(lanes)::value;
+          hipLaunchKernelGGL((emb_rows_kernel<T, O, I, L>), dim3(static_cast<unsigned>((count + 256 / L - 1) / (256 / L))), dim3(256), 0, s, tk,
+                             static_cast<const T*>(table), ld, static_cast<int>(width), scale, static_cast<O*>(out));
+          return check_launch();
+        };
+        // as many lanes as a row has vectors, 8 to 64
+        const int64_t vectors = (width + 16 / static_cast<int64_t>(sizeof(T)) - 1) / (16 / static_cast<int64_t>(sizeof(T)));
+        return vectors <= 8 ? launch(std::integral_constant<int, 8>{}) : vectors <= 32 ? launch(std::integral_constant<int, 32>{})
+                                                                                       : launch(std::integral_constant<int, 64>{});
+      });
+    };
+    if (out_dtype == dtype) return go(t);
+    return go(Type<float>{});
+  });
+}
+
+extern "C" size_t ak_embedding_backward_ws_bytes(int64_t count, int64_t rows, int64_t width) {
+  if (count < 0 || rows < 0 || width <= 0 || count > (1ll << 30) || rows > (1ll << 30) || width > (1ll << 24)) return 0;
+  return std::max(ak::emb_space(count, rows, width, 4, nullptr).bytes, ak::emb_space(count, rows, width, 8, nullptr).bytes);
+}
+
+extern "C" int ak_embedding_backward(const void* g, int dtype, int64_t ldg, const void* tokens, int token_type, int64_t count, int64_t rows,
+                                     int64_t width, float scale, int64_t padding, float beta, void* out, int out_dtype, int64_t ldo, void* ws,
+                                     size_t ws_bytes, ak_stream_t stream) {
+  using namespace ak;
+  int rc = emb_check(token_type, count, rows, width, ldo);
+  if (rc != AK_OK) return rc;
+  if (!is_element_type(dtype) || !is_element_type(out_dtype) || ldg < width) return AK_ERR_ARG;
+  if (rows == 0) return AK_OK;
+  if (out == nullptr || (count > 0 && (g == nullptr || tokens == nullptr))) return AK_ERR_ARG;
+  if (ws == nullptr || ws_bytes < ak_embedding_backward_ws_bytes(count, rows, width)) return AK_ERR_WORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int elements = dtype == AK_F32 ? 4 : 8;
+  const EmbSpace s = emb_space(count, rows, width, elements, ws);
+  rc = with_tokens(token_type, [&](auto i) {
+    using I = typename decltype(i)::type;
+    const Tokens<I> tk{static_cast<const I*>(tokens), count, static_cast<int>(rows), padding};
+    // 256 ranges where they hold the table
+    const int64_t bins = std::min<int64_t>((rows + 255) / 256, kEmbBins);
+    hipLaunchKernelGGL(emb_sort_kernel<I>, dim3(static_cast<unsigned>((rows + bins - 1) / bins)), dim3(64 * kEmbWaves), 0, st, tk, static_cast<int>(bins),
+                       s.starts, s.order, s.sorted);
+    return check_launch();
+  });
+  if (rc != AK_OK) return rc;
+  EmbSums p;
+  p.starts = s.starts; p.order = s.order; p.sorted = s.sorted;
+  p.g = g; p.out = out; p.lead = s.lead; p.trail = s.trail;
+  p.ldg = ldg; p.ldo = ldo; p.ldp = s.ldp;
+  p.rows = static_cast<int>(rows); p.D = static_cast<int>(width);
+  p.chunk = s.chunk; p.chunks = s.chunks;
+  p.slabs = static_cast<int>((width + 64 * elements - 1) / (64 * elements));
+  p.row_groups = static_cast<int>((rows + 63) / 64);
+  p.scale = scale; p.beta = beta;
+  const int64_t units = static_cast<int64_t>(p.chunks) * p.slabs + p.row_groups;
+  if ((units + 3) / 4 > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  return with_type(out_dtype, [&](auto o) {
+    using O = typename decltype(o)::type;
+    const int done = with_type(dtype, [&](auto t) {
+      using G = typename decltype(t)::type;
+      hipLaunchKernelGGL((emb_sums_kernel<G, O>), dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, st, p);
+      return check_launch();
+    });
+    if (done != AK_OK || p.chunks < 2) return done;
+    hipLaunchKernelGGL(emb_joins_kernel<O>, dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>((width + 255) / 256)), dim3(256), 0, st, p);
+    return check_launch();
+  });
+}

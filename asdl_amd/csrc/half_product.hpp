@@ -1,0 +1,410 @@
+// Products of 16-bit matrices (bf16 or fp16, fp32 sums) on the matrix cores, for operators whose epilogue is their own:
+//   D[i][j] = sum_k A[i][k] B[k][j]
+// Either operand lies in memory with its contraction index along the rows ("by k": row i or j holds its k values) or across them ("by
+// row": row k holds all i or j).  A work group has one BI x BJ tile of D; a lane of a wave has, for every 32 x 32 block, one column j and
+// 16 rows i, four of them consecutive: an epilogue that writes D transposed writes four neighbouring elements, one that reduces over i
+// stays in the lane.
+// Panels of 32 k go from memory to the LDS without passing registers (syrk_dtl_tile.hpp: load_to_lds), kHpStages of them in flight.  Both
+// kinds of panel are blocks of 2 KB, 32 rows of 64 bytes:
+//   by k:   [32 i][32 k], 16-byte chunks of a row exchanged by (row / 4) % 4, so that the 16 rows a ds_read_b128 serves at once lie in
+//           different banks; the exchange is made on the memory side of the load, within the 64 bytes of a row
+//   by row: [32 k][32 i], read by ds_read_b64_tr_b16
+// The base of an operand's descriptor moves with the k-tile (scalar arithmetic), so offsets of a lane are constants and no size of the
+// contraction is too large for them; what lies outside the matrix reads as zero: rows beyond it by the number of records or an offset
+// beyond it, the last k by a comparison.
+#pragma once
+#include <atomic>
+#include "elements.hpp"
+#include "syrk_dtl_tile.hpp"
+
+namespace ak {
+
+constexpr int kHpStages = 4;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename E>
+__device__ __forceinline__ floatx16 hp_mfma(short8v a, short8v b, floatx16 c) {
+  if constexpr (sizeof(E) == 2 && __is_same(E, __bf16))
+    return mfma_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+struct HpOperand {
+  const void* p;           // 16-byte aligned
+  int64_t ld;              // bytes between rows, a multiple of 16
+  int rows;                // by k: rows i (or j) there are
+  int cols;                // by row: elements of a row, a multiple of 8 (what lies behind the matrix is not stored)
+  int64_t k;               // k there are (by row: rows; a contraction that is longer takes zeros)
+};
+
+struct HpProblem {
+  HpOperand A, B;
+  int64_t K, k_per_split;  // k_per_split a multiple of 32
+  int tiles_i, tiles_j, splits;
+};
+
+template <int WR_, int WC_, int FR_, int FC_, bool A_BY_K_, bool B_BY_K_>
+struct HpCfg {
+  static constexpr int WR = WR_, WC = WC_, FR = FR_, FC = FC_, NW = WR * WC, THREADS = 64 * NW;
+  static constexpr bool A_BY_K = A_BY_K_, B_BY_K = B_BY_K_;
+  static constexpr int BI = 32 * FR * WR, BJ = 32 * FC * WC, BK = 32;
+  static constexpr int BLOCK = 2048, PANEL_A = BI * 64, PANEL_B = BJ * 64, STAGE = PANEL_A + PANEL_B, LDS_BYTES = kHpStages * STAGE;
+  static constexpr int IA = BI / 16 / NW, IB = BJ / 16 / NW, LPT = IA + IB;      // wave-wide loads of a k-tile, per wave
+  static_assert(BI / 16 % NW == 0 && BJ / 16 % NW == 0 && LDS_BYTES <= 160 * 1024, "loads split evenly, panels fit the LDS");
+};
+
+// What one wave loads of an operand: N wave-wide loads a k-tile.
+template <bool BY_K, int N>
+struct HpLoader {
+  uint64_t base;           // of the next k-tile
+  int64_t step, left;      // bytes to the k-tile behind it; k from there to the end
+  uint32_t off[N];
+  int64_t ld;
+  int k_of_lane, first;
+
+  __device__ __forceinline__ void init(const HpOperand& o, int wave, int lane, int at0, int64_t k0, int64_t k_count) {
+    ld = o.ld;
+    left = k_count < o.k - k0 ? k_count : o.k - k0;
+    if constexpr (BY_K) {
+      const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+      base = reinterpret_cast<uint64_t>(o.p) + static_cast<uint64_t>(at0) * o.ld + static_cast<uint64_t>(k0) * 2;
+      step = 64;
+      k_of_lane = 8 * chunk;
+      first = wave * N * 1024;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = 16 * (wave * N + i) + (lane >> 2);
+        off[i] = at0 + row < o.rows ? static_cast<uint32_t>(row) * static_cast<uint32_t>(o.ld) + 16u * chunk : kDtlOob;
+      }
+    } else {
+      const int half = wave & 1, cb = (wave >> 1) * N, row = 16 * half + (lane >> 2);
+      base = reinterpret_cast<uint64_t>(o.p) + static_cast<uint64_t>(k0) * o.ld;
+      step = 32 * o.ld;
+      first = cb * 2048 + half * 1024;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int col = at0 + 32 * (cb + i) + 8 * (lane & 3);
+        off[i] = col < o.cols ? static_cast<uint32_t>(row) * static_cast<uint32_t>(o.ld) + 2u * static_cast<uint32_t>(col) : kDtlOob;
+      }
+    }
+  }
+
+  // Load i of the k-tile that base stands at, to the panel at `lds`.
+  __device__ __forceinline__ void load(int i, uint32_t lds) const {
+    u32x4 rsrc;
+    rsrc[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base));
+    rsrc[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base >> 32) & 0xffffu);
+    rsrc[3] = 0x00020000u;
+    uint32_t at = off[i];
+    if constexpr (BY_K) {
+      rsrc[2] = kDtlRange;
+      if (k_of_lane >= left) at = kDtlOob;
+    } else {
+      // rows of the tile that exist, in bytes: an offset into a row behind them is at least that
+      const int64_t bytes = (left < 32 ? (left < 0 ? 0 : left) : 32) * ld;
+      rsrc[2] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes));
+    }
+    load_to_lds<true>(rsrc, lds + first + i * (BY_K ? 1024 : 2048), at);
+  }
+
+  __device__ __forceinline__ void next() {
+    base += step;
+    left -= 32;
+  }
+};
+
+// Offsets of a lane's fragments within the blocks of a panel: of the first and of the second 16 k of a k-tile.
+template <bool BY_K>
+__device__ __forceinline__ int hp_fragment(int lane, int kk) {
+  const int g = lane >> 5, l32 = lane & 31, j16 = lane & 15, hl = (lane >> 4) & 1;
+  if constexpr (BY_K) return l32 * 64 + (((2 * kk + g) ^ ((l32 >> 2) & 3)) << 4);
+  return (16 * kk + 8 * g + (j16 >> 2)) * 64 + hl * 32 + (j16 & 3) * 8;
+}
+
+template <bool BY_K>
+__device__ __forceinline__ short8v hp_read(AK_LDS const unsigned char* q) {
+  if constexpr (BY_K) return *reinterpret_cast<AK_LDS const short8v*>(q);
+  const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AK_LDS short4v*)(q));
+  const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AK_LDS short4v*)(q + 256));
+  return short8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// The tile (ti, tj) of D over k0 .. k0 + k_count: acc[a][b], block (FR wr + a, FC wc + b) of the tile.
+template <class Cfg, typename E>
+__device__ __forceinline__ void hp_tile(const HpProblem& p, int ti, int tj, int64_t k0, int64_t k_count, floatx16 (&acc)[Cfg::FR][Cfg::FC]) {
+  constexpr int FR = Cfg::FR, FC = Cfg::FC, S = kHpStages, LPT = Cfg::LPT;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char hp_smem[];
+  AK_LDS unsigned char* lds = (AK_LDS unsigned char*)hp_smem;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave / Cfg::WC, wc = wave % Cfg::WC;
+
+  HpLoader<Cfg::A_BY_K, Cfg::IA> la;
+  HpLoader<Cfg::B_BY_K, Cfg::IB> lb;
+  la.init(p.A, wave, lane, ti * Cfg::BI, k0, k_count);
+  lb.init(p.B, wave, lane, tj * Cfg::BJ, k0, k_count);
+#pragma unroll
+  for (int a = 0; a < FR; ++a)
+#pragma unroll
+    for (int b = 0; b < FC; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+
+  auto load_one = [&](int l, int stage) {
+    const uint32_t at = lds0 + stage * Cfg::STAGE;
+    if (l < Cfg::IA) la.load(l, at);
+    else lb.load(l - Cfg::IA, at + Cfg::PANEL_A);
+  };
+  const int fa_off[2] = {hp_fragment<Cfg::A_BY_K>(lane, 0), hp_fragment<Cfg::A_BY_K>(lane, 1)};
+  const int fb_off[2] = {hp_fragment<Cfg::B_BY_K>(lane, 0), hp_fragment<Cfg::B_BY_K>(lane, 1)};
+  AK_LDS const unsigned char* pa = lds + wr * FR * Cfg::BLOCK;
+  AK_LDS const unsigned char* pb = lds + Cfg::PANEL_A + wc * FC * Cfg::BLOCK;
+  // fragment u of 16 k, in the order in which the matrix instructions want them: a0, b0 .. b(FC-1), a1 .. a(FR-1)
+  auto read_unit = [&](short8v (&fa)[FR], short8v (&fb)[FC], int stage, int kk, int u) {
+    const int s = stage * Cfg::STAGE;
+    if (u == 0 || u > FC) fa[u == 0 ? 0 : u - FC] = hp_read<Cfg::A_BY_K>(pa + s + (u == 0 ? 0 : u - FC) * Cfg::BLOCK + fa_off[kk]);
+    else fb[u - 1] = hp_read<Cfg::B_BY_K>(pb + s + (u - 1) * Cfg::BLOCK + fb_off[kk]);
+  };
+  // The matrix instructions of 16 k, with the reads of the next 16 and (LOADS) the loads of a k-tile further ahead spread between them.
+  auto half_step = [&](auto loads_tag, const short8v (&ca)[FR], const short8v (&cb)[FC], short8v (&na)[FR], short8v (&nb)[FC], int stage,
+                       int kk, int to) {
+    constexpr int NLOAD = decltype(loads_tag)::value, NM = FR * FC, NS = NLOAD + FR + FC;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      const int a = m / FC, b = m % FC;
+      acc[a][b] = hp_mfma<E>(ca[a], cb[b], acc[a][b]);
+#pragma unroll
+      for (int s = (m * NS) / NM; s < ((m + 1) * NS) / NM; ++s) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (s < NLOAD) load_one(s, to);
+        else read_unit(na, nb, stage, kk, s - NLOAD);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  const int nk = static_cast<int>((k_count + 31) / 32);
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) {              // k-tiles beyond the last load zeros: the counts stay uniform
+#pragma unroll
+    for (int l = 0; l < LPT; ++l) load_one(l, t);
+    la.next();
+    lb.next();
+  }
+  wait_vmcnt<(S - 2) * LPT>();                   // this wave's loads of k-tile 0 have landed
+  __syncthreads();                               // ... and everybody's
+  short8v fa0[FR], fb0[FC], fa1[FR], fb1[FC];
+#pragma unroll
+  for (int u = 0; u < FR + FC; ++u) read_unit(fa0, fb0, 0, 0, u);
+  int rd = 0, to = S - 1;
+  for (int kt = 0; kt < nk; ++kt) {
+    half_step(std::integral_constant<int, 0>{}, fa0, fb0, fa1, fb1, rd, 1, 0);
+    wait_vmcnt<(S - 3) * LPT>();                 // own loads of k-tile kt + 1 have landed
+    __syncthreads();                             // everybody's have; nobody reads k-tile kt - 1 any more
+    rd = (rd + 1 == S) ? 0 : rd + 1;
+    half_step(std::integral_constant<int, LPT>{}, fa1, fb1, fa0, fb0, rd, 0, to);
+    la.next();
+    lb.next();
+    to = (to + 1 == S) ? 0 : to + 1;
+  }
+  wait_vmcnt<0>();                               // the loads of zeros have landed before the LDS is used again
+}
+
+// Tiles in groups of eight along i, so that the tiles an XCD works on at a time share panels in its L2.
+__device__ __forceinline__ void hp_place(int id, int tiles_i, int tiles_j, int& ti, int& tj) {
+  constexpr int GROUP = 8;
+  const int per = GROUP * tiles_j, group = id / per, i0 = group * GROUP, height = min(GROUP, tiles_i - i0), rest = id - group * per;
+  ti = i0 + rest % height;
+  tj = rest / height;
+}
+
+template <class Cfg, typename E, class Epilogue>
+static __global__ __launch_bounds__(Cfg::THREADS) void hp_kernel(HpProblem p, typename Epilogue::Params e) {
+  const int tiles = p.tiles_i * p.tiles_j;
+  const int id = static_cast<int>(xcd_contiguous_id(blockIdx.x, gridDim.x));
+  const int split = id / tiles;
+  int ti, tj;
+  hp_place(id - split * tiles, p.tiles_i, p.tiles_j, ti, tj);
+  const int64_t k0 = split * p.k_per_split;
+  const int64_t k_count = p.K - k0 < p.k_per_split ? p.K - k0 : p.k_per_split;
+  floatx16 acc[Cfg::FR][Cfg::FC];
+  hp_tile<Cfg, E>(p, ti, tj, k0, k_count, acc);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Epilogue::template run<Cfg>(e, acc, ti, tj, split, wave / Cfg::WC, wave % Cfg::WC);
+}
+
+// f(i, j, values of rows i .. i + 3) for a lane's part of the tile.
+template <class Cfg, typename F>
+__device__ __forceinline__ void hp_quads(floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int wr, int wc, F&& f) {
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int i0 = ti * Cfg::BI + 32 * Cfg::FR * wr + 4 * g, j0 = tj * Cfg::BJ + 32 * Cfg::FC * wc + l32;
+#pragma unroll
+  for (int b = 0; b < Cfg::FC; ++b)
+#pragma unroll
+    for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        f(i0 + 32 * a + 8 * q, j0 + 32 * b, floatx4{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]});
+}
+
+// out[j][i] = scale * D[i][j] as T
+template <typename T>
+struct HpStore {
+  struct Params {
+    T* out;
+    int64_t ldo;
+    int I, J;
+    float scale;
+    const float* factor;     // optional further one, on the device
+  };
+  template <class Cfg>
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc) {
+    const float s = e.factor != nullptr ? e.scale * *e.factor : e.scale;
+    hp_quads<Cfg>(acc, ti, tj, wr, wc, [&](int i, int j, floatx4 v) {
+      if (j >= e.J || i >= e.I) return;
+      T* __restrict__ to = e.out + static_cast<int64_t>(j) * e.ldo + i;
+      Some<T, 4> some;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) some.set(k, v[k] * s);
+      if (i + 4 <= e.I) {
+        some.store(to);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          if (i + k < e.I) to[k] = some.v[k];
+      }
+    });
+  }
+};
+
+// sum[split][j][i] = or += D[i][j], fp32
+struct HpSum {
+  struct Params {
+    float* sum;
+    int64_t ldo, stride;     // elements between rows, between splits; rows are whole multiples of four
+    int I, J, first;         // first: set, else add
+  };
+  template <class Cfg>
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int split, int wr, int wc) {
+    float* __restrict__ sum = e.sum + split * e.stride;
+    const bool first = e.first != 0;
+    hp_quads<Cfg>(acc, ti, tj, wr, wc, [&](int i, int j, floatx4 v) {
+      if (j >= e.J || i >= e.I) return;
+      floatx4* to = reinterpret_cast<floatx4*>(sum + static_cast<int64_t>(j) * e.ldo + i);
+      *to = first ? v : *to + v;
+    });
+  }
+};
+
+// dst[row][c] = T(scale * factor * sum over the splits of sum[split][row][c])
+template <typename T>
+static __global__ __launch_bounds__(256) void hp_total_kernel(const float* __restrict__ sum, int64_t ld, int64_t stride, int splits, int64_t rows,
+                                                              int cols, float scale, const float* __restrict__ factor, T* __restrict__ dst) {
+  const int64_t n = rows * ld;
+  const float u = factor != nullptr ? scale * *factor : scale;
+  for (int64_t i = 4 * (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x); i < n; i += 4 * static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / ld;
+    const int c = static_cast<int>(i - row * ld);
+    floatx4 t = *reinterpret_cast<const floatx4*>(sum + i);
+    for (int s = 1; s < splits; ++s) t += *reinterpret_cast<const floatx4*>(sum + s * stride + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k < cols) dst[row * cols + c + k] = static_cast<T>(t[k] * u);
+  }
+}
+
+template <typename T>
+inline int hp_total(const float* sum, int64_t ld, int64_t stride, int splits, int64_t rows, int cols, float scale, const float* factor, T* dst,
+                    hipStream_t stream) {
+  const int64_t groups = (rows * ld + 1023) / 1024;
+  hipLaunchKernelGGL(hp_total_kernel<T>, dim3(static_cast<unsigned>(groups < 8192 ? groups : 8192)), dim3(256), 0, stream, sum, ld, stride, splits, rows,
+                     cols, scale, factor, dst);
+  return check_launch();
+}
+
+// Rows at a pitch of ldo elements, zeros behind them: what the panels' loads need where an operand has another pitch or alignment.
+template <typename T>
+static __global__ __launch_bounds__(256) void hp_pad_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, T* __restrict__ out, int ldo) {
+  const int64_t n = rows * ldo;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / ldo;
+    const int c = static_cast<int>(i - row * ldo);
+    out[i] = c < cols ? x[row * ld + c] : static_cast<T>(0.f);
+  }
+}
+
+template <typename T>
+inline int hp_pad(const T* x, int64_t ld, int64_t rows, int64_t cols, T* out, int64_t ldo, hipStream_t stream) {
+  const int64_t groups = (rows * ldo + 1023) / 1024;
+  hipLaunchKernelGGL(hp_pad_kernel<T>, dim3(static_cast<unsigned>(groups < 1 ? 1 : groups < 8192 ? groups : 8192)), dim3(256), 0, stream, x, ld, rows,
+                     static_cast<int>(cols), out, static_cast<int>(ldo));
+  return check_launch();
+}
+
+// 16-bit elements whose rows the panels' loads can read where they lie.
+inline bool hp_aligned(const void* x, int64_t ld, int64_t cols) {
+  return cols % 8 == 0 && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+}
+
+inline int64_t align_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// rows x cols, row pitch ld elements
+inline HpOperand hp_operand(const void* p, int64_t ld, int64_t rows, int64_t cols, bool by_k) {
+  return HpOperand{p, ld * 2, static_cast<int>(rows), static_cast<int>(align_up(cols, 8)), by_k ? align_up(cols, 8) : rows};
+}
+
+// An I x J result; the contraction in (at most) `splits` parts.
+template <class Cfg>
+inline HpProblem hp_problem(const HpOperand& A, const HpOperand& B, int64_t I, int64_t J, int64_t K, int splits = 1) {
+  HpProblem p;
+  p.A = A; p.B = B;
+  p.K = K;
+  p.k_per_split = align_up((K + splits - 1) / splits, 32);
+  p.tiles_i = static_cast<int>((I + Cfg::BI - 1) / Cfg::BI);
+  p.tiles_j = static_cast<int>((J + Cfg::BJ - 1) / Cfg::BJ);
+  p.splits = static_cast<int>((K + p.k_per_split - 1) / p.k_per_split);
+  return p;
+}
+
+// Consecutive parts of a workspace, each at a multiple of 256 bytes (without a base: their size).
+struct Carver {
+  unsigned char* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(int64_t count) {
+    T* at = base != nullptr ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += static_cast<size_t>(align_up(count * static_cast<int64_t>(sizeof(T)), 256));
+    return at;
+  }
+};
+
+template <bool A_BY_K, bool B_BY_K>
+using HpWide = HpCfg<2, 4, 4, 2, A_BY_K, B_BY_K>;      // 256 x 256
+template <bool A_BY_K, bool B_BY_K>
+using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K>;     // 128 x 128
+
+// 256 x 256 tiles where they fill the device, 128 x 128 ones below that.
+inline bool hp_wide(int64_t I, int64_t J) { return ((I + 255) / 256) * ((J + 255) / 256) >= 256; }
+
+template <class Cfg, typename E, class Epilogue>
+inline int hp_launch(const HpProblem& p, const typename Epilogue::Params& e, hipStream_t stream) {
+  const int64_t groups = static_cast<int64_t>(p.tiles_i) * p.tiles_j * p.splits;
+  if (groups <= 0) return AK_OK;
+  if (groups > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  auto kernel = hp_kernel<Cfg, E, Epilogue>;
+  static std::atomic<uint64_t> known{0};         // devices that know the kernel's LDS (setting it twice is harmless)
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) return AK_ERR_LAUNCH;
+  const uint64_t bit = 1ull << (device & 63);
+  if ((known.load(std::memory_order_relaxed) & bit) == 0) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Cfg::LDS_BYTES) != hipSuccess)
+      return AK_ERR_LAUNCH;
+    if (device < 64) known.fetch_or(bit, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(Cfg::THREADS), Cfg::LDS_BYTES, stream, p, e);
+  return check_launch();
+}
+
+}  // namespace ak

@@ -1,0 +1,387 @@
+// Activations kept in 8 bits between the passes, and what the backward pass makes of them.
+// A block of 128 features of a row shares a power of two: e is the least integer with max |x| 2^-e <= 448, clamped to -127 .. 127, and a
+// value is kept as the nearest e4m3 number (4 bits of exponent, 3 of fraction, ties to even) of x 2^-e, which stands for code 2^e.  Scaling by a
+// power of two rounds nothing, and a floating code loses no accuracy by it: normal codes reach down to 2^-15 of the largest value, at
+// a relative error of at most 2^-4.  Infinities and NaN are kept as NaN and do not count for e; what would be rounded to 2^128 is kept as
+// 1.875 2^127.
+//   gelu:    y = x P(x) and the kept x in one pass;  dx = g (P(x') + x' P'(x')) with the kept x', P the normal distribution or its
+//            approximation by tanh
+//   linear:  dw = g^T x',  db = sum g.  x' is a bfloat16 number exactly, so the products are exact and their sums fp32: g in
+//            bfloat16 as it is, in fp16 and fp32 as two and three bfloat16 pieces that add up to it exactly
+// The elementwise passes are bound by the memory, the products by the matrix cores.
+#include <algorithm>
+#include "column_sums.hpp"
+#include "half_product.hpp"
+
+namespace ak {
+
+constexpr int kKeepBlock = 128, kKeepLanes = 16, kKeepEach = 8;      // a block is 16 lanes of 8 elements
+constexpr float kKeepLargest = 448.f;
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float v) {
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)));
+}
+// The largest over 16 neighbouring lanes, in each of them (the moves of lanes_sum()).
+__device__ __forceinline__ float lanes16_max(float v) {
+  v = max_dpp<0xB1>(v);
+  v = max_dpp<0x4E>(v);
+  v = max_dpp<0x141>(v);
+  return max_dpp<0x140>(v);
+}
+
+__device__ __forceinline__ int keep_exponent(float most) {
+  if (most == 0.f) return -127;
+  const int e = __builtin_amdgcn_frexp_expf(most) - 1;                       // most = m 2^e, 1 <= m < 2
+  const float m = 2.f * __builtin_amdgcn_frexp_mantf(most);
+  return max(-127, min(127, e - 8 + (m > kKeepLargest / 256.f ? 1 : 0)));
+}
+
+// (e = 120 is that of values from 1.75 2^127 on, the largest of which would be rounded to 2^128: they are kept as 240 2^120)
+__device__ __forceinline__ float keep_scaled(float x, int e) {
+  const float v = ldexpf(x, -e), most = e == 120 ? 240.f : kKeepLargest;
+  return fabsf(x) < INFINITY ? fminf(fmaxf(v, -most), most) : NAN;
+}
+
+__device__ __forceinline__ u32x2 keep_codes(const float (&x)[kKeepEach], int e) {
+  u32x2 o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(keep_scaled(x[4 * h], e), keep_scaled(x[4 * h + 1], e), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(keep_scaled(x[4 * h + 2], e), keep_scaled(x[4 * h + 3], e), w, true);
+    o[h] = static_cast<uint32_t>(w);
+  }
+  return o;
+}
+
+__device__ __forceinline__ void keep_values(u32x2 codes, int e, float (&x)[kKeepEach]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes[h]), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes[h]), true);
+    x[4 * h] = ldexpf(lo[0], e);
+    x[4 * h + 1] = ldexpf(lo[1], e);
+    x[4 * h + 2] = ldexpf(hi[0], e);
+    x[4 * h + 3] = ldexpf(hi[1], e);
+  }
+}
+
+enum { kGeluExact = 0, kGeluTanh = 1 };
+
+// P(x), and with SLOPE P'(x)
+template <int KIND, bool SLOPE>
+__device__ __forceinline__ void gelu_share(float x, float& below, float& slope) {
+  if constexpr (KIND == kGeluExact) {
+    below = 0.5f * erfcf(x * -0.70710678118654752f);
+    if constexpr (SLOPE) slope = 0.39894228040143268f * __expf(-0.5f * x * x);
+  } else {
+    // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+    // (beyond 20 the share is 0 or 1; the cube of a large number is no float32.  A NaN stays.)
+    x = fabsf(x) > 20.f ? copysignf(20.f, x) : x;
+    const float u2 = 1.5957691216057308f * (x + 0.044715f * x * x * x);
+    below = 1.f / (1.f + __expf(-u2));
+    if constexpr (SLOPE) slope = below * (1.f / (1.f + __expf(u2))) * 1.5957691216057308f * (1.f + 0.134145f * x * x);
+  }
+}
+
+struct Keep {
+  const void* x;           // the activations, or the gradient of the result on the way back
+  void* y;                 // the result, or the gradient of the activations
+  uint8_t* codes;          // [rows][F]
+  int8_t* exponents;       // [rows][blocks]
+  int64_t ldx, rows;
+  int F, blocks;
+};
+
+// The elements of a lane: eight, fewer at the end of a row.
+struct KeepPlace {
+  int64_t row, block;
+  int c, count;
+  __device__ __forceinline__ KeepPlace(const Keep& p, int64_t group) {
+    const uint32_t b = static_cast<uint32_t>(p.blocks);
+    row = group / b;
+    block = group - row * b;
+    c = static_cast<int>(block) * kKeepBlock + static_cast<int>(threadIdx.x % kKeepLanes) * kKeepEach;
+    count = row < p.rows ? min(max(p.F - c, 0), kKeepEach) : 0;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void keep_load(const T* __restrict__ p, int count, float (&x)[kKeepEach]) {
+  if (count == kKeepEach) {
+    Some<T, kKeepEach> v;
+    v.load(p);
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e) x[e] = v.get(e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e) x[e] = e < count ? static_cast<float>(p[e]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void keep_store(T* __restrict__ p, int count, const float (&x)[kKeepEach]) {
+  if (count == kKeepEach) {
+    Some<T, kKeepEach> v;
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e) v.set(e, x[e]);
+    v.store(p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e)
+      if (e < count) p[e] = static_cast<T>(x[e]);
+  }
+}
+
+// KIND -1: the kept values alone
+template <typename T, int KIND>
+static __global__ __launch_bounds__(256) void keep_kernel(Keep p) {
+  const KeepPlace at(p, static_cast<int64_t>(blockIdx.x) * (256 / kKeepLanes) + threadIdx.x / kKeepLanes);
+  float x[kKeepEach];
+  keep_load(static_cast<const T*>(p.x) + at.row * p.ldx + at.c, at.count, x);
+  float most = 0.f;
+#pragma unroll
+  for (int e = 0; e < kKeepEach; ++e) most = fmaxf(most, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+  const int exponent = keep_exponent(lanes16_max(most));
+  if (at.count == 0) return;
+  const u32x2 codes = keep_codes(x, exponent);
+  uint8_t* __restrict__ to = p.codes + at.row * p.F + at.c;
+  if (at.count == kKeepEach) {
+    __builtin_memcpy(to, &codes, 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e)
+      if (e < at.count) to[e] = static_cast<uint8_t>(codes[e >> 2] >> 8 * (e & 3));
+  }
+  if (threadIdx.x % kKeepLanes == 0) p.exponents[at.row * p.blocks + at.block] = static_cast<int8_t>(exponent);
+  if constexpr (KIND >= 0) {
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e) {
+      float below, slope;
+      gelu_share<KIND, false>(x[e], below, slope);
+      x[e] = x[e] * below;
+    }
+    keep_store(static_cast<T*>(p.y) + at.row * p.F + at.c, at.count, x);
+  }
+}
+
+__device__ __forceinline__ u32x2 keep_fetch(const uint8_t* __restrict__ from, int count) {
+  u32x2 codes = {0, 0};
+  if (count == kKeepEach) {
+    __builtin_memcpy(&codes, from, 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e)
+      if (e < count) codes[e >> 2] |= static_cast<uint32_t>(from[e]) << 8 * (e & 3);
+  }
+  return codes;
+}
+
+// KIND -1: y = the kept values (pitch ldy, zeros up to it); else y = x (P + x' P')
+template <typename T, int KIND>
+static __global__ __launch_bounds__(256) void keep_back_kernel(Keep p, int64_t ldy, int padded) {
+  const KeepPlace at(p, static_cast<int64_t>(blockIdx.x) * (256 / kKeepLanes) + threadIdx.x / kKeepLanes);
+  if (at.row >= p.rows) return;
+  float x[kKeepEach] = {};
+  if (at.count > 0) {
+    const int exponent = p.exponents[at.row * p.blocks + at.block];
+    keep_values(keep_fetch(p.codes + at.row * p.F + at.c, at.count), exponent, x);
+  }
+  if constexpr (KIND >= 0) {
+    if (at.count == 0) return;
+    float g[kKeepEach];
+    keep_load(static_cast<const T*>(p.x) + at.row * p.ldx + at.c, at.count, g);
+#pragma unroll
+    for (int e = 0; e < kKeepEach; ++e) {
+      float below, slope;
+      gelu_share<KIND, true>(x[e], below, slope);
+      x[e] = g[e] * (below + x[e] * slope);
+    }
+    keep_store(static_cast<T*>(p.y) + at.row * ldy + at.c, at.count, x);
+  } else {
+    const int count = min(max(padded - at.c, 0), kKeepEach);
+    if (count > 0) keep_store(static_cast<T*>(p.y) + at.row * ldy + at.c, count, x);
+  }
+}
+
+// The bfloat16 pieces of a gradient, [piece][rows][ldo], zeros behind its columns: they add up to it exactly.
+template <typename T, int PIECES>
+static __global__ __launch_bounds__(256) void keep_pieces_kernel(const T* __restrict__ g, int64_t ld, int64_t rows, int cols, __bf16* __restrict__ out,
+                                                                 int ldo) {
+  const int64_t n = rows * ldo;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / ldo;
+    const int c = static_cast<int>(i - row * ldo);
+    float rest = c < cols ? static_cast<float>(g[row * ld + c]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const __bf16 piece = static_cast<__bf16>(rest);
+      out[k * n + i] = piece;
+      // (infinities and NaN in the first piece alone)
+      rest = fabsf(rest) < INFINITY ? rest - static_cast<float>(piece) : 0.f;
+    }
+  }
+}
+
+// ---- host side
+struct KeepPlan {
+  int pieces, splits;
+  int64_t ldf, ldg, ld_sum;
+  bool direct;             // the products' epilogue writes dw
+};
+
+inline KeepPlan keep_plan(int dtype, int64_t rows, int64_t F, int64_t out) {
+  KeepPlan p;
+  p.pieces = dtype == AK_BF16 ? 1 : dtype == AK_F16 ? 2 : 3;
+  p.ldf = align_up(F, 8);
+  p.ldg = align_up(out, 8);
+  p.ld_sum = align_up(F, 4);
+  const bool wide = hp_wide(F, out);
+  const int64_t tile = wide ? 256 : 128, tiles = ((F + tile - 1) / tile) * ((out + tile - 1) / tile);
+  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((wide ? 256 : 512) / tiles, rows / 256), 64));
+  const int64_t per = align_up((rows + s - 1) / s, 32);
+  p.splits = static_cast<int>((rows + per - 1) / per);
+  p.direct = p.pieces == 1 && p.splits == 1;
+  return p;
+}
+
+struct KeepSpace {
+  __bf16 *x, *g;
+  float *sum, *columns;
+  size_t bytes;
+};
+
+inline KeepSpace keep_space(const KeepPlan& p, int64_t rows, int64_t out, bool copy, bool bias, void* ws) {
+  Carver c{static_cast<unsigned char*>(ws)};
+  KeepSpace s = {};
+  s.x = c.take<__bf16>(rows * p.ldf);
+  if (copy) s.g = c.take<__bf16>(p.pieces * rows * p.ldg);
+  if (!p.direct) s.sum = c.take<float>(p.splits * out * p.ld_sum);
+  if (bias) s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(rows, out) / sizeof(float)));
+  s.bytes = c.used;
+  return s;
+}
+
+inline int keep_check(int dtype, int64_t ld, int64_t rows, int64_t F) {
+  if (!is_element_type(dtype) || rows < 0 || F <= 0 || ld < F) return AK_ERR_ARG;
+  // blocks in 32 bits, and a launch's work groups
+  if (F > (1ll << 24) || rows > (1ll << 31) || rows * ((F + kKeepBlock - 1) / kKeepBlock) > (1ll << 34)) return AK_ERR_TOO_LARGE;
+  return AK_OK;
+}
+
+inline dim3 keep_grid(const Keep& p) {
+  return dim3(static_cast<unsigned>((p.rows * p.blocks + 256 / kKeepLanes - 1) / (256 / kKeepLanes)));
+}
+
+}  // namespace ak
+
+extern "C" int ak_quantize_8bit(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t width, int gelu, void* y, uint8_t* codes, int8_t* exponents,
+                                ak_stream_t stream) {
+  using namespace ak;
+  const int rc = keep_check(dtype, ldx, rows, width);
+  if (rc != AK_OK) return rc;
+  if (gelu < -1 || gelu > kGeluTanh) return AK_ERR_ARG;
+  if (rows == 0) return AK_OK;
+  if (x == nullptr || codes == nullptr || exponents == nullptr || (gelu >= 0 && y == nullptr)) return AK_ERR_ARG;
+  const Keep p{x, y, codes, exponents, ldx, rows, static_cast<int>(width), static_cast<int>((width + kKeepBlock - 1) / kKeepBlock)};
+  return with_type(dtype, [&](auto t) {
+    using T = typename decltype(t)::type;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (gelu == kGeluExact) hipLaunchKernelGGL((keep_kernel<T, kGeluExact>), keep_grid(p), dim3(256), 0, s, p);
+    else if (gelu == kGeluTanh) hipLaunchKernelGGL((keep_kernel<T, kGeluTanh>), keep_grid(p), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((keep_kernel<T, -1>), keep_grid(p), dim3(256), 0, s, p);
+    return check_launch();
+  });
+}
+
+extern "C" int ak_dequantize_8bit(const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width, int gelu, const void* g, int64_t ldg,
+                                  void* y, int dtype, ak_stream_t stream) {
+  using namespace ak;
+  const int rc = keep_check(dtype, gelu >= 0 ? ldg : width, rows, width);
+  if (rc != AK_OK) return rc;
+  if (gelu < -1 || gelu > kGeluTanh) return AK_ERR_ARG;
+  if (rows == 0) return AK_OK;
+  if (codes == nullptr || exponents == nullptr || y == nullptr || (gelu >= 0 && g == nullptr)) return AK_ERR_ARG;
+  const int F = static_cast<int>(width);
+  const Keep p{g, y, const_cast<uint8_t*>(codes), const_cast<int8_t*>(exponents), ldg, rows, F, (F + kKeepBlock - 1) / kKeepBlock};
+  return with_type(dtype, [&](auto t) {
+    using T = typename decltype(t)::type;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (gelu == kGeluExact) hipLaunchKernelGGL((keep_back_kernel<T, kGeluExact>), keep_grid(p), dim3(256), 0, s, p, width, F);
+    else if (gelu == kGeluTanh) hipLaunchKernelGGL((keep_back_kernel<T, kGeluTanh>), keep_grid(p), dim3(256), 0, s, p, width, F);
+    else hipLaunchKernelGGL((keep_back_kernel<T, -1>), keep_grid(p), dim3(256), 0, s, p, width, F);
+    return check_launch();
+  });
+}
+
+extern "C" size_t ak_weight_grad_8bit_ws_bytes(int dtype, int64_t rows, int64_t width, int64_t out) {
+  if (!ak::is_element_type(dtype) || rows <= 0 || width <= 0 || out <= 0 || rows > (1ll << 30) || width > (1 << 20) || out > (1 << 20)) return 0;
+  return ak::keep_space(ak::keep_plan(dtype, rows, width, out), rows, out, true, true, nullptr).bytes;
+}
+
+extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width,
+                                   int64_t out, void* dw, void* db, int grad_dtype, void* ws, size_t ws_bytes, ak_stream_t stream) {
+  using namespace ak;
+  int rc = keep_check(dtype, ldg, rows, out);
+  if (rc != AK_OK) return rc;
+  if (!is_element_type(grad_dtype) || width <= 0 || rows == 0) return AK_ERR_ARG;
+  if (rows > (1ll << 30) || width > (1 << 20) || out > (1 << 20) || ldg > (1ll << 24)) return AK_ERR_TOO_LARGE;
+  if (dw == nullptr && db == nullptr) return AK_OK;
+  if (g == nullptr || (dw != nullptr && (codes == nullptr || exponents == nullptr))) return AK_ERR_ARG;
+  const KeepPlan plan = keep_plan(dtype, rows, width, out);
+  const bool copy = dtype != AK_BF16 || !hp_aligned(g, ldg, out);
+  const KeepSpace s = keep_space(plan, rows, out, copy, db != nullptr, ws);
+  if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dw != nullptr) {
+    const int F = static_cast<int>(width);
+    const Keep k{nullptr, s.x, const_cast<uint8_t*>(codes), const_cast<int8_t*>(exponents), 0, rows, F, (F + kKeepBlock - 1) / kKeepBlock};
+    hipLaunchKernelGGL((keep_back_kernel<__bf16, -1>), keep_grid(k), dim3(256), 0, st, k, plan.ldf, static_cast<int>(plan.ldf));
+    const __bf16* from = static_cast<const __bf16*>(g);
+    int64_t ld = ldg;
+    if (copy) {
+      const int64_t groups = std::max<int64_t>(1, std::min<int64_t>((rows * plan.ldg + 1023) / 1024, 8192));
+      const dim3 grid(static_cast<unsigned>(groups));
+      const int cols = static_cast<int>(out), ldo = static_cast<int>(plan.ldg);
+      if (dtype == AK_BF16)
+        hipLaunchKernelGGL((keep_pieces_kernel<__bf16, 1>), grid, dim3(256), 0, st, static_cast<const __bf16*>(g), ldg, rows, cols, s.g, ldo);
+      else if (dtype == AK_F16)
+        hipLaunchKernelGGL((keep_pieces_kernel<_Float16, 2>), grid, dim3(256), 0, st, static_cast<const _Float16*>(g), ldg, rows, cols, s.g, ldo);
+      else
+        hipLaunchKernelGGL((keep_pieces_kernel<float, 3>), grid, dim3(256), 0, st, static_cast<const float*>(g), ldg, rows, cols, s.g, ldo);
+      from = s.g;
+      ld = plan.ldg;
+    }
+    rc = check_launch();
+    if (rc != AK_OK) return rc;
+    rc = with_type(grad_dtype, [&](auto o) {
+      using O = typename decltype(o)::type;
+      // i features, j outputs, k rows
+      auto products = [&](auto cfg) {
+        using Cfg = decltype(cfg);
+        for (int piece = plan.pieces - 1; piece >= 0; --piece) {            // the smallest first
+          const HpProblem q = hp_problem<Cfg>(hp_operand(s.x, plan.ldf, rows, width, false), hp_operand(from + piece * rows * ld, ld, rows, out, false),
+                                              width, out, rows, plan.splits);
+          const int done = plan.direct
+                               ? hp_launch<Cfg, __bf16, HpStore<O>>(q, typename HpStore<O>::Params{static_cast<O*>(dw), width, F, static_cast<int>(out), 1.f, nullptr}, st)
+                               : hp_launch<Cfg, __bf16, HpSum>(q, HpSum::Params{s.sum, plan.ld_sum, out * plan.ld_sum, F, static_cast<int>(out),
+                                                                               piece == plan.pieces - 1}, st);
+          if (done != AK_OK) return done;
+        }
+        return plan.direct ? AK_OK : hp_total(s.sum, plan.ld_sum, out * plan.ld_sum, plan.splits, out, F, 1.f, nullptr, static_cast<O*>(dw), st);
+      };
+      return hp_wide(width, out) ? products(HpWide<false, false>{}) : products(HpSmall<false, false>{});
+    });
+    if (rc != AK_OK) return rc;
+  }
+  if (db == nullptr) return AK_OK;
+  return with_type(grad_dtype, [&](auto o) {
+    using O = typename decltype(o)::type;
+    return with_type(dtype, [&](auto t) {
+      using T = typename decltype(t)::type;
+      return column_sums(static_cast<const T*>(g), ldg, rows, out, 1.f, nullptr, static_cast<O*>(db), s.columns, st);
+    });
+  });
+}

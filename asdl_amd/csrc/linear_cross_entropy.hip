@@ -1,0 +1,643 @@
+// Softmax cross entropy of a linear layer, in pieces of the classes, without its logits:
+//   s = h w^T + b,  lse_n = log sum_v exp s_nv,  loss_n = lse_n - s_n,t(n)  (0 for an ignored row)
+//   back, with c_n the gradient of loss_n (0 for an ignored row):
+//   d_nv = c_n (exp(s_nv - lse_n) - [v = t(n)]),  dh = d w,  dw = d^T h,  db_v = sum_n d_nv
+// Forward, the product's tiles leave the largest logit and the sum of exponentials of their classes for each row, and the target's
+// logit; a second launch joins them.  Backward, the logits of a piece of the classes are formed again (2 N V D operations more than
+// with kept logits, which would be written, read and written again: 1.6 GB in fp32 for 8192 rows of 50257 classes), and become the piece
+// of d in their tile's epilogue; both gradients are products with it.
+// 16-bit operands: fp32 sums.  d is rounded to the operands' type, which the matrix cores need and which is what a framework's own
+// backward pass in that type has; it holds c_n over the next power of two above the largest |c_n| (fp16: times 2^14, so that shares
+// of the classes down to 2^-28 are normal numbers), and the products' epilogues put the power back.
+// fp32 operands: the framework's three-piece products (gemm_x3.hpp), through pieces of fp32 logits.
+#include <algorithm>
+#include "column_sums.hpp"
+#include "gemm_f32.hpp"
+#include "half_product.hpp"
+
+namespace ak {
+
+enum { kLossNone = 0, kLossSum = 1, kLossMean = 2 };
+
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
+// (largest, sum of exp(s - largest)) of two sets of classes together; -inf and 0 of an empty one.
+__device__ __forceinline__ floatx2 lce_join2(floatx2 a, floatx2 b) {
+  const float m = fmaxf(a[0], b[0]);
+  // (m is -inf where nothing is there; a NaN is in the sums)
+  const float base = m == -INFINITY ? 0.f : m;
+  return floatx2{m, a[1] * __expf(a[0] - base) + b[1] * __expf(b[0] - base)};
+}
+
+struct LceRows {
+  const int64_t* targets;
+  const float* bias;       // fp32, or null
+  int64_t ignore;
+  int rows, classes;
+};
+
+// Tiles of the forward pass: i classes, j rows.
+struct LceStats {
+  struct Params {
+    LceRows r;
+    floatx2* part;         // [tile of classes][rows]
+    float* at_target;      // [rows]
+  };
+  template <class Cfg>
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char hp_smem[];
+    floatx2* joined = reinterpret_cast<floatx2*>(hp_smem);       // [WR][BJ]
+    const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+    const int i0 = ti * Cfg::BI + 32 * Cfg::FR * wr + 4 * g;
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + 32 * a + 8 * q + k;
+          const float shift = e.r.bias != nullptr && i < e.r.classes ? e.r.bias[i] : 0.f;
+#pragma unroll
+          for (int b = 0; b < Cfg::FC; ++b) acc[a][b][4 * q + k] = i < e.r.classes ? acc[a][b][4 * q + k] + shift : -INFINITY;
+        }
+#pragma unroll
+    for (int b = 0; b < Cfg::FC; ++b) {
+      const int jl = 32 * Cfg::FC * wc + 32 * b + l32, j = tj * Cfg::BJ + jl;
+      const int64_t target = j < e.r.rows ? e.r.targets[j] : -1;
+      const int64_t at = target - i0;      // 32 a + 8 q + k where this lane has the target's logit
+      float m = -INFINITY;
+#pragma unroll
+      for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) m = fmaxf(m, acc[a][b][x]);
+      const float base = m == -INFINITY ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          s += __expf(acc[a][b][x] - base);
+          if (at == 32 * a + 8 * (x >> 2) + (x & 3) && target < e.r.classes) e.at_target[j] = acc[a][b][x];
+        }
+      floatx2 ms = {m, s};
+      ms = lce_join2(ms, floatx2{__shfl_xor(m, 32), __shfl_xor(s, 32)});
+      if (g == 0) joined[wr * Cfg::BJ + jl] = ms;
+    }
+    __syncthreads();
+    for (int jl = threadIdx.x; jl < Cfg::BJ; jl += Cfg::THREADS) {
+      const int j = tj * Cfg::BJ + jl;
+      if (j >= e.r.rows) continue;
+      floatx2 ms = joined[jl];
+#pragma unroll
+      for (int w = 1; w < Cfg::WR; ++w) ms = lce_join2(ms, joined[w * Cfg::BJ + jl]);
+      e.part[static_cast<int64_t>(ti) * e.r.rows + j] = ms;
+    }
+  }
+};
+
+// Tiles of a piece of d: i classes from c0 on, j rows; d[j][i - c0], zeros up to a multiple of eight classes.
+template <typename E>
+struct LceGrad {
+  struct Params {
+    LceRows r;
+    const float* lse;
+    const float* share;    // c_n over the power of two, times 2^14 for fp16
+    E* d;
+    int64_t ldd;
+    int c0, width;         // classes of the piece, a multiple of eight (those from r.classes on are zeros)
+  };
+  template <class Cfg>
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc) {
+    hp_quads<Cfg>(acc, ti, tj, wr, wc, [&](int i, int j, floatx4 v) {
+      if (j >= e.r.rows || i >= e.width) return;
+      const float lse = e.lse[j], share = e.share[j];
+      const int64_t target = e.r.targets[j] - e.c0 - i;
+      Some<E, 4> some;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = e.c0 + i + k;
+        const bool in = c < e.r.classes;
+        const float s = v[k] + (in && e.r.bias != nullptr ? e.r.bias[c] : 0.f);
+        const float p = __expf(s - lse) - (target == k ? 1.f : 0.f);
+        some.set(k, in && share != 0.f ? p * share : 0.f);
+      }
+      some.store(e.d + static_cast<int64_t>(j) * e.ldd + i);
+    });
+  }
+};
+
+// A few rows: a wave takes 16 classes at a time, weights straight to the matrix instruction (16 x 16 x 32).  A lane has 32 consecutive
+// k of every 128 of one class: what the four lanes of a class read at once is a part of each 128-byte line, all of it in four loads.
+// The order of k is the same for both operands.
+template <typename E, int NB>
+static __global__ __launch_bounds__(512) void lce_few_kernel(const E* __restrict__ h, int64_t ldh, const E* __restrict__ w, int64_t ldw, int D,
+                                                             LceRows r, floatx2* __restrict__ part, float* __restrict__ at_target) {
+  __shared__ floatx2 joined[8][16 * NB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4, l16 = lane & 15;
+  const int c0 = (blockIdx.x * 8 + wave) * 16;
+  const E* __restrict__ wr = w + static_cast<int64_t>(min(c0 + l16, r.classes - 1)) * ldw + 32 * quarter;
+  const E* hr[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) hr[b] = h + static_cast<int64_t>(min(16 * b + l16, r.rows - 1)) * ldh + 32 * quarter;
+  floatx4 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto mma = [&](short8v a, short8v b, floatx4 c) {
+    if constexpr (__is_same(E, __bf16))
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  };
+  auto get = [](const E* p) {
+    short8v v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+  };
+  const int whole = D / 128 * 128;
+  short8v wn[4];
+  if (whole > 0)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) wn[e] = get(wr + 8 * e);
+  for (int k = 0; k < whole; k += 128) {
+    short8v wc[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) wc[e] = wn[e];
+    if (k + 128 < whole)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wn[e] = get(wr + k + 128 + 8 * e);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[b] = mma(wc[e], get(hr[b] + k + 8 * e), acc[b]);
+  }
+  if (whole < D) {
+    auto some_of = [&](const E* p, int n) {      // n of eight, zeros behind them
+      short8v v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) v[e] = __builtin_bit_cast(short, p[e]);
+      return v;
+    };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = D - whole - 32 * quarter - 8 * e;
+      const short8v a = some_of(wr + whole + 8 * e, n);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[b] = mma(a, some_of(hr[b] + whole + 8 * e, n), acc[b]);
+    }
+  }
+  // acc[b][x]: class c0 + 4 quarter + x, row 16 b + l16
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int j = 16 * b + l16;
+    const int64_t target = j < r.rows ? r.targets[j] : -1;
+    float m = -INFINITY, v[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int c = c0 + 4 * quarter + x;
+      v[x] = c < r.classes ? acc[b][x] + (r.bias != nullptr ? r.bias[c] : 0.f) : -INFINITY;
+      if (c == target && c < r.classes) at_target[j] = v[x];
+      m = fmaxf(m, v[x]);
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) s += __expf(v[x] - base);
+    floatx2 ms = {m, s};
+    ms = lce_join2(ms, floatx2{__shfl_xor(ms[0], 16), __shfl_xor(ms[1], 16)});
+    ms = lce_join2(ms, floatx2{__shfl_xor(ms[0], 32), __shfl_xor(ms[1], 32)});
+    if (quarter == 0) joined[wave][j] = ms;
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < 16 * NB && j < r.rows; j += 512) {
+    floatx2 ms = joined[0][j];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) ms = lce_join2(ms, joined[k][j]);
+    part[static_cast<int64_t>(blockIdx.x) * r.rows + j] = ms;
+  }
+}
+
+// lse and loss of 64 rows from the parts of all classes, a part of them a wave.
+static __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRows r, const floatx2* __restrict__ part, int parts, const float* __restrict__ at_target,
+                                                               float* __restrict__ losses, float* __restrict__ lse) {
+  __shared__ floatx2 joined[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int j = blockIdx.x * 64 + lane;
+  floatx2 ms = {-INFINITY, 0.f};
+  if (j < r.rows) {
+#pragma unroll 4
+    for (int t = wave; t < parts; t += 16) ms = lce_join2(ms, part[static_cast<int64_t>(t) * r.rows + j]);
+  }
+  joined[wave][lane] = ms;
+  __syncthreads();
+  if (wave != 0 || j >= r.rows) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) ms = lce_join2(ms, joined[k][lane]);
+  const float l = ms[0] + __logf(ms[1]);
+  const int64_t target = r.targets[j];
+  lse[j] = l;
+  // (a target that is no class and not the ignored one: NaN)
+  losses[j] = target == r.ignore ? 0.f : target < 0 || target >= r.classes ? NAN : ms[0] - at_target[j] + __logf(ms[1]);
+}
+
+// The sum or mean over the rows, in double.
+static __global__ __launch_bounds__(1024) void lce_total_kernel(LceRows r, const float* __restrict__ losses, int reduction, float* __restrict__ loss) {
+  __shared__ double red[16];
+  __shared__ u64 count_of[16];
+  double s = 0.;
+  u64 count = 0;
+  for (int j = threadIdx.x; j < r.rows; j += 1024) {
+    s += losses[j];
+    count += r.targets[j] != r.ignore ? 1 : 0;
+  }
+  s = group_sum<16>(s, red);
+  count = group_sum<16>(count, count_of);
+  if (threadIdx.x == 0) *loss = static_cast<float>(reduction == kLossMean ? s / static_cast<double>(count) : s);
+}
+
+// share[n] = c_n / 2^e 2^lift with 2^e > |c_n| for all n (plain: c_n itself), unit = 2^(e - lift).
+static __global__ __launch_bounds__(1024) void lce_shares_kernel(LceRows r, const float* __restrict__ g, int reduction, int plain, int lift,
+                                                                 float* __restrict__ share, float* __restrict__ unit) {
+  __shared__ float red[16];
+  __shared__ u64 count_of[16];
+  float common = 0.f;
+  if (reduction != kLossNone) {
+    u64 count = 0;
+    if (reduction == kLossMean) {
+      for (int j = threadIdx.x; j < r.rows; j += 1024) count += r.targets[j] != r.ignore ? 1 : 0;
+      count = group_sum<16>(count, count_of);
+    } else {
+      count = 1;
+    }
+    common = count == 0 ? 0.f : *g / static_cast<float>(count);
+  }
+  int e = 0;
+  if (!plain) {
+    float most = fabsf(common);
+    if (reduction == kLossNone) {
+      most = 0.f;
+      for (int j = threadIdx.x; j < r.rows; j += 1024) most = fmaxf(most, r.targets[j] != r.ignore ? fabsf(g[j]) : 0.f);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < 16; ++w) most = fmaxf(most, red[w]);
+    }
+    if (most > 0.f && most < INFINITY) frexpf(most, &e);
+    e = min(max(e, -100), 127);        // (2^(e - lift) is a normal number)
+  }
+  if (threadIdx.x == 0) *unit = ldexpf(1.f, e - lift);
+  for (int j = threadIdx.x; j < r.rows; j += 1024) {
+    const int64_t target = r.targets[j];
+    const float c = reduction == kLossNone ? g[j] : common;
+    share[j] = target == r.ignore ? 0.f : target < 0 || target >= r.classes ? NAN : ldexpf(c, lift - e);
+  }
+}
+
+template <typename T>
+static __global__ __launch_bounds__(256) void lce_bias_kernel(const T* __restrict__ x, int n, float* __restrict__ out) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) out[i] = static_cast<float>(x[i]);
+}
+
+// ---- fp32: pieces of logits in memory
+static __global__ __launch_bounds__(256) void lce_piece_stats_kernel(const float* __restrict__ logits, int64_t ld, LceRows r, int c0, int width,
+                                                                     floatx2* __restrict__ part, float* __restrict__ at_target) {
+  __shared__ floatx2 joined[4];
+  const int j = blockIdx.x;
+  const float* __restrict__ x = logits + static_cast<int64_t>(j) * ld;
+  const int64_t target = r.targets[j] - c0;
+  float m = -INFINITY;
+  for (int c = threadIdx.x; c < width; c += 256) m = fmaxf(m, x[c] + (r.bias != nullptr ? r.bias[c0 + c] : 0.f));
+  const float base = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  for (int c = threadIdx.x; c < width; c += 256) {
+    const float v = x[c] + (r.bias != nullptr ? r.bias[c0 + c] : 0.f);
+    s += __expf(v - base);
+    if (c == target) at_target[j] = v;
+  }
+  floatx2 ms = {m, s};
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ms = lce_join2(ms, floatx2{__shfl_xor(ms[0], o), __shfl_xor(ms[1], o)});
+  if ((threadIdx.x & 63) == 0) joined[threadIdx.x >> 6] = ms;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) ms = lce_join2(ms, joined[w]);
+  part[j] = ms;
+}
+
+static __global__ __launch_bounds__(256) void lce_piece_grad_kernel(float* __restrict__ logits, int64_t ld, LceRows r, int c0, int width,
+                                                                    const float* __restrict__ lse, const float* __restrict__ share) {
+  const int j = blockIdx.x;
+  float* __restrict__ x = logits + static_cast<int64_t>(j) * ld;
+  const int64_t target = r.targets[j] - c0;
+  const float l = lse[j], f = share[j];
+  for (int c = threadIdx.x; c < width; c += 256) {
+    const float p = __expf(x[c] + (r.bias != nullptr ? r.bias[c0 + c] : 0.f) - l) - (c == target ? 1.f : 0.f);
+    x[c] = f != 0.f ? p * f : 0.f;
+  }
+}
+
+// ---- host side
+constexpr int64_t kLcePieceBytes = 256ll << 20;       // of d (fp32: of logits): what the last-level cache holds
+constexpr int kLceFewRows = 64;
+
+// Sizes that both the workspace query and the launches use.
+struct LcePlan {
+  int64_t N, V, D;
+  int es;                  // bytes of an element
+  int64_t piece, pieces;   // classes of a piece, a multiple of 256 (the last may have fewer)
+  int64_t ldp;             // row pitch of padded operands
+  int splits;              // of the contraction over a piece's classes
+  int64_t ld_sum;          // row pitch of the fp32 sums of dh
+};
+
+inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D) {
+  LcePlan p;
+  p.N = N; p.V = V; p.D = D;
+  p.es = dtype == AK_F32 ? 4 : 2;
+  const int64_t fit = std::max<int64_t>(kLcePieceBytes / (N * p.es) / 256 * 256, 256);
+  p.pieces = (V + fit - 1) / fit;
+  p.piece = align_up((V + p.pieces - 1) / p.pieces, 256);
+  p.pieces = (V + p.piece - 1) / p.piece;
+  p.ldp = align_up(D, 8);
+  p.ld_sum = align_up(D, 4);
+  const int64_t tiles = ((N + 127) / 128) * ((D + 127) / 128), k = std::min(p.piece, V);
+  int64_t s = std::min((512 + tiles - 1) / tiles, k / 256);
+  s = std::max<int64_t>(1, std::min<int64_t>(s, 64));
+  const int64_t per = align_up((align_up(k, 8) + s - 1) / s, 32);
+  p.splits = static_cast<int>((align_up(k, 8) + per - 1) / per);       // (all of them are set by the first piece; a shorter one has no more)
+  return p;
+}
+
+struct LceSpace {
+  unsigned char *h, *w;    // padded operands
+  float* bias;
+  floatx2* part;
+  float *at_target, *losses;
+  // backward
+  float *share, *unit;
+  unsigned char* d;
+  float *sum, *columns;
+  size_t bytes;
+};
+
+inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_w, bool bias, void* ws) {
+  Carver c{static_cast<unsigned char*>(ws)};
+  LceSpace s = {};
+  if (pad_h) s.h = c.take<unsigned char>(p.N * p.ldp * p.es);
+  if (pad_w) s.w = c.take<unsigned char>(p.V * p.ldp * p.es);
+  if (bias) s.bias = c.take<float>(p.V);
+  if (!backward) {
+    const int64_t parts = p.es == 4 ? p.pieces : (p.V + 127) / 128;
+    s.part = c.take<floatx2>(parts * p.N);
+    s.at_target = c.take<float>(p.N);
+    s.losses = c.take<float>(p.N);
+    if (p.es == 4) s.d = c.take<unsigned char>(p.N * p.piece * p.es);
+  } else {
+    s.share = c.take<float>(p.N);
+    s.unit = c.take<float>(1);
+    s.d = c.take<unsigned char>(p.N * p.piece * p.es);
+    if (p.es != 4) s.sum = c.take<float>(static_cast<int64_t>(p.splits) * p.N * p.ld_sum);
+    s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(p.N, p.piece) / sizeof(float)));
+  }
+  s.bytes = c.used;
+  return s;
+}
+
+struct LceCall {
+  const void* h; int64_t ldh;
+  const void* w; int64_t ldw;
+  const void* bias; int bias_dtype;
+  LceRows r;
+  int64_t D;
+  int dtype;
+  hipStream_t stream;
+};
+
+// Operands at the pitch that the panels need, copied where theirs is another.
+template <typename E>
+inline int lce_operands(LceCall& c, const LcePlan& p, const LceSpace& s) {
+  auto pad = [&](const void*& x, int64_t& ld, int64_t rows, unsigned char* to) {
+    if (to == nullptr) return AK_OK;
+    const int rc = hp_pad(static_cast<const E*>(x), ld, rows, p.D, reinterpret_cast<E*>(to), p.ldp, c.stream);
+    x = to;
+    ld = p.ldp;
+    return rc;
+  };
+  const int rc = pad(c.h, c.ldh, p.N, s.h);
+  return rc != AK_OK ? rc : pad(c.w, c.ldw, p.V, s.w);
+}
+
+inline int lce_bias(LceCall& c, const LcePlan& p, const LceSpace& s) {
+  if (c.bias == nullptr) return AK_OK;
+  if (c.bias_dtype == AK_F32) {
+    c.r.bias = static_cast<const float*>(c.bias);
+    return AK_OK;
+  }
+  c.r.bias = s.bias;
+  return with_type(c.bias_dtype, [&](auto t) {
+    using T = typename decltype(t)::type;
+    hipLaunchKernelGGL(lce_bias_kernel<T>, dim3(static_cast<unsigned>((p.V + 255) / 256)), dim3(256), 0, c.stream, static_cast<const T*>(c.bias),
+                       static_cast<int>(p.V), s.bias);
+    return check_launch();
+  });
+}
+
+template <typename E>
+inline int lce_forward_half(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
+  if (p.N <= kLceFewRows) {
+    const int64_t groups = (p.V + 127) / 128;
+    *parts = static_cast<int>(groups);
+    auto go = [&](auto nb) {
+      hipLaunchKernelGGL((lce_few_kernel<E, decltype(nb)::value>), dim3(static_cast<unsigned>(groups)), dim3(512), 0, c.stream, static_cast<const E*>(c.h),
+                         c.ldh, static_cast<const E*>(c.w), c.ldw, static_cast<int>(p.D), c.r, s.part, s.at_target);
+      return check_launch();
+    };
+    if (p.N <= 16) return go(std::integral_constant<int, 1>{});
+    if (p.N <= 32) return go(std::integral_constant<int, 2>{});
+    return go(std::integral_constant<int, 4>{});
+  }
+  int rc = lce_operands<E>(c, p, s);
+  if (rc != AK_OK) return rc;
+  const HpOperand A = hp_operand(c.w, c.ldw, p.V, p.D, true), B = hp_operand(c.h, c.ldh, p.N, p.D, true);
+  auto go = [&](auto cfg) {
+    using Cfg = decltype(cfg);
+    const HpProblem q = hp_problem<Cfg>(A, B, p.V, p.N, align_up(p.D, 8));
+    *parts = q.tiles_i;
+    return hp_launch<Cfg, E, LceStats>(q, LceStats::Params{c.r, s.part, s.at_target}, c.stream);
+  };
+  return hp_wide(p.V, p.N) ? go(HpWide<true, true>{}) : go(HpSmall<true, true>{});
+}
+
+inline int lce_forward_f32(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
+  float* x = reinterpret_cast<float*>(s.d);
+  *parts = static_cast<int>(p.pieces);
+  for (int64_t k = 0; k < p.pieces; ++k) {
+    const int64_t c0 = k * p.piece, width = std::min(p.piece, p.V - c0);
+    GemmParams g = make_gemm(0, 1, static_cast<int>(p.N), static_cast<int>(width), static_cast<int>(p.D), 1.f, static_cast<const float*>(c.h), c.ldh,
+                             static_cast<const float*>(c.w) + c0 * c.ldw, c.ldw, 0.f, x, p.piece);
+    g.split = 3;
+    const int rc = launch_gemm(g, 1, c.stream);
+    if (rc != AK_OK) return rc;
+    hipLaunchKernelGGL(lce_piece_stats_kernel, dim3(static_cast<unsigned>(p.N)), dim3(256), 0, c.stream, x, p.piece, c.r, static_cast<int>(c0),
+                       static_cast<int>(width), s.part + k * p.N, s.at_target);
+  }
+  return check_launch();
+}
+
+struct LceGrads {
+  void *dh, *dw, *db;
+  int db_dtype;
+};
+
+template <typename T>
+inline int lce_db(const T* d, int64_t ldd, const LcePlan& p, int64_t c0, int64_t width, const LceSpace& s, const LceGrads& out, hipStream_t stream) {
+  if (out.db == nullptr) return AK_OK;
+  return with_type(out.db_dtype, [&](auto t) {
+    using O = typename decltype(t)::type;
+    return column_sums(d, ldd, p.N, width, 1.f, s.unit, static_cast<O*>(out.db) + c0, s.columns, stream);
+  });
+}
+
+template <typename E>
+inline int lce_backward_half(LceCall c, const float* lse, const LcePlan& p, const LceSpace& s, const LceGrads& out) {
+  int rc = lce_operands<E>(c, p, s);
+  if (rc != AK_OK) return rc;
+  E* d = reinterpret_cast<E*>(s.d);
+  for (int64_t k = 0; k < p.pieces; ++k) {
+    const int64_t c0 = k * p.piece, width = std::min(p.piece, p.V - c0), padded = align_up(width, 8);
+    const E* w = static_cast<const E*>(c.w) + c0 * c.ldw;
+    auto grad = [&](auto cfg) {
+      using Cfg = decltype(cfg);
+      const HpProblem q = hp_problem<Cfg>(hp_operand(w, c.ldw, width, p.D, true), hp_operand(c.h, c.ldh, p.N, p.D, true), padded, p.N, align_up(p.D, 8));
+      typename LceGrad<E>::Params e{c.r, lse, s.share, d, p.piece, static_cast<int>(c0), static_cast<int>(padded)};
+      return hp_launch<Cfg, E, LceGrad<E>>(q, e, c.stream);
+    };
+    rc = hp_wide(padded, p.N) ? grad(HpWide<true, true>{}) : grad(HpSmall<true, true>{});
+    if (rc != AK_OK) return rc;
+    if (out.dh != nullptr) {
+      // i features, j rows, k classes; the splits of the last piece may be fewer, or shorter
+      using Cfg = HpSmall<false, true>;
+      const HpProblem q = hp_problem<Cfg>(hp_operand(w, c.ldw, width, p.D, false), hp_operand(d, p.piece, p.N, padded, true), p.D, p.N, padded, p.splits);
+      rc = hp_launch<Cfg, E, HpSum>(q, HpSum::Params{s.sum, p.ld_sum, p.N * p.ld_sum, static_cast<int>(p.D), static_cast<int>(p.N), k == 0}, c.stream);
+      if (rc != AK_OK) return rc;
+    }
+    if (out.dw != nullptr) {
+      // i features, j classes, k rows
+      auto weight = [&](auto cfg) {
+        using Cfg = decltype(cfg);
+        const HpProblem q = hp_problem<Cfg>(hp_operand(c.h, c.ldh, p.N, p.D, false), hp_operand(d, p.piece, p.N, padded, false), p.D, width, p.N);
+        typename HpStore<E>::Params e{static_cast<E*>(out.dw) + c0 * p.D, p.D, static_cast<int>(p.D), static_cast<int>(width), 1.f, s.unit};
+        return hp_launch<Cfg, E, HpStore<E>>(q, e, c.stream);
+      };
+      rc = hp_wide(p.D, width) ? weight(HpWide<false, false>{}) : weight(HpSmall<false, false>{});
+      if (rc != AK_OK) return rc;
+    }
+    rc = lce_db(d, p.piece, p, c0, width, s, out, c.stream);
+    if (rc != AK_OK) return rc;
+  }
+  if (out.dh == nullptr) return AK_OK;
+  return hp_total(s.sum, p.ld_sum, p.N * p.ld_sum, p.splits, p.N, static_cast<int>(p.D), 1.f, s.unit, static_cast<E*>(out.dh), c.stream);
+}
+
+inline int lce_backward_f32(LceCall c, const float* lse, const LcePlan& p, const LceSpace& s, const LceGrads& out) {
+  float* x = reinterpret_cast<float*>(s.d);
+  const float *h = static_cast<const float*>(c.h), *w = static_cast<const float*>(c.w);
+  const int N = static_cast<int>(p.N), D = static_cast<int>(p.D);
+  for (int64_t k = 0; k < p.pieces; ++k) {
+    const int64_t c0 = k * p.piece, width = std::min(p.piece, p.V - c0);
+    auto product = [&](GemmParams g) {
+      g.split = 3;
+      return launch_gemm(g, 1, c.stream);
+    };
+    int rc = product(make_gemm(0, 1, N, static_cast<int>(width), D, 1.f, h, c.ldh, w + c0 * c.ldw, c.ldw, 0.f, x, p.piece));
+    if (rc != AK_OK) return rc;
+    hipLaunchKernelGGL(lce_piece_grad_kernel, dim3(static_cast<unsigned>(N)), dim3(256), 0, c.stream, x, p.piece, c.r, static_cast<int>(c0),
+                       static_cast<int>(width), lse, s.share);
+    if (out.dh != nullptr)
+      rc = product(make_gemm(0, 0, N, D, static_cast<int>(width), 1.f, x, p.piece, w + c0 * c.ldw, c.ldw, k == 0 ? 0.f : 1.f, static_cast<float*>(out.dh), D));
+    if (rc != AK_OK) return rc;
+    if (out.dw != nullptr)
+      rc = product(make_gemm(1, 0, static_cast<int>(width), D, N, 1.f, x, p.piece, h, c.ldh, 0.f, static_cast<float*>(out.dw) + c0 * p.D, D));
+    if (rc != AK_OK) return rc;
+    rc = lce_db(x, p.piece, p, c0, width, s, out, c.stream);
+    if (rc != AK_OK) return rc;
+  }
+  return check_launch();
+}
+
+inline int lce_check(const void* h, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype, const int64_t* targets, int64_t rows,
+                     int64_t classes, int64_t width, int dtype, int reduction) {
+  if (h == nullptr || w == nullptr || targets == nullptr || rows < 0 || classes <= 0 || width <= 0 || ldh < width || ldw < width) return AK_ERR_ARG;
+  if (!is_element_type(dtype) || (bias != nullptr && bias_dtype != AK_F32 && bias_dtype != dtype)) return AK_ERR_ARG;
+  if (reduction < kLossNone || reduction > kLossMean) return AK_ERR_ARG;
+  // counts in 32 bits; 256 rows of a panel within 32-bit byte offsets
+  if (rows > (1 << 28) || classes > (1 << 28) || width > (1 << 20) || ldh > (1 << 21) || ldw > (1 << 21)) return AK_ERR_TOO_LARGE;
+  return AK_OK;
+}
+
+}  // namespace ak
+
+extern "C" size_t ak_linear_cross_entropy_ws_bytes(int dtype, int64_t rows, int64_t classes, int64_t width, int backward) {
+  if (!ak::is_element_type(dtype) || rows <= 0 || classes <= 0 || width <= 0 || rows > (1 << 28) || classes > (1 << 28) || width > (1 << 20)) return 0;
+  const ak::LcePlan p = ak::lce_plan(dtype, rows, classes, width);
+  // enough for operands of any alignment
+  const bool pad = p.es == 2 && (backward != 0 || rows > ak::kLceFewRows);
+  return ak::lce_space(p, backward != 0, pad, pad, true, nullptr).bytes;
+}
+
+extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype,
+                                       const int64_t* targets, int64_t rows, int64_t classes, int64_t width, int64_t ignore_index, int reduction,
+                                       float* loss, float* lse, void* ws, size_t ws_bytes, ak_stream_t stream) {
+  using namespace ak;
+  int rc = lce_check(h, ldh, w, ldw, bias, bias_dtype, targets, rows, classes, width, dtype, reduction);
+  if (rc != AK_OK) return rc;
+  if (rows == 0) return reduction == kLossNone ? AK_OK : AK_ERR_ARG;
+  if (loss == nullptr || lse == nullptr) return AK_ERR_ARG;
+  const LcePlan p = lce_plan(dtype, rows, classes, width);
+  const bool few = p.es == 4 || rows <= kLceFewRows;
+  const LceSpace s = lce_space(p, false, !few && !hp_aligned(h, ldh, width), !few && !hp_aligned(w, ldw, width),
+                               bias != nullptr && bias_dtype != AK_F32, ws);
+  if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  LceCall c{h, ldh, w, ldw, bias, bias_dtype, LceRows{targets, nullptr, ignore_index, static_cast<int>(rows), static_cast<int>(classes)}, width, dtype, st};
+  rc = lce_bias(c, p, s);
+  if (rc != AK_OK) return rc;
+  int parts = 0;
+  rc = dtype == AK_F32 ? lce_forward_f32(c, p, s, &parts) : dtype == AK_BF16 ? lce_forward_half<__bf16>(c, p, s, &parts)
+                                                                             : lce_forward_half<_Float16>(c, p, s, &parts);
+  if (rc != AK_OK) return rc;
+  float* losses = reduction == kLossNone ? loss : s.losses;
+  hipLaunchKernelGGL(lce_rows_kernel, dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(1024), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
+  if (reduction != kLossNone) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, c.r, losses, reduction, loss);
+  return check_launch();
+}
+
+extern "C" int ak_linear_cross_entropy_backward(const float* g, const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias,
+                                                int bias_dtype, const int64_t* targets, const float* lse, int64_t rows, int64_t classes, int64_t width,
+                                                int64_t ignore_index, int reduction, void* dh, void* dw, void* db, void* ws, size_t ws_bytes,
+                                                ak_stream_t stream) {
+  using namespace ak;
+  int rc = lce_check(h, ldh, w, ldw, bias, bias_dtype, targets, rows, classes, width, dtype, reduction);
+  if (rc != AK_OK) return rc;
+  if (g == nullptr || lse == nullptr || rows == 0) return AK_ERR_ARG;
+  if (dh == nullptr && dw == nullptr && db == nullptr) return AK_OK;
+  const LcePlan p = lce_plan(dtype, rows, classes, width);
+  const bool half = p.es == 2;
+  const LceSpace s = lce_space(p, true, half && !hp_aligned(h, ldh, width), half && !hp_aligned(w, ldw, width),
+                               bias != nullptr && bias_dtype != AK_F32, ws);
+  if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  LceCall c{h, ldh, w, ldw, bias, bias_dtype, LceRows{targets, nullptr, ignore_index, static_cast<int>(rows), static_cast<int>(classes)}, width, dtype, st};
+  rc = lce_bias(c, p, s);
+  if (rc != AK_OK) return rc;
+  hipLaunchKernelGGL(lce_shares_kernel, dim3(1), dim3(1024), 0, st, c.r, g, reduction, half ? 0 : 1, dtype == AK_F16 ? 14 : 0, s.share, s.unit);
+  const LceGrads out{dh, dw, db, bias == nullptr ? dtype : bias_dtype};
+  return !half ? lce_backward_f32(c, lse, p, s, out) : dtype == AK_BF16 ? lce_backward_half<__bf16>(c, lse, p, s, out)
+                                                                        : lce_backward_half<_Float16>(c, lse, p, s, out);
+}

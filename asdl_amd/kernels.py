@@ -9,6 +9,7 @@ import contextlib
 import ctypes
 import struct
 import threading
+import typing
 
 import torch
 
@@ -1617,6 +1618,327 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, outs=None):
         raise ValueError(f'{len(grads)} gradients and {len(outs)} results.')
     with _device_of(grads[0].device):
         return _launch_norm(grads, outs, norm_type, max_norm)
+
+
+# ------------------------------------------------------------------------------ cross entropy of a linear layer
+_REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
+
+
+def _like_first(t, what, device):
+    if t.device != device:
+        _require_gpu(t)
+        _require_one_gpu(device, **{what: t})
+
+
+def _loss_operands(h, weight, targets, bias, reduction):
+    """(type code, rows, classes, features, code of the reduction) of a linear cross entropy."""
+    code = _ELEMENT_TYPES.get(h.dtype)
+    if code is None or not h.is_cuda:
+        _require_gpu(h)
+        _element_type(h, 'h')
+    if h.ndim == 0 or h.shape[-1] == 0:
+        raise ValueError(f'h has to have features in its last dimension. Got the shape {tuple(h.shape)}.')
+    D = h.shape[-1]
+    if weight.ndim != 2 or weight.shape[1] != D or weight.shape[0] == 0:
+        raise ValueError(f'weight has to be [classes, {D}]. Got {tuple(weight.shape)}.')
+    if weight.dtype != h.dtype:
+        raise TypeError(f'h and weight have to be of one type. Got {h.dtype} and {weight.dtype}.')
+    if targets.dtype != torch.int64 or targets.shape != h.shape[:-1]:
+        raise ValueError(f'targets have to be int64 of the shape {tuple(h.shape[:-1])}. Got {targets.dtype}, {tuple(targets.shape)}.')
+    if bias is not None:
+        if bias.shape != weight.shape[:1]:
+            raise ValueError(f'bias has to have the shape {tuple(weight.shape[:1])}. Got {tuple(bias.shape)}.')
+        if bias.dtype != torch.float32 and bias.dtype != h.dtype:
+            raise TypeError(f'bias has to be {h.dtype} or float32. Got {bias.dtype}.')
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f'reduction has to be one of {list(_REDUCTIONS)}. Got {reduction!r}.')
+    for what, t in (('weight', weight), ('targets', targets), ('bias', bias)):
+        if t is not None:
+            _like_first(t, what, h.device)
+    return code, targets.numel(), weight.shape[0], D, _REDUCTIONS[reduction]
+
+
+def linear_cross_entropy(h, weight, targets, bias=None, ignore_index=-100, reduction='mean'):
+    """(loss, lse) of torch.nn.functional.cross_entropy(h @ weight.t() + bias, targets) without the logits, which are formed in pieces and
+    not kept.  h [..., features], weight [classes, features]: both float32, bfloat16 or float16, rows of any stride; bias (may be None)
+    of their type or float32; targets [...] int64.  loss (float32): one number, or one per row with reduction='none'.  Rows whose target is
+    ``ignore_index`` have none; a target that is neither it nor a class gives NaN (the host does not look at targets).  lse (float32, one
+    per row, the log of the sum of exponentials) is what linear_cross_entropy_backward() needs."""
+    code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, reduction)
+    device = h.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return linear_cross_entropy(h, weight, targets, bias, ignore_index, reduction)
+    empty = _allocator()
+    lse = empty(targets.shape, dtype=torch.float32, device=device)
+    loss = empty(targets.shape if kind == 0 else (), dtype=torch.float32, device=device)
+    if rows == 0:
+        with _on_launch_stream():
+            return loss if kind == 0 else loss.fill_(0.0 if kind == 1 else float('nan')), lse
+    h, ldh = _rows_of(h, D)
+    weight, ldw = _rows_of(weight, D)
+    targets = _contiguous(targets)
+    bias = None if bias is None else _contiguous(bias)
+    need = _ws_need('ak_linear_cross_entropy_ws_bytes', code, rows, classes, D, 0)
+    ws = empty(need, dtype=torch.uint8, device=device)         # (not workspace(): a graph that is captured has its own)
+    rc = _lib.load().ak_linear_cross_entropy(h.data_ptr(), code, ldh, weight.data_ptr(), ldw, _pointer(bias), code if bias is None else _ELEMENT_TYPES[bias.dtype],
+                                             targets.data_ptr(), rows, classes, D, ignore_index, kind, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), need,
+                                             _stream_handle(device))
+    _lib.check(rc, 'ak_linear_cross_entropy')
+    return loss, lse
+
+
+def linear_cross_entropy_backward(g, h, weight, targets, lse, bias=None, ignore_index=-100, reduction='mean', need_h=True, need_weight=True,
+                                  need_bias=True):
+    """(dh, dw, db) of linear_cross_entropy() for the gradient ``g`` (float32, of the loss's shape); None for what is not needed.  They have the
+    types of h, weight and bias.  The logits are formed again, in pieces; for 16-bit operands their gradient, which both products read, is
+    rounded to the operands' type, as a framework's backward pass in that type does."""
+    code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, reduction)
+    for what, t, shape in (('g', g, targets.shape if kind == 0 else ()), ('lse', lse, targets.shape)):
+        if t.dtype != torch.float32 or t.shape != shape:
+            raise ValueError(f'{what} has to be float32 of the shape {tuple(shape)}. Got {t.dtype}, {tuple(t.shape)}.')
+        _like_first(t, what, h.device)
+    device = h.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return linear_cross_entropy_backward(g, h, weight, targets, lse, bias, ignore_index, reduction, need_h, need_weight, need_bias)
+    empty = _allocator()
+    dh = empty(h.shape, dtype=h.dtype, device=device) if need_h else None
+    dw = empty(weight.shape, dtype=weight.dtype, device=device) if need_weight else None
+    db = empty(bias.shape, dtype=bias.dtype, device=device) if need_bias and bias is not None else None
+    if rows == 0:
+        with _on_launch_stream():
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        return dh, dw, db
+    if dh is None and dw is None and db is None:
+        return dh, dw, db
+    h, ldh = _rows_of(h, D)
+    weight, ldw = _rows_of(weight, D)
+    targets, g, lse = _contiguous(targets), _contiguous(g), _contiguous(lse)
+    bias = None if bias is None else _contiguous(bias)
+    need = _ws_need('ak_linear_cross_entropy_ws_bytes', code, rows, classes, D, 1)
+    ws = empty(need, dtype=torch.uint8, device=device)
+    rc = _lib.load().ak_linear_cross_entropy_backward(
+        g.data_ptr(), h.data_ptr(), code, ldh, weight.data_ptr(), ldw, _pointer(bias), code if bias is None else _ELEMENT_TYPES[bias.dtype],
+        targets.data_ptr(), lse.data_ptr(), rows, classes, D, ignore_index, kind, _pointer(dh), _pointer(dw), _pointer(db), ws.data_ptr(), need,
+        _stream_handle(device))
+    _lib.check(rc, 'ak_linear_cross_entropy_backward')
+    return dh, dw, db
+
+
+# ------------------------------------------------------------------------------ embedding
+_TOKEN_TYPES = {torch.int32: 5, torch.int64: 6}
+
+
+def _tokens_of(tokens, device):
+    code = _TOKEN_TYPES.get(tokens.dtype)
+    if code is None:
+        raise TypeError(f'tokens have to be int32 or int64. Got {tokens.dtype}.')
+    _like_first(tokens, 'tokens', device)
+    return code, _contiguous(tokens)
+
+
+def embedding(tokens, weight, scale=1.0, out_dtype=None):
+    """scale * weight[tokens]: rows of ``weight`` [rows, features] (float32, bfloat16 or float16, any row stride) for int32 or int64 ``tokens``
+    of any shape, in weight's type, or float32 with ``out_dtype=torch.float32``; rounded once.  A token that names no row gives a row of NaN (the host
+    does not look at tokens)."""
+    code = _ELEMENT_TYPES.get(weight.dtype)
+    if code is None or not weight.is_cuda:
+        _require_gpu(weight)
+        _element_type(weight, 'weight')
+    if weight.ndim != 2 or weight.shape[1] == 0:
+        raise ValueError(f'weight has to be [rows, features]. Got {tuple(weight.shape)}.')
+    if out_dtype is None:
+        out_dtype = weight.dtype
+    elif out_dtype != weight.dtype and out_dtype != torch.float32:
+        raise TypeError(f'the result is {weight.dtype} or float32. Got {out_dtype}.')
+    device, (rows, D) = weight.device, weight.shape
+    token_code, tokens = _tokens_of(tokens, device)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return embedding(tokens, weight, scale, out_dtype)
+    weight, ld = _rows_of(weight, D)
+    out = _allocator()((*tokens.shape, D), dtype=out_dtype, device=device)
+    rc = _lib.load().ak_embedding(tokens.data_ptr(), token_code, tokens.numel(), weight.data_ptr(), code, ld, rows, D, scale, out.data_ptr(),
+                                  _ELEMENT_TYPES[out_dtype], _stream_handle(device))
+    _lib.check(rc, 'ak_embedding')
+    return out
+
+
+def embedding_backward(g, tokens, num_embeddings, scale=1.0, padding_idx=None, out=None, beta=0.0, dtype=None):
+    """The gradient of embedding()'s weight, [num_embeddings, features], for the gradient ``g`` [*tokens.shape, features] of its result:
+    out <- beta*out + scale * (sums of the rows of g of each token), by tokens in sorted order: fp32 sums in an order that does not change,
+    each row rounded once.  Without ``out`` it is made, of the type ``dtype`` (g's); with it, ``out`` has rows of stride 1 elements (float32,
+    bfloat16 or float16).  Rows that no token names are written, too (with beta = 1 they stay).  ``padding_idx``: a token that adds nothing,
+    as tokens that name no row do."""
+    code = _ELEMENT_TYPES.get(g.dtype)
+    if code is None or not g.is_cuda:
+        _require_gpu(g)
+        _element_type(g, 'g')
+    if g.ndim == 0 or g.shape[-1] == 0 or g.shape[:-1] != tokens.shape:
+        raise ValueError(f'g has to have the shape {(*tokens.shape, "features")}. Got {tuple(g.shape)}.')
+    D, rows, device = g.shape[-1], int(num_embeddings), g.device
+    if rows < 0:
+        raise ValueError(f'num_embeddings has to be at least 0. Got {rows}.')
+    if padding_idx is None:
+        padding = -1
+    else:
+        padding = padding_idx + rows if padding_idx < 0 else padding_idx
+        if not 0 <= padding < rows:
+            raise ValueError(f'padding_idx has to be within {rows} rows. Got {padding_idx}.')
+    token_code, tokens = _tokens_of(tokens, device)
+    if out is not None:
+        if out.shape != (rows, D) or out.stride(1) != 1 or (rows > 1 and out.stride(0) < D):
+            raise ValueError(f'out has to be [{rows}, {D}] with contiguous rows. Got {tuple(out.shape)}, strides {out.stride()}.')
+        _element_type(out, 'out')
+        _like_first(out, 'out', device)
+        if dtype is not None and dtype != out.dtype:
+            raise TypeError(f'out is {out.dtype}, not {dtype}.')
+    elif dtype is not None and dtype not in _ELEMENT_TYPES:
+        raise TypeError(f'the gradient is float32, bfloat16 or float16. Got {dtype}.')
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return embedding_backward(g, tokens, rows, scale, padding_idx, out, beta, dtype)
+    empty = _allocator()
+    if out is None:
+        out, beta = empty((rows, D), dtype=dtype or g.dtype, device=device), 0.0
+    g, ldg = _rows_of(g, D)
+    need = _ws_need('ak_embedding_backward_ws_bytes', tokens.numel(), rows, D)
+    ws = empty(need, dtype=torch.uint8, device=device)
+    rc = _lib.load().ak_embedding_backward(g.data_ptr(), code, ldg, tokens.data_ptr(), token_code, tokens.numel(), rows, D, scale, padding, beta,
+                                           out.data_ptr(), _ELEMENT_TYPES[out.dtype], max(out.stride(0), D), ws.data_ptr(), need, _stream_handle(device))
+    _lib.check(rc, 'ak_embedding_backward')
+    return out
+
+
+# ------------------------------------------------------------------------------ activations in 8 bits
+class Quantized8(typing.NamedTuple):
+    """Activations in 8 bits: a value stands for code * 2^exponent.  Blocks of 128 features of a row share an exponent."""
+    codes: torch.Tensor          # float8_e4m3fn, the activations' shape
+    exponents: torch.Tensor      # int8, [..., ceil(features / 128)]
+
+
+_GELU = {'none': 0, 'tanh': 1}
+
+
+def _gelu_code(approximate):
+    if approximate not in _GELU:
+        raise ValueError(f'approximate has to be one of {list(_GELU)}. Got {approximate!r}.')
+    return _GELU[approximate]
+
+
+def _quantize(x, gelu):
+    code, F, rows = _norm_rows(x)
+    device = x.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _quantize(x, gelu)
+    empty = _allocator()
+    kept = Quantized8(empty(x.shape, dtype=torch.float8_e4m3fn, device=device), empty((*x.shape[:-1], -(-F // 128)), dtype=torch.int8, device=device))
+    y = empty(x.shape, dtype=x.dtype, device=device) if gelu >= 0 else None
+    x, ld = _rows_of(x, F)
+    rc = _lib.load().ak_quantize_8bit(x.data_ptr(), code, ld, rows, F, gelu, _pointer(y), kept.codes.data_ptr(), kept.exponents.data_ptr(),
+                                      _stream_handle(device))
+    _lib.check(rc, 'ak_quantize_8bit')
+    return y, kept
+
+
+def _check_kept(kept):
+    """(rows, features) of a Quantized8."""
+    codes, exponents = kept
+    _require_gpu(codes, exponents)
+    if codes.dtype != torch.float8_e4m3fn or exponents.dtype != torch.int8 or not codes.is_contiguous() or not exponents.is_contiguous() or \
+            codes.ndim == 0 or codes.shape[-1] == 0 or exponents.shape != (*codes.shape[:-1], -(-codes.shape[-1] // 128)):
+        raise ValueError('the kept activations have to be the contiguous float8_e4m3fn codes and int8 exponents of quantize_8bit().')
+    _require_one_gpu(codes.device, exponents=exponents)
+    return codes.numel() // codes.shape[-1], codes.shape[-1]
+
+
+def quantize_8bit(x):
+    """``x`` (float32, bfloat16 or float16, any row stride) in 8 bits, for the backward pass: a block of 128 features of a row shares a power of
+    two, the least 2^e with max |x| 2^-e <= 448 (e within -127 .. 127), and a value is the nearest e4m3 number (ties to even) times it:
+    off by at most 2^-4 of itself, or 2^(e - 10).  Infinities and NaN become NaN and do not count for e; what would be rounded to 2^128 is
+    kept as 1.875 * 2^127."""
+    return _quantize(x, -1)[1]
+
+
+def dequantize_8bit(kept, dtype=torch.float32):
+    """The values that quantize_8bit() has kept, as float32, bfloat16 (both exact within float32's range) or float16."""
+    return _dequantize(kept, -1, None, dtype)
+
+
+def gelu_8bit(x, approximate='none'):
+    """(gelu(x), quantize_8bit(x)) in one pass; ``approximate``: 'none' or 'tanh', as torch.nn.functional.gelu."""
+    return _quantize(x, _gelu_code(approximate))
+
+
+def gelu_8bit_backward(g, kept, approximate='none'):
+    """The gradient of gelu_8bit()'s input for the gradient ``g`` of its result, from the kept input: g times the derivative at the kept
+    values, of the type of g."""
+    way = _gelu_code(approximate)
+    _check_kept(kept)
+    if g.shape != kept.codes.shape:
+        raise ValueError(f'shapes differ: {tuple(g.shape)} vs {tuple(kept.codes.shape)}')
+    _like_first(g, 'g', kept.codes.device)
+    return _dequantize(kept, way, g, g.dtype)
+
+
+def _dequantize(kept, gelu, g, dtype):
+    rows, F = _check_kept(kept)
+    code = _ELEMENT_TYPES.get(dtype)
+    if code is None:
+        raise TypeError(f'the values are float32, bfloat16 or float16. Got {dtype}.')
+    device = kept.codes.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _dequantize(kept, gelu, g, dtype)
+    ld = F
+    if g is not None:
+        g, ld = _rows_of(g, F)
+    out = _allocator()(kept.codes.shape, dtype=dtype, device=device)
+    rc = _lib.load().ak_dequantize_8bit(kept.codes.data_ptr(), kept.exponents.data_ptr(), rows, F, gelu, _pointer(g), ld, out.data_ptr(), code,
+                                        _stream_handle(device))
+    _lib.check(rc, 'ak_dequantize_8bit')
+    return out
+
+
+def weight_grad_8bit(g, kept, need_weight=True, need_bias=True, dtype=None):
+    """(dw, db) of a linear layer whose input was kept with quantize_8bit(): dw = g^T x [out, features] and db = the sums of g [out], for the
+    gradient ``g`` [..., out] of its result (float32, bfloat16 or float16, any row stride); None for what is not needed.  ``dtype``: of both (g's).
+    The products are exact (the kept values and the pieces that g is taken apart into are bfloat16 numbers), their sums fp32."""
+    rows, F = _check_kept(kept)
+    code = _ELEMENT_TYPES.get(g.dtype)
+    if code is None or not g.is_cuda:
+        _require_gpu(g)
+        _element_type(g, 'g')
+    if g.ndim == 0 or g.shape[-1] == 0 or g.shape[:-1] != kept.codes.shape[:-1]:
+        raise ValueError(f'g has to have the shape {(*kept.codes.shape[:-1], "out")}. Got {tuple(g.shape)}.')
+    dtype = dtype or g.dtype
+    if dtype not in _ELEMENT_TYPES:
+        raise TypeError(f'the gradients are float32, bfloat16 or float16. Got {dtype}.')
+    device, n = g.device, g.shape[-1]
+    _like_first(kept.codes, 'the kept input', device)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return weight_grad_8bit(g, kept, need_weight, need_bias, dtype)
+    empty = _allocator()
+    dw = empty((n, F), dtype=dtype, device=device) if need_weight else None
+    db = empty(n, dtype=dtype, device=device) if need_bias else None
+    if rows == 0 or (dw is None and db is None):
+        with _on_launch_stream():
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        return dw, db
+    g, ld = _rows_of(g, n)
+    need = _ws_need('ak_weight_grad_8bit_ws_bytes', code, rows, F, n)
+    ws = empty(need, dtype=torch.uint8, device=device)
+    rc = _lib.load().ak_weight_grad_8bit(g.data_ptr(), code, ld, kept.codes.data_ptr(), kept.exponents.data_ptr(), rows, F, n, _pointer(dw), _pointer(db),
+                                         _ELEMENT_TYPES[dtype], ws.data_ptr(), need, _stream_handle(device))
+    _lib.check(rc, 'ak_weight_grad_8bit')
+    return dw, db
 
 
 # ------------------------------------------------------------------------------ low-rank (swift) factors

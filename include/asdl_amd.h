@@ -43,7 +43,10 @@ extern "C" {
                               * for statistics whose inverse roots are taken with a ridge of 1e-6 of the largest eigenvalue,
                               * where another order moves the root of a rank-deficient statistic by 0.5-1 % */
 
-#define AK_F16 4             /* IEEE half: ak_layer_norm*, ak_grad_norm, ak_clip_grad_norm, ak_sample_filtered */
+#define AK_F16 4             /* IEEE half: ak_layer_norm*, ak_grad_norm, ak_clip_grad_norm, ak_sample_filtered, ak_linear_cross_entropy*,
+                              * ak_embedding*, ak_*_8bit */
+#define AK_I32 5             /* tokens of ak_embedding* */
+#define AK_I64 6
 
 #define AK_OK 0
 #define AK_ERR_ARG -1        /* null pointer, negative size, unknown dtype */
@@ -501,6 +504,52 @@ int ak_inv_root_group(int phases, int iters, int groups, float* const* S, const 
                       const int64_t* strideS, const int* p, float ridge_eps, const float* const* v0, int max_power_iter,
                       float power_tol, int max_iter, float tol, float* const* out, const int64_t* strideOut,
                       float* const* stats, void* ws, size_t ws_bytes, ak_stream_t stream);
+
+/* ---- the vocabulary's ends and the activations of a decoder's training step (no counterpart in the reference) ------------------ */
+
+/* Softmax cross entropy of a linear layer, without its logits: s = h w^T + bias, lse_n = log sum_v exp s_nv, loss_n = lse_n - s_n,target(n);
+ * rows whose target is ignore_index have no loss and no gradient, a target that is neither it nor a class gives NaN.
+ * h [rows, width], w [classes, width]: one type (AK_F32, AK_BF16, AK_F16); bias [classes] (may be null): that type or AK_F32;
+ * targets int64.  reduction 0: loss [rows]; 1: loss [1], their sum; 2: loss [1], their mean over the rows that are not ignored.  lse [rows]
+ * is what the backward pass needs.  g: gradient of the loss, [rows] or [1]; dh [rows, width], dw [classes, width] (dense rows) of the
+ * type of h, db [classes] of the bias's type; each may be null.  Sums and exponentials are fp32; 16-bit operands: the gradient
+ * of the logits is rounded to their type.  The workspace (enough for either alignment; backward != 0: for the backward pass) holds a piece
+ * of the logits' gradient of at most 256 MB, or 256 classes, and copies of 16-bit operands whose width is no multiple of eight or whose rows
+ * are not 16-byte aligned.  rows, classes <= 2^28, width <= 2^20, row pitches <= 2^21, else AK_ERR_TOO_LARGE. */
+size_t ak_linear_cross_entropy_ws_bytes(int dtype, int64_t rows, int64_t classes, int64_t width, int backward);
+int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype,
+                            const int64_t* targets, int64_t rows, int64_t classes, int64_t width, int64_t ignore_index, int reduction,
+                            float* loss, float* lse, void* ws, size_t ws_bytes, ak_stream_t stream);
+int ak_linear_cross_entropy_backward(const float* g, const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias,
+                                     int bias_dtype, const int64_t* targets, const float* lse, int64_t rows, int64_t classes, int64_t width,
+                                     int64_t ignore_index, int reduction, void* dh, void* dw, void* db, void* ws, size_t ws_bytes,
+                                     ak_stream_t stream);
+
+/* out[n] = scale * table[tokens[n]], rows of `width` elements (out: dense, of the table's type or AK_F32); a token that names no row
+ * gives a row of NaN.  Backward: out[v] <- beta*out[v] + scale * sum of g[n] over n with tokens[n] = v, summed in fp32 in ascending order
+ * of n (in parts of up to 64 positions of the sorted tokens), for every row; tokens that name no row, and the token `padding` (-1: none),
+ * add nothing.  g and out: any two of AK_F32, AK_BF16, AK_F16.  beta == 0 never reads out. */
+int ak_embedding(const void* tokens, int token_type, int64_t count, const void* table, int dtype, int64_t ld, int64_t rows, int64_t width,
+                 float scale, void* out, int out_dtype, ak_stream_t stream);
+size_t ak_embedding_backward_ws_bytes(int64_t count, int64_t rows, int64_t width);
+int ak_embedding_backward(const void* g, int dtype, int64_t ldg, const void* tokens, int token_type, int64_t count, int64_t rows,
+                          int64_t width, float scale, int64_t padding, float beta, void* out, int out_dtype, int64_t ldo, void* ws,
+                          size_t ws_bytes, ak_stream_t stream);
+
+/* Activations in 8 bits: codes [rows, width] (e4m3, dense) and exponents [rows, ceil(width / 128)]; a value of a block of 128 features of
+ * a row stands for code * 2^e, e the least integer with max |x| 2^-e <= 448, within -127 .. 127 (infinities and NaN: kept as NaN, not
+ * counted for e; what would be rounded to 2^128: kept as 1.875 * 2^127).  gelu 0 or 1: y (dense, the type of x) = x times the normal distribution's share below x or its approximation by tanh
+ * in the same pass; -1: y is not written.
+ * ak_dequantize_8bit, gelu -1: y (dense) = the kept values; 0 or 1: y = g * derivative of that function at the kept values.
+ * ak_weight_grad_8bit: dw [out, width] = g^T x', db [out] = sums of g over the rows, x' the kept values; each may be null, g [rows, out].
+ * The products of g's pieces with x' are exact, their sums fp32. */
+int ak_quantize_8bit(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t width, int gelu, void* y, uint8_t* codes, int8_t* exponents,
+                     ak_stream_t stream);
+int ak_dequantize_8bit(const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width, int gelu, const void* g, int64_t ldg,
+                       void* y, int dtype, ak_stream_t stream);
+size_t ak_weight_grad_8bit_ws_bytes(int dtype, int64_t rows, int64_t width, int64_t out);
+int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width,
+                        int64_t out, void* dw, void* db, int grad_dtype, void* ws, size_t ws_bytes, ak_stream_t stream);
 
 /* ---- stream helpers (no counterpart in the reference) ------------------------------------ */
 
