@@ -4,7 +4,7 @@
 // row": row k holds all i or j).  A work group has one BI x BJ tile of D; a lane of a wave has, for every 32 x 32 block, one column j and
 // 16 rows i, four of them consecutive: an epilogue that writes D transposed writes four neighbouring elements, one that reduces over i
 // stays in the lane.
-// Panels of 32 k go from memory to the LDS without passing registers (syrk_dtl_tile.hpp: load_to_lds), kHpStages of them in flight.  Both
+// Panels of 32 k go from memory to the LDS without passing registers (syrk_dtl_tile.hpp: load_to_lds), Cfg::STAGES of them in flight.  Both
 // kinds of panel are blocks of 2 KB, 32 rows of 64 bytes:
 //   by k:   [32 i][32 k], 16-byte chunks of a row exchanged by (row / 4) % 4, so that the 16 rows a ds_read_b128 serves at once lie in
 //           different banks; the exchange is made on the memory side of the load, within the 64 bytes of a row
@@ -18,8 +18,6 @@
 #include "syrk_dtl_tile.hpp"
 
 namespace ak {
-
-constexpr int kHpStages = 4;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -45,12 +43,12 @@ struct HpProblem {
   int tiles_i, tiles_j, splits;
 };
 
-template <int WR_, int WC_, int FR_, int FC_, bool A_BY_K_, bool B_BY_K_>
+template <int WR_, int WC_, int FR_, int FC_, bool A_BY_K_, bool B_BY_K_, int STAGES_>
 struct HpCfg {
-  static constexpr int WR = WR_, WC = WC_, FR = FR_, FC = FC_, NW = WR * WC, THREADS = 64 * NW;
+  static constexpr int WR = WR_, WC = WC_, FR = FR_, FC = FC_, NW = WR * WC, THREADS = 64 * NW, STAGES = STAGES_;
   static constexpr bool A_BY_K = A_BY_K_, B_BY_K = B_BY_K_;
   static constexpr int BI = 32 * FR * WR, BJ = 32 * FC * WC, BK = 32;
-  static constexpr int BLOCK = 2048, PANEL_A = BI * 64, PANEL_B = BJ * 64, STAGE = PANEL_A + PANEL_B, LDS_BYTES = kHpStages * STAGE;
+  static constexpr int BLOCK = 2048, PANEL_A = BI * 64, PANEL_B = BJ * 64, STAGE = PANEL_A + PANEL_B, LDS_BYTES = STAGES * STAGE;
   static constexpr int IA = BI / 16 / NW, IB = BJ / 16 / NW, LPT = IA + IB;      // wave-wide loads of a k-tile, per wave
   static_assert(BI / 16 % NW == 0 && BJ / 16 % NW == 0 && LDS_BYTES <= 160 * 1024, "loads split evenly, panels fit the LDS");
 };
@@ -131,27 +129,33 @@ __device__ __forceinline__ short8v hp_read(AK_LDS const unsigned char* q) {
   return short8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// The tile (ti, tj) of D over k0 .. k0 + k_count: acc[a][b], block (FR wr + a, FC wc + b) of the tile.
-template <class Cfg, typename E>
-__device__ __forceinline__ void hp_tile(const HpProblem& p, int ti, int tj, int64_t k0, int64_t k_count, floatx16 (&acc)[Cfg::FR][Cfg::FC]) {
-  constexpr int FR = Cfg::FR, FC = Cfg::FC, S = kHpStages, LPT = Cfg::LPT;
+// Tiles in groups of eight along i, so that the tiles an XCD works on at a time share panels in its L2.
+__device__ __forceinline__ void hp_place(int id, int tiles_i, int tiles_j, int& ti, int& tj) {
+  constexpr int GROUP = 8;
+  const int per = GROUP * tiles_j, group = id / per, i0 = group * GROUP, height = min(GROUP, tiles_i - i0), rest = id - group * per;
+  ti = i0 + rest % height;
+  tj = rest / height;
+}
+
+// One tile of D.  The loop alone sustains 1.3 PFLOP/s (512 k-tiles of 256 x 256, both operands by row), where the device is at its power
+// limit (1.9 GHz).  A work group that goes on to another tile, with its loads running on into that one under the epilogue, was not
+// faster: 649 -> 626 us for the 6304 tiles of 24 k-tiles of a 50257-class forward pass, but 1982 -> 2068 us for 8000 of 64.
+template <class Cfg, typename E, class Epilogue>
+__device__ __forceinline__ void hp_run(const HpProblem& p, const typename Epilogue::Params& e, uint32_t block, uint32_t blocks) {
+  constexpr int FR = Cfg::FR, FC = Cfg::FC, S = Cfg::STAGES, LPT = Cfg::LPT;
   extern __shared__ __attribute__((aligned(1024))) unsigned char hp_smem[];
   AK_LDS unsigned char* lds = (AK_LDS unsigned char*)hp_smem;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave / Cfg::WC, wc = wave % Cfg::WC;
-
+  const int tiles = p.tiles_i * p.tiles_j, id = static_cast<int>(xcd_contiguous_id(block, blocks)), split = id / tiles;
+  int ti, tj;
+  hp_place(id - split * tiles, p.tiles_i, p.tiles_j, ti, tj);
+  const int64_t k0 = split * p.k_per_split, k_count = p.K - k0 < p.k_per_split ? p.K - k0 : p.k_per_split;
   HpLoader<Cfg::A_BY_K, Cfg::IA> la;
   HpLoader<Cfg::B_BY_K, Cfg::IB> lb;
   la.init(p.A, wave, lane, ti * Cfg::BI, k0, k_count);
   lb.init(p.B, wave, lane, tj * Cfg::BJ, k0, k_count);
-#pragma unroll
-  for (int a = 0; a < FR; ++a)
-#pragma unroll
-    for (int b = 0; b < FC; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
-
   auto load_one = [&](int l, int stage) {
     const uint32_t at = lds0 + stage * Cfg::STAGE;
     if (l < Cfg::IA) la.load(l, at);
@@ -167,6 +171,7 @@ __device__ __forceinline__ void hp_tile(const HpProblem& p, int ti, int tj, int6
     if (u == 0 || u > FC) fa[u == 0 ? 0 : u - FC] = hp_read<Cfg::A_BY_K>(pa + s + (u == 0 ? 0 : u - FC) * Cfg::BLOCK + fa_off[kk]);
     else fb[u - 1] = hp_read<Cfg::B_BY_K>(pb + s + (u - 1) * Cfg::BLOCK + fb_off[kk]);
   };
+  floatx16 acc[FR][FC];
   // The matrix instructions of 16 k, with the reads of the next 16 and (LOADS) the loads of a k-tile further ahead spread between them.
   auto half_step = [&](auto loads_tag, const short8v (&ca)[FR], const short8v (&cb)[FC], short8v (&na)[FR], short8v (&nb)[FC], int stage,
                        int kk, int to) {
@@ -185,24 +190,30 @@ __device__ __forceinline__ void hp_tile(const HpProblem& p, int ti, int tj, int6
     }
   };
 
-  const int nk = static_cast<int>((k_count + 31) / 32);
 #pragma unroll
-  for (int t = 0; t < S - 1; ++t) {              // k-tiles beyond the last load zeros: the counts stay uniform
+  for (int a = 0; a < FR; ++a)
+#pragma unroll
+    for (int b = 0; b < FC; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) {              // k-tiles behind the last load zeros: the counts stay uniform
 #pragma unroll
     for (int l = 0; l < LPT; ++l) load_one(l, t);
     la.next();
     lb.next();
   }
-  wait_vmcnt<(S - 2) * LPT>();                   // this wave's loads of k-tile 0 have landed
+  wait_vmcnt<(S - 2) * LPT>();                   // this wave's loads of the first k-tile have landed
   __syncthreads();                               // ... and everybody's
   short8v fa0[FR], fb0[FC], fa1[FR], fb1[FC];
 #pragma unroll
   for (int u = 0; u < FR + FC; ++u) read_unit(fa0, fb0, 0, 0, u);
   int rd = 0, to = S - 1;
+  const int nk = static_cast<int>((k_count + 31) / 32);
   for (int kt = 0; kt < nk; ++kt) {
     half_step(std::integral_constant<int, 0>{}, fa0, fb0, fa1, fb1, rd, 1, 0);
-    wait_vmcnt<(S - 3) * LPT>();                 // own loads of k-tile kt + 1 have landed
-    __syncthreads();                             // everybody's have; nobody reads k-tile kt - 1 any more
+    wait_vmcnt<(S - 3) * LPT>();                 // own loads of the next k-tile have landed
+    __syncthreads();                             // everybody's have; nobody reads the k-tile before this one any more
     rd = (rd + 1 == S) ? 0 : rd + 1;
     half_step(std::integral_constant<int, LPT>{}, fa1, fb1, fa0, fb0, rd, 0, to);
     la.next();
@@ -210,29 +221,25 @@ __device__ __forceinline__ void hp_tile(const HpProblem& p, int ti, int tj, int6
     to = (to + 1 == S) ? 0 : to + 1;
   }
   wait_vmcnt<0>();                               // the loads of zeros have landed before the LDS is used again
-}
-
-// Tiles in groups of eight along i, so that the tiles an XCD works on at a time share panels in its L2.
-__device__ __forceinline__ void hp_place(int id, int tiles_i, int tiles_j, int& ti, int& tj) {
-  constexpr int GROUP = 8;
-  const int per = GROUP * tiles_j, group = id / per, i0 = group * GROUP, height = min(GROUP, tiles_i - i0), rest = id - group * per;
-  ti = i0 + rest % height;
-  tj = rest / height;
+  Epilogue::template run<Cfg>(e, acc, ti, tj, split, wr, wc, lds);
 }
 
 template <class Cfg, typename E, class Epilogue>
-static __global__ __launch_bounds__(Cfg::THREADS) void hp_kernel(HpProblem p, typename Epilogue::Params e) {
-  const int tiles = p.tiles_i * p.tiles_j;
-  const int id = static_cast<int>(xcd_contiguous_id(blockIdx.x, gridDim.x));
-  const int split = id / tiles;
-  int ti, tj;
-  hp_place(id - split * tiles, p.tiles_i, p.tiles_j, ti, tj);
-  const int64_t k0 = split * p.k_per_split;
-  const int64_t k_count = p.K - k0 < p.k_per_split ? p.K - k0 : p.k_per_split;
-  floatx16 acc[Cfg::FR][Cfg::FC];
-  hp_tile<Cfg, E>(p, ti, tj, k0, k_count, acc);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Epilogue::template run<Cfg>(e, acc, ti, tj, split, wave / Cfg::WC, wave % Cfg::WC);
+static __global__ __launch_bounds__(Cfg::THREADS, Cfg::FR * Cfg::FC > 8 ? 1 : 2) void hp_kernel(HpProblem p, typename Epilogue::Params e) {
+  hp_run<Cfg, E, Epilogue>(p, e, blockIdx.x, gridDim.x);
+}
+
+// Two products in one launch, the first work groups to the first: what one leaves of the device the other fills.
+template <class Cfg1, class Epilogue1, class Cfg2, class Epilogue2, typename E>
+static __global__ __launch_bounds__(Cfg1::THREADS, Cfg1::FR * Cfg1::FC > 8 ? 1 : 2) void hp_both_kernel(HpProblem p1, typename Epilogue1::Params e1, uint32_t blocks1,
+                                                                                                       HpProblem p2, typename Epilogue2::Params e2, uint32_t blocks2,
+                                                                                                       int second_first) {
+  static_assert(Cfg1::THREADS == Cfg2::THREADS && Cfg1::LDS_BYTES == Cfg2::LDS_BYTES, "one launch");
+  const uint32_t front = second_first ? blocks2 : blocks1;
+  const bool in_front = blockIdx.x < front;
+  const uint32_t block = in_front ? blockIdx.x : blockIdx.x - front;
+  if (in_front == (second_first != 0)) hp_run<Cfg2, E, Epilogue2>(p2, e2, block, blocks2);
+  else hp_run<Cfg1, E, Epilogue1>(p1, e1, block, blocks1);
 }
 
 // f(i, j, values of rows i .. i + 3) for a lane's part of the tile.
@@ -249,6 +256,45 @@ __device__ __forceinline__ void hp_quads(floatx16 (&acc)[Cfg::FR][Cfg::FC], int 
         f(i0 + 32 * a + 8 * q, j0 + 32 * b, floatx4{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]});
 }
 
+// f(i, j, eight values of rows i .. i + 7, as 16-bit elements of type T) for a lane's part of the tile, whose halves exchange their
+// quads of two neighbouring blocks of eight rows for that: 16-byte stores.  make(a, b, x): the value of register x of block (a, b).
+template <class Cfg, typename T, typename Make, typename F>
+__device__ __forceinline__ void hp_eights(int ti, int tj, int wr, int wc, Make&& make, F&& f) {
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int i0 = ti * Cfg::BI + 32 * Cfg::FR * wr + 8 * g, j0 = tj * Cfg::BJ + 32 * Cfg::FC * wc + l32;
+  typedef T vec2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int b = 0; b < Cfg::FC; ++b)
+#pragma unroll
+    for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {
+        u32x4 out;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const vec2 lo = {static_cast<T>(make(a, b, 4 * q + 2 * h)), static_cast<T>(make(a, b, 4 * q + 2 * h + 1))};
+          const vec2 hi = {static_cast<T>(make(a, b, 4 * q + 4 + 2 * h)), static_cast<T>(make(a, b, 4 * q + 5 + 2 * h))};
+          // lower lanes: (own quad of the first block, the upper lanes' of it); upper lanes: (the lower lanes' of the second block, own)
+          const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi), false, false);
+          out[h] = both[0];
+          out[2 + h] = both[1];
+        }
+        f(i0 + 32 * a + 8 * q, j0 + 32 * b, out);
+      }
+}
+
+// Up to eight 16-bit elements of a row that ends at element `end`.
+template <typename T>
+__device__ __forceinline__ void hp_store8(T* __restrict__ row, int i, int end, u32x4 v) {
+  if (i + 8 <= end) {
+    __builtin_memcpy(row + i, &v, 16);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 7; ++k)
+      if (i + k < end) row[i + k] = __builtin_bit_cast(T, static_cast<unsigned short>(v[k >> 1] >> 16 * (k & 1)));
+  }
+}
+
 // out[j][i] = scale * D[i][j] as T
 template <typename T>
 struct HpStore {
@@ -260,22 +306,28 @@ struct HpStore {
     const float* factor;     // optional further one, on the device
   };
   template <class Cfg>
-  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc) {
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc,
+                                             AK_LDS unsigned char*) {
     const float s = e.factor != nullptr ? e.scale * *e.factor : e.scale;
-    hp_quads<Cfg>(acc, ti, tj, wr, wc, [&](int i, int j, floatx4 v) {
-      if (j >= e.J || i >= e.I) return;
-      T* __restrict__ to = e.out + static_cast<int64_t>(j) * e.ldo + i;
-      Some<T, 4> some;
+    if constexpr (sizeof(T) == 2) {
+      hp_eights<Cfg, T>(ti, tj, wr, wc, [&](int a, int b, int x) { return acc[a][b][x] * s; },
+                        [&](int i, int j, u32x4 v) {
+                          if (j < e.J && i < e.I) hp_store8(e.out + static_cast<int64_t>(j) * e.ldo, i, e.I, v);
+                        });
+    } else {
+      hp_quads<Cfg>(acc, ti, tj, wr, wc, [&](int i, int j, floatx4 v) {
+        if (j >= e.J || i >= e.I) return;
+        T* __restrict__ to = e.out + static_cast<int64_t>(j) * e.ldo + i;
+        v *= s;
+        if (i + 4 <= e.I) {
+          __builtin_memcpy(to, &v, 16);
+        } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) some.set(k, v[k] * s);
-      if (i + 4 <= e.I) {
-        some.store(to);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          if (i + k < e.I) to[k] = some.v[k];
-      }
-    });
+          for (int k = 0; k < 3; ++k)
+            if (i + k < e.I) to[k] = v[k];
+        }
+      });
+    }
   }
 };
 
@@ -287,7 +339,8 @@ struct HpSum {
     int I, J, first;         // first: set, else add
   };
   template <class Cfg>
-  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int split, int wr, int wc) {
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int split, int wr, int wc,
+                                             AK_LDS unsigned char*) {
     float* __restrict__ sum = e.sum + split * e.stride;
     const bool first = e.first != 0;
     hp_quads<Cfg>(acc, ti, tj, wr, wc, [&](int i, int j, floatx4 v) {
@@ -381,29 +434,56 @@ struct Carver {
 };
 
 template <bool A_BY_K, bool B_BY_K>
-using HpWide = HpCfg<2, 4, 4, 2, A_BY_K, B_BY_K>;      // 256 x 256
+using HpWide = HpCfg<2, 4, 4, 2, A_BY_K, B_BY_K, 4>;      // 256 x 256
+// 256 x 256 by four waves of 128 x 128, one a SIMD, for long contractions: a third less of the LDS is read for a product (the product of
+// 4096 x 4096 x 16384 424 -> 410 us at the power limit); an epilogue that needs registers does not fit beside the sums.
 template <bool A_BY_K, bool B_BY_K>
-using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K>;     // 128 x 128
+using HpLong = HpCfg<2, 2, 4, 4, A_BY_K, B_BY_K, 4>;
+template <bool A_BY_K, bool B_BY_K>
+using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K, 4>;     // 128 x 128
 
 // 256 x 256 tiles where they fill the device, 128 x 128 ones below that.
 inline bool hp_wide(int64_t I, int64_t J) { return ((I + 255) / 256) * ((J + 255) / 256) >= 256; }
 
-template <class Cfg, typename E, class Epilogue>
-inline int hp_launch(const HpProblem& p, const typename Epilogue::Params& e, hipStream_t stream) {
-  const int64_t groups = static_cast<int64_t>(p.tiles_i) * p.tiles_j * p.splits;
-  if (groups <= 0) return AK_OK;
-  if (groups > 0x7fffffff) return AK_ERR_TOO_LARGE;
-  auto kernel = hp_kernel<Cfg, E, Epilogue>;
-  static std::atomic<uint64_t> known{0};         // devices that know the kernel's LDS (setting it twice is harmless)
+// The device's LDS is more than a kernel has without asking; once a kernel and device.
+template <typename Kernel>
+inline int hp_ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& known) {
   int device = 0;
   if (hipGetDevice(&device) != hipSuccess) return AK_ERR_LAUNCH;
   const uint64_t bit = 1ull << (device & 63);
-  if ((known.load(std::memory_order_relaxed) & bit) == 0) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Cfg::LDS_BYTES) != hipSuccess)
-      return AK_ERR_LAUNCH;
-    if (device < 64) known.fetch_or(bit, std::memory_order_relaxed);
-  }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(Cfg::THREADS), Cfg::LDS_BYTES, stream, p, e);
+  if (device < 64 && (known.load(std::memory_order_relaxed) & bit) != 0) return AK_OK;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return AK_ERR_LAUNCH;
+  if (device < 64) known.fetch_or(bit, std::memory_order_relaxed);
+  return AK_OK;
+}
+
+inline int64_t hp_blocks(const HpProblem& p) { return static_cast<int64_t>(p.tiles_i) * p.tiles_j * p.splits; }
+
+template <class Cfg, typename E, class Epilogue>
+inline int hp_launch(const HpProblem& p, const typename Epilogue::Params& e, hipStream_t stream) {
+  const int64_t blocks = hp_blocks(p);
+  if (blocks <= 0) return AK_OK;
+  if (blocks > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  auto kernel = hp_kernel<Cfg, E, Epilogue>;
+  static std::atomic<uint64_t> known{0};
+  const int rc = hp_ask_lds(kernel, Cfg::LDS_BYTES, known);
+  if (rc != AK_OK) return rc;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(Cfg::THREADS), Cfg::LDS_BYTES, stream, p, e);
+  return check_launch();
+}
+
+// The product whose work groups take longer goes first.
+template <class Cfg1, class Epilogue1, class Cfg2, class Epilogue2, typename E>
+inline int hp_launch_both(const HpProblem& p1, const typename Epilogue1::Params& e1, const HpProblem& p2, const typename Epilogue2::Params& e2,
+                          hipStream_t stream) {
+  const int64_t b1 = hp_blocks(p1), b2 = hp_blocks(p2);
+  if (b1 + b2 > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  auto kernel = hp_both_kernel<Cfg1, Epilogue1, Cfg2, Epilogue2, E>;
+  static std::atomic<uint64_t> known{0};
+  const int rc = hp_ask_lds(kernel, Cfg1::LDS_BYTES, known);
+  if (rc != AK_OK) return rc;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(b1 + b2)), dim3(Cfg1::THREADS), Cfg1::LDS_BYTES, stream, p1, e1, static_cast<uint32_t>(b1), p2, e2,
+                     static_cast<uint32_t>(b2), p2.k_per_split > p1.k_per_split ? 1 : 0);
   return check_launch();
 }
 

@@ -372,7 +372,7 @@ extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const 
         }
         return plan.direct ? AK_OK : hp_total(s.sum, plan.ld_sum, out * plan.ld_sum, plan.splits, out, F, 1.f, nullptr, static_cast<O*>(dw), st);
       };
-      return hp_wide(width, out) ? products(HpWide<false, false>{}) : products(HpSmall<false, false>{});
+      return hp_wide(width, out) ? products(HpLong<false, false>{}) : products(HpSmall<false, false>{});
     });
     if (rc != AK_OK) return rc;
   }

@@ -36,6 +36,37 @@ struct LceRows {
   int rows, classes;
 };
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// exp(s - shift) = exp(s) * rest, a fused multiplication and addition and the power of two an element: the product of the shift is rounded
+// to float32 (2^-24 of a shift of 60 is 4e-6), and what that loses, exact by a fused operation, is a factor that all elements share.
+struct Shifted {
+  float by, rest;
+  __device__ __forceinline__ explicit Shifted(float shift) : by(shift * kLog2e) {
+    const float lost = __builtin_fmaf(shift, kLog2e, -by);
+    rest = fabsf(lost) < 1.f ? __builtin_amdgcn_exp2f(-lost) : 1.f;          // (NaN of an infinite shift)
+  }
+  __device__ __forceinline__ float exp(float s) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, kLog2e, -by)); }
+};
+
+// What a tile's sums become: the bias is added, and classes behind the last are -inf.  Most tiles have neither.  (c0: first class of the
+// product, i_tile: first one of the tile behind it)
+template <class Cfg>
+__device__ __forceinline__ void lce_scores(const LceRows& r, floatx16 (&acc)[Cfg::FR][Cfg::FC], int i_tile, int c0, int wr) {
+  const int first = c0 + i_tile;
+  if (r.bias == nullptr && first + Cfg::BI <= r.classes) return;
+  const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int c = first + 32 * (Cfg::FR * wr + a) + 8 * (x >> 2) + 4 * g + (x & 3);
+      const float shift = r.bias != nullptr && c < r.classes ? r.bias[c] : 0.f;
+#pragma unroll
+      for (int b = 0; b < Cfg::FC; ++b) acc[a][b][x] = c < r.classes ? acc[a][b][x] + shift : -INFINITY;
+    }
+}
+
 // Tiles of the forward pass: i classes, j rows.
 struct LceStats {
   struct Params {
@@ -44,23 +75,13 @@ struct LceStats {
     float* at_target;      // [rows]
   };
   template <class Cfg>
-  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc) {
-    extern __shared__ __attribute__((aligned(1024))) unsigned char hp_smem[];
-    floatx2* joined = reinterpret_cast<floatx2*>(hp_smem);       // [WR][BJ]
-    const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc,
+                                             AK_LDS unsigned char* lds) {
+    AK_LDS floatx2* joined = reinterpret_cast<AK_LDS floatx2*>(lds);       // [WR][BJ]
+        const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
     const int i0 = ti * Cfg::BI + 32 * Cfg::FR * wr + 4 * g;
-    __syncthreads();
-#pragma unroll
-    for (int a = 0; a < Cfg::FR; ++a)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = i0 + 32 * a + 8 * q + k;
-          const float shift = e.r.bias != nullptr && i < e.r.classes ? e.r.bias[i] : 0.f;
-#pragma unroll
-          for (int b = 0; b < Cfg::FC; ++b) acc[a][b][4 * q + k] = i < e.r.classes ? acc[a][b][4 * q + k] + shift : -INFINITY;
-        }
+    __syncthreads();                           // everybody has read the last panels
+    lce_scores<Cfg>(e.r, acc, ti * Cfg::BI, 0, wr);
 #pragma unroll
     for (int b = 0; b < Cfg::FC; ++b) {
       const int jl = 32 * Cfg::FC * wc + 32 * b + l32, j = tj * Cfg::BJ + jl;
@@ -71,15 +92,20 @@ struct LceStats {
       for (int a = 0; a < Cfg::FR; ++a)
 #pragma unroll
         for (int x = 0; x < 16; ++x) m = fmaxf(m, acc[a][b][x]);
-      const float base = m == -INFINITY ? 0.f : m;
+      const Shifted by(m == -INFINITY ? 0.f : m);
       float s = 0.f;
 #pragma unroll
       for (int a = 0; a < Cfg::FR; ++a)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          s += __expf(acc[a][b][x] - base);
-          if (at == 32 * a + 8 * (x >> 2) + (x & 3) && target < e.r.classes) e.at_target[j] = acc[a][b][x];
-        }
+        for (int x = 0; x < 16; ++x) s += by.exp(acc[a][b][x]);
+      s *= by.rest;
+      if (__any(at >= 0 && at < 32 * Cfg::FR)) {
+#pragma unroll
+        for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (at == 32 * a + 8 * (x >> 2) + (x & 3) && target < e.r.classes) e.at_target[j] = acc[a][b][x];
+      }
       floatx2 ms = {m, s};
       ms = lce_join2(ms, floatx2{__shfl_xor(m, 32), __shfl_xor(s, 32)});
       if (g == 0) joined[wr * Cfg::BJ + jl] = ms;
@@ -108,22 +134,38 @@ struct LceGrad {
     int c0, width;         // classes of the piece, a multiple of eight (those from r.classes on are zeros)
   };
   template <class Cfg>
-  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc) {
-    hp_quads<Cfg>(acc, ti, tj, wr, wc, [&](int i, int j, floatx4 v) {
-      if (j >= e.r.rows || i >= e.width) return;
-      const float lse = e.lse[j], share = e.share[j];
-      const int64_t target = e.r.targets[j] - e.c0 - i;
-      Some<E, 4> some;
+  static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc,
+                                             AK_LDS unsigned char*) {
+    lce_scores<Cfg>(e.r, acc, ti * Cfg::BI, e.c0, wr);
+    const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+    const int i0 = ti * Cfg::BI + 32 * Cfg::FR * wr + 4 * g, j0 = tj * Cfg::BJ + 32 * Cfg::FC * wc + l32;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = e.c0 + i + k;
-        const bool in = c < e.r.classes;
-        const float s = v[k] + (in && e.r.bias != nullptr ? e.r.bias[c] : 0.f);
-        const float p = __expf(s - lse) - (target == k ? 1.f : 0.f);
-        some.set(k, in && share != 0.f ? p * share : 0.f);
+    for (int b = 0; b < Cfg::FC; ++b) {
+      const int j = j0 + 32 * b;
+      const bool in = j < e.r.rows;
+      const float share = in ? e.share[j] : 0.f, lse = in ? e.lse[j] : 0.f;
+      const Shifted by(lse);
+      const float times = share * by.rest;
+      const int64_t at = in && share != 0.f ? e.r.targets[j] - e.c0 - i0 : -1;
+      // (ignored rows: 0, whatever their scores; the share of a class of no probability: 0)
+#pragma unroll
+      for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          acc[a][b][x] = share != 0.f ? by.exp(acc[a][b][x]) * times : 0.f;
+        }
+      if (__any(at >= 0 && at < 32 * Cfg::FR)) {
+#pragma unroll
+        for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (at == 32 * a + 8 * (x >> 2) + (x & 3)) acc[a][b][x] -= share;
       }
-      some.store(e.d + static_cast<int64_t>(j) * e.ldd + i);
-    });
+    }
+    hp_eights<Cfg, E>(ti, tj, wr, wc, [&](int a, int b, int x) { return acc[a][b][x]; },
+                      [&](int i, int j, u32x4 v) {
+                        if (j < e.r.rows && i < e.width) __builtin_memcpy(e.d + static_cast<int64_t>(j) * e.ldd + i, &v, 16);
+                      });
   }
 };
 
@@ -343,7 +385,7 @@ static __global__ __launch_bounds__(256) void lce_piece_grad_kernel(float* __res
 }
 
 // ---- host side
-constexpr int64_t kLcePieceBytes = 256ll << 20;       // of d (fp32: of logits): what the last-level cache holds
+constexpr int64_t kLcePieceBytes = 512ll << 20;       // of d (fp32: of logits)
 constexpr int kLceFewRows = 64;
 
 // Sizes that both the workspace query and the launches use.
@@ -352,6 +394,7 @@ struct LcePlan {
   int es;                  // bytes of an element
   int64_t piece, pieces;   // classes of a piece, a multiple of 256 (the last may have fewer)
   int64_t ldp;             // row pitch of padded operands
+  bool wide;               // tiles of 256 in the gradients' products
   int splits;              // of the contraction over a piece's classes
   int64_t ld_sum;          // row pitch of the fp32 sums of dh
 };
@@ -366,11 +409,20 @@ inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D) {
   p.pieces = (V + p.piece - 1) / p.piece;
   p.ldp = align_up(D, 8);
   p.ld_sum = align_up(D, 4);
-  const int64_t tiles = ((N + 127) / 128) * ((D + 127) / 128), k = std::min(p.piece, V);
-  int64_t s = std::min((512 + tiles - 1) / tiles, k / 256);
-  s = std::max<int64_t>(1, std::min<int64_t>(s, 64));
-  const int64_t per = align_up((align_up(k, 8) + s - 1) / s, 32);
-  p.splits = static_cast<int>((align_up(k, 8) + per - 1) / per);       // (all of them are set by the first piece; a shorter one has no more)
+  // The gradients' products of a piece: tiles of 256 where their work groups fill the device.  The contraction over the classes goes in as
+  // many splits as make its work groups a sixth of a CU's share of the work, so that the last ones to run leave little of the device idle;
+  // every split has sums of its own.
+  const int64_t k = std::min(p.piece, V);
+  for (int64_t tile : {256, 128}) {
+    p.wide = tile == 256;
+    const int64_t across = (D + tile - 1) / tile, of_dw = across * ((k + tile - 1) / tile), of_dh = across * ((N + tile - 1) / tile);
+    const int64_t places = p.wide ? 256 : 512, share = (of_dw * ((N + 31) / 32) + of_dh * ((k + 31) / 32)) / places;
+    int64_t s = (k / 32) / std::max<int64_t>(share / 6, 8);
+    s = std::max<int64_t>(1, std::min<int64_t>(s, p.wide ? 8 : 32));
+    const int64_t per = align_up((align_up(k, 8) + s - 1) / s, 32);
+    p.splits = static_cast<int>((align_up(k, 8) + per - 1) / per);
+    if (of_dw + of_dh * p.splits >= places) break;
+  }
   return p;
 }
 
@@ -520,24 +572,21 @@ inline int lce_backward_half(LceCall c, const float* lse, const LcePlan& p, cons
     };
     rc = hp_wide(padded, p.N) ? grad(HpWide<true, true>{}) : grad(HpSmall<true, true>{});
     if (rc != AK_OK) return rc;
-    if (out.dh != nullptr) {
-      // i features, j rows, k classes; the splits of the last piece may be fewer, or shorter
-      using Cfg = HpSmall<false, true>;
-      const HpProblem q = hp_problem<Cfg>(hp_operand(w, c.ldw, width, p.D, false), hp_operand(d, p.piece, p.N, padded, true), p.D, p.N, padded, p.splits);
-      rc = hp_launch<Cfg, E, HpSum>(q, HpSum::Params{s.sum, p.ld_sum, p.N * p.ld_sum, static_cast<int>(p.D), static_cast<int>(p.N), k == 0}, c.stream);
-      if (rc != AK_OK) return rc;
-    }
-    if (out.dw != nullptr) {
-      // i features, j classes, k rows
-      auto weight = [&](auto cfg) {
-        using Cfg = decltype(cfg);
-        const HpProblem q = hp_problem<Cfg>(hp_operand(c.h, c.ldh, p.N, p.D, false), hp_operand(d, p.piece, p.N, padded, false), p.D, width, p.N);
-        typename HpStore<E>::Params e{static_cast<E*>(out.dw) + c0 * p.D, p.D, static_cast<int>(p.D), static_cast<int>(width), 1.f, s.unit};
-        return hp_launch<Cfg, E, HpStore<E>>(q, e, c.stream);
-      };
-      rc = hp_wide(p.D, width) ? weight(HpWide<false, false>{}) : weight(HpSmall<false, false>{});
-      if (rc != AK_OK) return rc;
-    }
+    // dw: i features, j classes, k rows.  dh: i features, j rows, k classes (a shorter last piece has no more splits)
+    auto gradients = [&](auto dw_cfg, auto dh_cfg) {
+      using W = decltype(dw_cfg);
+      using H = decltype(dh_cfg);
+      const HpProblem qw = hp_problem<W>(hp_operand(c.h, c.ldh, p.N, p.D, false), hp_operand(d, p.piece, p.N, padded, false), p.D, width, p.N);
+      const HpProblem qh = hp_problem<H>(hp_operand(w, c.ldw, width, p.D, false), hp_operand(d, p.piece, p.N, padded, true), p.D, p.N, padded, p.splits);
+      typename HpStore<E>::Params ew{static_cast<E*>(out.dw) + c0 * p.D, p.D, static_cast<int>(p.D), static_cast<int>(width), 1.f, s.unit};
+      const HpSum::Params eh{s.sum, p.ld_sum, p.N * p.ld_sum, static_cast<int>(p.D), static_cast<int>(p.N), k == 0};
+      if (out.dh == nullptr) return hp_launch<W, E, HpStore<E>>(qw, ew, c.stream);
+      if (out.dw == nullptr) return hp_launch<H, E, HpSum>(qh, eh, c.stream);
+      return hp_launch_both<W, HpStore<E>, H, HpSum, E>(qw, ew, qh, eh, c.stream);
+    };
+    if (out.dh != nullptr || out.dw != nullptr)
+      rc = p.wide ? gradients(HpLong<false, false>{}, HpLong<false, true>{}) : gradients(HpSmall<false, false>{}, HpSmall<false, true>{});
+    if (rc != AK_OK) return rc;
     rc = lce_db(d, p.piece, p, c0, width, s, out, c.stream);
     if (rc != AK_OK) return rc;
   }
