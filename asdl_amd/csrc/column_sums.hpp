@@ -59,16 +59,19 @@ inline int column_chunks(int64_t rows) {
 
 inline size_t column_sums_ws_bytes(int64_t rows, int64_t cols) { return static_cast<size_t>(column_chunks(rows)) * cols * sizeof(float); }
 
-// out[c] = scale * factor * sum over rows of x[r][c]
+// out[c] = scale * factor * sum over rows and pieces of x[r][piece * pitch + c]; `part`: column_sums_ws_bytes of pieces * cols columns
 template <typename T, typename O>
-inline int column_sums(const T* x, int64_t ld, int64_t rows, int64_t cols, float scale, const float* factor, O* out, float* part, hipStream_t s) {
+inline int column_sums(const T* x, int64_t ld, int64_t rows, int64_t cols, float scale, const float* factor, O* out, float* part, hipStream_t s, int pieces = 1,
+                       int64_t pitch = 0) {
   if (cols <= 0) return AK_OK;
   if (cols > (1ll << 30)) return AK_ERR_TOO_LARGE;
   const int chunks = column_chunks(rows);
   const int64_t per = (rows + chunks - 1) / chunks;
   const unsigned groups = static_cast<unsigned>((cols + 255) / 256);
-  hipLaunchKernelGGL(column_chunks_kernel<T>, dim3(groups, static_cast<unsigned>(chunks)), dim3(256), 0, s, x, ld, rows, cols, per, part);
-  hipLaunchKernelGGL(column_total_kernel<O>, dim3(groups), dim3(256), 0, s, part, cols, chunks, scale, factor, out);
+  for (int k = pieces - 1; k >= 0; --k)
+    hipLaunchKernelGGL(column_chunks_kernel<T>, dim3(groups, static_cast<unsigned>(chunks)), dim3(256), 0, s, x + k * pitch, ld, rows, cols, per,
+                       part + (pieces - 1 - k) * chunks * cols);
+  hipLaunchKernelGGL(column_total_kernel<O>, dim3(groups), dim3(256), 0, s, part, cols, pieces * chunks, scale, factor, out);
   return check_launch();
 }
 

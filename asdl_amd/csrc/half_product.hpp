@@ -37,16 +37,25 @@ struct HpOperand {
   int64_t k;               // k there are (by row: rows; a contraction that is longer takes zeros)
 };
 
+// Operands in pieces that add up to their values, side by side in a row: D is the sum of the products of `count` pairs of them, one after
+// the other in the contraction.  fp32 values are three bf16 pieces exactly, of whose nine products the six that matter are taken (the others are
+// below 2^-24 of the product), the smallest first.
+struct HpPieces {
+  int count;
+  int a[6], b[6];          // bytes from a row's first piece
+};
+
 struct HpProblem {
   HpOperand A, B;
+  HpPieces pieces;         // of a configuration with PIECES
   int64_t K, k_per_split;  // k_per_split a multiple of 32
   int tiles_i, tiles_j, splits;
 };
 
-template <int WR_, int WC_, int FR_, int FC_, bool A_BY_K_, bool B_BY_K_, int STAGES_>
+template <int WR_, int WC_, int FR_, int FC_, bool A_BY_K_, bool B_BY_K_, int STAGES_, bool PIECES_ = false>
 struct HpCfg {
   static constexpr int WR = WR_, WC = WC_, FR = FR_, FC = FC_, NW = WR * WC, THREADS = 64 * NW, STAGES = STAGES_;
-  static constexpr bool A_BY_K = A_BY_K_, B_BY_K = B_BY_K_;
+  static constexpr bool A_BY_K = A_BY_K_, B_BY_K = B_BY_K_, PIECES = PIECES_;
   static constexpr int BI = 32 * FR * WR, BJ = 32 * FC * WC, BK = 32;
   static constexpr int BLOCK = 2048, PANEL_A = BI * 64, PANEL_B = BJ * 64, STAGE = PANEL_A + PANEL_B, LDS_BYTES = STAGES * STAGE;
   static constexpr int IA = BI / 16 / NW, IB = BJ / 16 / NW, LPT = IA + IB;      // wave-wide loads of a k-tile, per wave
@@ -111,6 +120,11 @@ struct HpLoader {
     base += step;
     left -= 32;
   }
+  // Back by `tiles` k-tiles and on by `bytes`: to the start of another piece.
+  __device__ __forceinline__ void again(int tiles, int64_t bytes) {
+    base += static_cast<uint64_t>(bytes - tiles * step);
+    left += 32 * static_cast<int64_t>(tiles);
+  }
 };
 
 // Offsets of a lane's fragments within the blocks of a panel: of the first and of the second 16 k of a k-tile.
@@ -156,6 +170,24 @@ __device__ __forceinline__ void hp_run(const HpProblem& p, const typename Epilog
   HpLoader<Cfg::B_BY_K, Cfg::IB> lb;
   la.init(p.A, wave, lane, ti * Cfg::BI, k0, k_count);
   lb.init(p.B, wave, lane, tj * Cfg::BJ, k0, k_count);
+  const int nk = static_cast<int>((k_count + 31) / 32);        // k-tiles (of a piece)
+  int piece = 0, left_of_piece = nk;
+  if constexpr (Cfg::PIECES) {
+    la.base += p.pieces.a[0];
+    lb.base += p.pieces.b[0];
+  }
+  auto load_next = [&]() {
+    la.next();
+    lb.next();
+    if constexpr (Cfg::PIECES) {
+      if (--left_of_piece == 0 && piece + 1 < p.pieces.count) {
+        la.again(nk, p.pieces.a[piece + 1] - p.pieces.a[piece]);
+        lb.again(nk, p.pieces.b[piece + 1] - p.pieces.b[piece]);
+        ++piece;
+        left_of_piece = nk;
+      }
+    }
+  };
   auto load_one = [&](int l, int stage) {
     const uint32_t at = lds0 + stage * Cfg::STAGE;
     if (l < Cfg::IA) la.load(l, at);
@@ -200,8 +232,7 @@ __device__ __forceinline__ void hp_run(const HpProblem& p, const typename Epilog
   for (int t = 0; t < S - 1; ++t) {              // k-tiles behind the last load zeros: the counts stay uniform
 #pragma unroll
     for (int l = 0; l < LPT; ++l) load_one(l, t);
-    la.next();
-    lb.next();
+    load_next();
   }
   wait_vmcnt<(S - 2) * LPT>();                   // this wave's loads of the first k-tile have landed
   __syncthreads();                               // ... and everybody's
@@ -209,15 +240,14 @@ __device__ __forceinline__ void hp_run(const HpProblem& p, const typename Epilog
 #pragma unroll
   for (int u = 0; u < FR + FC; ++u) read_unit(fa0, fb0, 0, 0, u);
   int rd = 0, to = S - 1;
-  const int nk = static_cast<int>((k_count + 31) / 32);
-  for (int kt = 0; kt < nk; ++kt) {
+  const int steps = Cfg::PIECES ? nk * p.pieces.count : nk;
+  for (int kt = 0; kt < steps; ++kt) {
     half_step(std::integral_constant<int, 0>{}, fa0, fb0, fa1, fb1, rd, 1, 0);
     wait_vmcnt<(S - 3) * LPT>();                 // own loads of the next k-tile have landed
     __syncthreads();                             // everybody's have; nobody reads the k-tile before this one any more
     rd = (rd + 1 == S) ? 0 : rd + 1;
     half_step(std::integral_constant<int, LPT>{}, fa1, fb1, fa0, fb0, rd, 0, to);
-    la.next();
-    lb.next();
+    load_next();
     to = (to + 1 == S) ? 0 : to + 1;
   }
   wait_vmcnt<0>();                               // the loads of zeros have landed before the LDS is used again
@@ -396,6 +426,73 @@ inline int hp_pad(const T* x, int64_t ld, int64_t rows, int64_t cols, T* out, in
   return check_launch();
 }
 
+// x in bf16 pieces that add up to it exactly (fp16: two, fp32: three), side by side in rows of PIECES * ldo, zeros behind the columns.
+template <int PIECES>
+__device__ __forceinline__ void hp_split(float x, __bf16 (&piece)[PIECES]) {
+#pragma unroll
+  for (int k = 0; k < PIECES; ++k) {
+    piece[k] = static_cast<__bf16>(x);
+    x = fabsf(x) < INFINITY ? x - static_cast<float>(piece[k]) : 0.f;          // (infinities and NaN in the first piece alone)
+  }
+}
+
+template <typename T, int PIECES>
+static __global__ __launch_bounds__(256) void hp_pieces_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, __bf16* __restrict__ out, int ldo) {
+  // eight columns a thread
+  const int per = ldo / 8;
+  const int64_t n = rows * per;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / per;
+    const int c = static_cast<int>(i - row * per) * 8;
+    const T* __restrict__ from = x + row * ld + c;
+    Some<T, 8> v;
+    v.clear();
+    if (c + 8 <= cols) {
+      v.load(from);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < cols) v.v[e] = from[e];
+    }
+    Some<__bf16, 8> o[PIECES];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      __bf16 piece[PIECES];
+      hp_split(v.get(e), piece);
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) o[k].v[e] = piece[k];
+    }
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) o[k].store(out + (row * PIECES + k) * ldo + c);
+  }
+}
+
+template <int PIECES, typename T>
+inline int hp_pieces(const T* x, int64_t ld, int64_t rows, int64_t cols, __bf16* out, int64_t ldo, hipStream_t stream) {
+  const int64_t groups = (rows * (ldo / 8) + 255) / 256;
+  hipLaunchKernelGGL((hp_pieces_kernel<T, PIECES>), dim3(static_cast<unsigned>(groups < 1 ? 1 : groups < 16384 ? groups : 16384)), dim3(256), 0, stream, x, ld,
+                     rows, static_cast<int>(cols), out, static_cast<int>(ldo));
+  return check_launch();
+}
+
+// Both operands fp32: the six products.  pa, pb: elements between the pieces of a row.
+inline HpPieces hp_six(int64_t pa, int64_t pb) {
+  static constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
+  HpPieces p = {6, {}, {}};
+  for (int i = 0; i < 6; ++i) {
+    p.a[i] = static_cast<int>(A[i] * pa * 2);
+    p.b[i] = static_cast<int>(B[i] * pb * 2);
+  }
+  return p;
+}
+
+// B alone in pieces.
+inline HpPieces hp_pieces_of_b(int count, int64_t pb) {
+  HpPieces p = {count, {}, {}};
+  for (int i = 0; i < count; ++i) p.b[i] = static_cast<int>((count - 1 - i) * pb * 2);
+  return p;
+}
+
 // 16-bit elements whose rows the panels' loads can read where they lie.
 inline bool hp_aligned(const void* x, int64_t ld, int64_t cols) {
   return cols % 8 == 0 && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
@@ -411,7 +508,7 @@ inline HpOperand hp_operand(const void* p, int64_t ld, int64_t rows, int64_t col
 // An I x J result; the contraction in (at most) `splits` parts.
 template <class Cfg>
 inline HpProblem hp_problem(const HpOperand& A, const HpOperand& B, int64_t I, int64_t J, int64_t K, int splits = 1) {
-  HpProblem p;
+  HpProblem p = {};
   p.A = A; p.B = B;
   p.K = K;
   p.k_per_split = align_up((K + splits - 1) / splits, 32);
@@ -433,17 +530,18 @@ struct Carver {
   }
 };
 
-template <bool A_BY_K, bool B_BY_K>
-using HpWide = HpCfg<2, 4, 4, 2, A_BY_K, B_BY_K, 4>;      // 256 x 256
+template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
+using HpWide = HpCfg<2, 4, 4, 2, A_BY_K, B_BY_K, 4, PIECES>;      // 256 x 256
 // 256 x 256 by four waves of 128 x 128, one a SIMD, for long contractions: a third less of the LDS is read for a product (the product of
 // 4096 x 4096 x 16384 424 -> 410 us at the power limit); an epilogue that needs registers does not fit beside the sums.
-template <bool A_BY_K, bool B_BY_K>
-using HpLong = HpCfg<2, 2, 4, 4, A_BY_K, B_BY_K, 4>;
-template <bool A_BY_K, bool B_BY_K>
-using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K, 4>;     // 128 x 128
+template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
+using HpLong = HpCfg<2, 2, 4, 4, A_BY_K, B_BY_K, 4, PIECES>;
+template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
+using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K, 4, PIECES>;     // 128 x 128
 
-// 256 x 256 tiles where they fill the device, 128 x 128 ones below that.
-inline bool hp_wide(int64_t I, int64_t J) { return ((I + 255) / 256) * ((J + 255) / 256) >= 256; }
+// 256 x 256 tiles, but for results that 128 x 128 ones of at most one place each cover: two of those take 0.83 of the time of one wide
+// tile on a CU (1000 x 10007 x 513 in six products: 632 small tiles 126 us, 160 wide ones WIDE_US us).
+inline bool hp_wide(int64_t I, int64_t J) { return ((I + 127) / 128) * ((J + 127) / 128) > 512; }
 
 // The device's LDS is more than a kernel has without asking; once a kernel and device.
 template <typename Kernel>

@@ -206,30 +206,10 @@ static __global__ __launch_bounds__(256) void keep_back_kernel(Keep p, int64_t l
   }
 }
 
-// The bfloat16 pieces of a gradient, [piece][rows][ldo], zeros behind its columns: they add up to it exactly.
-template <typename T, int PIECES>
-static __global__ __launch_bounds__(256) void keep_pieces_kernel(const T* __restrict__ g, int64_t ld, int64_t rows, int cols, __bf16* __restrict__ out,
-                                                                 int ldo) {
-  const int64_t n = rows * ldo;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / ldo;
-    const int c = static_cast<int>(i - row * ldo);
-    float rest = c < cols ? static_cast<float>(g[row * ld + c]) : 0.f;
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const __bf16 piece = static_cast<__bf16>(rest);
-      out[k * n + i] = piece;
-      // (infinities and NaN in the first piece alone)
-      rest = fabsf(rest) < INFINITY ? rest - static_cast<float>(piece) : 0.f;
-    }
-  }
-}
-
 // ---- host side
 struct KeepPlan {
   int pieces, splits;
   int64_t ldf, ldg, ld_sum;
-  bool direct;             // the products' epilogue writes dw
 };
 
 inline KeepPlan keep_plan(int dtype, int64_t rows, int64_t F, int64_t out) {
@@ -243,7 +223,6 @@ inline KeepPlan keep_plan(int dtype, int64_t rows, int64_t F, int64_t out) {
   const int64_t s = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((wide ? 256 : 512) / tiles, rows / 256), 64));
   const int64_t per = align_up((rows + s - 1) / s, 32);
   p.splits = static_cast<int>((rows + per - 1) / per);
-  p.direct = p.pieces == 1 && p.splits == 1;
   return p;
 }
 
@@ -258,7 +237,7 @@ inline KeepSpace keep_space(const KeepPlan& p, int64_t rows, int64_t out, bool c
   KeepSpace s = {};
   s.x = c.take<__bf16>(rows * p.ldf);
   if (copy) s.g = c.take<__bf16>(p.pieces * rows * p.ldg);
-  if (!p.direct) s.sum = c.take<float>(p.splits * out * p.ld_sum);
+  if (p.splits > 1) s.sum = c.take<float>(p.splits * out * p.ld_sum);
   if (bias) s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(rows, out) / sizeof(float)));
   s.bytes = c.used;
   return s;
@@ -341,37 +320,28 @@ extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const 
     hipLaunchKernelGGL((keep_back_kernel<__bf16, -1>), keep_grid(k), dim3(256), 0, st, k, plan.ldf, static_cast<int>(plan.ldf));
     const __bf16* from = static_cast<const __bf16*>(g);
     int64_t ld = ldg;
-    if (copy) {
-      const int64_t groups = std::max<int64_t>(1, std::min<int64_t>((rows * plan.ldg + 1023) / 1024, 8192));
-      const dim3 grid(static_cast<unsigned>(groups));
-      const int cols = static_cast<int>(out), ldo = static_cast<int>(plan.ldg);
-      if (dtype == AK_BF16)
-        hipLaunchKernelGGL((keep_pieces_kernel<__bf16, 1>), grid, dim3(256), 0, st, static_cast<const __bf16*>(g), ldg, rows, cols, s.g, ldo);
-      else if (dtype == AK_F16)
-        hipLaunchKernelGGL((keep_pieces_kernel<_Float16, 2>), grid, dim3(256), 0, st, static_cast<const _Float16*>(g), ldg, rows, cols, s.g, ldo);
-      else
-        hipLaunchKernelGGL((keep_pieces_kernel<float, 3>), grid, dim3(256), 0, st, static_cast<const float*>(g), ldg, rows, cols, s.g, ldo);
-      from = s.g;
-      ld = plan.ldg;
-    }
     rc = check_launch();
+    if (rc == AK_OK && copy) {
+      rc = dtype == AK_BF16  ? hp_pad(from, ldg, rows, out, s.g, plan.ldg, st)
+           : dtype == AK_F16 ? hp_pieces<2>(static_cast<const _Float16*>(g), ldg, rows, out, s.g, plan.ldg, st)
+                             : hp_pieces<3>(static_cast<const float*>(g), ldg, rows, out, s.g, plan.ldg, st);
+      from = s.g;
+      ld = plan.pieces * plan.ldg;
+    }
     if (rc != AK_OK) return rc;
     rc = with_type(grad_dtype, [&](auto o) {
       using O = typename decltype(o)::type;
       // i features, j outputs, k rows
       auto products = [&](auto cfg) {
         using Cfg = decltype(cfg);
-        for (int piece = plan.pieces - 1; piece >= 0; --piece) {            // the smallest first
-          const HpProblem q = hp_problem<Cfg>(hp_operand(s.x, plan.ldf, rows, width, false), hp_operand(from + piece * rows * ld, ld, rows, out, false),
-                                              width, out, rows, plan.splits);
-          const int done = plan.direct
-                               ? hp_launch<Cfg, __bf16, HpStore<O>>(q, typename HpStore<O>::Params{static_cast<O*>(dw), width, F, static_cast<int>(out), 1.f, nullptr}, st)
-                               : hp_launch<Cfg, __bf16, HpSum>(q, HpSum::Params{s.sum, plan.ld_sum, out * plan.ld_sum, F, static_cast<int>(out),
-                                                                               piece == plan.pieces - 1}, st);
-          if (done != AK_OK) return done;
-        }
-        return plan.direct ? AK_OK : hp_total(s.sum, plan.ld_sum, out * plan.ld_sum, plan.splits, out, F, 1.f, nullptr, static_cast<O*>(dw), st);
+        HpProblem q = hp_problem<Cfg>(hp_operand(s.x, plan.ldf, rows, width, false), hp_operand(from, ld, rows, out, false), width, out, rows, plan.splits);
+        if (Cfg::PIECES) q.pieces = hp_pieces_of_b(plan.pieces, plan.ldg);
+        if (plan.splits == 1)
+          return hp_launch<Cfg, __bf16, HpStore<O>>(q, typename HpStore<O>::Params{static_cast<O*>(dw), width, F, static_cast<int>(out), 1.f, nullptr}, st);
+        const int done = hp_launch<Cfg, __bf16, HpSum>(q, HpSum::Params{s.sum, plan.ld_sum, out * plan.ld_sum, F, static_cast<int>(out), 1}, st);
+        return done != AK_OK ? done : hp_total(s.sum, plan.ld_sum, out * plan.ld_sum, plan.splits, out, F, 1.f, nullptr, static_cast<O*>(dw), st);
       };
+      if (plan.pieces > 1) return hp_wide(width, out) ? products(HpLong<false, false, true>{}) : products(HpSmall<false, false, true>{});
       return hp_wide(width, out) ? products(HpLong<false, false>{}) : products(HpSmall<false, false>{});
     });
     if (rc != AK_OK) return rc;

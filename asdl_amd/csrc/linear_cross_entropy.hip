@@ -9,13 +9,24 @@
 // 16-bit operands: fp32 sums.  d is rounded to the operands' type, which the matrix cores need and which is what a framework's own
 // backward pass in that type has; it holds c_n over the next power of two above the largest |c_n| (fp16: times 2^14, so that shares
 // of the classes down to 2^-28 are normal numbers), and the products' epilogues put the power back.
-// fp32 operands: the framework's three-piece products (gemm_x3.hpp), through pieces of fp32 logits.
+// fp32 operands: three bf16 pieces each, six of their products a product (half_product.hpp), through the same tiles; d in three pieces, too.
 #include <algorithm>
 #include "column_sums.hpp"
-#include "gemm_f32.hpp"
 #include "half_product.hpp"
 
 namespace ak {
+
+// What the matrix cores take of an operand type: the element and how many of them a value is.
+template <typename E>
+struct LceKind {
+  using type = E;
+  static constexpr int pieces = 1;
+};
+template <>
+struct LceKind<float> {
+  using type = __bf16;
+  static constexpr int pieces = 3;
+};
 
 enum { kLossNone = 0, kLossSum = 1, kLossMean = 2 };
 
@@ -125,12 +136,13 @@ struct LceStats {
 // Tiles of a piece of d: i classes from c0 on, j rows; d[j][i - c0], zeros up to a multiple of eight classes.
 template <typename E>
 struct LceGrad {
+  using M = typename LceKind<E>::type;
   struct Params {
     LceRows r;
     const float* lse;
     const float* share;    // c_n over the power of two, times 2^14 for fp16
-    E* d;
-    int64_t ldd;
+    M* d;                  // a row: its pieces side by side
+    int64_t ldd, pitch;    // elements between rows, between pieces
     int c0, width;         // classes of the piece, a multiple of eight (those from r.classes on are zeros)
   };
   template <class Cfg>
@@ -162,12 +174,64 @@ struct LceGrad {
             if (at == 32 * a + 8 * (x >> 2) + (x & 3)) acc[a][b][x] -= share;
       }
     }
-    hp_eights<Cfg, E>(ti, tj, wr, wc, [&](int a, int b, int x) { return acc[a][b][x]; },
-                      [&](int i, int j, u32x4 v) {
-                        if (j < e.r.rows && i < e.width) __builtin_memcpy(e.d + static_cast<int64_t>(j) * e.ldd + i, &v, 16);
-                      });
+#pragma unroll
+    for (int k = 0; k < LceKind<E>::pieces; ++k) {
+      hp_eights<Cfg, M>(ti, tj, wr, wc, [&](int a, int b, int x) { return acc[a][b][x]; },
+                        [&](int i, int j, u32x4 v) {
+                          if (j < e.r.rows && i < e.width) __builtin_memcpy(e.d + static_cast<int64_t>(j) * e.ldd + k * e.pitch + i, &v, 16);
+                        });
+      if (k + 1 == LceKind<E>::pieces) break;
+#pragma unroll
+      for (int a = 0; a < Cfg::FR; ++a)
+#pragma unroll
+        for (int b = 0; b < Cfg::FC; ++b)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const float v = acc[a][b][x];
+            acc[a][b][x] = fabsf(v) < INFINITY ? v - static_cast<float>(static_cast<M>(v)) : 0.f;
+          }
+    }
   }
 };
+
+// Eight consecutive k of a row on their way to the matrix instruction 16 x 16 x 32.
+template <typename E>
+struct LceEight {
+  E v[8];
+  __device__ __forceinline__ void load(const E* p) { __builtin_memcpy(v, p, sizeof(v)); }
+  __device__ __forceinline__ void some(const E* p, int n) {      // n of them, zeros behind
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : static_cast<E>(0.f);
+  }
+};
+
+template <typename E>
+__device__ __forceinline__ floatx4 lce_mma(const LceEight<E>& a, const LceEight<E>& b, floatx4 c) {
+  if constexpr (__is_same(E, float)) {
+    __bf16 pa[8][3], pb[8][3];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      hp_split(a.v[e], pa[e]);
+      hp_split(b.v[e], pb[e]);
+    }
+    constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int t = 0; t < 6; ++t) {
+      bf16x8 x, y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = pa[e][A[t]];
+        y[e] = pb[e][B[t]];
+      }
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+    }
+    return c;
+  } else if constexpr (__is_same(E, __bf16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
 
 // A few rows: a wave takes 16 classes at a time, weights straight to the matrix instruction (16 x 16 x 32).  A lane has 32 consecutive
 // k of every 128 of one class: what the four lanes of a class read at once is a part of each 128-byte line, all of it in four loads.
@@ -185,48 +249,38 @@ static __global__ __launch_bounds__(512) void lce_few_kernel(const E* __restrict
   floatx4 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-  auto mma = [&](short8v a, short8v b, floatx4 c) {
-    if constexpr (__is_same(E, __bf16))
-      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else
-      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  };
-  auto get = [](const E* p) {
-    short8v v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
-  };
   const int whole = D / 128 * 128;
-  short8v wn[4];
+  LceEight<E> wn[4];
   if (whole > 0)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) wn[e] = get(wr + 8 * e);
+    for (int e = 0; e < 4; ++e) wn[e].load(wr + 8 * e);
   for (int k = 0; k < whole; k += 128) {
-    short8v wc[4];
+    LceEight<E> wc[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) wc[e] = wn[e];
     if (k + 128 < whole)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) wn[e] = get(wr + k + 128 + 8 * e);
+      for (int e = 0; e < 4; ++e) wn[e].load(wr + k + 128 + 8 * e);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[b] = mma(wc[e], get(hr[b] + k + 8 * e), acc[b]);
+      for (int e = 0; e < 4; ++e) {
+        LceEight<E> x;
+        x.load(hr[b] + k + 8 * e);
+        acc[b] = lce_mma(wc[e], x, acc[b]);
+      }
   }
   if (whole < D) {
-    auto some_of = [&](const E* p, int n) {      // n of eight, zeros behind them
-      short8v v = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) v[e] = __builtin_bit_cast(short, p[e]);
-      return v;
-    };
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int n = D - whole - 32 * quarter - 8 * e;
-      const short8v a = some_of(wr + whole + 8 * e, n);
+      LceEight<E> a, x;
+      a.some(wr + whole + 8 * e, n);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) acc[b] = mma(a, some_of(hr[b] + whole + 8 * e, n), acc[b]);
+      for (int b = 0; b < NB; ++b) {
+        x.some(hr[b] + whole + 8 * e, n);
+        acc[b] = lce_mma(a, x, acc[b]);
+      }
     }
   }
   // acc[b][x]: class c0 + 4 quarter + x, row 16 b + l16
@@ -345,53 +399,14 @@ static __global__ __launch_bounds__(256) void lce_bias_kernel(const T* __restric
   if (i < n) out[i] = static_cast<float>(x[i]);
 }
 
-// ---- fp32: pieces of logits in memory
-static __global__ __launch_bounds__(256) void lce_piece_stats_kernel(const float* __restrict__ logits, int64_t ld, LceRows r, int c0, int width,
-                                                                     floatx2* __restrict__ part, float* __restrict__ at_target) {
-  __shared__ floatx2 joined[4];
-  const int j = blockIdx.x;
-  const float* __restrict__ x = logits + static_cast<int64_t>(j) * ld;
-  const int64_t target = r.targets[j] - c0;
-  float m = -INFINITY;
-  for (int c = threadIdx.x; c < width; c += 256) m = fmaxf(m, x[c] + (r.bias != nullptr ? r.bias[c0 + c] : 0.f));
-  const float base = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
-  for (int c = threadIdx.x; c < width; c += 256) {
-    const float v = x[c] + (r.bias != nullptr ? r.bias[c0 + c] : 0.f);
-    s += __expf(v - base);
-    if (c == target) at_target[j] = v;
-  }
-  floatx2 ms = {m, s};
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) ms = lce_join2(ms, floatx2{__shfl_xor(ms[0], o), __shfl_xor(ms[1], o)});
-  if ((threadIdx.x & 63) == 0) joined[threadIdx.x >> 6] = ms;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-#pragma unroll
-  for (int w = 1; w < 4; ++w) ms = lce_join2(ms, joined[w]);
-  part[j] = ms;
-}
-
-static __global__ __launch_bounds__(256) void lce_piece_grad_kernel(float* __restrict__ logits, int64_t ld, LceRows r, int c0, int width,
-                                                                    const float* __restrict__ lse, const float* __restrict__ share) {
-  const int j = blockIdx.x;
-  float* __restrict__ x = logits + static_cast<int64_t>(j) * ld;
-  const int64_t target = r.targets[j] - c0;
-  const float l = lse[j], f = share[j];
-  for (int c = threadIdx.x; c < width; c += 256) {
-    const float p = __expf(x[c] + (r.bias != nullptr ? r.bias[c0 + c] : 0.f) - l) - (c == target ? 1.f : 0.f);
-    x[c] = f != 0.f ? p * f : 0.f;
-  }
-}
-
 // ---- host side
-constexpr int64_t kLcePieceBytes = 512ll << 20;       // of d (fp32: of logits)
+constexpr int64_t kLcePieceBytes = 512ll << 20;       // of d
 constexpr int kLceFewRows = 64;
 
 // Sizes that both the workspace query and the launches use.
 struct LcePlan {
   int64_t N, V, D;
-  int es;                  // bytes of an element
+  int k;                   // 16-bit pieces of a value
   int64_t piece, pieces;   // classes of a piece, a multiple of 256 (the last may have fewer)
   int64_t ldp;             // row pitch of padded operands
   bool wide;               // tiles of 256 in the gradients' products
@@ -402,8 +417,8 @@ struct LcePlan {
 inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D) {
   LcePlan p;
   p.N = N; p.V = V; p.D = D;
-  p.es = dtype == AK_F32 ? 4 : 2;
-  const int64_t fit = std::max<int64_t>(kLcePieceBytes / (N * p.es) / 256 * 256, 256);
+  p.k = dtype == AK_F32 ? 3 : 1;
+  const int64_t fit = std::max<int64_t>(kLcePieceBytes / (N * p.k * 2) / 256 * 256, 256);
   p.pieces = (V + fit - 1) / fit;
   p.piece = align_up((V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (V + p.piece - 1) / p.piece;
@@ -421,13 +436,13 @@ inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D) {
     s = std::max<int64_t>(1, std::min<int64_t>(s, p.wide ? 8 : 32));
     const int64_t per = align_up((align_up(k, 8) + s - 1) / s, 32);
     p.splits = static_cast<int>((align_up(k, 8) + per - 1) / per);
-    if (of_dw + of_dh * p.splits >= places) break;
+    if (of_dw + of_dh * p.splits >= places * 3 / 4) break;
   }
   return p;
 }
 
 struct LceSpace {
-  unsigned char *h, *w;    // padded operands
+  unsigned char *h, *w;    // padded operands, or operands in pieces
   float* bias;
   floatx2* part;
   float *at_target, *losses;
@@ -441,21 +456,19 @@ struct LceSpace {
 inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_w, bool bias, void* ws) {
   Carver c{static_cast<unsigned char*>(ws)};
   LceSpace s = {};
-  if (pad_h) s.h = c.take<unsigned char>(p.N * p.ldp * p.es);
-  if (pad_w) s.w = c.take<unsigned char>(p.V * p.ldp * p.es);
+  if (pad_h) s.h = c.take<unsigned char>(p.N * p.ldp * p.k * 2);
+  if (pad_w) s.w = c.take<unsigned char>(p.V * p.ldp * p.k * 2);
   if (bias) s.bias = c.take<float>(p.V);
   if (!backward) {
-    const int64_t parts = p.es == 4 ? p.pieces : (p.V + 127) / 128;
-    s.part = c.take<floatx2>(parts * p.N);
+    s.part = c.take<floatx2>((p.V + 127) / 128 * p.N);
     s.at_target = c.take<float>(p.N);
     s.losses = c.take<float>(p.N);
-    if (p.es == 4) s.d = c.take<unsigned char>(p.N * p.piece * p.es);
   } else {
     s.share = c.take<float>(p.N);
     s.unit = c.take<float>(1);
-    s.d = c.take<unsigned char>(p.N * p.piece * p.es);
-    if (p.es != 4) s.sum = c.take<float>(static_cast<int64_t>(p.splits) * p.N * p.ld_sum);
-    s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(p.N, p.piece) / sizeof(float)));
+    s.d = c.take<unsigned char>(p.N * p.piece * p.k * 2);
+    s.sum = c.take<float>(static_cast<int64_t>(p.splits) * p.N * p.ld_sum);
+    s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(p.N, p.k * p.piece) / sizeof(float)));
   }
   s.bytes = c.used;
   return s;
@@ -471,18 +484,20 @@ struct LceCall {
   hipStream_t stream;
 };
 
-// Operands at the pitch that the panels need, copied where theirs is another.
+// Operands as the panels need them: copied where their pitch or alignment is another, or in pieces.
 template <typename E>
 inline int lce_operands(LceCall& c, const LcePlan& p, const LceSpace& s) {
-  auto pad = [&](const void*& x, int64_t& ld, int64_t rows, unsigned char* to) {
+  auto as_needed = [&](const void*& x, int64_t& ld, int64_t rows, unsigned char* to) {
     if (to == nullptr) return AK_OK;
-    const int rc = hp_pad(static_cast<const E*>(x), ld, rows, p.D, reinterpret_cast<E*>(to), p.ldp, c.stream);
+    const E* from = static_cast<const E*>(x);
+    const int64_t from_ld = ld;
     x = to;
-    ld = p.ldp;
-    return rc;
+    ld = p.k * p.ldp;
+    if constexpr (__is_same(E, float)) return hp_pieces<3>(from, from_ld, rows, p.D, reinterpret_cast<__bf16*>(to), p.ldp, c.stream);
+    else return hp_pad(from, from_ld, rows, p.D, reinterpret_cast<E*>(to), p.ldp, c.stream);
   };
-  const int rc = pad(c.h, c.ldh, p.N, s.h);
-  return rc != AK_OK ? rc : pad(c.w, c.ldw, p.V, s.w);
+  const int rc = as_needed(c.h, c.ldh, p.N, s.h);
+  return rc != AK_OK ? rc : as_needed(c.w, c.ldw, p.V, s.w);
 }
 
 inline int lce_bias(LceCall& c, const LcePlan& p, const LceSpace& s) {
@@ -501,7 +516,7 @@ inline int lce_bias(LceCall& c, const LcePlan& p, const LceSpace& s) {
 }
 
 template <typename E>
-inline int lce_forward_half(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
+inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
   if (p.N <= kLceFewRows) {
     const int64_t groups = (p.V + 127) / 128;
     *parts = static_cast<int>(groups);
@@ -514,32 +529,19 @@ inline int lce_forward_half(LceCall c, const LcePlan& p, const LceSpace& s, int*
     if (p.N <= 32) return go(std::integral_constant<int, 2>{});
     return go(std::integral_constant<int, 4>{});
   }
-  int rc = lce_operands<E>(c, p, s);
+  const int rc = lce_operands<E>(c, p, s);
   if (rc != AK_OK) return rc;
+  using M = typename LceKind<E>::type;
+  constexpr bool PIECES = LceKind<E>::pieces > 1;
   const HpOperand A = hp_operand(c.w, c.ldw, p.V, p.D, true), B = hp_operand(c.h, c.ldh, p.N, p.D, true);
   auto go = [&](auto cfg) {
     using Cfg = decltype(cfg);
-    const HpProblem q = hp_problem<Cfg>(A, B, p.V, p.N, align_up(p.D, 8));
+    HpProblem q = hp_problem<Cfg>(A, B, p.V, p.N, align_up(p.D, 8));
+    if (PIECES) q.pieces = hp_six(p.ldp, p.ldp);
     *parts = q.tiles_i;
-    return hp_launch<Cfg, E, LceStats>(q, LceStats::Params{c.r, s.part, s.at_target}, c.stream);
+    return hp_launch<Cfg, M, LceStats>(q, LceStats::Params{c.r, s.part, s.at_target}, c.stream);
   };
-  return hp_wide(p.V, p.N) ? go(HpWide<true, true>{}) : go(HpSmall<true, true>{});
-}
-
-inline int lce_forward_f32(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
-  float* x = reinterpret_cast<float*>(s.d);
-  *parts = static_cast<int>(p.pieces);
-  for (int64_t k = 0; k < p.pieces; ++k) {
-    const int64_t c0 = k * p.piece, width = std::min(p.piece, p.V - c0);
-    GemmParams g = make_gemm(0, 1, static_cast<int>(p.N), static_cast<int>(width), static_cast<int>(p.D), 1.f, static_cast<const float*>(c.h), c.ldh,
-                             static_cast<const float*>(c.w) + c0 * c.ldw, c.ldw, 0.f, x, p.piece);
-    g.split = 3;
-    const int rc = launch_gemm(g, 1, c.stream);
-    if (rc != AK_OK) return rc;
-    hipLaunchKernelGGL(lce_piece_stats_kernel, dim3(static_cast<unsigned>(p.N)), dim3(256), 0, c.stream, x, p.piece, c.r, static_cast<int>(c0),
-                       static_cast<int>(width), s.part + k * p.N, s.at_target);
-  }
-  return check_launch();
+  return hp_wide(p.V, p.N) ? go(HpWide<true, true, PIECES>{}) : go(HpSmall<true, true, PIECES>{});
 }
 
 struct LceGrads {
@@ -547,77 +549,51 @@ struct LceGrads {
   int db_dtype;
 };
 
-template <typename T>
-inline int lce_db(const T* d, int64_t ldd, const LcePlan& p, int64_t c0, int64_t width, const LceSpace& s, const LceGrads& out, hipStream_t stream) {
-  if (out.db == nullptr) return AK_OK;
-  return with_type(out.db_dtype, [&](auto t) {
-    using O = typename decltype(t)::type;
-    return column_sums(d, ldd, p.N, width, 1.f, s.unit, static_cast<O*>(out.db) + c0, s.columns, stream);
-  });
-}
-
 template <typename E>
-inline int lce_backward_half(LceCall c, const float* lse, const LcePlan& p, const LceSpace& s, const LceGrads& out) {
+inline int lce_backward(LceCall c, const float* lse, const LcePlan& p, const LceSpace& s, const LceGrads& out) {
+  using M = typename LceKind<E>::type;
+  constexpr bool PIECES = LceKind<E>::pieces > 1;
   int rc = lce_operands<E>(c, p, s);
   if (rc != AK_OK) return rc;
-  E* d = reinterpret_cast<E*>(s.d);
+  M* d = reinterpret_cast<M*>(s.d);
+  const int64_t ldd = p.k * p.piece;
   for (int64_t k = 0; k < p.pieces; ++k) {
     const int64_t c0 = k * p.piece, width = std::min(p.piece, p.V - c0), padded = align_up(width, 8);
-    const E* w = static_cast<const E*>(c.w) + c0 * c.ldw;
+    const M* w = static_cast<const M*>(c.w) + c0 * c.ldw;
     auto grad = [&](auto cfg) {
       using Cfg = decltype(cfg);
-      const HpProblem q = hp_problem<Cfg>(hp_operand(w, c.ldw, width, p.D, true), hp_operand(c.h, c.ldh, p.N, p.D, true), padded, p.N, align_up(p.D, 8));
-      typename LceGrad<E>::Params e{c.r, lse, s.share, d, p.piece, static_cast<int>(c0), static_cast<int>(padded)};
-      return hp_launch<Cfg, E, LceGrad<E>>(q, e, c.stream);
+      HpProblem q = hp_problem<Cfg>(hp_operand(w, c.ldw, width, p.D, true), hp_operand(c.h, c.ldh, p.N, p.D, true), padded, p.N, align_up(p.D, 8));
+      if (PIECES) q.pieces = hp_six(p.ldp, p.ldp);
+      typename LceGrad<E>::Params e{c.r, lse, s.share, d, ldd, p.piece, static_cast<int>(c0), static_cast<int>(padded)};
+      return hp_launch<Cfg, M, LceGrad<E>>(q, e, c.stream);
     };
-    rc = hp_wide(padded, p.N) ? grad(HpWide<true, true>{}) : grad(HpSmall<true, true>{});
+    rc = hp_wide(padded, p.N) ? grad(HpWide<true, true, PIECES>{}) : grad(HpSmall<true, true, PIECES>{});
     if (rc != AK_OK) return rc;
     // dw: i features, j classes, k rows.  dh: i features, j rows, k classes (a shorter last piece has no more splits)
     auto gradients = [&](auto dw_cfg, auto dh_cfg) {
       using W = decltype(dw_cfg);
       using H = decltype(dh_cfg);
-      const HpProblem qw = hp_problem<W>(hp_operand(c.h, c.ldh, p.N, p.D, false), hp_operand(d, p.piece, p.N, padded, false), p.D, width, p.N);
-      const HpProblem qh = hp_problem<H>(hp_operand(w, c.ldw, width, p.D, false), hp_operand(d, p.piece, p.N, padded, true), p.D, p.N, padded, p.splits);
+      HpProblem qw = hp_problem<W>(hp_operand(c.h, c.ldh, p.N, p.D, false), hp_operand(d, ldd, p.N, padded, false), p.D, width, p.N);
+      HpProblem qh = hp_problem<H>(hp_operand(w, c.ldw, width, p.D, false), hp_operand(d, ldd, p.N, padded, true), p.D, p.N, padded, p.splits);
+      if (PIECES) qw.pieces = qh.pieces = hp_six(p.ldp, p.piece);
       typename HpStore<E>::Params ew{static_cast<E*>(out.dw) + c0 * p.D, p.D, static_cast<int>(p.D), static_cast<int>(width), 1.f, s.unit};
       const HpSum::Params eh{s.sum, p.ld_sum, p.N * p.ld_sum, static_cast<int>(p.D), static_cast<int>(p.N), k == 0};
-      if (out.dh == nullptr) return hp_launch<W, E, HpStore<E>>(qw, ew, c.stream);
-      if (out.dw == nullptr) return hp_launch<H, E, HpSum>(qh, eh, c.stream);
-      return hp_launch_both<W, HpStore<E>, H, HpSum, E>(qw, ew, qh, eh, c.stream);
+      if (out.dh == nullptr) return hp_launch<W, M, HpStore<E>>(qw, ew, c.stream);
+      if (out.dw == nullptr) return hp_launch<H, M, HpSum>(qh, eh, c.stream);
+      return hp_launch_both<W, HpStore<E>, H, HpSum, M>(qw, ew, qh, eh, c.stream);
     };
     if (out.dh != nullptr || out.dw != nullptr)
-      rc = p.wide ? gradients(HpLong<false, false>{}, HpLong<false, true>{}) : gradients(HpSmall<false, false>{}, HpSmall<false, true>{});
-    if (rc != AK_OK) return rc;
-    rc = lce_db(d, p.piece, p, c0, width, s, out, c.stream);
+      rc = p.wide ? gradients(HpLong<false, false, PIECES>{}, HpLong<false, true, PIECES>{})
+                  : gradients(HpSmall<false, false, PIECES>{}, HpSmall<false, true, PIECES>{});
+    if (rc == AK_OK && out.db != nullptr)
+      rc = with_type(out.db_dtype, [&](auto t) {
+        using O = typename decltype(t)::type;
+        return column_sums(d, ldd, p.N, width, 1.f, s.unit, static_cast<O*>(out.db) + c0, s.columns, c.stream, p.k, p.piece);
+      });
     if (rc != AK_OK) return rc;
   }
   if (out.dh == nullptr) return AK_OK;
   return hp_total(s.sum, p.ld_sum, p.N * p.ld_sum, p.splits, p.N, static_cast<int>(p.D), 1.f, s.unit, static_cast<E*>(out.dh), c.stream);
-}
-
-inline int lce_backward_f32(LceCall c, const float* lse, const LcePlan& p, const LceSpace& s, const LceGrads& out) {
-  float* x = reinterpret_cast<float*>(s.d);
-  const float *h = static_cast<const float*>(c.h), *w = static_cast<const float*>(c.w);
-  const int N = static_cast<int>(p.N), D = static_cast<int>(p.D);
-  for (int64_t k = 0; k < p.pieces; ++k) {
-    const int64_t c0 = k * p.piece, width = std::min(p.piece, p.V - c0);
-    auto product = [&](GemmParams g) {
-      g.split = 3;
-      return launch_gemm(g, 1, c.stream);
-    };
-    int rc = product(make_gemm(0, 1, N, static_cast<int>(width), D, 1.f, h, c.ldh, w + c0 * c.ldw, c.ldw, 0.f, x, p.piece));
-    if (rc != AK_OK) return rc;
-    hipLaunchKernelGGL(lce_piece_grad_kernel, dim3(static_cast<unsigned>(N)), dim3(256), 0, c.stream, x, p.piece, c.r, static_cast<int>(c0),
-                       static_cast<int>(width), lse, s.share);
-    if (out.dh != nullptr)
-      rc = product(make_gemm(0, 0, N, D, static_cast<int>(width), 1.f, x, p.piece, w + c0 * c.ldw, c.ldw, k == 0 ? 0.f : 1.f, static_cast<float*>(out.dh), D));
-    if (rc != AK_OK) return rc;
-    if (out.dw != nullptr)
-      rc = product(make_gemm(1, 0, static_cast<int>(width), D, N, 1.f, x, p.piece, h, c.ldh, 0.f, static_cast<float*>(out.dw) + c0 * p.D, D));
-    if (rc != AK_OK) return rc;
-    rc = lce_db(x, p.piece, p, c0, width, s, out, c.stream);
-    if (rc != AK_OK) return rc;
-  }
-  return check_launch();
 }
 
 inline int lce_check(const void* h, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype, const int64_t* targets, int64_t rows,
@@ -636,7 +612,7 @@ extern "C" size_t ak_linear_cross_entropy_ws_bytes(int dtype, int64_t rows, int6
   if (!ak::is_element_type(dtype) || rows <= 0 || classes <= 0 || width <= 0 || rows > (1 << 28) || classes > (1 << 28) || width > (1 << 20)) return 0;
   const ak::LcePlan p = ak::lce_plan(dtype, rows, classes, width);
   // enough for operands of any alignment
-  const bool pad = p.es == 2 && (backward != 0 || rows > ak::kLceFewRows);
+  const bool pad = backward != 0 || rows > ak::kLceFewRows;
   return ak::lce_space(p, backward != 0, pad, pad, true, nullptr).bytes;
 }
 
@@ -649,8 +625,8 @@ extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, co
   if (rows == 0) return reduction == kLossNone ? AK_OK : AK_ERR_ARG;
   if (loss == nullptr || lse == nullptr) return AK_ERR_ARG;
   const LcePlan p = lce_plan(dtype, rows, classes, width);
-  const bool few = p.es == 4 || rows <= kLceFewRows;
-  const LceSpace s = lce_space(p, false, !few && !hp_aligned(h, ldh, width), !few && !hp_aligned(w, ldw, width),
+  const bool few = rows <= kLceFewRows, split = dtype == AK_F32;
+  const LceSpace s = lce_space(p, false, !few && (split || !hp_aligned(h, ldh, width)), !few && (split || !hp_aligned(w, ldw, width)),
                                bias != nullptr && bias_dtype != AK_F32, ws);
   if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -658,8 +634,7 @@ extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, co
   rc = lce_bias(c, p, s);
   if (rc != AK_OK) return rc;
   int parts = 0;
-  rc = dtype == AK_F32 ? lce_forward_f32(c, p, s, &parts) : dtype == AK_BF16 ? lce_forward_half<__bf16>(c, p, s, &parts)
-                                                                             : lce_forward_half<_Float16>(c, p, s, &parts);
+  rc = with_type(dtype, [&](auto t) { return lce_forward<typename decltype(t)::type>(c, p, s, &parts); });
   if (rc != AK_OK) return rc;
   float* losses = reduction == kLossNone ? loss : s.losses;
   hipLaunchKernelGGL(lce_rows_kernel, dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(1024), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
@@ -677,16 +652,15 @@ extern "C" int ak_linear_cross_entropy_backward(const float* g, const void* h, i
   if (g == nullptr || lse == nullptr || rows == 0) return AK_ERR_ARG;
   if (dh == nullptr && dw == nullptr && db == nullptr) return AK_OK;
   const LcePlan p = lce_plan(dtype, rows, classes, width);
-  const bool half = p.es == 2;
-  const LceSpace s = lce_space(p, true, half && !hp_aligned(h, ldh, width), half && !hp_aligned(w, ldw, width),
+  const bool split = dtype == AK_F32;
+  const LceSpace s = lce_space(p, true, split || !hp_aligned(h, ldh, width), split || !hp_aligned(w, ldw, width),
                                bias != nullptr && bias_dtype != AK_F32, ws);
   if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   LceCall c{h, ldh, w, ldw, bias, bias_dtype, LceRows{targets, nullptr, ignore_index, static_cast<int>(rows), static_cast<int>(classes)}, width, dtype, st};
   rc = lce_bias(c, p, s);
   if (rc != AK_OK) return rc;
-  hipLaunchKernelGGL(lce_shares_kernel, dim3(1), dim3(1024), 0, st, c.r, g, reduction, half ? 0 : 1, dtype == AK_F16 ? 14 : 0, s.share, s.unit);
+  hipLaunchKernelGGL(lce_shares_kernel, dim3(1), dim3(1024), 0, st, c.r, g, reduction, split ? 1 : 0, dtype == AK_F16 ? 14 : 0, s.share, s.unit);
   const LceGrads out{dh, dw, db, bias == nullptr ? dtype : bias_dtype};
-  return !half ? lce_backward_f32(c, lse, p, s, out) : dtype == AK_BF16 ? lce_backward_half<__bf16>(c, lse, p, s, out)
-                                                                        : lce_backward_half<_Float16>(c, lse, p, s, out);
+  return with_type(dtype, [&](auto t) { return lce_backward<typename decltype(t)::type>(c, lse, p, s, out); });
 }
