@@ -71,7 +71,8 @@ template <typename I>
 struct EmbSorted {
   Tokens<I> t;
   int bins, ranges, chunk, chunks;       // rows of a range, tokens of a chunk
-  int* counts;                           // [range][chunk]
+  int* counts;                           // [chunk][range]
+  int* firsts;                           // first sorted position of each range, and behind the last
   int *token, *place;                    // tokens and their positions by range
   int *starts, *order, *sorted;          // first sorted position of each row's tokens; position in the text and token of each
 };
@@ -88,7 +89,7 @@ static __global__ __launch_bounds__(1024) void emb_count_kernel(EmbSorted<I> p) 
     if (v >= 0) atomicAdd(&count[v / p.bins], 1);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < p.ranges; i += 1024) p.counts[i * p.chunks + blockIdx.x] = count[i];
+  for (int i = threadIdx.x; i < p.ranges; i += 1024) p.counts[blockIdx.x * p.ranges + i] = count[i];
 }
 
 // A stable counting sort by one work group: every wave goes through a part of its own, twice, counting keys and then placing them.
@@ -107,16 +108,8 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
     end = begin + p.chunk < p.t.count ? begin + p.chunk : p.t.count;
   }
   if constexpr (MODE == kSortRange) {
-    // the ranges in front of this one, and its own
-    int front = 0, own = 0;
-    const int in_front = static_cast<int>(blockIdx.x) * p.chunks;
-    for (int i = threadIdx.x; i < in_front; i += 64 * kEmbWaves) front += p.counts[i];
-    for (int i = threadIdx.x; i < p.chunks; i += 64 * kEmbWaves) own += p.counts[in_front + i];
-    front = group_sum<kEmbWaves>(front, sums);
-    own = group_sum<kEmbWaves>(own, below_of);
-    __syncthreads();
-    begin = first = front;
-    end = begin + own;
+    begin = first = p.firsts[blockIdx.x];
+    end = p.firsts[blockIdx.x + 1];
   }
   __syncthreads();
   const int64_t part = (end - begin + 64 * kEmbWaves - 1) / (64 * kEmbWaves) * 64, n0 = begin + wave * part, n1 = n0 + part < end ? n0 + part : end;
@@ -163,8 +156,9 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
   int mine = 0, earlier = 0;             // of this key: tokens behind it that count for the next key, tokens in front of this work group's
   if constexpr (MODE == kSortChunk) {
     if (threadIdx.x < keys)
+#pragma unroll 8
       for (int c = 0; c < p.chunks; ++c) {
-        const int n = p.counts[threadIdx.x * p.chunks + c];
+        const int n = p.counts[c * p.ranges + threadIdx.x];
         mine += n;
         earlier += c < static_cast<int>(blockIdx.x) ? n : 0;
       }
@@ -191,6 +185,11 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
         if (v == p.t.rows - 1) p.starts[p.t.rows] = at + mine;
       }
     }
+    if constexpr (MODE == kSortChunk)
+      if (blockIdx.x == 0 && threadIdx.x < keys) {
+        p.firsts[threadIdx.x] = at;
+        if (static_cast<int>(threadIdx.x) == keys - 1) p.firsts[keys] = at + mine;
+      }
     at += earlier;
 #pragma unroll
     for (int w = 0; w < kEmbWaves; ++w) {
@@ -228,6 +227,7 @@ struct EmbSums {
   const int *starts, *order, *sorted;
   const void* g;
   void* out;
+  int2* joins;             // [chunks] token and chunks of the run that begins in a chunk and ends in a later one; no chunks: none
   float *lead, *trail;     // [chunks][ldp] parts of runs that began in front of a chunk; that begin in it and go on behind it
   int64_t ldg, ldo, ldp;
   int rows, D, chunk, chunks, slabs, row_groups;
@@ -280,7 +280,10 @@ static __global__ __launch_bounds__(256) void emb_sums_kernel(EmbSums p) {
   const int chunk = static_cast<int>(unit / p.slabs), slab = static_cast<int>(unit - static_cast<int64_t>(chunk) * p.slabs);
   const int total = p.starts[p.rows];
   const int p0 = chunk * p.chunk, p1 = min(p0 + p.chunk, total);
-  if (p0 >= p1) return;
+  if (p0 >= p1) {
+    if (slab == 0 && lane == 0) p.joins[chunk] = int2{0, 0};
+    return;
+  }
   const int c = slab * 64 * E + lane * E;
   const bool has = c < p.D, full = c + E <= p.D;
   const int my_row = p0 + lane < p1 ? p.order[p0 + lane] : 0;
@@ -298,6 +301,12 @@ static __global__ __launch_bounds__(256) void emb_sums_kernel(EmbSums p) {
 #pragma unroll
     for (int e = 0; e < E; ++e) to[e] = sum[e];
   };
+  if (slab == 0 && lane == 0) {
+    const int last = p.sorted[p1 - 1];
+    int2 join = {last, 0};
+    if (last == behind && p.starts[last] >= p0) join.y = (p.starts[last + 1] - 1) / p.chunk - chunk + 1;
+    p.joins[chunk] = join;
+  }
   int token = __builtin_amdgcn_readlane(my_token, 0);
   bool first = true;
   for (int i = 0; i < p1 - p0; i += U) {
@@ -334,32 +343,48 @@ static __global__ __launch_bounds__(256) void emb_sums_kernel(EmbSums p) {
   flush(token, first, true);
 }
 
-// The run that begins in a chunk and ends in a later one; four waves take a part of the chunks each, 256 columns a work group.
-template <typename O>
-static __global__ __launch_bounds__(256) void emb_joins_kernel(EmbSums p) {
-  __shared__ floatx4 joined[4][64];
-  const int chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int total = p.starts[p.rows], p0 = chunk * p.chunk, p1 = p0 + p.chunk;
-  if (p1 >= total) return;
-  const int token = p.sorted[p1 - 1];
-  const int s0 = p.starts[token], s1 = p.starts[token + 1];
-  if (s0 < p0 || s1 <= p1) return;             // begins in front of this chunk, ends with it
-  const int last = (s1 - 1) / p.chunk, parts = last - chunk + 1, per = (parts + 3) / 4;
-  const int c = blockIdx.y * 256 + 4 * lane;
+// Parts k0 .. k1 - 1 of the run that begins in a chunk, four columns from c on.
+__device__ __forceinline__ floatx4 emb_parts(const EmbSums& p, int chunk, int k0, int k1, int c) {
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (c < p.D) {
-    const int k1 = min((wave + 1) * per, parts);
 #pragma unroll 8
-    for (int k = wave * per; k < k1; ++k)
-      sum += *reinterpret_cast<const floatx4*>((k == 0 ? p.trail : p.lead) + static_cast<int64_t>(chunk + k) * p.ldp + c);
-  }
-  joined[wave][lane] = sum;
-  __syncthreads();
-  if (wave != 0 || c >= p.D) return;
-  float v[4];
+  for (int k = k0; k < k1; ++k) sum += *reinterpret_cast<const floatx4*>((k == 0 ? p.trail : p.lead) + static_cast<int64_t>(chunk + k) * p.ldp + c);
+  return sum;
+}
+
+// Runs that begin in a chunk and end in a later one, 256 columns at a time.  The first work groups take the long ones: a run of more than
+// 16 chunks begins in no more than one of 16 neighbouring chunks; four waves take a quarter of its parts each.  Behind them, a wave
+// takes the run of a chunk alone.  (All four waves for every run: 17 us for 131072 tokens of 1024 columns, most of it waves that wait.)
+constexpr int kEmbLong = 16;
+
+template <typename O>
+static __global__ __launch_bounds__(256) void emb_joins_kernel(EmbSums p, int long_groups, int column_blocks) {
+  __shared__ floatx4 joined[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (static_cast<int>(blockIdx.x) < long_groups) {
+    const int first = static_cast<int>(blockIdx.x) / column_blocks * kEmbLong, c = static_cast<int>(blockIdx.x) % column_blocks * 256 + 4 * lane;
+    int2 mine = {0, 0};
+    if (lane < kEmbLong && first + lane < p.chunks) mine = p.joins[first + lane];
+    const u64 runs = __ballot(mine.y > kEmbLong);          // (the same in every wave)
+    if (runs == 0) return;
+    const int at = __builtin_ctzll(runs), token = __builtin_amdgcn_readlane(mine.x, at), parts = __builtin_amdgcn_readlane(mine.y, at), per = (parts + 3) / 4;
+    joined[wave][lane] = c < p.D ? emb_parts(p, first + at, wave * per, min((wave + 1) * per, parts), c) : floatx4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    if (wave != 0 || c >= p.D) return;
+    float v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ((joined[0][lane][e] + joined[1][lane][e]) + joined[2][lane][e]) + joined[3][lane][e];
-  emb_write<O, 4>(p, token, c, v);
+    for (int e = 0; e < 4; ++e) v[e] = ((joined[0][lane][e] + joined[1][lane][e]) + joined[2][lane][e]) + joined[3][lane][e];
+    emb_write<O, 4>(p, token, c, v);
+    return;
+  }
+  const int64_t unit = static_cast<int64_t>(blockIdx.x - long_groups) * 4 + wave;
+  const int64_t chunk = unit / column_blocks;
+  const int c = static_cast<int>(unit - chunk * column_blocks) * 256 + 4 * lane;
+  if (chunk >= p.chunks || c >= p.D) return;
+  const int2 join = p.joins[chunk];
+  if (join.y == 0 || join.y > kEmbLong) return;
+  const floatx4 sum = emb_parts(p, static_cast<int>(chunk), 0, join.y, c);
+  const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+  emb_write<O, 4>(p, join.x, c, v);
 }
 
 // Sorted positions of a chunk: enough chunks for 32 waves a CU, few enough for little to be joined.
@@ -378,8 +403,9 @@ inline int with_tokens(int type, F&& f) {
 }
 
 struct EmbSpace {
-  int *starts, *order, *sorted, *token, *place, *counts;
+  int *starts, *order, *sorted, *token, *place, *counts, *firsts;
   int bins, ranges, cut, cuts;           // rows of a range; tokens of a chunk of the sort, or all of them at once: cuts == 0
+  int2* joins;
   float *lead, *trail;
   int chunk, chunks;
   int64_t ldp;
@@ -410,7 +436,9 @@ inline EmbSpace emb_space(int64_t tokens, int64_t rows, int64_t D, int elements,
     s.token = static_cast<int*>(take(tokens));
     s.place = static_cast<int*>(take(tokens));
     s.counts = static_cast<int*>(take(static_cast<int64_t>(s.ranges) * s.cuts));
+    s.firsts = static_cast<int*>(take(s.ranges + 1));
   }
+  s.joins = static_cast<int2*>(take(2 * static_cast<int64_t>(s.chunks)));
   s.lead = static_cast<float*>(take(s.chunks * s.ldp));
   s.trail = static_cast<float*>(take(s.chunks * s.ldp));
   s.bytes = used;
@@ -479,7 +507,7 @@ extern "C" int ak_embedding_backward(const void* g, int dtype, int64_t ldg, cons
   rc = with_tokens(token_type, [&](auto i) {
     using I = typename decltype(i)::type;
     const Tokens<I> tk{static_cast<const I*>(tokens), count, static_cast<int>(rows), padding};
-    const EmbSorted<I> q{tk, s.bins, s.ranges, s.cut, s.cuts, s.counts, s.token, s.place, s.starts, s.order, s.sorted};
+    const EmbSorted<I> q{tk, s.bins, s.ranges, s.cut, s.cuts, s.counts, s.firsts, s.token, s.place, s.starts, s.order, s.sorted};
     const dim3 ranges(static_cast<unsigned>(s.ranges)), cuts(static_cast<unsigned>(s.cuts)), threads(64 * kEmbWaves);
     if (s.cuts == 0) {
       hipLaunchKernelGGL((emb_sort_kernel<I, kSortAll>), ranges, threads, 0, st, q);
@@ -493,7 +521,7 @@ extern "C" int ak_embedding_backward(const void* g, int dtype, int64_t ldg, cons
   if (rc != AK_OK) return rc;
   EmbSums p;
   p.starts = s.starts; p.order = s.order; p.sorted = s.sorted;
-  p.g = g; p.out = out; p.lead = s.lead; p.trail = s.trail;
+  p.g = g; p.out = out; p.joins = s.joins; p.lead = s.lead; p.trail = s.trail;
   p.ldg = ldg; p.ldo = ldo; p.ldp = s.ldp;
   p.rows = static_cast<int>(rows); p.D = static_cast<int>(width);
   p.chunk = s.chunk; p.chunks = s.chunks;
@@ -510,7 +538,10 @@ extern "C" int ak_embedding_backward(const void* g, int dtype, int64_t ldg, cons
       return check_launch();
     });
     if (done != AK_OK || p.chunks < 2) return done;
-    hipLaunchKernelGGL(emb_joins_kernel<O>, dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>((width + 255) / 256)), dim3(256), 0, st, p);
+    const int64_t column_blocks = (width + 255) / 256, longs = (p.chunks + kEmbLong - 1) / kEmbLong * column_blocks, shorts = (p.chunks * column_blocks + 3) / 4;
+    if (longs + shorts > 0x7fffffff) return AK_ERR_TOO_LARGE;
+    hipLaunchKernelGGL(emb_joins_kernel<O>, dim3(static_cast<unsigned>(longs + shorts)), dim3(256), 0, st, p, static_cast<int>(longs),
+                       static_cast<int>(column_blocks));
     return check_launch();
   });
 }

@@ -233,15 +233,14 @@ __device__ __forceinline__ floatx4 lce_mma(const LceEight<E>& a, const LceEight<
   }
 }
 
-// A few rows: a wave takes 16 classes at a time, weights straight to the matrix instruction (16 x 16 x 32).  A lane has 32 consecutive
+// A few rows: a wave (and work group: the device is filled evenly) takes 16 classes, weights straight to the matrix instruction (16 x 16 x 32).  A lane has 32 consecutive
 // k of every 128 of one class: what the four lanes of a class read at once is a part of each 128-byte line, all of it in four loads.
 // The order of k is the same for both operands.
 template <typename E, int NB>
-static __global__ __launch_bounds__(512) void lce_few_kernel(const E* __restrict__ h, int64_t ldh, const E* __restrict__ w, int64_t ldw, int D,
+static __global__ __launch_bounds__(64) void lce_few_kernel(const E* __restrict__ h, int64_t ldh, const E* __restrict__ w, int64_t ldw, int D,
                                                              LceRows r, floatx2* __restrict__ part, float* __restrict__ at_target) {
-  __shared__ floatx2 joined[8][16 * NB];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4, l16 = lane & 15;
-  const int c0 = (blockIdx.x * 8 + wave) * 16;
+  const int lane = threadIdx.x, quarter = lane >> 4, l16 = lane & 15;
+  const int c0 = blockIdx.x * 16;
   const E* __restrict__ wr = w + static_cast<int64_t>(min(c0 + l16, r.classes - 1)) * ldw + 32 * quarter;
   const E* hr[NB];
 #pragma unroll
@@ -303,18 +302,20 @@ static __global__ __launch_bounds__(512) void lce_few_kernel(const E* __restrict
     floatx2 ms = {m, s};
     ms = lce_join2(ms, floatx2{__shfl_xor(ms[0], 16), __shfl_xor(ms[1], 16)});
     ms = lce_join2(ms, floatx2{__shfl_xor(ms[0], 32), __shfl_xor(ms[1], 32)});
-    if (quarter == 0) joined[wave][j] = ms;
-  }
-  __syncthreads();
-  for (int j = threadIdx.x; j < 16 * NB && j < r.rows; j += 512) {
-    floatx2 ms = joined[0][j];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) ms = lce_join2(ms, joined[k][j]);
-    part[static_cast<int64_t>(blockIdx.x) * r.rows + j] = ms;
+    if (quarter == 0 && j < r.rows) part[static_cast<int64_t>(blockIdx.x) * r.rows + j] = ms;
   }
 }
 
-// lse and loss of 64 rows from the parts of all classes, a part of them a wave.
+__device__ __forceinline__ void lce_row(const LceRows& r, int j, floatx2 ms, const float* __restrict__ at_target, float* __restrict__ losses,
+                                        float* __restrict__ lse) {
+  const int64_t target = r.targets[j];
+  const float l = __logf(ms[1]);
+  lse[j] = ms[0] + l;
+  // (a target that is no class and not the ignored one: NaN)
+  losses[j] = target == r.ignore ? 0.f : target < 0 || target >= r.classes ? NAN : ms[0] - at_target[j] + l;
+}
+
+// lse and loss of 64 rows from the parts of all classes, a sixteenth of them a wave.
 static __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRows r, const floatx2* __restrict__ part, int parts, const float* __restrict__ at_target,
                                                                float* __restrict__ losses, float* __restrict__ lse) {
   __shared__ floatx2 joined[16][64];
@@ -330,11 +331,25 @@ static __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRows r, const 
   if (wave != 0 || j >= r.rows) return;
 #pragma unroll
   for (int k = 1; k < 16; ++k) ms = lce_join2(ms, joined[k][lane]);
-  const float l = ms[0] + __logf(ms[1]);
-  const int64_t target = r.targets[j];
-  lse[j] = l;
-  // (a target that is no class and not the ignored one: NaN)
-  losses[j] = target == r.ignore ? 0.f : target < 0 || target >= r.classes ? NAN : ms[0] - at_target[j] + __logf(ms[1]);
+  lce_row(r, j, ms, at_target, losses, lse);
+}
+
+// A row a work group, for few rows of many parts.
+static __global__ __launch_bounds__(512) void lce_row_kernel(LceRows r, const floatx2* __restrict__ part, int parts, const float* __restrict__ at_target,
+                                                             float* __restrict__ losses, float* __restrict__ lse) {
+  __shared__ floatx2 joined[8];
+  const int j = blockIdx.x;
+  floatx2 ms = {-INFINITY, 0.f};
+#pragma unroll 8
+  for (int t = threadIdx.x; t < parts; t += 512) ms = lce_join2(ms, part[static_cast<int64_t>(t) * r.rows + j]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ms = lce_join2(ms, floatx2{__shfl_xor(ms[0], o), __shfl_xor(ms[1], o)});
+  if ((threadIdx.x & 63) == 0) joined[threadIdx.x >> 6] = ms;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) ms = lce_join2(ms, joined[w]);
+  lce_row(r, j, ms, at_target, losses, lse);
 }
 
 // The sum or mean over the rows, in double.
@@ -460,7 +475,8 @@ inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_
   if (pad_w) s.w = c.take<unsigned char>(p.V * p.ldp * p.k * 2);
   if (bias) s.bias = c.take<float>(p.V);
   if (!backward) {
-    s.part = c.take<floatx2>((p.V + 127) / 128 * p.N);
+    const int64_t tile = p.N <= kLceFewRows ? 16 : 128;      // the fewest classes of a part
+    s.part = c.take<floatx2>((p.V + tile - 1) / tile * p.N);
     s.at_target = c.take<float>(p.N);
     s.losses = c.take<float>(p.N);
   } else {
@@ -518,10 +534,10 @@ inline int lce_bias(LceCall& c, const LcePlan& p, const LceSpace& s) {
 template <typename E>
 inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
   if (p.N <= kLceFewRows) {
-    const int64_t groups = (p.V + 127) / 128;
+    const int64_t groups = (p.V + 15) / 16;
     *parts = static_cast<int>(groups);
     auto go = [&](auto nb) {
-      hipLaunchKernelGGL((lce_few_kernel<E, decltype(nb)::value>), dim3(static_cast<unsigned>(groups)), dim3(512), 0, c.stream, static_cast<const E*>(c.h),
+      hipLaunchKernelGGL((lce_few_kernel<E, decltype(nb)::value>), dim3(static_cast<unsigned>(groups)), dim3(64), 0, c.stream, static_cast<const E*>(c.h),
                          c.ldh, static_cast<const E*>(c.w), c.ldw, static_cast<int>(p.D), c.r, s.part, s.at_target);
       return check_launch();
     };
@@ -637,7 +653,10 @@ extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, co
   rc = with_type(dtype, [&](auto t) { return lce_forward<typename decltype(t)::type>(c, p, s, &parts); });
   if (rc != AK_OK) return rc;
   float* losses = reduction == kLossNone ? loss : s.losses;
-  hipLaunchKernelGGL(lce_rows_kernel, dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(1024), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
+  if (few)
+    hipLaunchKernelGGL(lce_row_kernel, dim3(static_cast<unsigned>(rows)), dim3(512), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
+  else
+    hipLaunchKernelGGL(lce_rows_kernel, dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(1024), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
   if (reduction != kLossNone) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, c.r, losses, reduction, loss);
   return check_launch();
 }
