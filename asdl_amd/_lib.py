@@ -171,9 +171,13 @@ def load_host():
     spec = importlib.util.spec_from_file_location('asdl_amd_host_calls', HOST_PATH)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                  for name in ('ak_layer_norm', 'ak_layer_norm_backward', 'ak_layer_norm_backward_ws_bytes', 'ak_sample_filtered', 'ak_grad_norm',
-                               'ak_clip_grad_norm', 'ak_grad_norm_ws_bytes')))
+    def addresses(*names):
+        return (ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names)
+    module.bind(*addresses('ak_layer_norm', 'ak_layer_norm_backward', 'ak_layer_norm_backward_ws_bytes', 'ak_sample_filtered', 'ak_grad_norm',
+                           'ak_clip_grad_norm', 'ak_grad_norm_ws_bytes'))
+    module.bind_step(*addresses('ak_linear_cross_entropy', 'ak_linear_cross_entropy_backward', 'ak_linear_cross_entropy_ws_bytes', 'ak_embedding',
+                                'ak_embedding_backward', 'ak_embedding_backward_ws_bytes', 'ak_quantize_8bit', 'ak_dequantize_8bit',
+                                'ak_weight_grad_8bit', 'ak_weight_grad_8bit_ws_bytes'))
     _host = module
     return module
 

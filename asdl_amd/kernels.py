@@ -1664,6 +1664,11 @@ def linear_cross_entropy(h, weight, targets, bias=None, ignore_index=-100, reduc
     of their type or float32; targets [...] int64.  loss (float32): one number, or one per row with reduction='none'.  Rows whose target is
     ``ignore_index`` have none; a target that is neither it nor a class gives NaN (the host does not look at targets).  lse (float32, one
     per row, the log of the sum of exponentials) is what linear_cross_entropy_backward() needs."""
+    host = _usual(h) if reduction in _REDUCTIONS else None
+    if host is not None:
+        done = host.linear_cross_entropy(h, weight, targets, bias, ignore_index, _REDUCTIONS[reduction], _raw_stream(h.get_device()))
+        if done is not None:
+            return done if type(done) is tuple else _lib.check(done, 'ak_linear_cross_entropy')
     code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, reduction)
     device = h.device
     if device.index != torch.cuda.current_device():
@@ -1693,6 +1698,12 @@ def linear_cross_entropy_backward(g, h, weight, targets, lse, bias=None, ignore_
     """(dh, dw, db) of linear_cross_entropy() for the gradient ``g`` (float32, of the loss's shape); None for what is not needed.  They have the
     types of h, weight and bias.  The logits are formed again, in pieces; for 16-bit operands their gradient, which both products read, is
     rounded to the operands' type, as a framework's backward pass in that type does."""
+    host = _usual(h) if reduction in _REDUCTIONS else None
+    if host is not None:
+        done = host.linear_cross_entropy_backward(h, weight, targets, bias, ignore_index, _REDUCTIONS[reduction], g, lse,
+                                                  (1 if need_h else 0) | (2 if need_weight else 0) | (4 if need_bias else 0), _raw_stream(h.get_device()))
+        if done is not None:
+            return done if type(done) is tuple else _lib.check(done, 'ak_linear_cross_entropy_backward')
     code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, reduction)
     for what, t, shape in (('g', g, targets.shape if kind == 0 else ()), ('lse', lse, targets.shape)):
         if t.dtype != torch.float32 or t.shape != shape:
@@ -1744,6 +1755,11 @@ def embedding(tokens, weight, scale=1.0, out_dtype=None):
     """scale * weight[tokens]: rows of ``weight`` [rows, features] (float32, bfloat16 or float16, any row stride) for int32 or int64 ``tokens``
     of any shape, in weight's type, or float32 with ``out_dtype=torch.float32``; rounded once.  A token that names no row gives a row of NaN (the host
     does not look at tokens)."""
+    host = _usual(weight)
+    if host is not None and (out_dtype is None or out_dtype == torch.float32 or out_dtype == weight.dtype):
+        done = host.embedding(tokens, weight, float(scale), out_dtype == torch.float32, _raw_stream(weight.get_device()))
+        if done is not None:
+            return done if type(done) is not int else _lib.check(done, 'ak_embedding')
     code = _ELEMENT_TYPES.get(weight.dtype)
     if code is None or not weight.is_cuda:
         _require_gpu(weight)
@@ -1773,6 +1789,11 @@ def embedding_backward(g, tokens, num_embeddings, scale=1.0, padding_idx=None, o
     each row rounded once.  Without ``out`` it is made, of the type ``dtype`` (g's); with it, ``out`` has rows of stride 1 elements (float32,
     bfloat16 or float16).  Rows that no token names are written, too (with beta = 1 they stay).  ``padding_idx``: a token that adds nothing,
     as tokens that name no row do."""
+    host = _usual(g) if out is None and padding_idx is None and (dtype is None or dtype == g.dtype) else None
+    if host is not None:
+        done = host.embedding_backward(g, tokens, num_embeddings, float(scale), -1, _raw_stream(g.get_device()))
+        if done is not None:
+            return done if type(done) is not int else _lib.check(done, 'ak_embedding_backward')
     code = _ELEMENT_TYPES.get(g.dtype)
     if code is None or not g.is_cuda:
         _require_gpu(g)
@@ -1830,6 +1851,11 @@ def _gelu_code(approximate):
 
 
 def _quantize(x, gelu):
+    host = _usual(x)
+    if host is not None:
+        done = host.quantize_8bit(x, gelu, _raw_stream(x.get_device()))
+        if done is not None:
+            return (done[0], Quantized8(done[1], done[2])) if type(done) is tuple else _lib.check(done, 'ak_quantize_8bit')
     code, F, rows = _norm_rows(x)
     device = x.device
     if device.index != torch.cuda.current_device():
@@ -1866,6 +1892,11 @@ def quantize_8bit(x):
 
 def dequantize_8bit(kept, dtype=torch.float32):
     """The values that quantize_8bit() has kept, as float32, bfloat16 (both exact within float32's range) or float16."""
+    host = _usual(kept[0]) if dtype in _ELEMENT_TYPES else None
+    if host is not None:
+        done = host.dequantize_8bit(*kept, -1, None, _ELEMENT_TYPES[dtype], _raw_stream(kept[0].get_device()))
+        if done is not None:
+            return done if type(done) is not int else _lib.check(done, 'ak_dequantize_8bit')
     return _dequantize(kept, -1, None, dtype)
 
 
@@ -1878,6 +1909,13 @@ def gelu_8bit_backward(g, kept, approximate='none'):
     """The gradient of gelu_8bit()'s input for the gradient ``g`` of its result, from the kept input: g times the derivative at the kept
     values, of the type of g."""
     way = _gelu_code(approximate)
+    if g.dtype not in _ELEMENT_TYPES:
+        _element_type(g, 'g')
+    host = _usual(g)
+    if host is not None:
+        done = host.dequantize_8bit(*kept, way, g, _ELEMENT_TYPES[g.dtype], _raw_stream(g.get_device()))
+        if done is not None:
+            return done if type(done) is not int else _lib.check(done, 'ak_dequantize_8bit')
     _check_kept(kept)
     if g.shape != kept.codes.shape:
         raise ValueError(f'shapes differ: {tuple(g.shape)} vs {tuple(kept.codes.shape)}')
@@ -1908,6 +1946,12 @@ def weight_grad_8bit(g, kept, need_weight=True, need_bias=True, dtype=None):
     """(dw, db) of a linear layer whose input was kept with quantize_8bit(): dw = g^T x [out, features] and db = the sums of g [out], for the
     gradient ``g`` [..., out] of its result (float32, bfloat16 or float16, any row stride); None for what is not needed.  ``dtype``: of both (g's).
     The products are exact (the kept values and the pieces that g is taken apart into are bfloat16 numbers), their sums fp32."""
+    code = _ELEMENT_TYPES.get(dtype or g.dtype)
+    host = _usual(g) if code is not None else None
+    if host is not None:
+        done = host.weight_grad_8bit(*kept, g, (1 if need_weight else 0) | (2 if need_bias else 0), code, _raw_stream(g.get_device()))
+        if done is not None:
+            return done if type(done) is tuple else _lib.check(done, 'ak_weight_grad_8bit')
     rows, F = _check_kept(kept)
     code = _ELEMENT_TYPES.get(g.dtype)
     if code is None or not g.is_cuda:
