@@ -16,6 +16,7 @@ from .prec_grad_maker import (PreconditionedGradientMaker, PreconditioningConfig
                               INTERVAL_CONSTANT, INTERVAL_STEP, INTERVAL_LINEAR, INTERVAL_TYPES)
 from .natural_gradient import NaturalGradientMaker, KfacGradientMaker
 from .shampoo import ShampooGradientMaker, Preconditioner, BlockPartitioner, compute_power
-from .layers import layer_norm, FusedLayerNorm, fuse_layer_norms
+from .layers import (layer_norm, FusedLayerNorm, fuse_layer_norms, linear_cross_entropy, embedding, FusedEmbedding, fuse_embeddings, gelu_8bit,
+                     linear_8bit, GELU8bit, Linear8bit, keep_activations_8bit)
 from .clipping import clip_grad_norm_
 from . import kernels

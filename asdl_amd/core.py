@@ -8,7 +8,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.graph import get_gradient_edge
 
-from .layers import FusedLayerNorm
+from .layers import FusedLayerNorm, Linear8bit
 from .matrices import *
 from .operations import *
 from .operations import FWD_OPS, BWD_OPS, BWD_OPS_WITH_INPUTS
@@ -226,6 +226,8 @@ def module_wise_assignments(model, *assign_rules, ignore_modules=None, map_rule=
             values = specified[module.__class__]
         elif isinstance(module, FusedLayerNorm) and nn.LayerNorm in specified:      # it stands in for one
             values = specified[nn.LayerNorm]
+        elif isinstance(module, Linear8bit) and nn.Linear in specified:
+            values = specified[nn.Linear]
         else:
             if len(common) == 0:
                 continue

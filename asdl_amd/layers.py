@@ -1,14 +1,18 @@
-"""Layer norm on the kernels of csrc/layer_norm.hip as a function and as a module that stands in for torch.nn.LayerNorm.
+"""Layers on the framework's own kernels, as functions and as modules that stand in for torch's: layer norm (csrc/layer_norm.hip),
+embeddings (csrc/embedding.hip), the cross entropy of a model's last linear layer (csrc/linear_cross_entropy.hip), and linear layers and
+GELU that keep their inputs in 8 bits for the backward pass (csrc/keep_8bit.hip).
 
-Under the hooks of a gradient maker such a module has its unit-wise Fisher blocks computed by its own backward pass, from the values
+Under the hooks of a gradient maker a FusedLayerNorm has its unit-wise Fisher blocks computed by its own backward pass, from the values
 that pass reads anyway, where torch.nn.LayerNorm has its output and output gradient read once more
 (asdl/operations/layernorm.py:69-78)."""
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from . import kernels
 
-__all__ = ['layer_norm', 'FusedLayerNorm', 'fuse_layer_norms']
+__all__ = ['layer_norm', 'FusedLayerNorm', 'fuse_layer_norms', 'linear_cross_entropy', 'embedding', 'FusedEmbedding', 'fuse_embeddings', 'gelu_8bit',
+           'linear_8bit', 'GELU8bit', 'Linear8bit', 'keep_activations_8bit']
 
 
 class BlocksRequest:
@@ -131,3 +135,204 @@ def fuse_layer_norms(model: nn.Module) -> int:
     for m in found:
         m.__class__ = FusedLayerNorm
     return len(found)
+
+
+class _Last(torch.autograd.Function):
+    """Gradients in a graph of their own, which has no way back (see _Once).  gradients(g) is called once; ``tensors``: what it reads."""
+
+    @staticmethod
+    def forward(ctx, gradients, name, g, *tensors):
+        ctx.name = name
+        return gradients(g)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f'{ctx.name}() is differentiable once (once_differentiable): it has no second derivative.')
+
+
+def _last(gradients, name, g, *tensors):
+    """gradients(g), or the same in a graph where one is asked for (create_graph)."""
+    return _Last.apply(gradients, name, g, *tensors) if torch.is_grad_enabled() else gradients(g)
+
+
+def _through(t):
+    """A leaf behind a node of its own, which _wanted() can ask about (the engine does not say it of leaves themselves)."""
+    return t.view_as(t) if t is not None and t.requires_grad and t.grad_fn is None and torch.is_grad_enabled() else t
+
+
+def _wanted(ctx, index):
+    """Whether the running backward pass takes the gradient of an input: one that is restricted to other leaves or edges, as the passes
+    of a sampled Fisher matrix are, does not."""
+    node = ctx.next_functions[index][0] if ctx.needs_input_grad[index] else None
+    return node is not None and torch._C._will_engine_execute_node(node)
+
+
+def _autocast(*tensors):
+    """Floating-point tensors in the type that a linear layer computes in, autocast's where it is on; leaves behind nodes of their own."""
+    if torch.is_autocast_enabled('cuda'):
+        dtype = torch.get_autocast_dtype('cuda')
+        tensors = (t if t is None else t.to(dtype) for t in tensors)
+    return tuple(_through(t) for t in tensors)
+
+
+# ------------------------------------------------------------------------------ the loss at the vocabulary's end
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, weight, target, bias, ignore_index, reduction):
+        loss, lse = kernels.linear_cross_entropy(h, weight, target, bias, ignore_index, reduction)
+        ctx.save_for_backward(h, weight, target, bias, lse)
+        ctx.options = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        h, weight, target, bias, lse = ctx.saved_tensors
+        need = [_wanted(ctx, i) for i in (0, 1, 3)]
+        dh, dw, db = _last(lambda g: kernels.linear_cross_entropy_backward(g, h, weight, target, lse, bias, *ctx.options, *need), 'linear_cross_entropy', g,
+                           h, weight, bias)
+        return dh, dw, None, db, None, None
+
+
+def linear_cross_entropy(input, weight, target, bias=None, ignore_index=-100, reduction='mean'):
+    """torch.nn.functional.cross_entropy(torch.nn.functional.linear(input, weight, bias), target) without the logits: they are formed in pieces of
+    the classes, forward and once more on the way back, and never kept.  input [..., features] and weight [classes, features] (a model's head)
+    of one type, float32, bfloat16 or float16; under autocast both are cast to its type, as a linear layer does.  target [...] int64;
+    the loss is float32.  Differentiable once.  A gradient maker takes it as its loss call: the model call then returns the input of the head,
+    e.g. ``maker.setup_loss_call(linear_cross_entropy, maker.setup_model_call(features, x), head.weight, target)`` (not with a sampled or
+    exact Fisher matrix, which need the logits)."""
+    input, weight, bias = _autocast(input, weight, bias)
+    return _LinearCrossEntropy.apply(input, weight, target, bias, ignore_index, reduction)
+
+
+# ------------------------------------------------------------------------------ embeddings
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, padding_idx, scale):
+        ctx.save_for_backward(tokens)
+        ctx.options = weight.shape[0], scale, padding_idx
+        ctx.weight_dtype = weight.dtype
+        return kernels.embedding(tokens, weight, scale)
+
+    @staticmethod
+    def backward(ctx, g):
+        tokens, = ctx.saved_tensors
+        rows, scale, padding_idx = ctx.options
+        # (linear in g: a second derivative with respect to it would be another lookup, which nobody asks for)
+        return None, _last(lambda g: kernels.embedding_backward(g, tokens, rows, scale, padding_idx, dtype=ctx.weight_dtype), 'embedding', g), None, None
+
+
+def embedding(input, weight, padding_idx=None, scale=1.0):
+    """scale * torch.nn.functional.embedding(input, weight, padding_idx): rows of ``weight`` for int32 or int64 ``input``, differentiable once.  The
+    gradient is summed by tokens in sorted order, in fp32: the same bits every time, where torch's adds rows in the order in which
+    they come.  A token that names no row gives NaN and takes no gradient."""
+    return _Embedding.apply(input, weight, padding_idx, float(scale))
+
+
+class FusedEmbedding(nn.Embedding):
+    """torch.nn.Embedding (the same arguments, parameters and state dict) on embedding() above; ``scale``: a factor of the rows that are looked
+    up.  max_norm, scale_grad_by_freq and sparse are not taken."""
+    scale = 1.0
+
+    def __init__(self, *args, scale=1.0, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.scale = scale
+        _plain_embedding(self)
+
+    def forward(self, input):
+        return embedding(input, self.weight, self.padding_idx, self.scale)
+
+
+def _plain_embedding(module, refuse=True):
+    plain = module.max_norm is None and not module.scale_grad_by_freq and not module.sparse
+    if refuse and not plain:
+        raise ValueError('max_norm, scale_grad_by_freq and sparse are not taken by a FusedEmbedding.')
+    return plain
+
+
+def _stand_in(model, kinds):
+    """Modules of exactly these classes become their stand-ins in place: parameters, hooks and names stay.  Returns how many there were."""
+    found = [m for m in model.modules() if type(m) in kinds and (type(m) is not nn.Embedding or _plain_embedding(m, refuse=False))]
+    for m in found:
+        m.__class__ = kinds[type(m)]
+    return len(found)
+
+
+def fuse_embeddings(model: nn.Module) -> int:
+    """Makes every torch.nn.Embedding of ``model`` (not subclasses of it, nor those with max_norm, scale_grad_by_freq or sparse) a
+    FusedEmbedding, in place.  Returns how many there were.  The model then runs on a ROCm device only."""
+    return _stand_in(model, {nn.Embedding: FusedEmbedding})
+
+
+# ------------------------------------------------------------------------------ activations in 8 bits
+class _GELU8bit(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, approximate):
+        y, kept = kernels.gelu_8bit(x, approximate)
+        ctx.save_for_backward(*kept)
+        ctx.approximate = approximate
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        kept = kernels.Quantized8(*ctx.saved_tensors)
+        return _last(lambda g: kernels.gelu_8bit_backward(g, kept, ctx.approximate), 'gelu_8bit', g), None
+
+
+def gelu_8bit(input, approximate='none'):
+    """torch.nn.functional.gelu whose backward pass reads the input from 8 bits (kernels.quantize_8bit): the result is that of the input
+    itself, its gradient that of the kept values.  Differentiable once."""
+    if not (input.requires_grad and torch.is_grad_enabled()):
+        return F.gelu(input, approximate=approximate)
+    return _GELU8bit.apply(input, approximate)
+
+
+class _Linear8bit(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        kept = kernels.quantize_8bit(x) if ctx.needs_input_grad[1] else (None, None)
+        ctx.save_for_backward(weight, *kept)
+        return F.linear(x, weight, bias)
+
+    @staticmethod
+    def backward(ctx, g):
+        weight, codes, exponents = ctx.saved_tensors
+        need_x, need_weight, need_bias = (_wanted(ctx, i) for i in range(3))
+
+        def gradients(g):
+            dx = torch.matmul(g, weight) if need_x else None
+            if need_weight:
+                dw, db = kernels.weight_grad_8bit(g, kernels.Quantized8(codes, exponents), True, need_bias, weight.dtype)
+            else:
+                dw, db = None, g.reshape(-1, g.shape[-1]).sum(0) if need_bias else None
+            return dx, dw, db
+        return _last(gradients, 'linear_8bit', g, weight)
+
+
+def linear_8bit(input, weight, bias=None):
+    """torch.nn.functional.linear whose backward pass reads the input from 8 bits (kernels.quantize_8bit): the result and the gradient of the
+    input are those of torch's, the gradient of the weight is that of the kept values.  float32, bfloat16 or float16, autocast as there.
+    Differentiable once."""
+    input, weight, bias = _autocast(input, weight, bias)
+    return _Linear8bit.apply(input, weight, bias)
+
+
+class GELU8bit(nn.GELU):
+    """torch.nn.GELU on gelu_8bit() above."""
+
+    def forward(self, input):
+        return gelu_8bit(input, self.approximate)
+
+
+class Linear8bit(nn.Linear):
+    """torch.nn.Linear (the same arguments, parameters and state dict) on linear_8bit() above.  The Kronecker factors that a gradient maker takes of
+    it are those of the input itself."""
+
+    def forward(self, input):
+        return linear_8bit(input, self.weight, self.bias)
+
+
+def keep_activations_8bit(model: nn.Module) -> int:
+    """Makes every torch.nn.Linear and torch.nn.GELU of ``model`` (not subclasses of them) a Linear8bit and a GELU8bit, in place: they keep their
+    inputs for the backward pass in a byte a value, and one for 128 of them.  Returns how many there were.  The model then runs on a ROCm
+    device only, in float32, bfloat16 or float16."""
+    return _stand_in(model, {nn.Linear: Linear8bit, nn.GELU: GELU8bit})
