@@ -74,6 +74,11 @@ def parse():
                          'and the brief runs of the linear4096, resnet18_cifar and shampoo_gpt2 workloads (the `secondary` object)')
     ap.add_argument('--fused-layer-norm', action='store_true',
                     help='shampoo_gpt2: the layer norms of the model on this framework\'s kernels (asdl_amd.fuse_layer_norms)')
+    ap.add_argument('--fused-ends', action='store_true',
+                    help='shampoo_gpt2: the loss from the input of the head, without the logits, and the embeddings on this framework\'s '
+                         'kernels (asdl_amd.linear_cross_entropy, asdl_amd.fuse_embeddings)')
+    ap.add_argument('--activations-8bit', action='store_true',
+                    help='shampoo_gpt2: linear layers and GELUs keep their inputs in 8 bits (asdl_amd.keep_activations_8bit)')
     ap.add_argument('--no-inverse-roofline', action='store_true',
                     help='skip the stand-alone timing of the damped inverses (the `roofline_inverse` object)')
     ap.add_argument('--factor-launches', choices=['default', 'single', 'grouped'], default='default',
@@ -585,13 +590,22 @@ def main_shampoo(args, dev, steps=None, warmup=None, emit=True):
     returned instead of printed."""
     import torch
     import torch.nn.functional as F
+    import asdl_amd
     import bench_models
     from asdl_amd import PreconditioningConfig, ShampooGradientMaker
     torch.backends.cudnn.benchmark = False
     model = bench_models.gpt2_small().to(dev)       # token embedding and output head frozen (50257-wide)
+    options = []
     if getattr(args, 'fused_layer_norm', False):
-        import asdl_amd
         asdl_amd.fuse_layer_norms(model)
+        options.append('layer norms on the framework\'s kernels')
+    ends = getattr(args, 'fused_ends', False)
+    if ends:
+        asdl_amd.fuse_embeddings(model)
+        options.append('loss without logits and embeddings on the framework\'s kernels')
+    if getattr(args, 'activations_8bit', False):
+        asdl_amd.keep_activations_8bit(model)
+        options.append('inputs of linear layers and GELUs kept in 8 bits')
     bs = 8
     x = torch.randint(0, 50257, (bs, 1024)).to(dev)
     t = torch.randint(0, 50257, (bs * 1024,)).to(dev)
@@ -618,10 +632,18 @@ def main_shampoo(args, dev, steps=None, warmup=None, emit=True):
     def token_loss(y, target):
         return F.cross_entropy(y.reshape(-1, y.shape[-1]), target)
 
+    def features(inp):
+        with torch.autocast('cuda', dtype=torch.bfloat16):
+            return model.features(inp)
+
+    def head_loss(h, target):
+        with torch.autocast('cuda', dtype=torch.bfloat16):
+            return asdl_amd.linear_cross_entropy(h.flatten(0, 1), model.lm_head.weight, target)
+
     def step():
         opt.zero_grad(set_to_none=True)
-        dummy_y = gm.setup_model_call(fwd, x)
-        gm.setup_loss_call(token_loss, dummy_y, t)
+        dummy_y = gm.setup_model_call(features if ends else fwd, x)
+        gm.setup_loss_call(head_loss if ends else token_loss, dummy_y, t)
         gm.forward_and_backward()
         opt.step()
 
@@ -645,7 +667,7 @@ def main_shampoo(args, dev, steps=None, warmup=None, emit=True):
                                'every step, inverse 4th roots every 10 steps, epsilon 1e-6) on a 12-layer '
                                'GPT-2-small-shaped decoder (d 768, 12 heads, MLP 3072; token embedding and output '
                                'head frozen), 8 x 1024 uniform random tokens, bf16 autocast forward/backward, '
-                               'fp32 statistics and roots', 'batch': bs}}
+                               'fp32 statistics and roots' + ''.join(f', {o}' for o in options), 'batch': bs}}
     if root_records:
         from asdl_amd import _lib
 

@@ -140,6 +140,7 @@ class GPT2Block(nn.Module):
         self.c_proj = nn.Linear(d, d)
         self.ln_2 = nn.LayerNorm(d)
         self.c_fc = nn.Linear(d, 4 * d)
+        self.act = nn.GELU()
         self.c_proj2 = nn.Linear(4 * d, d)
 
     def forward(self, x):
@@ -148,7 +149,7 @@ class GPT2Block(nn.Module):
         q, k, v = (z.view(b, t, self.n_head, d // self.n_head).transpose(1, 2) for z in (q, k, v))
         y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         x = x + self.c_proj(y.transpose(1, 2).reshape(b, t, d))
-        return x + self.c_proj2(F.gelu(self.c_fc(self.ln_2(x))))
+        return x + self.c_proj2(self.act(self.c_fc(self.ln_2(x))))
 
 
 class GPT2Small(nn.Module):
@@ -166,12 +167,16 @@ class GPT2Small(nn.Module):
         self.wte.weight.requires_grad_(False)
         self.lm_head.weight.requires_grad_(False)
 
-    def forward(self, idx):
+    def features(self, idx):
+        """What the head takes."""
         t = idx.shape[1]
         x = self.wte(idx) + self.wpe(torch.arange(t, device=idx.device))
         for blk in self.h:
             x = blk(x)
-        return self.lm_head(self.ln_f(x))
+        return self.ln_f(x)
+
+    def forward(self, idx):
+        return self.lm_head(self.features(idx))
 
 
 def gpt2_small(**kw):
