@@ -7,14 +7,13 @@ namespace ak {
 
 constexpr int kColumnsPerGroup = 256, kColumnChunks = 64;
 
-// A thread has eight columns and every eighth row of its chunk; grid (columns / 256, chunks).
+// A work group's chunk of 256 columns: a thread has eight columns and every eighth row of it.
 template <typename T>
-static __global__ __launch_bounds__(256) void column_chunks_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
-                                                                   int64_t rows_per_chunk, float* __restrict__ part) {
-  __shared__ float joined[8][kColumnsPerGroup];
+__device__ __forceinline__ void column_chunk(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols, int64_t rows_per_chunk,
+                                             float* __restrict__ part, int64_t group, int64_t chunk, float (*joined)[kColumnsPerGroup]) {
   const int lane = threadIdx.x & 31, row_of = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kColumnsPerGroup + 8 * lane;
-  const int64_t r0 = blockIdx.y * rows_per_chunk, r1 = r0 + rows_per_chunk < rows ? r0 + rows_per_chunk : rows;
+  const int64_t c = group * kColumnsPerGroup + 8 * lane;
+  const int64_t r0 = chunk * rows_per_chunk, r1 = r0 + rows_per_chunk < rows ? r0 + rows_per_chunk : rows;
   float s[8] = {};
   if (c + 8 <= cols) {
 #pragma unroll 4
@@ -33,23 +32,37 @@ static __global__ __launch_bounds__(256) void column_chunks_kernel(const T* __re
 #pragma unroll
   for (int e = 0; e < 8; ++e) joined[row_of][8 * lane + e] = s[e];
   __syncthreads();
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kColumnsPerGroup + threadIdx.x;
+  const int64_t col = group * kColumnsPerGroup + threadIdx.x;
   if (col >= cols) return;
   float t = joined[0][threadIdx.x];
 #pragma unroll
   for (int k = 1; k < 8; ++k) t += joined[k][threadIdx.x];
-  part[blockIdx.y * cols + col] = t;
+  part[chunk * cols + col] = t;
+}
+
+// grid (columns / 256, chunks)
+template <typename T>
+static __global__ __launch_bounds__(256) void column_chunks_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                                   int64_t rows_per_chunk, float* __restrict__ part) {
+  __shared__ float joined[8][kColumnsPerGroup];
+  column_chunk(x, ld, rows, cols, rows_per_chunk, part, blockIdx.x, blockIdx.y, joined);
 }
 
 template <typename T>
-static __global__ __launch_bounds__(256) void column_total_kernel(const float* __restrict__ part, int64_t cols, int chunks, float scale,
-                                                                  const float* __restrict__ factor, T* __restrict__ out) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+__device__ __forceinline__ void column_total(const float* __restrict__ part, int64_t cols, int chunks, float scale, const float* __restrict__ factor,
+                                             T* __restrict__ out, int64_t group) {
+  const int64_t c = group * 256 + threadIdx.x;
   if (c >= cols) return;
   float t = 0.f;
 #pragma unroll 8
   for (int k = 0; k < chunks; ++k) t += part[k * cols + c];
   out[c] = static_cast<T>(t * (factor != nullptr ? scale * *factor : scale));
+}
+
+template <typename T>
+static __global__ __launch_bounds__(256) void column_total_kernel(const float* __restrict__ part, int64_t cols, int chunks, float scale,
+                                                                  const float* __restrict__ factor, T* __restrict__ out) {
+  column_total(part, cols, chunks, scale, factor, out, blockIdx.x);
 }
 
 inline int column_chunks(int64_t rows) {

@@ -4,7 +4,7 @@
 // groups run (atomics on the 3 KB rows of a frequent token would also wait for each other: a twentieth of a text is its commonest token).
 //   sort:   a work group per range of rows reads all tokens, counts those in front of its range and those of each row, and puts the
 //           positions of its own in order: a stable counting sort without a word between work groups, one launch.  Of more tokens than
-//           kEmbScan that costs more than two further launches, which bring the tokens into ranges first (131072 tokens: SORT_US)
+//           kEmbScan that costs more than two further launches, which bring the tokens into ranges first (131072 tokens: 116 -> 36 us)
 //   sums:   a wave per chunk of sorted positions and 1 KB of columns; runs of equal tokens inside a chunk are written, parts of runs that
 //           cross its ends go to the workspace; other waves write the rows that no token names
 //   joins:  the parts of a run, in order

@@ -13,6 +13,7 @@
 // contraction is too large for them; what lies outside the matrix reads as zero: rows beyond it by the number of records or an offset
 // beyond it, the last k by a comparison.
 #pragma once
+#include <algorithm>
 #include <atomic>
 #include "elements.hpp"
 #include "syrk_dtl_tile.hpp"
@@ -58,8 +59,9 @@ struct HpCfg {
   static constexpr bool A_BY_K = A_BY_K_, B_BY_K = B_BY_K_, PIECES = PIECES_;
   static constexpr int BI = 32 * FR * WR, BJ = 32 * FC * WC, BK = 32;
   static constexpr int BLOCK = 2048, PANEL_A = BI * 64, PANEL_B = BJ * 64, STAGE = PANEL_A + PANEL_B, LDS_BYTES = STAGES * STAGE;
+  static constexpr int LDS_ALL = LDS_BYTES > BJ * (BI * 2 + 16) ? LDS_BYTES : BJ * (BI * 2 + 16);        // or a tile of 16-bit rows
   static constexpr int IA = BI / 16 / NW, IB = BJ / 16 / NW, LPT = IA + IB;      // wave-wide loads of a k-tile, per wave
-  static_assert(BI / 16 % NW == 0 && BJ / 16 % NW == 0 && LDS_BYTES <= 160 * 1024, "loads split evenly, panels fit the LDS");
+  static_assert(BI / 16 % NW == 0 && BJ / 16 % NW == 0 && LDS_ALL <= 160 * 1024, "loads split evenly, panels fit the LDS");
 };
 
 // What one wave loads of an operand: N wave-wide loads a k-tile.
@@ -151,9 +153,10 @@ __device__ __forceinline__ void hp_place(int id, int tiles_i, int tiles_j, int& 
   tj = rest / height;
 }
 
-// One tile of D.  The loop alone sustains 1.3 PFLOP/s (512 k-tiles of 256 x 256, both operands by row), where the device is at its power
-// limit (1.9 GHz).  A work group that goes on to another tile, with its loads running on into that one under the epilogue, was not
-// faster: 649 -> 626 us for the 6304 tiles of 24 k-tiles of a 50257-class forward pass, but 1982 -> 2068 us for 8000 of 64.
+// One tile of D.  The loop alone sustains 1.3 PFLOP/s (512 k-tiles of 256 x 256, both operands by row, bf16), where the device is at its
+// power limit (1.9 GHz, the matrix cores busy for 66 % of the cycles; fp16 operands 1.5 GHz and 71 %).  A work group that goes on to another
+// tile, with its loads running on into that one under the epilogue, was not faster: 649 -> 626 us for the 6304 tiles of 24 k-tiles of
+// a 50257-class forward pass, but 1982 -> 2068 us for 8000 of 64.
 template <class Cfg, typename E, class Epilogue>
 __device__ __forceinline__ void hp_run(const HpProblem& p, const typename Epilogue::Params& e, uint32_t block, uint32_t blocks) {
   constexpr int FR = Cfg::FR, FC = Cfg::FC, S = Cfg::STAGES, LPT = Cfg::LPT;
@@ -204,67 +207,105 @@ __device__ __forceinline__ void hp_run(const HpProblem& p, const typename Epilog
     else fb[u - 1] = hp_read<Cfg::B_BY_K>(pb + s + (u - 1) * Cfg::BLOCK + fb_off[kk]);
   };
   floatx16 acc[FR][FC];
-  // The matrix instructions of 16 k, with the reads of the next 16 and (LOADS) the loads of a k-tile further ahead spread between them.
-  auto half_step = [&](auto loads_tag, const short8v (&ca)[FR], const short8v (&cb)[FC], short8v (&na)[FR], short8v (&nb)[FC], int stage,
-                       int kk, int to) {
-    constexpr int NLOAD = decltype(loads_tag)::value, NM = FR * FC, NS = NLOAD + FR + FC;
-#pragma unroll
-    for (int m = 0; m < NM; ++m) {
-      const int a = m / FC, b = m % FC;
-      acc[a][b] = hp_mfma<E>(ca[a], cb[b], acc[a][b]);
-#pragma unroll
-      for (int s = (m * NS) / NM; s < ((m + 1) * NS) / NM; ++s) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (s < NLOAD) load_one(s, to);
-        else read_unit(na, nb, stage, kk, s - NLOAD);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-
 #pragma unroll
   for (int a = 0; a < FR; ++a)
 #pragma unroll
     for (int b = 0; b < FC; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+  const int steps = Cfg::PIECES ? nk * p.pieces.count : nk;
 #pragma unroll
   for (int t = 0; t < S - 1; ++t) {              // k-tiles behind the last load zeros: the counts stay uniform
 #pragma unroll
     for (int l = 0; l < LPT; ++l) load_one(l, t);
     load_next();
   }
-  wait_vmcnt<(S - 2) * LPT>();                   // this wave's loads of the first k-tile have landed
-  __syncthreads();                               // ... and everybody's
-  short8v fa0[FR], fb0[FC], fa1[FR], fb1[FC];
+  if constexpr (Cfg::NW == 8) {
+    // Two groups of four waves, one wave of each on every SIMD, take turns: while one reads the LDS and asks for a k-tile further
+    // ahead, the other has the matrix cores, and a barrier changes their parts.  A wave's fragments of a k-tile have arrived before
+    // its turn, its loads of the next one before the barrier in front of it.  (With reads and loads spread between the matrix instructions
+    // of the same wave, as below: 8192 x 768 x 50257 bf16 622 -> 616 us, 4096 x 2048 x 128000 fp16 2010 -> 1934 us.)
+    const bool second = wave >= 4;
+    wait_vmcnt<(S - 2) * LPT>();                 // this wave's loads of the first k-tile have landed
+    __syncthreads();                             // ... and everybody's
+    if (second) asm volatile("s_barrier" ::: "memory");
+    int rd = 0, to = S - 1;
+    for (int kt = 0; kt < steps; ++kt) {
+      short8v fa[2][FR], fb[2][FC];
 #pragma unroll
-  for (int u = 0; u < FR + FC; ++u) read_unit(fa0, fb0, 0, 0, u);
-  int rd = 0, to = S - 1;
-  const int steps = Cfg::PIECES ? nk * p.pieces.count : nk;
-  for (int kt = 0; kt < steps; ++kt) {
-    half_step(std::integral_constant<int, 0>{}, fa0, fb0, fa1, fb1, rd, 1, 0);
-    wait_vmcnt<(S - 3) * LPT>();                 // own loads of the next k-tile have landed
-    __syncthreads();                             // everybody's have; nobody reads the k-tile before this one any more
-    rd = (rd + 1 == S) ? 0 : rd + 1;
-    half_step(std::integral_constant<int, LPT>{}, fa1, fb1, fa0, fb0, rd, 0, to);
-    load_next();
-    to = (to + 1 == S) ? 0 : to + 1;
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int u = 0; u < FR + FC; ++u) read_unit(fa[kk], fb[kk], rd, kk, u);
+#pragma unroll
+      for (int l = 0; l < LPT; ++l) load_one(l, to);
+      load_next();
+      rd = (rd + 1 == S) ? 0 : rd + 1;
+      to = (to + 1 == S) ? 0 : to + 1;
+      // own loads of the next k-tile have landed, own fragments have arrived
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * LPT) : "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int a = 0; a < FR; ++a)
+#pragma unroll
+          for (int b = 0; b < FC; ++b) acc[a][b] = hp_mfma<E>(fa[kk][a], fb[kk][b], acc[a][b]);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_barrier" ::: "memory");
+    }
+    if (!second) asm volatile("s_barrier" ::: "memory");
+  } else {
+    // Four waves, two work groups a CU.  The matrix instructions of 16 k, with the reads of the next 16 and (NLOAD) the loads of a k-tile
+    // further ahead spread between them.
+    auto half_step = [&](auto loads_tag, const short8v (&ca)[FR], const short8v (&cb)[FC], short8v (&na)[FR], short8v (&nb)[FC], int stage,
+                         int kk, int to) {
+      constexpr int NLOAD = decltype(loads_tag)::value, NM = FR * FC, NS = NLOAD + FR + FC;
+#pragma unroll
+      for (int m = 0; m < NM; ++m) {
+        const int a = m / FC, b = m % FC;
+        acc[a][b] = hp_mfma<E>(ca[a], cb[b], acc[a][b]);
+#pragma unroll
+        for (int s = (m * NS) / NM; s < ((m + 1) * NS) / NM; ++s) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (s < NLOAD) load_one(s, to);
+          else read_unit(na, nb, stage, kk, s - NLOAD);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+
+    wait_vmcnt<(S - 2) * LPT>();                   // this wave's loads of the first k-tile have landed
+    __syncthreads();                               // ... and everybody's
+    short8v fa0[FR], fb0[FC], fa1[FR], fb1[FC];
+#pragma unroll
+    for (int u = 0; u < FR + FC; ++u) read_unit(fa0, fb0, 0, 0, u);
+    int rd = 0, to = S - 1;
+    for (int kt = 0; kt < steps; ++kt) {
+      half_step(std::integral_constant<int, 0>{}, fa0, fb0, fa1, fb1, rd, 1, 0);
+      wait_vmcnt<(S - 3) * LPT>();                 // own loads of the next k-tile have landed
+      __syncthreads();                             // everybody's have; nobody reads the k-tile before this one any more
+      rd = (rd + 1 == S) ? 0 : rd + 1;
+      half_step(std::integral_constant<int, LPT>{}, fa1, fb1, fa0, fb0, rd, 0, to);
+      load_next();
+      to = (to + 1 == S) ? 0 : to + 1;
+    }
   }
   wait_vmcnt<0>();                               // the loads of zeros have landed before the LDS is used again
   Epilogue::template run<Cfg>(e, acc, ti, tj, split, wr, wc, lds);
 }
 
 template <class Cfg, typename E, class Epilogue>
-static __global__ __launch_bounds__(Cfg::THREADS, Cfg::FR * Cfg::FC > 8 ? 1 : 2) void hp_kernel(HpProblem p, typename Epilogue::Params e) {
+static __global__ __launch_bounds__(Cfg::THREADS, 2) void hp_kernel(HpProblem p, typename Epilogue::Params e) {
   hp_run<Cfg, E, Epilogue>(p, e, blockIdx.x, gridDim.x);
 }
 
 // Two products in one launch, the first work groups to the first: what one leaves of the device the other fills.
 template <class Cfg1, class Epilogue1, class Cfg2, class Epilogue2, typename E>
-static __global__ __launch_bounds__(Cfg1::THREADS, Cfg1::FR * Cfg1::FC > 8 ? 1 : 2) void hp_both_kernel(HpProblem p1, typename Epilogue1::Params e1, uint32_t blocks1,
-                                                                                                       HpProblem p2, typename Epilogue2::Params e2, uint32_t blocks2,
-                                                                                                       int second_first) {
-  static_assert(Cfg1::THREADS == Cfg2::THREADS && Cfg1::LDS_BYTES == Cfg2::LDS_BYTES, "one launch");
+static __global__ __launch_bounds__(Cfg1::THREADS, 2) void hp_both_kernel(HpProblem p1, typename Epilogue1::Params e1, uint32_t blocks1, HpProblem p2,
+                                                                            typename Epilogue2::Params e2, uint32_t blocks2, int second_first) {
+  static_assert(Cfg1::THREADS == Cfg2::THREADS && Cfg1::LDS_ALL == Cfg2::LDS_ALL, "one launch");
   const uint32_t front = second_first ? blocks2 : blocks1;
   const bool in_front = blockIdx.x < front;
   const uint32_t block = in_front ? blockIdx.x : blockIdx.x - front;
@@ -325,6 +366,26 @@ __device__ __forceinline__ void hp_store8(T* __restrict__ row, int i, int end, u
   }
 }
 
+// out[j][i] = make(block a, b, register x) for a tile, as 16-bit elements, j < J, i < I, through the LDS: a wave writes whole rows of
+// the tile, 512 bytes each, where stores straight from the accumulators are 32 bytes of 32 rows and keep the loads behind them waiting (the
+// piece of d of 4096 x 64000 fp16, beside the forward pass's tiles of the same products, which write nothing: 1.20 times their time,
+// 1.10 through the LDS).  Rows in the LDS are 16 bytes longer than in the tile, so that the banks of 16 rows differ.
+template <class Cfg, typename T, typename Make>
+__device__ __forceinline__ void hp_store_rows(AK_LDS unsigned char* lds, int ti, int tj, int wr, int wc, Make&& make, T* __restrict__ out, int64_t ldo, int I, int J) {
+  constexpr int PITCH = Cfg::BI * 2 + 16, LANES = Cfg::BI / 8, ROWS = Cfg::THREADS / LANES;
+  static_assert(Cfg::BJ * PITCH <= Cfg::LDS_ALL, "the tile fits the LDS");
+  __syncthreads();                               // the panels have been read
+  hp_eights<Cfg, T>(0, 0, wr, wc, make, [&](int i, int j, u32x4 v) { *reinterpret_cast<AK_LDS u32x4*>(lds + j * PITCH + 2 * i) = v; });
+  __syncthreads();
+  const int i = ti * Cfg::BI + 8 * (static_cast<int>(threadIdx.x) % LANES), row = static_cast<int>(threadIdx.x) / LANES;
+  if (i >= I) return;
+  const int rows = min(Cfg::BJ, J - tj * Cfg::BJ);
+  T* __restrict__ to = out + static_cast<int64_t>(tj) * Cfg::BJ * ldo;
+  AK_LDS const unsigned char* from = lds + 16 * (static_cast<int>(threadIdx.x) % LANES);
+#pragma unroll 4
+  for (int r = row; r < rows; r += ROWS) hp_store8(to + r * ldo, i, I, *reinterpret_cast<AK_LDS const u32x4*>(from + r * PITCH));
+}
+
 // out[j][i] = scale * D[i][j] as T
 template <typename T>
 struct HpStore {
@@ -383,11 +444,11 @@ struct HpSum {
 
 // dst[row][c] = T(scale * factor * sum over the splits of sum[split][row][c])
 template <typename T>
-static __global__ __launch_bounds__(256) void hp_total_kernel(const float* __restrict__ sum, int64_t ld, int64_t stride, int splits, int64_t rows,
-                                                              int cols, float scale, const float* __restrict__ factor, T* __restrict__ dst) {
+__device__ __forceinline__ void hp_total_part(const float* __restrict__ sum, int64_t ld, int64_t stride, int splits, int64_t rows, int cols, float scale,
+                                              const float* __restrict__ factor, T* __restrict__ dst, int64_t group, int64_t groups) {
   const int64_t n = rows * ld;
   const float u = factor != nullptr ? scale * *factor : scale;
-  for (int64_t i = 4 * (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x); i < n; i += 4 * static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t i = 4 * (group * 256 + threadIdx.x); i < n; i += 4 * groups * 256) {
     const int64_t row = i / ld;
     const int c = static_cast<int>(i - row * ld);
     floatx4 t = *reinterpret_cast<const floatx4*>(sum + i);
@@ -399,11 +460,17 @@ static __global__ __launch_bounds__(256) void hp_total_kernel(const float* __res
 }
 
 template <typename T>
+static __global__ __launch_bounds__(256) void hp_total_kernel(const float* __restrict__ sum, int64_t ld, int64_t stride, int splits, int64_t rows,
+                                                              int cols, float scale, const float* __restrict__ factor, T* __restrict__ dst) {
+  hp_total_part(sum, ld, stride, splits, rows, cols, scale, factor, dst, blockIdx.x, gridDim.x);
+}
+
+inline unsigned hp_total_groups(int64_t rows, int64_t ld) { return static_cast<unsigned>(std::min<int64_t>((rows * ld + 1023) / 1024, 8192)); }
+
+template <typename T>
 inline int hp_total(const float* sum, int64_t ld, int64_t stride, int splits, int64_t rows, int cols, float scale, const float* factor, T* dst,
                     hipStream_t stream) {
-  const int64_t groups = (rows * ld + 1023) / 1024;
-  hipLaunchKernelGGL(hp_total_kernel<T>, dim3(static_cast<unsigned>(groups < 8192 ? groups : 8192)), dim3(256), 0, stream, sum, ld, stride, splits, rows,
-                     cols, scale, factor, dst);
+  hipLaunchKernelGGL(hp_total_kernel<T>, dim3(hp_total_groups(rows, ld)), dim3(256), 0, stream, sum, ld, stride, splits, rows, cols, scale, factor, dst);
   return check_launch();
 }
 
@@ -532,10 +599,6 @@ struct Carver {
 
 template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
 using HpWide = HpCfg<2, 4, 4, 2, A_BY_K, B_BY_K, 4, PIECES>;      // 256 x 256
-// 256 x 256 by four waves of 128 x 128, one a SIMD, for long contractions: a third less of the LDS is read for a product (the product of
-// 4096 x 4096 x 16384 424 -> 410 us at the power limit); an epilogue that needs registers does not fit beside the sums.
-template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
-using HpLong = HpCfg<2, 2, 4, 4, A_BY_K, B_BY_K, 4, PIECES>;
 template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
 using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K, 4, PIECES>;     // 128 x 128
 
@@ -564,9 +627,9 @@ inline int hp_launch(const HpProblem& p, const typename Epilogue::Params& e, hip
   if (blocks > 0x7fffffff) return AK_ERR_TOO_LARGE;
   auto kernel = hp_kernel<Cfg, E, Epilogue>;
   static std::atomic<uint64_t> known{0};
-  const int rc = hp_ask_lds(kernel, Cfg::LDS_BYTES, known);
+  const int rc = hp_ask_lds(kernel, Cfg::LDS_ALL, known);
   if (rc != AK_OK) return rc;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(Cfg::THREADS), Cfg::LDS_BYTES, stream, p, e);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(Cfg::THREADS), Cfg::LDS_ALL, stream, p, e);
   return check_launch();
 }
 
@@ -578,9 +641,9 @@ inline int hp_launch_both(const HpProblem& p1, const typename Epilogue1::Params&
   if (b1 + b2 > 0x7fffffff) return AK_ERR_TOO_LARGE;
   auto kernel = hp_both_kernel<Cfg1, Epilogue1, Cfg2, Epilogue2, E>;
   static std::atomic<uint64_t> known{0};
-  const int rc = hp_ask_lds(kernel, Cfg1::LDS_BYTES, known);
+  const int rc = hp_ask_lds(kernel, Cfg1::LDS_ALL, known);
   if (rc != AK_OK) return rc;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(b1 + b2)), dim3(Cfg1::THREADS), Cfg1::LDS_BYTES, stream, p1, e1, static_cast<uint32_t>(b1), p2, e2,
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(b1 + b2)), dim3(Cfg1::THREADS), Cfg1::LDS_ALL, stream, p1, e1, static_cast<uint32_t>(b1), p2, e2,
                      static_cast<uint32_t>(b2), p2.k_per_split > p1.k_per_split ? 1 : 0);
   return check_launch();
 }

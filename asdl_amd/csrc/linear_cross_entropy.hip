@@ -89,7 +89,7 @@ struct LceStats {
   static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc,
                                              AK_LDS unsigned char* lds) {
     AK_LDS floatx2* joined = reinterpret_cast<AK_LDS floatx2*>(lds);       // [WR][BJ]
-        const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+    const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
     const int i0 = ti * Cfg::BI + 32 * Cfg::FR * wr + 4 * g;
     __syncthreads();                           // everybody has read the last panels
     lce_scores<Cfg>(e.r, acc, ti * Cfg::BI, 0, wr);
@@ -147,7 +147,7 @@ struct LceGrad {
   };
   template <class Cfg>
   static __device__ __forceinline__ void run(const Params& e, floatx16 (&acc)[Cfg::FR][Cfg::FC], int ti, int tj, int, int wr, int wc,
-                                             AK_LDS unsigned char*) {
+                                             AK_LDS unsigned char* lds) {
     lce_scores<Cfg>(e.r, acc, ti * Cfg::BI, e.c0, wr);
     const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
     const int i0 = ti * Cfg::BI + 32 * Cfg::FR * wr + 4 * g, j0 = tj * Cfg::BJ + 32 * Cfg::FC * wc + l32;
@@ -174,22 +174,25 @@ struct LceGrad {
             if (at == 32 * a + 8 * (x >> 2) + (x & 3)) acc[a][b][x] -= share;
       }
     }
+    if constexpr (LceKind<E>::pieces == 1) {
+      hp_store_rows<Cfg>(lds, ti, tj, wr, wc, [&](int a, int b, int x) { return acc[a][b][x]; }, e.d, e.ldd, e.width, e.r.rows);
+    } else {
 #pragma unroll
-    for (int k = 0; k < LceKind<E>::pieces; ++k) {
-      hp_eights<Cfg, M>(ti, tj, wr, wc, [&](int a, int b, int x) { return acc[a][b][x]; },
-                        [&](int i, int j, u32x4 v) {
-                          if (j < e.r.rows && i < e.width) __builtin_memcpy(e.d + static_cast<int64_t>(j) * e.ldd + k * e.pitch + i, &v, 16);
-                        });
-      if (k + 1 == LceKind<E>::pieces) break;
+      for (int k = 0; k < LceKind<E>::pieces; ++k) {
+        hp_eights<Cfg, M>(ti, tj, wr, wc, [&](int a, int b, int x) { return acc[a][b][x]; },
+                          [&](int i, int j, u32x4 v) {
+                            if (j < e.r.rows && i < e.width) __builtin_memcpy(e.d + static_cast<int64_t>(j) * e.ldd + k * e.pitch + i, &v, 16);
+                          });
 #pragma unroll
-      for (int a = 0; a < Cfg::FR; ++a)
+        for (int a = 0; a < Cfg::FR; ++a)
 #pragma unroll
-        for (int b = 0; b < Cfg::FC; ++b)
+          for (int b = 0; b < Cfg::FC; ++b)
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const float v = acc[a][b][x];
-            acc[a][b][x] = fabsf(v) < INFINITY ? v - static_cast<float>(static_cast<M>(v)) : 0.f;
-          }
+            for (int x = 0; x < 16; ++x) {
+              const float v = acc[a][b][x];
+              acc[a][b][x] = fabsf(v) < INFINITY ? v - static_cast<float>(static_cast<M>(v)) : 0.f;
+            }
+      }
     }
   }
 };
@@ -599,7 +602,7 @@ inline int lce_backward(LceCall c, const float* lse, const LcePlan& p, const Lce
       return hp_launch_both<W, HpStore<E>, H, HpSum, M>(qw, ew, qh, eh, c.stream);
     };
     if (out.dh != nullptr || out.dw != nullptr)
-      rc = p.wide ? gradients(HpLong<false, false, PIECES>{}, HpLong<false, true, PIECES>{})
+      rc = p.wide ? gradients(HpWide<false, false, PIECES>{}, HpWide<false, true, PIECES>{})
                   : gradients(HpSmall<false, false, PIECES>{}, HpSmall<false, true, PIECES>{});
     if (rc == AK_OK && out.db != nullptr)
       rc = with_type(out.db_dtype, [&](auto t) {

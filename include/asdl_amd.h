@@ -514,7 +514,7 @@ int ak_inv_root_group(int phases, int iters, int groups, float* const* S, const 
  * is what the backward pass needs.  g: gradient of the loss, [rows] or [1]; dh [rows, width], dw [classes, width] (dense rows) of the
  * type of h, db [classes] of the bias's type; each may be null.  Sums and exponentials are fp32; 16-bit operands: the gradient
  * of the logits is rounded to their type.  The workspace (enough for either alignment; backward != 0: for the backward pass) holds a piece
- * of the logits' gradient of at most 256 MB, or 256 classes, and copies of 16-bit operands whose width is no multiple of eight or whose rows
+ * of the logits' gradient of at most 512 MB, or 256 classes, and copies of 16-bit operands whose width is no multiple of eight or whose rows
  * are not 16-byte aligned.  rows, classes <= 2^28, width <= 2^20, row pitches <= 2^21, else AK_ERR_TOO_LARGE. */
 size_t ak_linear_cross_entropy_ws_bytes(int dtype, int64_t rows, int64_t classes, int64_t width, int backward);
 int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype,
