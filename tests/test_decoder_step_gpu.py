@@ -242,9 +242,11 @@ def test_linear_cross_entropy_gives_what_is_asked_for(K, dtype):
     assert all(torch.equal(x, y) for x, y in zip(whole, K.linear_cross_entropy_backward(g, h, w, t, lse, b)))       # the same bits every time
 
 
-@pytest.mark.parametrize('dtype,rows,classes,width', [(BF16, 2100, 70001, 64), (F16, 4200, 33000, 40), (F32, 1030, 66000, 36), (BF16, 9000, 16500, 72)])
+@pytest.mark.parametrize('dtype,rows,classes,width', [(BF16, 2100, 70001, 64), (F16, 4200, 33000, 40), (F32, 1030, 66000, 36), (BF16, 9000, 16500, 72),
+                                                      (BF16, 4200, 70001, 64), (F16, 9000, 33000, 40), (F32, 1030, 90001, 36), (BF16, 1100000, 600, 8)])
 def test_linear_cross_entropy_in_pieces(K, dtype, rows, classes, width):
-    """More than 256 MB of logits of the type: several pieces of the classes, the last one shorter."""
+    """Up to 512 MB of the logits' gradient, as float32 in three pieces of 16 bits, and more: several pieces of the classes, the last one shorter;
+    with very many rows pieces of 256 classes."""
     print(f'linear_cross_entropy {rows}x{classes}x{width} {dtype}', flush=True)
     h, w = rand(rows, width, seed=1, dtype=dtype), rand(classes, width, seed=2, dtype=dtype, scale=0.2)
     t = ints(classes, rows, seed=3)
@@ -403,6 +405,91 @@ def test_embedding_refuses(K):
         with pytest.raises(RuntimeError, match='ROCm device'):
             call()
     assert torch.equal(K.embedding_backward(g, tokens, 10, padding_idx=-1), K.embedding_backward(g, tokens, 10, padding_idx=9))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_embedding_of_many_rows(K, dtype):
+    """More rows than the ranges that many tokens are brought into first."""
+    rows, width = 300001, 8
+    for tokens in (20000, 70001):
+        print(f'embedding {tokens} of {rows}x{width} {dtype}', flush=True)
+        at = ints(rows, tokens, seed=tokens)
+        at[::3] = rows - 1
+        check_embedding(K, at, rand(rows, width, seed=1, dtype=dtype), 1.5, None, rand(tokens, width, seed=2, dtype=dtype))
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+def ends(n, k):
+    """Positions at both ends of n, in order."""
+    return torch.cat([torch.arange(k, device='cuda'), n - k + torch.arange(k, device='cuda')])
+
+
+def test_linear_cross_entropy_of_very_many_rows(K):
+    """h of more than 2^32 bytes: only rows at both ends have a gradient."""
+    rows, width, classes = 2200001, 1000, 70
+    print(f'linear_cross_entropy {rows}x{classes}x{width}', flush=True)
+    h = rand(rows, width, seed=1, dtype=BF16)
+    w, b = rand(classes, width, seed=2, dtype=BF16, scale=0.05), rand(classes, seed=3, dtype=BF16)
+    t, at = ints(classes, rows, seed=4), ends(rows, 300)
+    g = torch.zeros(rows, device='cuda')
+    g[at] = gradient_of('none', t[at], 6)
+    loss, lse = K.linear_cross_entropy(h, w, t, b, reduction='none')
+    dh, dw, db = K.linear_cross_entropy_backward(g, h, w, t, lse, b, reduction='none')
+    want = loss64(h[at], w, t[at], b, reduction='none', g=g[at])
+    for name, got in (('lse', lse[at]), ('loss', loss[at]), ('dh', dh[at]), ('dw', dw), ('db', db)):
+        within(got, *want[name], name)
+    assert bool((dh[300:-300].view(-1) == 0).all())
+
+
+def test_embedding_of_very_large_tables(K):
+    """A table, and gradients, of more than 2^32 elements."""
+    rows, width = 4300001, 1000
+    print(f'embedding of {rows}x{width}', flush=True)
+    table = torch.zeros(rows, width, device='cuda', dtype=BF16)
+    at = ends(rows, 500)
+    table[at] = rand(len(at), width, seed=2, dtype=BF16)
+    tokens = at[ints(len(at), 20000, seed=3)]
+    assert torch.equal(K.embedding(tokens, table), table[tokens])
+    g = rand(20000, width, seed=4, dtype=BF16)
+    got = K.embedding_backward(g, tokens, rows)
+    few = torch.searchsorted(at, tokens)
+    assert torch.equal(got[at], K.embedding_backward(g, few, len(at)))
+    got[at] = 0
+    assert bool((got == 0).all())
+    del got, table
+    print(f'embedding of {rows} tokens', flush=True)
+    small = rand(700, width, seed=5, dtype=BF16)
+    tokens = ints(700, rows, seed=6)
+    assert torch.equal(K.embedding(tokens, small)[-500:], small[tokens[-500:]])
+    g = torch.zeros(rows, width, device='cuda', dtype=BF16)
+    g[at] = rand(len(at), width, seed=7, dtype=BF16)
+    want = torch.zeros(700, width, dtype=torch.float64, device='cuda').index_add_(0, tokens[at], g[at].double())
+    size = torch.zeros(700, width, dtype=torch.float64, device='cuda').index_add_(0, tokens[at], g[at].double().abs())
+    within(K.embedding_backward(g, tokens, 700), want, 20 * U * size + half_step(BF16) * want.abs(), 'gradient')     # (at most 16 of a row's are not zero)
+    assert int(torch.bincount(tokens[at]).max()) <= 16
+
+
+def test_activations_of_very_many_rows_are_kept(K):
+    """Codes of more than 2^32 bytes."""
+    rows, width, out = 4300001, 1000, 24
+    print(f'quantize_8bit {rows}x{width}', flush=True)
+    x = torch.zeros(rows, width, device='cuda', dtype=BF16)
+    at = ends(rows, 500)
+    x[at] = rand(len(at), width, seed=1, dtype=BF16)
+    kept, few = K.quantize_8bit(x), K.quantize_8bit(x[at])
+    assert torch.equal(kept.codes.view(torch.uint8)[at], few.codes.view(torch.uint8)) and torch.equal(kept.exponents[at], few.exponents)
+    assert torch.equal(K.dequantize_8bit(kept, BF16)[at], K.dequantize_8bit(few, BF16))
+    y, also = K.gelu_8bit(x)
+    assert torch.equal(y[at], K.gelu_8bit(x[at])[0]) and torch.equal(also.codes.view(torch.uint8)[at], few.codes.view(torch.uint8))
+    del also
+    assert torch.equal(K.gelu_8bit_backward(y, kept)[at], K.gelu_8bit_backward(y[at], few))
+    del y, x
+    g = torch.zeros(rows, out, device='cuda', dtype=BF16)
+    g[at] = rand(len(at), out, seed=2, dtype=BF16)
+    dw, db = K.weight_grad_8bit(g, kept, dtype=F32)
+    values, gd = K.dequantize_8bit(few).double(), g[at].double()
+    within(dw, gd.t() @ values, 2 * (len(at) + 8) * U * (gd.abs().t() @ values.abs()), 'dw')
+    within(db, gd.sum(0), (len(at) + 8) * U * gd.abs().sum(0), 'db')
 
 
 # ------------------------------------------------------------------------------------------------ activations in 8 bits
