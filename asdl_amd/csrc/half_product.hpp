@@ -452,6 +452,7 @@ __device__ __forceinline__ void hp_total_part(const float* __restrict__ sum, int
     const int64_t row = i / ld;
     const int c = static_cast<int>(i - row * ld);
     floatx4 t = *reinterpret_cast<const floatx4*>(sum + i);
+#pragma unroll 4
     for (int s = 1; s < splits; ++s) t += *reinterpret_cast<const floatx4*>(sum + s * stride + i);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -477,18 +478,30 @@ inline int hp_total(const float* sum, int64_t ld, int64_t stride, int splits, in
 // Rows at a pitch of ldo elements, zeros behind them: what the panels' loads need where an operand has another pitch or alignment.
 template <typename T>
 static __global__ __launch_bounds__(256) void hp_pad_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, T* __restrict__ out, int ldo) {
-  const int64_t n = rows * ldo;
+  // eight columns a thread
+  const int per = ldo / 8;
+  const int64_t n = rows * per;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / ldo;
-    const int c = static_cast<int>(i - row * ldo);
-    out[i] = c < cols ? x[row * ld + c] : static_cast<T>(0.f);
+    const int64_t row = i / per;
+    const int c = static_cast<int>(i - row * per) * 8;
+    const T* __restrict__ from = x + row * ld + c;
+    Some<T, 8> v;
+    v.clear();
+    if (c + 8 <= cols) {
+      v.load(from);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < cols) v.v[e] = from[e];
+    }
+    v.store(out + row * ldo + c);
   }
 }
 
 template <typename T>
 inline int hp_pad(const T* x, int64_t ld, int64_t rows, int64_t cols, T* out, int64_t ldo, hipStream_t stream) {
-  const int64_t groups = (rows * ldo + 1023) / 1024;
-  hipLaunchKernelGGL(hp_pad_kernel<T>, dim3(static_cast<unsigned>(groups < 1 ? 1 : groups < 8192 ? groups : 8192)), dim3(256), 0, stream, x, ld, rows,
+  const int64_t groups = (rows * (ldo / 8) + 255) / 256;
+  hipLaunchKernelGGL(hp_pad_kernel<T>, dim3(static_cast<unsigned>(groups < 1 ? 1 : groups < 16384 ? groups : 16384)), dim3(256), 0, stream, x, ld, rows,
                      static_cast<int>(cols), out, static_cast<int>(ldo));
   return check_launch();
 }

@@ -423,13 +423,16 @@ constexpr int64_t kLcePieceBytes = 512ll << 20;       // of d
 constexpr int kLceFewRows = 64;
 
 // Sizes that both the workspace query and the launches use.
+constexpr int64_t kLceSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+constexpr double kLceSumUs = 6. / 4.5e6;                  // of an element of a split's sum
+
 struct LcePlan {
   int64_t N, V, D;
   int k;                   // 16-bit pieces of a value
   int64_t piece, pieces;   // classes of a piece, a multiple of 256 (the last may have fewer)
   int64_t ldp;             // row pitch of padded operands
   bool wide;               // tiles of 256 in the gradients' products
-  int splits;              // of the contraction over a piece's classes
+  int splits, splits_dw;   // of the contractions over a piece's classes, over the rows
   int64_t ld_sum;          // row pitch of the fp32 sums of dh
 };
 
@@ -443,20 +446,40 @@ inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D) {
   p.pieces = (V + p.piece - 1) / p.piece;
   p.ldp = align_up(D, 8);
   p.ld_sum = align_up(D, 4);
-  // The gradients' products of a piece: tiles of 256 where their work groups fill the device.  The contraction over the classes goes in as
-  // many splits as make its work groups a sixth of a CU's share of the work, so that the last ones to run leave little of the device idle;
-  // every split has sums of its own.
-  const int64_t k = std::min(p.piece, V);
-  for (int64_t tile : {256, 128}) {
-    p.wide = tile == 256;
+  // The gradients' products of a piece, in one launch: the tiles of 256 or 128 and the splits of either contraction that are least in an
+  // estimate of the time: k-tiles of 0.82 us, or of 0.6 us where two small ones share a CU, over as many work groups as run at once, the
+  // longest first; what the last of them wait for; and the sums of the splits, written and read.  (With 8 splits of the classes at most,
+  // none of the rows and tiles of 256 wherever they fill the device: 10 rows of 103083 classes of 302 210 us, with up to 64 34 us;
+  // 2987 x 2680 x 1600 in fp32 487 us, with three splits of the rows 362 us.)
+  const int64_t k = std::min(p.piece, V), k_dw = (N + 31) / 32, k_dh = (align_up(k, 8) + 31) / 32, products = p.k == 1 ? 1 : 6;
+  double least = 1e30;
+  for (const int64_t tile : {256, 128}) {
     const int64_t across = (D + tile - 1) / tile, of_dw = across * ((k + tile - 1) / tile), of_dh = across * ((N + tile - 1) / tile);
-    const int64_t places = p.wide ? 256 : 512, share = (of_dw * ((N + 31) / 32) + of_dh * ((k + 31) / 32)) / places;
-    int64_t s = (k / 32) / std::max<int64_t>(share / 6, 8);
-    s = std::max<int64_t>(1, std::min<int64_t>(s, p.wide ? 8 : 32));
-    const int64_t per = align_up((align_up(k, 8) + s - 1) / s, 32);
-    p.splits = static_cast<int>((align_up(k, 8) + per - 1) / per);
-    if (of_dw + of_dh * p.splits >= places) break;
+    const int64_t places = tile == 256 ? 256 : 512;
+    const double share = static_cast<double>(of_dw * k_dw + of_dh * k_dh) / places;
+    for (const int64_t w : kLceSplits) {
+      if (w > 1 && (k_dw / w < 4 || of_dw * w > 2 * places)) break;
+      for (const int64_t h : kLceSplits) {
+        if (h > 1 && k_dh / h < 4) break;
+        const double of_w = (k_dw + w - 1) / w, of_h = (k_dh + h - 1) / h;
+        const double longest = std::max(of_w, of_h), tiles = std::max(longest, share + longest / 8 + std::min(of_w, of_h) / 2);
+        const double sums = static_cast<double>(h) * N * D + (w > 1 ? static_cast<double>(w) * k * D : 0.);
+        const double us = tiles * products * (tile == 256 ? 0.82 : 0.6) + sums * kLceSumUs + (w > 1 ? 5. : 0.);
+        if (us < least) {
+          least = us;
+          p.wide = tile == 256;
+          p.splits_dw = static_cast<int>(w);
+          p.splits = static_cast<int>(h);
+        }
+      }
+    }
   }
+  auto whole = [](int64_t n, int splits) {           // splits of whole k-tiles
+    const int64_t per = align_up((n + splits - 1) / splits, 32);
+    return static_cast<int>((n + per - 1) / per);
+  };
+  p.splits = whole(align_up(k, 8), p.splits);
+  p.splits_dw = whole(N, p.splits_dw);
   return p;
 }
 
@@ -468,7 +491,7 @@ struct LceSpace {
   // backward
   float *share, *unit;
   unsigned char* d;
-  float *sum, *columns;
+  float *sum, *sum_dw, *columns;
   size_t bytes;
 };
 
@@ -488,6 +511,7 @@ inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_
     s.unit = c.take<float>(1);
     s.d = c.take<unsigned char>(p.N * p.piece * p.k * 2);
     s.sum = c.take<float>(static_cast<int64_t>(p.splits) * p.N * p.ld_sum);
+    if (p.splits_dw > 1) s.sum_dw = c.take<float>(p.splits_dw * std::min(p.piece, p.V) * p.ld_sum);
     s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(p.N, p.k * p.piece) / sizeof(float)));
   }
   s.bytes = c.used;
@@ -593,14 +617,21 @@ inline int lce_backward(LceCall c, const float* lse, const LcePlan& p, const Lce
     auto gradients = [&](auto dw_cfg, auto dh_cfg) {
       using W = decltype(dw_cfg);
       using H = decltype(dh_cfg);
-      HpProblem qw = hp_problem<W>(hp_operand(c.h, c.ldh, p.N, p.D, false), hp_operand(d, ldd, p.N, padded, false), p.D, width, p.N);
+      HpProblem qw = hp_problem<W>(hp_operand(c.h, c.ldh, p.N, p.D, false), hp_operand(d, ldd, p.N, padded, false), p.D, width, p.N, p.splits_dw);
       HpProblem qh = hp_problem<H>(hp_operand(w, c.ldw, width, p.D, false), hp_operand(d, ldd, p.N, padded, true), p.D, p.N, padded, p.splits);
       if (PIECES) qw.pieces = qh.pieces = hp_six(p.ldp, p.piece);
-      typename HpStore<E>::Params ew{static_cast<E*>(out.dw) + c0 * p.D, p.D, static_cast<int>(p.D), static_cast<int>(width), 1.f, s.unit};
-      const HpSum::Params eh{s.sum, p.ld_sum, p.N * p.ld_sum, static_cast<int>(p.D), static_cast<int>(p.N), k == 0};
-      if (out.dh == nullptr) return hp_launch<W, M, HpStore<E>>(qw, ew, c.stream);
+      E* dw = static_cast<E*>(out.dw) + c0 * p.D;
+      const int D = static_cast<int>(p.D), classes = static_cast<int>(width);
+      const HpSum::Params eh{s.sum, p.ld_sum, p.N * p.ld_sum, D, static_cast<int>(p.N), k == 0};
       if (out.dw == nullptr) return hp_launch<H, M, HpSum>(qh, eh, c.stream);
-      return hp_launch_both<W, HpStore<E>, H, HpSum, M>(qw, ew, qh, eh, c.stream);
+      if (p.splits_dw == 1) {
+        const typename HpStore<E>::Params ew{dw, p.D, D, classes, 1.f, s.unit};
+        if (out.dh == nullptr) return hp_launch<W, M, HpStore<E>>(qw, ew, c.stream);
+        return hp_launch_both<W, HpStore<E>, H, HpSum, M>(qw, ew, qh, eh, c.stream);
+      }
+      const HpSum::Params ew{s.sum_dw, p.ld_sum, width * p.ld_sum, D, classes, 1};
+      const int done = out.dh == nullptr ? hp_launch<W, M, HpSum>(qw, ew, c.stream) : hp_launch_both<W, HpSum, H, HpSum, M>(qw, ew, qh, eh, c.stream);
+      return done != AK_OK ? done : hp_total(s.sum_dw, p.ld_sum, width * p.ld_sum, p.splits_dw, width, D, 1.f, s.unit, dw, c.stream);
     };
     if (out.dh != nullptr || out.dw != nullptr)
       rc = p.wide ? gradients(HpWide<false, false, PIECES>{}, HpWide<false, true, PIECES>{})
