@@ -204,9 +204,16 @@ template <typename E>
 struct LceEight {
   E v[8];
   __device__ __forceinline__ void load(const E* p) { __builtin_memcpy(v, p, sizeof(v)); }
-  __device__ __forceinline__ void some(const E* p, int n) {      // n of them, zeros behind
+  // n of them, zeros behind: all eight loaded (the row's end, and the next row's beginning) unless that is behind the matrix
+  __device__ __forceinline__ void some(const E* p, int n, const E* end) {
+    if (n > 0 && end - p >= 8) {
+      load(p);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : static_cast<E>(0.f);
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : static_cast<E>(0.f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : static_cast<E>(0.f);
+    }
   }
 };
 
@@ -238,9 +245,9 @@ __device__ __forceinline__ floatx4 lce_mma(const LceEight<E>& a, const LceEight<
   }
 }
 
-// A few rows: a wave (and work group: the device is filled evenly) takes 16 classes, weights straight to the matrix instruction (16 x 16 x 32).  A lane has 32 consecutive
-// k of every 128 of one class: what the four lanes of a class read at once is a part of each 128-byte line, all of it in four loads.
-// The order of k is the same for both operands.
+// A few rows: a wave (and work group: the device is filled evenly) takes 16 classes, weights straight to the matrix instruction
+// (16 x 16 x 32).  A lane has 32 consecutive k of every 128 of one class: what the four lanes of a class read at once is a part of each
+// 128-byte line, all of it in four loads.  The order of k is the same for both operands.
 template <typename E, int NB>
 static __global__ __launch_bounds__(64) void lce_few_kernel(const E* __restrict__ h, int64_t ldh, const E* __restrict__ w, int64_t ldw, int D,
                                                              LceRows r, floatx2* __restrict__ part, float* __restrict__ at_target) {
@@ -275,14 +282,15 @@ static __global__ __launch_bounds__(64) void lce_few_kernel(const E* __restrict_
       }
   }
   if (whole < D) {
+    const E *w_end = w + static_cast<int64_t>(r.classes - 1) * ldw + D, *h_end = h + static_cast<int64_t>(r.rows - 1) * ldh + D;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int n = D - whole - 32 * quarter - 8 * e;
       LceEight<E> a, x;
-      a.some(wr + whole + 8 * e, n);
+      a.some(wr + whole + 8 * e, n, w_end);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        x.some(hr[b] + whole + 8 * e, n);
+        x.some(hr[b] + whole + 8 * e, n, h_end);
         acc[b] = lce_mma(a, x, acc[b]);
       }
     }
@@ -420,7 +428,10 @@ static __global__ __launch_bounds__(256) void lce_bias_kernel(const T* __restric
 
 // ---- host side
 constexpr int64_t kLcePieceBytes = 512ll << 20;       // of d
-constexpr int kLceFewRows = 64;
+// Rows that lce_few_kernel() takes rather than the tiles; copied: the tiles want copies of the operands first, of another pitch or in pieces.
+// (50257 x 768: bf16 4 rows 21 us, 16 rows 26 us, the tiles of 128 24 us for any number of these, but 103083 x 302 with copies 58 us, 10 rows
+// without 25 us, 120757 x 461 80 us either way for 17 rows; fp32 55 us for up to 16, 87 us for 32 and 135 us for 64 rows, by the tiles 172 us.)
+inline int64_t lce_few_rows(int dtype, bool copied) { return dtype == AK_F32 ? 64 : copied ? 16 : 8; }
 
 // Sizes that both the workspace query and the launches use.
 constexpr int64_t kLceSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
@@ -429,6 +440,7 @@ constexpr double kLceSumUs = 6. / 4.5e6;                  // of an element of a 
 struct LcePlan {
   int64_t N, V, D;
   int k;                   // 16-bit pieces of a value
+  bool few;                // the forward pass of few rows
   int64_t piece, pieces;   // classes of a piece, a multiple of 256 (the last may have fewer)
   int64_t ldp;             // row pitch of padded operands
   bool wide;               // tiles of 256 in the gradients' products
@@ -436,16 +448,18 @@ struct LcePlan {
   int64_t ld_sum;          // row pitch of the fp32 sums of dh
 };
 
-inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D) {
-  LcePlan p;
+inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D, bool backward, bool copied) {
+  LcePlan p = {};
   p.N = N; p.V = V; p.D = D;
   p.k = dtype == AK_F32 ? 3 : 1;
+  p.few = !backward && N <= lce_few_rows(dtype, copied);
   const int64_t fit = std::max<int64_t>(kLcePieceBytes / (N * p.k * 2) / 256 * 256, 256);
   p.pieces = (V + fit - 1) / fit;
   p.piece = align_up((V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (V + p.piece - 1) / p.piece;
   p.ldp = align_up(D, 8);
   p.ld_sum = align_up(D, 4);
+  if (!backward) return p;
   // The gradients' products of a piece, in one launch: the tiles of 256 or 128 and the splits of either contraction that are least in an
   // estimate of the time: k-tiles of 0.82 us, or of 0.6 us where two small ones share a CU, over as many work groups as run at once, the
   // longest first; what the last of them wait for; and the sums of the splits, written and read.  (With 8 splits of the classes at most,
@@ -502,7 +516,7 @@ inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_
   if (pad_w) s.w = c.take<unsigned char>(p.V * p.ldp * p.k * 2);
   if (bias) s.bias = c.take<float>(p.V);
   if (!backward) {
-    const int64_t tile = p.N <= kLceFewRows ? 16 : 128;      // the fewest classes of a part
+    const int64_t tile = p.few ? 16 : 128;      // the fewest classes of a part
     s.part = c.take<floatx2>((p.V + tile - 1) / tile * p.N);
     s.at_target = c.take<float>(p.N);
     s.losses = c.take<float>(p.N);
@@ -561,7 +575,7 @@ inline int lce_bias(LceCall& c, const LcePlan& p, const LceSpace& s) {
 
 template <typename E>
 inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
-  if (p.N <= kLceFewRows) {
+  if (p.few) {
     const int64_t groups = (p.V + 15) / 16;
     *parts = static_cast<int>(groups);
     auto go = [&](auto nb) {
@@ -569,9 +583,11 @@ inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, int* part
                          c.ldh, static_cast<const E*>(c.w), c.ldw, static_cast<int>(p.D), c.r, s.part, s.at_target);
       return check_launch();
     };
-    if (p.N <= 16) return go(std::integral_constant<int, 1>{});
-    if (p.N <= 32) return go(std::integral_constant<int, 2>{});
-    return go(std::integral_constant<int, 4>{});
+    if constexpr (__is_same(E, float)) {
+      if (p.N > 32) return go(std::integral_constant<int, 4>{});
+      if (p.N > 16) return go(std::integral_constant<int, 2>{});
+    }
+    return go(std::integral_constant<int, 1>{});
   }
   const int rc = lce_operands<E>(c, p, s);
   if (rc != AK_OK) return rc;
@@ -661,10 +677,12 @@ inline int lce_check(const void* h, int64_t ldh, const void* w, int64_t ldw, con
 
 extern "C" size_t ak_linear_cross_entropy_ws_bytes(int dtype, int64_t rows, int64_t classes, int64_t width, int backward) {
   if (!ak::is_element_type(dtype) || rows <= 0 || classes <= 0 || width <= 0 || rows > (1 << 28) || classes > (1 << 28) || width > (1 << 20)) return 0;
-  const ak::LcePlan p = ak::lce_plan(dtype, rows, classes, width);
   // enough for operands of any alignment
-  const bool pad = backward != 0 || rows > ak::kLceFewRows;
-  return ak::lce_space(p, backward != 0, pad, pad, true, nullptr).bytes;
+  auto bytes = [&](bool copied) {
+    const ak::LcePlan p = ak::lce_plan(dtype, rows, classes, width, backward != 0, copied);
+    return ak::lce_space(p, backward != 0, copied && !p.few, copied && !p.few, true, nullptr).bytes;
+  };
+  return backward != 0 ? bytes(true) : std::max(bytes(false), bytes(true));
 }
 
 extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype,
@@ -675,9 +693,9 @@ extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, co
   if (rc != AK_OK) return rc;
   if (rows == 0) return reduction == kLossNone ? AK_OK : AK_ERR_ARG;
   if (loss == nullptr || lse == nullptr) return AK_ERR_ARG;
-  const LcePlan p = lce_plan(dtype, rows, classes, width);
-  const bool few = rows <= kLceFewRows, split = dtype == AK_F32;
-  const LceSpace s = lce_space(p, false, !few && (split || !hp_aligned(h, ldh, width)), !few && (split || !hp_aligned(w, ldw, width)),
+  const bool copy_h = dtype == AK_F32 || !hp_aligned(h, ldh, width), copy_w = dtype == AK_F32 || !hp_aligned(w, ldw, width);
+  const LcePlan p = lce_plan(dtype, rows, classes, width, false, copy_h || copy_w);
+  const LceSpace s = lce_space(p, false, !p.few && copy_h, !p.few && copy_w,
                                bias != nullptr && bias_dtype != AK_F32, ws);
   if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -688,7 +706,7 @@ extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, co
   rc = with_type(dtype, [&](auto t) { return lce_forward<typename decltype(t)::type>(c, p, s, &parts); });
   if (rc != AK_OK) return rc;
   float* losses = reduction == kLossNone ? loss : s.losses;
-  if (few)
+  if (p.few)
     hipLaunchKernelGGL(lce_row_kernel, dim3(static_cast<unsigned>(rows)), dim3(512), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
   else
     hipLaunchKernelGGL(lce_rows_kernel, dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(1024), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
@@ -705,7 +723,7 @@ extern "C" int ak_linear_cross_entropy_backward(const float* g, const void* h, i
   if (rc != AK_OK) return rc;
   if (g == nullptr || lse == nullptr || rows == 0) return AK_ERR_ARG;
   if (dh == nullptr && dw == nullptr && db == nullptr) return AK_OK;
-  const LcePlan p = lce_plan(dtype, rows, classes, width);
+  const LcePlan p = lce_plan(dtype, rows, classes, width, true, true);
   const bool split = dtype == AK_F32;
   const LceSpace s = lce_space(p, true, split || !hp_aligned(h, ldh, width), split || !hp_aligned(w, ldw, width),
                                bias != nullptr && bias_dtype != AK_F32, ws);

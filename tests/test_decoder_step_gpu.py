@@ -229,6 +229,17 @@ def test_linear_cross_entropy_reads_strided_operands_of_any_alignment(K, dtype, 
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('rows', [8, 9, 16, 17, 40, 64])
+def test_linear_cross_entropy_of_few_rows_of_any_alignment(K, rows, dtype):
+    """Either operand where vectors do not begin; rows that end with the tensors' memory."""
+    for off_h, off_w, width in ((0, 0, 64), (1, 0, 64), (0, 1, 64), (3, 1, 151), (0, 0, 151)):
+        h = rand(rows * (width + off_h), seed=1, dtype=dtype).view(rows, -1)[:, off_h:]
+        w = rand(300 * (width + off_w), seed=2, dtype=dtype, scale=0.2).view(300, -1)[:, off_w:]
+        t = ints(300, rows, seed=3)
+        check_loss(K, h, w, t, reduction='sum', g=gradient_of('sum', t, 4))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
 def test_linear_cross_entropy_gives_what_is_asked_for(K, dtype):
     h, w, t, b = rand(90, 64, seed=1, dtype=dtype), rand(500, 64, seed=2, dtype=dtype), ints(500, 90, seed=3), rand(500, seed=4)
     loss, lse = K.linear_cross_entropy(h, w, t, b)
