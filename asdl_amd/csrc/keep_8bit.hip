@@ -280,6 +280,8 @@ inline KeepPlan keep_plan(int dtype, int64_t rows, int64_t F, int64_t out) {
   p.ldf = align_up(F, 8);
   p.ldg = align_up(out, 8);
   p.ld_sum = align_up(F, 4);
+  p.splits = 1;
+  if (F == 0) return p;          // (sums of columns alone)
   const bool wide = hp_wide(F, out);
   const int64_t tile = wide ? 256 : 128, tiles = ((F + tile - 1) / tile) * ((out + tile - 1) / tile);
   const int64_t s = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((wide ? 256 : 512) / tiles, rows / 256), 64));
@@ -294,12 +296,12 @@ struct KeepSpace {
   size_t bytes;
 };
 
-inline KeepSpace keep_space(const KeepPlan& p, int64_t rows, int64_t out, bool copy, bool bias, void* ws) {
+inline KeepSpace keep_space(const KeepPlan& p, int64_t rows, int64_t out, bool weight, bool copy, bool bias, void* ws) {
   Carver c{static_cast<unsigned char*>(ws)};
   KeepSpace s = {};
-  s.x = c.take<__bf16>(rows * p.ldf);
-  if (copy) s.g = c.take<__bf16>(p.pieces * rows * p.ldg);
-  if (p.splits > 1) s.sum = c.take<float>(p.splits * out * p.ld_sum);
+  if (weight) s.x = c.take<__bf16>(rows * p.ldf);
+  if (weight && copy) s.g = c.take<__bf16>(p.pieces * rows * p.ldg);
+  if (weight && p.splits > 1) s.sum = c.take<float>(p.splits * out * p.ld_sum);
   if (bias) s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(rows, out) / sizeof(float)));
   s.bytes = c.used;
   return s;
@@ -358,8 +360,8 @@ extern "C" int ak_dequantize_8bit(const uint8_t* codes, const int8_t* exponents,
 }
 
 extern "C" size_t ak_weight_grad_8bit_ws_bytes(int dtype, int64_t rows, int64_t width, int64_t out) {
-  if (!ak::is_element_type(dtype) || rows <= 0 || width <= 0 || out <= 0 || rows > (1ll << 30) || width > (1 << 20) || out > (1 << 20)) return 0;
-  return ak::keep_space(ak::keep_plan(dtype, rows, width, out), rows, out, true, true, nullptr).bytes;
+  if (!ak::is_element_type(dtype) || rows <= 0 || width < 0 || out <= 0 || rows > (1ll << 30) || width > (1 << 20) || out > (1 << 20)) return 0;
+  return ak::keep_space(ak::keep_plan(dtype, rows, width, out), rows, out, width > 0, true, true, nullptr).bytes;
 }
 
 extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width,
@@ -367,13 +369,13 @@ extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const 
   using namespace ak;
   int rc = keep_check(dtype, ldg, rows, out);
   if (rc != AK_OK) return rc;
-  if (!is_element_type(grad_dtype) || width <= 0 || rows == 0) return AK_ERR_ARG;
+  if (!is_element_type(grad_dtype) || width < 0 || (dw != nullptr && width == 0) || rows == 0) return AK_ERR_ARG;
   if (rows > (1ll << 30) || width > (1 << 20) || out > (1 << 20) || ldg > (1ll << 24)) return AK_ERR_TOO_LARGE;
   if (dw == nullptr && db == nullptr) return AK_OK;
   if (g == nullptr || (dw != nullptr && (codes == nullptr || exponents == nullptr))) return AK_ERR_ARG;
   const KeepPlan plan = keep_plan(dtype, rows, width, out);
   const bool copy = dtype != AK_BF16 || !hp_aligned(g, ldg, out);
-  const KeepSpace s = keep_space(plan, rows, out, copy, db != nullptr, ws);
+  const KeepSpace s = keep_space(plan, rows, out, dw != nullptr, copy, db != nullptr, ws);
   if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int F = static_cast<int>(width), chunks = column_chunks(rows);

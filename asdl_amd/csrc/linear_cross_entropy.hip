@@ -380,7 +380,7 @@ static __global__ __launch_bounds__(1024) void lce_total_kernel(LceRows r, const
   if (threadIdx.x == 0) *loss = static_cast<float>(reduction == kLossMean ? s / static_cast<double>(count) : s);
 }
 
-// share[n] = c_n / most 2^lift, unit = most 2^-lift, with the largest |c_n| for most (plain: 1).
+// share[n] = c_n / most 2^lift, unit = most 2^-lift, with the largest finite |c_n| for most (plain: 1).
 static __global__ __launch_bounds__(1024) void lce_shares_kernel(LceRows r, const float* __restrict__ g, int reduction, int plain, int lift,
                                                                  float* __restrict__ share, float* __restrict__ unit) {
   __shared__ float red[16];
@@ -401,7 +401,7 @@ static __global__ __launch_bounds__(1024) void lce_shares_kernel(LceRows r, cons
     most = fabsf(common);
     if (reduction == kLossNone) {
       most = 0.f;
-      for (int j = threadIdx.x; j < r.rows; j += 1024) most = fmaxf(most, r.targets[j] != r.ignore ? fabsf(g[j]) : 0.f);
+      for (int j = threadIdx.x; j < r.rows; j += 1024) most = fmaxf(most, r.targets[j] != r.ignore && fabsf(g[j]) < INFINITY ? fabsf(g[j]) : 0.f);
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
       __syncthreads();

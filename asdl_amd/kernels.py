@@ -1944,26 +1944,32 @@ def _dequantize(kept, gelu, g, dtype):
 
 def weight_grad_8bit(g, kept, need_weight=True, need_bias=True, dtype=None):
     """(dw, db) of a linear layer whose input was kept with quantize_8bit(): dw = g^T x [out, features] and db = the sums of g [out], for the
-    gradient ``g`` [..., out] of its result (float32, bfloat16 or float16, any row stride); None for what is not needed.  ``dtype``: of both (g's).
-    The products are exact (the kept values and the pieces that g is taken apart into are bfloat16 numbers), their sums fp32."""
+    gradient ``g`` [..., out] of its result (float32, bfloat16 or float16, any row stride); None for what is not needed (without dw,
+    ``kept`` is not read and may be None).  ``dtype``: of both (g's).  The products are exact (the kept values and the pieces that g is taken
+    apart into are bfloat16 numbers), their sums fp32."""
     code = _ELEMENT_TYPES.get(dtype or g.dtype)
-    host = _usual(g) if code is not None else None
+    host = _usual(g) if code is not None and kept is not None else None
     if host is not None:
         done = host.weight_grad_8bit(*kept, g, (1 if need_weight else 0) | (2 if need_bias else 0), code, _raw_stream(g.get_device()))
         if done is not None:
             return done if type(done) is tuple else _lib.check(done, 'ak_weight_grad_8bit')
-    rows, F = _check_kept(kept)
+    if kept is None and need_weight:
+        raise ValueError('dw needs the kept input.')
+    if kept is not None:
+        _check_kept(kept)
     code = _ELEMENT_TYPES.get(g.dtype)
     if code is None or not g.is_cuda:
         _require_gpu(g)
         _element_type(g, 'g')
-    if g.ndim == 0 or g.shape[-1] == 0 or g.shape[:-1] != kept.codes.shape[:-1]:
-        raise ValueError(f'g has to have the shape {(*kept.codes.shape[:-1], "out")}. Got {tuple(g.shape)}.')
+    if g.ndim == 0 or g.shape[-1] == 0 or (kept is not None and g.shape[:-1] != kept.codes.shape[:-1]):
+        raise ValueError(f'g has to have the shape {(*(("...",) if kept is None else kept.codes.shape[:-1]), "out")}. Got {tuple(g.shape)}.')
+    rows, F = g.numel() // g.shape[-1], kept.codes.shape[-1] if need_weight else 0
     dtype = dtype or g.dtype
     if dtype not in _ELEMENT_TYPES:
         raise TypeError(f'the gradients are float32, bfloat16 or float16. Got {dtype}.')
     device, n = g.device, g.shape[-1]
-    _like_first(kept.codes, 'the kept input', device)
+    if kept is not None:
+        _like_first(kept.codes, 'the kept input', device)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return weight_grad_8bit(g, kept, need_weight, need_bias, dtype)
@@ -1979,7 +1985,8 @@ def weight_grad_8bit(g, kept, need_weight=True, need_bias=True, dtype=None):
     g, ld = _rows_of(g, n)
     need = _ws_need('ak_weight_grad_8bit_ws_bytes', code, rows, F, n)
     ws = empty(need, dtype=torch.uint8, device=device)
-    rc = _lib.load().ak_weight_grad_8bit(g.data_ptr(), code, ld, kept.codes.data_ptr(), kept.exponents.data_ptr(), rows, F, n, _pointer(dw), _pointer(db),
+    codes, exponents = kept if need_weight else (None, None)
+    rc = _lib.load().ak_weight_grad_8bit(g.data_ptr(), code, ld, _pointer(codes), _pointer(exponents), rows, F, n, _pointer(dw), _pointer(db),
                                          _ELEMENT_TYPES[dtype], ws.data_ptr(), need, _stream_handle(device))
     _lib.check(rc, 'ak_weight_grad_8bit')
     return dw, db

@@ -225,6 +225,8 @@ def embedding(input, weight, padding_idx=None, scale=1.0):
     """scale * torch.nn.functional.embedding(input, weight, padding_idx): rows of ``weight`` for int32 or int64 ``input``, differentiable once.  The
     gradient is summed by tokens in sorted order, in fp32: the same bits every time, where torch's adds rows in the order in which
     they come.  A token that names no row gives NaN and takes no gradient."""
+    if padding_idx is not None and not -weight.shape[0] <= padding_idx < weight.shape[0]:
+        raise ValueError(f'padding_idx has to be within {weight.shape[0]} rows. Got {padding_idx}.')
     return _Embedding.apply(input, weight, padding_idx, float(scale))
 
 
@@ -300,11 +302,9 @@ class _Linear8bit(torch.autograd.Function):
 
         def gradients(g):
             dx = torch.matmul(g, weight) if need_x else None
-            if need_weight:
-                dw, db = kernels.weight_grad_8bit(g, kernels.Quantized8(codes, exponents), True, need_bias, weight.dtype)
-            else:
-                dw, db = None, g.reshape(-1, g.shape[-1]).sum(0) if need_bias else None
-            return dx, dw, db
+            if not (need_weight or need_bias):
+                return dx, None, None
+            return dx, *kernels.weight_grad_8bit(g, kernels.Quantized8(codes, exponents) if need_weight else None, need_weight, need_bias, weight.dtype)
         return _last(gradients, 'linear_8bit', g, weight)
 
 

@@ -538,11 +538,12 @@ int ak_embedding_backward(const void* g, int dtype, int64_t ldg, const void* tok
 
 /* Activations in 8 bits: codes [rows, width] (e4m3, dense) and exponents [rows, ceil(width / 128)]; a value of a block of 128 features of
  * a row stands for code * 2^e, e the least integer with max |x| 2^-e <= 448, within -127 .. 127 (infinities and NaN: kept as NaN, not
- * counted for e; what would be rounded to 2^128: kept as 1.875 * 2^127).  gelu 0 or 1: y (dense, the type of x) = x times the normal distribution's share below x or its approximation by tanh
- * in the same pass; -1: y is not written.
+ * counted for e; what would be rounded to 2^128: kept as 1.875 * 2^127).  gelu 0 or 1: y (dense, the type of x) = x times the normal
+ * distribution's share below x or its approximation by tanh in the same pass; -1: y is not written.
  * ak_dequantize_8bit, gelu -1: y (dense) = the kept values; 0 or 1: y = g * derivative of that function at the kept values.
  * ak_weight_grad_8bit: dw [out, width] = g^T x', db [out] = sums of g over the rows, x' the kept values; each may be null, g [rows, out].
- * The products of g's pieces with x' are exact, their sums fp32. */
+ * Without dw, codes and exponents may be null and width 0, also for the bytes of the workspace.  The products of g's pieces with x' are exact,
+ * their sums fp32. */
 int ak_quantize_8bit(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t width, int gelu, void* y, uint8_t* codes, int8_t* exponents,
                      ak_stream_t stream);
 int ak_dequantize_8bit(const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width, int gelu, const void* g, int64_t ldg,

@@ -87,6 +87,8 @@ def test_entry_points_refuse_bad_arguments():
         return lib.ak_weight_grad_8bit(g, dtype, ldg, codes, exponents, rows, width, out, dw, db, grad_dtype, ws, need, None)
     for kw in (dict(g=None), dict(codes=None), dict(exponents=None), dict(dtype=BAD), dict(grad_dtype=BAD), dict(ldg=63), dict(rows=0), dict(width=0), dict(out=0)):
         assert weight(**kw) == -1, kw
+    assert weight(codes=None, exponents=None, dw=None, width=0, need=64) == -2
+    assert 0 < lib.ak_weight_grad_8bit_ws_bytes(F32, 4, 0, 64) < lib.ak_weight_grad_8bit_ws_bytes(F32, 4, 64, 64)
     assert weight(dw=None, db=None) == 0 and weight(ws=None) == -2 and weight(need=64) == -2 and weight(width=(1 << 20) + 1) == -5
     assert lib.ak_weight_grad_8bit_ws_bytes(F32, 0, 64, 64) == 0
 
@@ -152,8 +154,8 @@ class Stand:
 
     def weight_grad_8bit(self, g, kept, need_weight=True, need_bias=True, dtype=None):
         self.calls.append(('weight', need_weight, need_bias))
-        x, g = kept.codes.float().flatten(0, -2), g.flatten(0, -2).float()
-        return (g.t() @ x).to(dtype) if need_weight else None, g.sum(0).to(dtype) if need_bias else None
+        g = g.flatten(0, -2).float()
+        return (g.t() @ kept.codes.float().flatten(0, -2)).to(dtype) if need_weight else None, g.sum(0).to(dtype) if need_bias else None
 
 
 @pytest.fixture
@@ -226,7 +228,7 @@ def test_only_what_a_pass_takes_is_computed(stand):
     torch.autograd.grad(y.sum(), [x], retain_graph=True)
     assert last() == []
     torch.autograd.grad(y.sum(), [b], retain_graph=True)
-    assert last() == []
+    assert last() == [('weight', False, True)]
     y.sum().backward()
     assert last() == [('weight', True, True)]
     asdl_amd.linear_8bit(x, w.detach(), None).sum().backward()
@@ -320,3 +322,14 @@ def test_a_sampled_fisher_leaves_the_weights_of_8_bit_layers_out(stand, monkeypa
 def test_public_names():
     for name in layers.__all__:
         assert getattr(asdl_amd, name) is getattr(layers, name)
+
+
+def test_embedding_refuses_a_padding_outside_the_table():
+    for padding in (7, -8):
+        with pytest.raises(ValueError, match='within 7 rows'):
+            asdl_amd.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(7, 4), padding)
+
+
+def test_weight_gradient_refuses_to_go_without_the_input():
+    with pytest.raises(ValueError, match='kept input'):
+        kernels.weight_grad_8bit(torch.zeros(3, 4), None)

@@ -282,6 +282,22 @@ def test_linear_cross_entropy_of_scaled_gradients(K, dtype, scale):
     assert all(bool(y.isfinite().all()) for y in scaled[:2]) or (dtype == F16 and scale > 1)
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+def test_linear_cross_entropy_of_gradients_that_are_no_numbers(K, dtype):
+    """An infinite or NaN gradient of one row leaves the other rows' alone."""
+    h, w, t = rand(70, 64, seed=1, dtype=dtype), rand(300, 64, seed=2, dtype=dtype, scale=0.1), ints(300, 70, seed=3)
+    loss, lse = K.linear_cross_entropy(h, w, t, reduction='none')
+    g = gradient_of('none', t, 4) * 50
+    g[5] = g[9] = 0
+    want = loss64(h, w, t, reduction='none', g=g)['dh']
+    g[5], g[9] = INF, NAN
+    dh = K.linear_cross_entropy_backward(g, h, w, t, lse, reduction='none')[0]
+    rest = torch.ones(70, dtype=torch.bool, device='cuda')
+    rest[[5, 9]] = False
+    within(dh[rest], want[0][rest], want[1][rest], 'dh')
+    assert not bool(dh[~rest].isfinite().any())
+
+
 def test_linear_cross_entropy_refuses(K):
     h, w, t, b = rand(6, 8, seed=1), rand(10, 8, seed=2), ints(10, 6, seed=3), rand(10, seed=4)
     loss, lse = K.linear_cross_entropy(h, w, t, b)
@@ -640,6 +656,8 @@ def test_weight_gradients_from_kept_inputs(K, rows, width, out, dtype):
         within(db, gd.sum(0), half_step(made) * gd.sum(0).abs() + (rows + 8) * U * gd.abs().sum(0) + tiny, 'db')
         again = K.weight_grad_8bit(g, kept, dtype=made)
         assert torch.equal(dw, again[0]) and torch.equal(db, again[1])
+    none, alone = K.weight_grad_8bit(g, None, need_weight=False)
+    assert none is None and torch.equal(alone, K.weight_grad_8bit(g, kept)[1])
     assert K.weight_grad_8bit(g, kept, need_bias=False)[1] is None and K.weight_grad_8bit(g, kept, need_weight=False)[0] is None
 
 
