@@ -40,12 +40,13 @@ __device__ __forceinline__ void column_chunk(const T* __restrict__ x, int64_t ld
   part[chunk * cols + col] = t;
 }
 
-// grid (columns / 256, chunks)
+// grid (columns / 256, chunks, pieces); the last piece's chunks are the first.
 template <typename T>
 static __global__ __launch_bounds__(256) void column_chunks_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
-                                                                   int64_t rows_per_chunk, float* __restrict__ part) {
+                                                                   int64_t rows_per_chunk, int64_t pitch, float* __restrict__ part) {
   __shared__ float joined[8][kColumnsPerGroup];
-  column_chunk(x, ld, rows, cols, rows_per_chunk, part, blockIdx.x, blockIdx.y, joined);
+  column_chunk(x + (gridDim.z - 1 - blockIdx.z) * pitch, ld, rows, cols, rows_per_chunk, part + static_cast<int64_t>(blockIdx.z) * gridDim.y * cols, blockIdx.x,
+               blockIdx.y, joined);
 }
 
 template <typename T>
@@ -81,9 +82,8 @@ inline int column_sums(const T* x, int64_t ld, int64_t rows, int64_t cols, float
   const int chunks = column_chunks(rows);
   const int64_t per = (rows + chunks - 1) / chunks;
   const unsigned groups = static_cast<unsigned>((cols + 255) / 256);
-  for (int k = pieces - 1; k >= 0; --k)
-    hipLaunchKernelGGL(column_chunks_kernel<T>, dim3(groups, static_cast<unsigned>(chunks)), dim3(256), 0, s, x + k * pitch, ld, rows, cols, per,
-                       part + (pieces - 1 - k) * chunks * cols);
+  hipLaunchKernelGGL(column_chunks_kernel<T>, dim3(groups, static_cast<unsigned>(chunks), static_cast<unsigned>(pieces)), dim3(256), 0, s, x, ld, rows, cols,
+                     per, pitch, part);
   hipLaunchKernelGGL(column_total_kernel<O>, dim3(groups), dim3(256), 0, s, part, cols, pieces * chunks, scale, factor, out);
   return check_launch();
 }
