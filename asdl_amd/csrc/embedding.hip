@@ -8,7 +8,8 @@
 //   sums:   a wave per chunk of sorted positions and 1 KB of columns; runs of equal tokens inside a chunk are written, parts of runs that
 //           cross its ends go to the workspace; other waves write the rows that no token names
 //   joins:  the parts of a run, in order
-// Bound by the memory: the gradients are read once, the table's gradient is written once.
+// Bound by the memory: the gradients are read once, the table's gradient is written once (131072 tokens of 131072 x 1024 bf16: lookup 80 to 87 us,
+// sort 34, sums 127, 4.2 TB/s, joins 13), few tokens by the launches (4.5 us each).
 #include <algorithm>
 #include "elements.hpp"
 

@@ -8,7 +8,8 @@
 //            approximation by tanh
 //   linear:  dw = g^T x',  db = sum g.  x' is a bfloat16 number exactly, so the products are exact and their sums fp32: g in
 //            bfloat16 as it is, in fp16 and fp32 as two and three bfloat16 pieces that add up to it exactly
-// The elementwise passes are bound by the memory, the products by the matrix cores.
+// The elementwise passes are bound by the memory (gelu of 8192 x 4096 bf16 36 us each way, 4.7 TB/s), the products by the matrix cores (16384
+// rows of 4096 to 4096 bf16 400 to 430 us, 1.3 PFLOP/s at the power limit; of 768 to 2304 from 8192 rows 39 us, too few tiles).
 #include <algorithm>
 #include "column_sums.hpp"
 #include "half_product.hpp"
