@@ -15,7 +15,7 @@
 
 namespace ak {
 
-constexpr int kEmbBins = 512, kEmbWaves = 16;        // keys of a sorting work group at most, its waves
+constexpr int kEmbBins = 1024, kEmbWaves = 16;        // keys of a sorting work group at most, its waves
 constexpr int64_t kEmbScan = 16384;
 constexpr int kEmbChunk = 4096;                      // tokens of a chunk
 #define AK_LDS __attribute__((address_space(3)))
@@ -100,7 +100,10 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
   __shared__ int sums[kEmbWaves], below_of[kEmbWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int keys = MODE == kSortChunk ? p.ranges : p.bins, v0 = MODE == kSortChunk ? 0 : blockIdx.x * p.bins, v1 = min(v0 + p.bins, p.t.rows);
-  for (int i = threadIdx.x; i < kEmbWaves * kEmbBins; i += 64 * kEmbWaves) (&count[0][0])[i] = 0;
+  static_assert(kEmbBins <= 64 * kEmbWaves, "a key a thread");
+  if (threadIdx.x < keys)
+#pragma unroll
+    for (int w = 0; w < kEmbWaves; ++w) count[w][threadIdx.x] = 0;
   // what there is to go through; the sorted position of the first
   int64_t begin = 0, end = p.t.count;
   int first = 0;
@@ -153,7 +156,7 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
   if constexpr (MODE == kSortAll)
 #pragma unroll
     for (int w = 0; w < kEmbWaves; ++w) first += below_of[w];
-  // thread i < kEmbBins: key i; places of the waves' tokens of that key from the exclusive sums over keys and waves
+  // thread i: key i; places of the waves' tokens of that key from the exclusive sums over keys and waves
   int mine = 0, earlier = 0;             // of this key: tokens behind it that count for the next key, tokens in front of this work group's
   if constexpr (MODE == kSortChunk) {
     if (threadIdx.x < keys)
@@ -163,7 +166,7 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
         mine += n;
         earlier += c < static_cast<int>(blockIdx.x) ? n : 0;
       }
-  } else if (threadIdx.x < kEmbBins) {
+  } else if (threadIdx.x < keys) {
 #pragma unroll
     for (int w = 0; w < kEmbWaves; ++w) mine += count[w][threadIdx.x];
   }
@@ -178,7 +181,7 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
   int at = first + incl - mine;
 #pragma unroll
   for (int w = 0; w < kEmbWaves; ++w) at += w < wave ? sums[w] : 0;
-  if (threadIdx.x < kEmbBins) {
+  if (threadIdx.x < keys) {
     if constexpr (MODE != kSortChunk) {
       const int v = v0 + threadIdx.x;
       if (v < v1) {
@@ -187,7 +190,7 @@ static __global__ __launch_bounds__(64 * kEmbWaves) void emb_sort_kernel(EmbSort
       }
     }
     if constexpr (MODE == kSortChunk)
-      if (blockIdx.x == 0 && threadIdx.x < keys) {
+      if (blockIdx.x == 0) {
         p.firsts[threadIdx.x] = at;
         if (static_cast<int>(threadIdx.x) == keys - 1) p.firsts[keys] = at + mine;
       }
