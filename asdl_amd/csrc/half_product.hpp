@@ -614,10 +614,21 @@ template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
 using HpWide = HpCfg<2, 4, 4, 2, A_BY_K, B_BY_K, 4, PIECES>;      // 256 x 256
 template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
 using HpSmall = HpCfg<2, 2, 2, 2, A_BY_K, B_BY_K, 4, PIECES>;     // 128 x 128
+template <bool A_BY_K, bool B_BY_K, bool PIECES = false>
+using HpTiny = HpCfg<2, 2, 1, 1, A_BY_K, B_BY_K, 4, PIECES>;      // 64 x 64
 
 // 256 x 256 tiles, but for results that 128 x 128 ones of at most one place each cover: two of those take 0.83 of the time of one wide
 // tile on a CU (1000 x 10007 x 513 in six products: 632 small tiles 126 us, 160 wide ones 97 us).
 inline bool hp_wide(int64_t I, int64_t J) { return ((I + 127) / 128) * ((J + 127) / 128) > 512; }
+// Tiles of 64 where those of 128 are for at most half of the CUs (533 x 865 x 2971, 35 tiles of 128: bf16 48 -> 37 us, six products 186 ->
+// 126 us; 1024 x 2048 x 768, 128 of them: 14.2 -> 13.0 us, 59 -> 55 us).
+inline bool hp_tiny(int64_t I, int64_t J) { return ((I + 127) / 128) * ((J + 127) / 128) <= 128; }
+
+// go(the tile form for a product whose contraction is in one piece)
+template <bool A_BY_K, bool B_BY_K, bool PIECES, typename F>
+inline int hp_form(int64_t I, int64_t J, F&& go) {
+  return hp_wide(I, J) ? go(HpWide<A_BY_K, B_BY_K, PIECES>{}) : hp_tiny(I, J) ? go(HpTiny<A_BY_K, B_BY_K, PIECES>{}) : go(HpSmall<A_BY_K, B_BY_K, PIECES>{});
+}
 
 // The device's LDS is more than a kernel has without asking; once a kernel and device.
 template <typename Kernel>

@@ -519,7 +519,7 @@ inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_
   if (pad_w) s.w = c.take<unsigned char>(p.V * p.ldp * p.k * 2);
   if (bias) s.bias = c.take<float>(p.V);
   if (!backward) {
-    const int64_t tile = p.few ? 16 : 128;      // the fewest classes of a part
+    const int64_t tile = p.few ? 16 : hp_tiny(p.V, p.N) ? 64 : 128;      // the fewest classes of a part
     s.part = c.take<floatx2>((p.V + tile - 1) / tile * p.N);
     s.at_target = c.take<float>(p.N);
     s.losses = c.take<float>(p.N);
@@ -604,7 +604,7 @@ inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, int* part
     *parts = q.tiles_i;
     return hp_launch<Cfg, M, LceStats>(q, LceStats::Params{c.r, s.part, s.at_target}, c.stream);
   };
-  return hp_wide(p.V, p.N) ? go(HpWide<true, true, PIECES>{}) : go(HpSmall<true, true, PIECES>{});
+  return hp_form<true, true, PIECES>(p.V, p.N, go);
 }
 
 struct LceGrads {
@@ -630,7 +630,7 @@ inline int lce_backward(LceCall c, const float* lse, const LcePlan& p, const Lce
       typename LceGrad<E>::Params e{c.r, lse, s.share, d, ldd, p.piece, static_cast<int>(c0), static_cast<int>(padded)};
       return hp_launch<Cfg, M, LceGrad<E>>(q, e, c.stream);
     };
-    rc = hp_wide(padded, p.N) ? grad(HpWide<true, true, PIECES>{}) : grad(HpSmall<true, true, PIECES>{});
+    rc = hp_form<true, true, PIECES>(padded, p.N, grad);
     if (rc != AK_OK) return rc;
     // dw: i features, j classes, k rows.  dh: i features, j rows, k classes (a shorter last piece has no more splits)
     auto gradients = [&](auto dw_cfg, auto dh_cfg) {
