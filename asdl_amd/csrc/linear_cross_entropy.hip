@@ -456,7 +456,8 @@ inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D, bool backwar
   p.N = N; p.V = V; p.D = D;
   p.k = dtype == AK_F32 ? 3 : 1;
   p.few = !backward && N <= lce_few_rows(dtype, copied);
-  const int64_t fit = std::max<int64_t>(kLcePieceBytes / (N * p.k * 2) / 256 * 256, 256);
+  // (at most 2^24: 32 rows of d within 32-bit byte offsets)
+  const int64_t fit = std::min<int64_t>(std::max<int64_t>(kLcePieceBytes / (N * p.k * 2) / 256 * 256, 256), 1 << 24);
   p.pieces = (V + fit - 1) / fit;
   p.piece = align_up((V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (V + p.piece - 1) / p.piece;

@@ -254,10 +254,10 @@ def test_linear_cross_entropy_gives_what_is_asked_for(K, dtype):
 
 
 @pytest.mark.parametrize('dtype,rows,classes,width', [(BF16, 2100, 70001, 64), (F16, 4200, 33000, 40), (F32, 1030, 66000, 36), (BF16, 9000, 16500, 72),
-                                                      (BF16, 4200, 70001, 64), (F16, 9000, 33000, 40), (F32, 1030, 90001, 36), (BF16, 1100000, 600, 8)])
+                                                      (BF16, 4200, 70001, 64), (F16, 9000, 33000, 40), (F32, 1030, 90001, 36), (BF16, 1100000, 600, 8), (BF16, 3, (1 << 24) + 300, 8)])
 def test_linear_cross_entropy_in_pieces(K, dtype, rows, classes, width):
     """Up to 512 MB of the logits' gradient, as float32 in three pieces of 16 bits, and more: several pieces of the classes, the last one shorter;
-    with very many rows pieces of 256 classes."""
+    with very many rows pieces of 256 classes, with very many classes pieces of 2^24."""
     print(f'linear_cross_entropy {rows}x{classes}x{width} {dtype}', flush=True)
     h, w = rand(rows, width, seed=1, dtype=dtype), rand(classes, width, seed=2, dtype=dtype, scale=0.2)
     t = ints(classes, rows, seed=3)
