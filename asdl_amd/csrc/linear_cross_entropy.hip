@@ -56,13 +56,22 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 // exp(s - shift) = exp(s) * rest, a fused multiplication and addition and the power of two an element: the product of the shift is rounded
 // to float32 (2^-24 of a shift of 60 is 4e-6), and what that loses, exact by a fused operation, is a factor that all elements share.
+// From 2^20 on (all classes of a tile masked by a type's lowest value, -1e10, -1e30) that factor would be no number or the product
+// infinite: the difference itself goes into the power there.  That is one more operation an element, for waves that have such a row;
+// the other rows of theirs subtract 0, so that their bits are the same beside it.
 struct Shifted {
-  float by, rest;
-  __device__ __forceinline__ explicit Shifted(float shift) : by(shift * kLog2e) {
-    const float lost = __builtin_fmaf(shift, kLog2e, -by);
-    rest = fabsf(lost) < 1.f ? __builtin_amdgcn_exp2f(-lost) : 1.f;          // (NaN of an infinite shift)
+  float from, by, rest;
+  __device__ __forceinline__ explicit Shifted(float shift) {
+    const bool near = fabsf(shift) < 0x1p20f;           // (neither infinite nor NaN)
+    from = near ? 0.f : shift;
+    by = near ? shift * kLog2e : 0.f;
+    rest = near ? __builtin_amdgcn_exp2f(-__builtin_fmaf(shift, kLog2e, -by)) : 1.f;
   }
-  __device__ __forceinline__ float exp(float s) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, kLog2e, -by)); }
+  __device__ __forceinline__ bool far() const { return __any(from != 0.f); }
+  template <bool FAR>
+  __device__ __forceinline__ float exp(float s) const {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(FAR ? s - from : s, kLog2e, -by));
+  }
 };
 
 // What a tile's sums become: the bias is added, and classes behind the last are -inf.  Most tiles have neither.  (c0: first class of the
@@ -110,10 +119,14 @@ struct LceStats {
         for (int x = 0; x < 16; ++x) m = fmaxf(m, acc[a][b][x]);
       const Shifted by(m == -INFINITY ? 0.f : m);
       float s = 0.f;
+      auto add = [&](auto far) {
 #pragma unroll
-      for (int a = 0; a < Cfg::FR; ++a)
+        for (int a = 0; a < Cfg::FR; ++a)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) s += by.exp(acc[a][b][x]);
+          for (int x = 0; x < 16; ++x) s += by.exp<decltype(far)::value>(acc[a][b][x]);
+      };
+      if (by.far()) add(std::true_type{});
+      else add(std::false_type{});
       s *= by.rest;
       if (__any(at >= 0 && at < 32 * Cfg::FR)) {
 #pragma unroll
@@ -165,12 +178,14 @@ struct LceGrad {
       const float times = share * by.rest;
       const int64_t at = in && share != 0.f ? e.r.targets[j] - e.c0 - i0 : -1;
       // (ignored rows: 0, whatever their scores; the share of a class of no probability: 0)
+      auto shares = [&](auto far) {
 #pragma unroll
-      for (int a = 0; a < Cfg::FR; ++a)
+        for (int a = 0; a < Cfg::FR; ++a)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          acc[a][b][x] = share != 0.f ? by.exp(acc[a][b][x]) * times : 0.f;
-        }
+          for (int x = 0; x < 16; ++x) acc[a][b][x] = share != 0.f ? by.exp<decltype(far)::value>(acc[a][b][x]) * times : 0.f;
+      };
+      if (by.far()) shares(std::true_type{});
+      else shares(std::false_type{});
       if (__any(at >= 0 && at < 32 * Cfg::FR)) {
 #pragma unroll
         for (int a = 0; a < Cfg::FR; ++a)

@@ -1,0 +1,55 @@
+"""The cross entropy of a linear layer, embeddings and activations in 8 bits at the ends of what they take, against their definitions in
+64 bits.  The tolerances are those of test_decoder_step_gpu; what a test adds to them it derives."""
+import math
+
+import pytest
+import torch
+
+from tests.test_decoder_step_gpu import BF16, F16, F32, INF, K, U, check_loss, gradient_of, half_step, ints, loss64, rand, within     # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ cross entropy of a linear layer
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('rows', [8, 100, 700])
+@pytest.mark.parametrize('mask', [-INF, torch.finfo(F32).min, -1e30, -1e10, -3e6, -1e5])
+def test_linear_cross_entropy_of_neighbouring_masked_classes(K, mask, rows, dtype):     # noqa: F811
+    """The classes of whole tiles taken out, as those behind a vocabulary that is padded: loss and gradients are those of the others.  (A
+    share of the masked classes is 0 in 64 bits, too.)"""
+    classes, width = 2000, 64
+    h, w = rand(rows, width, seed=1, dtype=dtype), rand(classes, width, seed=2, dtype=dtype, scale=0.2)
+    b = rand(classes, seed=3)
+    b[:300], b[1100:] = mask, mask
+    t = 300 + ints(800, rows, seed=4)
+    check_loss(K, h, w, t, b, g=gradient_of('mean', t, 5))
+    loss, lse = K.linear_cross_entropy(h, w, t, b, reduction='none')
+    _, dw, db = K.linear_cross_entropy_backward(torch.ones_like(loss), h, w, t, lse, b, reduction='none')
+    for d in (dw, db):
+        assert bool((d[:300] == 0).all()) and bool((d[1100:] == 0).all()) and bool((d[300:1100] != 0).any())
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('rows', [8, 100, 700])
+def test_linear_cross_entropy_of_a_row_of_the_lowest_values(K, rows, dtype):     # noqa: F811
+    """All scores are the lowest float32 number (scores of less than half a step of it, 2^103, are lost in the sum): the loss is the log of
+    the number of classes, as torch's."""
+    h, w = rand(rows, 64, seed=1, dtype=dtype), rand(2000, 64, seed=2, dtype=dtype)
+    loss, _ = K.linear_cross_entropy(h, w, ints(2000, rows, seed=3), torch.full((2000,), torch.finfo(F32).min, device='cuda'), reduction='none')
+    within(loss, torch.full_like(loss, math.log(2000), dtype=torch.float64), torch.full_like(loss, 2.0 ** -20 * 9, dtype=torch.float64), 'loss')
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+def test_linear_cross_entropy_beside_rows_of_large_scores(K, dtype):     # noqa: F811
+    """A row of scores beyond 2^20 leaves the bits of its neighbours as they are."""
+    h, w, t = rand(300, 64, seed=1, dtype=dtype), rand(900, 64, seed=2, dtype=dtype, scale=0.5), ints(900, 300, seed=3)
+    loss, lse = K.linear_cross_entropy(h, w, t, reduction='none')
+    g = gradient_of('none', t, 4)
+    dh = K.linear_cross_entropy_backward(g, h, w, t, lse, reduction='none')[0]
+    large = h.clone()
+    large[[5, 177]] = 6e4 * w[t[[5, 177]]].float().sign().to(dtype)          # (some 6e4 * 64 * 0.4 = 1.5e6)
+    other, lse = K.linear_cross_entropy(large, w, t, reduction='none')
+    rest = torch.ones(300, dtype=torch.bool, device='cuda')
+    rest[[5, 177]] = False
+    assert torch.equal(other[rest], loss[rest])
+    assert torch.equal(K.linear_cross_entropy_backward(g, large, w, t, lse, reduction='none')[0][rest], dh[rest])
