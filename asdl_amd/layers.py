@@ -266,18 +266,25 @@ def fuse_embeddings(model: nn.Module) -> int:
 
 
 # ------------------------------------------------------------------------------ activations in 8 bits
+# The gradients below depend on an input of which only codes are kept.  For a second derivative to come across their end, whatever it is
+# taken of, _last() needs a tensor whose graph leads to that input: a result without elements does, and holds nothing of it.
 class _GELU8bit(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, approximate):
         y, kept = kernels.gelu_8bit(x, approximate)
-        ctx.save_for_backward(*kept)
+        link = x.new_empty(0)
+        ctx.save_for_backward(*kept, link)
+        ctx.set_materialize_grads(False)
         ctx.approximate = approximate
-        return y
+        return y, link
 
     @staticmethod
-    def backward(ctx, g):
-        kept = kernels.Quantized8(*ctx.saved_tensors)
-        return _last(lambda g: kernels.gelu_8bit_backward(g, kept, ctx.approximate), 'gelu_8bit', g), None
+    def backward(ctx, g, _):
+        if g is None:
+            return None, None
+        codes, exponents, link = ctx.saved_tensors
+        kept = kernels.Quantized8(codes, exponents)
+        return _last(lambda g: kernels.gelu_8bit_backward(g, kept, ctx.approximate), 'gelu_8bit', g, link), None
 
 
 def gelu_8bit(input, approximate='none'):
@@ -285,27 +292,29 @@ def gelu_8bit(input, approximate='none'):
     itself, its gradient that of the kept values.  Differentiable once."""
     if not (input.requires_grad and torch.is_grad_enabled()):
         return F.gelu(input, approximate=approximate)
-    return _GELU8bit.apply(input, approximate)
+    return _GELU8bit.apply(input, approximate)[0]
 
 
 class _Linear8bit(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         kept = kernels.quantize_8bit(x) if ctx.needs_input_grad[1] else (None, None)
-        ctx.save_for_backward(weight, *kept)
-        return F.linear(x, weight, bias)
+        link = x.new_empty(0) if ctx.needs_input_grad[0] and ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(weight, *kept, link)
+        ctx.set_materialize_grads(False)
+        return F.linear(x, weight, bias), link
 
     @staticmethod
-    def backward(ctx, g):
-        weight, codes, exponents = ctx.saved_tensors
+    def backward(ctx, g, _):
+        if g is None:
+            return None, None, None
+        weight, codes, exponents, link = ctx.saved_tensors
         need_x, need_weight, need_bias = (_wanted(ctx, i) for i in range(3))
-
-        def gradients(g):
-            dx = torch.matmul(g, weight) if need_x else None
-            if not (need_weight or need_bias):
-                return dx, None, None
-            return dx, *kernels.weight_grad_8bit(g, kernels.Quantized8(codes, exponents) if need_weight else None, need_weight, need_bias, weight.dtype)
-        return _last(gradients, 'linear_8bit', g, weight)
+        dx = _last(lambda g: torch.matmul(g, weight), 'linear_8bit', g, weight) if need_x else None
+        if not (need_weight or need_bias):
+            return dx, None, None
+        kept = kernels.Quantized8(codes, exponents) if need_weight else None
+        return dx, *_last(lambda g: kernels.weight_grad_8bit(g, kept, need_weight, need_bias, weight.dtype), 'linear_8bit', g, link if need_weight else None)
 
 
 def linear_8bit(input, weight, bias=None):
@@ -313,7 +322,7 @@ def linear_8bit(input, weight, bias=None):
     input are those of torch's, the gradient of the weight is that of the kept values.  float32, bfloat16 or float16, autocast as there.
     Differentiable once."""
     input, weight, bias = _autocast(input, weight, bias)
-    return _Linear8bit.apply(input, weight, bias)
+    return _Linear8bit.apply(input, weight, bias)[0]
 
 
 class GELU8bit(nn.GELU):
