@@ -321,6 +321,8 @@ def linear_8bit(input, weight, bias=None):
     """torch.nn.functional.linear whose backward pass reads the input from 8 bits (kernels.quantize_8bit): the result and the gradient of the
     input are those of torch's, the gradient of the weight is that of the kept values.  float32, bfloat16 or float16, autocast as there.
     Differentiable once."""
+    if not torch.is_grad_enabled():          # (needs_input_grad says true of a parameter there, too)
+        return F.linear(input, weight, bias)
     input, weight, bias = _autocast(input, weight, bias)
     return _Linear8bit.apply(input, weight, bias)[0]
 

@@ -64,3 +64,29 @@ def test_nothing_of_the_input_is_held(stand):     # noqa: F811
         assert not values.expired()
         del x
         assert values.expired() and y.requires_grad
+
+
+# ------------------------------------------------------------------------------------------------ passes without a way back
+def test_nothing_is_kept_where_nothing_goes_back(stand):     # noqa: F811
+    """Evaluation, and the first pass of a reentrant checkpoint: parameters need gradients there, too."""
+    model = nn.Sequential(nn.Linear(4, 6), nn.GELU(), nn.Linear(6, 3))
+    want = model(coarse(5, 4, seed=1)).detach()
+    asdl_amd.keep_activations_8bit(model)
+
+    def kept():
+        count, stand.calls[:] = len([c for c in stand.calls if c[0] == 'keep']), []
+        return count
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert torch.equal(model(coarse(5, 4, seed=1)), want)
+        assert kept() == 0
+    x = coarse(5, 4, seed=1).requires_grad_()
+    y = checkpoint(model, x, use_reentrant=True)
+    assert kept() == 0 and torch.equal(y, want)
+    y.sum().backward()
+    assert kept() == 3 and all(p.grad is not None for p in model.parameters())
+    model(x.detach())
+    assert kept() == 3
+    model.requires_grad_(False)
+    model(x.detach())
+    assert kept() == 0
