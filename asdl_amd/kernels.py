@@ -1308,8 +1308,9 @@ def sample_filtered(logits, u=None, temperature=1.0, top_k=None, top_p=None, min
 
 
 # ------------------------------------------------------------------------------ layer norm
-def _rows_of(t, F):
-    """``t`` as rows of F contiguous elements: (tensor that holds them, row stride).  Copied where one stride cannot reach the rows."""
+def _rows_of(t, F, most=None):
+    """``t`` as rows of F contiguous elements: (tensor that holds them, row stride).  Copied where one stride cannot reach the rows, and where
+    it is more than ``most``, the largest that the entry point takes."""
     if t.is_contiguous():
         return t, F
     if t.stride(-1) == 1 or F == 1:
@@ -1327,7 +1328,7 @@ def _rows_of(t, F):
         else:
             if expect is None:
                 return t, F
-        if first is not None and first >= F:
+        if first is not None and first >= F and (most is None or first <= most):
             return t, first
     return _contiguous(t.detach()), F
 
@@ -1622,6 +1623,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, outs=None):
 
 # ------------------------------------------------------------------------------ cross entropy of a linear layer
 _REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
+_LOSS_PITCH = 1 << 21          # the largest row stride that the entry points take: the last token of sequences of 4096 x 768 has a larger one
 
 
 def _like_first(t, what, device):
@@ -1680,8 +1682,8 @@ def linear_cross_entropy(h, weight, targets, bias=None, ignore_index=-100, reduc
     if rows == 0:
         with _on_launch_stream():
             return loss if kind == 0 else loss.fill_(0.0 if kind == 1 else float('nan')), lse
-    h, ldh = _rows_of(h, D)
-    weight, ldw = _rows_of(weight, D)
+    h, ldh = _rows_of(h, D, _LOSS_PITCH)
+    weight, ldw = _rows_of(weight, D, _LOSS_PITCH)
     targets = _contiguous(targets)
     bias = None if bias is None else _contiguous(bias)
     need = _ws_need('ak_linear_cross_entropy_ws_bytes', code, rows, classes, D, 0)
@@ -1725,8 +1727,8 @@ def linear_cross_entropy_backward(g, h, weight, targets, lse, bias=None, ignore_
         return dh, dw, db
     if dh is None and dw is None and db is None:
         return dh, dw, db
-    h, ldh = _rows_of(h, D)
-    weight, ldw = _rows_of(weight, D)
+    h, ldh = _rows_of(h, D, _LOSS_PITCH)
+    weight, ldw = _rows_of(weight, D, _LOSS_PITCH)
     targets, g, lse = _contiguous(targets), _contiguous(g), _contiguous(lse)
     bias = None if bias is None else _contiguous(bias)
     need = _ws_need('ak_linear_cross_entropy_ws_bytes', code, rows, classes, D, 1)
@@ -1982,7 +1984,7 @@ def weight_grad_8bit(g, kept, need_weight=True, need_bias=True, dtype=None):
                 if t is not None:
                     t.zero_()
         return dw, db
-    g, ld = _rows_of(g, n)
+    g, ld = _rows_of(g, n, 1 << 24)
     need = _ws_need('ak_weight_grad_8bit_ws_bytes', code, rows, F, n)
     ws = empty(need, dtype=torch.uint8, device=device)
     codes, exponents = kept if need_weight else (None, None)

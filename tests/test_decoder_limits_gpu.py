@@ -53,3 +53,25 @@ def test_linear_cross_entropy_beside_rows_of_large_scores(K, dtype):     # noqa:
     rest[[5, 177]] = False
     assert torch.equal(other[rest], loss[rest])
     assert torch.equal(K.linear_cross_entropy_backward(g, large, w, t, lse, reduction='none')[0][rest], dh[rest])
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('rows', [3, 70])
+def test_linear_cross_entropy_of_the_last_token_of_long_sequences(K, rows, dtype):     # noqa: F811
+    """Rows further apart than the entry point takes them: 4096 * 768 elements."""
+    hidden = rand(rows, 4096, 768, seed=1, dtype=dtype)
+    w, t = rand(500, 768, seed=2, dtype=dtype, scale=0.07), ints(500, rows, seed=3)
+    check_loss(K, hidden[:, -1], w, t, g=gradient_of('mean', t, 4))
+    assert all(torch.equal(a, b) for a, b in zip(K.linear_cross_entropy(hidden[:, -1], w, t), K.linear_cross_entropy(hidden[:, -1].contiguous(), w, t)))
+
+
+def test_linear_cross_entropy_of_weights_far_apart(K):     # noqa: F811
+    w = rand(40, (1 << 21) + 8, seed=1, dtype=BF16)[:, 3:75]
+    h, t = rand(90, 72, seed=2, dtype=BF16), ints(40, 90, seed=3)
+    check_loss(K, h, w, t, g=gradient_of('mean', t, 4))
+
+
+def test_weight_gradients_of_rows_far_apart(K):     # noqa: F811
+    g = rand(40, (1 << 24) + 8, seed=1, dtype=BF16)[:, 5:29]
+    kept = K.quantize_8bit(rand(40, 72, seed=2, dtype=BF16))
+    assert all(torch.equal(a, b) for a, b in zip(K.weight_grad_8bit(g, kept), K.weight_grad_8bit(g.contiguous(), kept)))
