@@ -75,6 +75,7 @@ _SIGNATURES = {
     'ak_grad_norm': (c_int, [c_ptr, c_int, c_int, c_ptr, c_ptr, c_size, c_ptr]),
     'ak_clip_grad_norm': (c_int, [c_ptr, c_int, c_int, c_f64, c_ptr, c_ptr, c_size, c_ptr]),
     'ak_linear_cross_entropy_ws_bytes': (c_size, [c_int, c_i64, c_i64, c_i64, c_int]),
+    'ak_linear_cross_entropy_ws_bytes_of': (c_size, [c_ptr, c_int, c_i64, c_ptr, c_i64, c_int, c_i64, c_i64, c_i64, c_int]),
     'ak_linear_cross_entropy': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_i64, c_ptr, c_int, c_ptr, c_i64, c_i64, c_i64, c_i64, c_int, c_ptr,
                                         c_ptr, c_ptr, c_size, c_ptr]),
     'ak_linear_cross_entropy_backward': (c_int, [c_ptr, c_ptr, c_int, c_i64, c_ptr, c_i64, c_ptr, c_int, c_ptr, c_ptr, c_i64, c_i64, c_i64,
@@ -86,6 +87,7 @@ _SIGNATURES = {
     'ak_quantize_8bit': (c_int, [c_ptr, c_int, c_i64, c_i64, c_i64, c_int, c_ptr, c_ptr, c_ptr, c_ptr]),
     'ak_dequantize_8bit': (c_int, [c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr, c_i64, c_ptr, c_int, c_ptr]),
     'ak_weight_grad_8bit_ws_bytes': (c_size, [c_int, c_i64, c_i64, c_i64]),
+    'ak_weight_grad_8bit_ws_bytes_of': (c_size, [c_ptr, c_int, c_i64, c_i64, c_i64, c_i64, c_int]),
     'ak_weight_grad_8bit': (c_int, [c_ptr, c_int, c_i64, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_int, c_ptr, c_size, c_ptr]),
     'ak_event_synchronize': (c_int, [c_ptr]),
     'ak_kron_finish': (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_int, c_ptr, c_ptr]),
@@ -175,9 +177,9 @@ def load_host():
         return (ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names)
     module.bind(*addresses('ak_layer_norm', 'ak_layer_norm_backward', 'ak_layer_norm_backward_ws_bytes', 'ak_sample_filtered', 'ak_grad_norm',
                            'ak_clip_grad_norm', 'ak_grad_norm_ws_bytes'))
-    module.bind_step(*addresses('ak_linear_cross_entropy', 'ak_linear_cross_entropy_backward', 'ak_linear_cross_entropy_ws_bytes', 'ak_embedding',
+    module.bind_step(*addresses('ak_linear_cross_entropy', 'ak_linear_cross_entropy_backward', 'ak_linear_cross_entropy_ws_bytes_of', 'ak_embedding',
                                 'ak_embedding_backward', 'ak_embedding_backward_ws_bytes', 'ak_quantize_8bit', 'ak_dequantize_8bit',
-                                'ak_weight_grad_8bit', 'ak_weight_grad_8bit_ws_bytes'))
+                                'ak_weight_grad_8bit', 'ak_weight_grad_8bit_ws_bytes_of'))
     _host = module
     return module
 

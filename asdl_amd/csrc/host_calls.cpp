@@ -28,14 +28,14 @@ struct Entries {
   decltype(&ak_grad_norm_ws_bytes) grad_norm_ws_bytes;
   decltype(&ak_linear_cross_entropy) linear_cross_entropy;
   decltype(&ak_linear_cross_entropy_backward) linear_cross_entropy_backward;
-  decltype(&ak_linear_cross_entropy_ws_bytes) linear_cross_entropy_ws_bytes;
+  decltype(&ak_linear_cross_entropy_ws_bytes_of) linear_cross_entropy_ws_bytes_of;
   decltype(&ak_embedding) embedding;
   decltype(&ak_embedding_backward) embedding_backward;
   decltype(&ak_embedding_backward_ws_bytes) embedding_backward_ws_bytes;
   decltype(&ak_quantize_8bit) quantize_8bit;
   decltype(&ak_dequantize_8bit) dequantize_8bit;
   decltype(&ak_weight_grad_8bit) weight_grad_8bit;
-  decltype(&ak_weight_grad_8bit_ws_bytes) weight_grad_8bit_ws_bytes;
+  decltype(&ak_weight_grad_8bit_ws_bytes_of) weight_grad_8bit_ws_bytes_of;
 } entries;
 
 // The code of an element type; -1: none of the three.
@@ -94,9 +94,9 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
 
 // bind_step(the addresses behind those)
 PyObject* bind_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
-  return bind_to(args, count, entries.linear_cross_entropy, entries.linear_cross_entropy_backward, entries.linear_cross_entropy_ws_bytes, entries.embedding,
+  return bind_to(args, count, entries.linear_cross_entropy, entries.linear_cross_entropy_backward, entries.linear_cross_entropy_ws_bytes_of, entries.embedding,
                  entries.embedding_backward, entries.embedding_backward_ws_bytes, entries.quantize_8bit, entries.dequantize_8bit, entries.weight_grad_8bit,
-                 entries.weight_grad_8bit_ws_bytes);
+                 entries.weight_grad_8bit_ws_bytes_of);
 }
 
 // layer_norm(x, weight, bias, eps, float32 result, stream) -> (y, mean, rstd)
@@ -338,7 +338,8 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t coun
     pybind11::gil_scoped_release release;
     loss = kind == 0 ? made(t->sizes(), *h, at::kFloat) : made({}, *h, at::kFloat);
     lse = made(t->sizes(), *h, at::kFloat);
-    const size_t bytes = entries.linear_cross_entropy_ws_bytes(l.code, l.rows, l.classes, l.width, 0);
+    const size_t bytes = entries.linear_cross_entropy_ws_bytes_of(h->data_ptr(), l.code, l.width, w->data_ptr(), l.width, l.bias.defined() ? l.bias_code : -1, l.rows,
+                                                                  l.classes, l.width, 0);
     at::Tensor ws = made({static_cast<int64_t>(bytes)}, *h, at::kByte);
     rc = entries.linear_cross_entropy(h->data_ptr(), l.code, l.width, w->data_ptr(), l.width, address(l.bias), l.bias_code, t->data_ptr<int64_t>(), l.rows,
                                       l.classes, l.width, ignore, static_cast<int>(kind), loss.data_ptr<float>(), lse.data_ptr<float>(), ws.data_ptr(), bytes,
@@ -373,7 +374,8 @@ PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssi
     if (need & 2) dw = made(w->sizes(), *h, h->scalar_type());
     if ((need & 4) && l.bias.defined()) db = made(l.bias.sizes(), *h, l.bias.scalar_type());
     if (dh.defined() || dw.defined() || db.defined()) {
-      const size_t bytes = entries.linear_cross_entropy_ws_bytes(l.code, l.rows, l.classes, l.width, 1);
+      const size_t bytes = entries.linear_cross_entropy_ws_bytes_of(h->data_ptr(), l.code, l.width, w->data_ptr(), l.width, l.bias.defined() ? l.bias_code : -1,
+                                                                    l.rows, l.classes, l.width, (dh.defined() ? 1 : 0) | (dw.defined() ? 2 : 0) | (db.defined() ? 4 : 0));
       at::Tensor ws = made({static_cast<int64_t>(bytes)}, *h, at::kByte);
       rc = entries.linear_cross_entropy_backward(g.data_ptr<float>(), h->data_ptr(), l.code, l.width, w->data_ptr(), l.width, address(l.bias), l.bias_code,
                                                  t->data_ptr<int64_t>(), lse.data_ptr<float>(), l.rows, l.classes, l.width, ignore, static_cast<int>(kind),
@@ -530,7 +532,7 @@ PyObject* weight_grad_8bit(PyObject*, PyObject* const* args, Py_ssize_t count) {
     const int64_t F = codes->size(-1), out = g.size(-1), rows = g.numel() / out;
     if (need & 1) dw = made({out, F}, g, kTypes[type]);
     if (need & 2) db = made({out}, g, kTypes[type]);
-    const size_t bytes = entries.weight_grad_8bit_ws_bytes(code, rows, F, out);
+    const size_t bytes = entries.weight_grad_8bit_ws_bytes_of(g.data_ptr(), code, out, rows, F, out, static_cast<int>(need));
     at::Tensor ws = made({static_cast<int64_t>(bytes)}, g, at::kByte);
     rc = entries.weight_grad_8bit(g.data_ptr(), code, out, static_cast<const uint8_t*>(codes->data_ptr()), static_cast<const int8_t*>(exponents->data_ptr()), rows,
                                   F, out, address(dw), address(db), static_cast<int>(type), ws.data_ptr(), bytes, stream);

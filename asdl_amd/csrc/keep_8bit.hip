@@ -365,6 +365,12 @@ extern "C" size_t ak_weight_grad_8bit_ws_bytes(int dtype, int64_t rows, int64_t 
   return ak::keep_space(ak::keep_plan(dtype, rows, width, out), rows, out, width > 0, true, true, nullptr).bytes;
 }
 
+extern "C" size_t ak_weight_grad_8bit_ws_bytes_of(const void* g, int dtype, int64_t ldg, int64_t rows, int64_t width, int64_t out, int gradients) {
+  if (ak_weight_grad_8bit_ws_bytes(dtype, rows, width, out) == 0) return 0;
+  return ak::keep_space(ak::keep_plan(dtype, rows, width, out), rows, out, (gradients & 1) != 0, dtype != AK_BF16 || !ak::hp_aligned(g, ldg, out),
+                        (gradients & 2) != 0, nullptr).bytes;
+}
+
 extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width,
                                    int64_t out, void* dw, void* db, int grad_dtype, void* ws, size_t ws_bytes, ak_stream_t stream) {
   using namespace ak;

@@ -528,14 +528,20 @@ struct LceSpace {
   size_t bytes;
 };
 
-inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_w, bool bias, void* ws) {
+// What a call makes in its workspace beside what all calls do: copies of operands, sums of the gradients that are asked for.
+struct LceNeeds {
+  bool h, w, bias;         // copied
+  bool dh, dw, db;
+};
+
+inline LceSpace lce_space(const LcePlan& p, bool backward, const LceNeeds& need, void* ws) {
   Carver c{static_cast<unsigned char*>(ws)};
   LceSpace s = {};
-  if (pad_h) s.h = c.take<unsigned char>(p.N * p.ldp * p.k * 2);
-  if (pad_w) s.w = c.take<unsigned char>(p.V * p.ldp * p.k * 2);
-  if (bias) s.bias = c.take<float>(p.V);
+  if (need.h) s.h = c.take<unsigned char>(p.N * p.ldp * p.k * 2);
+  if (need.w) s.w = c.take<unsigned char>(p.V * p.ldp * p.k * 2);
+  if (need.bias) s.bias = c.take<float>(p.V);
   if (!backward) {
-    const int64_t tile = p.few ? 16 : hp_tiny(p.V, p.N) ? 64 : 128;      // the fewest classes of a part
+    const int64_t tile = p.few ? 16 : hp_wide(p.V, p.N) ? 256 : hp_tiny(p.V, p.N) ? 64 : 128;      // classes of a part
     s.part = c.take<floatx2>((p.V + tile - 1) / tile * p.N);
     s.at_target = c.take<float>(p.N);
     s.losses = c.take<float>(p.N);
@@ -543,9 +549,9 @@ inline LceSpace lce_space(const LcePlan& p, bool backward, bool pad_h, bool pad_
     s.share = c.take<float>(p.N);
     s.unit = c.take<float>(1);
     s.d = c.take<unsigned char>(p.N * p.piece * p.k * 2);
-    s.sum = c.take<float>(static_cast<int64_t>(p.splits) * p.N * p.ld_sum);
-    if (p.splits_dw > 1) s.sum_dw = c.take<float>(p.splits_dw * std::min(p.piece, p.V) * p.ld_sum);
-    s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(p.N, p.k * p.piece) / sizeof(float)));
+    if (need.dh) s.sum = c.take<float>(static_cast<int64_t>(p.splits) * p.N * p.ld_sum);
+    if (need.dw && p.splits_dw > 1) s.sum_dw = c.take<float>(p.splits_dw * std::min(p.piece, p.V) * p.ld_sum);
+    if (need.db) s.columns = c.take<float>(static_cast<int64_t>(column_sums_ws_bytes(p.N, p.k * p.piece) / sizeof(float)));
   }
   s.bytes = c.used;
   return s;
@@ -699,9 +705,33 @@ extern "C" size_t ak_linear_cross_entropy_ws_bytes(int dtype, int64_t rows, int6
   // enough for operands of any alignment
   auto bytes = [&](bool copied) {
     const ak::LcePlan p = ak::lce_plan(dtype, rows, classes, width, backward != 0, copied);
-    return ak::lce_space(p, backward != 0, copied && !p.few, copied && !p.few, true, nullptr).bytes;
+    return ak::lce_space(p, backward != 0, {copied && !p.few, copied && !p.few, true, true, true, true}, nullptr).bytes;
   };
   return backward != 0 ? bytes(true) : std::max(bytes(false), bytes(true));
+}
+
+namespace ak {
+
+// Plan and workspace of a call.
+struct LceLayout {
+  LcePlan plan;
+  LceSpace space;
+};
+
+inline LceLayout lce_layout(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, bool narrow_bias, int64_t rows, int64_t classes, int64_t width,
+                            bool backward, bool dh, bool dw, bool db, void* ws) {
+  const bool copy_h = dtype == AK_F32 || !hp_aligned(h, ldh, width), copy_w = dtype == AK_F32 || !hp_aligned(w, ldw, width);
+  const LcePlan p = lce_plan(dtype, rows, classes, width, backward, copy_h || copy_w);
+  return LceLayout{p, lce_space(p, backward, {!p.few && copy_h, !p.few && copy_w, narrow_bias, dh, dw, db}, ws)};
+}
+
+}  // namespace ak
+
+extern "C" size_t ak_linear_cross_entropy_ws_bytes_of(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, int bias_dtype, int64_t rows,
+                                                      int64_t classes, int64_t width, int gradients) {
+  if (ak_linear_cross_entropy_ws_bytes(dtype, rows, classes, width, 0) == 0) return 0;
+  return ak::lce_layout(h, dtype, ldh, w, ldw, bias_dtype >= 0 && bias_dtype != AK_F32, rows, classes, width, gradients != 0, (gradients & 1) != 0,
+                        (gradients & 2) != 0, (gradients & 4) != 0, nullptr).space.bytes;
 }
 
 extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype,
@@ -712,10 +742,9 @@ extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, co
   if (rc != AK_OK) return rc;
   if (rows == 0) return reduction == kLossNone ? AK_OK : AK_ERR_ARG;
   if (loss == nullptr || lse == nullptr) return AK_ERR_ARG;
-  const bool copy_h = dtype == AK_F32 || !hp_aligned(h, ldh, width), copy_w = dtype == AK_F32 || !hp_aligned(w, ldw, width);
-  const LcePlan p = lce_plan(dtype, rows, classes, width, false, copy_h || copy_w);
-  const LceSpace s = lce_space(p, false, !p.few && copy_h, !p.few && copy_w,
-                               bias != nullptr && bias_dtype != AK_F32, ws);
+  const LceLayout layout = lce_layout(h, dtype, ldh, w, ldw, bias != nullptr && bias_dtype != AK_F32, rows, classes, width, false, false, false, false, ws);
+  const LcePlan& p = layout.plan;
+  const LceSpace& s = layout.space;
   if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   LceCall c{h, ldh, w, ldw, bias, bias_dtype, LceRows{targets, nullptr, ignore_index, static_cast<int>(rows), static_cast<int>(classes)}, width, dtype, st};
@@ -742,16 +771,16 @@ extern "C" int ak_linear_cross_entropy_backward(const float* g, const void* h, i
   if (rc != AK_OK) return rc;
   if (g == nullptr || lse == nullptr || rows == 0) return AK_ERR_ARG;
   if (dh == nullptr && dw == nullptr && db == nullptr) return AK_OK;
-  const LcePlan p = lce_plan(dtype, rows, classes, width, true, true);
-  const bool split = dtype == AK_F32;
-  const LceSpace s = lce_space(p, true, split || !hp_aligned(h, ldh, width), split || !hp_aligned(w, ldw, width),
-                               bias != nullptr && bias_dtype != AK_F32, ws);
+  const LceLayout layout = lce_layout(h, dtype, ldh, w, ldw, bias != nullptr && bias_dtype != AK_F32, rows, classes, width, true, dh != nullptr, dw != nullptr,
+                                      db != nullptr, ws);
+  const LcePlan& p = layout.plan;
+  const LceSpace& s = layout.space;
   if (ws == nullptr || ws_bytes < s.bytes) return AK_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   LceCall c{h, ldh, w, ldw, bias, bias_dtype, LceRows{targets, nullptr, ignore_index, static_cast<int>(rows), static_cast<int>(classes)}, width, dtype, st};
   rc = lce_bias(c, p, s);
   if (rc != AK_OK) return rc;
-  hipLaunchKernelGGL(lce_shares_kernel, dim3(1), dim3(1024), 0, st, c.r, g, reduction, split ? 1 : 0, dtype == AK_F16 ? 14 : 0, s.share, s.unit);
+  hipLaunchKernelGGL(lce_shares_kernel, dim3(1), dim3(1024), 0, st, c.r, g, reduction, dtype == AK_F32 ? 1 : 0, dtype == AK_F16 ? 14 : 0, s.share, s.unit);
   const LceGrads out{dh, dw, db, bias == nullptr ? dtype : bias_dtype};
   return with_type(dtype, [&](auto t) { return lce_backward<typename decltype(t)::type>(c, lse, p, s, out); });
 }

@@ -1686,9 +1686,10 @@ def linear_cross_entropy(h, weight, targets, bias=None, ignore_index=-100, reduc
     weight, ldw = _rows_of(weight, D, _LOSS_PITCH)
     targets = _contiguous(targets)
     bias = None if bias is None else _contiguous(bias)
-    need = _ws_need('ak_linear_cross_entropy_ws_bytes', code, rows, classes, D, 0)
+    bias_code = -1 if bias is None else _ELEMENT_TYPES[bias.dtype]
+    need = _lib.load().ak_linear_cross_entropy_ws_bytes_of(h.data_ptr(), code, ldh, weight.data_ptr(), ldw, bias_code, rows, classes, D, 0)
     ws = empty(need, dtype=torch.uint8, device=device)         # (not workspace(): a graph that is captured has its own)
-    rc = _lib.load().ak_linear_cross_entropy(h.data_ptr(), code, ldh, weight.data_ptr(), ldw, _pointer(bias), code if bias is None else _ELEMENT_TYPES[bias.dtype],
+    rc = _lib.load().ak_linear_cross_entropy(h.data_ptr(), code, ldh, weight.data_ptr(), ldw, _pointer(bias), bias_code,
                                              targets.data_ptr(), rows, classes, D, ignore_index, kind, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), need,
                                              _stream_handle(device))
     _lib.check(rc, 'ak_linear_cross_entropy')
@@ -1731,10 +1732,12 @@ def linear_cross_entropy_backward(g, h, weight, targets, lse, bias=None, ignore_
     weight, ldw = _rows_of(weight, D, _LOSS_PITCH)
     targets, g, lse = _contiguous(targets), _contiguous(g), _contiguous(lse)
     bias = None if bias is None else _contiguous(bias)
-    need = _ws_need('ak_linear_cross_entropy_ws_bytes', code, rows, classes, D, 1)
+    bias_code = -1 if bias is None else _ELEMENT_TYPES[bias.dtype]
+    need = _lib.load().ak_linear_cross_entropy_ws_bytes_of(h.data_ptr(), code, ldh, weight.data_ptr(), ldw, bias_code, rows, classes, D,
+                                                           (dh is not None) + 2 * (dw is not None) + 4 * (db is not None))
     ws = empty(need, dtype=torch.uint8, device=device)
     rc = _lib.load().ak_linear_cross_entropy_backward(
-        g.data_ptr(), h.data_ptr(), code, ldh, weight.data_ptr(), ldw, _pointer(bias), code if bias is None else _ELEMENT_TYPES[bias.dtype],
+        g.data_ptr(), h.data_ptr(), code, ldh, weight.data_ptr(), ldw, _pointer(bias), bias_code,
         targets.data_ptr(), lse.data_ptr(), rows, classes, D, ignore_index, kind, _pointer(dh), _pointer(dw), _pointer(db), ws.data_ptr(), need,
         _stream_handle(device))
     _lib.check(rc, 'ak_linear_cross_entropy_backward')
@@ -1985,7 +1988,7 @@ def weight_grad_8bit(g, kept, need_weight=True, need_bias=True, dtype=None):
                     t.zero_()
         return dw, db
     g, ld = _rows_of(g, n, 1 << 24)
-    need = _ws_need('ak_weight_grad_8bit_ws_bytes', code, rows, F, n)
+    need = _lib.load().ak_weight_grad_8bit_ws_bytes_of(g.data_ptr(), code, ld, rows, F, n, (dw is not None) + 2 * (db is not None))
     ws = empty(need, dtype=torch.uint8, device=device)
     codes, exponents = kept if need_weight else (None, None)
     rc = _lib.load().ak_weight_grad_8bit(g.data_ptr(), code, ld, _pointer(codes), _pointer(exponents), rows, F, n, _pointer(dw), _pointer(db),

@@ -513,10 +513,20 @@ int ak_inv_root_group(int phases, int iters, int groups, float* const* S, const 
  * targets int64.  reduction 0: loss [rows]; 1: loss [1], their sum; 2: loss [1], their mean over the rows that are not ignored.  lse [rows]
  * is what the backward pass needs.  g: gradient of the loss, [rows] or [1]; dh [rows, width], dw [classes, width] (dense rows) of the
  * type of h, db [classes] of the bias's type; each may be null.  Sums and exponentials are fp32; 16-bit operands: the gradient
- * of the logits is rounded to their type.  The workspace (enough for either alignment; backward != 0: for the backward pass) holds a piece
- * of the logits' gradient of at most 512 MB, or 256 classes, and copies of 16-bit operands whose width is no multiple of eight or whose rows
- * are not 16-byte aligned.  rows, classes <= 2^28, width <= 2^20, row pitches <= 2^21, else AK_ERR_TOO_LARGE. */
+ * of the logits is rounded to their type.  Workspace, of
+ * copies    16-bit operands whose width is no multiple of eight or whose rows are not 16-byte aligned: (rows + classes) * width * 2 bytes, the width
+ *           rounded up to eight; fp32 operands, always, but for the loss of at most 64 rows: as three 16-bit pieces, three times that; a 16-bit bias
+ *           as fp32
+ * forward   a sum of 8 bytes for each row and 256, 128, 64 (the smaller the operands) or 16 (few rows) classes
+ * backward  a piece of the logits' gradient (fp32: in three 16-bit pieces) of at most 512 MB, or 256 classes of it; the fp32 sums of dh, rows * width * 4,
+ *           and of dw, min(classes, a piece's) * width * 4 where the sum over the rows is in parts, each times its parts (1 to 64 of
+ *           them: so many that the device is filled); 64 * classes of a piece * 4 for db (fp32: three times)
+ * ..._ws_bytes: enough for operands of any alignment and all gradients.  ..._ws_bytes_of: what a call with these addresses and pitches needs;
+ * bias_dtype -1 without a bias; gradients 0 for the loss, else the sum of 1 for dh, 2 for dw, 4 for db.
+ * rows, classes <= 2^28, width <= 2^20, row pitches <= 2^21, else AK_ERR_TOO_LARGE. */
 size_t ak_linear_cross_entropy_ws_bytes(int dtype, int64_t rows, int64_t classes, int64_t width, int backward);
+size_t ak_linear_cross_entropy_ws_bytes_of(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, int bias_dtype, int64_t rows, int64_t classes,
+                                           int64_t width, int gradients);
 int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype,
                             const int64_t* targets, int64_t rows, int64_t classes, int64_t width, int64_t ignore_index, int reduction,
                             float* loss, float* lse, void* ws, size_t ws_bytes, ak_stream_t stream);
@@ -543,12 +553,15 @@ int ak_embedding_backward(const void* g, int dtype, int64_t ldg, const void* tok
  * ak_dequantize_8bit, gelu -1: y (dense) = the kept values; 0 or 1: y = g * derivative of that function at the kept values.
  * ak_weight_grad_8bit: dw [out, width] = g^T x', db [out] = sums of g over the rows, x' the kept values; each may be null, g [rows, out].
  * Without dw, codes and exponents may be null and width 0, also for the bytes of the workspace.  The products of g's pieces with x' are exact,
- * their sums fp32. */
+ * their sums fp32.  Workspace: x' as bf16; g as bf16 pieces (fp16: two, fp32: three), or copied where it is bf16 and its width no multiple of eight or its
+ * rows not 16-byte aligned; fp32 sums of dw where the sum over the rows is in parts, and of db.  ..._ws_bytes: enough for any alignment and both
+ * gradients; ..._ws_bytes_of: what a call with this address and pitch needs, gradients the sum of 1 for dw and 2 for db. */
 int ak_quantize_8bit(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t width, int gelu, void* y, uint8_t* codes, int8_t* exponents,
                      ak_stream_t stream);
 int ak_dequantize_8bit(const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width, int gelu, const void* g, int64_t ldg,
                        void* y, int dtype, ak_stream_t stream);
 size_t ak_weight_grad_8bit_ws_bytes(int dtype, int64_t rows, int64_t width, int64_t out);
+size_t ak_weight_grad_8bit_ws_bytes_of(const void* g, int dtype, int64_t ldg, int64_t rows, int64_t width, int64_t out, int gradients);
 int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const uint8_t* codes, const int8_t* exponents, int64_t rows, int64_t width,
                         int64_t out, void* dw, void* db, int grad_dtype, void* ws, size_t ws_bytes, ak_stream_t stream);
 

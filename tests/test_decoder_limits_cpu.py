@@ -90,3 +90,51 @@ def test_nothing_is_kept_where_nothing_goes_back(stand):     # noqa: F811
     model.requires_grad_(False)
     model(x.detach())
     assert kept() == 0
+
+
+# ------------------------------------------------------------------------------------------------ workspaces
+def test_workspaces_hold_what_a_call_makes():
+    """No copies of operands that are read where they lie, no sums of gradients that are not asked for; never more than the query for any operands."""
+    from asdl_amd import _lib
+    lib = _lib.load()
+    F32, BF16, F16 = 0, 1, 4
+    even, odd = 4096, 4098                       # stand for addresses
+
+    def loss(dtype, rows, classes, width, gradients, h=even, w=even, pitch=None, bias=-1):
+        return lib.ak_linear_cross_entropy_ws_bytes_of(h, dtype, pitch or width, w, pitch or width, bias, rows, classes, width, gradients)
+    for dtype in (F32, BF16, F16):
+        for rows in (1, 8, 9, 16, 17, 64, 65, 500, 8192):
+            for classes in (1, 300, 50257, 1 << 25):
+                for width in (1, 8, 151, 768):
+                    if rows * classes > 1 << 32:
+                        continue
+                    for kw in (dict(), dict(h=odd), dict(w=odd), dict(pitch=width + 1), dict(bias=dtype)):
+                        assert 0 < loss(dtype, rows, classes, width, 0, **kw) <= lib.ak_linear_cross_entropy_ws_bytes(dtype, rows, classes, width, 0)
+                        whole = loss(dtype, rows, classes, width, 7, **kw)
+                        assert whole <= lib.ak_linear_cross_entropy_ws_bytes(dtype, rows, classes, width, 1)
+                        assert all(0 < loss(dtype, rows, classes, width, bits, **kw) <= whole for bits in range(1, 7))
+    # the operands of 4096 x 128000 x 2048: 541 MB
+    copies = (4096 + 128000) * 2048 * 2
+    assert loss(F16, 4096, 128000, 2048, 0) < 40e6 and loss(F16, 4096, 128000, 2048, 0, h=odd, w=odd) - loss(F16, 4096, 128000, 2048, 0) == copies
+    assert loss(F16, 4096, 128000, 2048, 7, h=odd, w=odd) - loss(F16, 4096, 128000, 2048, 7) == copies
+    assert loss(F16, 4096, 128000, 2048, 7) - loss(F16, 4096, 128000, 2048, 6) >= 4096 * 2048 * 4
+    assert loss(F32, 4096, 128000, 2048, 7) > 3 * copies and loss(9, 8, 8, 8, 0) == loss(BF16, 0, 8, 8, 0) == loss(BF16, 8, 8, 1 << 21, 0) == 0
+
+    def weight(dtype, rows, width, out, gradients=3, g=even, pitch=None):
+        return lib.ak_weight_grad_8bit_ws_bytes_of(g, dtype, pitch or out, rows, width, out, gradients)
+    for dtype in (F32, BF16, F16):
+        for rows, width, out in ((1, 1, 1), (40, 33, 70), (8192, 768, 2304), (16384, 4096, 4096)):
+            for kw in (dict(), dict(g=odd), dict(pitch=out + 3), dict(gradients=1), dict(gradients=2)):
+                assert 0 < weight(dtype, rows, width, out, **kw) <= lib.ak_weight_grad_8bit_ws_bytes(dtype, rows, width, out)
+    assert weight(BF16, 16384, 4096, 4096, g=odd) - weight(BF16, 16384, 4096, 4096) == 16384 * 4096 * 2
+    assert weight(BF16, 16384, 4096, 4096) < 16384 * 4096 * 2 + 3e6 and weight(BF16, 16384, 4096, 4096, 2) < 3e6 and weight(9, 4, 4, 4) == weight(BF16, 0, 4, 4) == 0
+
+    # the entry points ask for no more and no less (the call itself is not made: a byte is missing)
+    a = even
+    need = loss(BF16, 8192, 50257, 768, 0)
+    assert lib.ak_linear_cross_entropy(a, BF16, 768, a, 768, None, -1, a, 8192, 50257, 768, -100, 2, a, a, a, need - 1, None) == -2
+    for bits in (1, 2, 3, 7):
+        need = loss(BF16, 8192, 50257, 768, bits, bias=BF16)
+        out = [a if bits & b else None for b in (1, 2, 4)]
+        assert lib.ak_linear_cross_entropy_backward(a, a, BF16, 768, a, 768, a, BF16, a, a, 8192, 50257, 768, -100, 2, *out, a, need - 1, None) == -2
+    assert lib.ak_weight_grad_8bit(a, BF16, 4096, a, a, 16384, 4096, 4096, a, a, BF16, a, weight(BF16, 16384, 4096, 4096) - 1, None) == -2

@@ -75,3 +75,32 @@ def test_weight_gradients_of_rows_far_apart(K):     # noqa: F811
     g = rand(40, (1 << 24) + 8, seed=1, dtype=BF16)[:, 5:29]
     kept = K.quantize_8bit(rand(40, 72, seed=2, dtype=BF16))
     assert all(torch.equal(a, b) for a, b in zip(K.weight_grad_8bit(g, kept), K.weight_grad_8bit(g.contiguous(), kept)))
+
+
+def test_memory_of_a_decoders_loss(K):     # noqa: F811
+    """8192 x 768 x 50257: no copies of the operands (90 MB), and nothing for a gradient that is not asked for."""
+    h, w, t = rand(8192, 768, seed=1, dtype=BF16), rand(50257, 768, seed=2, dtype=BF16, scale=0.03), ints(50257, 8192, seed=3)
+
+    def peak(call):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = call()
+        return out, torch.cuda.max_memory_allocated() - before
+    (loss, lse), used = peak(lambda: K.linear_cross_entropy(h, w, t))
+    assert used < 20e6                            # (8 bytes for a row and 256 classes: 13 MB)
+    piece, results, sums = 8192 * 25344 * 2, (8192 + 50257) * 768 * 2, 8192 * 768 * 4
+    g = torch.ones_like(loss)
+    for at in (h, torch.cat([h, h[:, :8]], 1)[:, :768]):          # (in one step, and by Python's way)
+        _, used = peak(lambda: K.linear_cross_entropy_backward(g, at, w, t, lse))
+        # (the sum over a piece's 25344 classes is in six parts: the query says 566.3 MB with dh, 415.3 MB without, which is 6 * 25.2 MB)
+        assert used < piece + results + 6 * sums + 3e6
+        _, used = peak(lambda: K.linear_cross_entropy_backward(g, at, w, t, lse, need_h=False))
+        assert used < piece + 50257 * 768 * 2 + 3e6
+    g = rand(8192, 2304, seed=4, dtype=BF16)
+    kept = K.quantize_8bit(h)
+    for at in (g, torch.cat([g, g[:, :8]], 1)[:, :2304]):
+        _, used = peak(lambda: K.weight_grad_8bit(at, kept))
+        assert used < 8192 * 768 * 2 + 4 * 2304 * 768 * 4 + 2304 * 768 * 2 + 2e6          # (the input, four parts of the sum, the result)
+        _, used = peak(lambda: K.weight_grad_8bit(at, kept, need_weight=False))
+        assert used < 2e6
