@@ -329,6 +329,9 @@ size_t conv_window_f32_ws_bytes(int64_t N, int64_t C, int64_t H, int64_t W, int 
 int conv_window_syrk_f32(const float* x, int64_t N, int64_t C, int64_t H, int64_t W, int kh, int kw, int sh, int sw, int ph, int pw, float alpha,
                          float beta, float* A, int64_t lda, void* ws, size_t ws_bytes, hipStream_t stream);
 
+// The threads of a launch are counted in 32 bits: a grid with more loses its last work groups without an error.
+inline bool fits_a_launch(int64_t groups, int64_t threads) { return groups * threads < (1ll << 32); }
+
 inline int check_launch() { return hipGetLastError() == hipSuccess ? AK_OK : AK_ERR_LAUNCH; }
 
 // Split-K factor shared by the SYRK front ends: enough work groups to fill 256 CUs twice over

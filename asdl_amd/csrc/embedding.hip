@@ -472,11 +472,14 @@ extern "C" int ak_embedding(const void* tokens, int token_type, int64_t count, c
       using O = typename decltype(o)::type;
       return with_tokens(token_type, [&](auto i) {
         using I = typename decltype(i)::type;
-        const Tokens<I> tk{static_cast<const I*>(tokens), count, static_cast<int>(rows), -1};
         auto launch = [&](auto lanes) {
           constexpr int L = decltype(lanes)::value;
-          hipLaunchKernelGGL((emb_rows_kernel<T, O, I, L>), dim3(static_cast<unsigned>((count + 256 / L - 1) / (256 / L))), dim3(256), 0, s, tk,
-                             static_cast<const T*>(table), ld, static_cast<int>(width), scale, static_cast<O*>(out));
+          constexpr int64_t kMost = 1ll << 25;       // tokens of a launch: 2^31 threads of 64 a token
+          for (int64_t n = 0; n < count; n += kMost) {
+            const Tokens<I> tk{static_cast<const I*>(tokens) + n, std::min(count - n, kMost), static_cast<int>(rows), -1};
+            hipLaunchKernelGGL((emb_rows_kernel<T, O, I, L>), dim3(static_cast<unsigned>((tk.count + 256 / L - 1) / (256 / L))), dim3(256), 0, s, tk,
+                               static_cast<const T*>(table), ld, static_cast<int>(width), scale, static_cast<O*>(out) + n * width);
+          }
           return check_launch();
         };
         // as many lanes as a row has vectors, 8 to 64
@@ -534,17 +537,17 @@ extern "C" int ak_embedding_backward(const void* g, int dtype, int64_t ldg, cons
   p.rows_of = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(64, rows / 8192)));
   p.scale = scale; p.beta = beta;
   const int64_t units = static_cast<int64_t>(p.chunks) * p.slabs + (rows + p.rows_of - 1) / p.rows_of;
-  if ((units + 3) / 4 > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  if (!fits_a_launch((units + 3) / 4, 256)) return AK_ERR_TOO_LARGE;
   return with_type(out_dtype, [&](auto o) {
     using O = typename decltype(o)::type;
+    const int64_t column_blocks = (width + 255) / 256, longs = (p.chunks + kEmbLong - 1) / kEmbLong * column_blocks, shorts = (p.chunks * column_blocks + 3) / 4;
+    if (!fits_a_launch(longs + shorts, 256)) return AK_ERR_TOO_LARGE;
     const int done = with_type(dtype, [&](auto t) {
       using G = typename decltype(t)::type;
       hipLaunchKernelGGL((emb_sums_kernel<G, O>), dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, st, p);
       return check_launch();
     });
     if (done != AK_OK || p.chunks < 2) return done;
-    const int64_t column_blocks = (width + 255) / 256, longs = (p.chunks + kEmbLong - 1) / kEmbLong * column_blocks, shorts = (p.chunks * column_blocks + 3) / 4;
-    if (longs + shorts > 0x7fffffff) return AK_ERR_TOO_LARGE;
     hipLaunchKernelGGL(emb_joins_kernel<O>, dim3(static_cast<unsigned>(longs + shorts)), dim3(256), 0, st, p, static_cast<int>(longs),
                        static_cast<int>(column_blocks));
     return check_launch();

@@ -648,7 +648,7 @@ template <class Cfg, typename E, class Epilogue>
 inline int hp_launch(const HpProblem& p, const typename Epilogue::Params& e, hipStream_t stream) {
   const int64_t blocks = hp_blocks(p);
   if (blocks <= 0) return AK_OK;
-  if (blocks > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  if (!fits_a_launch(blocks, Cfg::THREADS)) return AK_ERR_TOO_LARGE;
   auto kernel = hp_kernel<Cfg, E, Epilogue>;
   static std::atomic<uint64_t> known{0};
   const int rc = hp_ask_lds(kernel, Cfg::LDS_ALL, known);
@@ -662,7 +662,7 @@ template <class Cfg1, class Epilogue1, class Cfg2, class Epilogue2, typename E>
 inline int hp_launch_both(const HpProblem& p1, const typename Epilogue1::Params& e1, const HpProblem& p2, const typename Epilogue2::Params& e2,
                           hipStream_t stream) {
   const int64_t b1 = hp_blocks(p1), b2 = hp_blocks(p2);
-  if (b1 + b2 > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  if (!fits_a_launch(b1 + b2, Cfg1::THREADS)) return AK_ERR_TOO_LARGE;
   auto kernel = hp_both_kernel<Cfg1, Epilogue1, Cfg2, Epilogue2, E>;
   static std::atomic<uint64_t> known{0};
   const int rc = hp_ask_lds(kernel, Cfg1::LDS_ALL, known);

@@ -252,12 +252,12 @@ static __global__ __launch_bounds__(256) void keep_back_kernel(Keep p, int64_t l
 // What a weight gradient's product needs: the kept values as bfloat16, and the chunks of g's column sums, by work groups behind them.
 // (This and the totals in one launch, where each had its own: the bias's gradient of 2304 outputs from 8192 rows 10.5 -> 1.7 us.)
 template <typename T>
-static __global__ __launch_bounds__(256) void keep_prepare_kernel(Keep p, int64_t ldx, uint32_t front, const T* __restrict__ g, int64_t ldg, int64_t cols,
-                                                                  int64_t rows_per_chunk, float* __restrict__ part) {
+static __global__ __launch_bounds__(256) void keep_prepare_kernel(Keep p, int64_t ldx, uint32_t front, const T* __restrict__ g, int64_t ldg, int64_t rows,
+                                                                  int64_t cols, int64_t rows_per_chunk, float* __restrict__ part) {
   __shared__ float joined[8][kColumnsPerGroup];
   if (blockIdx.x < front) return keep_back<__bf16, -1>(p, ldx, static_cast<int>(ldx));
   const uint32_t at = blockIdx.x - front, groups = static_cast<uint32_t>((cols + kColumnsPerGroup - 1) / kColumnsPerGroup);
-  column_chunk(g, ldg, p.rows, cols, rows_per_chunk, part, at % groups, at / groups, joined);
+  column_chunk(g, ldg, rows, cols, rows_per_chunk, part, at % groups, at / groups, joined);
 }
 
 // The totals of the splits' sums and, by work groups behind them, of the columns' chunks.
@@ -310,13 +310,30 @@ inline KeepSpace keep_space(const KeepPlan& p, int64_t rows, int64_t out, bool w
 
 inline int keep_check(int dtype, int64_t ld, int64_t rows, int64_t F) {
   if (!is_element_type(dtype) || rows < 0 || F <= 0 || ld < F) return AK_ERR_ARG;
-  // blocks in 32 bits, and a launch's work groups
   if (F > (1ll << 24) || rows > (1ll << 31) || rows * ((F + kKeepBlock - 1) / kKeepBlock) > (1ll << 34)) return AK_ERR_TOO_LARGE;
   return AK_OK;
 }
 
 inline dim3 keep_grid(const Keep& p) {
   return dim3(static_cast<unsigned>((p.rows * p.blocks + 256 / kKeepLanes - 1) / (256 / kKeepLanes)));
+}
+
+// launch(a piece of the rows) for all of them, in pieces of 2^27 blocks, 2^31 threads; x and y: bytes of an element, ldy: pitch of y.
+// The last piece is left to the caller.
+template <typename F>
+inline Keep keep_pieces(Keep p, int64_t x, int64_t y, int64_t ldy, F&& launch) {
+  const int64_t most = (1ll << 27) / p.blocks;             // (at most 2^17 blocks a row)
+  while (p.rows > most) {
+    Keep piece = p;
+    piece.rows = most;
+    launch(piece);
+    if (p.x != nullptr) p.x = static_cast<const char*>(p.x) + most * p.ldx * x;
+    if (p.y != nullptr) p.y = static_cast<char*>(p.y) + most * ldy * y;
+    p.codes += most * p.F;
+    p.exponents += most * p.blocks;
+    p.rows -= most;
+  }
+  return p;
 }
 
 }  // namespace ak
@@ -333,9 +350,12 @@ extern "C" int ak_quantize_8bit(const void* x, int dtype, int64_t ldx, int64_t r
   return with_type(dtype, [&](auto t) {
     using T = typename decltype(t)::type;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (gelu == kGeluExact) hipLaunchKernelGGL((keep_kernel<T, kGeluExact>), keep_grid(p), dim3(256), 0, s, p);
-    else if (gelu == kGeluTanh) hipLaunchKernelGGL((keep_kernel<T, kGeluTanh>), keep_grid(p), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((keep_kernel<T, -1>), keep_grid(p), dim3(256), 0, s, p);
+    auto launch = [&](const Keep& q) {
+      if (gelu == kGeluExact) hipLaunchKernelGGL((keep_kernel<T, kGeluExact>), keep_grid(q), dim3(256), 0, s, q);
+      else if (gelu == kGeluTanh) hipLaunchKernelGGL((keep_kernel<T, kGeluTanh>), keep_grid(q), dim3(256), 0, s, q);
+      else hipLaunchKernelGGL((keep_kernel<T, -1>), keep_grid(q), dim3(256), 0, s, q);
+    };
+    launch(keep_pieces(p, sizeof(T), sizeof(T), width, launch));
     return check_launch();
   });
 }
@@ -353,9 +373,12 @@ extern "C" int ak_dequantize_8bit(const uint8_t* codes, const int8_t* exponents,
   return with_type(dtype, [&](auto t) {
     using T = typename decltype(t)::type;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (gelu == kGeluExact) hipLaunchKernelGGL((keep_back_kernel<T, kGeluExact>), keep_grid(p), dim3(256), 0, s, p, width, F);
-    else if (gelu == kGeluTanh) hipLaunchKernelGGL((keep_back_kernel<T, kGeluTanh>), keep_grid(p), dim3(256), 0, s, p, width, F);
-    else hipLaunchKernelGGL((keep_back_kernel<T, -1>), keep_grid(p), dim3(256), 0, s, p, width, F);
+    auto launch = [&](const Keep& q) {
+      if (gelu == kGeluExact) hipLaunchKernelGGL((keep_back_kernel<T, kGeluExact>), keep_grid(q), dim3(256), 0, s, q, width, F);
+      else if (gelu == kGeluTanh) hipLaunchKernelGGL((keep_back_kernel<T, kGeluTanh>), keep_grid(q), dim3(256), 0, s, q, width, F);
+      else hipLaunchKernelGGL((keep_back_kernel<T, -1>), keep_grid(q), dim3(256), 0, s, q, width, F);
+    };
+    launch(keep_pieces(p, sizeof(T), sizeof(T), width, launch));
     return check_launch();
   });
 }
@@ -394,13 +417,16 @@ extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const 
         return column_sums(static_cast<const T*>(g), ldg, rows, out, 1.f, nullptr, static_cast<O*>(db), s.columns, st);
       });
     });
-  const Keep k{nullptr, s.x, const_cast<uint8_t*>(codes), const_cast<int8_t*>(exponents), 0, rows, F, (F + kKeepBlock - 1) / kKeepBlock};
-  const int64_t front = (rows * k.blocks + 256 / kKeepLanes - 1) / (256 / kKeepLanes), behind = db != nullptr ? chunks * ((out + kColumnsPerGroup - 1) / kColumnsPerGroup) : 0;
-  if (front + behind > 0x7fffffff) return AK_ERR_TOO_LARGE;
+  const Keep all{nullptr, s.x, const_cast<uint8_t*>(codes), const_cast<int8_t*>(exponents), 0, rows, F, (F + kKeepBlock - 1) / kKeepBlock};
+  const Keep k = keep_pieces(all, 0, sizeof(__bf16), plan.ldf, [&](const Keep& q) {
+    hipLaunchKernelGGL((keep_back_kernel<__bf16, -1>), keep_grid(q), dim3(256), 0, st, q, plan.ldf, static_cast<int>(plan.ldf));
+  });
+  const unsigned front = keep_grid(k).x;
+  const int64_t behind = db != nullptr ? chunks * ((out + kColumnsPerGroup - 1) / kColumnsPerGroup) : 0;         // (at most 2^18: fits the launch)
   with_type(dtype, [&](auto t) {
     using T = typename decltype(t)::type;
-    hipLaunchKernelGGL(keep_prepare_kernel<T>, dim3(static_cast<unsigned>(front + behind)), dim3(256), 0, st, k, plan.ldf, static_cast<uint32_t>(front),
-                       static_cast<const T*>(g), ldg, out, (rows + chunks - 1) / chunks, s.columns);
+    hipLaunchKernelGGL(keep_prepare_kernel<T>, dim3(front + static_cast<unsigned>(behind)), dim3(256), 0, st, k, plan.ldf, front, static_cast<const T*>(g), ldg,
+                       rows, out, (rows + chunks - 1) / chunks, s.columns);
     return AK_OK;
   });
   const __bf16* from = static_cast<const __bf16*>(g);

@@ -451,6 +451,8 @@ constexpr int64_t kLcePieceBytes = 512ll << 20;       // of d
 // without 25 us, 120757 x 461 80 us either way for 17 rows; fp32 55 us for up to 16, 87 us for 32 and 135 us for 64 rows, by the tiles 172 us.)
 inline int64_t lce_few_rows(int dtype, bool copied) { return dtype == AK_F32 ? 64 : copied ? 16 : 8; }
 
+constexpr int64_t kLcePartBytes = 512ll << 20;        // of the forward pass's sums of tiles
+
 // Sizes that both the workspace query and the launches use.
 constexpr int64_t kLceSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
 constexpr double kLceSumUs = 6. / 4.5e6;                  // of an element of a split's sum
@@ -459,6 +461,7 @@ struct LcePlan {
   int64_t N, V, D;
   int k;                   // 16-bit pieces of a value
   bool few;                // the forward pass of few rows
+  int64_t part, rows;      // classes of a part of the forward pass; rows that it takes at a time
   int64_t piece, pieces;   // classes of a piece, a multiple of 256 (the last may have fewer)
   int64_t ldp;             // row pitch of padded operands
   bool wide;               // tiles of 256 in the gradients' products
@@ -471,6 +474,9 @@ inline LcePlan lce_plan(int dtype, int64_t N, int64_t V, int64_t D, bool backwar
   p.N = N; p.V = V; p.D = D;
   p.k = dtype == AK_F32 ? 3 : 1;
   p.few = !backward && N <= lce_few_rows(dtype, copied);
+  p.part = p.few ? 16 : hp_wide(V, N) ? 256 : hp_tiny(V, N) ? 64 : 128;
+  // (at least 256 rows: 2^20 tiles at most, far from the 2^23 whose threads 32 bits count)
+  p.rows = std::min(N, std::max<int64_t>(kLcePartBytes / (((V + p.part - 1) / p.part) * static_cast<int64_t>(sizeof(float) * 2)) / 256 * 256, 256));
   // (at most 2^24: 32 rows of d within 32-bit byte offsets)
   const int64_t fit = std::min<int64_t>(std::max<int64_t>(kLcePieceBytes / (N * p.k * 2) / 256 * 256, 256), 1 << 24);
   p.pieces = (V + fit - 1) / fit;
@@ -541,9 +547,8 @@ inline LceSpace lce_space(const LcePlan& p, bool backward, const LceNeeds& need,
   if (need.w) s.w = c.take<unsigned char>(p.V * p.ldp * p.k * 2);
   if (need.bias) s.bias = c.take<float>(p.V);
   if (!backward) {
-    const int64_t tile = p.few ? 16 : hp_wide(p.V, p.N) ? 256 : hp_tiny(p.V, p.N) ? 64 : 128;      // classes of a part
-    s.part = c.take<floatx2>((p.V + tile - 1) / tile * p.N);
-    s.at_target = c.take<float>(p.N);
+    s.part = c.take<floatx2>((p.V + p.part - 1) / p.part * p.rows);
+    s.at_target = c.take<float>(p.rows);
     s.losses = c.take<float>(p.N);
   } else {
     s.share = c.take<float>(p.N);
@@ -598,14 +603,15 @@ inline int lce_bias(LceCall& c, const LcePlan& p, const LceSpace& s) {
   });
 }
 
+// losses and lse of all rows
 template <typename E>
-inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, int* parts) {
+inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, float* losses, float* lse) {
   if (p.few) {
     const int64_t groups = (p.V + 15) / 16;
-    *parts = static_cast<int>(groups);
     auto go = [&](auto nb) {
       hipLaunchKernelGGL((lce_few_kernel<E, decltype(nb)::value>), dim3(static_cast<unsigned>(groups)), dim3(64), 0, c.stream, static_cast<const E*>(c.h),
                          c.ldh, static_cast<const E*>(c.w), c.ldw, static_cast<int>(p.D), c.r, s.part, s.at_target);
+      hipLaunchKernelGGL(lce_row_kernel, dim3(static_cast<unsigned>(p.N)), dim3(512), 0, c.stream, c.r, s.part, static_cast<int>(groups), s.at_target, losses, lse);
       return check_launch();
     };
     if constexpr (__is_same(E, float)) {
@@ -618,15 +624,26 @@ inline int lce_forward(LceCall c, const LcePlan& p, const LceSpace& s, int* part
   if (rc != AK_OK) return rc;
   using M = typename LceKind<E>::type;
   constexpr bool PIECES = LceKind<E>::pieces > 1;
-  const HpOperand A = hp_operand(c.w, c.ldw, p.V, p.D, true), B = hp_operand(c.h, c.ldh, p.N, p.D, true);
-  auto go = [&](auto cfg) {
-    using Cfg = decltype(cfg);
-    HpProblem q = hp_problem<Cfg>(A, B, p.V, p.N, align_up(p.D, 8));
-    if (PIECES) q.pieces = hp_six(p.ldp, p.ldp);
-    *parts = q.tiles_i;
-    return hp_launch<Cfg, M, LceStats>(q, LceStats::Params{c.r, s.part, s.at_target}, c.stream);
-  };
-  return hp_form<true, true, PIECES>(p.V, p.N, go);
+  const HpOperand A = hp_operand(c.w, c.ldw, p.V, p.D, true);
+  for (int64_t n = 0; n < p.N; n += p.rows) {
+    LceRows r = c.r;
+    r.targets += n;
+    r.rows = static_cast<int>(std::min(p.N - n, p.rows));
+    const HpOperand B = hp_operand(static_cast<const M*>(c.h) + n * c.ldh, c.ldh, r.rows, p.D, true);
+    auto go = [&](auto cfg) {
+      using Cfg = decltype(cfg);
+      HpProblem q = hp_problem<Cfg>(A, B, p.V, r.rows, align_up(p.D, 8));
+      if (PIECES) q.pieces = hp_six(p.ldp, p.ldp);
+      const int done = hp_launch<Cfg, M, LceStats>(q, LceStats::Params{r, s.part, s.at_target}, c.stream);
+      if (done != AK_OK) return done;
+      hipLaunchKernelGGL(lce_rows_kernel, dim3(static_cast<unsigned>((r.rows + 63) / 64)), dim3(1024), 0, c.stream, r, s.part, q.tiles_i, s.at_target, losses + n,
+                         lse + n);
+      return check_launch();
+    };
+    const int done = hp_form<true, true, PIECES>(p.V, p.N, go);
+    if (done != AK_OK) return done;
+  }
+  return AK_OK;
 }
 
 struct LceGrads {
@@ -750,14 +767,9 @@ extern "C" int ak_linear_cross_entropy(const void* h, int dtype, int64_t ldh, co
   LceCall c{h, ldh, w, ldw, bias, bias_dtype, LceRows{targets, nullptr, ignore_index, static_cast<int>(rows), static_cast<int>(classes)}, width, dtype, st};
   rc = lce_bias(c, p, s);
   if (rc != AK_OK) return rc;
-  int parts = 0;
-  rc = with_type(dtype, [&](auto t) { return lce_forward<typename decltype(t)::type>(c, p, s, &parts); });
-  if (rc != AK_OK) return rc;
   float* losses = reduction == kLossNone ? loss : s.losses;
-  if (p.few)
-    hipLaunchKernelGGL(lce_row_kernel, dim3(static_cast<unsigned>(rows)), dim3(512), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
-  else
-    hipLaunchKernelGGL(lce_rows_kernel, dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(1024), 0, st, c.r, s.part, parts, s.at_target, losses, lse);
+  rc = with_type(dtype, [&](auto t) { return lce_forward<typename decltype(t)::type>(c, p, s, losses, lse); });
+  if (rc != AK_OK) return rc;
   if (reduction != kLossNone) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, c.r, losses, reduction, loss);
   return check_launch();
 }

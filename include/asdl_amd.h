@@ -517,7 +517,8 @@ int ak_inv_root_group(int phases, int iters, int groups, float* const* S, const 
  * copies    16-bit operands whose width is no multiple of eight or whose rows are not 16-byte aligned: (rows + classes) * width * 2 bytes, the width
  *           rounded up to eight; fp32 operands, always, but for the loss of at most 64 rows: as three 16-bit pieces, three times that; a 16-bit bias
  *           as fp32
- * forward   a sum of 8 bytes for each row and 256, 128, 64 (the smaller the operands) or 16 (few rows) classes
+ * forward   a sum of 8 bytes for each row and 256, 128, 64 (the smaller the operands) or 16 (few rows) classes, of so many rows at a time that this
+ *           takes at most 512 MB (or of 256)
  * backward  a piece of the logits' gradient (fp32: in three 16-bit pieces) of at most 512 MB, or 256 classes of it; the fp32 sums of dh, rows * width * 4,
  *           and of dw, min(classes, a piece's) * width * 4 where the sum over the rows is in parts, each times its parts (1 to 64 of
  *           them: so many that the device is filled); 64 * classes of a piece * 4 for db (fp32: three times)

@@ -104,3 +104,57 @@ def test_memory_of_a_decoders_loss(K):     # noqa: F811
         assert used < 8192 * 768 * 2 + 4 * 2304 * 768 * 4 + 2304 * 768 * 2 + 2e6          # (the input, four parts of the sum, the result)
         _, used = peak(lambda: K.weight_grad_8bit(at, kept, need_weight=False))
         assert used < 2e6
+
+
+# ------------------------------------------------------------------------------------------------ launches of 2^32 threads and more
+def test_linear_cross_entropy_of_more_tiles_than_a_launch_takes(K):     # noqa: F811
+    """2^23 tiles of 512 threads and more: rows at both ends, and the sum of all."""
+    rows, classes, width = (1 << 22) + 1000, (1 << 17) + 300, 8
+    print(f'linear_cross_entropy {rows}x{classes}x{width}', flush=True)
+    h, w = rand(rows, width, seed=1, dtype=BF16), rand(classes, width, seed=2, dtype=BF16, scale=0.3)
+    t, at = ints(classes, rows, seed=3), torch.cat([torch.arange(300, device='cuda'), rows - 300 + torch.arange(300, device='cuda')])
+    loss, lse = K.linear_cross_entropy(h, w, t, reduction='none')
+    want = loss64(h[at], w, t[at], reduction='none')
+    within(lse[at], *want['lse'], 'lse')
+    within(loss[at], *want['loss'], 'loss')
+    total = loss.double().sum()
+    within(K.linear_cross_entropy(h, w, t, reduction='sum')[0], total, 2 * U * total, 'sum')
+
+
+def test_activations_of_more_blocks_than_a_launch_takes(K):     # noqa: F811
+    """Rows of one feature, 16 threads each."""
+    rows = (1 << 28) + 1000
+    print(f'quantize_8bit {rows}x1', flush=True)
+    at = torch.cat([torch.arange(700, device='cuda'), (1 << 27) - 300 + torch.arange(700, device='cuda'), rows - 700 + torch.arange(700, device='cuda')])
+    x = torch.zeros(rows, 1, device='cuda', dtype=BF16)
+    x[at] = rand(len(at), 1, seed=1, dtype=BF16)
+    kept, few = K.quantize_8bit(x), K.quantize_8bit(x[at])
+    rest = torch.ones(rows, dtype=torch.bool, device='cuda')
+    rest[at] = False
+    assert torch.equal(kept.codes.view(torch.uint8)[at], few.codes.view(torch.uint8)) and torch.equal(kept.exponents[at], few.exponents)
+    assert bool((kept.codes.view(torch.uint8)[rest] == 0).all()) and bool((kept.exponents[rest] == -127).all())
+    values = K.dequantize_8bit(kept, BF16)
+    assert torch.equal(values[at], K.dequantize_8bit(few, BF16)) and bool((values[rest] == 0).all())
+    y, also = K.gelu_8bit(x)
+    assert torch.equal(y[at], K.gelu_8bit(x[at])[0]) and bool((y[rest] == 0).all()) and torch.equal(also.exponents, kept.exponents)
+    back = K.gelu_8bit_backward(y, kept)
+    assert torch.equal(back[at], K.gelu_8bit_backward(y[at], few)) and bool((back[rest] == 0).all())
+    del y, also, back, values
+    g = torch.zeros(rows, 3, device='cuda', dtype=BF16)
+    g[at] = rand(len(at), 3, seed=2, dtype=BF16)
+    dw, db = K.weight_grad_8bit(g, kept, dtype=F32)
+    values, gd = K.dequantize_8bit(few).double(), g[at].double()
+    # (the other rows add zeros)
+    within(dw, gd.t() @ values, 2 * (len(at) + 8) * U * (gd.abs().t() @ values.abs()), 'dw')
+    within(db, gd.sum(0), (len(at) + 8) * U * gd.abs().sum(0), 'db')
+
+
+def test_embedding_of_more_tokens_than_a_launch_takes(K):     # noqa: F811
+    """Rows of one feature, eight threads each."""
+    tokens = (1 << 29) + 1000
+    print(f'embedding of {tokens} tokens', flush=True)
+    table = rand(7, 1, seed=1, dtype=BF16)
+    t = torch.arange(tokens, device='cuda', dtype=torch.int32).remainder_(7)
+    y = K.embedding(t, table)
+    for i in range(7):
+        assert bool((y[i::7] == table[i]).all())
