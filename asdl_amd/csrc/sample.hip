@@ -79,12 +79,17 @@ extern "C" int ak_sample_categorical(const float* logits, const float* q, int64_
   if (logits == nullptr || q == nullptr || targets == nullptr || rows <= 0 || classes <= 0) return AK_ERR_ARG;
   if (classes > (1 << 30) || rows > 0x7fffffff) return AK_ERR_TOO_LARGE;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  // a wave covers 256 classes per step of four: up to 1024 classes one wave per row leaves no lane idle for long
-  if (classes <= 1024)
-    hipLaunchKernelGGL(ak::sample_categorical_kernel<1>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, logits,
-                       q, rows, static_cast<int>(classes), targets, invalid);
-  else
-    hipLaunchKernelGGL(ak::sample_categorical_kernel<4>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, logits, q, rows,
-                       static_cast<int>(classes), targets, invalid);
+  // (a launch's threads are counted in 32 bits: so many rows at a time that they are 2^31 at most)
+  const int64_t most = classes <= 1024 ? 1 << 25 : 1 << 23;
+  for (int64_t n = 0; n < rows; n += most) {
+    const int64_t some = rows - n < most ? rows - n : most;
+    // a wave covers 256 classes per step of four: up to 1024 classes one wave per row leaves no lane idle for long
+    if (classes <= 1024)
+      hipLaunchKernelGGL(ak::sample_categorical_kernel<1>, dim3(static_cast<unsigned>((some + 3) / 4)), dim3(256), 0, s, logits + n * classes,
+                         q + n * classes, some, static_cast<int>(classes), targets + n, invalid);
+    else
+      hipLaunchKernelGGL(ak::sample_categorical_kernel<4>, dim3(static_cast<unsigned>(some)), dim3(256), 0, s, logits + n * classes, q + n * classes, some,
+                         static_cast<int>(classes), targets + n, invalid);
+  }
   return ak::check_launch();
 }
