@@ -1792,8 +1792,8 @@ def embedding_backward(g, tokens, num_embeddings, scale=1.0, padding_idx=None, o
     """The gradient of embedding()'s weight, [num_embeddings, features], for the gradient ``g`` [*tokens.shape, features] of its result:
     out <- beta*out + scale * (sums of the rows of g of each token), by tokens in sorted order: fp32 sums in an order that does not change,
     each row rounded once.  Without ``out`` it is made, of the type ``dtype`` (g's); with it, ``out`` has rows of stride 1 elements (float32,
-    bfloat16 or float16).  Rows that no token names are written, too (with beta = 1 they stay).  ``padding_idx``: a token that adds nothing,
-    as tokens that name no row do."""
+    bfloat16 or float16) and counts as changed in place for autograd.  Rows that no token names are written, too (with beta = 1 they
+    stay).  ``padding_idx``: a token that adds nothing, as tokens that name no row do."""
     host = _usual(g) if out is None and padding_idx is None and (dtype is None or dtype == g.dtype) else None
     if host is not None:
         done = host.embedding_backward(g, tokens, num_embeddings, float(scale), -1, _raw_stream(g.get_device()))
@@ -1828,7 +1828,8 @@ def embedding_backward(g, tokens, num_embeddings, scale=1.0, padding_idx=None, o
         with torch.cuda.device(device):
             return embedding_backward(g, tokens, rows, scale, padding_idx, out, beta, dtype)
     empty = _allocator()
-    if out is None:
+    made = out is None
+    if made:
         out, beta = empty((rows, D), dtype=dtype or g.dtype, device=device), 0.0
     g, ldg = _rows_of(g, D)
     need = _ws_need('ak_embedding_backward_ws_bytes', tokens.numel(), rows, D)
@@ -1836,6 +1837,8 @@ def embedding_backward(g, tokens, num_embeddings, scale=1.0, padding_idx=None, o
     rc = _lib.load().ak_embedding_backward(g.data_ptr(), code, ldg, tokens.data_ptr(), token_code, tokens.numel(), rows, D, scale, padding, beta,
                                            out.data_ptr(), _ELEMENT_TYPES[out.dtype], max(out.stride(0), D), ws.data_ptr(), need, _stream_handle(device))
     _lib.check(rc, 'ak_embedding_backward')
+    if not made and not out.is_inference():
+        torch.autograd.graph.increment_version(out)
     return out
 
 

@@ -158,3 +158,18 @@ def test_embedding_of_more_tokens_than_a_launch_takes(K):     # noqa: F811
     y = K.embedding(t, table)
     for i in range(7):
         assert bool((y[i::7] == table[i]).all())
+
+
+# ------------------------------------------------------------------------------------------------ what is written in place
+def test_an_embeddings_gradient_that_is_added_to_counts_as_changed(K):     # noqa: F811
+    """A graph that has saved the tensor does not go on with other values in it."""
+    out, tokens, g = rand(10, 8, seed=1), ints(10, 30, seed=2), rand(30, 8, seed=3)
+    x = torch.ones(10, 8, device='cuda', requires_grad=True)
+    y = (x * out).sum()
+    version = out._version
+    K.embedding_backward(g, tokens, 10, out=out, beta=1.0)
+    assert out._version > version
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
+    with torch.inference_mode():
+        K.embedding_backward(g, tokens, 10, out=rand(10, 8, seed=1), beta=1.0)
