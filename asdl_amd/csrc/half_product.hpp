@@ -506,13 +506,23 @@ inline int hp_pad(const T* x, int64_t ld, int64_t rows, int64_t cols, T* out, in
   return check_launch();
 }
 
+// From here on the bf16 number nearest to a float32 number is infinite: the first of its pieces is the largest finite one.
+constexpr float kHpLarge = 0x1.ffp127f;
+
 // x in bf16 pieces that add up to it exactly (fp16: two, fp32: three), side by side in rows of PIECES * ldo, zeros behind the columns.
-template <int PIECES>
+// BELOW: |x| is known to be below kHpLarge, or x is NaN.
+template <int PIECES, bool BELOW = false>
 __device__ __forceinline__ void hp_split(float x, __bf16 (&piece)[PIECES]) {
 #pragma unroll
   for (int k = 0; k < PIECES; ++k) {
-    piece[k] = static_cast<__bf16>(x);
-    x = fabsf(x) < INFINITY ? x - static_cast<float>(piece[k]) : 0.f;          // (infinities and NaN in the first piece alone)
+    if constexpr (BELOW) {
+      piece[k] = static_cast<__bf16>(x);
+      x -= static_cast<float>(piece[k]);
+    } else {
+      const bool finite = fabsf(x) < INFINITY;
+      piece[k] = static_cast<__bf16>(k == 0 && finite ? __builtin_amdgcn_fmed3f(x, -0x1.fep127f, 0x1.fep127f) : x);
+      x = finite ? x - static_cast<float>(piece[k]) : 0.f;          // (infinities and NaN in the first piece alone)
+    }
   }
 }
 

@@ -235,14 +235,16 @@ struct LceEight {
   }
 };
 
-template <typename E>
-__device__ __forceinline__ floatx4 lce_mma(const LceEight<E>& a, const LceEight<E>& b, floatx4 c) {
+// BELOW, float32: numbers below kHpLarge; the largest there are, to `most`.
+template <bool BELOW, typename E>
+__device__ __forceinline__ floatx4 lce_mma(const LceEight<E>& a, const LceEight<E>& b, floatx4 c, float& most) {
   if constexpr (__is_same(E, float)) {
     __bf16 pa[8][3], pb[8][3];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      hp_split(a.v[e], pa[e]);
-      hp_split(b.v[e], pb[e]);
+      hp_split<3, BELOW>(a.v[e], pa[e]);
+      hp_split<3, BELOW>(b.v[e], pb[e]);
+      if constexpr (BELOW) most = fmaxf(most, fmaxf(fabsf(a.v[e]), fabsf(b.v[e])));
     }
     constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
@@ -276,43 +278,51 @@ static __global__ __launch_bounds__(64) void lce_few_kernel(const E* __restrict_
 #pragma unroll
   for (int b = 0; b < NB; ++b) hr[b] = h + static_cast<int64_t>(min(16 * b + l16, r.rows - 1)) * ldh + 32 * quarter;
   floatx4 acc[NB];
+  float most = 0.f;
+  auto products = [&](auto below) {
+    constexpr bool BELOW = decltype(below)::value;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) acc[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const int whole = D / 128 * 128;
-  LceEight<E> wn[4];
-  if (whole > 0)
+    for (int b = 0; b < NB; ++b) acc[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const int whole = D / 128 * 128;
+    LceEight<E> wn[4];
+    if (whole > 0)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) wn[e].load(wr + 8 * e);
-  for (int k = 0; k < whole; k += 128) {
-    LceEight<E> wc[4];
+      for (int e = 0; e < 4; ++e) wn[e].load(wr + 8 * e);
+    for (int k = 0; k < whole; k += 128) {
+      LceEight<E> wc[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) wc[e] = wn[e];
-    if (k + 128 < whole)
+      for (int e = 0; e < 4; ++e) wc[e] = wn[e];
+      if (k + 128 < whole)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) wn[e].load(wr + k + 128 + 8 * e);
+        for (int e = 0; e < 4; ++e) wn[e].load(wr + k + 128 + 8 * e);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          LceEight<E> x;
+          x.load(hr[b] + k + 8 * e);
+          acc[b] = lce_mma<BELOW>(wc[e], x, acc[b], most);
+        }
+    }
+    if (whole < D) {
+      const E *w_end = w + static_cast<int64_t>(r.classes - 1) * ldw + D, *h_end = h + static_cast<int64_t>(r.rows - 1) * ldh + D;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        LceEight<E> x;
-        x.load(hr[b] + k + 8 * e);
-        acc[b] = lce_mma(wc[e], x, acc[b]);
-      }
-  }
-  if (whole < D) {
-    const E *w_end = w + static_cast<int64_t>(r.classes - 1) * ldw + D, *h_end = h + static_cast<int64_t>(r.rows - 1) * ldh + D;
+        const int n = D - whole - 32 * quarter - 8 * e;
+        LceEight<E> a, x;
+        a.some(wr + whole + 8 * e, n, w_end);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = D - whole - 32 * quarter - 8 * e;
-      LceEight<E> a, x;
-      a.some(wr + whole + 8 * e, n, w_end);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        x.some(hr[b] + whole + 8 * e, n, h_end);
-        acc[b] = lce_mma(a, x, acc[b]);
+        for (int b = 0; b < NB; ++b) {
+          x.some(hr[b] + whole + 8 * e, n, h_end);
+          acc[b] = lce_mma<BELOW>(a, x, acc[b], most);
+        }
       }
     }
-  }
+  };
+  products(std::true_type{});
+  // (once more, slower, where a wave has met one: infinities, and what bf16 rounds to them)
+  if constexpr (__is_same(E, float))
+    if (__any(most >= kHpLarge)) products(std::false_type{});
   // acc[b][x]: class c0 + 4 quarter + x, row 16 b + l16
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -448,7 +458,7 @@ static __global__ __launch_bounds__(256) void lce_bias_kernel(const T* __restric
 constexpr int64_t kLcePieceBytes = 512ll << 20;       // of d
 // Rows that lce_few_kernel() takes rather than the tiles; copied: the tiles want copies of the operands first, of another pitch or in pieces.
 // (50257 x 768: bf16 4 rows 21 us, 16 rows 26 us, the tiles of 128 24 us for any number of these, but 103083 x 302 with copies 58 us, 10 rows
-// without 25 us, 120757 x 461 80 us either way for 17 rows; fp32 55 us for up to 16, 87 us for 32 and 135 us for 64 rows, by the tiles 172 us.)
+// without 25 us, 120757 x 461 80 us either way for 17 rows; fp32 55 us for up to 16, 75 us for 32 and 114 us for 64 rows, by the tiles 172 us.)
 inline int64_t lce_few_rows(int dtype, bool copied) { return dtype == AK_F32 ? 64 : copied ? 16 : 8; }
 
 constexpr int64_t kLcePartBytes = 512ll << 20;        // of the forward pass's sums of tiles

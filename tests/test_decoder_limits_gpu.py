@@ -173,3 +173,22 @@ def test_an_embeddings_gradient_that_is_added_to_counts_as_changed(K):     # noq
         y.backward()
     with torch.inference_mode():
         K.embedding_backward(g, tokens, 10, out=rand(10, 8, seed=1), beta=1.0)
+
+
+# ------------------------------------------------------------------------------------------------ the largest float32 numbers
+def test_numbers_that_bfloat16_rounds_to_infinity(K):     # noqa: F811
+    """From 2^128 - 2^119 on, in the operands that go through the matrix cores in pieces."""
+    most = torch.finfo(F32).max
+    large = torch.tensor([most, 2.0 ** 128 - 2.0 ** 119, 2.0 ** 128 - 2.0 ** 119 - 2.0 ** 104, 2.0 ** 127], device='cuda', dtype=torch.float64).to(F32)
+    g = torch.zeros(20, 5, device='cuda')
+    g[3:7, 2], g[9, 1] = large, -most
+    x = torch.zeros(20, 9, device='cuda')
+    x[3:7, :4], x[9, 8] = torch.eye(4, device='cuda') / 4, 0.5
+    dw, db = K.weight_grad_8bit(g, K.quantize_8bit(x), need_bias=False)
+    within(dw, g.double().t() @ x.double(), torch.zeros(5, 9, device='cuda', dtype=torch.float64), 'dw')         # (one product each: exact)
+    for rows in (8, 100):
+        h, w, t = rand(rows, 24, seed=1), rand(300, 24, seed=2), ints(300, rows, seed=3)
+        h[:, 5], w[:, 5] = 0, 0
+        h[::2, 5], w[7, 5], w[9, 5] = 2.0 ** -126, most, -large[1]
+        check_loss(K, h, w, t, reduction='none', g=gradient_of('none', t, 4))
+        check_loss(K, w[:rows].contiguous(), h, ints(rows, rows, seed=5), reduction='none')
