@@ -192,3 +192,33 @@ def test_numbers_that_bfloat16_rounds_to_infinity(K):     # noqa: F811
         h[::2, 5], w[7, 5], w[9, 5] = 2.0 ** -126, most, -large[1]
         check_loss(K, h, w, t, reduction='none', g=gradient_of('none', t, 4))
         check_loss(K, w[:rows].contiguous(), h, ints(rows, rows, seed=5), reduction='none')
+
+
+# ------------------------------------------------------------------------------------------------ tiles of 256
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('rows,classes,width', [(1030, 5003, 1000), (2050, 5003, 1000), (300, 9001, 2050), (4100, 4100, 1030), (4200, 70001, 520)])
+def test_linear_cross_entropy_of_the_widest_tiles(K, rows, classes, width, dtype):     # noqa: F811
+    """Gradients whose products go by tiles of 256: with the sum over the rows in one part and (fp32) several, in several pieces of the classes, of operands
+    that are copied (1030 and 2050 features) and that are not."""
+    print(f'linear_cross_entropy {rows}x{classes}x{width} {dtype}', flush=True)
+    h, w = rand(rows, width, seed=1, dtype=dtype), rand(classes, width, seed=2, dtype=dtype, scale=2 / math.sqrt(width))
+    t = ints(classes, rows, seed=3)
+    t[::7] = -100
+    check_loss(K, h, w, t, rand(classes, seed=4, dtype=dtype), g=torch.tensor(1.5 if dtype != F16 else 300.0, device='cuda'))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('rows,width,out', [(300, 2900, 3000), (1030, 4100, 2304), (70, 130, 70001)])
+def test_weight_gradients_of_the_widest_tiles(K, rows, width, out, dtype):     # noqa: F811
+    """More than 512 tiles of 128."""
+    print(f'weight_grad_8bit {rows}x{width}->{out} {dtype}', flush=True)
+    x, g = rand(rows, width, seed=rows, dtype=dtype), rand(rows, out, seed=out, dtype=dtype)
+    kept = K.quantize_8bit(x)
+    values, gd = K.dequantize_8bit(kept).double(), g.double()
+    want, size = gd.t() @ values, gd.abs().t() @ values.abs()
+    for made in (dtype, F32):
+        dw, db = K.weight_grad_8bit(g, kept, dtype=made)
+        tiny = 2.0 ** -25 if made == F16 else 0
+        within(dw, want, half_step(made) * want.abs() + 2 * (rows + 8) * U * size + tiny, 'dw')
+        within(db, gd.sum(0), half_step(made) * gd.sum(0).abs() + (rows + 8) * U * gd.abs().sum(0) + tiny, 'db')
+        assert torch.equal(dw, K.weight_grad_8bit(g, kept, dtype=made)[0])
