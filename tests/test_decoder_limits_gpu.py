@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_decoder_step_gpu import BF16, F16, F32, INF, K, U, check_loss, gradient_of, half_step, ints, loss64, rand, within     # noqa: F401
+from tests.test_decoder_step_gpu import BF16, F16, F32, INF, K, U, check_loss, gelu64, gradient_of, half_step, ints, loss64, rand, within     # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -222,3 +222,19 @@ def test_weight_gradients_of_the_widest_tiles(K, rows, width, out, dtype):     #
         within(dw, want, half_step(made) * want.abs() + 2 * (rows + 8) * U * size + tiny, 'dw')
         within(db, gd.sum(0), half_step(made) * gd.sum(0).abs() + (rows + 8) * U * gd.abs().sum(0) + tiny, 'db')
         assert torch.equal(dw, K.weight_grad_8bit(g, kept, dtype=made)[0])
+
+
+# ------------------------------------------------------------------------------------------------ the tail of GELU
+def test_gelu_of_negative_numbers(K):     # noqa: F811
+    """Relative to the result, which falls to 1e-32: the argument of exp(-x^2 / 2) is rounded twice and has a rounded factor, 3 u of x^2 / 2; the rest (the
+    reciprocal, a polynomial of eight terms, four products, the power of two) is at most 16 u."""
+    x = torch.cat([torch.linspace(-12, -1, 4001, device='cuda'), -torch.rand(4000, device='cuda', generator=torch.Generator('cuda').manual_seed(1)) * 11 - 1])
+    x = x.to(F32).view(-1, 1)                     # (a block each: the kept values are x to 2^-4, all of them)
+    y, kept = K.gelu_8bit(x)
+    at = x.double()
+    want = gelu64(x, 'none')[0]
+    within(y, want, (1.5 * at * at + 16) * U * want.abs(), 'gelu')
+    at = K.dequantize_8bit(kept).double()
+    below = 0.5 * torch.special.erfc(-at / math.sqrt(2))
+    slope = at * torch.exp(-at * at / 2) / math.sqrt(2 * math.pi)
+    within(K.gelu_8bit_backward(torch.ones_like(x), kept), below + slope, (1.5 * at * at + 16) * U * (below + slope.abs()), 'its gradient')
