@@ -285,9 +285,9 @@ inline KeepPlan keep_plan(int dtype, int64_t rows, int64_t F, int64_t out) {
   p.ld_sum = align_up(F, 4);
   p.splits = 1;
   if (F == 0) return p;          // (sums of columns alone)
-  const bool wide = hp_wide(F, out);
-  const int64_t tile = wide ? 256 : 128, tiles = ((F + tile - 1) / tile) * ((out + tile - 1) / tile);
-  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((wide ? 256 : 512) / tiles, rows / 256), 64));
+  if (hp_wide(F, out)) return p;          // (129 tiles of 256 and more: two splits of them would not run at once)
+  const int64_t tiles = ((F + 127) / 128) * ((out + 127) / 128);
+  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / tiles, rows / 256), 64));
   const int64_t per = align_up((rows + s - 1) / s, 32);
   p.splits = static_cast<int>((rows + per - 1) / per);
   return p;
@@ -449,9 +449,9 @@ extern "C" int ak_weight_grad_8bit(const void* g, int dtype, int64_t ldg, const 
       using Cfg = decltype(cfg);
       HpProblem q = hp_problem<Cfg>(hp_operand(s.x, plan.ldf, rows, width, false), hp_operand(from, ld, rows, out, false), width, out, rows, plan.splits);
       if (Cfg::PIECES) q.pieces = hp_pieces_of_b(plan.pieces, plan.ldg);
-      if (plan.splits == 1)
-        return hp_launch<Cfg, __bf16, HpStore<O>>(q, typename HpStore<O>::Params{static_cast<O*>(dw), width, F, static_cast<int>(out), 1.f, nullptr}, st);
-      return hp_launch<Cfg, __bf16, HpSum>(q, HpSum::Params{s.sum, plan.ld_sum, out * plan.ld_sum, F, static_cast<int>(out), 1}, st);
+      if constexpr (Cfg::BI == 128)
+        if (plan.splits > 1) return hp_launch<Cfg, __bf16, HpSum>(q, HpSum::Params{s.sum, plan.ld_sum, out * plan.ld_sum, F, static_cast<int>(out), 1}, st);
+      return hp_launch<Cfg, __bf16, HpStore<O>>(q, typename HpStore<O>::Params{static_cast<O*>(dw), width, F, static_cast<int>(out), 1.f, nullptr}, st);
     };
     auto of_form = [&](auto pieces) {
       constexpr bool P = decltype(pieces)::value;
