@@ -1632,7 +1632,7 @@ def _like_first(t, what, device):
         _require_one_gpu(device, **{what: t})
 
 
-def _loss_operands(h, weight, targets, bias, reduction):
+def _loss_operands(h, weight, targets, bias, ignore_index, reduction):
     """(type code, rows, classes, features, code of the reduction) of a linear cross entropy."""
     code = _ELEMENT_TYPES.get(h.dtype)
     if code is None or not h.is_cuda:
@@ -1654,6 +1654,8 @@ def _loss_operands(h, weight, targets, bias, reduction):
             raise TypeError(f'bias has to be {h.dtype} or float32. Got {bias.dtype}.')
     if reduction not in _REDUCTIONS:
         raise ValueError(f'reduction has to be one of {list(_REDUCTIONS)}. Got {reduction!r}.')
+    if not -(1 << 63) <= ignore_index < 1 << 63:           # (ctypes would take its last 64 bits)
+        raise ValueError(f'ignore_index has to be an int64 number. Got {ignore_index}.')
     for what, t in (('weight', weight), ('targets', targets), ('bias', bias)):
         if t is not None:
             _like_first(t, what, h.device)
@@ -1671,7 +1673,7 @@ def linear_cross_entropy(h, weight, targets, bias=None, ignore_index=-100, reduc
         done = host.linear_cross_entropy(h, weight, targets, bias, ignore_index, _REDUCTIONS[reduction], _raw_stream(h.get_device()))
         if done is not None:
             return done if type(done) is tuple else _lib.check(done, 'ak_linear_cross_entropy')
-    code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, reduction)
+    code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, ignore_index, reduction)
     device = h.device
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
@@ -1707,7 +1709,7 @@ def linear_cross_entropy_backward(g, h, weight, targets, lse, bias=None, ignore_
                                                   (1 if need_h else 0) | (2 if need_weight else 0) | (4 if need_bias else 0), _raw_stream(h.get_device()))
         if done is not None:
             return done if type(done) is tuple else _lib.check(done, 'ak_linear_cross_entropy_backward')
-    code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, reduction)
+    code, rows, classes, D, kind = _loss_operands(h, weight, targets, bias, ignore_index, reduction)
     for what, t, shape in (('g', g, targets.shape if kind == 0 else ()), ('lse', lse, targets.shape)):
         if t.dtype != torch.float32 or t.shape != shape:
             raise ValueError(f'{what} has to be float32 of the shape {tuple(shape)}. Got {t.dtype}, {tuple(t.shape)}.')

@@ -238,3 +238,14 @@ def test_gelu_of_negative_numbers(K):     # noqa: F811
     below = 0.5 * torch.special.erfc(-at / math.sqrt(2))
     slope = at * torch.exp(-at * at / 2) / math.sqrt(2 * math.pi)
     within(K.gelu_8bit_backward(torch.ones_like(x), kept), below + slope, (1.5 * at * at + 16) * U * (below + slope.abs()), 'its gradient')
+
+
+def test_linear_cross_entropy_refuses_an_ignored_target_that_is_no_int64(K):     # noqa: F811
+    """2^64 is not class 0."""
+    h, w, t = rand(6, 8, seed=1), rand(10, 8, seed=2), torch.zeros(6, dtype=torch.int64, device='cuda')
+    loss, lse = K.linear_cross_entropy(h, w, t)
+    for ignore in (1 << 64, 1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match='int64'):
+            K.linear_cross_entropy(h, w, t, ignore_index=ignore)
+        with pytest.raises(ValueError, match='int64'):
+            K.linear_cross_entropy_backward(loss, h, w, t, lse, ignore_index=ignore)
