@@ -1,16 +1,15 @@
 // Activations kept in 8 bits between the passes, and what the backward pass makes of them.
 // A block of 128 features of a row shares a power of two: e is the least integer with max |x| 2^-e <= 448, clamped to -127 .. 127, and a
 // value is kept as the nearest e4m3 number (4 bits of exponent, 3 of fraction, ties to even) of x 2^-e, which stands for code 2^e.  Scaling by a
-// power of two rounds nothing, and a floating code loses no accuracy by it: the largest code of a block is
-// above 224, so normal codes (from 2^-6 on, off by at most 2^-4 of themselves) reach down to 2^-13.8 of its largest value, to 2^-14.8 at best; what is
-// smaller is off by at most 2^(e - 10).  Infinities and NaN are kept as NaN and do not count for e; what would be rounded to 2^128 is kept as
-// 1.875 2^127.
+// power of two rounds nothing, and a floating code loses no accuracy by it: the largest code of a block is above 224, so normal codes (from
+// 2^-6 on, off by at most 2^-4 of themselves) reach down to 2^-13.8 of its largest value, to 2^-14.8 at best; what is smaller is off by at
+// most 2^(e - 10).  Infinities and NaN are kept as NaN and do not count for e; what would be rounded to 2^128 is kept as 1.875 2^127.
 //   gelu:    y = x P(x) and the kept x in one pass;  dx = g (P(x') + x' P'(x')) with the kept x', P the normal distribution or its
 //            approximation by tanh
 //   linear:  dw = g^T x',  db = sum g.  x' is a bfloat16 number exactly, so the products are exact and their sums fp32: g in
 //            bfloat16 as it is, in fp16 and fp32 as two and three bfloat16 pieces that add up to it exactly
 // The elementwise passes are bound by the memory (gelu of 8192 x 4096 bf16 36 us each way, 4.7 TB/s), the products by the matrix cores (16384
-// rows of 4096 to 4096 bf16 400 to 430 us, 1.3 PFLOP/s at the power limit; of 768 to 2304 from 8192 rows 39 us, too few tiles).
+// rows of 4096 to 4096 bf16 400 to 435 us, 1.3 PFLOP/s at the power limit; of 768 to 2304 from 8192 rows 39 us, too few tiles).
 #include <algorithm>
 #include "column_sums.hpp"
 #include "half_product.hpp"
@@ -100,7 +99,7 @@ enum { kGeluExact = 0, kGeluTanh = 1 };
 // Exact: P(-|x|) = exp(-x^2 / 2) t q(t), t = 1 / (1 + 0.3 |x|), with a polynomial fitted to half the scaled complementary error
 // function of |x| / sqrt(2) over t = 1 ... 1 / 5.2 at least relative error (1.5e-7; its steps in fp32 4.5e-7).  The
 // exponential is that of P'; its rounded argument is off by up to 1.5 x^2 2^-24, and the tail by as much of itself (measured 2.6e-6 at |x| = 4 to 8,
-// 7.6e-6 at 8 to 13; next to P = 1 nothing of it is seen).  (The library's erfc: gelu of 8192 x 4096 bf16 56 us each way, which is the
+// 7.8e-6 at 8 to 13; next to P = 1 nothing of it is seen).  (The library's erfc: gelu of 8192 x 4096 bf16 56 us each way, which is the
 // arithmetic's time.)
 template <int KIND, bool SLOPE>
 __device__ __forceinline__ void gelu_share(float x, float& below, float& slope) {

@@ -12,9 +12,9 @@
 // far from sure, -1 + exp(..), is rounded by next to nothing, where a power of two in its place would round all of these alike by up to 2^-9
 // (error of dh of 8192 x 768 x 50257, bf16: 0.0030 -> 0.0018 of its size).
 // fp32 operands: three bf16 pieces each, six of their products a product (half_product.hpp), through the same tiles; d in three pieces, too.
-// Bound by the matrix cores at the device's power limit where rows are many (both ways 8192 x 768 x 50257 bf16 2.55 ms, 0.99 PFLOP/s of
-// the four products; 4096 x 2048 x 128000 fp16 7.6 to 7.8 ms, 1.1 PFLOP/s), by the memory where they are few (4 rows of 50257 x 768, forward
-// alone: 21 us, 3.7 TB/s).
+// Bound by the matrix cores at the device's power limit where rows are many (both ways, on several cards: 8192 x 768 x 50257 bf16 2.5 to
+// 2.65 ms, 1.0 PFLOP/s of the four products; 4096 x 2048 x 128000 fp16 7.4 to 8.1 ms, 1.1 PFLOP/s), by the memory where they are few
+// (4 rows of 50257 x 768, forward alone: 21 us, 3.7 TB/s).
 #include <algorithm>
 #include "column_sums.hpp"
 #include "half_product.hpp"

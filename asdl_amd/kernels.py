@@ -1667,7 +1667,8 @@ def linear_cross_entropy(h, weight, targets, bias=None, ignore_index=-100, reduc
     not kept.  h [..., features], weight [classes, features]: both float32, bfloat16 or float16, rows of any stride; bias (may be None)
     of their type or float32; targets [...] int64.  loss (float32): one number, or one per row with reduction='none'.  Rows whose target is
     ``ignore_index`` have none; a target that is neither it nor a class gives NaN (the host does not look at targets).  lse (float32, one
-    per row, the log of the sum of exponentials) is what linear_cross_entropy_backward() needs."""
+    per row, the log of the sum of exponentials) is what linear_cross_entropy_backward() needs; rounded to float32, it puts the shares of a
+    row off by up to 2^-24 of its size, as scores of that size are."""
     host = _usual(h) if reduction in _REDUCTIONS else None
     if host is not None:
         done = host.linear_cross_entropy(h, weight, targets, bias, ignore_index, _REDUCTIONS[reduction], _raw_stream(h.get_device()))
@@ -1701,7 +1702,8 @@ def linear_cross_entropy(h, weight, targets, bias=None, ignore_index=-100, reduc
 def linear_cross_entropy_backward(g, h, weight, targets, lse, bias=None, ignore_index=-100, reduction='mean', need_h=True, need_weight=True,
                                   need_bias=True):
     """(dh, dw, db) of linear_cross_entropy() for the gradient ``g`` (float32, of the loss's shape); None for what is not needed.  They have the
-    types of h, weight and bias.  The logits are formed again, in pieces; for 16-bit operands their gradient, which both products read, is
+    types of h, weight and bias.  Ignored rows add zeros: times NaN or infinity in their h, as in torch's backward pass, these are NaN in
+    dw.  The logits are formed again, in pieces; for 16-bit operands their gradient, which both products read, is
     rounded to the operands' type, as a framework's backward pass in that type does."""
     host = _usual(h) if reduction in _REDUCTIONS else None
     if host is not None:

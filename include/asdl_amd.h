@@ -508,7 +508,8 @@ int ak_inv_root_group(int phases, int iters, int groups, float* const* S, const 
 /* ---- the vocabulary's ends and the activations of a decoder's training step (no counterpart in the reference) ------------------ */
 
 /* Softmax cross entropy of a linear layer, without its logits: s = h w^T + bias, lse_n = log sum_v exp s_nv, loss_n = lse_n - s_n,target(n);
- * rows whose target is ignore_index have no loss and no gradient, a target that is neither it nor a class gives NaN.
+ * rows whose target is ignore_index have no loss and no gradient (dw adds 0 times their h: NaN where that is no number), a target that is
+ * neither it nor a class gives NaN.
  * h [rows, width], w [classes, width]: one type (AK_F32, AK_BF16, AK_F16); bias [classes] (may be null): that type or AK_F32;
  * targets int64.  reduction 0: loss [rows]; 1: loss [1], their sum; 2: loss [1], their mean over the rows that are not ignored.  lse [rows]
  * is what the backward pass needs.  g: gradient of the loss, [rows] or [1]; dh [rows, width], dw [classes, width] (dense rows) of the
